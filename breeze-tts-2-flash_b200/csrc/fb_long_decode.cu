@@ -1,0 +1,690 @@
+// flashb: single-token attention over a long cache, with a sliding window and first tokens that stay visible
+// ("sinks"), over bf16 or 4-bit keys and values, optionally adding each slot's attention weight to an accumulator.
+//
+//   s_j = scaling (q . k_j),  p = softmax(s) over the visible slots,  out = sum_j p_j v_j        (0 without any)
+//   acc_out[j] = decay acc[j] + sum over the q heads of the group of p_j   (every slot; p_j = 0 where not visible)
+//
+// Bound: the visible K and V are read once (512 bytes a key and KV head in bf16, 144 in 4 bits) and do 4 G flops per
+// value, so HBM bounds it; below some megabytes the launch and one memory round trip do.
+//
+// Two launches.  long_decode_kernel: the visible keys of every (row, KV head), in chunks, form one list; CTA c of N
+// takes the c-th N-th of it whatever the rows' lengths are, so ragged batches leave no CTA idle.  A CTA's share is
+// one or more pieces (a contiguous run of one row's keys); each leaves (max, sum, unnormalised out) in a slot of the
+// workspace.  long_merge_kernel joins a row's pieces in order (no atomics: the same inputs give the same bits) and,
+// when weights are wanted, turns the scores that the first kernel left in the workspace into weights.
+//
+// In a piece each of the 4 warps takes tiles of 16 keys (4-bit: 32) on its own, straight from global memory into the
+// fragments of mma.m16n8k16 (no shared memory, no barrier until the piece ends):
+//   S^T[keys x heads] = K Q^T : a lane's 16-byte loads hold 8 dims of a key; the contraction takes dims in that order
+//     for K and q alike, so no shuffle is needed
+//   O^T[dims x heads] += V^T P^T : a lane loads 16 dims of 4 keys and pairs neighbouring keys by byte permutes; P^T
+//     comes from S^T by movmatrix.
+// fp32 scores, statistics and sums.  The tensor cores take P in the type of V's operand.  fp16 for the 4-bit cache
+// (its values are exact in fp16): 11 bits, below the bf16 output's 8.  For a bf16 cache P is the sum of two bf16
+// values, 16 bits: with G <= 4 the eight columns of the product hold each head twice (q is loaded so), the upper four
+// take the second part, and a shuffle at the piece's end adds them -- no instruction more on the tensor cores; with
+// G = 8 the second part is a second product.  One bf16 part alone measured 1.3 times the error of fp32 weights.
+// The maximum moves only when a tile's exceeds it by 2^8: the sums are exact either way, and the 32 accumulators are
+// rescaled a few times a piece instead of every tile.
+#include <cmath>
+
+#include "fb_long.cuh"
+
+namespace fb {
+
+constexpr int LD_WARPS = 4;
+constexpr int LD_THREADS = 32 * LD_WARPS;
+constexpr int LD_CTAS = 3;              // CTAs per SM (168 registers a thread)
+constexpr int LD_MAXB = 2048;           // batch rows (their geometry sits in shared memory)
+constexpr int LM_THREADS = 256;
+constexpr int LD_SLICE = 2048;          // slots per accumulator CTA of the merge
+
+struct LongDecodeArgs {
+  LongCache c;
+  const bf16* q;
+  long long q_sb, q_sh;
+  const long long *lengths, *starts;
+  int B, NH, NKV, G, S, window, sinks, ncta;
+  float scale;                          // scaling x log2(e) (x the cache's key scale)
+  float v_scale;
+  const float* acc;
+  float* acc_out;
+  float decay;
+  long long acc_sb, acc_sh, acco_sb, acco_sh;
+  float *po, *pm, *pl;                  // pieces: [slot][G][128], [slot][G], [slot][G]
+  float* sc;                            // scores [row][cap][G] in log2 units (weights wanted), else null
+  int cap;                              // visible keys a row can have
+  bf16* out;
+};
+
+template <int BITS>
+struct LongTile {
+  static constexpr int KEYS = BITS == 16 ? 16 : 32;      // keys per warp and step
+  static constexpr int CHUNK = KEYS * LD_WARPS;
+  static constexpr float SHIFT = BITS == 16 ? 0.f : 6.f; // P x 2^6 in fp16: with the 2^8 of slack below its 65504
+};
+
+__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                         uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ uint2 ld_nc_v2(const void* p) {
+  uint2 r;
+  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p));
+  return r;
+}
+
+// Geometry of every batch row and the running chunk counts, in shared memory; returns the chunks of one KV head of
+// all rows.  Every thread of the CTA calls it.
+template <int THREADS>
+__device__ __forceinline__ long long long_plan(const LongDecodeArgs& a, int chunk, int* s_cum, LongRow* s_row) {
+  __shared__ int s_w[THREADS / 32];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  int base = 0;
+  for (int b0 = 0; b0 < a.B; b0 += THREADS) {
+    const int b = b0 + tid;
+    int n = 0;
+    if (b < a.B) {
+      const LongRow r = long_row(a.lengths[b], a.starts ? a.starts[b] : 0, a.S, a.window, a.sinks);
+      s_row[b] = r;
+      n = (r.n + chunk - 1) / chunk;
+    }
+    int x = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(FULL, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) s_w[warp] = x;
+    __syncthreads();
+    int before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w) {
+      if (w < warp) before += s_w[w];
+      all += s_w[w];
+    }
+    if (b < a.B) s_cum[b] = base + before + x - n;
+    base += all;
+    __syncthreads();
+  }
+  if (tid == 0) s_cum[a.B] = base;
+  __syncthreads();
+  return base;
+}
+
+struct LongStat {
+  float mA, mB, lA, lB;   // heads 2t, 2t + 1: the subtracted maximum (the same in the eight lanes of a t), partial sums
+};
+
+// Scores of a step (rows g, g + 8 of each 16-key tile, heads 2t, 2t + 1) -> weights as the B fragments of P^T; bf16:
+// the second parts of the weights in the upper columns (G <= 4) or in pl (G = 8).
+template <int BITS, bool SCORED, int NT>
+__device__ __forceinline__ void long_softmax(float (&s)[NT][4], uint32_t (&pf)[NT][2], uint32_t (&pl)[2], LongStat& st,
+                                             float (&o)[8][4], int i0, int n, float scA, float scB, float* scp, int G, int g, int t) {
+  constexpr float SHIFT = LongTile<BITS>::SHIFT;
+  float xA = -INFINITY, xB = -INFINITY;
+#pragma unroll
+  for (int k = 0; k < NT; ++k) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int i = i0 + 16 * k + g + 8 * e;
+      const bool ok = i < n;
+      s[k][2 * e] = ok ? s[k][2 * e] * scA : -INFINITY;
+      s[k][2 * e + 1] = ok ? s[k][2 * e + 1] * scB : -INFINITY;
+      if (SCORED && ok) {
+        if (2 * t < G) scp[(long long)i * G + 2 * t] = s[k][2 * e];
+        if (2 * t + 1 < G) scp[(long long)i * G + 2 * t + 1] = s[k][2 * e + 1];
+      }
+      xA = fmaxf(xA, s[k][2 * e]);
+      xB = fmaxf(xB, s[k][2 * e + 1]);
+    }
+  }
+#pragma unroll
+  for (int x = 4; x < 32; x <<= 1) {
+    xA = fmaxf(xA, __shfl_xor_sync(FULL, xA, x));
+    xB = fmaxf(xB, __shfl_xor_sync(FULL, xB, x));
+  }
+  xA -= SHIFT;
+  xB -= SHIFT;
+  const bool up = xA > st.mA + 8.f || xB > st.mB + 8.f;   // also the first tile: the maximum is -inf
+  if (__any_sync(FULL, up)) {
+    const float nA = fmaxf(st.mA, xA), nB = fmaxf(st.mB, xB);
+    const float fA = st.mA > -INFINITY ? ex2(st.mA - nA) : 0.f, fB = st.mB > -INFINITY ? ex2(st.mB - nB) : 0.f;
+    st.mA = nA;
+    st.mB = nB;
+    st.lA *= fA;
+    st.lB *= fB;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      o[i][0] *= fA;
+      o[i][1] *= fB;
+      o[i][2] *= fA;
+      o[i][3] *= fB;
+    }
+  }
+  const float mA = st.mA > -INFINITY ? st.mA : 0.f, mB = st.mB > -INFINITY ? st.mB : 0.f;
+#pragma unroll
+  for (int k = 0; k < NT; ++k) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float pA = ex2(s[k][2 * e] - mA), pB = ex2(s[k][2 * e + 1] - mB);
+      st.lA += pA;
+      st.lB += pB;
+      if (BITS == 16) {
+        const uint32_t hi = pack2(pA, pB), lo = pack2(pA - lo_f(hi), pB - hi_f(hi));
+        pf[k][e] = movmatrix(G <= 4 && t >= 2 ? lo : hi);
+        if (G == 8) pl[e] = movmatrix(lo);
+      } else {
+        pf[k][e] = movmatrix(pack_h2(pA, pB));
+      }
+    }
+  }
+}
+
+template <int BITS, bool SCORED>
+__global__ void __launch_bounds__(LD_THREADS, LD_CTAS) long_decode_kernel(const __grid_constant__ LongDecodeArgs a) {
+  using T = LongTile<BITS>;
+  extern __shared__ __align__(16) unsigned char smem[];
+  LongRow* s_row = reinterpret_cast<LongRow*>(smem);
+  int* s_cum = reinterpret_cast<int*>(s_row + a.B);
+  __shared__ __align__(16) float s_o[LD_WARPS][8][LG_D];
+  __shared__ float s_m[LD_WARPS][8], s_l[LD_WARPS][8];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int G = a.G;
+
+  pdl_wait();
+  pdl_trigger();
+  const long long per_head = long_plan<LD_THREADS>(a, T::CHUNK, s_cum, s_row);
+  const long long total = per_head * a.NKV;
+  const long long ncta = min((long long)a.ncta, total);   // every CTA below it has a chunk at least
+  if (blockIdx.x >= ncta) return;
+  long long pos = total * blockIdx.x / ncta;
+  const long long end = total * (blockIdx.x + 1) / ncta;
+  int b = 0;
+  {
+    int hi = a.B;                                    // the last row whose chunks begin at or before pos
+    while (hi - b > 1) {
+      const int mid = (b + hi) >> 1;
+      if ((long long)s_cum[mid] * a.NKV <= pos) b = mid;
+      else hi = mid;
+    }
+  }
+  while (pos < end) {
+    const int nb = s_cum[b + 1] - s_cum[b];
+    if (nb == 0) {
+      ++b;
+      continue;
+    }
+    const long long rem = pos - (long long)s_cum[b] * a.NKV;
+    const int h = (int)(rem / nb), ch0 = (int)(rem - (long long)h * nb);
+    const int ch1 = (int)min((long long)nb, ch0 + (end - pos));
+    const LongRow row = s_row[b];
+    const int r = b * a.NKV + h;
+
+    // ---- q of the group, column g: the head's values at the dims this lane's keys hold, zero beyond the group
+    uint32_t qf[8][2];
+    const int qh = BITS == 16 && G <= 4 ? g & 3 : g;
+    float scA = a.scale, scB = a.scale;
+    {
+      const bf16* qp = a.q + b * a.q_sb + (long long)(h * G + qh) * a.q_sh;
+      uint4 w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        w[i] = make_uint4(0, 0, 0, 0);
+        // 16-bit keys: dims 32 i + 8 t .. + 7;  4-bit keys: dims 32 t + 8 i .. + 7
+        if (qh < G) w[i] = *reinterpret_cast<const uint4*>(qp + (BITS == 16 ? 32 * i + 8 * t : 32 * t + 8 * i));
+      }
+      if (BITS == 16) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          qf[2 * i][0] = w[i].x;
+          qf[2 * i][1] = w[i].y;
+          qf[2 * i + 1][0] = w[i].z;
+          qf[2 * i + 1][1] = w[i].w;
+        }
+      } else {
+        // fp16 operands: the head is scaled by a power of two to a largest value in [8, 16), so that values down to
+        // 2^-18 of it stay exact and none overflows; the score takes the power back
+        float amax = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float f[8];
+          cvt8(w[i], f);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(f[e]));
+        }
+        amax = fmaxf(amax, __shfl_xor_sync(FULL, amax, 1));
+        amax = fmaxf(amax, __shfl_xor_sync(FULL, amax, 2));
+        int ex = (int)(__float_as_uint(amax) >> 23) - 127 - 3;
+        if (amax == 0.f || ex > 120 || ex < -120) ex = ex > 120 ? 120 : (amax == 0.f ? 0 : -120);
+        const float down = __uint_as_float((uint32_t)(127 - ex) << 23);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float f[8];
+          cvt8(w[i], f);
+          qf[2 * i][0] = pack_h2(f[0] * down, f[1] * down);
+          qf[2 * i][1] = pack_h2(f[2] * down, f[3] * down);
+          qf[2 * i + 1][0] = pack_h2(f[4] * down, f[5] * down);
+          qf[2 * i + 1][1] = pack_h2(f[6] * down, f[7] * down);
+        }
+        const float up = __uint_as_float((uint32_t)(127 + ex) << 23);
+        scA = a.scale * __shfl_sync(FULL, up, 8 * t);          // head 2t lives in lanes 4 (2t) ..
+        scB = a.scale * __shfl_sync(FULL, up, 8 * t + 4);
+      }
+    }
+
+    float o[8][4];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
+    LongStat st{-INFINITY, -INFINITY, 0.f, 0.f};
+
+    const unsigned char* kb = a.c.k + b * a.c.k_sb + h * a.c.k_sh;
+    const unsigned char* vb = a.c.v + b * a.c.v_sb + h * a.c.v_sh;
+    float* scp = SCORED ? a.sc + (long long)r * a.cap * G : nullptr;
+    const int i_end = min(row.n, ch1 * T::CHUNK);
+    for (int i0 = ch0 * T::CHUNK + warp * T::KEYS; i0 < i_end; i0 += T::CHUNK) {
+      float s[T::KEYS / 16][4];
+      uint32_t pf[T::KEYS / 16][2], pl[2];
+      if constexpr (BITS == 16) {
+        // keys past the row's end read its last key (a visible one) and get no weight
+        __align__(16) uint32_t kw[2][16], vw[4][8];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const unsigned char* p = kb + row.slot(min(i0 + g + 8 * e, row.n - 1)) * a.c.k_sp + 16 * t;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(&kw[e][4 * i]) = ld_nc_v4(p + 64 * i);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const unsigned char* p =
+              vb + row.slot(min(i0 + 2 * t + (e & 1) + 8 * (e >> 1), row.n - 1)) * a.c.v_sp + 16 * g;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) *reinterpret_cast<uint4*>(&vw[e][4 * i]) = ld_nc_v4(p + 128 * i);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[0][e] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          mma_bf16(s[0], kw[0][2 * i], kw[1][2 * i], kw[0][2 * i + 1], kw[1][2 * i + 1], qf[i][0], qf[i][1]);
+        long_softmax<BITS, SCORED>(s, pf, pl, st, o, i0, row.n, scA, scB, scp, G, g, t);
+        // dims: row g of tile i is 8 g + i, row g + 8 is 64 + 8 g + i
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int w = i >> 1;
+          const uint32_t sel = (i & 1) ? 0x7632u : 0x5410u;
+          const uint32_t a0 = __byte_perm(vw[0][w], vw[1][w], sel), a1 = __byte_perm(vw[0][4 + w], vw[1][4 + w], sel);
+          const uint32_t a2 = __byte_perm(vw[2][w], vw[3][w], sel), a3 = __byte_perm(vw[2][4 + w], vw[3][4 + w], sel);
+          mma_bf16(o[i], a0, a1, a2, a3, pf[0][0], pf[0][1]);
+          if (G == 8) mma_bf16(o[i], a0, a1, a2, a3, pl[0], pl[1]);
+        }
+      } else {
+        const unsigned char* ksb = a.c.ks + b * a.c.ks_sb + h * a.c.ks_sh;
+        const unsigned char* vsb = a.c.vs + b * a.c.vs_sb + h * a.c.vs_sh;
+        __align__(16) uint32_t kw[2][2][4], vw[2][4][2];
+        uint16_t ksc[2][2];
+        unsigned char vsc[2][4];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const long long sl = row.slot(min(i0 + 16 * n + g + 8 * e, row.n - 1));
+            *reinterpret_cast<uint4*>(&kw[n][e][0]) = ld_nc_v4(kb + sl * a.c.k_sp + 16 * t);
+            ksc[n][e] = __ldg(reinterpret_cast<const uint16_t*>(ksb + sl * a.c.ks_sp + 2 * t));
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const long long sl = row.slot(min(i0 + 16 * n + 2 * t + (e & 1) + 8 * (e >> 1), row.n - 1));
+            *reinterpret_cast<uint2*>(&vw[n][e][0]) = ld_nc_v2(vb + sl * a.c.v_sp + 8 * g);
+            vsc[n][e] = __ldg(vsb + sl * a.c.vs_sp + g);
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+          const uint32_t sg = e4m3x2_to_h2(ksc[n][0]), sh = e4m3x2_to_h2(ksc[n][1]);   // blocks 2t, 2t + 1
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            uint32_t x[4], y[4];
+            e2m1x8_to_h2(kw[n][0][w], x);
+            e2m1x8_to_h2(kw[n][1][w], y);
+            const uint32_t sel = w < 2 ? 0x1010u : 0x3232u;
+            const uint32_t fx = __byte_perm(sg, sg, sel), fy = __byte_perm(sh, sh, sel);
+            mma_f16(s[n], hmul2(x[0], fx), hmul2(y[0], fy), hmul2(x[1], fx), hmul2(y[1], fy), qf[2 * w][0],
+                    qf[2 * w][1]);
+            mma_f16(s[n], hmul2(x[2], fx), hmul2(y[2], fy), hmul2(x[3], fx), hmul2(y[3], fy), qf[2 * w + 1][0],
+                    qf[2 * w + 1][1]);
+          }
+        }
+        long_softmax<BITS, SCORED>(s, pf, pl, st, o, i0, row.n, scA, scB, scp, G, g, t);
+        // dims: row g of tile i is 16 g + i (first code word), row g + 8 is 16 g + 8 + i (second)
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const uint32_t f0 = e4m3x2_to_h2((uint16_t)(vsc[n][0] | (vsc[n][1] << 8)));   // scales of keys 2t, 2t + 1
+          const uint32_t f1 = e4m3x2_to_h2((uint16_t)(vsc[n][2] | (vsc[n][3] << 8)));
+          uint32_t lo[4][4], hi[4][4];   // [2 word + key pair][byte]: even dims, odd dims, (first key, second key)
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const uint32_t x = vw[n][2 * e][w], y = vw[n][2 * e + 1][w];
+              e2m1x8_to_h2((x & 0x0f0f0f0fu) | ((y << 4) & 0xf0f0f0f0u), lo[2 * w + e]);
+              e2m1x8_to_h2(((x >> 4) & 0x0f0f0f0fu) | (y & 0xf0f0f0f0u), hi[2 * w + e]);
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            mma_f16(o[2 * i], hmul2(lo[0][i], f0), hmul2(lo[2][i], f0), hmul2(lo[1][i], f1), hmul2(lo[3][i], f1),
+                    pf[n][0], pf[n][1]);
+            mma_f16(o[2 * i + 1], hmul2(hi[0][i], f0), hmul2(hi[2][i], f0), hmul2(hi[1][i], f1), hmul2(hi[3][i], f1),
+                    pf[n][0], pf[n][1]);
+          }
+        }
+      }
+    }
+
+    if (BITS == 16 && G <= 4) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[i][e] += __shfl_down_sync(FULL, o[i][e], 2);
+    }
+    // ---- the four warps' parts of the piece, joined in warp order
+#pragma unroll
+    for (int x = 4; x < 32; x <<= 1) {
+      st.lA += __shfl_xor_sync(FULL, st.lA, x);
+      st.lB += __shfl_xor_sync(FULL, st.lB, x);
+    }
+    if (g == 0) {
+      s_m[warp][2 * t] = st.mA;
+      s_m[warp][2 * t + 1] = st.mB;
+      s_l[warp][2 * t] = st.lA;
+      s_l[warp][2 * t + 1] = st.lB;
+    }
+    {
+      const int d0 = BITS == 16 ? 8 * g : 16 * g, d1 = d0 + (BITS == 16 ? 64 : 8);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        if (2 * t + e < G) {
+#pragma unroll
+          for (int i = 0; i < 8; i += 4) {
+            *reinterpret_cast<float4*>(&s_o[warp][2 * t + e][d0 + i]) =
+                make_float4(o[i][e], o[i + 1][e], o[i + 2][e], o[i + 3][e]);
+            *reinterpret_cast<float4*>(&s_o[warp][2 * t + e][d1 + i]) =
+                make_float4(o[i][2 + e], o[i + 1][2 + e], o[i + 2][2 + e], o[i + 3][2 + e]);
+          }
+        }
+      }
+    }
+    __syncthreads();
+    const long long piece = (long long)blockIdx.x + r;   // pieces in list order have increasing CTA or row: unique
+    for (int gg = 0; gg < G; ++gg) {
+      float M = s_m[0][gg];
+#pragma unroll
+      for (int w = 1; w < LD_WARPS; ++w) M = fmaxf(M, s_m[w][gg]);
+      float L = 0.f, O = 0.f;
+#pragma unroll
+      for (int w = 0; w < LD_WARPS; ++w) {
+        const float f = s_m[w][gg] > -INFINITY ? ex2(s_m[w][gg] - M) : 0.f;
+        if (f != 0.f) {                                    // a warp without a tile holds nothing
+          L += f * s_l[w][gg];
+          O += f * s_o[w][gg][tid];
+        }
+      }
+      a.po[(piece * G + gg) * LG_D + tid] = O;
+      if (tid == 0) {
+        a.pm[piece * G + gg] = M;
+        a.pl[piece * G + gg] = L;
+      }
+    }
+    __syncthreads();
+    pos += ch1 - ch0;
+    if (h == a.NKV - 1 && ch1 == nb) ++b;
+  }
+}
+
+// Joins a row's pieces: CTA (row, y), y < G: head y's output; y >= G: weights of LD_SLICE slots.
+template <int BITS, bool SCORED>
+__global__ void __launch_bounds__(LM_THREADS) long_merge_kernel(const __grid_constant__ LongDecodeArgs a) {
+  using T = LongTile<BITS>;
+  extern __shared__ __align__(16) unsigned char smem[];
+  LongRow* s_row = reinterpret_cast<LongRow*>(smem);
+  int* s_cum = reinterpret_cast<int*>(s_row + a.B);
+  constexpr int W = LM_THREADS / 32;
+  __shared__ __align__(16) float s_o[W][LG_D];
+  __shared__ float s_l[W], s_m[8], s_inv[8];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int r = blockIdx.x, b = r / a.NKV, h = r - b * a.NKV, G = a.G;
+  pdl_wait();
+  pdl_trigger();
+  const long long per_head = long_plan<LM_THREADS>(a, T::CHUNK, s_cum, s_row);
+  const long long total = per_head * a.NKV;
+  const LongRow row = s_row[b];
+  const int nb = s_cum[b + 1] - s_cum[b];
+  // CTAs [c0, c1] hold pieces of this row: CTA c takes chunks [total c / ncta, total (c + 1) / ncta)
+  const long long ncta = min((long long)a.ncta, total);
+  const long long p0 = (long long)s_cum[b] * a.NKV + (long long)h * nb;
+  long long c0 = 0, c1 = -1;
+  if (nb > 0) {
+    c0 = ((p0 + 1) * ncta - 1) / total;
+    c1 = ((p0 + nb) * ncta - 1) / total;
+  }
+  if ((int)blockIdx.y < G) {
+    const int gg = blockIdx.y;
+    float M = -INFINITY;
+    for (long long c = c0; c <= c1; ++c) M = fmaxf(M, a.pm[(c + r) * G + gg]);
+    float L = 0.f;
+    float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (long long c = c0 + warp; c <= c1; c += W) {
+      const long long at = (c + r) * G + gg;
+      const float m = a.pm[at];
+      const float f = m > -INFINITY ? ex2(m - M) : 0.f;
+      if (f != 0.f) {
+        const float4 x = *reinterpret_cast<const float4*>(a.po + at * LG_D + 4 * lane);
+        L += f * a.pl[at];
+        O.x += f * x.x;
+        O.y += f * x.y;
+        O.z += f * x.z;
+        O.w += f * x.w;
+      }
+    }
+    *reinterpret_cast<float4*>(&s_o[warp][4 * lane]) = O;
+    if (lane == 0) s_l[warp] = L;
+    __syncthreads();
+    if (tid < LG_D) {
+      float l = 0.f, v = 0.f;
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        l += s_l[w];
+        v += s_o[w][tid];
+      }
+      // no visible key: l = 0 and the row is 0; a NaN sum stays one
+      a.out[((long long)b * a.NH + h * G + gg) * LG_D + tid] = __float2bfloat16_rn(l == 0.f ? 0.f : v / l * a.v_scale);
+    }
+    return;
+  }
+  if constexpr (SCORED) {
+    for (int gg = warp; gg < G; gg += W) {
+      float M = -INFINITY, L = 0.f;
+      for (long long c = c0 + lane; c <= c1; c += 32) M = fmaxf(M, a.pm[(c + r) * G + gg]);
+      M = warp_max(M);
+      for (long long c = c0 + lane; c <= c1; c += 32) {
+        const float m = a.pm[(c + r) * G + gg];
+        if (m > -INFINITY) L += ex2(m - M) * a.pl[(c + r) * G + gg];
+      }
+      L = warp_sum(L);
+      if (lane == 0) {
+        s_m[gg] = M;
+        s_inv[gg] = L == 0.f ? 0.f : 1.f / L;
+      }
+    }
+    __syncthreads();
+    const float* scp = a.sc + (long long)r * a.cap * G;
+    const float* ap = a.acc + b * a.acc_sb + h * a.acc_sh;
+    float* op = a.acc_out + b * a.acco_sb + h * a.acco_sh;
+    const int j0 = (blockIdx.y - G) * LD_SLICE, j1 = min(a.S, j0 + LD_SLICE);
+    for (int j = j0 + tid; j < j1; j += LM_THREADS) {
+      int i = -1;
+      if (j >= row.lo) i = row.ns + (j - row.lo);
+      else if (j >= row.st && j < row.st + row.ns) i = j - row.st;
+      float w = 0.f;
+      if (i >= 0 && i < row.n)
+        for (int gg = 0; gg < G; ++gg) w += ex2(scp[(long long)i * G + gg] - s_m[gg]) * s_inv[gg];
+      op[j] = a.decay * ap[j] + w;
+    }
+  }
+}
+
+}  // namespace fb
+
+namespace fbh {
+
+int long_cache(const fb_kv_cache* c, fb::LongCache* out) {
+  FB_CHECK_ARG(c, "long cache: null descriptor");
+  FB_CHECK_ARG(c->bits == 16 || c->bits == 4, "long cache: bits %d (16 or 4)", c->bits);
+  FB_CHECK_ARG(c->B >= 1 && c->NKV >= 1 && c->S >= 1, "long cache: bad shape B=%d NKV=%d S=%d", c->B, c->NKV, c->S);
+  FB_CHECK_ARG(c->k && c->v, "long cache: null keys or values");
+  const bool four = c->bits == 4;
+  const int64_t es = four ? 1 : 2, row = four ? fb::LG_D / 2 : fb::LG_D;
+  const int64_t st[6] = {c->k_sb, c->k_sh, c->k_sp, c->v_sb, c->v_sh, c->v_sp};
+  for (int64_t x : st)
+    FB_CHECK_ARG(x >= 0 && x * es % 16 == 0, "long cache: strides must be multiples of 16 bytes");
+  FB_CHECK_ARG(c->k_sp >= row && c->v_sp >= row, "long cache: position strides below the row (%lld)", (long long)row);
+  FB_CHECK_ARG(((uintptr_t)c->k & 15) == 0 && ((uintptr_t)c->v & 15) == 0, "long cache: keys and values 16-byte aligned");
+  out->k = (const unsigned char*)c->k;
+  out->v = (const unsigned char*)c->v;
+  out->k_sb = c->k_sb * es, out->k_sh = c->k_sh * es, out->k_sp = c->k_sp * es;
+  out->v_sb = c->v_sb * es, out->v_sh = c->v_sh * es, out->v_sp = c->v_sp * es;
+  out->ks = out->vs = nullptr;
+  out->ks_sb = out->ks_sh = out->ks_sp = out->vs_sb = out->vs_sh = out->vs_sp = 0;
+  if (four) {
+    FB_CHECK_ARG(c->ks && c->vs, "long cache: null scales");
+    const int64_t ss[6] = {c->ks_sb, c->ks_sh, c->ks_sp, c->vs_sb, c->vs_sh, c->vs_sp};
+    for (int64_t x : ss) FB_CHECK_ARG(x >= 0 && x % 8 == 0, "long cache: scale strides must be multiples of 8 bytes");
+    FB_CHECK_ARG(c->ks_sp >= 8 && c->vs_sp >= 8, "long cache: scale position strides below 8");
+    FB_CHECK_ARG(((uintptr_t)c->ks & 7) == 0 && ((uintptr_t)c->vs & 7) == 0, "long cache: scales 8-byte aligned");
+    out->ks = (const unsigned char*)c->ks;
+    out->vs = (const unsigned char*)c->vs;
+    out->ks_sb = c->ks_sb, out->ks_sh = c->ks_sh, out->ks_sp = c->ks_sp;
+    out->vs_sb = c->vs_sb, out->vs_sh = c->vs_sh, out->vs_sp = c->vs_sp;
+    const float sc[2] = {c->k_scale, c->v_scale};
+    for (float x : sc) {
+      int e;
+      FB_CHECK_ARG(x > 0.f && std::isfinite(x) && std::frexp(x, &e) == 0.5f && e > -60 && e < 60,
+                   "long cache: the tensor scales must be powers of two between 2^-60 and 2^58");
+    }
+  }
+  return FB_OK;
+}
+
+}  // namespace fbh
+
+namespace {
+using namespace fb;
+
+struct LongPlan {
+  int ncta, cap, slices;
+  size_t smem;
+  int64_t slots, ws_floats, off_m, off_l, off_s;   // float offsets of the workspace's parts
+};
+
+int long_plan_host(const fb_kv_cache* c, int NH, int window, int sinks, bool scored, LongPlan* p) {
+  FB_CHECK_ARG(NH >= c->NKV && NH % c->NKV == 0, "long_decode: %d query heads over %d key/value heads", NH, c->NKV);
+  const int G = NH / c->NKV;
+  if (G != 1 && G != 2 && G != 4 && G != 8) {
+    fbh::set_msg("long_decode: GQA group %d not built (1, 2, 4, 8)", G);
+    return FB_ERR_UNSUPPORTED;
+  }
+  if (c->B > LD_MAXB) {
+    fbh::set_msg("long_decode: %d batch rows (at most %d)", c->B, LD_MAXB);
+    return FB_ERR_UNSUPPORTED;
+  }
+  FB_CHECK_ARG((int64_t)c->B * c->NKV <= (1ll << 30), "long_decode: too many rows");
+  FB_CHECK_ARG(sinks >= 0, "long_decode: sinks %d", sinks);
+  p->cap = window > 0 && (int64_t)window + sinks < c->S ? window + sinks : c->S;
+  const int chunk = c->bits == 16 ? LongTile<16>::CHUNK : LongTile<4>::CHUNK;
+  const int64_t most = (int64_t)c->B * c->NKV * ((p->cap + chunk - 1) / chunk);
+  const int64_t want = (int64_t)fbh::grid_sms() * LD_CTAS;
+  p->ncta = (int)(most < want ? most : want);
+  p->slots = (int64_t)p->ncta + (int64_t)c->B * c->NKV;
+  p->slices = scored ? (c->S + LD_SLICE - 1) / LD_SLICE : 0;
+  FB_CHECK_ARG(G + p->slices <= 65535, "long_decode: cache too long for the accumulator grid");
+  p->smem = (size_t)c->B * sizeof(LongRow) + ((size_t)c->B + 1) * sizeof(int);
+  p->off_m = p->slots * G * LG_D;
+  p->off_l = p->off_m + p->slots * G;
+  p->off_s = p->off_l + p->slots * G;
+  p->ws_floats = p->off_s + (scored ? (int64_t)c->B * c->NKV * p->cap * G : 0);
+  return FB_OK;
+}
+
+template <int BITS, bool SCORED>
+int long_launch(LongDecodeArgs& a, const LongPlan& p, cudaStream_t st) {
+  void* args[] = {(void*)&a};
+  int rc = fbh::launch_pdl((const void*)long_decode_kernel<BITS, SCORED>, dim3(p.ncta), dim3(LD_THREADS), p.smem, st,
+                           args, true);
+  if (rc) return rc;
+  return fbh::launch_pdl((const void*)long_merge_kernel<BITS, SCORED>, dim3(a.B * a.NKV, a.G + p.slices),
+                         dim3(LM_THREADS), p.smem, st, args, true);
+}
+
+}  // namespace
+
+extern "C" int64_t flashb_long_decode_ws_floats(const fb_kv_cache* cache, int NH, int window, int sinks, int scored) {
+  fb::LongCache lc;
+  LongPlan p;
+  if (fbh::long_cache(cache, &lc) != FB_OK || long_plan_host(cache, NH, window, sinks, scored != 0, &p) != FB_OK)
+    return -1;
+  return p.ws_floats;
+}
+
+extern "C" int flashb_long_decode(const fb_kv_cache* cache, const void* q, int64_t q_sb, int64_t q_sh, int NH,
+                                  const int64_t* lengths, const int64_t* starts, int window, int sinks, float scaling,
+                                  const float* acc, int64_t acc_sb, int64_t acc_sh, float* acc_out, int64_t acco_sb,
+                                  int64_t acco_sh, float decay, float* ws, int64_t ws_floats, void* out, void* stream) {
+  LongDecodeArgs a{};
+  int rc = fbh::long_cache(cache, &a.c);
+  if (rc) return rc;
+  FB_CHECK_ARG(q && lengths && ws && out, "long_decode: null pointer argument");
+  FB_CHECK_ARG((acc == nullptr) == (acc_out == nullptr), "long_decode: acc and acc_out come together");
+  LongPlan p;
+  rc = long_plan_host(cache, NH, window, sinks, acc != nullptr, &p);
+  if (rc) return rc;
+  FB_CHECK_ARG(((uintptr_t)q & 15) == 0 && q_sb % 8 == 0 && q_sh % 8 == 0,
+               "long_decode: q must be 16-byte aligned with strides multiple of 8 elements");
+  FB_CHECK_ARG(((uintptr_t)ws & 15) == 0 && ws_floats >= p.ws_floats, "long_decode: workspace of %lld floats, %lld needed",
+               (long long)ws_floats, (long long)p.ws_floats);
+  a.q = (const bf16*)q, a.q_sb = q_sb, a.q_sh = q_sh;
+  a.lengths = (const long long*)lengths, a.starts = (const long long*)starts;
+  a.B = cache->B, a.NH = NH, a.NKV = cache->NKV, a.G = NH / cache->NKV, a.S = cache->S;
+  a.window = window > 0 ? window : 0, a.sinks = sinks, a.ncta = p.ncta;
+  const bool four = cache->bits == 4;
+  a.scale = scaling * LG_LOG2E * (four ? cache->k_scale : 1.f);
+  a.v_scale = four ? cache->v_scale : 1.f;
+  a.acc = acc, a.acc_out = acc_out, a.decay = decay;
+  a.acc_sb = acc_sb, a.acc_sh = acc_sh, a.acco_sb = acco_sb, a.acco_sh = acco_sh;
+  a.po = ws, a.pm = ws + p.off_m, a.pl = ws + p.off_l, a.sc = ws + p.off_s;
+  a.cap = p.cap, a.out = (bf16*)out;
+  const cudaStream_t s = (cudaStream_t)stream;
+  if (four) return acc ? long_launch<4, true>(a, p, s) : long_launch<4, false>(a, p, s);
+  return acc ? long_launch<16, true>(a, p, s) : long_launch<16, false>(a, p, s);
+}

@@ -63,6 +63,12 @@ _PROTOS = {
     'flashb_prefill_attn_tiles': (I, [P, L, L, L, P, L, L, L, P, L, L, L, P, I, L, L, I, I, I, I, I, I, F, I, I, I,
                                       I, I, P, L, L, L, P]),
     'flashb_prefill_qkv': (I, [P, L, I, I, I, I, P, P, F, P, P, I, P, P, P, P, L, L, I, P]),
+    'flashb_long_decode_ws_floats': (L, [P, I, I, I, I]),
+    'flashb_long_decode': (I, [P, P, L, L, I, P, P, I, I, F, P, L, L, P, L, L, F, P, L, P, P]),
+    'flashb_long_prefill': (I, [P, L, L, L, P, L, L, L, P, L, L, L, I, I, I, I, I, I, P, I, I, F, P, L, L, L, P]),
+    'flashb_kv4_store': (I, [P, P, L, L, L, P, L, L, L, P, L, I, P]),
+    'flashb_kv4_read': (I, [P, P, L, I, P, P, P]),
+    'flashb_kv_evict': (I, [P, P, L, L, P, P, I, I, I, P, P, L, L, I, P, P, P]),
     'flashb_ln12_decode': (I, [P, P, P, ctypes.c_uint32, ctypes.c_uint32, I, I, P, L, P]),
     'flashb_lm_head_rows': (I, [P, L, I, I, P, I, P, P]),
     'flashb_dd_scratch_bytes': (L, [P]),
@@ -92,6 +98,14 @@ class FbLn12Mat(ctypes.Structure):
     """fb_ln12_mat of include/flashb.h."""
     _fields_ = [('data', P), ('meta', P), ('ovf', P), ('n_ovf', L), ('lut_lo', ctypes.c_uint32),
                 ('lut_hi', ctypes.c_uint32)]
+
+
+class FbKVCache(ctypes.Structure):
+    """fb_kv_cache of include/flashb.h."""
+    _fields_ = ([(n, I) for n in ('bits', 'B', 'NKV', 'S')] + [('k', P), ('v', P)] +
+                [(n, L) for n in ('k_sb', 'k_sh', 'k_sp', 'v_sb', 'v_sh', 'v_sp')] + [('ks', P), ('vs', P)] +
+                [(n, L) for n in ('ks_sb', 'ks_sh', 'ks_sp', 'vs_sb', 'vs_sh', 'vs_sp')] +
+                [('k_scale', F), ('v_scale', F)])
 
 
 def lib_path():

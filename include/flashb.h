@@ -226,6 +226,61 @@ int flashb_prefill_qkv(void* qkv, int64_t ldq, int B, int L, int NH, int NKV, co
 int flashb_lm_head_rows(const void* hidden, int64_t ldh, int B, int H, const float* W32, int V, float* logits,
                         void* stream);
 
+/* ---------------------------------------------------------------------------------------------- long speech
+ * A cache whose bytes stay bounded over a long reading: attention with a sliding window and first tokens that stay
+ * visible, a cache held in 4 bits, eviction by accumulated attention weight.  No reference counterpart (the reference
+ * decodes over a bf16 cache of the whole sequence).  Row b's keys are slots [starts[b], lengths[b]) (device int64;
+ * starts NULL = 0; both are clamped to the cache); the token at slot p sees slot j when starts[b] <= j <= p and
+ * (j > p - window or j < starts[b] + sinks); window <= 0 = no window.  D is 128, NH / NKV in {1, 2, 4, 8}.  Slots
+ * that are not visible are not read, or get no weight, whatever they hold; without a visible slot the output is 0. */
+typedef struct {
+  int bits;              /* 16: bf16 rows [B, NKV, S, 128].  4: e2m1 codes [B, NKV, S, 64] uint8 (two per byte, the
+                          * even element in the low half) and e4m3 scales [B, NKV, S, 8] uint8, one per 16 values */
+  int B, NKV, S;
+  void *k, *v;           /* 16-byte aligned; strides per batch row, head and position in elements (bf16 or bytes), */
+  int64_t k_sb, k_sh, k_sp, v_sb, v_sh, v_sp; /* multiples of 16 bytes; the innermost stride is 1 */
+  void *ks, *vs;         /* bits 4: the scales, 8-byte aligned, strides in bytes, multiples of 8; else NULL */
+  int64_t ks_sb, ks_sh, ks_sp, vs_sb, vs_sh, vs_sp;
+  float k_scale, v_scale; /* bits 4: powers of two; a stored value stands for code x scale x this */
+} fb_kv_cache;
+/* Single-token attention: q [B, NH, 1, 128] bf16 (strides q_sb, q_sh), the token at slot lengths[b] - 1 of each row;
+ * out [B, 1, NH, 128] bf16 contiguous.  fp32 scores, softmax and sums, rounded to bf16 once.  acc / acc_out (both or
+ * neither; fp32 [B, NKV, S], unit stride per slot, may be the same buffer): acc_out[b, h, j] = decay acc[b, h, j] +
+ * the weight of slot j summed over the group's query heads, for every slot of the cache.  ws: 16-byte aligned, at
+ * least flashb_long_decode_ws_floats() floats, not shared by calls that can overlap, contents free before and after.
+ * The same inputs give the same bits.  B <= 2048. */
+int64_t flashb_long_decode_ws_floats(const fb_kv_cache* cache, int NH, int window, int sinks, int scored);
+int flashb_long_decode(const fb_kv_cache* cache, const void* q, int64_t q_sb, int64_t q_sh, int NH,
+                       const int64_t* lengths, const int64_t* starts, int window, int sinks, float scaling,
+                       const float* acc, int64_t acc_sb, int64_t acc_sh, float* acc_out, int64_t acco_sb,
+                       int64_t acco_sh, float decay, float* ws, int64_t ws_floats, void* out, void* stream);
+/* Attention of the tokens at slots q_start .. q_start + L - 1: q [B, NH, L, 128] bf16 over k / v [B, NKV, S, 128] bf16
+ * (strides per batch row, head and position in elements, multiples of 8; 16-byte aligned; q_start + L <= S; later
+ * slots are not read); out [B, L, NH, 128] bf16 with strides o_sb, o_sl, o_sh.  Arithmetic as above. */
+int flashb_long_prefill(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_sl, const void* k, int64_t k_sb,
+                        int64_t k_sh, int64_t k_sl, const void* v, int64_t v_sb, int64_t v_sh, int64_t v_sl, int B,
+                        int NH, int NKV, int L, int S, int q_start, const int64_t* starts, int window, int sinks,
+                        float scaling, void* out, int64_t o_sb, int64_t o_sl, int64_t o_sh, void* stream);
+/* Stores bf16 heads k / v [B, NKV, L, 128] (strides in elements, multiples of 8; 16-byte aligned) into the 4-bit cache
+ * at slots[b * slot_sb + l] (device int64; distinct within a row; slots outside [0, S) are skipped).  Per block of 16
+ * values x (divided by the tensor scale): s = e4m3(max |x| / 6), code = e2m1(x / s), to nearest, ties to even,
+ * saturating; a block with a NaN or an infinity reads back as NaN.  The result is that of exact arithmetic. */
+int flashb_kv4_store(const fb_kv_cache* cache, const void* k, int64_t k_sb, int64_t k_sh, int64_t k_sl, const void* v,
+                     int64_t v_sb, int64_t v_sh, int64_t v_sl, const int64_t* slots, int64_t slot_sb, int L,
+                     void* stream);
+/* The values at those slots: k_out / v_out [B, NKV, L, 128] bf16 contiguous (exact; 0 for slots outside [0, S)). */
+int flashb_kv4_read(const fb_kv_cache* cache, const int64_t* slots, int64_t slot_sb, int L, void* k_out, void* v_out,
+                    void* stream);
+/* Eviction by accumulated attention weight: of row b's slots [starts[b], lengths[b]) at most `keep` move, in slot
+ * order, to slots 0, 1, .. of `into` (a cache of the same bits, rows, heads and tensor scales that shares no memory
+ * with `cache`): all when there are no more, else the first `sinks`, the last `recent` (sinks + recent <= keep) and
+ * the others of largest acc[b, h, .] (fp32, unit stride per slot; equal weights: the lower slot; NaN above all), each
+ * KV head for itself.  kept [B, NKV, keep] int32: the slot each came from, -1 beyond; lengths_out [B] int64: how many
+ * (may not be `lengths`); acc_out (or NULL) [B, NKV, acc_n >= keep] fp32: the weights moved along, 0 beyond. */
+int flashb_kv_evict(const fb_kv_cache* cache, const float* acc, int64_t acc_sb, int64_t acc_sh, const int64_t* lengths,
+                    const int64_t* starts, int keep, int sinks, int recent, const fb_kv_cache* into, float* acc_out,
+                    int64_t acco_sb, int64_t acco_sh, int acc_n, int32_t* kept, int64_t* lengths_out, void* stream);
+
 /* LN12 -> bf16 on the device (the reference's lossless 12-bit weight storage, flash/ln12_format.py, read by its depth
  * kernels through dd2_init_ln12, flash/csrc/depth_frame.cu:800-823): a matrix W[N, K] (K % 1024 == 0) stored as
  * data [N][K / 1024][3][32][16 B] (slot 0: low bytes of the chunks 0, 1 of lane l's elements k = 1024 g + 256 c +
