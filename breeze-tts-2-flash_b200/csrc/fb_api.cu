@@ -206,6 +206,40 @@ int tmap_heads(CUtensorMap* out, const void* base, int B, int NH, long long S, l
   return FB_OK;
 }
 
+int tmap_bf16(CUtensorMap* out, const void* base, int rank, const unsigned long long* dims,
+              const unsigned long long* strides, const unsigned* box) {
+  static PFN_cuTensorMapEncodeTiled_v12000 enc = nullptr;
+  static std::mutex mu;
+  {
+    std::lock_guard<std::mutex> lk(mu);
+    if (!enc) {
+      cudaDriverEntryPointQueryResult q;
+      void* fn = nullptr;
+      if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess || !fn) {
+        set_msg("tensor map: cuTensorMapEncodeTiled unavailable");
+        return FB_ERR_CUDA;
+      }
+      enc = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+    }
+  }
+  cuuint64_t d[5], st[4];
+  cuuint32_t bx[5], estr[5];
+  for (int i = 0; i < rank; ++i) {
+    d[i] = dims[i];
+    bx[i] = box[i];
+    estr[i] = 1;
+    if (i > 0) st[i - 1] = strides[i - 1];
+  }
+  const CUresult r = enc(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t)rank, const_cast<void*>(base), d, st, bx, estr,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_msg("tensor map: cuTensorMapEncodeTiled failed (%d) for a rank-%d bf16 tensor", (int)r, rank);
+    return FB_ERR_CUDA;
+  }
+  return FB_OK;
+}
+
 int grid_sms() {
   const int n = num_sms();
   return (t_sm_budget > 0 && t_sm_budget < n) ? t_sm_budget : n;

@@ -206,6 +206,10 @@ int tmap_ln12(CUtensorMap* out, const void* data, long long N, int K, int box_ro
 // groups).  Rows past S read as zeros.  Cached per (base, shape, strides).
 int tmap_heads(CUtensorMap* out, const void* base, int B, int NH, long long S, long long sl, long long sh,
                long long sb);
+// Tensor map of a bf16 tensor of rank <= 5 (innermost first; strides in bytes of dimensions 1 .., multiples of 16) with
+// the 128-byte swizzle; nothing is cached.
+int tmap_bf16(CUtensorMap* out, const void* base, int rank, const unsigned long long* dims,
+              const unsigned long long* strides, const unsigned* box);
 }  // namespace fbh
 
 #define FB_CHECK_ARG(cond, ...)          \

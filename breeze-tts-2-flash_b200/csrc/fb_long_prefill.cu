@@ -1,80 +1,363 @@
-// flashb: attention of a run of tokens over a long cache with a sliding window and first tokens that stay visible.
+// flashb: attention of a run of tokens over a long cache with a sliding window and first tokens that stay visible, on
+// the 5th-generation tensor cores.
 //
 // q [B, NH, L, 128] holds the tokens at slots q_start .. q_start + L - 1 of k / v [B, NKV, S, 128].  The token at slot
 // p of row b sees slot j when start_b <= j <= p and (j > p - window or j < start_b + sinks);
 //   out = softmax(scaling q k^T over those) v in fp32, rounded once; a token without a visible key (p < start_b) gives 0.
 //
-// long_row_kernel: a CTA per (token, head, row), a warp per quarter of the visible keys, four dims a lane.
+// A CTA computes 128 rows: the G query heads of a KV head for 128 / G tokens.  Packing the group makes the keys that a
+// tile must visit window + 128 / G instead of window + 128, and reads each K and V tile once for the group.  Those keys
+// are cut into segments of 32: the sinks that the window of the CTA's first token does not reach, then the slots from
+// that window's beginning to the CTA's last token.  Four segments are a tile (the last tile may have fewer, and costs
+// as many MMAs as it has); no tile is spent on a handful of sinks alone.
+//
+// Per tile: S = Q K^T (TMEM, 128 fp32 columns); warps 0-3 (a thread per row) read their row, subtract the running
+// maximum, take exponentials and write P as bf16 pairs over S's first columns; O += P V with P as the MMA's TMEM
+// operand (128 more columns); one more warp issues the copies and the MMAs.  The chain S -> softmax -> O of one CTA is
+// serial; two CTAs share an SM (96 KB of shared memory, 256 TMEM columns each) and fill each other's gaps.  The running
+// maximum moves only when a tile's exceeds it by 2^8 (the sums are exact either way), so O is hardly ever rescaled.
+// Masks are applied to the segments that need one for some row of the CTA.
+//
+// Rounding: fp32 scores, statistics and sums; P goes to bf16, the type of V's operand, unnormalised.
+//
+// A slot that a row does not see gets weight 0, and 0 times an infinity or a NaN in V is NaN.  Slots past the tokens
+// read as zeros (the tensor maps end there), sink segments are zeroed past the sinks; what is left are slots that other
+// rows of the CTA see.  So a row whose output is not finite is computed again, one visible key at a time.
 #include "fb_long.cuh"
+#include "fb_tc.cuh"
 
 namespace fb {
 
-struct LongPrefillArgs {
+constexpr int LP_ROWS = 128;                      // rows of a CTA (TMEM lanes)
+constexpr int LP_SEG = 32, LP_TILE = 128;         // keys per segment and tile
+constexpr int LP_THREADS = 160;                   // 4 softmax warps, 1 issuing warp
+constexpr int LP_OPND = 128 * LG_D * 2;           // bytes of a 128 x 128 operand
+constexpr int LP_SMEM = 3 * LP_OPND + 1024;       // Q, K, V at a 1024-byte boundary
+constexpr uint32_t LP_COLS = 256;                 // TMEM: S (and P over it) in columns 0-127, O in 128-255
+constexpr float LP_SLACK = 8.f;
+
+struct alignas(64) LongPrefillArgs {
+  CUtensorMap tq, tk, tv, tk32, tv32;             // Q tile; K, V: boxes of 128 and of 32 slots
   const bf16 *q, *k, *v;
   long long q_sb, q_sh, q_sl, k_sb, k_sh, k_sl, v_sb, v_sh, v_sl;
   const long long* starts;
-  int B, NH, NKV, L, q_start, window, sinks;
-  float scale;                          // scaling x log2(e)
+  int NH, NKV, G, nq, L, q_start, window, sinks;  // nq = 128 / G tokens a CTA; window 0: none
+  float scale;                                    // scaling x log2(e)
   bf16* out;
   long long o_sb, o_sl, o_sh;
+  unsigned* err;
 };
 
-__global__ void __launch_bounds__(128) long_row_kernel(const __grid_constant__ LongPrefillArgs a) {
-  __shared__ float s_o[4][LG_D], s_m[4], s_l[4];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int l = blockIdx.x, hq = blockIdx.y, b = blockIdx.z, h = hq / (a.NH / a.NKV);
-  pdl_wait();
-  pdl_trigger();
-  const int p = a.q_start + l;
-  // the tokens up to p; a row that begins after p has none
-  const LongRow row = long_row(p + 1, a.starts ? a.starts[b] : 0, p + 1, a.window, a.sinks);
-  float qf[4];
-  const bf16* qp = a.q + b * a.q_sb + hq * a.q_sh + l * a.q_sl;
+__device__ __forceinline__ void lp_load(void* dst, const CUtensorMap* m, int c1, int c2, int c3, int c4, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, "
+      "%6}], [%7];" ::"r"(smem_u32(dst)),
+      "l"(m), "r"(0), "r"(c1), "r"(c2), "r"(c3), "r"(c4), "r"(smem_u32(bar))
+      : "memory");
+}
+// D (+)= P V: P in TMEM (row = lane, two bf16 per column), V in shared memory with the dims contiguous
+__device__ __forceinline__ void lp_mma_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate));
+}
+__device__ __forceinline__ void lp_ld32(uint32_t taddr, float* f) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
 #pragma unroll
-  for (int e = 0; e < 4; ++e) qf[e] = b2f(qp[4 * lane + e]) * a.scale;
-  const bf16* kb = a.k + b * a.k_sb + h * a.k_sh + 4 * lane;
-  const bf16* vb = a.v + b * a.v_sb + h * a.v_sh + 4 * lane;
-  float m = -INFINITY, sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int i = warp; i < row.n; i += 4) {
+  for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void lp_st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};\n\t"
+      "tcgen05.wait::st.sync.aligned;" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
+      "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
+      "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
+      : "memory");
+}
+
+// One row over its visible keys, one at a time (the case of a non-finite output; see the header).  o: the thread's
+// column of a [128 dims][128 threads] array.
+__device__ __noinline__ void long_row_again(const LongPrefillArgs& a, int b, int hq, int l, long long start, float* o) {
+  const int p = a.q_start + l, h = hq / a.G;
+  const LongRow row = long_row(p + 1, start, p + 1, a.window, a.sinks);
+  const bf16* qp = a.q + b * a.q_sb + hq * a.q_sh + l * a.q_sl;
+  const bf16* kb = a.k + b * a.k_sb + h * a.k_sh;
+  const bf16* vb = a.v + b * a.v_sb + h * a.v_sh;
+  float m = -INFINITY, sum = 0.f;
+  for (int d = 0; d < LG_D; ++d) o[d * LP_ROWS] = 0.f;
+  for (int i = 0; i < row.n; ++i) {
     const long long j = row.slot(i);
-    const uint2 kw = *reinterpret_cast<const uint2*>(kb + j * a.k_sl), vw = *reinterpret_cast<const uint2*>(vb + j * a.v_sl);
-    const float s = warp_sum(qf[0] * lo_f(kw.x) + qf[1] * hi_f(kw.x) + qf[2] * lo_f(kw.y) + qf[3] * hi_f(kw.y));
-    const float mn = fmaxf(m, s), f = m > -INFINITY ? ex2(m - mn) : 0.f, w = mn > -INFINITY ? ex2(s - mn) : 0.f;
+    float s = 0.f;
+    for (int d = 0; d < LG_D; ++d) s += b2f(qp[d]) * b2f(kb[j * a.k_sl + d]);
+    s *= a.scale;
+    const float mn = fmaxf(m, s), f = m > -INFINITY ? ex2(m - mn) : 0.f, w = mn > -INFINITY ? ex2(s - mn) : (s == -INFINITY ? 0.f : s);
     m = mn;
     sum = sum * f + w;
-    o[0] = o[0] * f + w * lo_f(vw.x);
-    o[1] = o[1] * f + w * hi_f(vw.x);
-    o[2] = o[2] * f + w * lo_f(vw.y);
-    o[3] = o[3] * f + w * hi_f(vw.y);
+    for (int d = 0; d < LG_D; ++d) o[d * LP_ROWS] = o[d * LP_ROWS] * f + w * b2f(vb[j * a.v_sl + d]);
   }
-#pragma unroll
-  for (int e = 0; e < 4; ++e) s_o[warp][4 * lane + e] = o[e];
-  if (lane == 0) {
-    s_m[warp] = m;
-    s_l[warp] = sum;
+  for (int d = 0; d < LG_D; ++d) o[d * LP_ROWS] = sum == 0.f ? 0.f : o[d * LP_ROWS] / sum;
+}
+
+__global__ void __launch_bounds__(LP_THREADS, 2) long_prefill_kernel(const __grid_constant__ LongPrefillArgs a) {
+  extern __shared__ __align__(16) unsigned char raw[];
+  unsigned char* sq = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
+  unsigned char* sk = sq + LP_OPND;
+  unsigned char* sv = sk + LP_OPND;
+  __shared__ __align__(8) uint64_t bar_k, bar_v, bar_s, bar_p, bar_o;
+  __shared__ uint32_t tslot;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int qt = gridDim.x - 1 - blockIdx.x;       // the latest tokens first: they have the most keys
+  const int h = blockIdx.y, b = blockIdx.z, q0 = qt * a.nq;
+  if (tid == 0) {
+    mbar_init(&bar_k, 1);
+    mbar_init(&bar_v, 1);
+    mbar_init(&bar_s, 1);
+    mbar_init(&bar_p, LP_ROWS);
+    mbar_init(&bar_o, 1);
+    fence_mbar_init();
   }
+  if (warp == 4) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tslot)), "r"(LP_COLS)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_before();
   __syncthreads();
-  const float M = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
-  float L = 0.f, O = 0.f;
+  tc_after();
+  const uint32_t tmem = tslot, t_o = tmem + 128;
+  pdl_wait();
+  pdl_trigger();
+
+  // ---- the CTA's keys: nss segments of sinks from st, then segments from lo to the last token
+  const int p_lo = a.q_start + q0, p_hi = a.q_start + min(q0 + a.nq, a.L) - 1;
+  const long long start = a.starts ? a.starts[b] : 0;
+  const int st = (int)(start < 0 ? 0 : (start > p_hi + 1 ? p_hi + 1 : start));
+  const int lo = a.window > 0 && p_lo - a.window + 1 > st ? p_lo - a.window + 1 : st;
+  const int ns = min(a.sinks, lo - st), nss = (ns + LP_SEG - 1) / LP_SEG;
+  const int segs = nss + (p_hi + 1 - lo + LP_SEG - 1) / LP_SEG;
+  const int tiles = (segs + 3) >> 2;
+  auto seg_base = [&](int s) { return s < nss ? st + LP_SEG * s : lo + LP_SEG * (s - nss); };
+
+  if (warp == 4) {
+    auto load = [&](bool is_v, int t) {
+      const int n = min(4, segs - 4 * t);
+      uint64_t* bar = is_v ? &bar_v : &bar_k;
+      unsigned char* dst = is_v ? sv : sk;
+      mbar_arrive_expect_tx(bar, (unsigned)(n * (LP_OPND / 4) + (!is_v && t == 0 ? LP_OPND : 0)));
+      if (n == 4 && 4 * t >= nss) {
+        lp_load(dst, is_v ? &a.tv : &a.tk, seg_base(4 * t), 0, h, b, bar);
+      } else {
+        for (int s = 0; s < n; ++s)
+          for (int half = 0; half < 2; ++half)
+            lp_load(dst + half * (LP_OPND / 2) + s * 4096, is_v ? &a.tv32 : &a.tk32, seg_base(4 * t + s), half, h, b, bar);
+      }
+    };
+    bool ok = true;
+    int kl = 0, vl = 0;                            // K and V copies issued
+    int kw = 0, vw = 0;                            // ... and waited for
+    if (tiles > 0) {
+      if (lane == 0) {
+        load(false, 0);
+        lp_load(sq, &a.tq, q0, h * a.G, 0, b, &bar_k);
+        load(true, 0);
+      }
+      kl = vl = 1;
+    }
+    const uint32_t aq = smem_u32(sq), ak = smem_u32(sk), av = smem_u32(sv);
+    for (int t = 0; t < tiles && ok; ++t) {
+      const int n = min(4, segs - 4 * t);
+      ok = mbar_wait_warp(&bar_k, t & 1, a.err);
+      if (!ok) break;
+      ++kw;
+      if (t > 0) {                                 // P V of the last tile done: P's columns and V's buffer are free
+        ok = mbar_wait_warp(&bar_o, (t - 1) & 1, a.err);
+        if (!ok) break;
+        if (lane == 0) load(true, t);
+        ++vl;
+      }
+      tc_after();
+      if (lane == 0) {
+        const uint32_t idesc = tc_idesc(32 * n);
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    const float f = s_m[w] > -INFINITY ? ex2(s_m[w] - M) : 0.f;
-    if (f != 0.f) {
-      L += f * s_l[w];
-      O += f * s_o[w][threadIdx.x];
+        for (int s = 0; s < LG_D / 16; ++s) {
+          const uint32_t at = (s >> 2) * (LP_OPND / 2) + (s & 3) * 32;
+          tc_mma(tmem, tc_desc_sw128(aq + at), tc_desc_sw128(ak + at), s > 0, idesc);
+        }
+        tc_commit(&bar_s);
+      }
+      __syncwarp();
+      ok = mbar_wait_warp(&bar_s, t & 1, a.err);   // K's buffer is free
+      if (!ok) break;
+      if (t + 1 < tiles) {
+        if (lane == 0) load(false, t + 1);
+        ++kl;
+      }
+      ok = mbar_wait_warp(&bar_v, t & 1, a.err);
+      if (!ok) break;
+      ++vw;
+      if (4 * t < nss && 4 * t + 4 >= nss && (ns & 31)) {   // the last sink segment: zero past the sinks
+        const int s = nss - 1 - 4 * t;
+        for (int i = (ns & 31) * 8 + lane; i < LP_SEG * 8; i += 32)
+          for (int half = 0; half < 2; ++half)
+            *reinterpret_cast<uint4*>(sv + half * (LP_OPND / 2) + s * 4096 + i * 16) = make_uint4(0, 0, 0, 0);
+        fence_proxy_async();
+        __syncwarp();
+      }
+      ok = mbar_wait_warp(&bar_p, t & 1, a.err);
+      if (!ok) break;
+      tc_after();
+      if (lane == 0) {
+        const uint32_t idesc = tc_idesc(LG_D) | (1u << 16);   // V: N-major
+        for (int s = 0; s < 2 * n; ++s)
+          lp_mma_ts(t_o, tmem + 8 * s, tc_desc(av + 2048 * s, LP_OPND / 2, 1024, 2), idesc, (t > 0 || s > 0) ? 1u : 0u);
+        tc_commit(&bar_o);
+      }
+      __syncwarp();
+    }
+    // after a wait that gave up: no copy may be in flight when the CTA ends
+    if (kl > kw) mbar_wait_warp(&bar_k, kw & 1, a.err);
+    if (vl > vw) mbar_wait_warp(&bar_v, vw & 1, a.err);
+  } else {
+    const int r = tid, g = r / a.nq, l = q0 + r - g * a.nq, p = a.q_start + l, hq = h * a.G + g;
+    const uint32_t my = (uint32_t)(warp * 32) << 16;
+    const int wnd = a.window > 0 ? a.window : 0x7fffffff;
+    float m = -INFINITY, sum = 0.f;
+    bool ok = true;
+    for (int t = 0; t < tiles; ++t) {
+      const int n = min(4, segs - 4 * t);
+      ok = mbar_wait_warp(&bar_s, t & 1, a.err);
+      if (!ok) break;
+      tc_after();
+      float s[LP_TILE];
+      float mx = -INFINITY;
+#pragma unroll
+      for (int sg = 0; sg < 4; ++sg) {
+        if (sg < n) {
+          lp_ld32(tmem + my + 32 * sg, s + 32 * sg);
+          const int j0 = seg_base(4 * t + sg);
+          const bool sink = 4 * t + sg < nss;
+          if (sink || j0 + LP_SEG - 1 > p_lo || p_hi - j0 >= wnd) {
+            // sinks: those of the segment; window: 0 <= p - j < window, or a sink the window has reached
+            const int hi = sink ? st + ns : min(p + 1, st + a.sinks);
+#pragma unroll
+            for (int c = 0; c < 32; ++c) {
+              const int j = j0 + c;
+              const bool see = j < hi || (!sink && (unsigned)(p - j) < (unsigned)wnd);
+              s[32 * sg + c] = see && p >= st ? s[32 * sg + c] : -INFINITY;
+            }
+          }
+#pragma unroll
+          for (int c = 0; c < 32; ++c) mx = fmaxf(mx, s[32 * sg + c]);
+        }
+      }
+      mx *= a.scale;                               // scale > 0 (checked): the maximum of the scaled scores
+      const bool up = mx > m + LP_SLACK;
+      if (__any_sync(FULL, up)) {
+        const float mn = up ? mx : m, f = up ? (m > -INFINITY ? ex2(m - mn) : 0.f) : 1.f;
+        m = mn;
+        sum *= f;
+        if (t > 0) {
+#pragma unroll 1
+          for (int c = 0; c < LG_D; c += 32) {
+            float o[32];
+            lp_ld32(t_o + my + c, o);
+            uint32_t w[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(o[i] * f);
+            lp_st32(t_o + my + c, w);
+          }
+        }
+      }
+      const float off = m > -INFINITY ? -m : 0.f;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        if (2 * half < n) {
+          uint32_t w[32];
+#pragma unroll
+          for (int c = 0; c < 32; ++c) {
+            const float p0 = ex2(fmaf(s[64 * half + 2 * c], a.scale, off));
+            const float p1 = ex2(fmaf(s[64 * half + 2 * c + 1], a.scale, off));
+            if (2 * half + c / 16 < n) sum += p0 + p1;
+            w[c] = pack2(p0, p1);
+          }
+          lp_st32(tmem + my + 32 * half, w);
+        }
+      }
+      tc_before();
+      mbar_arrive(&bar_p);
+    }
+    if (ok && tiles > 0) {
+      ok = mbar_wait_warp(&bar_o, (tiles - 1) & 1, a.err);
+      tc_after();
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    bf16* op = a.out + b * a.o_sb + l * a.o_sl + hq * a.o_sh;
+    bool bad = !isfinite(sum);
+#pragma unroll 1
+    for (int c = 0; c < LG_D; c += 32) {
+      float o[32];
+      if (tiles > 0 && ok) lp_ld32(t_o + my + c, o);
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        bad |= !isfinite(o[i]) && tiles > 0;
+        o[i] = sum == 0.f ? 0.f : o[i] * inv;
+      }
+      if (l < a.L) {
+#pragma unroll
+        for (int i = 0; i < 32; i += 8)
+          *reinterpret_cast<uint4*>(op + c + i) =
+              make_uint4(pack2(o[i], o[i + 1]), pack2(o[i + 2], o[i + 3]), pack2(o[i + 4], o[i + 5]), pack2(o[i + 6], o[i + 7]));
+      }
+    }
+    if (bad && ok && l < a.L) {
+      float* o = reinterpret_cast<float*>(sk) + r;   // K's and V's buffers: every copy and MMA is done
+      long_row_again(a, b, hq, l, start, o);
+      for (int d = 0; d < LG_D; ++d) op[d] = __float2bfloat16_rn(o[d * LP_ROWS]);
     }
   }
-  a.out[b * a.o_sb + l * a.o_sl + hq * a.o_sh + threadIdx.x] = __float2bfloat16_rn(L == 0.f ? 0.f : O / L);
+  tc_before();
+  __syncthreads();
+  if (warp == 4) {
+    tc_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(LP_COLS));
+  }
 }
 
 }  // namespace fb
+
+namespace {
+using namespace fb;
+
+// [B][heads][slots][128] as (64 dims, slots, half, heads, B); boxes of `box` slots x both halves, or 32 x one half
+int lp_map(CUtensorMap* m, const void* base, long long n, int heads, int B, long long sl, long long sh, long long sb,
+           int box) {
+  const unsigned long long dims[5] = {64, (unsigned long long)n, 2, (unsigned long long)heads, (unsigned long long)B};
+  const unsigned long long st[4] = {(unsigned long long)sl * 2, 128, (unsigned long long)(heads > 1 ? sh : LG_D) * 2,
+                                    (unsigned long long)(B > 1 ? sb : LG_D) * 2};
+  const unsigned bx[5] = {64, (unsigned)box, box == LP_SEG ? 1u : 2u, 1, 1};
+  return fbh::tmap_bf16(m, base, 5, dims, st, bx);
+}
+
+}  // namespace
 
 extern "C" int flashb_long_prefill(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_sl, const void* k, int64_t k_sb,
                                    int64_t k_sh, int64_t k_sl, const void* v, int64_t v_sb, int64_t v_sh, int64_t v_sl,
                                    int B, int NH, int NKV, int L, int S, int q_start, const int64_t* starts, int window,
                                    int sinks, float scaling, void* out, int64_t o_sb, int64_t o_sl, int64_t o_sh,
                                    void* stream) {
-  using namespace fb;
   FB_CHECK_ARG(q && k && v && out, "long_prefill: null pointer argument");
   FB_CHECK_ARG(B >= 1 && L >= 1 && NKV >= 1 && NH >= NKV && NH % NKV == 0, "long_prefill: bad shape B=%d NH=%d NKV=%d L=%d",
                B, NH, NKV, L);
@@ -84,14 +367,51 @@ extern "C" int flashb_long_prefill(const void* q, int64_t q_sb, int64_t q_sh, in
     return FB_ERR_UNSUPPORTED;
   }
   FB_CHECK_ARG(q_start >= 0 && (int64_t)q_start + L <= S, "long_prefill: tokens at slots %d .. of a cache of %d", q_start, S);
+  FB_CHECK_ARG(S <= 0x7fffff00, "long_prefill: %d slots", S);
   FB_CHECK_ARG(sinks >= 0, "long_prefill: sinks %d", sinks);
+  FB_CHECK_ARG(scaling > 0.f, "long_prefill: scaling must be positive");
   FB_CHECK_ARG((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & 15) == 0 &&
                    (q_sb | q_sh | q_sl | k_sb | k_sh | k_sl | v_sb | v_sh | v_sl | o_sb | o_sl | o_sh) % 8 == 0,
                "long_prefill: tensors must be 16-byte aligned with strides multiple of 8 elements");
-  FB_CHECK_ARG(q_sl >= LG_D && k_sl >= LG_D && v_sl >= LG_D && NH <= 65535 && B <= 65535, "long_prefill: bad strides or grid");
-  LongPrefillArgs a{(const bf16*)q, (const bf16*)k, (const bf16*)v, q_sb, q_sh, q_sl, k_sb, k_sh, k_sl, v_sb, v_sh, v_sl,
-                    (const long long*)starts, B, NH, NKV, L, q_start, window > 0 ? window : 0, sinks,
-                    scaling * LG_LOG2E, (bf16*)out, o_sb, o_sl, o_sh};
+  FB_CHECK_ARG(q_sl >= LG_D && k_sl >= LG_D && v_sl >= LG_D && NKV <= 65535 && B <= 65535, "long_prefill: bad strides or grid");
+  FB_CHECK_ARG((q_sb | q_sh | k_sb | k_sh | v_sb | v_sh) >= 0 && (B == 1 || (q_sb > 0 && k_sb > 0 && v_sb > 0)) &&
+                   (NH == 1 || q_sh > 0) && (NKV == 1 || (k_sh > 0 && v_sh > 0)),
+               "long_prefill: batch and head strides must be positive");
+  LongPrefillArgs a{};
+  const int nq = LP_ROWS / G;
+  {
+    const unsigned long long dims[5] = {64, (unsigned long long)L, (unsigned long long)NH, 2, (unsigned long long)B};
+    const unsigned long long st[4] = {(unsigned long long)q_sl * 2, (unsigned long long)(NH > 1 ? q_sh : LG_D) * 2, 128,
+                                      (unsigned long long)(B > 1 ? q_sb : LG_D) * 2};
+    const unsigned bx[5] = {64, (unsigned)nq, (unsigned)G, 2, 1};
+    const int rc = fbh::tmap_bf16(&a.tq, q, 5, dims, st, bx);
+    if (rc) return rc;
+  }
+  const long long n = (long long)q_start + L;     // later slots read as zeros
+  int rc = lp_map(&a.tk, k, n, NKV, B, k_sl, k_sh, k_sb, LP_TILE);
+  if (!rc) rc = lp_map(&a.tk32, k, n, NKV, B, k_sl, k_sh, k_sb, LP_SEG);
+  if (!rc) rc = lp_map(&a.tv, v, n, NKV, B, v_sl, v_sh, v_sb, LP_TILE);
+  if (!rc) rc = lp_map(&a.tv32, v, n, NKV, B, v_sl, v_sh, v_sb, LP_SEG);
+  if (rc) return rc;
+  a.q = (const bf16*)q, a.k = (const bf16*)k, a.v = (const bf16*)v;
+  a.q_sb = q_sb, a.q_sh = q_sh, a.q_sl = q_sl, a.k_sb = k_sb, a.k_sh = k_sh, a.k_sl = k_sl;
+  a.v_sb = v_sb, a.v_sh = v_sh, a.v_sl = v_sl;
+  a.starts = (const long long*)starts;
+  a.NH = NH, a.NKV = NKV, a.G = G, a.nq = nq, a.L = L, a.q_start = q_start, a.window = window > 0 ? window : 0, a.sinks = sinks;
+  a.scale = scaling * LG_LOG2E, a.out = (bf16*)out, a.o_sb = o_sb, a.o_sl = o_sl, a.o_sh = o_sh;
+  a.err = fbh::device_err_ptr();
+  static int attr_done[64] = {0};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 64 || !attr_done[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(long_prefill_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, LP_SMEM);
+    if (e != cudaSuccess) {
+      fbh::set_msg("long_prefill: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+      return FB_ERR_CUDA;
+    }
+    if (dev < 64) attr_done[dev] = 1;
+  }
   void* args[] = {(void*)&a};
-  return fbh::launch_pdl((const void*)long_row_kernel, dim3(L, NH, B), dim3(128), 0, (cudaStream_t)stream, args, true);
+  return fbh::launch_pdl((const void*)long_prefill_kernel, dim3((L + nq - 1) / nq, NKV, B), dim3(LP_THREADS), LP_SMEM,
+                         (cudaStream_t)stream, args, true);
 }
