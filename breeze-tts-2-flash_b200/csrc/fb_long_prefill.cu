@@ -8,15 +8,15 @@
 // A CTA computes 128 rows: the G query heads of a KV head for 128 / G tokens.  Packing the group makes the keys that a
 // tile must visit window + 128 / G instead of window + 128, and reads each K and V tile once for the group.  Those keys
 // are cut into segments of 32: the sinks that the window of the CTA's first token does not reach, then the slots from
-// that window's beginning to the CTA's last token.  Four segments are a tile (the last tile may have fewer, and costs
-// as many MMAs as it has); no tile is spent on a handful of sinks alone.
+// that window's beginning to the CTA's last token.  Two segments are a tile (the last one may be half a tile, and costs
+// as many MMAs); no tile is spent on a handful of sinks alone.
 //
-// Per tile: S = Q K^T (TMEM, 128 fp32 columns); warps 0-3 (a thread per row) read their row, subtract the running
-// maximum, take exponentials and write P as bf16 pairs over S's first columns; O += P V with P as the MMA's TMEM
-// operand (128 more columns); one more warp issues the copies and the MMAs.  The chain S -> softmax -> O of one CTA is
-// serial; two CTAs share an SM (96 KB of shared memory, 256 TMEM columns each) and fill each other's gaps.  The running
-// maximum moves only when a tile's exceeds it by 2^8 (the sums are exact either way), so O is hardly ever rescaled.
-// Masks are applied to the segments that need one for some row of the CTA.
+// Per tile: S = Q K^T (TMEM, 64 fp32 columns, two buffers); warps 0-3 (a thread per row) read their row, subtract the
+// running maximum, take exponentials and write P as bf16 pairs over S's first columns; O += P V with P as the MMA's TMEM
+// operand (128 more columns); one more warp issues the copies and the MMAs.  S of the next tile is computed while the
+// exponentials of this one are taken, and two CTAs share an SM (96 KB of shared memory, 256 TMEM columns each).  The
+// running maximum moves only when a tile's exceeds it by 2^8 (the sums are exact either way), so O is hardly ever
+// rescaled.  Masks are applied to the segments that need one for some row of the CTA.
 //
 // Rounding: fp32 scores, statistics and sums; P goes to bf16, the type of V's operand, unnormalised.
 //
@@ -29,15 +29,16 @@
 namespace fb {
 
 constexpr int LP_ROWS = 128;                      // rows of a CTA (TMEM lanes)
-constexpr int LP_SEG = 32, LP_TILE = 128;         // keys per segment and tile
+constexpr int LP_SEG = 32, LP_TILE = 64;          // keys per segment and tile
 constexpr int LP_THREADS = 160;                   // 4 softmax warps, 1 issuing warp
-constexpr int LP_OPND = 128 * LG_D * 2;           // bytes of a 128 x 128 operand
-constexpr int LP_SMEM = 3 * LP_OPND + 1024;       // Q, K, V at a 1024-byte boundary
-constexpr uint32_t LP_COLS = 256;                 // TMEM: S (and P over it) in columns 0-127, O in 128-255
+constexpr int LP_Q = LP_ROWS * LG_D * 2;          // bytes of the Q tile
+constexpr int LP_KV = LP_TILE * LG_D * 2;         // ... of a K or V tile
+constexpr int LP_SMEM = LP_Q + 4 * LP_KV + 1024;  // Q, K and V twice, at a 1024-byte boundary
+constexpr uint32_t LP_COLS = 256;                 // TMEM: S twice (and P over it) in columns 0-127, O in 128-255
 constexpr float LP_SLACK = 8.f;
 
 struct alignas(64) LongPrefillArgs {
-  CUtensorMap tq, tk, tv, tk32, tv32;             // Q tile; K, V: boxes of 128 and of 32 slots
+  CUtensorMap tq, to, tk, tv, tk32, tv32;         // Q and out tiles; K, V: boxes of 64 and of 32 slots
   const bf16 *q, *k, *v;
   long long q_sb, q_sh, q_sl, k_sb, k_sh, k_sl, v_sb, v_sh, v_sl;
   const long long* starts;
@@ -76,6 +77,58 @@ __device__ __forceinline__ void lp_ld32(uint32_t taddr, float* f) {
 #pragma unroll
   for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(r[i]);
 }
+// 64 consecutive fp32 columns of this thread's TMEM lane.
+__device__ __forceinline__ void lp_ld64(uint32_t taddr, float* f) {
+  uint32_t r[64];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
+      "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
+      "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+        "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
+        "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
+        "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+        "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+      : "r"(taddr));
+#pragma unroll
+  for (int i = 0; i < 64; ++i) f[i] = __uint_as_float(r[i]);
+}
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ uint64_t f2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 f2_get(uint64_t x) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+  return r;
+}
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ uint32_t lp_pack(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
 __device__ __forceinline__ void lp_st32(uint32_t taddr, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
@@ -111,21 +164,32 @@ __device__ __noinline__ void long_row_again(const LongPrefillArgs& a, int b, int
   for (int d = 0; d < LG_D; ++d) o[d * LP_ROWS] = sum == 0.f ? 0.f : o[d * LP_ROWS] / sum;
 }
 
+// Bounded wait of a whole warp; the clock is read only after some hundred microseconds of polling.
+__device__ __forceinline__ bool lp_wait(uint64_t* bar, unsigned parity, unsigned* err) {
+  bool ok = false;
+#pragma unroll 1
+  for (int i = 0; i < 256 && !ok; ++i) ok = mbar_try_wait(bar, parity);
+  if (!ok) ok = mbar_wait(bar, parity, err);
+  return __all_sync(FULL, ok);
+}
+
 __global__ void __launch_bounds__(LP_THREADS, 2) long_prefill_kernel(const __grid_constant__ LongPrefillArgs a) {
   extern __shared__ __align__(16) unsigned char raw[];
-  unsigned char* sq = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
-  unsigned char* sk = sq + LP_OPND;
-  unsigned char* sv = sk + LP_OPND;
-  __shared__ __align__(8) uint64_t bar_k, bar_v, bar_s, bar_p, bar_o;
+  unsigned char* sq = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);   // Q; the output tile at the end
+  unsigned char* sk = sq + LP_Q;                                          // [2]
+  unsigned char* sv = sk + 2 * LP_KV;                                     // [2]
+  __shared__ __align__(8) uint64_t bar_k[2], bar_v[2], bar_s[2], bar_p[2], bar_o;
   __shared__ uint32_t tslot;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int qt = gridDim.x - 1 - blockIdx.x;       // the latest tokens first: they have the most keys
   const int h = blockIdx.y, b = blockIdx.z, q0 = qt * a.nq;
   if (tid == 0) {
-    mbar_init(&bar_k, 1);
-    mbar_init(&bar_v, 1);
-    mbar_init(&bar_s, 1);
-    mbar_init(&bar_p, LP_ROWS);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bar_k[i], 1);
+      mbar_init(&bar_v[i], 1);
+      mbar_init(&bar_s[i], 1);
+      mbar_init(&bar_p[i], LP_ROWS);
+    }
     mbar_init(&bar_o, 1);
     fence_mbar_init();
   }
@@ -148,107 +212,130 @@ __global__ void __launch_bounds__(LP_THREADS, 2) long_prefill_kernel(const __gri
   const int lo = a.window > 0 && p_lo - a.window + 1 > st ? p_lo - a.window + 1 : st;
   const int ns = min(a.sinks, lo - st), nss = (ns + LP_SEG - 1) / LP_SEG;
   const int segs = nss + (p_hi + 1 - lo + LP_SEG - 1) / LP_SEG;
-  const int tiles = (segs + 3) >> 2;
+  const int tiles = (segs + 1) >> 1;
   auto seg_base = [&](int s) { return s < nss ? st + LP_SEG * s : lo + LP_SEG * (s - nss); };
 
   if (warp == 4) {
-    auto load = [&](bool is_v, int t) {
-      const int n = min(4, segs - 4 * t);
-      uint64_t* bar = is_v ? &bar_v : &bar_k;
-      unsigned char* dst = is_v ? sv : sk;
-      mbar_arrive_expect_tx(bar, (unsigned)(n * (LP_OPND / 4) + (!is_v && t == 0 ? LP_OPND : 0)));
-      if (n == 4 && 4 * t >= nss) {
-        lp_load(dst, is_v ? &a.tv : &a.tk, seg_base(4 * t), 0, h, b, bar);
+    auto load = [&](bool is_v, int t) {            // lane 0
+      const int n = min(2, segs - 2 * t);
+      uint64_t* bar = is_v ? &bar_v[t & 1] : &bar_k[t & 1];
+      unsigned char* dst = (is_v ? sv : sk) + (t & 1) * LP_KV;
+      mbar_arrive_expect_tx(bar, (unsigned)(n * (LP_KV / 2) + (!is_v && t == 0 ? LP_Q : 0)));
+      if (n == 2 && 2 * t >= nss) {
+        lp_load(dst, is_v ? &a.tv : &a.tk, seg_base(2 * t), 0, h, b, bar);
       } else {
         for (int s = 0; s < n; ++s)
           for (int half = 0; half < 2; ++half)
-            lp_load(dst + half * (LP_OPND / 2) + s * 4096, is_v ? &a.tv32 : &a.tk32, seg_base(4 * t + s), half, h, b, bar);
+            lp_load(dst + half * (LP_KV / 2) + s * (LP_KV / 4), is_v ? &a.tv32 : &a.tk32, seg_base(2 * t + s), half, h, b,
+                    bar);
       }
     };
+    // descriptors are one constant plus a compile-time offset per MMA: built in the loop they cost the issuing thread
+    // more than twice an MMA's 64 cycles
+    const uint64_t dq = tc_desc_sw128(smem_u32(sq)), dk = tc_desc_sw128(smem_u32(sk));
+    const uint64_t dv = tc_desc(smem_u32(sv), LP_KV / 2, 1024, 2);        // dims contiguous: two halves of 64, 8-key groups
+    auto mma_s = [&](int t) {                      // lane 0
+      const uint32_t d = tmem + 64 * (t & 1), idesc = tc_idesc(LP_SEG * min(2, segs - 2 * t));
+      const uint64_t k = dk + (uint64_t)((t & 1) * (LP_KV >> 4));
+#pragma unroll
+      for (int s = 0; s < LG_D / 16; ++s)
+        tc_mma(d, dq + (((s >> 2) * (LP_Q / 2) + (s & 3) * 32) >> 4), k + (((s >> 2) * (LP_KV / 2) + (s & 3) * 32) >> 4),
+               s > 0, idesc);
+      tc_commit(&bar_s[t & 1]);
+    };
     bool ok = true;
-    int kl = 0, vl = 0;                            // K and V copies issued
-    int kw = 0, vw = 0;                            // ... and waited for
+    int seen_k = 0, seen_v = 0;                    // tiles waited for
     if (tiles > 0) {
       if (lane == 0) {
         load(false, 0);
-        lp_load(sq, &a.tq, q0, h * a.G, 0, b, &bar_k);
+        lp_load(sq, &a.tq, q0, h * a.G, 0, b, &bar_k[0]);
         load(true, 0);
-      }
-      kl = vl = 1;
-    }
-    const uint32_t aq = smem_u32(sq), ak = smem_u32(sk), av = smem_u32(sv);
-    for (int t = 0; t < tiles && ok; ++t) {
-      const int n = min(4, segs - 4 * t);
-      ok = mbar_wait_warp(&bar_k, t & 1, a.err);
-      if (!ok) break;
-      ++kw;
-      if (t > 0) {                                 // P V of the last tile done: P's columns and V's buffer are free
-        ok = mbar_wait_warp(&bar_o, (t - 1) & 1, a.err);
-        if (!ok) break;
-        if (lane == 0) load(true, t);
-        ++vl;
-      }
-      tc_after();
-      if (lane == 0) {
-        const uint32_t idesc = tc_idesc(32 * n);
-#pragma unroll
-        for (int s = 0; s < LG_D / 16; ++s) {
-          const uint32_t at = (s >> 2) * (LP_OPND / 2) + (s & 3) * 32;
-          tc_mma(tmem, tc_desc_sw128(aq + at), tc_desc_sw128(ak + at), s > 0, idesc);
+        if (tiles > 1) {
+          load(false, 1);
+          load(true, 1);
         }
-        tc_commit(&bar_s);
       }
-      __syncwarp();
-      ok = mbar_wait_warp(&bar_s, t & 1, a.err);   // K's buffer is free
-      if (!ok) break;
-      if (t + 1 < tiles) {
-        if (lane == 0) load(false, t + 1);
-        ++kl;
+      ok = lp_wait(&bar_k[0], 0, a.err);
+      if (ok) {
+        ++seen_k;
+        tc_after();
+        if (lane == 0) mma_s(0);
       }
-      ok = mbar_wait_warp(&bar_v, t & 1, a.err);
+    }
+    int loaded_k = min(tiles, 2), loaded_v = loaded_k;
+    for (int t = 0; t < tiles && ok; ++t) {
+      if (t + 1 < tiles) {                         // S of the next tile, into the buffer that P V of the last one read
+        ok = lp_wait(&bar_k[(t + 1) & 1], ((t + 1) >> 1) & 1, a.err);
+        if (!ok) break;
+        ++seen_k;
+        if (t > 0) {
+          ok = lp_wait(&bar_o, (t - 1) & 1, a.err);
+          if (!ok) break;
+          if (lane == 0) load(true, t + 1);
+          ++loaded_v;
+        }
+        tc_after();
+        if (lane == 0) mma_s(t + 1);
+        __syncwarp();
+      }
+      ok = lp_wait(&bar_v[t & 1], (t >> 1) & 1, a.err);
       if (!ok) break;
-      ++vw;
-      if (4 * t < nss && 4 * t + 4 >= nss && (ns & 31)) {   // the last sink segment: zero past the sinks
-        const int s = nss - 1 - 4 * t;
+      ++seen_v;
+      const int n = min(2, segs - 2 * t);
+      if ((ns & 31) && (nss - 1) >> 1 == t) {      // the last sink segment: zero past the sinks
+        unsigned char* z = sv + (t & 1) * LP_KV + ((nss - 1) & 1) * (LP_KV / 4);
         for (int i = (ns & 31) * 8 + lane; i < LP_SEG * 8; i += 32)
           for (int half = 0; half < 2; ++half)
-            *reinterpret_cast<uint4*>(sv + half * (LP_OPND / 2) + s * 4096 + i * 16) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(z + half * (LP_KV / 2) + i * 16) = make_uint4(0, 0, 0, 0);
         fence_proxy_async();
         __syncwarp();
       }
-      ok = mbar_wait_warp(&bar_p, t & 1, a.err);
+      ok = lp_wait(&bar_p[t & 1], (t >> 1) & 1, a.err);
       if (!ok) break;
       tc_after();
       if (lane == 0) {
-        const uint32_t idesc = tc_idesc(LG_D) | (1u << 16);   // V: N-major
-        for (int s = 0; s < 2 * n; ++s)
-          lp_mma_ts(t_o, tmem + 8 * s, tc_desc(av + 2048 * s, LP_OPND / 2, 1024, 2), idesc, (t > 0 || s > 0) ? 1u : 0u);
+        constexpr uint32_t idesc = tc_idesc(LG_D) | (1u << 16);   // V: dims contiguous
+        const uint64_t v = dv + (uint64_t)((t & 1) * (LP_KV >> 4));
+        const uint32_t p = tmem + 64 * (t & 1);
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+          if (s < 2 * n) lp_mma_ts(t_o, p + 8 * s, v + ((2048 * s) >> 4), idesc, s > 0 ? 1u : (t > 0 ? 1u : 0u));
         tc_commit(&bar_o);
+        if (t + 2 < tiles) load(false, t + 2);     // P of this tile is in, so its S is done with K
       }
+      if (t + 2 < tiles) ++loaded_k;
       __syncwarp();
     }
     // after a wait that gave up: no copy may be in flight when the CTA ends
-    if (kl > kw) mbar_wait_warp(&bar_k, kw & 1, a.err);
-    if (vl > vw) mbar_wait_warp(&bar_v, vw & 1, a.err);
+    for (; seen_k < loaded_k; ++seen_k) lp_wait(&bar_k[seen_k & 1], (seen_k >> 1) & 1, a.err);
+    for (; seen_v < loaded_v; ++seen_v) lp_wait(&bar_v[seen_v & 1], (seen_v >> 1) & 1, a.err);
   } else {
     const int r = tid, g = r / a.nq, l = q0 + r - g * a.nq, p = a.q_start + l, hq = h * a.G + g;
     const uint32_t my = (uint32_t)(warp * 32) << 16;
     const int wnd = a.window > 0 ? a.window : 0x7fffffff;
-    float m = -INFINITY, sum = 0.f;
+    const uint64_t scale2 = f2(a.scale, a.scale);
+    float m = -INFINITY;
+    uint64_t sum2[2] = {0, 0};
     bool ok = true;
     for (int t = 0; t < tiles; ++t) {
-      const int n = min(4, segs - 4 * t);
-      ok = mbar_wait_warp(&bar_s, t & 1, a.err);
+      const int n = min(2, segs - 2 * t);
+      const uint32_t ts = tmem + my + 64 * (t & 1);
+      ok = lp_wait(&bar_s[t & 1], (t >> 1) & 1, a.err);
       if (!ok) break;
       tc_after();
       float s[LP_TILE];
-      float mx = -INFINITY;
+      if (n == 2) {
+        lp_ld64(ts, s);
+      } else {
+        lp_ld32(ts, s);
 #pragma unroll
-      for (int sg = 0; sg < 4; ++sg) {
+        for (int c = 32; c < 64; ++c) s[c] = -INFINITY;
+      }
+#pragma unroll
+      for (int sg = 0; sg < 2; ++sg) {
         if (sg < n) {
-          lp_ld32(tmem + my + 32 * sg, s + 32 * sg);
-          const int j0 = seg_base(4 * t + sg);
-          const bool sink = 4 * t + sg < nss;
+          const int j0 = seg_base(2 * t + sg);
+          const bool sink = 2 * t + sg < nss;
           if (sink || j0 + LP_SEG - 1 > p_lo || p_hi - j0 >= wnd) {
             // sinks: those of the segment; window: 0 <= p - j < window, or a sink the window has reached
             const int hi = sink ? st + ns : min(p + 1, st + a.sinks);
@@ -259,17 +346,27 @@ __global__ void __launch_bounds__(LP_THREADS, 2) long_prefill_kernel(const __gri
               s[32 * sg + c] = see && p >= st ? s[32 * sg + c] : -INFINITY;
             }
           }
-#pragma unroll
-          for (int c = 0; c < 32; ++c) mx = fmaxf(mx, s[32 * sg + c]);
         }
       }
-      mx *= a.scale;                               // scale > 0 (checked): the maximum of the scaled scores
+      float x[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+      for (int c = 4; c < 64; c += 4) {
+        x[(c >> 2) & 3] = max3(x[(c >> 2) & 3], s[c], s[c + 1]);
+        x[((c >> 2) + 2) & 3] = max3(x[((c >> 2) + 2) & 3], s[c + 2], s[c + 3]);
+      }
+      // scale > 0 (checked): the maximum of the scaled scores
+      const float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * a.scale;
       const bool up = mx > m + LP_SLACK;
       if (__any_sync(FULL, up)) {
         const float mn = up ? mx : m, f = up ? (m > -INFINITY ? ex2(m - mn) : 0.f) : 1.f;
         m = mn;
-        sum *= f;
+        const float2 u = f2_get(f2_add(sum2[0], sum2[1]));
+        sum2[0] = f2(u.x * f, u.y * f);
+        sum2[1] = 0;
         if (t > 0) {
+          ok = lp_wait(&bar_o, (t - 1) & 1, a.err);   // the one before is done: S of this tile came after it
+          if (!ok) break;
+          tc_after();
 #pragma unroll 1
           for (int c = 0; c < LG_D; c += 32) {
             float o[32];
@@ -282,29 +379,25 @@ __global__ void __launch_bounds__(LP_THREADS, 2) long_prefill_kernel(const __gri
         }
       }
       const float off = m > -INFINITY ? -m : 0.f;
+      const uint64_t off2 = f2(off, off);
+      uint32_t w[32];
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        if (2 * half < n) {
-          uint32_t w[32];
-#pragma unroll
-          for (int c = 0; c < 32; ++c) {
-            const float p0 = ex2(fmaf(s[64 * half + 2 * c], a.scale, off));
-            const float p1 = ex2(fmaf(s[64 * half + 2 * c + 1], a.scale, off));
-            if (2 * half + c / 16 < n) sum += p0 + p1;
-            w[c] = pack2(p0, p1);
-          }
-          lp_st32(tmem + my + 32 * half, w);
-        }
+      for (int c = 0; c < 32; ++c) {
+        const float2 e = f2_get(f2_fma(f2(s[2 * c], s[2 * c + 1]), scale2, off2));
+        const float p0 = ex2(e.x), p1 = ex2(e.y);
+        sum2[c & 1] = f2_add(sum2[c & 1], f2(p0, p1));
+        w[c] = lp_pack(p0, p1);
       }
+      lp_st32(ts, w);
       tc_before();
-      mbar_arrive(&bar_p);
+      mbar_arrive(&bar_p[t & 1]);
     }
-    if (ok && tiles > 0) {
-      ok = mbar_wait_warp(&bar_o, (tiles - 1) & 1, a.err);
-      tc_after();
-    }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    bf16* op = a.out + b * a.o_sb + l * a.o_sl + hq * a.o_sh;
+    if (ok && tiles > 1) ok = lp_wait(&bar_o, (tiles - 2) & 1, a.err);
+    if (ok && tiles > 0) ok = lp_wait(&bar_o, (tiles - 1) & 1, a.err);
+    tc_after();
+    // ---- the row, in the layout of the output's tensor map (128-byte swizzle), over Q
+    const float2 u = f2_get(f2_add(sum2[0], sum2[1]));
+    const float sum = u.x + u.y, inv = sum == 0.f ? 0.f : 1.f / sum;
     bool bad = !isfinite(sum);
 #pragma unroll 1
     for (int c = 0; c < LG_D; c += 32) {
@@ -315,17 +408,27 @@ __global__ void __launch_bounds__(LP_THREADS, 2) long_prefill_kernel(const __gri
         bad |= !isfinite(o[i]) && tiles > 0;
         o[i] = sum == 0.f ? 0.f : o[i] * inv;
       }
-      if (l < a.L) {
+      unsigned char* d = sq + (c >> 6) * (LP_Q / 2) + r * 128;
 #pragma unroll
-        for (int i = 0; i < 32; i += 8)
-          *reinterpret_cast<uint4*>(op + c + i) =
-              make_uint4(pack2(o[i], o[i + 1]), pack2(o[i + 2], o[i + 3]), pack2(o[i + 4], o[i + 5]), pack2(o[i + 6], o[i + 7]));
-      }
+      for (int i = 0; i < 32; i += 8)
+        *reinterpret_cast<uint4*>(d + (((((c & 63) + i) >> 3) ^ (r & 7)) << 4)) =
+            make_uint4(lp_pack(o[i], o[i + 1]), lp_pack(o[i + 2], o[i + 3]), lp_pack(o[i + 4], o[i + 5]),
+                       lp_pack(o[i + 6], o[i + 7]));
     }
     if (bad && ok && l < a.L) {
       float* o = reinterpret_cast<float*>(sk) + r;   // K's and V's buffers: every copy and MMA is done
       long_row_again(a, b, hq, l, start, o);
-      for (int d = 0; d < LG_D; ++d) op[d] = __float2bfloat16_rn(o[d * LP_ROWS]);
+      for (int d = 0; d < LG_D; ++d)
+        *reinterpret_cast<bf16*>(sq + (d >> 6) * (LP_Q / 2) + r * 128 + ((((d & 63) >> 3) ^ (r & 7)) << 4) + (d & 7) * 2) =
+            __float2bfloat16_rn(o[d * LP_ROWS]);
+    }
+    fence_proxy_async();
+    named_sync(1, LP_ROWS);
+    if (tid == 0) {                                // tokens past L are outside the map and not written
+      asm volatile("cp.async.bulk.tensor.5d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3, %4, %5}], [%6];" ::"l"(&a.to),
+                   "r"(0), "r"(q0), "r"(h * a.G), "r"(0), "r"(b), "r"(smem_u32(sq))
+                   : "memory");
+      asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group 0;" ::: "memory");
     }
   }
   tc_before();
@@ -348,6 +451,16 @@ int lp_map(CUtensorMap* m, const void* base, long long n, int heads, int B, long
   const unsigned long long st[4] = {(unsigned long long)sl * 2, 128, (unsigned long long)(heads > 1 ? sh : LG_D) * 2,
                                     (unsigned long long)(B > 1 ? sb : LG_D) * 2};
   const unsigned bx[5] = {64, (unsigned)box, box == LP_SEG ? 1u : 2u, 1, 1};
+  return fbh::tmap_bf16(m, base, 5, dims, st, bx);
+}
+
+// [B][L][heads][128] (any strides) as (64 dims, L, heads, half, B); boxes of nq tokens of G heads
+int lp_map_rows(CUtensorMap* m, const void* base, int L, int heads, int B, long long sl, long long sh, long long sb, int nq,
+                int G) {
+  const unsigned long long dims[5] = {64, (unsigned long long)L, (unsigned long long)heads, 2, (unsigned long long)B};
+  const unsigned long long st[4] = {(unsigned long long)(L > 1 ? sl : LG_D) * 2, (unsigned long long)(heads > 1 ? sh : LG_D) * 2,
+                                    128, (unsigned long long)(B > 1 ? sb : LG_D) * 2};
+  const unsigned bx[5] = {64, (unsigned)nq, (unsigned)G, 2, 1};
   return fbh::tmap_bf16(m, base, 5, dims, st, bx);
 }
 
@@ -375,20 +488,15 @@ extern "C" int flashb_long_prefill(const void* q, int64_t q_sb, int64_t q_sh, in
                "long_prefill: tensors must be 16-byte aligned with strides multiple of 8 elements");
   FB_CHECK_ARG(q_sl >= LG_D && k_sl >= LG_D && v_sl >= LG_D && NKV <= 65535 && B <= 65535, "long_prefill: bad strides or grid");
   FB_CHECK_ARG((q_sb | q_sh | k_sb | k_sh | v_sb | v_sh) >= 0 && (B == 1 || (q_sb > 0 && k_sb > 0 && v_sb > 0)) &&
-                   (NH == 1 || q_sh > 0) && (NKV == 1 || (k_sh > 0 && v_sh > 0)),
+                   (NH == 1 || (q_sh > 0 && o_sh > 0)) && (NKV == 1 || (k_sh > 0 && v_sh > 0)) && (B == 1 || o_sb > 0) &&
+                   (L == 1 || o_sl > 0),
                "long_prefill: batch and head strides must be positive");
   LongPrefillArgs a{};
   const int nq = LP_ROWS / G;
-  {
-    const unsigned long long dims[5] = {64, (unsigned long long)L, (unsigned long long)NH, 2, (unsigned long long)B};
-    const unsigned long long st[4] = {(unsigned long long)q_sl * 2, (unsigned long long)(NH > 1 ? q_sh : LG_D) * 2, 128,
-                                      (unsigned long long)(B > 1 ? q_sb : LG_D) * 2};
-    const unsigned bx[5] = {64, (unsigned)nq, (unsigned)G, 2, 1};
-    const int rc = fbh::tmap_bf16(&a.tq, q, 5, dims, st, bx);
-    if (rc) return rc;
-  }
+  int rc = lp_map_rows(&a.tq, q, L, NH, B, q_sl, q_sh, q_sb, nq, G);
+  if (!rc) rc = lp_map_rows(&a.to, out, L, NH, B, o_sl, o_sh, o_sb, nq, G);
   const long long n = (long long)q_start + L;     // later slots read as zeros
-  int rc = lp_map(&a.tk, k, n, NKV, B, k_sl, k_sh, k_sb, LP_TILE);
+  if (!rc) rc = lp_map(&a.tk, k, n, NKV, B, k_sl, k_sh, k_sb, LP_TILE);
   if (!rc) rc = lp_map(&a.tk32, k, n, NKV, B, k_sl, k_sh, k_sb, LP_SEG);
   if (!rc) rc = lp_map(&a.tv, v, n, NKV, B, v_sl, v_sh, v_sb, LP_TILE);
   if (!rc) rc = lp_map(&a.tv32, v, n, NKV, B, v_sl, v_sh, v_sb, LP_SEG);
