@@ -13,7 +13,7 @@
 //
 // Per tile: S = Q K^T (TMEM, 64 fp32 columns, two buffers); warps 0-3 (a thread per row) read their row, subtract the
 // running maximum, take exponentials and write P as bf16 pairs over S's first columns; O += P V with P as the MMA's TMEM
-// operand (128 more columns); one more warp issues the copies and the MMAs.  S of the next tile is computed while the
+// operand (128 more columns); a warp each issues the copies, S and P V.  S of the next tile is computed while the
 // exponentials of this one are taken, and two CTAs share an SM (96 KB of shared memory, 256 TMEM columns each).  The
 // running maximum moves only when a tile's exceeds it by 2^8 (the sums are exact either way), so O is hardly ever
 // rescaled.  Masks are applied to the segments that need one for some row of the CTA.
@@ -23,6 +23,8 @@
 // A slot that a row does not see gets weight 0, and 0 times an infinity or a NaN in V is NaN.  Slots past the tokens
 // read as zeros (the tensor maps end there), sink segments are zeroed past the sinks; what is left are slots that other
 // rows of the CTA see.  So a row whose output is not finite is computed again, one visible key at a time.
+#include <type_traits>
+
 #include "fb_long.cuh"
 #include "fb_tc.cuh"
 
@@ -30,7 +32,7 @@ namespace fb {
 
 constexpr int LP_ROWS = 128;                      // rows of a CTA (TMEM lanes)
 constexpr int LP_SEG = 32, LP_TILE = 64;          // keys per segment and tile
-constexpr int LP_THREADS = 160;                   // 4 softmax warps, 1 issuing warp
+constexpr int LP_THREADS = 224;                   // 4 softmax warps; one each for copies, S and P V
 constexpr int LP_Q = LP_ROWS * LG_D * 2;          // bytes of the Q tile
 constexpr int LP_KV = LP_TILE * LG_D * 2;         // ... of a K or V tile
 constexpr int LP_SMEM = LP_Q + 4 * LP_KV + 1024;  // Q, K and V twice, at a 1024-byte boundary
@@ -164,13 +166,15 @@ __device__ __noinline__ void long_row_again(const LongPrefillArgs& a, int b, int
   for (int d = 0; d < LG_D; ++d) o[d * LP_ROWS] = sum == 0.f ? 0.f : o[d * LP_ROWS] / sum;
 }
 
-// Bounded wait of a whole warp; the clock is read only after some hundred microseconds of polling.
+// Bounded wait; the clock is read only after a long stretch of polling.
 __device__ __forceinline__ bool lp_wait(uint64_t* bar, unsigned parity, unsigned* err) {
-  bool ok = false;
 #pragma unroll 1
-  for (int i = 0; i < 256 && !ok; ++i) ok = mbar_try_wait(bar, parity);
-  if (!ok) ok = mbar_wait(bar, parity, err);
-  return __all_sync(FULL, ok);
+  for (int i = 0; i < 256; ++i)
+    if (mbar_try_wait(bar, parity)) return true;
+  return mbar_wait(bar, parity, err);
+}
+__device__ __forceinline__ bool lp_wait_warp(uint64_t* bar, unsigned parity, unsigned* err) {
+  return __all_sync(FULL, lp_wait(bar, parity, err));
 }
 
 __global__ void __launch_bounds__(LP_THREADS, 2) long_prefill_kernel(const __grid_constant__ LongPrefillArgs a) {
@@ -178,7 +182,7 @@ __global__ void __launch_bounds__(LP_THREADS, 2) long_prefill_kernel(const __gri
   unsigned char* sq = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);   // Q; the output tile at the end
   unsigned char* sk = sq + LP_Q;                                          // [2]
   unsigned char* sv = sk + 2 * LP_KV;                                     // [2]
-  __shared__ __align__(8) uint64_t bar_k[2], bar_v[2], bar_s[2], bar_p[2], bar_o;
+  __shared__ __align__(8) uint64_t bar_k[2], bar_v[2], bar_s[2], bar_p[2], bar_o[2];
   __shared__ uint32_t tslot;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int qt = gridDim.x - 1 - blockIdx.x;       // the latest tokens first: they have the most keys
@@ -189,8 +193,8 @@ __global__ void __launch_bounds__(LP_THREADS, 2) long_prefill_kernel(const __gri
       mbar_init(&bar_v[i], 1);
       mbar_init(&bar_s[i], 1);
       mbar_init(&bar_p[i], LP_ROWS);
+      mbar_init(&bar_o[i], 1);
     }
-    mbar_init(&bar_o, 1);
     fence_mbar_init();
   }
   if (warp == 4) {
@@ -215,8 +219,8 @@ __global__ void __launch_bounds__(LP_THREADS, 2) long_prefill_kernel(const __gri
   const int tiles = (segs + 1) >> 1;
   auto seg_base = [&](int s) { return s < nss ? st + LP_SEG * s : lo + LP_SEG * (s - nss); };
 
-  if (warp == 4) {
-    auto load = [&](bool is_v, int t) {            // lane 0
+  if (warp == 4) {                                 // copies: one thread
+    auto load = [&](bool is_v, int t) {
       const int n = min(2, segs - 2 * t);
       uint64_t* bar = is_v ? &bar_v[t & 1] : &bar_k[t & 1];
       unsigned char* dst = (is_v ? sv : sk) + (t & 1) * LP_KV;
@@ -230,85 +234,75 @@ __global__ void __launch_bounds__(LP_THREADS, 2) long_prefill_kernel(const __gri
                     bar);
       }
     };
-    // descriptors are one constant plus a compile-time offset per MMA: built in the loop they cost the issuing thread
-    // more than twice an MMA's 64 cycles
+    if (lane == 0) {
+      int nk = 0, nv = 0;                          // tiles copied
+      for (int t = 0; t < tiles; ++t) {
+        if (t >= 2 && !lp_wait(&bar_s[t & 1], ((t - 2) >> 1) & 1, a.err)) break;   // S of t - 2 has read its K
+        load(false, t);
+        ++nk;
+        if (t == 0) lp_load(sq, &a.tq, q0, h * a.G, 0, b, &bar_k[0]);
+        if (t >= 2 && !lp_wait(&bar_o[t & 1], ((t - 2) >> 1) & 1, a.err)) break;   // P V of t - 2 has read its V
+        load(true, t);
+        ++nv;
+      }
+      // no copy may be in flight when the CTA ends (after a wait that gave up: nobody else waits for them)
+      for (int t = max(0, nk - 2); t < nk; ++t) lp_wait(&bar_k[t & 1], (t >> 1) & 1, a.err);
+      for (int t = max(0, nv - 2); t < nv; ++t) lp_wait(&bar_v[t & 1], (t >> 1) & 1, a.err);
+    }
+    __syncwarp();
+  } else if (warp == 5) {                          // S: one thread
+    // descriptors are constants plus compile-time offsets: built in the loop they cost the issuing thread more than
+    // twice an MMA's 64 cycles
     const uint64_t dq = tc_desc_sw128(smem_u32(sq)), dk = tc_desc_sw128(smem_u32(sk));
-    const uint64_t dv = tc_desc(smem_u32(sv), LP_KV / 2, 1024, 2);        // dims contiguous: two halves of 64, 8-key groups
-    auto mma_s = [&](int t) {                      // lane 0
-      const uint32_t d = tmem + 64 * (t & 1), idesc = tc_idesc(LP_SEG * min(2, segs - 2 * t));
-      const uint64_t k = dk + (uint64_t)((t & 1) * (LP_KV >> 4));
+    auto step = [&](auto buf, int t) -> bool {
+      constexpr int B = decltype(buf)::value;
+      if (!lp_wait(&bar_k[B], (t >> 1) & 1, a.err)) return false;
+      if (t >= 2 && !lp_wait(&bar_o[B], ((t - 2) >> 1) & 1, a.err)) return false;   // P of t - 2 lay over this buffer
+      tc_after();
+      const uint32_t idesc = segs - 2 * t >= 2 ? tc_idesc(2 * LP_SEG) : tc_idesc(LP_SEG);
 #pragma unroll
       for (int s = 0; s < LG_D / 16; ++s)
-        tc_mma(d, dq + (((s >> 2) * (LP_Q / 2) + (s & 3) * 32) >> 4), k + (((s >> 2) * (LP_KV / 2) + (s & 3) * 32) >> 4),
-               s > 0, idesc);
-      tc_commit(&bar_s[t & 1]);
+        tc_mma(tmem + 64 * B, dq + (((s >> 2) * (LP_Q / 2) + (s & 3) * 32) >> 4),
+               dk + ((B * LP_KV + (s >> 2) * (LP_KV / 2) + (s & 3) * 32) >> 4), s > 0, idesc);
+      tc_commit(&bar_s[B]);
+      return true;
     };
-    bool ok = true;
-    int seen_k = 0, seen_v = 0;                    // tiles waited for
-    if (tiles > 0) {
-      if (lane == 0) {
-        load(false, 0);
-        lp_load(sq, &a.tq, q0, h * a.G, 0, b, &bar_k[0]);
-        load(true, 0);
-        if (tiles > 1) {
-          load(false, 1);
-          load(true, 1);
-        }
-      }
-      ok = lp_wait(&bar_k[0], 0, a.err);
-      if (ok) {
-        ++seen_k;
-        tc_after();
-        if (lane == 0) mma_s(0);
-      }
-    }
-    int loaded_k = min(tiles, 2), loaded_v = loaded_k;
-    for (int t = 0; t < tiles && ok; ++t) {
-      if (t + 1 < tiles) {                         // S of the next tile, into the buffer that P V of the last one read
-        ok = lp_wait(&bar_k[(t + 1) & 1], ((t + 1) >> 1) & 1, a.err);
-        if (!ok) break;
-        ++seen_k;
-        if (t > 0) {
-          ok = lp_wait(&bar_o, (t - 1) & 1, a.err);
-          if (!ok) break;
-          if (lane == 0) load(true, t + 1);
-          ++loaded_v;
-        }
-        tc_after();
-        if (lane == 0) mma_s(t + 1);
-        __syncwarp();
-      }
-      ok = lp_wait(&bar_v[t & 1], (t >> 1) & 1, a.err);
-      if (!ok) break;
-      ++seen_v;
-      const int n = min(2, segs - 2 * t);
+    if (lane == 0)
+      for (int t = 0; t < tiles; t += 2)
+        if (!step(std::integral_constant<int, 0>(), t) ||
+            (t + 1 < tiles && !step(std::integral_constant<int, 1>(), t + 1)))
+          break;
+    __syncwarp();
+  } else if (warp == 6) {                          // P V
+    const uint64_t dv = tc_desc(smem_u32(sv), LP_KV / 2, 1024, 2);   // dims contiguous: two halves of 64, 8-key groups
+    auto step = [&](auto buf, int t) -> bool {
+      constexpr int B = decltype(buf)::value;
+      if (!lp_wait_warp(&bar_v[B], (t >> 1) & 1, a.err)) return false;
       if ((ns & 31) && (nss - 1) >> 1 == t) {      // the last sink segment: zero past the sinks
-        unsigned char* z = sv + (t & 1) * LP_KV + ((nss - 1) & 1) * (LP_KV / 4);
+        unsigned char* z = sv + B * LP_KV + ((nss - 1) & 1) * (LP_KV / 4);
         for (int i = (ns & 31) * 8 + lane; i < LP_SEG * 8; i += 32)
           for (int half = 0; half < 2; ++half)
             *reinterpret_cast<uint4*>(z + half * (LP_KV / 2) + i * 16) = make_uint4(0, 0, 0, 0);
         fence_proxy_async();
         __syncwarp();
       }
-      ok = lp_wait(&bar_p[t & 1], (t >> 1) & 1, a.err);
-      if (!ok) break;
+      if (!lp_wait_warp(&bar_p[B], (t >> 1) & 1, a.err)) return false;
       tc_after();
       if (lane == 0) {
         constexpr uint32_t idesc = tc_idesc(LG_D) | (1u << 16);   // V: dims contiguous
-        const uint64_t v = dv + (uint64_t)((t & 1) * (LP_KV >> 4));
-        const uint32_t p = tmem + 64 * (t & 1);
+        const bool half = segs - 2 * t < 2;
 #pragma unroll
         for (int s = 0; s < 4; ++s)
-          if (s < 2 * n) lp_mma_ts(t_o, p + 8 * s, v + ((2048 * s) >> 4), idesc, s > 0 ? 1u : (t > 0 ? 1u : 0u));
-        tc_commit(&bar_o);
-        if (t + 2 < tiles) load(false, t + 2);     // P of this tile is in, so its S is done with K
+          if (s < 2 || !half)
+            lp_mma_ts(t_o, tmem + 64 * B + 8 * s, dv + ((B * LP_KV + 2048 * s) >> 4), idesc, s > 0 || t > 0);
+        tc_commit(&bar_o[B]);
       }
-      if (t + 2 < tiles) ++loaded_k;
       __syncwarp();
-    }
-    // after a wait that gave up: no copy may be in flight when the CTA ends
-    for (; seen_k < loaded_k; ++seen_k) lp_wait(&bar_k[seen_k & 1], (seen_k >> 1) & 1, a.err);
-    for (; seen_v < loaded_v; ++seen_v) lp_wait(&bar_v[seen_v & 1], (seen_v >> 1) & 1, a.err);
+      return true;
+    };
+    for (int t = 0; t < tiles; t += 2)
+      if (!step(std::integral_constant<int, 0>(), t) || (t + 1 < tiles && !step(std::integral_constant<int, 1>(), t + 1)))
+        break;
   } else {
     const int r = tid, g = r / a.nq, l = q0 + r - g * a.nq, p = a.q_start + l, hq = h * a.G + g;
     const uint32_t my = (uint32_t)(warp * 32) << 16;
@@ -320,7 +314,7 @@ __global__ void __launch_bounds__(LP_THREADS, 2) long_prefill_kernel(const __gri
     for (int t = 0; t < tiles; ++t) {
       const int n = min(2, segs - 2 * t);
       const uint32_t ts = tmem + my + 64 * (t & 1);
-      ok = lp_wait(&bar_s[t & 1], (t >> 1) & 1, a.err);
+      ok = lp_wait_warp(&bar_s[t & 1], (t >> 1) & 1, a.err);
       if (!ok) break;
       tc_after();
       float s[LP_TILE];
@@ -364,7 +358,7 @@ __global__ void __launch_bounds__(LP_THREADS, 2) long_prefill_kernel(const __gri
         sum2[0] = f2(u.x * f, u.y * f);
         sum2[1] = 0;
         if (t > 0) {
-          ok = lp_wait(&bar_o, (t - 1) & 1, a.err);   // the one before is done: S of this tile came after it
+          ok = lp_wait_warp(&bar_o[(t - 1) & 1], ((t - 1) >> 1) & 1, a.err);
           if (!ok) break;
           tc_after();
 #pragma unroll 1
@@ -392,8 +386,8 @@ __global__ void __launch_bounds__(LP_THREADS, 2) long_prefill_kernel(const __gri
       tc_before();
       mbar_arrive(&bar_p[t & 1]);
     }
-    if (ok && tiles > 1) ok = lp_wait(&bar_o, (tiles - 2) & 1, a.err);
-    if (ok && tiles > 0) ok = lp_wait(&bar_o, (tiles - 1) & 1, a.err);
+    if (ok && tiles > 1) ok = lp_wait_warp(&bar_o[tiles & 1], ((tiles - 2) >> 1) & 1, a.err);
+    if (ok && tiles > 0) ok = lp_wait_warp(&bar_o[(tiles - 1) & 1], ((tiles - 1) >> 1) & 1, a.err);
     tc_after();
     // ---- the row, in the layout of the output's tensor map (128-byte swizzle), over Q
     const float2 u = f2_get(f2_add(sum2[0], sum2[1]));
