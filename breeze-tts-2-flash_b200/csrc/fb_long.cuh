@@ -16,6 +16,11 @@ constexpr float LG_LOG2E = 1.4426950408889634f;
 struct LongRow {
   int st, lo, ns, n;
   __device__ __forceinline__ long long slot(int i) const { return i < ns ? st + i : lo + (i - ns); }
+  // the number of slot j, -1 if it is not visible
+  __device__ __forceinline__ int index(int j) const {
+    if (j >= lo) return ns + (j - lo) < n ? ns + (j - lo) : -1;
+    return j >= st && j < st + ns ? j - st : -1;
+  }
 };
 __device__ __forceinline__ LongRow long_row(long long len, long long start, int S, int window, int sinks) {
   const int e = (int)(len < 0 ? 0 : (len > S ? S : len));

@@ -7,7 +7,7 @@
 // Bound: the visible K and V are read once (512 bytes a key and KV head in bf16, 144 in 4 bits) and do 4 G flops per
 // value, so HBM bounds it; below some megabytes the launch and one memory round trip do.
 //
-// Two launches.  long_decode_kernel: the visible keys of every (row, KV head), in chunks, form one list; CTA c of N
+// Few rows: long_cluster_kernel, one launch (below).  Else two launches.  long_decode_kernel: the visible keys of every (row, KV head), in chunks, form one list; CTA c of N
 // takes the c-th N-th of it whatever the rows' lengths are, so ragged batches leave no CTA idle.  A CTA's share is
 // one or more pieces (a contiguous run of one row's keys); each leaves (max, sum, unnormalised out) in a slot of the
 // workspace.  long_merge_kernel joins a row's pieces in order (no atomics: the same inputs give the same bits) and,
@@ -26,9 +26,13 @@
 // G = 8 the second part is a second product.  One bf16 part alone measured 1.3 times the error of fp32 weights.
 // The maximum moves only when a tile's exceeds it by 2^8: the sums are exact either way, and the 32 accumulators are
 // rescaled a few times a piece instead of every tile.
+#include <cooperative_groups.h>
+
 #include <cmath>
 
 #include "fb_long.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace fb {
 
@@ -36,7 +40,9 @@ constexpr int LD_WARPS = 4;
 constexpr int LD_THREADS = 32 * LD_WARPS;
 constexpr int LD_CTAS = 3;              // CTAs per SM (168 registers a thread)
 constexpr int LD_MAXB = 2048;           // batch rows (their geometry sits in shared memory)
-constexpr int LM_THREADS = 256;
+constexpr int LM_THREADS = 256;         // the merge
+constexpr int LC_MAX = 16;              // CTAs of a cluster
+constexpr int LC_CHUNKS = 4;            // chunks a cluster's CTA may have
 constexpr int LD_SLICE = 2048;          // slots per accumulator CTA of the merge
 
 struct LongDecodeArgs {
@@ -199,6 +205,228 @@ __device__ __forceinline__ void long_softmax(float (&s)[NT][4], uint32_t (&pf)[N
   }
 }
 
+// Keys [i_first, i_end) of row (b, h) by the CTA's four warps; each leaves its (max, sum, unnormalised out) in shared
+// memory.  scp: score i of head g goes to scp[i G + g].
+template <int BITS, bool SCORED>
+__device__ __forceinline__ void long_piece(const LongDecodeArgs& a, int b, int h, const LongRow& row, int i_first, int i_end,
+                                           float* scp, float (*s_o)[8][LG_D], float (*s_m)[8], float (*s_l)[8]) {
+  using T = LongTile<BITS>;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int G = a.G;
+  // ---- q of the group, column g: the head's values at the dims this lane's keys hold, zero beyond the group
+  uint32_t qf[8][2];
+  const int qh = BITS == 16 && G <= 4 ? g & 3 : g;
+  float scA = a.scale, scB = a.scale;
+  {
+    const bf16* qp = a.q + b * a.q_sb + (long long)(h * G + qh) * a.q_sh;
+    uint4 w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w[i] = make_uint4(0, 0, 0, 0);
+      // 16-bit keys: dims 32 i + 8 t .. + 7;  4-bit keys: dims 32 t + 8 i .. + 7
+      if (qh < G) w[i] = *reinterpret_cast<const uint4*>(qp + (BITS == 16 ? 32 * i + 8 * t : 32 * t + 8 * i));
+    }
+    if (BITS == 16) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        qf[2 * i][0] = w[i].x;
+        qf[2 * i][1] = w[i].y;
+        qf[2 * i + 1][0] = w[i].z;
+        qf[2 * i + 1][1] = w[i].w;
+      }
+    } else {
+      // fp16 operands: the head is scaled by a power of two to a largest value in [8, 16), so that values down to
+      // 2^-18 of it stay exact and none overflows; the score takes the power back
+      float amax = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float f[8];
+        cvt8(w[i], f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(f[e]));
+      }
+      amax = fmaxf(amax, __shfl_xor_sync(FULL, amax, 1));
+      amax = fmaxf(amax, __shfl_xor_sync(FULL, amax, 2));
+      int ex = (int)(__float_as_uint(amax) >> 23) - 127 - 3;
+      if (amax == 0.f || ex > 120 || ex < -120) ex = ex > 120 ? 120 : (amax == 0.f ? 0 : -120);
+      const float down = __uint_as_float((uint32_t)(127 - ex) << 23);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float f[8];
+        cvt8(w[i], f);
+        qf[2 * i][0] = pack_h2(f[0] * down, f[1] * down);
+        qf[2 * i][1] = pack_h2(f[2] * down, f[3] * down);
+        qf[2 * i + 1][0] = pack_h2(f[4] * down, f[5] * down);
+        qf[2 * i + 1][1] = pack_h2(f[6] * down, f[7] * down);
+      }
+      const float up = __uint_as_float((uint32_t)(127 + ex) << 23);
+      scA = a.scale * __shfl_sync(FULL, up, 8 * t);          // head 2t lives in lanes 4 (2t) ..
+      scB = a.scale * __shfl_sync(FULL, up, 8 * t + 4);
+    }
+  }
+
+  float o[8][4];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
+  LongStat st{-INFINITY, -INFINITY, 0.f, 0.f};
+
+  const unsigned char* kb = a.c.k + b * a.c.k_sb + h * a.c.k_sh;
+  const unsigned char* vb = a.c.v + b * a.c.v_sb + h * a.c.v_sh;
+  for (int i0 = i_first + warp * T::KEYS; i0 < i_end; i0 += T::CHUNK) {
+    float s[T::KEYS / 16][4];
+    uint32_t pf[T::KEYS / 16][2], pl[2];
+    if constexpr (BITS == 16) {
+      // keys past the row's end read its last key (a visible one) and get no weight
+      __align__(16) uint32_t kw[2][16], vw[4][8];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const unsigned char* p = kb + row.slot(min(i0 + g + 8 * e, row.n - 1)) * a.c.k_sp + 16 * t;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(&kw[e][4 * i]) = ld_nc_v4(p + 64 * i);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const unsigned char* p =
+            vb + row.slot(min(i0 + 2 * t + (e & 1) + 8 * (e >> 1), row.n - 1)) * a.c.v_sp + 16 * g;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) *reinterpret_cast<uint4*>(&vw[e][4 * i]) = ld_nc_v4(p + 128 * i);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[0][e] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        mma_bf16(s[0], kw[0][2 * i], kw[1][2 * i], kw[0][2 * i + 1], kw[1][2 * i + 1], qf[i][0], qf[i][1]);
+      long_softmax<BITS, SCORED>(s, pf, pl, st, o, i0, row.n, scA, scB, scp, G, g, t);
+      // dims: row g of tile i is 8 g + i, row g + 8 is 64 + 8 g + i
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int w = i >> 1;
+        const uint32_t sel = (i & 1) ? 0x7632u : 0x5410u;
+        const uint32_t a0 = __byte_perm(vw[0][w], vw[1][w], sel), a1 = __byte_perm(vw[0][4 + w], vw[1][4 + w], sel);
+        const uint32_t a2 = __byte_perm(vw[2][w], vw[3][w], sel), a3 = __byte_perm(vw[2][4 + w], vw[3][4 + w], sel);
+        mma_bf16(o[i], a0, a1, a2, a3, pf[0][0], pf[0][1]);
+        if (G == 8) mma_bf16(o[i], a0, a1, a2, a3, pl[0], pl[1]);
+      }
+    } else {
+      const unsigned char* ksb = a.c.ks + b * a.c.ks_sb + h * a.c.ks_sh;
+      const unsigned char* vsb = a.c.vs + b * a.c.vs_sb + h * a.c.vs_sh;
+      __align__(16) uint32_t kw[2][2][4], vw[2][4][2];
+      uint16_t ksc[2][2];
+      unsigned char vsc[2][4];
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const long long sl = row.slot(min(i0 + 16 * n + g + 8 * e, row.n - 1));
+          *reinterpret_cast<uint4*>(&kw[n][e][0]) = ld_nc_v4(kb + sl * a.c.k_sp + 16 * t);
+          ksc[n][e] = __ldg(reinterpret_cast<const uint16_t*>(ksb + sl * a.c.ks_sp + 2 * t));
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const long long sl = row.slot(min(i0 + 16 * n + 2 * t + (e & 1) + 8 * (e >> 1), row.n - 1));
+          *reinterpret_cast<uint2*>(&vw[n][e][0]) = ld_nc_v2(vb + sl * a.c.v_sp + 8 * g);
+          vsc[n][e] = __ldg(vsb + sl * a.c.vs_sp + g);
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+        const uint32_t sg = e4m3x2_to_h2(ksc[n][0]), sh = e4m3x2_to_h2(ksc[n][1]);   // blocks 2t, 2t + 1
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          uint32_t x[4], y[4];
+          e2m1x8_to_h2(kw[n][0][w], x);
+          e2m1x8_to_h2(kw[n][1][w], y);
+          const uint32_t sel = w < 2 ? 0x1010u : 0x3232u;
+          const uint32_t fx = __byte_perm(sg, sg, sel), fy = __byte_perm(sh, sh, sel);
+          mma_f16(s[n], hmul2(x[0], fx), hmul2(y[0], fy), hmul2(x[1], fx), hmul2(y[1], fy), qf[2 * w][0],
+                  qf[2 * w][1]);
+          mma_f16(s[n], hmul2(x[2], fx), hmul2(y[2], fy), hmul2(x[3], fx), hmul2(y[3], fy), qf[2 * w + 1][0],
+                  qf[2 * w + 1][1]);
+        }
+      }
+      long_softmax<BITS, SCORED>(s, pf, pl, st, o, i0, row.n, scA, scB, scp, G, g, t);
+      // dims: row g of tile i is 16 g + i (first code word), row g + 8 is 16 g + 8 + i (second)
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const uint32_t f0 = e4m3x2_to_h2((uint16_t)(vsc[n][0] | (vsc[n][1] << 8)));   // scales of keys 2t, 2t + 1
+        const uint32_t f1 = e4m3x2_to_h2((uint16_t)(vsc[n][2] | (vsc[n][3] << 8)));
+        uint32_t lo[4][4], hi[4][4];   // [2 word + key pair][byte]: even dims, odd dims, (first key, second key)
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t x = vw[n][2 * e][w], y = vw[n][2 * e + 1][w];
+            e2m1x8_to_h2((x & 0x0f0f0f0fu) | ((y << 4) & 0xf0f0f0f0u), lo[2 * w + e]);
+            e2m1x8_to_h2(((x >> 4) & 0x0f0f0f0fu) | (y & 0xf0f0f0f0u), hi[2 * w + e]);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          mma_f16(o[2 * i], hmul2(lo[0][i], f0), hmul2(lo[2][i], f0), hmul2(lo[1][i], f1), hmul2(lo[3][i], f1),
+                  pf[n][0], pf[n][1]);
+          mma_f16(o[2 * i + 1], hmul2(hi[0][i], f0), hmul2(hi[2][i], f0), hmul2(hi[1][i], f1), hmul2(hi[3][i], f1),
+                  pf[n][0], pf[n][1]);
+        }
+      }
+    }
+  }
+
+  if (BITS == 16 && G <= 4) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[i][e] += __shfl_down_sync(FULL, o[i][e], 2);
+  }
+  // ---- the four warps' parts of the piece, joined in warp order
+#pragma unroll
+  for (int x = 4; x < 32; x <<= 1) {
+    st.lA += __shfl_xor_sync(FULL, st.lA, x);
+    st.lB += __shfl_xor_sync(FULL, st.lB, x);
+  }
+  if (g == 0) {
+    s_m[warp][2 * t] = st.mA;
+    s_m[warp][2 * t + 1] = st.mB;
+    s_l[warp][2 * t] = st.lA;
+    s_l[warp][2 * t + 1] = st.lB;
+  }
+  {
+    const int d0 = BITS == 16 ? 8 * g : 16 * g, d1 = d0 + (BITS == 16 ? 64 : 8);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      if (2 * t + e < G) {
+#pragma unroll
+        for (int i = 0; i < 8; i += 4) {
+          *reinterpret_cast<float4*>(&s_o[warp][2 * t + e][d0 + i]) =
+              make_float4(o[i][e], o[i + 1][e], o[i + 2][e], o[i + 3][e]);
+          *reinterpret_cast<float4*>(&s_o[warp][2 * t + e][d1 + i]) =
+              make_float4(o[i][2 + e], o[i + 1][2 + e], o[i + 2][2 + e], o[i + 3][2 + e]);
+        }
+      }
+    }
+  }
+}
+
+// Joins the four warps' parts in warp order: head gg's maximum, sum and this thread's dim.
+__device__ __forceinline__ void long_join(const float (*s_o)[8][LG_D], const float (*s_m)[8], const float (*s_l)[8], int gg,
+                                          float& M, float& L, float& O) {
+  M = s_m[0][gg];
+#pragma unroll
+  for (int w = 1; w < LD_WARPS; ++w) M = fmaxf(M, s_m[w][gg]);
+  L = O = 0.f;
+#pragma unroll
+  for (int w = 0; w < LD_WARPS; ++w) {
+    const float f = s_m[w][gg] > -INFINITY ? ex2(s_m[w][gg] - M) : 0.f;
+    if (f != 0.f) {                                      // a warp without a tile holds nothing
+      L += f * s_l[w][gg];
+      O += f * s_o[w][gg][threadIdx.x];
+    }
+  }
+}
+
 template <int BITS, bool SCORED>
 __global__ void __launch_bounds__(LD_THREADS, LD_CTAS) long_decode_kernel(const __grid_constant__ LongDecodeArgs a) {
   using T = LongTile<BITS>;
@@ -207,7 +435,7 @@ __global__ void __launch_bounds__(LD_THREADS, LD_CTAS) long_decode_kernel(const 
   int* s_cum = reinterpret_cast<int*>(s_row + a.B);
   __shared__ __align__(16) float s_o[LD_WARPS][8][LG_D];
   __shared__ float s_m[LD_WARPS][8], s_l[LD_WARPS][8];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int tid = threadIdx.x;
   const int G = a.G;
 
   pdl_wait();
@@ -239,218 +467,13 @@ __global__ void __launch_bounds__(LD_THREADS, LD_CTAS) long_decode_kernel(const 
     const LongRow row = s_row[b];
     const int r = b * a.NKV + h;
 
-    // ---- q of the group, column g: the head's values at the dims this lane's keys hold, zero beyond the group
-    uint32_t qf[8][2];
-    const int qh = BITS == 16 && G <= 4 ? g & 3 : g;
-    float scA = a.scale, scB = a.scale;
-    {
-      const bf16* qp = a.q + b * a.q_sb + (long long)(h * G + qh) * a.q_sh;
-      uint4 w[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        w[i] = make_uint4(0, 0, 0, 0);
-        // 16-bit keys: dims 32 i + 8 t .. + 7;  4-bit keys: dims 32 t + 8 i .. + 7
-        if (qh < G) w[i] = *reinterpret_cast<const uint4*>(qp + (BITS == 16 ? 32 * i + 8 * t : 32 * t + 8 * i));
-      }
-      if (BITS == 16) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          qf[2 * i][0] = w[i].x;
-          qf[2 * i][1] = w[i].y;
-          qf[2 * i + 1][0] = w[i].z;
-          qf[2 * i + 1][1] = w[i].w;
-        }
-      } else {
-        // fp16 operands: the head is scaled by a power of two to a largest value in [8, 16), so that values down to
-        // 2^-18 of it stay exact and none overflows; the score takes the power back
-        float amax = 0.f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float f[8];
-          cvt8(w[i], f);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(f[e]));
-        }
-        amax = fmaxf(amax, __shfl_xor_sync(FULL, amax, 1));
-        amax = fmaxf(amax, __shfl_xor_sync(FULL, amax, 2));
-        int ex = (int)(__float_as_uint(amax) >> 23) - 127 - 3;
-        if (amax == 0.f || ex > 120 || ex < -120) ex = ex > 120 ? 120 : (amax == 0.f ? 0 : -120);
-        const float down = __uint_as_float((uint32_t)(127 - ex) << 23);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float f[8];
-          cvt8(w[i], f);
-          qf[2 * i][0] = pack_h2(f[0] * down, f[1] * down);
-          qf[2 * i][1] = pack_h2(f[2] * down, f[3] * down);
-          qf[2 * i + 1][0] = pack_h2(f[4] * down, f[5] * down);
-          qf[2 * i + 1][1] = pack_h2(f[6] * down, f[7] * down);
-        }
-        const float up = __uint_as_float((uint32_t)(127 + ex) << 23);
-        scA = a.scale * __shfl_sync(FULL, up, 8 * t);          // head 2t lives in lanes 4 (2t) ..
-        scB = a.scale * __shfl_sync(FULL, up, 8 * t + 4);
-      }
-    }
-
-    float o[8][4];
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
-    LongStat st{-INFINITY, -INFINITY, 0.f, 0.f};
-
-    const unsigned char* kb = a.c.k + b * a.c.k_sb + h * a.c.k_sh;
-    const unsigned char* vb = a.c.v + b * a.c.v_sb + h * a.c.v_sh;
-    float* scp = SCORED ? a.sc + (long long)r * a.cap * G : nullptr;
-    const int i_end = min(row.n, ch1 * T::CHUNK);
-    for (int i0 = ch0 * T::CHUNK + warp * T::KEYS; i0 < i_end; i0 += T::CHUNK) {
-      float s[T::KEYS / 16][4];
-      uint32_t pf[T::KEYS / 16][2], pl[2];
-      if constexpr (BITS == 16) {
-        // keys past the row's end read its last key (a visible one) and get no weight
-        __align__(16) uint32_t kw[2][16], vw[4][8];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const unsigned char* p = kb + row.slot(min(i0 + g + 8 * e, row.n - 1)) * a.c.k_sp + 16 * t;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(&kw[e][4 * i]) = ld_nc_v4(p + 64 * i);
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const unsigned char* p =
-              vb + row.slot(min(i0 + 2 * t + (e & 1) + 8 * (e >> 1), row.n - 1)) * a.c.v_sp + 16 * g;
-#pragma unroll
-          for (int i = 0; i < 2; ++i) *reinterpret_cast<uint4*>(&vw[e][4 * i]) = ld_nc_v4(p + 128 * i);
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[0][e] = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          mma_bf16(s[0], kw[0][2 * i], kw[1][2 * i], kw[0][2 * i + 1], kw[1][2 * i + 1], qf[i][0], qf[i][1]);
-        long_softmax<BITS, SCORED>(s, pf, pl, st, o, i0, row.n, scA, scB, scp, G, g, t);
-        // dims: row g of tile i is 8 g + i, row g + 8 is 64 + 8 g + i
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int w = i >> 1;
-          const uint32_t sel = (i & 1) ? 0x7632u : 0x5410u;
-          const uint32_t a0 = __byte_perm(vw[0][w], vw[1][w], sel), a1 = __byte_perm(vw[0][4 + w], vw[1][4 + w], sel);
-          const uint32_t a2 = __byte_perm(vw[2][w], vw[3][w], sel), a3 = __byte_perm(vw[2][4 + w], vw[3][4 + w], sel);
-          mma_bf16(o[i], a0, a1, a2, a3, pf[0][0], pf[0][1]);
-          if (G == 8) mma_bf16(o[i], a0, a1, a2, a3, pl[0], pl[1]);
-        }
-      } else {
-        const unsigned char* ksb = a.c.ks + b * a.c.ks_sb + h * a.c.ks_sh;
-        const unsigned char* vsb = a.c.vs + b * a.c.vs_sb + h * a.c.vs_sh;
-        __align__(16) uint32_t kw[2][2][4], vw[2][4][2];
-        uint16_t ksc[2][2];
-        unsigned char vsc[2][4];
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const long long sl = row.slot(min(i0 + 16 * n + g + 8 * e, row.n - 1));
-            *reinterpret_cast<uint4*>(&kw[n][e][0]) = ld_nc_v4(kb + sl * a.c.k_sp + 16 * t);
-            ksc[n][e] = __ldg(reinterpret_cast<const uint16_t*>(ksb + sl * a.c.ks_sp + 2 * t));
-          }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const long long sl = row.slot(min(i0 + 16 * n + 2 * t + (e & 1) + 8 * (e >> 1), row.n - 1));
-            *reinterpret_cast<uint2*>(&vw[n][e][0]) = ld_nc_v2(vb + sl * a.c.v_sp + 8 * g);
-            vsc[n][e] = __ldg(vsb + sl * a.c.vs_sp + g);
-          }
-        }
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
-          const uint32_t sg = e4m3x2_to_h2(ksc[n][0]), sh = e4m3x2_to_h2(ksc[n][1]);   // blocks 2t, 2t + 1
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            uint32_t x[4], y[4];
-            e2m1x8_to_h2(kw[n][0][w], x);
-            e2m1x8_to_h2(kw[n][1][w], y);
-            const uint32_t sel = w < 2 ? 0x1010u : 0x3232u;
-            const uint32_t fx = __byte_perm(sg, sg, sel), fy = __byte_perm(sh, sh, sel);
-            mma_f16(s[n], hmul2(x[0], fx), hmul2(y[0], fy), hmul2(x[1], fx), hmul2(y[1], fy), qf[2 * w][0],
-                    qf[2 * w][1]);
-            mma_f16(s[n], hmul2(x[2], fx), hmul2(y[2], fy), hmul2(x[3], fx), hmul2(y[3], fy), qf[2 * w + 1][0],
-                    qf[2 * w + 1][1]);
-          }
-        }
-        long_softmax<BITS, SCORED>(s, pf, pl, st, o, i0, row.n, scA, scB, scp, G, g, t);
-        // dims: row g of tile i is 16 g + i (first code word), row g + 8 is 16 g + 8 + i (second)
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          const uint32_t f0 = e4m3x2_to_h2((uint16_t)(vsc[n][0] | (vsc[n][1] << 8)));   // scales of keys 2t, 2t + 1
-          const uint32_t f1 = e4m3x2_to_h2((uint16_t)(vsc[n][2] | (vsc[n][3] << 8)));
-          uint32_t lo[4][4], hi[4][4];   // [2 word + key pair][byte]: even dims, odd dims, (first key, second key)
-#pragma unroll
-          for (int w = 0; w < 2; ++w) {
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const uint32_t x = vw[n][2 * e][w], y = vw[n][2 * e + 1][w];
-              e2m1x8_to_h2((x & 0x0f0f0f0fu) | ((y << 4) & 0xf0f0f0f0u), lo[2 * w + e]);
-              e2m1x8_to_h2(((x >> 4) & 0x0f0f0f0fu) | (y & 0xf0f0f0f0u), hi[2 * w + e]);
-            }
-          }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            mma_f16(o[2 * i], hmul2(lo[0][i], f0), hmul2(lo[2][i], f0), hmul2(lo[1][i], f1), hmul2(lo[3][i], f1),
-                    pf[n][0], pf[n][1]);
-            mma_f16(o[2 * i + 1], hmul2(hi[0][i], f0), hmul2(hi[2][i], f0), hmul2(hi[1][i], f1), hmul2(hi[3][i], f1),
-                    pf[n][0], pf[n][1]);
-          }
-        }
-      }
-    }
-
-    if (BITS == 16 && G <= 4) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[i][e] += __shfl_down_sync(FULL, o[i][e], 2);
-    }
-    // ---- the four warps' parts of the piece, joined in warp order
-#pragma unroll
-    for (int x = 4; x < 32; x <<= 1) {
-      st.lA += __shfl_xor_sync(FULL, st.lA, x);
-      st.lB += __shfl_xor_sync(FULL, st.lB, x);
-    }
-    if (g == 0) {
-      s_m[warp][2 * t] = st.mA;
-      s_m[warp][2 * t + 1] = st.mB;
-      s_l[warp][2 * t] = st.lA;
-      s_l[warp][2 * t + 1] = st.lB;
-    }
-    {
-      const int d0 = BITS == 16 ? 8 * g : 16 * g, d1 = d0 + (BITS == 16 ? 64 : 8);
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        if (2 * t + e < G) {
-#pragma unroll
-          for (int i = 0; i < 8; i += 4) {
-            *reinterpret_cast<float4*>(&s_o[warp][2 * t + e][d0 + i]) =
-                make_float4(o[i][e], o[i + 1][e], o[i + 2][e], o[i + 3][e]);
-            *reinterpret_cast<float4*>(&s_o[warp][2 * t + e][d1 + i]) =
-                make_float4(o[i][2 + e], o[i + 1][2 + e], o[i + 2][2 + e], o[i + 3][2 + e]);
-          }
-        }
-      }
-    }
+    long_piece<BITS, SCORED>(a, b, h, row, ch0 * T::CHUNK, min(row.n, ch1 * T::CHUNK),
+                             SCORED ? a.sc + (long long)r * a.cap * G : nullptr, s_o, s_m, s_l);
     __syncthreads();
     const long long piece = (long long)blockIdx.x + r;   // pieces in list order have increasing CTA or row: unique
     for (int gg = 0; gg < G; ++gg) {
-      float M = s_m[0][gg];
-#pragma unroll
-      for (int w = 1; w < LD_WARPS; ++w) M = fmaxf(M, s_m[w][gg]);
-      float L = 0.f, O = 0.f;
-#pragma unroll
-      for (int w = 0; w < LD_WARPS; ++w) {
-        const float f = s_m[w][gg] > -INFINITY ? ex2(s_m[w][gg] - M) : 0.f;
-        if (f != 0.f) {                                    // a warp without a tile holds nothing
-          L += f * s_l[w][gg];
-          O += f * s_o[w][gg][tid];
-        }
-      }
+      float M, L, O;
+      long_join(s_o, s_m, s_l, gg, M, L, O);
       a.po[(piece * G + gg) * LG_D + tid] = O;
       if (tid == 0) {
         a.pm[piece * G + gg] = M;
@@ -461,6 +484,89 @@ __global__ void __launch_bounds__(LD_THREADS, LD_CTAS) long_decode_kernel(const 
     pos += ch1 - ch0;
     if (h == a.NKV - 1 && ch1 == nb) ++b;
   }
+}
+
+// Few rows: a thread-block cluster per (row, KV head), its CTAs on equal runs of chunks; one launch, no workspace.  The
+// parts are joined through distributed shared memory in rank order.  Scores stay in shared memory until the row's
+// maximum and sum are known.
+template <int BITS, bool SCORED>
+__global__ void __launch_bounds__(LD_THREADS, LD_CTAS) long_cluster_kernel(const __grid_constant__ LongDecodeArgs a) {
+  using T = LongTile<BITS>;
+  extern __shared__ __align__(16) unsigned char smem[];
+  float* s_sc = reinterpret_cast<float*>(smem);          // [LC_CHUNKS x CHUNK][G] (weights wanted)
+  __shared__ __align__(16) float s_o[LD_WARPS][8][LG_D];
+  __shared__ float s_m[LD_WARPS][8], s_l[LD_WARPS][8];
+  __shared__ float c_o[8][LG_D], c_m[8], c_l[8];         // this CTA's part, read by its peers
+  __shared__ float s_max[8], s_inv[8];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int tid = threadIdx.x, split = blockIdx.x, ns = gridDim.x;
+  const int r = blockIdx.y, b = r / a.NKV, h = r - b * a.NKV, G = a.G;
+  pdl_wait();
+  pdl_trigger();
+  const LongRow row = long_row(a.lengths[b], a.starts ? a.starts[b] : 0, a.S, a.window, a.sinks);
+  const int nb = (row.n + T::CHUNK - 1) / T::CHUNK;
+  const int i_first = nb * split / ns * T::CHUNK, i_end = min(row.n, nb * (split + 1) / ns * T::CHUNK);
+  long_piece<BITS, SCORED>(a, b, h, row, i_first, i_end, SCORED ? s_sc - (long long)i_first * G : nullptr, s_o, s_m, s_l);
+  __syncthreads();
+  for (int gg = 0; gg < G; ++gg) {
+    float M, L, O;
+    long_join(s_o, s_m, s_l, gg, M, L, O);
+    c_o[gg][tid] = O;
+    if (tid == 0) {
+      c_m[gg] = M;
+      c_l[gg] = L;
+    }
+  }
+  cluster.sync();
+  for (int gg = split; gg < G; gg += ns) {
+    float mv[LC_MAX], lv[LC_MAX], ov[LC_MAX];
+#pragma unroll
+    for (int c = 0; c < LC_MAX; ++c)
+      if (c < ns) {                                      // all peers' loads together
+        mv[c] = *cluster.map_shared_rank(&c_m[gg], c);
+        lv[c] = *cluster.map_shared_rank(&c_l[gg], c);
+        ov[c] = *cluster.map_shared_rank(&c_o[gg][tid], c);
+      }
+    float M = -INFINITY, L = 0.f, O = 0.f;
+#pragma unroll
+    for (int c = 0; c < LC_MAX; ++c)
+      if (c < ns) M = fmaxf(M, mv[c]);
+#pragma unroll
+    for (int c = 0; c < LC_MAX; ++c)
+      if (c < ns && mv[c] > -INFINITY) {
+        const float f = ex2(mv[c] - M);
+        if (f != 0.f) {
+          L += f * lv[c];
+          O += f * ov[c];
+        }
+      }
+    a.out[((long long)b * a.NH + h * G + gg) * LG_D + tid] = __float2bfloat16_rn(L == 0.f ? 0.f : O / L * a.v_scale);
+  }
+  if constexpr (SCORED) {
+    if (tid < G) {
+      float M = -INFINITY, L = 0.f;
+      for (int c = 0; c < ns; ++c) M = fmaxf(M, *cluster.map_shared_rank(&c_m[tid], c));
+      for (int c = 0; c < ns; ++c) {
+        const float m = *cluster.map_shared_rank(&c_m[tid], c);
+        if (m > -INFINITY) L += ex2(m - M) * *cluster.map_shared_rank(&c_l[tid], c);
+      }
+      s_max[tid] = M;
+      s_inv[tid] = L == 0.f ? 0.f : 1.f / L;
+    }
+    __syncthreads();
+    const float* ap = a.acc + b * a.acc_sb + h * a.acc_sh;
+    float* op = a.acc_out + b * a.acco_sb + h * a.acco_sh;
+    for (int i = i_first + tid; i < i_end; i += LD_THREADS) {
+      float w = 0.f;
+      for (int gg = 0; gg < G; ++gg) w += ex2(s_sc[(i - i_first) * G + gg] - s_max[gg]) * s_inv[gg];
+      const long long j = row.slot(i);
+      op[j] = a.decay * ap[j] + w;
+    }
+    if (ap != op || a.decay != 1.f)                      // slots that are not visible
+      for (int j = (int)((long long)a.S * split / ns) + tid; j < (int)((long long)a.S * (split + 1) / ns); j += LD_THREADS)
+        if (row.index(j) < 0) op[j] = a.decay * ap[j];
+  }
+  cluster.sync();                                        // a peer may still be reading this CTA's part
 }
 
 // Joins a row's pieces: CTA (row, y), y < G: head y's output; y >= G: weights of LD_SLICE slots.
@@ -544,11 +650,10 @@ __global__ void __launch_bounds__(LM_THREADS) long_merge_kernel(const __grid_con
     float* op = a.acc_out + b * a.acco_sb + h * a.acco_sh;
     const int j0 = (blockIdx.y - G) * LD_SLICE, j1 = min(a.S, j0 + LD_SLICE);
     for (int j = j0 + tid; j < j1; j += LM_THREADS) {
-      int i = -1;
-      if (j >= row.lo) i = row.ns + (j - row.lo);
-      else if (j >= row.st && j < row.st + row.ns) i = j - row.st;
+      const int i = row.index(j);
+      if (i < 0 && ap == op && a.decay == 1.f) continue;
       float w = 0.f;
-      if (i >= 0 && i < row.n)
+      if (i >= 0)
         for (int gg = 0; gg < G; ++gg) w += ex2(scp[(long long)i * G + gg] - s_m[gg]) * s_inv[gg];
       op[j] = a.decay * ap[j] + w;
     }
@@ -603,6 +708,7 @@ namespace {
 using namespace fb;
 
 struct LongPlan {
+  int split;                                       // CTAs of a row's cluster, 0: the two launches
   int ncta, cap, slices;
   size_t smem;
   int64_t slots, ws_floats, off_m, off_l, off_s;   // float offsets of the workspace's parts
@@ -625,6 +731,18 @@ int long_plan_host(const fb_kv_cache* c, int NH, int window, int sinks, bool sco
   const int chunk = c->bits == 16 ? LongTile<16>::CHUNK : LongTile<4>::CHUNK;
   const int64_t most = (int64_t)c->B * c->NKV * ((p->cap + chunk - 1) / chunk);
   const int64_t want = (int64_t)fbh::grid_sms() * LD_CTAS;
+  // One cluster per row when that fills the keys' work into one wave with few chunks a CTA
+  const int64_t rows = (int64_t)c->B * c->NKV, chunks = (p->cap + chunk - 1) / chunk;
+  int64_t split = want / rows;
+  if (split > LC_MAX) split = LC_MAX;
+  if (split > chunks) split = chunks;
+  p->split = split >= 1 && chunks <= LC_CHUNKS * split && rows <= 65535 ? (int)split : 0;
+  if (p->split) {
+    p->ncta = p->slices = 0;
+    p->smem = scored ? (size_t)LC_CHUNKS * chunk * G * sizeof(float) : 0;
+    p->ws_floats = 0;
+    return FB_OK;
+  }
   p->ncta = (int)(most < want ? most : want);
   p->slots = (int64_t)p->ncta + (int64_t)c->B * c->NKV;
   p->slices = scored ? (c->S + LD_SLICE - 1) / LD_SLICE : 0;
@@ -640,6 +758,22 @@ int long_plan_host(const fb_kv_cache* c, int NH, int window, int sinks, bool sco
 template <int BITS, bool SCORED>
 int long_launch(LongDecodeArgs& a, const LongPlan& p, cudaStream_t st) {
   void* args[] = {(void*)&a};
+  if (p.split) {
+    static int attr_done[64] = {0};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev >= 64 || !attr_done[dev]) {
+      const cudaError_t e =
+          cudaFuncSetAttribute(long_cluster_kernel<BITS, SCORED>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+      if (e != cudaSuccess) {
+        fbh::set_msg("long_decode: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+        return FB_ERR_CUDA;
+      }
+      if (dev < 64) attr_done[dev] = 1;
+    }
+    return fbh::launch_pdl((const void*)long_cluster_kernel<BITS, SCORED>, dim3(p.split, a.B * a.NKV), dim3(LD_THREADS),
+                           p.smem, st, args, true, p.split);
+  }
   int rc = fbh::launch_pdl((const void*)long_decode_kernel<BITS, SCORED>, dim3(p.ncta), dim3(LD_THREADS), p.smem, st,
                            args, true);
   if (rc) return rc;
@@ -664,14 +798,14 @@ extern "C" int flashb_long_decode(const fb_kv_cache* cache, const void* q, int64
   LongDecodeArgs a{};
   int rc = fbh::long_cache(cache, &a.c);
   if (rc) return rc;
-  FB_CHECK_ARG(q && lengths && ws && out, "long_decode: null pointer argument");
+  FB_CHECK_ARG(q && lengths && out, "long_decode: null pointer argument");
   FB_CHECK_ARG((acc == nullptr) == (acc_out == nullptr), "long_decode: acc and acc_out come together");
   LongPlan p;
   rc = long_plan_host(cache, NH, window, sinks, acc != nullptr, &p);
   if (rc) return rc;
   FB_CHECK_ARG(((uintptr_t)q & 15) == 0 && q_sb % 8 == 0 && q_sh % 8 == 0,
                "long_decode: q must be 16-byte aligned with strides multiple of 8 elements");
-  FB_CHECK_ARG(((uintptr_t)ws & 15) == 0 && ws_floats >= p.ws_floats, "long_decode: workspace of %lld floats, %lld needed",
+  FB_CHECK_ARG(p.ws_floats == 0 || (ws && ((uintptr_t)ws & 15) == 0 && ws_floats >= p.ws_floats), "long_decode: workspace of %lld floats, %lld needed",
                (long long)ws_floats, (long long)p.ws_floats);
   a.q = (const bf16*)q, a.q_sb = q_sb, a.q_sh = q_sh;
   a.lengths = (const long long*)lengths, a.starts = (const long long*)starts;

@@ -26,15 +26,17 @@ from . import _native
 from ._native import FB_ERR_ARG, FbKVCache, FlashbError, check
 
 D = 128
+_BF16, _I64, _F32 = torch.bfloat16, torch.int64, torch.float32
+_raw_stream = torch._C._cuda_getCurrentRawStream       # device index -> cudaStream_t (current_stream() builds an object)
+
+
+def _refuse(msg):
+    raise FlashbError(FB_ERR_ARG, msg)
 
 
 def _ensure(cond, msg):
     if not cond:
-        raise FlashbError(FB_ERR_ARG, msg)
-
-
-def _stream(dev):
-    return torch.cuda.current_stream(dev).cuda_stream
+        _refuse(msg)
 
 
 class KVCache:
@@ -52,8 +54,9 @@ class KVCache:
         self._set(keys, values)
 
     def _set(self, k, v, ks=None, vs=None, k_scale=1.0, v_scale=1.0):
-        self.device = k.device
+        self.device, self.index = k.device, k.get_device()
         self.B, self.NKV, self.S = k.shape[:3]
+        self._ws = {}
         st = list(k.stride()[:3]) + list(v.stride()[:3])
         # the stride of an axis of one entry is never used
         for i in range(6):
@@ -93,57 +96,67 @@ class KV4Cache(KVCache):
     @classmethod
     def empty(cls, B, NKV, S, device='cuda', k_scale=1.0, v_scale=1.0):
         """An empty (zeroed) cache of B rows, NKV heads and S slots."""
-        t = [torch.zeros(B, NKV, S, w, dtype=torch.uint8, device=device) for w in (D // 2, D // 16) * 2]
-        return cls(*t, k_scale=k_scale, v_scale=v_scale)
+        n = B * NKV * S
+        t = torch.zeros(n * 2 * (D // 2 + D // 16), dtype=torch.uint8, device=device).split(
+            [n * D // 2, n * D // 2, n * D // 16, n * D // 16])
+        kq, vq, ks, vs = (x.view(B, NKV, S, w) for x, w in zip(t, (D // 2, D // 2, D // 16, D // 16)))
+        return cls(kq, ks, vq, vs, k_scale=k_scale, v_scale=v_scale)
 
     def _slots(self, slots, L):
-        _ensure(slots.dtype == torch.int64 and slots.device == self.device and slots.shape[-1] == L and
-                slots.stride(-1) in (1, L) and (slots.dim() == 1 or slots.shape == (self.B, L)),
-                'slots: [L] or [B, L] int64 on the cache\'s device')
+        """The row stride of a slot list of L entries."""
+        shape = slots.shape
+        if slots.dtype != _I64 or slots.device != self.device or not (
+                slots.dim() == 1 and shape[0] == L or slots.dim() == 2 and shape == (self.B, L)) or (
+                L > 1 and slots.stride(-1) != 1):
+            _refuse('slots: [L] or [B, L] int64 on the cache\'s device')
         return slots.stride(0) if slots.dim() == 2 and self.B > 1 else 0
+
+    def _heads(self, t, L):
+        shape = t.shape
+        return (t.dtype == _BF16 and t.device == self.device and shape == (self.B, self.NKV, L, D) and t.stride(3) == 1)
 
     def store(self, k, v, slots):
         """Stores bf16 heads ``k`` / ``v`` [B, NKV, L, 128] at ``slots`` ([L], or [B, L]: one list per row; distinct
         within a row, those outside the cache are skipped).  To nearest, ties to even, as in exact arithmetic."""
-        for t, n in ((k, 'k'), (v, 'v')):
-            _ensure(t.dtype == torch.bfloat16 and t.device == self.device and t.dim() == 4 and t.shape[0] == self.B and
-                    t.shape[1] == self.NKV and t.shape[3] == D and t.stride(3) == 1 and t.shape[2] == k.shape[2],
-                    f'{n}: [B, NKV, L, 128] bf16 on the cache\'s device')
-        L = k.shape[2]
+        L = slots.shape[-1]
+        if not self._heads(k, L) or not self._heads(v, L):
+            _refuse('k, v: [B, NKV, L, 128] bf16 on the cache\'s device, L as in slots')
         sb = self._slots(slots, L)
         if L == 0:
             return
         check(_native.lib().flashb_kv4_store(self._ref, k.data_ptr(), *_strides(k), v.data_ptr(), *_strides(v),
-                                             slots.data_ptr(), sb, L, _stream(self.device)))
+                                             slots.data_ptr(), sb, L, _raw_stream(self.index)))
 
     def read(self, slots):
         """The values at ``slots`` ([L] or [B, L]) as (k, v), each [B, NKV, L, 128] bf16 (0 outside the cache)."""
         L = slots.shape[-1]
         sb = self._slots(slots, L)
-        out = torch.empty(2, self.B, self.NKV, L, D, dtype=torch.bfloat16, device=self.device)
-        k, v = out[0], out[1]
+        k = torch.empty(self.B, self.NKV, L, D, dtype=_BF16, device=self.device)
+        v = torch.empty_like(k)
         if L:
             check(_native.lib().flashb_kv4_read(self._ref, slots.data_ptr(), sb, L, k.data_ptr(), v.data_ptr(),
-                                                _stream(self.device)))
+                                                _raw_stream(self.index)))
         return k, v
 
 
 def _strides(t):
     """(batch, head, position) strides in elements, 0 (the row for the position) where the axis has one entry."""
-    s, n = t.stride(), t.shape
-    return (s[0] if n[0] > 1 else 0, s[1] if n[1] > 1 else 0, s[2] if n[2] > 1 else D)
+    sb, sh, sp, _ = t.stride()
+    nb, nh, n, _ = t.shape
+    return sb if nb > 1 else 0, sh if nh > 1 else 0, sp if n > 1 else D
 
 
 def _rows(t, name, B, dev):
-    _ensure(t.dtype == torch.int64 and t.device == dev and t.shape == (B,) and (B == 1 or t.stride(0) == 1),
-            f'{name}: [B] int64 on the cache\'s device')
+    if t.dtype != _I64 or t.device != dev or t.shape != (B,) or not t.is_contiguous():
+        _refuse(name + ': [B] int64 on the cache\'s device')
     return t.data_ptr()
 
 
 def _acc(t, name, cache, least):
-    _ensure(t.dtype == torch.float32 and t.device == cache.device and t.dim() == 3 and t.shape[0] == cache.B and
-            t.shape[1] == cache.NKV and t.shape[2] >= least and t.stride(2) == 1,
-            f'{name}: [B, NKV, {least}] fp32 on the cache\'s device with unit stride per slot')
+    shape = t.shape
+    if t.dtype != _F32 or t.device != cache.device or len(shape) != 3 or shape[0] != cache.B or shape[1] != cache.NKV or \
+            shape[2] < least or t.stride(2) != 1:
+        _refuse(f'{name}: [B, NKV, {least}] fp32 on the cache\'s device with unit stride per slot')
     return t.data_ptr(), t.stride(0), t.stride(1)
 
 
@@ -156,61 +169,78 @@ def decode(query, cache, lengths, *, starts=None, window=None, sinks=0, scaling=
     slot, summed over the query heads of its group, is added: acc_out = decay acc + weight (``acc_out`` None: in place).
     The same inputs give the same bits."""
     dev, B = cache.device, cache.B
-    _ensure(query.dtype == torch.bfloat16 and query.device == dev and query.dim() == 4 and query.shape[0] == B and
-            query.shape[2] == 1 and query.shape[3] == D and query.stride(3) == 1,
-            'query: [B, NH, 1, 128] bf16 on the cache\'s device')
-    _ensure(window is None or window >= 1, 'window: at least 1, or None')
-    NH = query.shape[1]
-    w = 0 if window is None else int(window)
+    shape, st = query.shape, query.stride()
+    if query.dtype != _BF16 or query.device != dev or len(shape) != 4 or shape[0] != B or shape[2] != 1 or \
+            shape[3] != D or st[3] != 1:
+        _refuse('query: [B, NH, 1, 128] bf16 on the cache\'s device')
+    if window is None:
+        window = 0
+    elif window < 1:
+        _refuse('window: at least 1, or None')
+    NH = shape[1]
     lib = _native.lib()
     if acc is not None:
         ap = _acc(acc, 'acc', cache, cache.S)
         op = ap if acc_out is None else _acc(acc_out, 'acc_out', cache, cache.S)
     else:
-        _ensure(acc_out is None, 'acc_out without acc')
-        ap = op = (None, 0, 0)
+        if acc_out is not None:
+            _refuse('acc_out without acc')
+        ap = op = _NO_ACC
     if out is None:
-        out = torch.empty(B, 1, NH, D, dtype=torch.bfloat16, device=dev)
-    else:
-        _ensure(out.dtype == torch.bfloat16 and out.device == dev and out.is_contiguous() and out.numel() == B * NH * D,
-                'out: [B, 1, NH, 128] bf16 contiguous')
-    n = lib.flashb_long_decode_ws_floats(cache._ref, NH, w, sinks, acc is not None)
-    if n < 0:
-        check(lib.flashb_long_decode(cache._ref, query.data_ptr(), 0, 0, NH, lengths.data_ptr(), None, w, sinks, 1.0,
-                                     None, 0, 0, None, 0, 0, 1.0, 16, 0, out.data_ptr(), None))
-    ws = torch.empty(n, dtype=torch.float32, device=dev)
+        out = torch.empty(B, 1, NH, D, dtype=_BF16, device=dev)
+    elif out.dtype != _BF16 or out.device != dev or not out.is_contiguous() or out.numel() != B * NH * D:
+        _refuse('out: [B, 1, NH, 128] bf16 contiguous')
+    key = (NH, window, sinks, acc is not None, lib.flashb_sm_budget())
+    n = cache._ws.get(key)                                # the workspace's size follows from the shapes alone
+    if n is None:
+        n = lib.flashb_long_decode_ws_floats(cache._ref, NH, window, sinks, acc is not None)
+        if n >= 0:
+            cache._ws[key] = n
+    ws = torch.empty(n, dtype=_F32, device=dev) if n > 0 else None
     check(lib.flashb_long_decode(
-        cache._ref, query.data_ptr(), query.stride(0) if B > 1 else 0, query.stride(1) if NH > 1 else 0, NH,
-        _rows(lengths, 'lengths', B, dev), None if starts is None else _rows(starts, 'starts', B, dev), w, sinks,
-        D ** -0.5 if scaling is None else scaling, *ap, *op, decay, ws.data_ptr(), n, out.data_ptr(), _stream(dev)))
+        cache._ref, query.data_ptr(), st[0] if B > 1 else 0, st[1] if NH > 1 else 0, NH,
+        _rows(lengths, 'lengths', B, dev), None if starts is None else _rows(starts, 'starts', B, dev), window, sinks,
+        D ** -0.5 if scaling is None else scaling, *ap, *op, decay, None if ws is None else ws.data_ptr(), n,
+        out.data_ptr(), _raw_stream(cache.index)))
     return out
+
+
+_NO_ACC = (None, 0, 0)
+
+
+def _bf16_heads(t, B, dev):
+    shape = t.shape
+    return t.dtype == _BF16 and t.device == dev and len(shape) == 4 and shape[0] == B and shape[3] == D and t.stride(3) == 1
 
 
 def prefill(query, key, value, *, window=None, sinks=0, starts=None, q_start=None, scaling=None, out=None):
     """Attention of L tokens, those at slots q_start .. q_start + L - 1 (``q_start`` None: the last L slots of
     ``key``): ``query`` [B, NH, L, 128] over ``key`` / ``value`` [B, NKV, S, 128], bf16 with any strides that are
-    multiples of 8 elements.  Returns out [B, L, NH, 128] bf16.  Slots from q_start + L on are not read."""
+    multiples of 8 elements; ``scaling`` > 0.  Returns out [B, L, NH, 128] bf16.  Slots from q_start + L on are not
+    read."""
     dev = query.device
-    for t, n in ((query, 'query'), (key, 'key'), (value, 'value')):
-        _ensure(t.is_cuda and t.device == dev and t.dtype == torch.bfloat16 and t.dim() == 4 and t.shape[3] == D and
-                t.stride(3) == 1 and t.shape[0] == query.shape[0], f'{n}: [B, heads, slots, 128] bf16 CUDA')
     B, NH, L = query.shape[:3]
-    NKV, S = key.shape[1:3]
-    _ensure(value.shape == key.shape, 'key and value differ in shape')
-    _ensure(window is None or window >= 1, 'window: at least 1, or None')
+    if not query.is_cuda or not (_bf16_heads(query, B, dev) and _bf16_heads(key, B, dev) and _bf16_heads(value, B, dev)):
+        _refuse('query, key, value: [B, heads, slots, 128] bf16 on one CUDA device')
+    NKV, S = key.shape[1], key.shape[2]
+    if value.shape != key.shape:
+        _refuse('key and value differ in shape')
+    if window is None:
+        window = 0
+    elif window < 1:
+        _refuse('window: at least 1, or None')
     if out is None:
-        out = torch.empty(B, L, NH, D, dtype=torch.bfloat16, device=dev)
-    else:
-        _ensure(out.dtype == torch.bfloat16 and out.device == dev and out.shape == (B, L, NH, D) and out.stride(3) == 1,
-                'out: [B, L, NH, 128] bf16')
+        out = torch.empty(B, L, NH, D, dtype=_BF16, device=dev)
+    elif not _bf16_heads(out, B, dev) or out.shape != (B, L, NH, D):
+        _refuse('out: [B, L, NH, 128] bf16')
     if L == 0:
         return out
-    o = out.stride()
+    ob, ol, oh, _ = out.stride()
     check(_native.lib().flashb_long_prefill(
         query.data_ptr(), *_strides(query), key.data_ptr(), *_strides(key), value.data_ptr(), *_strides(value), B, NH,
-        NKV, L, S, S - L if q_start is None else int(q_start), None if starts is None else _rows(starts, 'starts', B, dev),
-        0 if window is None else int(window), sinks, D ** -0.5 if scaling is None else scaling, out.data_ptr(), o[0],
-        o[1], o[2], _stream(dev)))
+        NKV, L, S, S - L if q_start is None else q_start, None if starts is None else _rows(starts, 'starts', B, dev),
+        window, sinks, D ** -0.5 if scaling is None else scaling, out.data_ptr(), ob, ol, oh,
+        _raw_stream(query.get_device())))
     return out
 
 
@@ -225,12 +255,15 @@ def evict(cache, acc, lengths, keep, *, into, starts=None, sinks=0, recent=0, ac
     slot 0."""
     dev, B = cache.device, cache.B
     a = _acc(acc, 'acc', cache, cache.S)
-    _ensure(into.bits == cache.bits and into.device == dev, 'into: a cache of the same kind on the same device')
+    if into.bits != cache.bits or into.device != dev:
+        _refuse('into: a cache of the same kind on the same device')
+    if keep < 1:
+        _refuse('keep: at least 1')
     kept = torch.empty(B, cache.NKV, keep, dtype=torch.int32, device=dev)
-    n = torch.empty(B, dtype=torch.int64, device=dev) if lengths_into is None else lengths_into
-    ao = torch.empty(B, cache.NKV, keep, dtype=torch.float32, device=dev) if acc_into is None else acc_into
+    n = torch.empty(B, dtype=_I64, device=dev) if lengths_into is None else lengths_into
+    ao = torch.empty(B, cache.NKV, keep, dtype=_F32, device=dev) if acc_into is None else acc_into
     check(_native.lib().flashb_kv_evict(
         cache._ref, *a, _rows(lengths, 'lengths', B, dev), None if starts is None else _rows(starts, 'starts', B, dev),
         keep, sinks, recent, into._ref, *_acc(ao, 'acc_into', into, keep), ao.shape[2], kept.data_ptr(),
-        _rows(n, 'lengths_into', B, dev), _stream(dev)))
+        _rows(n, 'lengths_into', B, dev), _raw_stream(cache.index)))
     return kept, n, ao

@@ -47,8 +47,9 @@ def test_bad_4bit_descriptors(bad):
 def test_bad_decode_arguments():
     d = desc()
     for kw in (dict(q=None), dict(lengths=None), dict(ws=None), dict(out=None), dict(q=(1 << 24) + 2), dict(q_sb=12),
-               dict(acc=1 << 20), dict(acc_out=1 << 20), dict(NH=7), dict(NH=1), dict(sinks=-1), dict(n=10)):
-        assert decode(d, **kw) == FB_ERR_ARG, kw
+               dict(acc=1 << 20), dict(acc_out=1 << 20), dict(NH=7), dict(NH=1), dict(sinks=-1)):
+        assert decode(desc(B=500), **kw) == FB_ERR_ARG, kw
+    assert decode(desc(B=500), n=10) == FB_ERR_ARG and 'workspace' in _native.last_error()
     assert decode(d, NH=6) == FB_ERR_UNSUPPORTED and 'group 3' in _native.last_error()
     assert decode(desc(B=5000)) == FB_ERR_UNSUPPORTED
 
@@ -56,9 +57,11 @@ def test_bad_decode_arguments():
 def test_workspace_sizes():
     L = _native.lib()
     ws = lambda d, NH, w, s, sc: L.flashb_long_decode_ws_floats(ctypes.byref(d), NH, w, s, sc)  # noqa: E731
-    assert ws(desc(), 8, 0, 0, 0) > 0
-    assert ws(desc(S=4096), 8, 0, 0, 1) - ws(desc(S=4096), 8, 0, 0, 0) == 2 * 2 * 4096 * 4   # the scores
-    assert ws(desc(S=4096), 8, 100, 28, 1) - ws(desc(S=4096), 8, 100, 28, 0) == 2 * 2 * 128 * 4
+    assert ws(desc(), 8, 0, 0, 0) == 0 and ws(desc(), 8, 0, 0, 1) == 0                 # few rows need none
+    many = desc(B=500, S=4096)
+    assert ws(many, 8, 0, 0, 0) > 0
+    assert ws(many, 8, 0, 0, 1) - ws(many, 8, 0, 0, 0) == 500 * 2 * 4096 * 4           # the scores
+    assert ws(many, 8, 100, 28, 1) - ws(many, 8, 100, 28, 0) == 500 * 2 * 128 * 4
     assert ws(desc(), 6, 0, 0, 0) == -1
 
 
