@@ -252,7 +252,7 @@ def evict(cache, acc, lengths, keep, *, into, starts=None, sinks=0, recent=0, ac
 
     Returns (kept [B, NKV, keep] int32: the slot each came from, -1 beyond; lengths [B] int64 of ``into``; the moved
     weights: ``acc_into`` [B, NKV, >= keep], all of it, or a new [B, NKV, keep]; 0 beyond).  ``into``'s rows start at
-    slot 0."""
+    slot 0.  Outputs may not be the inputs' tensors."""
     dev, B = cache.device, cache.B
     a = _acc(acc, 'acc', cache, cache.S)
     if into.bits != cache.bits or into.device != dev:

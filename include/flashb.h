@@ -277,7 +277,8 @@ int flashb_kv4_read(const fb_kv_cache* cache, const int64_t* slots, int64_t slot
  * with `cache`): all when there are no more, else the first `sinks`, the last `recent` (sinks + recent <= keep) and
  * the others of largest acc[b, h, .] (fp32, unit stride per slot; equal weights: the lower slot; NaN above all), each
  * KV head for itself.  kept [B, NKV, keep] int32: the slot each came from, -1 beyond; lengths_out [B] int64: how many
- * (may not be `lengths`); acc_out (or NULL) [B, NKV, acc_n >= keep] fp32: the weights moved along, 0 beyond. */
+ * (may not be `lengths`); acc_out (or NULL; may not be acc) [B, NKV, acc_n >= keep] fp32: the weights moved along, 0
+ * beyond. */
 int flashb_kv_evict(const fb_kv_cache* cache, const float* acc, int64_t acc_sb, int64_t acc_sh, const int64_t* lengths,
                     const int64_t* starts, int keep, int sinks, int recent, const fb_kv_cache* into, float* acc_out,
                     int64_t acco_sb, int64_t acco_sh, int acc_n, int32_t* kept, int64_t* lengths_out, void* stream);

@@ -85,14 +85,15 @@ def test_bad_prefill_store_and_evict_arguments():
         assert store(desc(bits=4), **kw) == FB_ERR_ARG, kw
     assert L.flashb_kv4_read(ctypes.byref(desc(bits=4)), p, 0, 4, p + 8, p, None) == FB_ERR_ARG
 
-    def evict(a, b, keep=8, sinks=0, recent=0, acc=p, acc_n=8):
-        return L.flashb_kv_evict(ctypes.byref(a), acc, 128, 64, p, None, keep, sinks, recent, ctypes.byref(b), p, 128, 64,
-                                 acc_n, p, p, None)
+    def evict(a, b, keep=8, sinks=0, recent=0, acc=p, acc_n=8, acc_out=2 * p, lengths_out=2 * p):
+        return L.flashb_kv_evict(ctypes.byref(a), acc, 128, 64, p, None, keep, sinks, recent, ctypes.byref(b), acc_out, 128, 64,
+                                 acc_n, p, lengths_out, None)
     other = dict(k=1 << 30, v=1 << 31)
     for a, b, kw in ((desc(), desc(), {}), (desc(), desc(bits=4, **other), {}), (desc(), desc(B=1, **other), {}),
                      (desc(), desc(**other), dict(keep=0)), (desc(), desc(**other), dict(keep=65)),
                      (desc(), desc(**other), dict(sinks=5, recent=4)), (desc(), desc(**other), dict(sinks=-1)),
                      (desc(), desc(**other), dict(acc=None)), (desc(), desc(**other), dict(acc_n=7)),
+                     (desc(), desc(**other), dict(acc_out=p)), (desc(), desc(**other), dict(lengths_out=p)),
                      (desc(bits=4), desc(bits=4, k_scale=2.0, **other), {})):
         assert evict(a, b, **kw) == FB_ERR_ARG, kw
 
