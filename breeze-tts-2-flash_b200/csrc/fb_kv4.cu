@@ -10,8 +10,9 @@
 // max / 6 with 8 against 7), while the product is off by less than 2^-22: rounding it to 16 fraction bits puts every
 // tie exactly on the tie and leaves all others on their side, so the codes are those of exact arithmetic.
 //
-// Bound: HBM, 328 bytes a head and token.  A thread owns 8 values (one 16-byte load, 4 bytes of codes); its block's
-// maximum is one shuffle away.
+// Bound: HBM, 328 bytes a head and token.  A thread owns a block (two 16-byte loads, 8 bytes of codes, one scale), so
+// the block's maximum, scale and reciprocal are its own; the maximum is taken on the bf16 bit patterns, two at a time,
+// where a NaN or an infinity shows as the largest.
 #include "fb_long.cuh"
 
 namespace fb {
@@ -25,87 +26,98 @@ struct KV4Args {
   const long long* slots;
   long long slot_sb;
   int NKV, L, S;
-  float k_scale, v_scale;
+  float k_scale, v_scale, k_inv, v_inv;    // powers of two and their inverses
 };
 
-// x to 16 fraction bits, nearest (see the header); NaN and infinity pass
-__device__ __forceinline__ float snap16(float x) {
-  return isfinite(x) ? __uint_as_float((__float_as_uint(x) + 0x40u) & 0xffffff80u) : x;
-}
+// x to 16 fraction bits, nearest (see the header); an infinity stays one
+__device__ __forceinline__ float snap16(float x) { return __uint_as_float((__float_as_uint(x) + 0x40u) & 0xffffff80u); }
 __device__ __forceinline__ unsigned char f_to_e4m3(float x) {
   uint16_t r;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(0.f), "f"(x));
   return (unsigned char)(r & 0xff);
 }
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
-// Block of 16 threads per head: grid (tokens / rows per CTA, B * NKV, K | V)
+// Eight threads per head: grid (tokens / heads per CTA, B * NKV, K | V)
 __global__ void __launch_bounds__(256) kv4_store_kernel(const __grid_constant__ KV4Args a) {
   pdl_wait();
   pdl_trigger();
-  const int l = blockIdx.x * (blockDim.x >> 4) + (threadIdx.x >> 4), j = threadIdx.x & 15;
+  const int l = blockIdx.x * (blockDim.x >> 3) + (threadIdx.x >> 3), j = threadIdx.x & 7;
+  if (l >= a.L) return;
   const int b = blockIdx.y / a.NKV, h = blockIdx.y - b * a.NKV;
   const bool is_v = blockIdx.z != 0;
-  const long long slot = l < a.L ? a.slots[b * a.slot_sb + l] : -1;
-  const bool ok = slot >= 0 && slot < a.S;
-  float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (ok) {
-    const bf16* x = is_v ? a.v + b * a.xv_sb + h * a.xv_sh + l * a.xv_sl : a.k + b * a.xk_sb + h * a.xk_sh + l * a.xk_sl;
-    cvt8(ld_nc_v4(x + 8 * j), f);
+  const bf16* x = is_v ? a.v + b * a.xv_sb + h * a.xv_sh + l * a.xv_sl : a.k + b * a.xk_sb + h * a.xk_sh + l * a.xk_sl;
+  uint32_t w[8];
+  {
+    const uint4 lo = ld_nc_v4(x + 16 * j), hi = ld_nc_v4(x + 16 * j + 8);
+    w[0] = lo.x, w[1] = lo.y, w[2] = lo.z, w[3] = lo.w;
+    w[4] = hi.x, w[5] = hi.y, w[6] = hi.z, w[7] = hi.w;
   }
-  const float down = 1.0f / (is_v ? a.v_scale : a.k_scale);   // a power of two: exact
-  float amax = 0.f;
-  bool odd = false;
+  const long long slot = a.slots[b * a.slot_sb + l];
+  if (slot < 0 || slot >= a.S) return;
+  uint32_t top = 0;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    odd |= !isfinite(f[e]);
-    f[e] *= down;                                             // may overflow: saturates below
-    amax = fmaxf(amax, fabsf(f[e]));
-  }
-  amax = fmaxf(amax, __shfl_xor_sync(FULL, amax, 1));
-  odd |= __shfl_xor_sync(FULL, (int)odd, 1) != 0;
-  unsigned char sb = f_to_e4m3(snap16(amax * (1.0f / 6.0f)));
+  for (int e = 0; e < 8; ++e) top = __vmaxu2(top, w[e] & 0x7fff7fffu);
+  top = max(top & 0xffffu, top >> 16);
+  const bool odd = top >= 0x7f80u;                            // a NaN or an infinity
+  const float down = is_v ? a.v_inv : a.k_inv;
+  unsigned char sb = f_to_e4m3(snap16(__uint_as_float(top << 16) * down * (1.0f / 6.0f)));   // overflow saturates
   const float s = __half2float(__ushort_as_half((unsigned short)(e4m3x2_to_h2(sb) & 0xffffu)));
-  const float inv = s > 0.f ? 1.0f / s : 0.f;
+  const float inv = odd || s == 0.f ? 0.f : rcp(s) * down;
+  uint32_t q[2];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) f[e] = odd || s == 0.f ? 0.f : snap16(f[e] * inv);
+  for (int e = 0; e < 2; ++e) {
+    float f[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[2 * i] = snap16(lo_f(w[4 * e + i]) * inv);
+      f[2 * i + 1] = snap16(hi_f(w[4 * e + i]) * inv);
+    }
+    q[e] = inv == 0.f ? 0u : f8_to_e2m1(f);
+  }
   if (odd) sb = 0x7f;
-  if (!ok) return;
-  unsigned char* q = is_v ? a.vq + b * a.v_sb + h * a.v_sh + slot * a.v_sp : a.kq + b * a.k_sb + h * a.k_sh + slot * a.k_sp;
+  unsigned char* qp = is_v ? a.vq + b * a.v_sb + h * a.v_sh + slot * a.v_sp : a.kq + b * a.k_sb + h * a.k_sh + slot * a.k_sp;
   unsigned char* sc =
       is_v ? a.vs + b * a.vs_sb + h * a.vs_sh + slot * a.vs_sp : a.ks + b * a.ks_sb + h * a.ks_sh + slot * a.ks_sp;
-  *reinterpret_cast<uint32_t*>(q + 4 * j) = f8_to_e2m1(f);
-  if ((j & 1) == 0) sc[j >> 1] = sb;
+  *reinterpret_cast<uint2*>(qp + 8 * j) = make_uint2(q[0], q[1]);
+  sc[j] = sb;
 }
 
 __global__ void __launch_bounds__(256) kv4_read_kernel(const __grid_constant__ KV4Args a) {
   pdl_wait();
   pdl_trigger();
-  const int l = blockIdx.x * (blockDim.x >> 4) + (threadIdx.x >> 4), j = threadIdx.x & 15;
+  const int l = blockIdx.x * (blockDim.x >> 3) + (threadIdx.x >> 3), j = threadIdx.x & 7;
   if (l >= a.L) return;
   const int b = blockIdx.y / a.NKV, h = blockIdx.y - b * a.NKV;
   const bool is_v = blockIdx.z != 0;
   const long long slot = a.slots[b * a.slot_sb + l];
-  uint4 w = make_uint4(0, 0, 0, 0);
+  uint32_t o[8] = {0, 0, 0, 0, 0, 0, 0, 0};
   if (slot >= 0 && slot < a.S) {
     const unsigned char* q =
         is_v ? a.vq + b * a.v_sb + h * a.v_sh + slot * a.v_sp : a.kq + b * a.k_sb + h * a.k_sh + slot * a.k_sp;
     const unsigned char* sc =
         is_v ? a.vs + b * a.vs_sb + h * a.vs_sh + slot * a.vs_sp : a.ks + b * a.ks_sb + h * a.ks_sh + slot * a.ks_sp;
-    const float up = is_v ? a.v_scale : a.k_scale;
-    uint32_t x[4];
-    e2m1x8_to_h2(*reinterpret_cast<const uint32_t*>(q + 4 * j), x);
-    const uint32_t s2 = e4m3x2_to_h2((uint16_t)(sc[j >> 1] * 0x0101u));
-    uint32_t o[4];
+    const uint2 w = *reinterpret_cast<const uint2*>(q + 8 * j);
+    const float s = __half2float(__ushort_as_half((unsigned short)(e4m3x2_to_h2(sc[j]) & 0xffffu))) *
+                    (is_v ? a.v_scale : a.k_scale);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const uint32_t p = hmul2(x[e], s2);   // exact in fp16: 2 + 4 significant bits, 2^-10 .. 2688
-      o[e] = pack2(__half2float(__ushort_as_half((unsigned short)(p & 0xffffu))) * up,
-                   __half2float(__ushort_as_half((unsigned short)(p >> 16))) * up);
+    for (int e = 0; e < 2; ++e) {
+      uint32_t x[4];
+      e2m1x8_to_h2(e ? w.y : w.x, x);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {                           // 2 + 4 significant bits: exact in bf16
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&x[i]));
+        o[4 * e + i] = pack_bf16(f.x * s, f.y * s);
+      }
     }
-    w = make_uint4(o[0], o[1], o[2], o[3]);
   }
-  bf16* out = (is_v ? a.vo : a.ko) + ((long long)blockIdx.y * a.L + l) * LG_D + 8 * j;
-  *reinterpret_cast<uint4*>(out) = w;
+  uint4* out = reinterpret_cast<uint4*>((is_v ? a.vo : a.ko) + ((long long)blockIdx.y * a.L + l) * LG_D + 16 * j);
+  out[0] = make_uint4(o[0], o[1], o[2], o[3]);
+  out[1] = make_uint4(o[4], o[5], o[6], o[7]);
 }
 
 }  // namespace fb
@@ -127,14 +139,15 @@ int kv4_fill(const fb_kv_cache* c, const int64_t* slots, int64_t slot_sb, int L,
   a->vs_sb = lc.vs_sb, a->vs_sh = lc.vs_sh, a->vs_sp = lc.vs_sp;
   a->slots = (const long long*)slots, a->slot_sb = slot_sb;
   a->NKV = c->NKV, a->L = L, a->S = c->S, a->k_scale = c->k_scale, a->v_scale = c->v_scale;
+  a->k_inv = 1.0f / c->k_scale, a->v_inv = 1.0f / c->v_scale;
   return FB_OK;
 }
 
 int kv4_launch(const void* kern, KV4Args& a, int rows, cudaStream_t st) {
-  int per = 2;                                   // heads per CTA: a warp at least, 16 at most
-  while (per < 16 && per < a.L) per *= 2;
+  int per = 4;                                   // heads per CTA: a warp at least, 32 at most
+  while (per < 32 && per < a.L) per *= 2;
   void* args[] = {(void*)&a};
-  return fbh::launch_pdl(kern, dim3((a.L + per - 1) / per, rows, 2), dim3(16 * per), 0, st, args, true);
+  return fbh::launch_pdl(kern, dim3((a.L + per - 1) / per, rows, 2), dim3(8 * per), 0, st, args, true);
 }
 
 }  // namespace

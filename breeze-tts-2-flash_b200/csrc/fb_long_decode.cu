@@ -195,7 +195,7 @@ __device__ __forceinline__ void long_softmax(float (&s)[NT][4], uint32_t (&pf)[N
       st.lA += pA;
       st.lB += pB;
       if (BITS == 16) {
-        const uint32_t hi = pack2(pA, pB), lo = pack2(pA - lo_f(hi), pB - hi_f(hi));
+        const uint32_t hi = pack_bf16(pA, pB), lo = pack_bf16(pA - lo_f(hi), pB - hi_f(hi));
         pf[k][e] = movmatrix(G <= 4 && t >= 2 ? lo : hi);
         if (G == 8) pl[e] = movmatrix(lo);
       } else {

@@ -126,11 +126,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-__device__ __forceinline__ uint32_t lp_pack(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
 __device__ __forceinline__ void lp_st32(uint32_t taddr, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
@@ -380,7 +375,7 @@ __global__ void __launch_bounds__(LP_THREADS, 2) long_prefill_kernel(const __gri
         const float2 e = f2_get(f2_fma(f2(s[2 * c], s[2 * c + 1]), scale2, off2));
         const float p0 = ex2(e.x), p1 = ex2(e.y);
         sum2[c & 1] = f2_add(sum2[c & 1], f2(p0, p1));
-        w[c] = lp_pack(p0, p1);
+        w[c] = pack_bf16(p0, p1);
       }
       lp_st32(ts, w);
       tc_before();
@@ -406,8 +401,8 @@ __global__ void __launch_bounds__(LP_THREADS, 2) long_prefill_kernel(const __gri
 #pragma unroll
       for (int i = 0; i < 32; i += 8)
         *reinterpret_cast<uint4*>(d + (((((c & 63) + i) >> 3) ^ (r & 7)) << 4)) =
-            make_uint4(lp_pack(o[i], o[i + 1]), lp_pack(o[i + 2], o[i + 3]), lp_pack(o[i + 4], o[i + 5]),
-                       lp_pack(o[i + 6], o[i + 7]));
+            make_uint4(pack_bf16(o[i], o[i + 1]), pack_bf16(o[i + 2], o[i + 3]), pack_bf16(o[i + 4], o[i + 5]),
+                       pack_bf16(o[i + 6], o[i + 7]));
     }
     if (bad && ok && l < a.L) {
       float* o = reinterpret_cast<float*>(sk) + r;   // K's and V's buffers: every copy and MMA is done
