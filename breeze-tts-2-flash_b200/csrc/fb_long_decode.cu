@@ -39,25 +39,28 @@ namespace fb {
 constexpr int LD_WARPS = 4;
 constexpr int LD_THREADS = 32 * LD_WARPS;
 constexpr int LD_CTAS = 3;              // CTAs per SM (168 registers a thread)
-constexpr int LD_MAXB = 2048;           // batch rows (their geometry sits in shared memory)
-constexpr int LM_THREADS = 256;         // the merge
+constexpr int LM_THREADS = 128;         // the merge
 constexpr int LC_MAX = 16;              // CTAs of a cluster
 constexpr int LC_CHUNKS = 4;            // chunks a cluster's CTA may have
-constexpr int LD_SLICE = 2048;          // slots per accumulator CTA of the merge
+constexpr int LD_SLICE = 512;           // slots per accumulator CTA of the merge
 
 struct LongDecodeArgs {
   LongCache c;
   const bf16* q;
   long long q_sb, q_sh;
   const long long *lengths, *starts;
-  int B, NH, NKV, G, S, window, sinks, ncta;
+  int B, NH, NKV, G, S, window, sinks;
+  int ncta, per, slices;                // CTAs, batch rows per lane of the plan, accumulator CTAs per row
+  int dense;                            // position strides are the row's own bytes
   float scale;                          // scaling x log2(e) (x the cache's key scale)
   float v_scale;
   const float* acc;
   float* acc_out;
   float decay;
   long long acc_sb, acc_sh, acco_sb, acco_sh;
-  float *po, *pm, *pl;                  // pieces: [slot][G][128], [slot][G], [slot][G]
+  float* po;                            // pieces: unnormalised out [slot][G][128],
+  float2* ml;                           //   maximum and sum [slot][G]
+  int2* own;                            // [row] first and last CTA with a piece of it
   float* sc;                            // scores [row][cap][G] in log2 units (weights wanted), else null
   int cap;                              // visible keys a row can have
   bf16* out;
@@ -67,6 +70,7 @@ template <int BITS>
 struct LongTile {
   static constexpr int KEYS = BITS == 16 ? 16 : 32;      // keys per warp and step
   static constexpr int CHUNK = KEYS * LD_WARPS;
+  static constexpr int EXTRA = 2;                        // empty chunks before a row's own (see long_count)
   static constexpr float SHIFT = BITS == 16 ? 0.f : 6.f; // P x 2^6 in fp16: with the 2^8 of slack below its 65504
 };
 
@@ -98,42 +102,60 @@ __device__ __forceinline__ uint2 ld_nc_v2(const void* p) {
   return r;
 }
 
-// Geometry of every batch row and the running chunk counts, in shared memory; returns the chunks of one KV head of
-// all rows.  Every thread of the CTA calls it.
-template <int THREADS>
-__device__ __forceinline__ long long long_plan(const LongDecodeArgs& a, int chunk, int* s_cum, LongRow* s_row) {
-  __shared__ int s_w[THREADS / 32];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  int base = 0;
-  for (int b0 = 0; b0 < a.B; b0 += THREADS) {
-    const int b = b0 + tid;
-    int n = 0;
-    if (b < a.B) {
-      const LongRow r = long_row(a.lengths[b], a.starts ? a.starts[b] : 0, a.S, a.window, a.sinks);
-      s_row[b] = r;
-      n = (r.n + chunk - 1) / chunk;
-    }
-    int x = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(FULL, x, o);
-      if (lane >= o) x += y;
-    }
-    if (lane == 31) s_w[warp] = x;
-    __syncthreads();
-    int before = 0, all = 0;
-#pragma unroll
-    for (int w = 0; w < THREADS / 32; ++w) {
-      if (w < warp) before += s_w[w];
-      all += s_w[w];
-    }
-    if (b < a.B) s_cum[b] = base + before + x - n;
-    base += all;
-    __syncthreads();
+// The list of chunks: row b's NKV heads in turn, ceil(visible / chunk) chunks each after EXTRA empty ones.  Beginning a
+// row costs a CTA some microseconds (q, the first loads, its part of the output), and the empty chunks stand for that:
+// with ragged rows the CTAs of many short ones came out last by a quarter of the time without them.  Every warp works the
+// list out for itself (no barrier): lane i counts the chunks of rows [i per, i per + per).
+struct LongPlace {
+  int b, before;                        // batch row, chunks of one KV head of all rows before it
+  LongRow row;
+};
+__device__ __forceinline__ LongRow long_row_of(const LongDecodeArgs& a, int b) {
+  return long_row(a.lengths[b], a.starts ? a.starts[b] : 0, a.S, a.window, a.sinks);
+}
+template <int BITS>
+__device__ __forceinline__ int long_chunks(const LongRow& row) {
+  using T = LongTile<BITS>;
+  return row.n > 0 ? (row.n + T::CHUNK - 1) / T::CHUNK + T::EXTRA : 0;
+}
+template <int BITS>
+__device__ __forceinline__ int long_count(const LongDecodeArgs& a, int per, int lane, int& upto) {   // total; upto: inclusive
+  int n = 0;
+#pragma unroll 4
+  for (int i = 0; i < per; ++i) {
+    const int b = lane * per + i;
+    if (b < a.B) n += long_chunks<BITS>(long_row_of(a, b));
   }
-  if (tid == 0) s_cum[a.B] = base;
-  __syncthreads();
-  return base;
+  upto = n;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(FULL, upto, o);
+    if (lane >= o) upto += y;
+  }
+  const int total = __shfl_sync(FULL, upto, 31);
+  upto -= n;                            // exclusive
+  return total;
+}
+// The batch row whose chunks hold number x of one KV head's list (x < total).
+template <int BITS>
+__device__ __forceinline__ LongPlace long_find(const LongDecodeArgs& a, int per, int lane, int before, int x) {
+  const int owner = 31 - __clz(__ballot_sync(FULL, before <= x));     // empty lanes share a count: the last of them
+  LongPlace p;
+  p.b = owner * per;
+  p.before = __shfl_sync(FULL, before, owner);
+  while (true) {
+    p.row = long_row_of(a, p.b);
+    const int n = long_chunks<BITS>(p.row);
+    if (x < p.before + n) return p;
+    p.before += n;
+    ++p.b;
+  }
+}
+// CTA c of n takes chunks [share(c), share(c + 1)); the inverse.
+__device__ __forceinline__ int long_share(int total, int n, int c) { return total / n * c + min(c, total % n); }
+__device__ __forceinline__ int long_owner(int total, int n, int x) {
+  const int q = total / n, big = total % n * (q + 1);
+  return x < big ? x / (q + 1) : total % n + (x - big) / q;
 }
 
 struct LongStat {
@@ -144,7 +166,8 @@ struct LongStat {
 // the second parts of the weights in the upper columns (G <= 4) or in pl (G = 8).
 template <int BITS, bool SCORED, int NT>
 __device__ __forceinline__ void long_softmax(float (&s)[NT][4], uint32_t (&pf)[NT][2], uint32_t (&pl)[2], LongStat& st,
-                                             float (&o)[8][4], int i0, int n, float scA, float scB, float* scp, int G, int g, int t) {
+                                             float (&o)[8][4], int i0, int n, bool whole, float scA, float scB, float* scp,
+                                             int G, int g, int t) {
   constexpr float SHIFT = LongTile<BITS>::SHIFT;
   float xA = -INFINITY, xB = -INFINITY;
 #pragma unroll
@@ -152,12 +175,12 @@ __device__ __forceinline__ void long_softmax(float (&s)[NT][4], uint32_t (&pf)[N
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int i = i0 + 16 * k + g + 8 * e;
-      const bool ok = i < n;
+      const bool ok = whole || i < n;
       s[k][2 * e] = ok ? s[k][2 * e] * scA : -INFINITY;
       s[k][2 * e + 1] = ok ? s[k][2 * e + 1] * scB : -INFINITY;
       if (SCORED && ok) {
-        if (2 * t < G) scp[(long long)i * G + 2 * t] = s[k][2 * e];
-        if (2 * t + 1 < G) scp[(long long)i * G + 2 * t + 1] = s[k][2 * e + 1];
+        if (2 * t + 1 < G) *reinterpret_cast<float2*>(scp + (long long)i * G + 2 * t) = make_float2(s[k][2 * e], s[k][2 * e + 1]);
+        else if (2 * t < G) scp[(long long)i * G + 2 * t] = s[k][2 * e];
       }
       xA = fmaxf(xA, s[k][2 * e]);
       xB = fmaxf(xB, s[k][2 * e + 1]);
@@ -277,28 +300,46 @@ __device__ __forceinline__ void long_piece(const LongDecodeArgs& a, int b, int h
   for (int i0 = i_first + warp * T::KEYS; i0 < i_end; i0 += T::CHUNK) {
     float s[T::KEYS / 16][4];
     uint32_t pf[T::KEYS / 16][2], pl[2];
+    // a tile of consecutive slots: with rows of the dense stride every load is one address and a constant
+    const bool whole = i0 + T::KEYS <= row.n && (i0 >= row.ns || i0 + T::KEYS <= row.ns);
+    const bool fast = whole && a.dense;
+    const long long slot0 = row.slot(i0);
     if constexpr (BITS == 16) {
-      // keys past the row's end read its last key (a visible one) and get no weight
       __align__(16) uint32_t kw[2][16], vw[4][8];
+      if (fast) {
+        const unsigned char* pk = kb + (slot0 + g) * 256 + 16 * t;
+        const unsigned char* pv = vb + (slot0 + 2 * t) * 256 + 16 * g;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const unsigned char* p = kb + row.slot(min(i0 + g + 8 * e, row.n - 1)) * a.c.k_sp + 16 * t;
+        for (int e = 0; e < 2; ++e)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(&kw[e][4 * i]) = ld_nc_v4(p + 64 * i);
-      }
+          for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(&kw[e][4 * i]) = ld_nc_v4(pk + 2048 * e + 64 * i);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const unsigned char* p =
-            vb + row.slot(min(i0 + 2 * t + (e & 1) + 8 * (e >> 1), row.n - 1)) * a.c.v_sp + 16 * g;
+        for (int e = 0; e < 4; ++e)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) *reinterpret_cast<uint4*>(&vw[e][4 * i]) = ld_nc_v4(p + 128 * i);
+          for (int i = 0; i < 2; ++i)
+            *reinterpret_cast<uint4*>(&vw[e][4 * i]) = ld_nc_v4(pv + 256 * ((e & 1) + 8 * (e >> 1)) + 128 * i);
+      } else {
+        // keys past the row's end read its last key (a visible one) and get no weight
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const unsigned char* p = kb + row.slot(min(i0 + g + 8 * e, row.n - 1)) * a.c.k_sp + 16 * t;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(&kw[e][4 * i]) = ld_nc_v4(p + 64 * i);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const unsigned char* p =
+              vb + row.slot(min(i0 + 2 * t + (e & 1) + 8 * (e >> 1), row.n - 1)) * a.c.v_sp + 16 * g;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) *reinterpret_cast<uint4*>(&vw[e][4 * i]) = ld_nc_v4(p + 128 * i);
+        }
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[0][e] = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i)
         mma_bf16(s[0], kw[0][2 * i], kw[1][2 * i], kw[0][2 * i + 1], kw[1][2 * i + 1], qf[i][0], qf[i][1]);
-      long_softmax<BITS, SCORED>(s, pf, pl, st, o, i0, row.n, scA, scB, scp, G, g, t);
+      long_softmax<BITS, SCORED>(s, pf, pl, st, o, i0, row.n, whole, scA, scB, scp, G, g, t);
       // dims: row g of tile i is 8 g + i, row g + 8 is 64 + 8 g + i
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -315,19 +356,40 @@ __device__ __forceinline__ void long_piece(const LongDecodeArgs& a, int b, int h
       __align__(16) uint32_t kw[2][2][4], vw[2][4][2];
       uint16_t ksc[2][2];
       unsigned char vsc[2][4];
+      if (fast) {
+        const unsigned char* pk = kb + (slot0 + g) * 64 + 16 * t;
+        const unsigned char* pv = vb + (slot0 + 2 * t) * 64 + 8 * g;
+        const unsigned char* pks = ksb + (slot0 + g) * 8 + 2 * t;
+        const unsigned char* pvs = vsb + (slot0 + 2 * t) * 8 + g;
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
+        for (int n = 0; n < 2; ++n) {
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const long long sl = row.slot(min(i0 + 16 * n + g + 8 * e, row.n - 1));
-          *reinterpret_cast<uint4*>(&kw[n][e][0]) = ld_nc_v4(kb + sl * a.c.k_sp + 16 * t);
-          ksc[n][e] = __ldg(reinterpret_cast<const uint16_t*>(ksb + sl * a.c.ks_sp + 2 * t));
+          for (int e = 0; e < 2; ++e) {
+            *reinterpret_cast<uint4*>(&kw[n][e][0]) = ld_nc_v4(pk + 64 * (16 * n + 8 * e));
+            ksc[n][e] = __ldg(reinterpret_cast<const uint16_t*>(pks + 8 * (16 * n + 8 * e)));
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int row_off = 16 * n + (e & 1) + 8 * (e >> 1);
+            *reinterpret_cast<uint2*>(&vw[n][e][0]) = ld_nc_v2(pv + 64 * row_off);
+            vsc[n][e] = __ldg(pvs + 8 * row_off);
+          }
         }
+      } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const long long sl = row.slot(min(i0 + 16 * n + 2 * t + (e & 1) + 8 * (e >> 1), row.n - 1));
-          *reinterpret_cast<uint2*>(&vw[n][e][0]) = ld_nc_v2(vb + sl * a.c.v_sp + 8 * g);
-          vsc[n][e] = __ldg(vsb + sl * a.c.vs_sp + g);
+        for (int n = 0; n < 2; ++n) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const long long sl = row.slot(min(i0 + 16 * n + g + 8 * e, row.n - 1));
+            *reinterpret_cast<uint4*>(&kw[n][e][0]) = ld_nc_v4(kb + sl * a.c.k_sp + 16 * t);
+            ksc[n][e] = __ldg(reinterpret_cast<const uint16_t*>(ksb + sl * a.c.ks_sp + 2 * t));
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const long long sl = row.slot(min(i0 + 16 * n + 2 * t + (e & 1) + 8 * (e >> 1), row.n - 1));
+            *reinterpret_cast<uint2*>(&vw[n][e][0]) = ld_nc_v2(vb + sl * a.c.v_sp + 8 * g);
+            vsc[n][e] = __ldg(vsb + sl * a.c.vs_sp + g);
+          }
         }
       }
 #pragma unroll
@@ -348,7 +410,7 @@ __device__ __forceinline__ void long_piece(const LongDecodeArgs& a, int b, int h
                   qf[2 * w + 1][1]);
         }
       }
-      long_softmax<BITS, SCORED>(s, pf, pl, st, o, i0, row.n, scA, scB, scp, G, g, t);
+      long_softmax<BITS, SCORED>(s, pf, pl, st, o, i0, row.n, whole, scA, scB, scp, G, g, t);
       // dims: row g of tile i is 16 g + i (first code word), row g + 8 is 16 g + 8 + i (second)
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
@@ -430,59 +492,45 @@ __device__ __forceinline__ void long_join(const float (*s_o)[8][LG_D], const flo
 template <int BITS, bool SCORED>
 __global__ void __launch_bounds__(LD_THREADS, LD_CTAS) long_decode_kernel(const __grid_constant__ LongDecodeArgs a) {
   using T = LongTile<BITS>;
-  extern __shared__ __align__(16) unsigned char smem[];
-  LongRow* s_row = reinterpret_cast<LongRow*>(smem);
-  int* s_cum = reinterpret_cast<int*>(s_row + a.B);
   __shared__ __align__(16) float s_o[LD_WARPS][8][LG_D];
   __shared__ float s_m[LD_WARPS][8], s_l[LD_WARPS][8];
-  const int tid = threadIdx.x;
-  const int G = a.G;
-
+  const int tid = threadIdx.x, lane = tid & 31, G = a.G;
   pdl_wait();
   pdl_trigger();
-  const long long per_head = long_plan<LD_THREADS>(a, T::CHUNK, s_cum, s_row);
-  const long long total = per_head * a.NKV;
-  const long long ncta = min((long long)a.ncta, total);   // every CTA below it has a chunk at least
-  if (blockIdx.x >= ncta) return;
-  long long pos = total * blockIdx.x / ncta;
-  const long long end = total * (blockIdx.x + 1) / ncta;
-  int b = 0;
-  {
-    int hi = a.B;                                    // the last row whose chunks begin at or before pos
-    while (hi - b > 1) {
-      const int mid = (b + hi) >> 1;
-      if ((long long)s_cum[mid] * a.NKV <= pos) b = mid;
-      else hi = mid;
-    }
-  }
-  while (pos < end) {
-    const int nb = s_cum[b + 1] - s_cum[b];
-    if (nb == 0) {
-      ++b;
-      continue;
-    }
-    const long long rem = pos - (long long)s_cum[b] * a.NKV;
-    const int h = (int)(rem / nb), ch0 = (int)(rem - (long long)h * nb);
-    const int ch1 = (int)min((long long)nb, ch0 + (end - pos));
-    const LongRow row = s_row[b];
-    const int r = b * a.NKV + h;
-
-    long_piece<BITS, SCORED>(a, b, h, row, ch0 * T::CHUNK, min(row.n, ch1 * T::CHUNK),
-                             SCORED ? a.sc + (long long)r * a.cap * G : nullptr, s_o, s_m, s_l);
-    __syncthreads();
-    const long long piece = (long long)blockIdx.x + r;   // pieces in list order have increasing CTA or row: unique
-    for (int gg = 0; gg < G; ++gg) {
-      float M, L, O;
-      long_join(s_o, s_m, s_l, gg, M, L, O);
-      a.po[(piece * G + gg) * LG_D + tid] = O;
-      if (tid == 0) {
-        a.pm[piece * G + gg] = M;
-        a.pl[piece * G + gg] = L;
+  int before;
+  const int total = long_count<BITS>(a, a.per, lane, before) * a.NKV;
+  const int ncta = min(a.ncta, total);                    // every CTA below it has a chunk at least
+  const int cta = blockIdx.x;
+  if (cta >= ncta) return;
+  int pos = long_share(total, ncta, cta);
+  const int end = long_share(total, ncta, cta + 1);
+  LongPlace at = long_find<BITS>(a, a.per, lane, before, pos / a.NKV);
+  while (true) {
+    const int nb = long_chunks<BITS>(at.row), rem = pos - at.before * a.NKV;
+    const int h = rem / nb, e0 = rem - h * nb, e1 = min(nb, e0 + (end - pos));
+    const int ch0 = max(0, e0 - T::EXTRA), ch1 = e1 - T::EXTRA;      // the row's own chunks
+    const int r = at.b * a.NKV + h;
+    if (ch1 > ch0) {
+      long_piece<BITS, SCORED>(a, at.b, h, at.row, ch0 * T::CHUNK, min(at.row.n, ch1 * T::CHUNK),
+                               SCORED ? a.sc + (long long)r * a.cap * G : nullptr, s_o, s_m, s_l);
+      __syncthreads();
+      const long long piece = (long long)cta + r;         // pieces in list order have increasing CTA or row: unique
+      for (int gg = 0; gg < G; ++gg) {
+        float M, L, O;
+        long_join(s_o, s_m, s_l, gg, M, L, O);
+        a.po[(piece * G + gg) * LG_D + tid] = O;
+        if (tid == 0) a.ml[piece * G + gg] = make_float2(M, L);
       }
+      if (ch0 == 0 && tid == 0) a.own[r] = make_int2(cta, long_owner(total, ncta, pos - e0 + nb - 1));
+    }
+    pos += e1 - e0;
+    if (pos == end) return;
+    if (h == a.NKV - 1 && e1 == nb) {                     // the next row that has keys
+      at.before += nb;
+      do at.row = long_row_of(a, ++at.b);
+      while (at.row.n == 0);
     }
     __syncthreads();
-    pos += ch1 - ch0;
-    if (h == a.NKV - 1 && ch1 == nb) ++b;
   }
 }
 
@@ -569,93 +617,119 @@ __global__ void __launch_bounds__(LD_THREADS, LD_CTAS) long_cluster_kernel(const
   cluster.sync();                                        // a peer may still be reading this CTA's part
 }
 
-// Joins a row's pieces: CTA (row, y), y < G: head y's output; y >= G: weights of LD_SLICE slots.
-template <int BITS, bool SCORED>
-__global__ void __launch_bounds__(LM_THREADS) long_merge_kernel(const __grid_constant__ LongDecodeArgs a) {
-  using T = LongTile<BITS>;
-  extern __shared__ __align__(16) unsigned char smem[];
-  LongRow* s_row = reinterpret_cast<LongRow*>(smem);
-  int* s_cum = reinterpret_cast<int*>(s_row + a.B);
-  constexpr int W = LM_THREADS / 32;
-  __shared__ __align__(16) float s_o[W][LG_D];
-  __shared__ float s_l[W], s_m[8], s_inv[8];
+// Slots j0, j0 + LM_THREADS, .. of a slice: the scores of the group's heads -> weights, added to the accumulator.  All loads
+// of a thread are under way while the heads' maxima and sums are worked out.
+template <int G, class Stats>
+__device__ __forceinline__ void long_weights(const LongDecodeArgs& a, const LongRow& row, int b, int h, int r, int j0,
+                                             Stats stats, float* s_m, float* s_inv) {
+  constexpr int N = LD_SLICE / LM_THREADS;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int r = blockIdx.x, b = r / a.NKV, h = r - b * a.NKV, G = a.G;
+  const float* ap = a.acc + b * a.acc_sb + h * a.acc_sh;
+  float* op = a.acc_out + b * a.acco_sb + h * a.acco_sh;
+  const float* scp = a.sc + (long long)r * a.cap * G;
+  float acc[N], s[N][G];
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const int j = j0 + k * LM_THREADS, i = j < a.S ? row.index(j) : -1;
+    acc[k] = j < a.S ? ap[j] : 0.f;
+#pragma unroll
+    for (int g = 0; g < G; g += G < 4 ? G : 4) {
+      const float* p = scp + (long long)i * G + g;
+      if constexpr (G >= 4) {
+        const float4 x = i >= 0 ? *reinterpret_cast<const float4*>(p) : make_float4(0.f, 0.f, 0.f, 0.f);
+        s[k][g] = x.x, s[k][g + 1] = x.y, s[k][g + 2] = x.z, s[k][g + 3] = x.w;
+      } else if constexpr (G == 2) {
+        const float2 x = i >= 0 ? *reinterpret_cast<const float2*>(p) : make_float2(0.f, 0.f);
+        s[k][0] = x.x, s[k][1] = x.y;
+      } else {
+        s[k][0] = i >= 0 ? *p : 0.f;
+      }
+    }
+  }
+  for (int gg = warp; gg < G; gg += LM_THREADS / 32) {
+    float M, L;
+    stats(gg, M, L);
+    if (lane == 0) {
+      s_m[gg] = M;
+      s_inv[gg] = L == 0.f ? 0.f : 1.f / L;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const int j = j0 + k * LM_THREADS;
+    if (j >= a.S) break;
+    const bool seen = row.index(j) >= 0;
+    if (!seen && ap == op && a.decay == 1.f) continue;
+    float w = 0.f;
+    if (seen) {
+#pragma unroll
+      for (int g = 0; g < G; ++g) w += ex2(s[k][g] - s_m[g]) * s_inv[g];
+    }
+    op[j] = a.decay * acc[k] + w;
+  }
+}
+
+// Joins the pieces of every row, in CTA order: a warp per (row, head); past those, CTAs of LD_SLICE slots turn scores into
+// weights.
+template <bool SCORED>
+__global__ void __launch_bounds__(LM_THREADS) long_merge_kernel(const __grid_constant__ LongDecodeArgs a) {
+  __shared__ float s_m[8], s_inv[8];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = a.G;
+  constexpr int W = LM_THREADS / 32;
+  const int heads = a.B * a.NKV * G, joins = (heads + W - 1) / W;
+  const bool join = (int)blockIdx.x < joins;
+  const int item = join ? blockIdx.x * W + warp : blockIdx.x - joins;
+  const int r = join ? min(item, heads - 1) / G : item / a.slices, b = r / a.NKV, h = r - b * a.NKV;
+  const LongRow row = long_row_of(a, b);        // written at least two launches back
   pdl_wait();
   pdl_trigger();
-  const long long per_head = long_plan<LM_THREADS>(a, T::CHUNK, s_cum, s_row);
-  const long long total = per_head * a.NKV;
-  const LongRow row = s_row[b];
-  const int nb = s_cum[b + 1] - s_cum[b];
-  // CTAs [c0, c1] hold pieces of this row: CTA c takes chunks [total c / ncta, total (c + 1) / ncta)
-  const long long ncta = min((long long)a.ncta, total);
-  const long long p0 = (long long)s_cum[b] * a.NKV + (long long)h * nb;
-  long long c0 = 0, c1 = -1;
-  if (nb > 0) {
-    c0 = ((p0 + 1) * ncta - 1) / total;
-    c1 = ((p0 + nb) * ncta - 1) / total;
-  }
-  if ((int)blockIdx.y < G) {
-    const int gg = blockIdx.y;
-    float M = -INFINITY;
-    for (long long c = c0; c <= c1; ++c) M = fmaxf(M, a.pm[(c + r) * G + gg]);
-    float L = 0.f;
+  const int2 own = row.n > 0 ? a.own[r] : make_int2(0, -1);   // CTAs [x, y] hold pieces of this row
+  // a head's maximum and sum over the pieces (every lane)
+  auto stats = [&](int gg, float& M, float& L) {
+    M = -INFINITY;
+    L = 0.f;
+    for (int c = own.x + lane; c <= own.y; c += 32) M = fmaxf(M, a.ml[(long long)(c + r) * G + gg].x);
+    M = warp_max(M);
+    for (int c = own.x + lane; c <= own.y; c += 32) {
+      const float2 x = a.ml[(long long)(c + r) * G + gg];
+      if (x.x > -INFINITY) L += ex2(x.x - M) * x.y;
+    }
+    L = warp_sum(L);
+  };
+  if (join) {
+    if (item >= heads) return;
+    const int gg = item - r * G;
+    float M, L;
+    stats(gg, M, L);
     float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (long long c = c0 + warp; c <= c1; c += W) {
-      const long long at = (c + r) * G + gg;
-      const float m = a.pm[at];
+#pragma unroll 4
+    for (int c = own.x; c <= own.y; ++c) {
+      const long long at = (long long)(c + r) * G + gg;
+      const float m = a.ml[at].x;
+      const float4 x = *reinterpret_cast<const float4*>(a.po + at * LG_D + 4 * lane);
       const float f = m > -INFINITY ? ex2(m - M) : 0.f;
-      if (f != 0.f) {
-        const float4 x = *reinterpret_cast<const float4*>(a.po + at * LG_D + 4 * lane);
-        L += f * a.pl[at];
+      if (f != 0.f) {                            // a piece far below the maximum, or of -inf scores alone, adds nothing
         O.x += f * x.x;
         O.y += f * x.y;
         O.z += f * x.z;
         O.w += f * x.w;
       }
     }
-    *reinterpret_cast<float4*>(&s_o[warp][4 * lane]) = O;
-    if (lane == 0) s_l[warp] = L;
-    __syncthreads();
-    if (tid < LG_D) {
-      float l = 0.f, v = 0.f;
-#pragma unroll
-      for (int w = 0; w < W; ++w) {
-        l += s_l[w];
-        v += s_o[w][tid];
-      }
-      // no visible key: l = 0 and the row is 0; a NaN sum stays one
-      a.out[((long long)b * a.NH + h * G + gg) * LG_D + tid] = __float2bfloat16_rn(l == 0.f ? 0.f : v / l * a.v_scale);
-    }
+    // no visible key: L = 0 and the row is 0; a NaN sum stays one
+    const float f = L == 0.f ? 0.f : a.v_scale / L;
+    const bool none = L == 0.f;
+    *reinterpret_cast<uint2*>(a.out + ((long long)b * a.NH + h * G + gg) * LG_D + 4 * lane) =
+        make_uint2(none ? 0u : pack_bf16(O.x * f, O.y * f), none ? 0u : pack_bf16(O.z * f, O.w * f));
     return;
   }
   if constexpr (SCORED) {
-    for (int gg = warp; gg < G; gg += W) {
-      float M = -INFINITY, L = 0.f;
-      for (long long c = c0 + lane; c <= c1; c += 32) M = fmaxf(M, a.pm[(c + r) * G + gg]);
-      M = warp_max(M);
-      for (long long c = c0 + lane; c <= c1; c += 32) {
-        const float m = a.pm[(c + r) * G + gg];
-        if (m > -INFINITY) L += ex2(m - M) * a.pl[(c + r) * G + gg];
-      }
-      L = warp_sum(L);
-      if (lane == 0) {
-        s_m[gg] = M;
-        s_inv[gg] = L == 0.f ? 0.f : 1.f / L;
-      }
-    }
-    __syncthreads();
-    const float* scp = a.sc + (long long)r * a.cap * G;
-    const float* ap = a.acc + b * a.acc_sb + h * a.acc_sh;
-    float* op = a.acc_out + b * a.acco_sb + h * a.acco_sh;
-    const int j0 = (blockIdx.y - G) * LD_SLICE, j1 = min(a.S, j0 + LD_SLICE);
-    for (int j = j0 + tid; j < j1; j += LM_THREADS) {
-      const int i = row.index(j);
-      if (i < 0 && ap == op && a.decay == 1.f) continue;
-      float w = 0.f;
-      if (i >= 0)
-        for (int gg = 0; gg < G; ++gg) w += ex2(scp[(long long)i * G + gg] - s_m[gg]) * s_inv[gg];
-      op[j] = a.decay * ap[j] + w;
+    const int j0 = (item - r * a.slices) * LD_SLICE + tid;
+    switch (G) {
+      case 1: long_weights<1>(a, row, b, h, r, j0, stats, s_m, s_inv); break;
+      case 2: long_weights<2>(a, row, b, h, r, j0, stats, s_m, s_inv); break;
+      case 4: long_weights<4>(a, row, b, h, r, j0, stats, s_m, s_inv); break;
+      default: long_weights<8>(a, row, b, h, r, j0, stats, s_m, s_inv);
     }
   }
 }
@@ -711,7 +785,7 @@ struct LongPlan {
   int split;                                       // CTAs of a row's cluster, 0: the two launches
   int ncta, cap, slices;
   size_t smem;
-  int64_t slots, ws_floats, off_m, off_l, off_s;   // float offsets of the workspace's parts
+  int64_t slots, ws_floats, off_ml, off_own, off_s;   // float offsets of the workspace's parts
 };
 
 int long_plan_host(const fb_kv_cache* c, int NH, int window, int sinks, bool scored, LongPlan* p) {
@@ -721,11 +795,6 @@ int long_plan_host(const fb_kv_cache* c, int NH, int window, int sinks, bool sco
     fbh::set_msg("long_decode: GQA group %d not built (1, 2, 4, 8)", G);
     return FB_ERR_UNSUPPORTED;
   }
-  if (c->B > LD_MAXB) {
-    fbh::set_msg("long_decode: %d batch rows (at most %d)", c->B, LD_MAXB);
-    return FB_ERR_UNSUPPORTED;
-  }
-  FB_CHECK_ARG((int64_t)c->B * c->NKV <= (1ll << 30), "long_decode: too many rows");
   FB_CHECK_ARG(sinks >= 0, "long_decode: sinks %d", sinks);
   p->cap = window > 0 && (int64_t)window + sinks < c->S ? window + sinks : c->S;
   const int chunk = c->bits == 16 ? LongTile<16>::CHUNK : LongTile<4>::CHUNK;
@@ -744,14 +813,15 @@ int long_plan_host(const fb_kv_cache* c, int NH, int window, int sinks, bool sco
     return FB_OK;
   }
   p->ncta = (int)(most < want ? most : want);
-  p->slots = (int64_t)p->ncta + (int64_t)c->B * c->NKV;
+  FB_CHECK_ARG(rows * (chunks + 4) <= (1ll << 30), "long_decode: too many keys");
+  p->slots = (int64_t)p->ncta + rows;
   p->slices = scored ? (c->S + LD_SLICE - 1) / LD_SLICE : 0;
-  FB_CHECK_ARG(G + p->slices <= 65535, "long_decode: cache too long for the accumulator grid");
-  p->smem = (size_t)c->B * sizeof(LongRow) + ((size_t)c->B + 1) * sizeof(int);
-  p->off_m = p->slots * G * LG_D;
-  p->off_l = p->off_m + p->slots * G;
-  p->off_s = p->off_l + p->slots * G;
-  p->ws_floats = p->off_s + (scored ? (int64_t)c->B * c->NKV * p->cap * G : 0);
+  FB_CHECK_ARG(rows * (G + p->slices) <= 0x7fffffff, "long_decode: too many rows");
+  p->smem = 0;
+  p->off_ml = p->slots * G * LG_D;
+  p->off_own = p->off_ml + p->slots * G * 2;
+  p->off_s = (p->off_own + rows * 2 + 3) / 4 * 4;
+  p->ws_floats = p->off_s + (scored ? rows * p->cap * G : 0);
   return FB_OK;
 }
 
@@ -777,8 +847,9 @@ int long_launch(LongDecodeArgs& a, const LongPlan& p, cudaStream_t st) {
   int rc = fbh::launch_pdl((const void*)long_decode_kernel<BITS, SCORED>, dim3(p.ncta), dim3(LD_THREADS), p.smem, st,
                            args, true);
   if (rc) return rc;
-  return fbh::launch_pdl((const void*)long_merge_kernel<BITS, SCORED>, dim3(a.B * a.NKV, a.G + p.slices),
-                         dim3(LM_THREADS), p.smem, st, args, true);
+  const int per = LM_THREADS / 32, joins = (a.B * a.NKV * a.G + per - 1) / per;
+  return fbh::launch_pdl((const void*)long_merge_kernel<SCORED>, dim3(joins + a.B * a.NKV * p.slices), dim3(LM_THREADS), 0,
+                         st, args, true);
 }
 
 }  // namespace
@@ -813,11 +884,12 @@ extern "C" int flashb_long_decode(const fb_kv_cache* cache, const void* q, int64
   a.window = window > 0 ? window : 0, a.sinks = sinks, a.ncta = p.ncta;
   const bool four = cache->bits == 4;
   a.scale = scaling * LG_LOG2E * (four ? cache->k_scale : 1.f);
+  a.dense = a.c.k_sp == (four ? 64 : 256) && a.c.v_sp == a.c.k_sp && (!four || (a.c.ks_sp == 8 && a.c.vs_sp == 8));
   a.v_scale = four ? cache->v_scale : 1.f;
   a.acc = acc, a.acc_out = acc_out, a.decay = decay;
   a.acc_sb = acc_sb, a.acc_sh = acc_sh, a.acco_sb = acco_sb, a.acco_sh = acco_sh;
-  a.po = ws, a.pm = ws + p.off_m, a.pl = ws + p.off_l, a.sc = ws + p.off_s;
-  a.cap = p.cap, a.out = (bf16*)out;
+  a.po = ws, a.ml = (float2*)(ws + p.off_ml), a.own = (int2*)(ws + p.off_own), a.sc = ws + p.off_s;
+  a.per = (a.B + 31) / 32, a.slices = p.slices, a.cap = p.cap, a.out = (bf16*)out;
   const cudaStream_t s = (cudaStream_t)stream;
   if (four) return acc ? long_launch<4, true>(a, p, s) : long_launch<4, false>(a, p, s);
   return acc ? long_launch<16, true>(a, p, s) : long_launch<16, false>(a, p, s);

@@ -51,7 +51,7 @@ def test_bad_decode_arguments():
         assert decode(desc(B=500), **kw) == FB_ERR_ARG, kw
     assert decode(desc(B=500), n=10) == FB_ERR_ARG and 'workspace' in _native.last_error()
     assert decode(d, NH=6) == FB_ERR_UNSUPPORTED and 'group 3' in _native.last_error()
-    assert decode(desc(B=5000)) == FB_ERR_UNSUPPORTED
+    assert decode(desc(B=1 << 29)) == FB_ERR_ARG                                       # more chunks than 32 bits hold
 
 
 def test_workspace_sizes():
