@@ -799,10 +799,11 @@ int long_plan_host(const fb_kv_cache* c, int NH, int window, int sinks, bool sco
   p->cap = window > 0 && (int64_t)window + sinks < c->S ? window + sinks : c->S;
   const int chunk = c->bits == 16 ? LongTile<16>::CHUNK : LongTile<4>::CHUNK;
   const int64_t most = (int64_t)c->B * c->NKV * ((p->cap + chunk - 1) / chunk);
-  const int64_t want = (int64_t)fbh::grid_sms() * LD_CTAS;
-  // One cluster per row when that fills the keys' work into one wave with few chunks a CTA
+  const int64_t all = (int64_t)fbh::num_sms() * LD_CTAS, want = (int64_t)fbh::grid_sms() * LD_CTAS;
+  // One cluster per row when that fills the keys' work into one wave with few chunks a CTA.  That choice and the
+  // workspace's size go by the device's SMs, so that they do not change with the calling thread's budget.
   const int64_t rows = (int64_t)c->B * c->NKV, chunks = (p->cap + chunk - 1) / chunk;
-  int64_t split = want / rows;
+  int64_t split = all / rows;
   if (split > LC_MAX) split = LC_MAX;
   if (split > chunks) split = chunks;
   p->split = split >= 1 && chunks <= LC_CHUNKS * split && rows <= 65535 ? (int)split : 0;
@@ -814,7 +815,7 @@ int long_plan_host(const fb_kv_cache* c, int NH, int window, int sinks, bool sco
   }
   p->ncta = (int)(most < want ? most : want);
   FB_CHECK_ARG(rows * (chunks + 4) <= (1ll << 30), "long_decode: too many keys");
-  p->slots = (int64_t)p->ncta + rows;
+  p->slots = (most < all ? most : all) + rows;
   p->slices = scored ? (c->S + LD_SLICE - 1) / LD_SLICE : 0;
   FB_CHECK_ARG(rows * (G + p->slices) <= 0x7fffffff, "long_decode: too many rows");
   p->smem = 0;

@@ -28,6 +28,14 @@ from ._native import FB_ERR_ARG, FbKVCache, FlashbError, check
 D = 128
 _BF16, _I64, _F32 = torch.bfloat16, torch.int64, torch.float32
 _raw_stream = torch._C._cuda_getCurrentRawStream       # device index -> cudaStream_t (current_stream() builds an object)
+_lib = None
+
+
+def _bind():
+    """The library, looked up once (``_native.lib()`` takes a lock)."""
+    global _lib
+    _lib = _native.lib()
+    return _lib
 
 
 def _refuse(msg):
@@ -104,12 +112,11 @@ class KV4Cache(KVCache):
 
     def _slots(self, slots, L):
         """The row stride of a slot list of L entries."""
-        shape = slots.shape
-        if slots.dtype != _I64 or slots.device != self.device or not (
-                slots.dim() == 1 and shape[0] == L or slots.dim() == 2 and shape == (self.B, L)) or (
-                L > 1 and slots.stride(-1) != 1):
+        shape, st = slots.shape, slots.stride()
+        if slots.dtype != _I64 or slots.device != self.device or (shape != (L,) and shape != (self.B, L)) or (
+                L > 1 and st[-1] != 1):
             _refuse('slots: [L] or [B, L] int64 on the cache\'s device')
-        return slots.stride(0) if slots.dim() == 2 and self.B > 1 else 0
+        return st[0] if len(st) == 2 and self.B > 1 else 0
 
     def _heads(self, t, L):
         shape = t.shape
@@ -124,8 +131,10 @@ class KV4Cache(KVCache):
         sb = self._slots(slots, L)
         if L == 0:
             return
-        check(_native.lib().flashb_kv4_store(self._ref, k.data_ptr(), *_strides(k), v.data_ptr(), *_strides(v),
-                                             slots.data_ptr(), sb, L, _raw_stream(self.index)))
+        rc = (_lib or _bind()).flashb_kv4_store(self._ref, k.data_ptr(), *_strides(k), v.data_ptr(), *_strides(v),
+                                                slots.data_ptr(), sb, L, _raw_stream(self.index))
+        if rc:
+            check(rc)
 
     def read(self, slots):
         """The values at ``slots`` ([L] or [B, L]) as (k, v), each [B, NKV, L, 128] bf16 (0 outside the cache)."""
@@ -134,8 +143,10 @@ class KV4Cache(KVCache):
         k = torch.empty(self.B, self.NKV, L, D, dtype=_BF16, device=self.device)
         v = torch.empty_like(k)
         if L:
-            check(_native.lib().flashb_kv4_read(self._ref, slots.data_ptr(), sb, L, k.data_ptr(), v.data_ptr(),
-                                                _raw_stream(self.index)))
+            rc = (_lib or _bind()).flashb_kv4_read(self._ref, slots.data_ptr(), sb, L, k.data_ptr(), v.data_ptr(),
+                                                   _raw_stream(self.index))
+            if rc:
+                check(rc)
         return k, v
 
 
@@ -178,8 +189,8 @@ def decode(query, cache, lengths, *, starts=None, window=None, sinks=0, scaling=
     elif window < 1:
         _refuse('window: at least 1, or None')
     NH = shape[1]
-    lib = _native.lib()
-    if acc is not None:
+    scored = acc is not None
+    if scored:
         ap = _acc(acc, 'acc', cache, cache.S)
         op = ap if acc_out is None else _acc(acc_out, 'acc_out', cache, cache.S)
     else:
@@ -190,21 +201,25 @@ def decode(query, cache, lengths, *, starts=None, window=None, sinks=0, scaling=
         out = torch.empty(B, 1, NH, D, dtype=_BF16, device=dev)
     elif out.dtype != _BF16 or out.device != dev or not out.is_contiguous() or out.numel() != B * NH * D:
         _refuse('out: [B, 1, NH, 128] bf16 contiguous')
-    key = (NH, window, sinks, acc is not None, lib.flashb_sm_budget())
-    n = cache._ws.get(key)                                # the workspace's size follows from the shapes alone
+    lib = _lib or _bind()
+    key = (NH, window, sinks, scored)                     # the workspace's size follows from the shapes alone
+    n = cache._ws.get(key)
     if n is None:
-        n = lib.flashb_long_decode_ws_floats(cache._ref, NH, window, sinks, acc is not None)
+        n = lib.flashb_long_decode_ws_floats(cache._ref, NH, window, sinks, scored)
         if n >= 0:
             cache._ws[key] = n
     ws = torch.empty(n, dtype=_F32, device=dev) if n > 0 else None
-    check(lib.flashb_long_decode(
+    rc = lib.flashb_long_decode(
         cache._ref, query.data_ptr(), st[0] if B > 1 else 0, st[1] if NH > 1 else 0, NH,
         _rows(lengths, 'lengths', B, dev), None if starts is None else _rows(starts, 'starts', B, dev), window, sinks,
-        D ** -0.5 if scaling is None else scaling, *ap, *op, decay, None if ws is None else ws.data_ptr(), n,
-        out.data_ptr(), _raw_stream(cache.index)))
+        _SCALING if scaling is None else scaling, *ap, *op, decay, None if ws is None else ws.data_ptr(), n,
+        out.data_ptr(), _raw_stream(cache.index))
+    if rc:
+        check(rc)
     return out
 
 
+_SCALING = D ** -0.5
 _NO_ACC = (None, 0, 0)
 
 
@@ -236,11 +251,13 @@ def prefill(query, key, value, *, window=None, sinks=0, starts=None, q_start=Non
     if L == 0:
         return out
     ob, ol, oh, _ = out.stride()
-    check(_native.lib().flashb_long_prefill(
+    rc = (_lib or _bind()).flashb_long_prefill(
         query.data_ptr(), *_strides(query), key.data_ptr(), *_strides(key), value.data_ptr(), *_strides(value), B, NH,
         NKV, L, S, S - L if q_start is None else q_start, None if starts is None else _rows(starts, 'starts', B, dev),
-        window, sinks, D ** -0.5 if scaling is None else scaling, out.data_ptr(), ob, ol, oh,
-        _raw_stream(query.get_device())))
+        window, sinks, _SCALING if scaling is None else scaling, out.data_ptr(), ob, ol, oh,
+        _raw_stream(query.get_device()))
+    if rc:
+        check(rc)
     return out
 
 
@@ -262,8 +279,10 @@ def evict(cache, acc, lengths, keep, *, into, starts=None, sinks=0, recent=0, ac
     kept = torch.empty(B, cache.NKV, keep, dtype=torch.int32, device=dev)
     n = torch.empty(B, dtype=_I64, device=dev) if lengths_into is None else lengths_into
     ao = torch.empty(B, cache.NKV, keep, dtype=_F32, device=dev) if acc_into is None else acc_into
-    check(_native.lib().flashb_kv_evict(
+    rc = (_lib or _bind()).flashb_kv_evict(
         cache._ref, *a, _rows(lengths, 'lengths', B, dev), None if starts is None else _rows(starts, 'starts', B, dev),
         keep, sinks, recent, into._ref, *_acc(ao, 'acc_into', into, keep), ao.shape[2], kept.data_ptr(),
-        _rows(n, 'lengths_into', B, dev), _raw_stream(cache.index)))
+        _rows(n, 'lengths_into', B, dev), _raw_stream(cache.index))
+    if rc:
+        check(rc)
     return kept, n, ao

@@ -248,7 +248,7 @@ typedef struct {
  * neither; fp32 [B, NKV, S], unit stride per slot, may be the same buffer): acc_out[b, h, j] = decay acc[b, h, j] +
  * the weight of slot j summed over the group's query heads, for every slot of the cache.  ws: 16-byte aligned, at
  * least flashb_long_decode_ws_floats() floats (0 for few rows: then it may be NULL), not shared by calls that can overlap,
- * contents free before and after; the number depends on flashb_set_sm_budget.
+ * contents free before and after.
  * The same inputs give the same bits. */
 int64_t flashb_long_decode_ws_floats(const fb_kv_cache* cache, int NH, int window, int sinks, int scored);
 int flashb_long_decode(const fb_kv_cache* cache, const void* q, int64_t q_sb, int64_t q_sh, int NH,
