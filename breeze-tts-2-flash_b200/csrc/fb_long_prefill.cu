@@ -11,10 +11,11 @@
 // that window's beginning to the CTA's last token.  Two segments are a tile (the last one may be half a tile, and costs
 // as many MMAs); no tile is spent on a handful of sinks alone.
 //
-// Per tile: S = Q K^T (TMEM, 64 fp32 columns, two buffers); warps 0-3 (a thread per row) read their row, subtract the
-// running maximum, take exponentials and write P as bf16 pairs over S's first columns; O += P V with P as the MMA's TMEM
-// operand (128 more columns); a warp each issues the copies, S and P V.  S of the next tile is computed while the
-// exponentials of this one are taken, and two CTAs share an SM (96 KB of shared memory, 256 TMEM columns each).  The
+// Per tile: S = Q K^T (64 fp32 TMEM columns); warps 0-3 (a thread per row) read their row into registers, which frees S
+// for the next tile, subtract the running maximum, take exponentials and write P as bf16 pairs (32 columns, twice); O +=
+// P V with P as the MMA's TMEM operand (128 columns); a warp each issues the copies, S and P V.  So S of the next tile
+// and P V of the last one run while exponentials are taken, and two CTAs share an SM (96 KB of shared memory, 256 TMEM
+// columns each).  (P over S's columns instead, and S twice: each S then waited for a P V, 88 us for 69 TFLOP.)  The
 // running maximum moves only when a tile's exceeds it by 2^8 (the sums are exact either way), so O is hardly ever
 // rescaled.  Masks are applied to the segments that need one for some row of the CTA.
 //
@@ -36,7 +37,7 @@ constexpr int LP_THREADS = 224;                   // 4 softmax warps; one each f
 constexpr int LP_Q = LP_ROWS * LG_D * 2;          // bytes of the Q tile
 constexpr int LP_KV = LP_TILE * LG_D * 2;         // ... of a K or V tile
 constexpr int LP_SMEM = LP_Q + 4 * LP_KV + 1024;  // Q, K and V twice, at a 1024-byte boundary
-constexpr uint32_t LP_COLS = 256;                 // TMEM: S twice (and P over it) in columns 0-127, O in 128-255
+constexpr uint32_t LP_COLS = 256;                 // TMEM: S in columns 0-63, P twice in 64-127, O in 128-255
 constexpr float LP_SLACK = 8.f;
 
 struct alignas(64) LongPrefillArgs {
@@ -121,6 +122,12 @@ __device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+// Bits [lo, hi) of 32, whatever the two are.
+__device__ __forceinline__ uint32_t lp_bits(int lo, int hi) {
+  lo = max(lo, 0);
+  hi = min(hi, 32);
+  return lo < hi ? (0xffffffffu >> (32 - hi)) & (0xffffffffu << lo) : 0u;
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -177,7 +184,7 @@ __global__ void __launch_bounds__(LP_THREADS, 2) long_prefill_kernel(const __gri
   unsigned char* sq = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);   // Q; the output tile at the end
   unsigned char* sk = sq + LP_Q;                                          // [2]
   unsigned char* sv = sk + 2 * LP_KV;                                     // [2]
-  __shared__ __align__(8) uint64_t bar_k[2], bar_v[2], bar_s[2], bar_p[2], bar_o[2];
+  __shared__ __align__(8) uint64_t bar_k[2], bar_v[2], bar_s[2], bar_f, bar_p[2], bar_o[2];
   __shared__ uint32_t tslot;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int qt = gridDim.x - 1 - blockIdx.x;       // the latest tokens first: they have the most keys
@@ -190,7 +197,10 @@ __global__ void __launch_bounds__(LP_THREADS, 2) long_prefill_kernel(const __gri
       mbar_init(&bar_p[i], LP_ROWS);
       mbar_init(&bar_o[i], 1);
     }
+    mbar_init(&bar_f, LP_ROWS);
     fence_mbar_init();
+    for (const CUtensorMap* m : {&a.tq, &a.tk, &a.tv, &a.tk32, &a.tv32, &a.to})
+      asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
   }
   if (warp == 4) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tslot)), "r"(LP_COLS)
@@ -252,12 +262,12 @@ __global__ void __launch_bounds__(LP_THREADS, 2) long_prefill_kernel(const __gri
     auto step = [&](auto buf, int t) -> bool {
       constexpr int B = decltype(buf)::value;
       if (!lp_wait(&bar_k[B], (t >> 1) & 1, a.err)) return false;
-      if (t >= 2 && !lp_wait(&bar_o[B], ((t - 2) >> 1) & 1, a.err)) return false;   // P of t - 2 lay over this buffer
+      if (t >= 1 && !lp_wait(&bar_f, (t - 1) & 1, a.err)) return false;   // the last tile's scores are in registers
       tc_after();
       const uint32_t idesc = segs - 2 * t >= 2 ? tc_idesc(2 * LP_SEG) : tc_idesc(LP_SEG);
 #pragma unroll
       for (int s = 0; s < LG_D / 16; ++s)
-        tc_mma(tmem + 64 * B, dq + (((s >> 2) * (LP_Q / 2) + (s & 3) * 32) >> 4),
+        tc_mma(tmem, dq + (((s >> 2) * (LP_Q / 2) + (s & 3) * 32) >> 4),
                dk + ((B * LP_KV + (s >> 2) * (LP_KV / 2) + (s & 3) * 32) >> 4), s > 0, idesc);
       tc_commit(&bar_s[B]);
       return true;
@@ -289,7 +299,7 @@ __global__ void __launch_bounds__(LP_THREADS, 2) long_prefill_kernel(const __gri
 #pragma unroll
         for (int s = 0; s < 4; ++s)
           if (s < 2 || !half)
-            lp_mma_ts(t_o, tmem + 64 * B + 8 * s, dv + ((B * LP_KV + 2048 * s) >> 4), idesc, s > 0 || t > 0);
+            lp_mma_ts(t_o, tmem + 64 + 32 * B + 8 * s, dv + ((B * LP_KV + 2048 * s) >> 4), idesc, s > 0 || t > 0);
         tc_commit(&bar_o[B]);
       }
       __syncwarp();
@@ -301,40 +311,30 @@ __global__ void __launch_bounds__(LP_THREADS, 2) long_prefill_kernel(const __gri
   } else {
     const int r = tid, g = r / a.nq, l = q0 + r - g * a.nq, p = a.q_start + l, hq = h * a.G + g;
     const uint32_t my = (uint32_t)(warp * 32) << 16;
-    const int wnd = a.window > 0 ? a.window : 0x7fffffff;
+    const int wnd = a.window > 0 ? a.window : 0x40000000;   // none: more than any cache has
     const uint64_t scale2 = f2(a.scale, a.scale);
     float m = -INFINITY;
     uint64_t sum2[2] = {0, 0};
     bool ok = true;
     for (int t = 0; t < tiles; ++t) {
-      const int n = min(2, segs - 2 * t);
-      const uint32_t ts = tmem + my + 64 * (t & 1);
       ok = lp_wait_warp(&bar_s[t & 1], (t >> 1) & 1, a.err);
       if (!ok) break;
       tc_after();
       float s[LP_TILE];
-      if (n == 2) {
-        lp_ld64(ts, s);
-      } else {
-        lp_ld32(ts, s);
-#pragma unroll
-        for (int c = 32; c < 64; ++c) s[c] = -INFINITY;
-      }
+      lp_ld64(tmem + my, s);                       // half a tile: the rest is old scores, past every p and masked below
+      tc_before();
+      mbar_arrive(&bar_f);
 #pragma unroll
       for (int sg = 0; sg < 2; ++sg) {
-        if (sg < n) {
-          const int j0 = seg_base(2 * t + sg);
-          const bool sink = 2 * t + sg < nss;
-          if (sink || j0 + LP_SEG - 1 > p_lo || p_hi - j0 >= wnd) {
-            // sinks: those of the segment; window: 0 <= p - j < window, or a sink the window has reached
-            const int hi = sink ? st + ns : min(p + 1, st + a.sinks);
+        const int j0 = seg_base(2 * t + sg);
+        const bool sink = 2 * t + sg < nss;
+        if (sink || j0 + LP_SEG - 1 > p_lo || p_hi - j0 >= wnd) {
+          // the row's keys of the segment as bits: sinks, those of the segment; else slots p - window + 1 .. p and the
+          // sinks that the window has reached
+          const uint32_t see = p < st ? 0u : sink ? lp_bits(0, st + ns - j0)
+                                                  : lp_bits(p - wnd + 1 - j0, p + 1 - j0) | lp_bits(0, min(p + 1, st + a.sinks) - j0);
 #pragma unroll
-            for (int c = 0; c < 32; ++c) {
-              const int j = j0 + c;
-              const bool see = j < hi || (!sink && (unsigned)(p - j) < (unsigned)wnd);
-              s[32 * sg + c] = see && p >= st ? s[32 * sg + c] : -INFINITY;
-            }
-          }
+          for (int c = 0; c < LP_SEG; ++c) s[LP_SEG * sg + c] = (see >> c) & 1u ? s[LP_SEG * sg + c] : -INFINITY;
         }
       }
       float x[4] = {s[0], s[1], s[2], s[3]};
@@ -367,6 +367,8 @@ __global__ void __launch_bounds__(LP_THREADS, 2) long_prefill_kernel(const __gri
           }
         }
       }
+      // P's buffer: free once P V of t - 2 is done (asked here, needed after the exponentials)
+      const bool free = t < 2 || mbar_test(&bar_o[t & 1], ((t - 2) >> 1) & 1);
       const float off = m > -INFINITY ? -m : 0.f;
       const uint64_t off2 = f2(off, off);
       uint32_t w[32];
@@ -377,7 +379,12 @@ __global__ void __launch_bounds__(LP_THREADS, 2) long_prefill_kernel(const __gri
         sum2[c & 1] = f2_add(sum2[c & 1], f2(p0, p1));
         w[c] = pack_bf16(p0, p1);
       }
-      lp_st32(ts, w);
+      if (!__all_sync(FULL, free)) {
+        ok = lp_wait_warp(&bar_o[t & 1], ((t - 2) >> 1) & 1, a.err);
+        if (!ok) break;
+      }
+      tc_after();
+      lp_st32(tmem + my + 64 + 32 * (t & 1), w);
       tc_before();
       mbar_arrive(&bar_p[t & 1]);
     }
@@ -387,23 +394,33 @@ __global__ void __launch_bounds__(LP_THREADS, 2) long_prefill_kernel(const __gri
     // ---- the row, in the layout of the output's tensor map (128-byte swizzle), over Q
     const float2 u = f2_get(f2_add(sum2[0], sum2[1]));
     const float sum = u.x + u.y, inv = sum == 0.f ? 0.f : 1.f / sum;
-    bool bad = !isfinite(sum);
+    const uint64_t inv2 = f2(inv, inv);
+    uint64_t odd = 0;                              // becomes NaN with the first value that is not finite
 #pragma unroll 1
     for (int c = 0; c < LG_D; c += 32) {
       float o[32];
-      if (tiles > 0 && ok) lp_ld32(t_o + my + c, o);
+      if (tiles > 0 && ok) {
+        lp_ld32(t_o + my + c, o);
+      } else {
 #pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        bad |= !isfinite(o[i]) && tiles > 0;
-        o[i] = sum == 0.f ? 0.f : o[i] * inv;
+        for (int i = 0; i < 32; ++i) o[i] = 0.f;
+      }
+      uint32_t w[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const uint64_t x = f2(o[2 * i], o[2 * i + 1]);
+        odd = f2_fma(x, 0, odd);
+        const float2 y = f2_get(f2_fma(x, inv2, 0));
+        w[i] = pack_bf16(y.x, y.y);
       }
       unsigned char* d = sq + (c >> 6) * (LP_Q / 2) + r * 128;
 #pragma unroll
-      for (int i = 0; i < 32; i += 8)
-        *reinterpret_cast<uint4*>(d + (((((c & 63) + i) >> 3) ^ (r & 7)) << 4)) =
-            make_uint4(pack_bf16(o[i], o[i + 1]), pack_bf16(o[i + 2], o[i + 3]), pack_bf16(o[i + 4], o[i + 5]),
-                       pack_bf16(o[i + 6], o[i + 7]));
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<uint4*>(d + (((((c & 63) >> 3) + i) ^ (r & 7)) << 4)) =
+            make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
     }
+    const float2 od = f2_get(odd);
+    const bool bad = !isfinite(sum) || !(od.x + od.y == 0.f);
     if (bad && ok && l < a.L) {
       float* o = reinterpret_cast<float*>(sk) + r;   // K's and V's buffers: every copy and MMA is done
       long_row_again(a, b, hq, l, start, o);
@@ -469,7 +486,7 @@ extern "C" int flashb_long_prefill(const void* q, int64_t q_sb, int64_t q_sh, in
     return FB_ERR_UNSUPPORTED;
   }
   FB_CHECK_ARG(q_start >= 0 && (int64_t)q_start + L <= S, "long_prefill: tokens at slots %d .. of a cache of %d", q_start, S);
-  FB_CHECK_ARG(S <= 0x7fffff00, "long_prefill: %d slots", S);
+  FB_CHECK_ARG(S <= 0x3fffff00, "long_prefill: %d slots", S);
   FB_CHECK_ARG(sinks >= 0, "long_prefill: sinks %d", sinks);
   FB_CHECK_ARG(scaling > 0.f, "long_prefill: scaling must be positive");
   FB_CHECK_ARG((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & 15) == 0 &&
