@@ -145,27 +145,34 @@ __device__ __forceinline__ void lp_st32(uint32_t taddr, const uint32_t* r) {
       : "memory");
 }
 
-// One row over its visible keys, one at a time (the case of a non-finite output; see the header).  o: the thread's
-// column of a [128 dims][128 threads] array.
-__device__ __noinline__ void long_row_again(const LongPrefillArgs& a, int b, int hq, int l, long long start, float* o) {
-  const int p = a.q_start + l, h = hq / a.G;
+// One row over its visible keys, one at a time (the case of a non-finite output; see the header): a warp, four dims a
+// lane.  d: the row in the output tile (its halves LP_Q / 2 apart), x: the swizzle of its 16-byte units.
+__device__ __noinline__ void long_row_again(const LongPrefillArgs& a, int b, int hq, int l, long long start, unsigned char* d,
+                                            int x) {
+  const int lane = threadIdx.x & 31, p = a.q_start + l, h = hq / a.G;
   const LongRow row = long_row(p + 1, start, p + 1, a.window, a.sinks);
-  const bf16* qp = a.q + b * a.q_sb + hq * a.q_sh + l * a.q_sl;
-  const bf16* kb = a.k + b * a.k_sb + h * a.k_sh;
-  const bf16* vb = a.v + b * a.v_sb + h * a.v_sh;
-  float m = -INFINITY, sum = 0.f;
-  for (int d = 0; d < LG_D; ++d) o[d * LP_ROWS] = 0.f;
+  const bf16* kb = a.k + b * a.k_sb + h * a.k_sh + 4 * lane;
+  const bf16* vb = a.v + b * a.v_sb + h * a.v_sh + 4 * lane;
+  const uint2 qw = *reinterpret_cast<const uint2*>(a.q + b * a.q_sb + hq * a.q_sh + l * a.q_sl + 4 * lane);
+  float m = -INFINITY, sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
   for (int i = 0; i < row.n; ++i) {
     const long long j = row.slot(i);
-    float s = 0.f;
-    for (int d = 0; d < LG_D; ++d) s += b2f(qp[d]) * b2f(kb[j * a.k_sl + d]);
-    s *= a.scale;
+    const uint2 kw = *reinterpret_cast<const uint2*>(kb + j * a.k_sl), vw = *reinterpret_cast<const uint2*>(vb + j * a.v_sl);
+    const float s = a.scale * warp_sum(lo_f(qw.x) * lo_f(kw.x) + hi_f(qw.x) * hi_f(kw.x) + lo_f(qw.y) * lo_f(kw.y) +
+                                       hi_f(qw.y) * hi_f(kw.y));
     const float mn = fmaxf(m, s), f = m > -INFINITY ? ex2(m - mn) : 0.f, w = mn > -INFINITY ? ex2(s - mn) : (s == -INFINITY ? 0.f : s);
     m = mn;
     sum = sum * f + w;
-    for (int d = 0; d < LG_D; ++d) o[d * LP_ROWS] = o[d * LP_ROWS] * f + w * b2f(vb[j * a.v_sl + d]);
+    o[0] = o[0] * f + w * lo_f(vw.x);
+    o[1] = o[1] * f + w * hi_f(vw.x);
+    o[2] = o[2] * f + w * lo_f(vw.y);
+    o[3] = o[3] * f + w * hi_f(vw.y);
   }
-  for (int d = 0; d < LG_D; ++d) o[d * LP_ROWS] = sum == 0.f ? 0.f : o[d * LP_ROWS] / sum;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  d += (lane >> 4) * (LP_Q / 2) + ((((lane & 15) >> 1) ^ x) << 4) + (lane & 1) * 8;
+  *reinterpret_cast<uint2*>(d) = sum == 0.f ? make_uint2(0u, 0u)
+                                            : make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
 }
 
 // Bounded wait; the clock is read only after a long stretch of polling.
@@ -240,15 +247,27 @@ __global__ void __launch_bounds__(LP_THREADS, 2) long_prefill_kernel(const __gri
       }
     };
     if (lane == 0) {
+      // K and V each as soon as their buffer is free (S of t - 2 has read its K, P V of t - 2 its V): waited for in one
+      // order, a V that is still in use holds up the next K
       int nk = 0, nv = 0;                          // tiles copied
-      for (int t = 0; t < tiles; ++t) {
-        if (t >= 2 && !lp_wait(&bar_s[t & 1], ((t - 2) >> 1) & 1, a.err)) break;   // S of t - 2 has read its K
-        load(false, t);
-        ++nk;
-        if (t == 0) lp_load(sq, &a.tq, q0, h * a.G, 0, b, &bar_k[0]);
-        if (t >= 2 && !lp_wait(&bar_o[t & 1], ((t - 2) >> 1) & 1, a.err)) break;   // P V of t - 2 has read its V
-        load(true, t);
-        ++nv;
+      uint64_t since = 0;
+      while (nk < tiles || nv < tiles) {
+        const bool k = nk < tiles && (nk < 2 || mbar_test(&bar_s[nk & 1], ((nk - 2) >> 1) & 1));
+        if (k) {
+          load(false, nk);
+          if (nk == 0) lp_load(sq, &a.tq, q0, h * a.G, 0, b, &bar_k[0]);
+          ++nk;
+        }
+        const bool v = nv < tiles && (nv < 2 || mbar_test(&bar_o[nv & 1], ((nv - 2) >> 1) & 1));
+        if (v) load(true, nv++);
+        if (k || v) {
+          since = 0;
+        } else if (since == 0) {
+          since = globaltimer();
+        } else if (globaltimer() - since > WAIT_LIMIT_NS) {
+          set_error(a.err, FB_ERR_TIMEOUT);
+          break;
+        }
       }
       // no copy may be in flight when the CTA ends (after a wait that gave up: nobody else waits for them)
       for (int t = max(0, nk - 2); t < nk; ++t) lp_wait(&bar_k[t & 1], (t >> 1) & 1, a.err);
@@ -421,12 +440,11 @@ __global__ void __launch_bounds__(LP_THREADS, 2) long_prefill_kernel(const __gri
     }
     const float2 od = f2_get(odd);
     const bool bad = !isfinite(sum) || !(od.x + od.y == 0.f);
-    if (bad && ok && l < a.L) {
-      float* o = reinterpret_cast<float*>(sk) + r;   // K's and V's buffers: every copy and MMA is done
-      long_row_again(a, b, hq, l, start, o);
-      for (int d = 0; d < LG_D; ++d)
-        *reinterpret_cast<bf16*>(sq + (d >> 6) * (LP_Q / 2) + r * 128 + ((((d & 63) >> 3) ^ (r & 7)) << 4) + (d & 7) * 2) =
-            __float2bfloat16_rn(o[d * LP_ROWS]);
+    // rows that are not finite, again: the warp, a row at a time
+    __syncwarp();
+    for (unsigned todo = __ballot_sync(FULL, bad && ok && l < a.L); todo; todo &= todo - 1) {
+      const int i = warp * 32 + __ffs(todo) - 1, gi = i / a.nq;
+      long_row_again(a, b, h * a.G + gi, q0 + i - gi * a.nq, start, sq + i * 128, i & 7);
     }
     fence_proxy_async();
     named_sync(1, LP_ROWS);
@@ -434,7 +452,7 @@ __global__ void __launch_bounds__(LP_THREADS, 2) long_prefill_kernel(const __gri
       asm volatile("cp.async.bulk.tensor.5d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3, %4, %5}], [%6];" ::"l"(&a.to),
                    "r"(0), "r"(q0), "r"(h * a.G), "r"(0), "r"(b), "r"(smem_u32(sq))
                    : "memory");
-      asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group 0;" ::: "memory");
+      asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group.read 0;" ::: "memory");   // shared memory is read
     }
   }
   tc_before();
