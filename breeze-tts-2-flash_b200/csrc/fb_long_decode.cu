@@ -38,7 +38,6 @@ namespace fb {
 
 constexpr int LD_WARPS = 4;
 constexpr int LD_THREADS = 32 * LD_WARPS;
-constexpr int LD_CTAS = 3;              // CTAs per SM (168 registers a thread)
 constexpr int LM_THREADS = 128;         // the merge
 constexpr int LC_MAX = 16;              // CTAs of a cluster
 constexpr int LC_CHUNKS = 4;            // chunks a cluster's CTA may have
@@ -68,6 +67,8 @@ struct LongDecodeArgs {
 
 template <int BITS>
 struct LongTile {
+  // per SM: 168 registers a thread, and 128 (44.2 us with three for 64 ragged rows of up to 8192 slots, 41.9 with four)
+  static constexpr int CTAS = BITS == 16 ? 3 : 4;
   static constexpr int KEYS = BITS == 16 ? 16 : 32;      // keys per warp and step
   static constexpr int CHUNK = KEYS * LD_WARPS;
   static constexpr int EXTRA = 2;                        // empty chunks before a row's own (see long_count)
@@ -490,7 +491,7 @@ __device__ __forceinline__ void long_join(const float (*s_o)[8][LG_D], const flo
 }
 
 template <int BITS, bool SCORED>
-__global__ void __launch_bounds__(LD_THREADS, LD_CTAS) long_decode_kernel(const __grid_constant__ LongDecodeArgs a) {
+__global__ void __launch_bounds__(LD_THREADS, LongTile<BITS>::CTAS) long_decode_kernel(const __grid_constant__ LongDecodeArgs a) {
   using T = LongTile<BITS>;
   __shared__ __align__(16) float s_o[LD_WARPS][8][LG_D];
   __shared__ float s_m[LD_WARPS][8], s_l[LD_WARPS][8];
@@ -538,7 +539,7 @@ __global__ void __launch_bounds__(LD_THREADS, LD_CTAS) long_decode_kernel(const 
 // parts are joined through distributed shared memory in rank order.  Scores stay in shared memory until the row's
 // maximum and sum are known.
 template <int BITS, bool SCORED>
-__global__ void __launch_bounds__(LD_THREADS, LD_CTAS) long_cluster_kernel(const __grid_constant__ LongDecodeArgs a) {
+__global__ void __launch_bounds__(LD_THREADS, LongTile<BITS>::CTAS) long_cluster_kernel(const __grid_constant__ LongDecodeArgs a) {
   using T = LongTile<BITS>;
   extern __shared__ __align__(16) unsigned char smem[];
   float* s_sc = reinterpret_cast<float*>(smem);          // [LC_CHUNKS x CHUNK][G] (weights wanted)
@@ -799,7 +800,8 @@ int long_plan_host(const fb_kv_cache* c, int NH, int window, int sinks, bool sco
   p->cap = window > 0 && (int64_t)window + sinks < c->S ? window + sinks : c->S;
   const int chunk = c->bits == 16 ? LongTile<16>::CHUNK : LongTile<4>::CHUNK;
   const int64_t most = (int64_t)c->B * c->NKV * ((p->cap + chunk - 1) / chunk);
-  const int64_t all = (int64_t)fbh::num_sms() * LD_CTAS, want = (int64_t)fbh::grid_sms() * LD_CTAS;
+  const int ctas = c->bits == 16 ? LongTile<16>::CTAS : LongTile<4>::CTAS;
+  const int64_t all = (int64_t)fbh::num_sms() * ctas, want = (int64_t)fbh::grid_sms() * ctas;
   // One cluster per row when that fills the keys' work into one wave with few chunks a CTA.  That choice and the
   // workspace's size go by the device's SMs, so that they do not change with the calling thread's budget.
   const int64_t rows = (int64_t)c->B * c->NKV, chunks = (p->cap + chunk - 1) / chunk;
