@@ -42,82 +42,107 @@ __device__ __forceinline__ float rcp(float x) {
   return y;
 }
 
-// Eight threads per head: grid (tokens / heads per CTA, B * NKV, K | V)
+// Eight threads per head, KV4_ROWS tokens each (their loads together): grid (tokens, B * NKV, K | V)
+constexpr int KV4_ROWS = 2;
+
 __global__ void __launch_bounds__(256) kv4_store_kernel(const __grid_constant__ KV4Args a) {
   pdl_wait();
   pdl_trigger();
-  const int l = blockIdx.x * (blockDim.x >> 3) + (threadIdx.x >> 3), j = threadIdx.x & 7;
-  if (l >= a.L) return;
+  const int per = blockDim.x >> 3, l0 = blockIdx.x * per * KV4_ROWS + (threadIdx.x >> 3), j = threadIdx.x & 7;
   const int b = blockIdx.y / a.NKV, h = blockIdx.y - b * a.NKV;
   const bool is_v = blockIdx.z != 0;
-  const bf16* x = is_v ? a.v + b * a.xv_sb + h * a.xv_sh + l * a.xv_sl : a.k + b * a.xk_sb + h * a.xk_sh + l * a.xk_sl;
-  uint32_t w[8];
-  {
-    const uint4 lo = ld_nc_v4(x + 16 * j), hi = ld_nc_v4(x + 16 * j + 8);
-    w[0] = lo.x, w[1] = lo.y, w[2] = lo.z, w[3] = lo.w;
-    w[4] = hi.x, w[5] = hi.y, w[6] = hi.z, w[7] = hi.w;
-  }
-  const long long slot = a.slots[b * a.slot_sb + l];
-  if (slot < 0 || slot >= a.S) return;
-  uint32_t top = 0;
+  const bf16* x = (is_v ? a.v + b * a.xv_sb + h * a.xv_sh : a.k + b * a.xk_sb + h * a.xk_sh) + 16 * j;
+  const long long sl = is_v ? a.xv_sl : a.xk_sl;
+  uint32_t w[KV4_ROWS][8];
+  long long slot[KV4_ROWS];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) top = __vmaxu2(top, w[e] & 0x7fff7fffu);
-  top = max(top & 0xffffu, top >> 16);
-  const bool odd = top >= 0x7f80u;                            // a NaN or an infinity
-  const float down = is_v ? a.v_inv : a.k_inv;
-  unsigned char sb = f_to_e4m3(snap16(__uint_as_float(top << 16) * down * (1.0f / 6.0f)));   // overflow saturates
-  const float s = __half2float(__ushort_as_half((unsigned short)(e4m3x2_to_h2(sb) & 0xffffu)));
-  const float inv = odd || s == 0.f ? 0.f : rcp(s) * down;
-  uint32_t q[2];
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    float f[8];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      f[2 * i] = snap16(lo_f(w[4 * e + i]) * inv);
-      f[2 * i + 1] = snap16(hi_f(w[4 * e + i]) * inv);
+  for (int i = 0; i < KV4_ROWS; ++i) {
+    const int l = l0 + i * per;
+    slot[i] = -1;
+    if (l < a.L) {
+      const uint4 lo = ld_nc_v4(x + l * sl), hi = ld_nc_v4(x + l * sl + 8);
+      w[i][0] = lo.x, w[i][1] = lo.y, w[i][2] = lo.z, w[i][3] = lo.w;
+      w[i][4] = hi.x, w[i][5] = hi.y, w[i][6] = hi.z, w[i][7] = hi.w;
+      slot[i] = a.slots[b * a.slot_sb + l];
     }
-    q[e] = inv == 0.f ? 0u : f8_to_e2m1(f);
   }
-  if (odd) sb = 0x7f;
-  unsigned char* qp = is_v ? a.vq + b * a.v_sb + h * a.v_sh + slot * a.v_sp : a.kq + b * a.k_sb + h * a.k_sh + slot * a.k_sp;
-  unsigned char* sc =
-      is_v ? a.vs + b * a.vs_sb + h * a.vs_sh + slot * a.vs_sp : a.ks + b * a.ks_sb + h * a.ks_sh + slot * a.ks_sp;
-  *reinterpret_cast<uint2*>(qp + 8 * j) = make_uint2(q[0], q[1]);
-  sc[j] = sb;
+  const float down = is_v ? a.v_inv : a.k_inv;
+  unsigned char* qp = (is_v ? a.vq + b * a.v_sb + h * a.v_sh : a.kq + b * a.k_sb + h * a.k_sh) + 8 * j;
+  unsigned char* sc = (is_v ? a.vs + b * a.vs_sb + h * a.vs_sh : a.ks + b * a.ks_sb + h * a.ks_sh) + j;
+  const long long sp = is_v ? a.v_sp : a.k_sp, ssp = is_v ? a.vs_sp : a.ks_sp;
+#pragma unroll
+  for (int i = 0; i < KV4_ROWS; ++i) {
+    if (slot[i] < 0 || slot[i] >= a.S) continue;
+    uint32_t top = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = __vmaxu2(top, w[i][e] & 0x7fff7fffu);
+    top = max(top & 0xffffu, top >> 16);
+    const bool odd = top >= 0x7f80u;                            // a NaN or an infinity
+    unsigned char sb = f_to_e4m3(snap16(__uint_as_float(top << 16) * down * (1.0f / 6.0f)));   // overflow saturates
+    const float s = __half2float(__ushort_as_half((unsigned short)(e4m3x2_to_h2(sb) & 0xffffu)));
+    const float inv = odd || s == 0.f ? 0.f : rcp(s) * down;
+    uint32_t q[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float f[8];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        f[2 * c] = snap16(lo_f(w[i][4 * e + c]) * inv);
+        f[2 * c + 1] = snap16(hi_f(w[i][4 * e + c]) * inv);
+      }
+      q[e] = inv == 0.f ? 0u : f8_to_e2m1(f);
+    }
+    if (odd) sb = 0x7f;
+    *reinterpret_cast<uint2*>(qp + slot[i] * sp) = make_uint2(q[0], q[1]);
+    sc[slot[i] * ssp] = sb;
+  }
 }
 
 __global__ void __launch_bounds__(256) kv4_read_kernel(const __grid_constant__ KV4Args a) {
   pdl_wait();
   pdl_trigger();
-  const int l = blockIdx.x * (blockDim.x >> 3) + (threadIdx.x >> 3), j = threadIdx.x & 7;
-  if (l >= a.L) return;
+  const int per = blockDim.x >> 3, l0 = blockIdx.x * per * KV4_ROWS + (threadIdx.x >> 3), j = threadIdx.x & 7;
   const int b = blockIdx.y / a.NKV, h = blockIdx.y - b * a.NKV;
   const bool is_v = blockIdx.z != 0;
-  const long long slot = a.slots[b * a.slot_sb + l];
-  uint32_t o[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  if (slot >= 0 && slot < a.S) {
-    const unsigned char* q =
-        is_v ? a.vq + b * a.v_sb + h * a.v_sh + slot * a.v_sp : a.kq + b * a.k_sb + h * a.k_sh + slot * a.k_sp;
-    const unsigned char* sc =
-        is_v ? a.vs + b * a.vs_sb + h * a.vs_sh + slot * a.vs_sp : a.ks + b * a.ks_sb + h * a.ks_sh + slot * a.ks_sp;
-    const uint2 w = *reinterpret_cast<const uint2*>(q + 8 * j);
-    const float s = __half2float(__ushort_as_half((unsigned short)(e4m3x2_to_h2(sc[j]) & 0xffffu))) *
-                    (is_v ? a.v_scale : a.k_scale);
+  const unsigned char* qp = (is_v ? a.vq + b * a.v_sb + h * a.v_sh : a.kq + b * a.k_sb + h * a.k_sh) + 8 * j;
+  const unsigned char* sc = (is_v ? a.vs + b * a.vs_sb + h * a.vs_sh : a.ks + b * a.ks_sb + h * a.ks_sh) + j;
+  const long long sp = is_v ? a.v_sp : a.k_sp, ssp = is_v ? a.vs_sp : a.ks_sp;
+  long long slot[KV4_ROWS];
+  uint2 w[KV4_ROWS];
+  unsigned char sb[KV4_ROWS];
+#pragma unroll
+  for (int i = 0; i < KV4_ROWS; ++i) slot[i] = l0 + i * per < a.L ? a.slots[b * a.slot_sb + l0 + i * per] : -1;
+#pragma unroll
+  for (int i = 0; i < KV4_ROWS; ++i) {
+    w[i] = make_uint2(0u, 0u);
+    sb[i] = 0;
+    if (slot[i] >= 0 && slot[i] < a.S) {
+      w[i] = *reinterpret_cast<const uint2*>(qp + slot[i] * sp);
+      sb[i] = sc[slot[i] * ssp];
+    }
+  }
+  const float up = is_v ? a.v_scale : a.k_scale;
+  bf16* op = (is_v ? a.vo : a.ko) + (long long)blockIdx.y * a.L * LG_D + 16 * j;
+#pragma unroll
+  for (int i = 0; i < KV4_ROWS; ++i) {
+    const int l = l0 + i * per;
+    if (l >= a.L) break;
+    const float s = __half2float(__ushort_as_half((unsigned short)(e4m3x2_to_h2(sb[i]) & 0xffffu))) * up;
+    uint32_t o[8];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       uint32_t x[4];
-      e2m1x8_to_h2(e ? w.y : w.x, x);
+      e2m1x8_to_h2(e ? w[i].y : w[i].x, x);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {                           // 2 + 4 significant bits: exact in bf16
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&x[i]));
-        o[4 * e + i] = pack_bf16(f.x * s, f.y * s);
+      for (int c = 0; c < 4; ++c) {                           // 2 + 4 significant bits: exact in bf16
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&x[c]));
+        o[4 * e + c] = pack_bf16(f.x * s, f.y * s);
       }
     }
+    uint4* out = reinterpret_cast<uint4*>(op + (long long)l * LG_D);
+    out[0] = make_uint4(o[0], o[1], o[2], o[3]);
+    out[1] = make_uint4(o[4], o[5], o[6], o[7]);
   }
-  uint4* out = reinterpret_cast<uint4*>((is_v ? a.vo : a.ko) + ((long long)blockIdx.y * a.L + l) * LG_D + 16 * j);
-  out[0] = make_uint4(o[0], o[1], o[2], o[3]);
-  out[1] = make_uint4(o[4], o[5], o[6], o[7]);
 }
 
 }  // namespace fb
@@ -147,7 +172,7 @@ int kv4_launch(const void* kern, KV4Args& a, int rows, cudaStream_t st) {
   int per = 4;                                   // heads per CTA: a warp at least, 32 at most
   while (per < 32 && per < a.L) per *= 2;
   void* args[] = {(void*)&a};
-  return fbh::launch_pdl(kern, dim3((a.L + per - 1) / per, rows, 2), dim3(8 * per), 0, st, args, true);
+  return fbh::launch_pdl(kern, dim3((a.L + per * KV4_ROWS - 1) / (per * KV4_ROWS), rows, 2), dim3(8 * per), 0, st, args, true);
 }
 
 }  // namespace
