@@ -42,6 +42,20 @@ __device__ __forceinline__ float rcp(float x) {
   return y;
 }
 
+// A thread's two 16-byte units of a row and its neighbour's are four in a row, (0, 1) and (2, 3).  Written as (0, 2) and
+// (1, 3) each store of the two covers whole 32-byte sectors: the read kernel takes 15.2 us instead of 20.8 at 8 x 4097
+// tokens.  (Loads come through the cache either way; the exchange made the store kernel 2 us slower.)
+__device__ __forceinline__ void swap_units(uint4& a, uint4& b) {
+  const bool second = threadIdx.x & 1;
+  uint4 x = second ? a : b;                                     // what the neighbour is to have
+  x.x = __shfl_xor_sync(FULL, x.x, 1);
+  x.y = __shfl_xor_sync(FULL, x.y, 1);
+  x.z = __shfl_xor_sync(FULL, x.z, 1);
+  x.w = __shfl_xor_sync(FULL, x.w, 1);
+  if (second) a = x;
+  else b = x;
+}
+
 // Eight threads per head, KV4_ROWS tokens each (their loads together): grid (tokens, B * NKV, K | V)
 constexpr int KV4_ROWS = 2;
 
@@ -59,12 +73,14 @@ __global__ void __launch_bounds__(256) kv4_store_kernel(const __grid_constant__ 
   for (int i = 0; i < KV4_ROWS; ++i) {
     const int l = l0 + i * per;
     slot[i] = -1;
+    uint4 lo = make_uint4(0u, 0u, 0u, 0u), hi = lo;
     if (l < a.L) {
-      const uint4 lo = ld_nc_v4(x + l * sl), hi = ld_nc_v4(x + l * sl + 8);
-      w[i][0] = lo.x, w[i][1] = lo.y, w[i][2] = lo.z, w[i][3] = lo.w;
-      w[i][4] = hi.x, w[i][5] = hi.y, w[i][6] = hi.z, w[i][7] = hi.w;
+      lo = ld_nc_v4(x + l * sl);
+      hi = ld_nc_v4(x + l * sl + 8);
       slot[i] = a.slots[b * a.slot_sb + l];
     }
+    w[i][0] = lo.x, w[i][1] = lo.y, w[i][2] = lo.z, w[i][3] = lo.w;
+    w[i][4] = hi.x, w[i][5] = hi.y, w[i][6] = hi.z, w[i][7] = hi.w;
   }
   const float down = is_v ? a.v_inv : a.k_inv;
   unsigned char* qp = (is_v ? a.vq + b * a.v_sb + h * a.v_sh : a.kq + b * a.k_sb + h * a.k_sh) + 8 * j;
@@ -122,11 +138,10 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const __grid_constant__ K
     }
   }
   const float up = is_v ? a.v_scale : a.k_scale;
-  bf16* op = (is_v ? a.vo : a.ko) + (long long)blockIdx.y * a.L * LG_D + 16 * j;
+  bf16* op = (is_v ? a.vo : a.ko) + (long long)blockIdx.y * a.L * LG_D + 32 * (j >> 1) + 8 * (j & 1);
 #pragma unroll
   for (int i = 0; i < KV4_ROWS; ++i) {
     const int l = l0 + i * per;
-    if (l >= a.L) break;
     const float s = __half2float(__ushort_as_half((unsigned short)(e4m3x2_to_h2(sb[i]) & 0xffffu))) * up;
     uint32_t o[8];
 #pragma unroll
@@ -139,9 +154,12 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const __grid_constant__ K
         o[4 * e + c] = pack_bf16(f.x * s, f.y * s);
       }
     }
-    uint4* out = reinterpret_cast<uint4*>(op + (long long)l * LG_D);
-    out[0] = make_uint4(o[0], o[1], o[2], o[3]);
-    out[1] = make_uint4(o[4], o[5], o[6], o[7]);
+    uint4 lo = make_uint4(o[0], o[1], o[2], o[3]), hi = make_uint4(o[4], o[5], o[6], o[7]);
+    swap_units(lo, hi);
+    if (l < a.L) {
+      *reinterpret_cast<uint4*>(op + (long long)l * LG_D) = lo;
+      *reinterpret_cast<uint4*>(op + (long long)l * LG_D + 16) = hi;
+    }
   }
 }
 
