@@ -5,10 +5,12 @@
 // both to nearest, ties to even; s saturates at 448 (values beyond 6 s at 6 s), s = 0 gives zeros, and a block with a
 // NaN or an infinity gets s = NaN.  64 bytes of codes and 8 of scales stand for 256 bytes of bf16.
 //
-// The quotients are formed as products with an fp32 reciprocal.  A bf16 x over an e4m3 s lies on a rounding tie of
-// the target or at least 2^-9 of itself away from it (8 + 4 significant bits against the tie's 3; the same for
-// max / 6 with 8 against 7), while the product is off by less than 2^-22: rounding it to 16 fraction bits puts every
-// tie exactly on the tie and leaves all others on their side, so the codes are those of exact arithmetic.
+// The quotients are formed as products with an fp32 reciprocal, off by less than 2^-22 of themselves.  A bf16 x over an
+// e4m3 s lies on a rounding tie of the target (0.25 .. 5) or at least 2^-9 of itself away from it (8 + 4 significant bits
+// against the tie's 3): rounding the product to a multiple of 2^-15 puts every tie exactly on the tie and leaves all
+// others on their side, so the codes are those of exact arithmetic.  That rounding is the addition of 384 in the same
+// fused multiply-add, and its subtraction, two values an instruction.  max / 6 is rounded to 16 fraction bits in the same
+// way (8 significant bits against the tie's 7).
 //
 // Bound: HBM, 328 bytes a head and token.  A thread owns a block (two 16-byte loads, 8 bytes of codes, one scale), so
 // the block's maximum, scale and reciprocal are its own; the maximum is taken on the bf16 bit patterns, two at a time,
@@ -103,8 +105,10 @@ __global__ void __launch_bounds__(256) kv4_store_kernel(const __grid_constant__ 
       float f[8];
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        f[2 * c] = snap16(lo_f(w[i][4 * e + c]) * inv);
-        f[2 * c + 1] = snap16(hi_f(w[i][4 * e + c]) * inv);
+        const float2 y = f2_get(f2_add(f2_fma(f2(lo_f(w[i][4 * e + c]), hi_f(w[i][4 * e + c])), f2(inv, inv), f2(384.f, 384.f)),
+                                       f2(-384.f, -384.f)));
+        f[2 * c] = y.x;
+        f[2 * c + 1] = y.y;
       }
       q[e] = inv == 0.f ? 0u : f8_to_e2m1(f);
     }
@@ -151,7 +155,8 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const __grid_constant__ K
 #pragma unroll
       for (int c = 0; c < 4; ++c) {                           // 2 + 4 significant bits: exact in bf16
         const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&x[c]));
-        o[4 * e + c] = pack_bf16(f.x * s, f.y * s);
+        const float2 y = f2_get(f2_mul(f2(f.x, f.y), f2(s, s)));
+        o[4 * e + c] = pack_bf16(y.x, y.y);
       }
     }
     uint4 lo = make_uint4(o[0], o[1], o[2], o[3]), hi = make_uint4(o[4], o[5], o[6], o[7]);

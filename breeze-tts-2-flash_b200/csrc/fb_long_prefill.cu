@@ -101,27 +101,6 @@ __device__ __forceinline__ void lp_ld64(uint32_t taddr, float* f) {
 #pragma unroll
   for (int i = 0; i < 64; ++i) f[i] = __uint_as_float(r[i]);
 }
-// Two fp32 operations in one instruction.
-__device__ __forceinline__ uint64_t f2(float lo, float hi) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-__device__ __forceinline__ float2 f2_get(uint64_t x) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
-  return r;
-}
-__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 // Bits [lo, hi) of 32, whatever the two are.
 __device__ __forceinline__ uint32_t lp_bits(int lo, int hi) {
   lo = max(lo, 0);
