@@ -9,6 +9,8 @@
 // integer keys, held in shared memory), counts the slots that stay below each thread's run of slots, and then copies its
 // share of them.  With few rows several CTAs share one: each selects for itself (a few microseconds, and no exchange),
 // and copies its part.  Bound: HBM, the kept rows read and written once (1 KB a slot in bf16).
+// Measured on a B200: 64 rows of up to 8192 slots to 2048 (503 MB) 101 us, 0.76 of the measured copy bandwidth (half the
+// warps copying while the others select took 102); one stream's 1920 slots to 1023 9 us.
 #include "fb_long.cuh"
 
 namespace fb {

@@ -4,14 +4,21 @@
 //   s_j = scaling (q . k_j),  p = softmax(s) over the visible slots,  out = sum_j p_j v_j        (0 without any)
 //   acc_out[j] = decay acc[j] + sum over the q heads of the group of p_j   (every slot; p_j = 0 where not visible)
 //
+// Measured on a B200: 128 rows of 4 KV heads over a window of 2048 (404 MB) 68 us, 0.91 of the measured copy bandwidth; 64
+// ragged rows of up to 8192 slots in 4 bits (152 MB) 42 us, 0.55 (bound by instruction issue: 640 a warp and 32 keys, half
+// of them conversions, scalings and MMAs); weights wanted, up to 4096 slots (277 MB), 54 to 58 us, 0.75; one stream over
+// some hundred keys 5 to 8 us.  K and V through rings of cp.async in shared memory instead of straight to registers took
+// 85 us at the first of these.
+//
 // Bound: the visible K and V are read once (512 bytes a key and KV head in bf16, 144 in 4 bits) and do 4 G flops per
 // value, so HBM bounds it; below some megabytes the launch and one memory round trip do.
 //
-// Few rows: long_cluster_kernel, one launch (below).  Else two launches.  long_decode_kernel: the visible keys of every (row, KV head), in chunks, form one list; CTA c of N
-// takes the c-th N-th of it whatever the rows' lengths are, so ragged batches leave no CTA idle.  A CTA's share is
-// one or more pieces (a contiguous run of one row's keys); each leaves (max, sum, unnormalised out) in a slot of the
-// workspace.  long_merge_kernel joins a row's pieces in order (no atomics: the same inputs give the same bits) and,
-// when weights are wanted, turns the scores that the first kernel left in the workspace into weights.
+// Few short rows: long_cluster_kernel, one launch (below).  Else two launches.  long_decode_kernel: the visible keys of
+// every (row, KV head), in chunks, form one list; CTA c of N takes the c-th N-th of it whatever the rows' lengths are, so
+// ragged batches leave no CTA idle.  A CTA's share is one or more pieces (a contiguous run of one row's keys); each leaves
+// (max, sum, unnormalised out) in a slot of the workspace.  long_merge_kernel joins a row's pieces in a fixed order (no
+// atomics: the same inputs give the same bits) and, when weights are wanted, turns the scores that the first kernel left
+// in the workspace into weights.
 //
 // In a piece each of the 4 warps takes tiles of 16 keys (4-bit: 32) on its own, straight from global memory into the
 // fragments of mma.m16n8k16 (no shared memory, no barrier until the piece ends):
@@ -40,7 +47,7 @@ constexpr int LD_WARPS = 4;
 constexpr int LD_THREADS = 32 * LD_WARPS;
 constexpr int LM_THREADS = 128;         // the merge
 constexpr int LC_MAX = 16;              // CTAs of a cluster
-constexpr int LC_CHUNKS = 4;            // chunks a cluster's CTA may have
+constexpr int LC_CHUNKS = 8;            // chunks a cluster's CTA may have (4 when the cluster is not a full one)
 constexpr int LD_SLICE = 512;           // slots per accumulator CTA of the merge
 
 struct LongDecodeArgs {
@@ -542,7 +549,7 @@ template <int BITS, bool SCORED>
 __global__ void __launch_bounds__(LD_THREADS, LongTile<BITS>::CTAS) long_cluster_kernel(const __grid_constant__ LongDecodeArgs a) {
   using T = LongTile<BITS>;
   extern __shared__ __align__(16) unsigned char smem[];
-  float* s_sc = reinterpret_cast<float*>(smem);          // [LC_CHUNKS x CHUNK][G] (weights wanted)
+  float* s_sc = reinterpret_cast<float*>(smem);          // [its chunks x CHUNK][G] (weights wanted)
   __shared__ __align__(16) float s_o[LD_WARPS][8][LG_D];
   __shared__ float s_m[LD_WARPS][8], s_l[LD_WARPS][8];
   __shared__ float c_o[8][LG_D], c_m[8], c_l[8];         // this CTA's part, read by its peers
@@ -671,16 +678,16 @@ __device__ __forceinline__ void long_weights(const LongDecodeArgs& a, const Long
   }
 }
 
-// Joins the pieces of every row, in CTA order: a warp per (row, head); past those, CTAs of LD_SLICE slots turn scores into
-// weights.
-template <bool SCORED>
+// Joins the pieces of every row: a warp per (row, head), in CTA order, or WIDE (few rows of many pieces each) a CTA, its
+// warps on every fourth piece and joined in warp order; past those, CTAs of LD_SLICE slots turn scores into weights.
+template <bool SCORED, bool WIDE>
 __global__ void __launch_bounds__(LM_THREADS) long_merge_kernel(const __grid_constant__ LongDecodeArgs a) {
   __shared__ float s_m[8], s_inv[8];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = a.G;
   constexpr int W = LM_THREADS / 32;
-  const int heads = a.B * a.NKV * G, joins = (heads + W - 1) / W;
+  const int heads = a.B * a.NKV * G, joins = WIDE ? heads : (heads + W - 1) / W;
   const bool join = (int)blockIdx.x < joins;
-  const int item = join ? blockIdx.x * W + warp : blockIdx.x - joins;
+  const int item = join && !WIDE ? blockIdx.x * W + warp : blockIdx.x - (join ? 0 : joins);
   const int r = join ? min(item, heads - 1) / G : item / a.slices, b = r / a.NKV, h = r - b * a.NKV;
   const LongRow row = long_row_of(a, b);        // written at least two launches back
   pdl_wait();
@@ -705,7 +712,7 @@ __global__ void __launch_bounds__(LM_THREADS) long_merge_kernel(const __grid_con
     stats(gg, M, L);
     float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-    for (int c = own.x; c <= own.y; ++c) {
+    for (int c = own.x + (WIDE ? warp : 0); c <= own.y; c += WIDE ? W : 1) {
       const long long at = (long long)(c + r) * G + gg;
       const float m = a.ml[at].x;
       const float4 x = *reinterpret_cast<const float4*>(a.po + at * LG_D + 4 * lane);
@@ -715,6 +722,20 @@ __global__ void __launch_bounds__(LM_THREADS) long_merge_kernel(const __grid_con
         O.y += f * x.y;
         O.z += f * x.z;
         O.w += f * x.w;
+      }
+    }
+    if constexpr (WIDE) {
+      __shared__ __align__(16) float4 s_o[W][32];
+      s_o[warp][lane] = O;
+      __syncthreads();
+      if (warp > 0) return;
+#pragma unroll
+      for (int w = 1; w < W; ++w) {
+        const float4 x = s_o[w][lane];
+        O.x += x.x;
+        O.y += x.y;
+        O.z += x.z;
+        O.w += x.w;
       }
     }
     // no visible key: L = 0 and the row is 0; a NaN sum stays one
@@ -802,16 +823,21 @@ int long_plan_host(const fb_kv_cache* c, int NH, int window, int sinks, bool sco
   const int64_t most = (int64_t)c->B * c->NKV * ((p->cap + chunk - 1) / chunk);
   const int ctas = c->bits == 16 ? LongTile<16>::CTAS : LongTile<4>::CTAS;
   const int64_t all = (int64_t)fbh::num_sms() * ctas, want = (int64_t)fbh::grid_sms() * ctas;
-  // One cluster per row when that fills the keys' work into one wave with few chunks a CTA.  That choice and the
-  // workspace's size go by the device's SMs, so that they do not change with the calling thread's budget.
+  // One cluster per row, of up to two CTAs an SM in all, while its CTAs have few chunks; else the list.  Measured, cluster
+  // against list, bf16: 4 rows of 16384 slots 18.1 / 19.0 us (16 chunks a CTA); 8 of 8192 13.6 / 15.2 (8), of 16384 24.9 /
+  // 19.6; 32 of 2048 11.6 / 12.1 (4), of 4096 18.2 / 16.2; 64 of 1024 11.5 / 12.9 (4), of 2048 18.5 / 17.0; 128 of 512 12.1 /
+  // 12.2 (4), of 1024 19.3 / 16.3; one chunk a CTA 5 to 8 / 7 to 11.  (Clusters that fill three CTAs an SM do not all fit:
+  // 32 of 1024 took 13.5 us against 8.2.)  That choice and the workspace's size go by the device's SMs, so that they do
+  // not change with the calling thread's budget.
   const int64_t rows = (int64_t)c->B * c->NKV, chunks = (p->cap + chunk - 1) / chunk;
-  int64_t split = all / rows;
+  int64_t split = 2 * (int64_t)fbh::num_sms() / rows;
   if (split > LC_MAX) split = LC_MAX;
   if (split > chunks) split = chunks;
-  p->split = split >= 1 && chunks <= LC_CHUNKS * split && rows <= 65535 ? (int)split : 0;
+  const int64_t most_chunks = split == LC_MAX ? LC_CHUNKS : LC_CHUNKS / 2;
+  p->split = split >= 1 && chunks <= most_chunks * split && rows <= 65535 ? (int)split : 0;
   if (p->split) {
     p->ncta = p->slices = 0;
-    p->smem = scored ? (size_t)LC_CHUNKS * chunk * G * sizeof(float) : 0;
+    p->smem = scored ? (size_t)((chunks + split - 1) / split) * chunk * G * sizeof(float) : 0;
     p->ws_floats = 0;
     return FB_OK;
   }
@@ -836,8 +862,10 @@ int long_launch(LongDecodeArgs& a, const LongPlan& p, cudaStream_t st) {
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev >= 64 || !attr_done[dev]) {
-      const cudaError_t e =
-          cudaFuncSetAttribute(long_cluster_kernel<BITS, SCORED>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+      cudaError_t e = cudaFuncSetAttribute(long_cluster_kernel<BITS, SCORED>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+      if (e == cudaSuccess && SCORED)
+        e = cudaFuncSetAttribute(long_cluster_kernel<BITS, SCORED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 LC_CHUNKS * LongTile<BITS>::CHUNK * 8 * (int)sizeof(float));
       if (e != cudaSuccess) {
         fbh::set_msg("long_decode: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
         return FB_ERR_CUDA;
@@ -850,9 +878,12 @@ int long_launch(LongDecodeArgs& a, const LongPlan& p, cudaStream_t st) {
   int rc = fbh::launch_pdl((const void*)long_decode_kernel<BITS, SCORED>, dim3(p.ncta), dim3(LD_THREADS), p.smem, st,
                            args, true);
   if (rc) return rc;
-  const int per = LM_THREADS / 32, joins = (a.B * a.NKV * a.G + per - 1) / per;
-  return fbh::launch_pdl((const void*)long_merge_kernel<SCORED>, dim3(joins + a.B * a.NKV * p.slices), dim3(LM_THREADS), 0,
-                         st, args, true);
+  const int rows = a.B * a.NKV, heads = rows * a.G, per = LM_THREADS / 32;
+  if (p.ncta > 8 * rows)                                 // more than eight pieces a row
+    return fbh::launch_pdl((const void*)long_merge_kernel<SCORED, true>, dim3(heads + rows * p.slices), dim3(LM_THREADS), 0, st,
+                           args, true);
+  return fbh::launch_pdl((const void*)long_merge_kernel<SCORED, false>, dim3((heads + per - 1) / per + rows * p.slices),
+                         dim3(LM_THREADS), 0, st, args, true);
 }
 
 }  // namespace

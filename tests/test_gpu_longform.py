@@ -461,3 +461,35 @@ def test_refusals():
         with pytest.raises(FlashbError):
             f()
     assert torch.cuda.is_available() and float(z(1).sum()) == 0.0      # the context is fine
+
+
+@pytest.mark.parametrize('bits', [16, 4])
+@pytest.mark.parametrize('B,S', [(1, 9000), (2, 8192), (8, 4500), (24, 640), (40, 300)])
+def test_decode_on_either_side_of_the_cluster_rule(B, S, bits):
+    """Few rows of many keys and more rows of fewer: one cluster a row, or the shared list (with many pieces a row)."""
+    NH, NKV = 16, 4
+    g = torch.Generator().manual_seed(70)
+    lengths = torch.randint(S // 2, S + 1, (B,), generator=g)
+    lengths[0] = S
+    q, k, v = randn((B, NH, 1, 128), 71), randn((B, NKV, S, 128), 72), randn((B, NKV, S, 128), 73)
+    if bits == 4:
+        cache, k, v = four(k, v)
+    else:
+        cache = lf().KVCache(k.cuda(), v.cuda())
+    out, wt, tol = ref.decode(q, k, v, lengths, None, None, 0, SC)
+    acc = torch.zeros(B, NKV, S, device='cuda')
+    ref.assert_within(lf().decode(q.cuda(), cache, lengths.cuda()), out, tol)
+    ref.assert_within(lf().decode(q.cuda(), cache, lengths.cuda(), acc=acc), out, tol)
+    ref.assert_within(acc, wt, 2.0 ** -18 * wt + 1e-30)
+
+
+def test_decode_scored_with_eight_heads_a_group_in_full_clusters():
+    """The most shared memory a cluster's CTA can want: 8 chunks of scores of 8 heads."""
+    B, NH, NKV, S = 1, 16, 2, 16384
+    q, k, v = randn((B, NH, 1, 128), 74), randn((B, NKV, S, 128), 75), randn((B, NKV, S, 128), 76)
+    cache, k, v = four(k, v)
+    n = rows([S])
+    out, wt, tol = ref.decode(q, k, v, n, None, None, 0, SC)
+    acc = torch.zeros(B, NKV, S, device='cuda')
+    ref.assert_within(lf().decode(q.cuda(), cache, n.cuda(), acc=acc), out, tol)
+    ref.assert_within(acc, wt, 2.0 ** -18 * wt + 1e-30)
