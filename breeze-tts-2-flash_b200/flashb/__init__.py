@@ -8,6 +8,8 @@ Drop-in modules with the call surface of the reference's hook package (AsherHou/
   flashb.prefill_attn  install / bz_prefill_attention                              (flash/prefill_attn.py)
   flashb.prefill       install / prefill_forward: the whole BackbonePrefillGraphCache._forward on flashb kernels
                        (no reference module: the reference runs the eager layers with its attention hook)
+  flashb.longform      windowed attention with sinks, 4-bit KV cache, eviction by attention weight (no reference module)
+  flashb.long_speech   the backbone prefill and decode step on those caches; ``python -m flashb.long_speech``
 
 ``install(api)`` installs the hot-path hooks on the official runtime, as ``flash.install`` does for them
 (``flash/__init__.py:37-70``; the reference's other hooks -- weight packing, codec, streaming loop, reference cache --
