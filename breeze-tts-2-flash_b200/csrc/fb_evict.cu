@@ -9,7 +9,7 @@
 // integer keys, held in shared memory), counts the slots that stay below each thread's run of slots, and then copies its
 // share of them.  With few rows several CTAs share one: each selects for itself (a few microseconds, and no exchange),
 // and copies its part.  Bound: HBM, the kept rows read and written once (1 KB a slot in bf16).
-// Measured on a B200: 64 rows of up to 8192 slots to 2048 (503 MB) 101 us, 0.76 of the measured copy bandwidth (half the
+// Measured on a B200: 64 rows of up to 8192 slots to 2048 (478 MB) 101 us, 0.72 of the measured copy bandwidth (half the
 // warps copying while the others select took 102); one stream's 1920 slots to 1023 9 us.
 #include "fb_long.cuh"
 
@@ -194,7 +194,7 @@ extern "C" int flashb_kv_evict(const fb_kv_cache* cache, const float* acc, int64
                "kv_evict: the two caches differ in bits, rows or heads");
   FB_CHECK_ARG(cache->bits == 16 || (into->k_scale == cache->k_scale && into->v_scale == cache->v_scale),
                "kv_evict: the two caches differ in their tensor scales");
-  FB_CHECK_ARG((const void*)acc_out != (const void*)acc && lengths_out != lengths,
+  FB_CHECK_ARG((const void*)acc_out != (const void*)acc && lengths_out != lengths && lengths_out != starts,
                "kv_evict: the outputs may not be the inputs");
   FB_CHECK_ARG(into->k != cache->k && into->v != cache->v, "kv_evict: the cache cannot be evicted into itself");
   FB_CHECK_ARG(keep >= 1 && keep <= into->S && sinks >= 0 && recent >= 0 && (int64_t)sinks + recent <= keep,

@@ -8,7 +8,6 @@
 namespace fb {
 
 constexpr int LG_D = 128;        // head dim
-constexpr int LG_BLK = 16;       // values per 4-bit block (one scale byte)
 constexpr float LG_LOG2E = 1.4426950408889634f;
 
 // Keys of one row: slots [st, len); the token at slot len - 1 sees the first ns of them ("sinks", when the window
@@ -75,9 +74,6 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {   // one ins
   uint32_t r;
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
-}
-__device__ __forceinline__ void cp_async8(void* dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
 }
 // Two fp32 operations in one instruction.
 __device__ __forceinline__ uint64_t f2(float lo, float hi) {

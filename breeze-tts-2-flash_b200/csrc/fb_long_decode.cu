@@ -35,6 +35,7 @@
 // rescaled a few times a piece instead of every tile.
 #include <cooperative_groups.h>
 
+#include <cfloat>
 #include <cmath>
 
 #include "fb_long.cuh"
@@ -457,6 +458,9 @@ __device__ __forceinline__ void long_piece(const LongDecodeArgs& a, int b, int h
     st.lA += __shfl_xor_sync(FULL, st.lA, x);
     st.lB += __shfl_xor_sync(FULL, st.lB, x);
   }
+  // a NaN score is in the sum and not in the maximum: as the largest part it cannot be lost in the joins
+  if (st.lA != st.lA) st.mA = FLT_MAX;
+  if (st.lB != st.lB) st.mB = FLT_MAX;
   if (g == 0) {
     s_m[warp][2 * t] = st.mA;
     s_m[warp][2 * t + 1] = st.mB;
@@ -490,10 +494,8 @@ __device__ __forceinline__ void long_join(const float (*s_o)[8][LG_D], const flo
 #pragma unroll
   for (int w = 0; w < LD_WARPS; ++w) {
     const float f = s_m[w][gg] > -INFINITY ? ex2(s_m[w][gg] - M) : 0.f;
-    if (f != 0.f) {                                      // a warp without a tile holds nothing
-      L += f * s_l[w][gg];
-      O += f * s_o[w][gg][threadIdx.x];
-    }
+    L += f * s_l[w][gg];
+    O += f * s_o[w][gg][threadIdx.x];                    // a warp without a tile: 0
   }
 }
 
@@ -589,14 +591,12 @@ __global__ void __launch_bounds__(LD_THREADS, LongTile<BITS>::CTAS) long_cluster
       if (c < ns) M = fmaxf(M, mv[c]);
 #pragma unroll
     for (int c = 0; c < LC_MAX; ++c)
-      if (c < ns && mv[c] > -INFINITY) {
-        const float f = ex2(mv[c] - M);
-        if (f != 0.f) {
-          L += f * lv[c];
-          O += f * ov[c];
-        }
+      if (c < ns) {
+        const float f = mv[c] > -INFINITY ? ex2(mv[c] - M) : 0.f;
+        L += f * lv[c];
+        O += f * ov[c];
       }
-    a.out[((long long)b * a.NH + h * G + gg) * LG_D + tid] = __float2bfloat16_rn(L == 0.f ? 0.f : O / L * a.v_scale);
+    a.out[((long long)b * a.NH + h * G + gg) * LG_D + tid] = __float2bfloat16_rn(row.n == 0 ? 0.f : O / L * a.v_scale);
   }
   if constexpr (SCORED) {
     if (tid < G) {
@@ -607,7 +607,7 @@ __global__ void __launch_bounds__(LD_THREADS, LongTile<BITS>::CTAS) long_cluster
         if (m > -INFINITY) L += ex2(m - M) * *cluster.map_shared_rank(&c_l[tid], c);
       }
       s_max[tid] = M;
-      s_inv[tid] = L == 0.f ? 0.f : 1.f / L;
+      s_inv[tid] = 1.f / L;
     }
     __syncthreads();
     const float* ap = a.acc + b * a.acc_sb + h * a.acc_sh;
@@ -659,7 +659,7 @@ __device__ __forceinline__ void long_weights(const LongDecodeArgs& a, const Long
     stats(gg, M, L);
     if (lane == 0) {
       s_m[gg] = M;
-      s_inv[gg] = L == 0.f ? 0.f : 1.f / L;
+      s_inv[gg] = 1.f / L;                       // not used for a row without a visible slot
     }
   }
   __syncthreads();
@@ -717,12 +717,10 @@ __global__ void __launch_bounds__(LM_THREADS) long_merge_kernel(const __grid_con
       const float m = a.ml[at].x;
       const float4 x = *reinterpret_cast<const float4*>(a.po + at * LG_D + 4 * lane);
       const float f = m > -INFINITY ? ex2(m - M) : 0.f;
-      if (f != 0.f) {                            // a piece far below the maximum, or of -inf scores alone, adds nothing
-        O.x += f * x.x;
-        O.y += f * x.y;
-        O.z += f * x.z;
-        O.w += f * x.w;
-      }
+      O.x += f * x.x;
+      O.y += f * x.y;
+      O.z += f * x.z;
+      O.w += f * x.w;
     }
     if constexpr (WIDE) {
       __shared__ __align__(16) float4 s_o[W][32];
@@ -738,9 +736,9 @@ __global__ void __launch_bounds__(LM_THREADS) long_merge_kernel(const __grid_con
         O.w += x.w;
       }
     }
-    // no visible key: L = 0 and the row is 0; a NaN sum stays one
-    const float f = L == 0.f ? 0.f : a.v_scale / L;
-    const bool none = L == 0.f;
+    // visible keys with scores of -inf alone: 0 / 0, as softmax has it
+    const float f = a.v_scale / L;
+    const bool none = row.n == 0;
     *reinterpret_cast<uint2*>(a.out + ((long long)b * a.NH + h * G + gg) * LG_D + 4 * lane) =
         make_uint2(none ? 0u : pack_bf16(O.x * f, O.y * f), none ? 0u : pack_bf16(O.z * f, O.w * f));
     return;
@@ -910,8 +908,8 @@ extern "C" int flashb_long_decode(const fb_kv_cache* cache, const void* q, int64
   if (rc) return rc;
   FB_CHECK_ARG(((uintptr_t)q & 15) == 0 && q_sb % 8 == 0 && q_sh % 8 == 0,
                "long_decode: q must be 16-byte aligned with strides multiple of 8 elements");
-  FB_CHECK_ARG(p.ws_floats == 0 || (ws && ((uintptr_t)ws & 15) == 0 && ws_floats >= p.ws_floats), "long_decode: workspace of %lld floats, %lld needed",
-               (long long)ws_floats, (long long)p.ws_floats);
+  FB_CHECK_ARG(p.ws_floats == 0 || (ws && ((uintptr_t)ws & 15) == 0 && ws_floats >= p.ws_floats),
+               "long_decode: workspace of %lld floats, %lld needed", (long long)ws_floats, (long long)p.ws_floats);
   a.q = (const bf16*)q, a.q_sb = q_sb, a.q_sh = q_sh;
   a.lengths = (const long long*)lengths, a.starts = (const long long*)starts;
   a.B = cache->B, a.NH = NH, a.NKV = cache->NKV, a.G = NH / cache->NKV, a.S = cache->S;

@@ -156,10 +156,9 @@ __device__ __noinline__ void long_row_again(const LongPrefillArgs& a, int b, int
     o[2] = o[2] * f + w * lo_f(vw.y);
     o[3] = o[3] * f + w * hi_f(vw.y);
   }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const float inv = 1.f / sum;                     // scores of -inf alone: 0 / 0, as softmax has it
   d += (lane >> 4) * (LP_Q / 2) + ((((lane & 15) >> 1) ^ x) << 4) + (lane & 1) * 8;
-  *reinterpret_cast<uint2*>(d) = sum == 0.f ? make_uint2(0u, 0u)
-                                            : make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
+  *reinterpret_cast<uint2*>(d) = make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
 }
 
 // Bounded wait; the clock is read only after a long stretch of polling.
@@ -426,7 +425,7 @@ __global__ void __launch_bounds__(LP_THREADS, 2) long_prefill_kernel(const __gri
             make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
     }
     const float2 od = f2_get(odd);
-    const bool bad = !isfinite(sum) || !(od.x + od.y == 0.f);
+    const bool bad = !isfinite(sum) || !(od.x + od.y == 0.f) || (sum == 0.f && p >= st);   // the last: -inf scores alone
     // rows that are not finite, again: the warp, a row at a time
     __syncwarp();
     for (unsigned todo = __ballot_sync(FULL, bad && ok && l < a.L); todo; todo &= todo - 1) {
@@ -516,7 +515,9 @@ extern "C" int flashb_long_prefill(const void* q, int64_t q_sb, int64_t q_sh, in
   a.q_sb = q_sb, a.q_sh = q_sh, a.q_sl = q_sl, a.k_sb = k_sb, a.k_sh = k_sh, a.k_sl = k_sl;
   a.v_sb = v_sb, a.v_sh = v_sh, a.v_sl = v_sl;
   a.starts = (const long long*)starts;
-  a.NH = NH, a.NKV = NKV, a.G = G, a.nq = nq, a.L = L, a.q_start = q_start, a.window = window > 0 ? window : 0, a.sinks = sinks;
+  a.NH = NH, a.NKV = NKV, a.G = G, a.nq = nq, a.L = L, a.q_start = q_start;
+  a.window = window > 0 && window < S ? window : 0;
+  a.sinks = sinks < S ? sinks : S;                 // slot + sinks stays an int
   a.scale = scaling * LG_LOG2E, a.out = (bf16*)out, a.o_sb = o_sb, a.o_sl = o_sl, a.o_sh = o_sh;
   a.err = fbh::device_err_ptr();
   static int attr_done[64] = {0};

@@ -26,6 +26,7 @@ from . import _native
 from ._native import FB_ERR_ARG, FbKVCache, FlashbError, check
 
 D = 128
+_INT = 2 ** 31 - 1
 _BF16, _I64, _F32 = torch.bfloat16, torch.int64, torch.float32
 _raw_stream = torch._C._cuda_getCurrentRawStream       # device index -> cudaStream_t (current_stream() builds an object)
 _lib = None
@@ -171,6 +172,19 @@ def _acc(t, name, cache, least):
     return t.data_ptr(), t.stride(0), t.stride(1)
 
 
+def _span(window, sinks):
+    """window (0: none) and sinks as the library's ints."""
+    if window is None:
+        window = 0
+    elif window < 1:
+        _refuse('window: at least 1, or None')
+    elif window > _INT:
+        window = 0                                        # longer than any cache
+    if sinks < 0:
+        _refuse('sinks: at least 0')
+    return window, sinks if sinks < _INT else _INT
+
+
 def decode(query, cache, lengths, *, starts=None, window=None, sinks=0, scaling=None, acc=None, acc_out=None,
            decay=1.0, out=None):
     """Attention of one token per row, the one at slot ``lengths[b] - 1``: ``query`` [B, NH, 1, 128] bf16 over a
@@ -184,10 +198,7 @@ def decode(query, cache, lengths, *, starts=None, window=None, sinks=0, scaling=
     if query.dtype != _BF16 or query.device != dev or len(shape) != 4 or shape[0] != B or shape[2] != 1 or \
             shape[3] != D or st[3] != 1:
         _refuse('query: [B, NH, 1, 128] bf16 on the cache\'s device')
-    if window is None:
-        window = 0
-    elif window < 1:
-        _refuse('window: at least 1, or None')
+    window, sinks = _span(window, sinks)
     NH = shape[1]
     scored = acc is not None
     if scored:
@@ -240,20 +251,20 @@ def prefill(query, key, value, *, window=None, sinks=0, starts=None, q_start=Non
     NKV, S = key.shape[1], key.shape[2]
     if value.shape != key.shape:
         _refuse('key and value differ in shape')
-    if window is None:
-        window = 0
-    elif window < 1:
-        _refuse('window: at least 1, or None')
+    window, sinks = _span(window, sinks)
     if out is None:
         out = torch.empty(B, L, NH, D, dtype=_BF16, device=dev)
     elif not _bf16_heads(out, B, dev) or out.shape != (B, L, NH, D):
         _refuse('out: [B, L, NH, 128] bf16')
+    q_start = S - L if q_start is None else q_start
+    if q_start < 0 or q_start + L > S:
+        _refuse(f'q_start: tokens at slots {q_start} .. {q_start + L - 1} of {S}')
     if L == 0:
         return out
     ob, ol, oh, _ = out.stride()
     rc = (_lib or _bind()).flashb_long_prefill(
         query.data_ptr(), *_strides(query), key.data_ptr(), *_strides(key), value.data_ptr(), *_strides(value), B, NH,
-        NKV, L, S, S - L if q_start is None else q_start, None if starts is None else _rows(starts, 'starts', B, dev),
+        NKV, L, S, q_start, None if starts is None else _rows(starts, 'starts', B, dev),
         window, sinks, _SCALING if scaling is None else scaling, out.data_ptr(), ob, ol, oh,
         _raw_stream(query.get_device()))
     if rc:
@@ -274,8 +285,8 @@ def evict(cache, acc, lengths, keep, *, into, starts=None, sinks=0, recent=0, ac
     a = _acc(acc, 'acc', cache, cache.S)
     if into.bits != cache.bits or into.device != dev:
         _refuse('into: a cache of the same kind on the same device')
-    if keep < 1:
-        _refuse('keep: at least 1')
+    if not 1 <= keep <= into.S or sinks < 0 or recent < 0 or sinks + recent > keep:
+        _refuse(f'keep: 1 to {into.S} slots, sinks and recent among them')
     kept = torch.empty(B, cache.NKV, keep, dtype=torch.int32, device=dev)
     n = torch.empty(B, dtype=_I64, device=dev) if lengths_into is None else lengths_into
     ao = torch.empty(B, cache.NKV, keep, dtype=_F32, device=dev) if acc_into is None else acc_into

@@ -257,7 +257,8 @@ int flashb_long_decode(const fb_kv_cache* cache, const void* q, int64_t q_sb, in
                        int64_t acco_sh, float decay, float* ws, int64_t ws_floats, void* out, void* stream);
 /* Attention of the tokens at slots q_start .. q_start + L - 1: q [B, NH, L, 128] bf16 over k / v [B, NKV, S, 128] bf16
  * (strides per batch row, head and position in elements, multiples of 8; 16-byte aligned; q_start + L <= S; later
- * slots are not read); out [B, L, NH, 128] bf16 with strides o_sb, o_sl, o_sh.  Arithmetic as above. */
+ * slots are not read; S <= 0x3fffff00; scaling > 0); out [B, L, NH, 128] bf16 with strides o_sb, o_sl, o_sh (multiples
+ * of 8; 16-byte aligned).  Arithmetic as above. */
 int flashb_long_prefill(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_sl, const void* k, int64_t k_sb,
                         int64_t k_sh, int64_t k_sl, const void* v, int64_t v_sb, int64_t v_sh, int64_t v_sl, int B,
                         int NH, int NKV, int L, int S, int q_start, const int64_t* starts, int window, int sinks,

@@ -493,3 +493,101 @@ def test_decode_scored_with_eight_heads_a_group_in_full_clusters():
     acc = torch.zeros(B, NKV, S, device='cuda')
     ref.assert_within(lf().decode(q.cuda(), cache, n.cuda(), acc=acc), out, tol)
     ref.assert_within(acc, wt, 2.0 ** -18 * wt + 1e-30)
+
+
+# slots (of the cache's last 300) that hold the odd key: the last one, alone in its tile; one among others; a tile's all
+ODD = [[299], [150], list(range(256, 288))]
+
+
+def at_the_end(B, S, n, at):
+    """A cache of B rows whose last n slots are visible, and the slots ``at`` of those."""
+    return [S - n + j for j in at], rows([S] * B)
+
+
+@pytest.mark.parametrize('at', ODD)
+@pytest.mark.parametrize('bits', [16, 4])
+@pytest.mark.parametrize('B,S', [(1, 300), (1, 9000), (64, 300), (40, 1100)])
+@pytest.mark.parametrize('scored', [False, True])
+def test_decode_shows_a_visible_nan_key_wherever_it_lies(at, bits, B, S, scored):
+    """One NaN score makes its head's softmax NaN, in whichever part of the row it is; other heads and rows stay."""
+    NH, NKV = 8, 2
+    q, k, v = randn((B, NH, 1, 128), 70), randn((B, NKV, S, 128), 71), randn((B, NKV, S, 128), 72)
+    slots, lengths = at_the_end(B, S, 300, at)
+    starts = torch.full((B,), S - 300, dtype=torch.int64).cuda()
+    def run(kk):
+        cache = four(kk, v)[0] if bits == 4 else lf().KVCache(kk.cuda(), v.cuda())
+        acc = torch.zeros(B, NKV, S, device='cuda') if scored else None
+        return lf().decode(q.cuda(), cache, lengths.cuda(), starts=starts, acc=acc), acc
+    clean, w0 = run(k)
+    kk = k.clone()
+    kk[B // 2, 1, slots] = float('nan')
+    got, w1 = run(kk)
+    assert torch.isnan(got[B // 2, 0, 4:]).all()
+    keep = torch.ones_like(got, dtype=torch.bool)
+    keep[B // 2, 0, 4:] = False
+    assert torch.equal(got[keep], clean[keep])
+    if scored:
+        assert torch.isnan(w1[B // 2, 1, S - 300:]).all()
+        keep = torch.ones_like(w1, dtype=torch.bool)
+        keep[B // 2, 1, S - 300:] = False
+        assert torch.equal(w1[keep], w0[keep])
+
+
+@pytest.mark.parametrize('B,S', [(1, 300), (64, 300), (40, 1100)])
+@pytest.mark.parametrize('scored', [False, True])
+def test_decode_scores_of_minus_infinity(B, S, scored):
+    """A key with a score of -inf weighs nothing; where all are, softmax has 0 / 0."""
+    NH, NKV = 4, 2
+    q, k, v = randn((B, NH, 1, 128), 73), randn((B, NKV, S, 128), 74), randn((B, NKV, S, 128), 75)
+    q[..., 0] = 1.0
+    k[0, :, ::3, 0] = float('-inf')
+    k[0, 0, S - 64:, 0] = float('-inf')                    # the last tiles whole
+    lengths = rows([S] * B)
+    acc = torch.zeros(B, NKV, S, device='cuda') if scored else None
+    out, wt, tol = ref.decode(q, k, v, lengths, None, None, 0, SC)
+    ref.assert_within(lf().decode(q.cuda(), lf().KVCache(k.cuda(), v.cuda()), lengths.cuda(), acc=acc), out, tol)
+    if scored:
+        assert (acc[0, :, ::3] == 0).all() and torch.isfinite(acc).all()
+    k[0, 1, :, 0] = float('-inf')
+    got = lf().decode(q.cuda(), lf().KVCache(k.cuda(), v.cuda()), lengths.cuda(), acc=acc)
+    assert torch.isnan(got[0, 0, 2:]).all() and torch.isfinite(got[0, 0, :2]).all() and torch.isfinite(got[1:]).all()
+    if scored:
+        assert torch.isnan(acc[0, 1]).all() and torch.isfinite(acc[0, 0]).all()
+
+
+def test_prefill_scores_of_minus_infinity():
+    NH, NKV, L, pad = 4, 2, 200, 3
+    q, k, v = randn((1, NH, L, 128), 76), randn((1, NKV, L, 128), 77), randn((1, NKV, L, 128), 78)
+    q[..., 0] = 1.0
+    k[0, :, 100:110, 0] = float('-inf')
+    starts = rows([pad])
+    for window in (None, 8):                                # 8: tokens 107 to 109 see such keys alone
+        out, tol = ref.prefill(q, k, v, 0, starts, window, 0, SC)
+        got = lf().prefill(q.cuda(), k.cuda(), v.cuda(), window=window, starts=starts.cuda()).cpu()
+        nan = torch.isnan(out)
+        assert torch.equal(torch.isnan(got), nan) and bool(nan.any()) == (window == 8)
+        ref.assert_within(got[~nan], out[~nan], tol[~nan])
+        assert (got[0, :pad] == 0).all()
+
+
+@pytest.mark.parametrize('big', [2 ** 31 - 1, 2 ** 31, 2 ** 32 + 5, 2 ** 62])
+def test_windows_and_sinks_of_any_size(big):
+    """More than the cache holds, past 32 bits too: no window, or every slot a sink."""
+    NH, NKV, S, L = 8, 2, 200, 70
+    q, k, v = randn((1, NH, L, 128), 79).cuda(), randn((1, NKV, S, 128), 80).cuda(), randn((1, NKV, S, 128), 81).cuda()
+    starts, n = torch.tensor([9], device='cuda'), torch.tensor([S], device='cuda')
+    cache = lf().KVCache(k, v)
+    whole, step = lf().prefill(q, k, v, starts=starts), lf().decode(q[:, :, -1:], cache, n, starts=starts)
+    for kw in (dict(window=big), dict(window=16, sinks=big), dict(window=big, sinks=big)):
+        # the same sums over other tiles: equal up to the rounding of the weights
+        torch.testing.assert_close(lf().prefill(q, k, v, starts=starts, **kw), whole, atol=2.0 ** -6, rtol=2.0 ** -6)
+        torch.testing.assert_close(lf().decode(q[:, :, -1:], cache, n, starts=starts, **kw), step, atol=2.0 ** -6, rtol=2.0 ** -6)
+    from flashb._native import FlashbError
+    into = lf().KVCache(torch.zeros_like(k), torch.zeros_like(v))
+    acc = torch.zeros(1, NKV, S, device='cuda')
+    for f in (lambda: lf().evict(cache, acc, n, big, into=into), lambda: lf().evict(cache, acc, n, 8, into=into, sinks=big),
+              lambda: lf().evict(cache, acc, n, 8, into=into, recent=big), lambda: lf().prefill(q, k, v, q_start=big),
+              lambda: lf().decode(q[:, :, -1:], cache, n, window=4, sinks=-big),
+              lambda: lf().evict(cache, acc, n, 8, into=into, starts=starts, lengths_into=starts)):
+        with pytest.raises(FlashbError):
+            f()

@@ -109,7 +109,7 @@ def test_python_refuses_cpu_tensors():
 
 
 def test_reference_quantiser_by_hand():
-    """The checker itself: ties, saturation and flushing of the 4-bit form."""
+    """The reference itself: ties, saturation and flushing of the 4-bit form."""
     x = torch.zeros(8, 16, dtype=torch.bfloat16)
     x[0, :8] = torch.tensor([6.0, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0])
     x[1] = -3 * x[0]
