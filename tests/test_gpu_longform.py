@@ -591,3 +591,22 @@ def test_windows_and_sinks_of_any_size(big):
               lambda: lf().evict(cache, acc, n, 8, into=into, starts=starts, lengths_into=starts)):
         with pytest.raises(FlashbError):
             f()
+
+
+@pytest.mark.parametrize('scaling', [-0.1, 0.0, 0.05])
+@pytest.mark.parametrize('heads', HEADS)
+@pytest.mark.parametrize('bits', [16, 4])
+@pytest.mark.parametrize('B', [1, 70])
+def test_decode_scalings_of_any_sign(scaling, heads, bits, B):
+    NH, NKV = heads
+    S = 150
+    q, k, v = randn((B, NH, 1, 128), 82), randn((B, NKV, S, 128), 83), randn((B, NKV, S, 128), 84)
+    lengths = rows([S - b % 9 for b in range(B)])
+    if bits == 4:
+        cache, k, v = four(k, v)
+    else:
+        cache = lf().KVCache(k.cuda(), v.cuda())
+    acc = torch.zeros(B, NKV, S, device='cuda')
+    out, wt, tol = ref.decode(q, k, v, lengths, None, None, 0, scaling)
+    ref.assert_within(lf().decode(q.cuda(), cache, lengths.cuda(), scaling=scaling, acc=acc), out, tol)
+    assert (acc.cpu().double() - wt).abs().max() <= 2.0 ** -12 * wt.max()
