@@ -18,11 +18,11 @@
 // columns each).  The running maximum moves only when a tile's exceeds it by 2^8 (the sums are exact either way), so O is
 // hardly ever rescaled.  Masks are applied to the segments that need one for some row of the CTA.
 //
-// Measured on a B200: 8192 tokens, 16 heads over 4, window 1024: 83 us, 775 TFLOP/s; windows of 512 and 2048 56 and 126 us,
+// Measured on a B200: 8192 tokens, 16 heads over 4, window 1024: 81 us, 795 TFLOP/s; windows of 512 and 2048 55 and 123 us,
 // so about 1150 TFLOP/s and 25 us that do not grow with the window (beginning and ending 3.5 waves of CTAs).  What bounds
 // it is the chain of one softmax warp (wait, TMEM read, maximum, exponentials, TMEM write; about 1700 cycles a tile, two
 // CTAs side by side): with three quarters of P V, seven eighths of S, the exponential unit's share or the copies' traffic
-// left out, the time moved by 5% at most.  Tried and slower: P over S's columns with S twice (88 us: S waits for P V),
+// left out, the time moved by 5% at most.  Tried, against 83 us then: P over S's columns with S twice (88 us: S waits for P V),
 // two threads per row (93), alternate tiles to two groups of warps (93 to 132), one warp issuing everything (113), CTAs
 // that go on to further units (85, and 301 instead of 257 us with a causal mask alone), part of the exponentials as
 // polynomials on the FMA pipe (98 to 106), 128-key tiles with S and P V in turn (127).
@@ -53,7 +53,7 @@ struct alignas(64) LongPrefillArgs {
   const bf16 *q, *k, *v;
   long long q_sb, q_sh, q_sl, k_sb, k_sh, k_sl, v_sb, v_sh, v_sl;
   const long long* starts;
-  int NH, NKV, G, nq, L, q_start, window, sinks;  // nq = 128 / G tokens a CTA; window 0: none
+  int B, NH, NKV, G, nq, L, q_start, window, sinks;  // nq = 128 / G tokens a CTA; window 0: none
   float scale;                                    // scaling x log2(e)
   bf16* out;
   long long o_sb, o_sl, o_sh;
@@ -180,8 +180,11 @@ __global__ void __launch_bounds__(LP_THREADS, 2) long_prefill_kernel(const __gri
   __shared__ __align__(8) uint64_t bar_k[2], bar_v[2], bar_s[2], bar_f, bar_p[2], bar_o[2];
   __shared__ uint32_t tslot;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int qt = gridDim.x - 1 - blockIdx.x;       // the latest tokens first: they have the most keys
-  const int h = blockIdx.y, b = blockIdx.z, q0 = qt * a.nq;
+  // the latest tokens of every row and head first: they have the most keys, and the short ones end the launch (head after
+  // head instead: 83.8 against 81.3 us at the size above, 70.3 against 65.7 at 4 rows of 2048; 16 rows of 8192, whose
+  // windows pass the L2, 1305 against 1317)
+  const int at = blockIdx.x / (a.B * a.NKV), bh = blockIdx.x - at * (a.B * a.NKV);
+  const int b = bh / a.NKV, h = bh - b * a.NKV, q0 = ((a.L - 1) / a.nq - at) * a.nq;
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bar_k[i], 1);
@@ -496,13 +499,15 @@ extern "C" int flashb_long_prefill(const void* q, int64_t q_sb, int64_t q_sh, in
   FB_CHECK_ARG((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & 15) == 0 &&
                    (q_sb | q_sh | q_sl | k_sb | k_sh | k_sl | v_sb | v_sh | v_sl | o_sb | o_sl | o_sh) % 8 == 0,
                "long_prefill: tensors must be 16-byte aligned with strides multiple of 8 elements");
-  FB_CHECK_ARG(q_sl >= LG_D && k_sl >= LG_D && v_sl >= LG_D && NKV <= 65535 && B <= 65535, "long_prefill: bad strides or grid");
+  FB_CHECK_ARG(q_sl >= LG_D && k_sl >= LG_D && v_sl >= LG_D, "long_prefill: position strides below the row");
   FB_CHECK_ARG((q_sb | q_sh | k_sb | k_sh | v_sb | v_sh) >= 0 && (B == 1 || (q_sb > 0 && k_sb > 0 && v_sb > 0)) &&
                    (NH == 1 || (q_sh > 0 && o_sh > 0)) && (NKV == 1 || (k_sh > 0 && v_sh > 0)) && (B == 1 || o_sb > 0) &&
                    (L == 1 || o_sl > 0),
                "long_prefill: batch and head strides must be positive");
   LongPrefillArgs a{};
   const int nq = LP_ROWS / G;
+  const int64_t pairs = (int64_t)B * NKV, ctas = pairs <= 0x7fffffff ? (L + nq - 1) / nq * pairs : pairs;
+  FB_CHECK_ARG(ctas <= 0x7fffffff, "long_prefill: too many rows, heads and tokens");
   int rc = lp_map_rows(&a.tq, q, L, NH, B, q_sl, q_sh, q_sb, nq, G);
   if (!rc) rc = lp_map_rows(&a.to, out, L, NH, B, o_sl, o_sh, o_sb, nq, G);
   const long long n = (long long)q_start + L;     // later slots read as zeros
@@ -515,7 +520,7 @@ extern "C" int flashb_long_prefill(const void* q, int64_t q_sb, int64_t q_sh, in
   a.q_sb = q_sb, a.q_sh = q_sh, a.q_sl = q_sl, a.k_sb = k_sb, a.k_sh = k_sh, a.k_sl = k_sl;
   a.v_sb = v_sb, a.v_sh = v_sh, a.v_sl = v_sl;
   a.starts = (const long long*)starts;
-  a.NH = NH, a.NKV = NKV, a.G = G, a.nq = nq, a.L = L, a.q_start = q_start;
+  a.B = B, a.NH = NH, a.NKV = NKV, a.G = G, a.nq = nq, a.L = L, a.q_start = q_start;
   a.window = window > 0 && window < S ? window : 0;
   a.sinks = sinks < S ? sinks : S;                 // slot + sinks stays an int
   a.scale = scaling * LG_LOG2E, a.out = (bf16*)out, a.o_sb = o_sb, a.o_sl = o_sl, a.o_sh = o_sh;
@@ -532,6 +537,6 @@ extern "C" int flashb_long_prefill(const void* q, int64_t q_sb, int64_t q_sh, in
     if (dev < 64) attr_done[dev] = 1;
   }
   void* args[] = {(void*)&a};
-  return fbh::launch_pdl((const void*)long_prefill_kernel, dim3((L + nq - 1) / nq, NKV, B), dim3(LP_THREADS), LP_SMEM,
+  return fbh::launch_pdl((const void*)long_prefill_kernel, dim3((unsigned)ctas), dim3(LP_THREADS), LP_SMEM,
                          (cudaStream_t)stream, args, true);
 }
