@@ -82,7 +82,7 @@ struct LongTile {
   static constexpr int CTAS = BITS == 16 ? 3 : 4;
   static constexpr int KEYS = BITS == 16 ? 16 : 32;      // keys per warp and step
   static constexpr int CHUNK = KEYS * LD_WARPS;
-  static constexpr int EXTRA = 2;                        // empty chunks before a row's own (see long_count)
+  static constexpr int EXTRA = 1;                        // empty chunks before a row's own (see LongPlace)
   static constexpr float SHIFT = BITS == 16 ? 0.f : 6.f; // P x 2^6 in fp16: with the 2^8 of slack below its 65504
 };
 
@@ -127,7 +127,8 @@ __device__ __forceinline__ uint2 ld_nc_v2(const void* p) {
 
 // The list of chunks: row b's NKV heads in turn, ceil(visible / chunk) chunks each after EXTRA empty ones.  Beginning a
 // row costs a CTA some microseconds (q, the first loads, its part of the output), and the empty chunks stand for that:
-// with ragged rows the CTAs of many short ones came out last by a quarter of the time without them.  Every warp works the
+// with ragged rows the CTAs of many short ones came out last by a quarter of the time without them (the 4-bit case above,
+// one to four of them: 38.4, 38.7, 39.2, 40.1 us).  Every warp works the
 // list out for itself (no barrier): lane i counts the chunks of rows [i per, i per + per).
 struct LongPlace {
   int b, before;                        // batch row, chunks of one KV head of all rows before it

@@ -232,7 +232,8 @@ int flashb_lm_head_rows(const void* hidden, int64_t ldh, int B, int H, const flo
  * decodes over a bf16 cache of the whole sequence).  Row b's keys are slots [starts[b], lengths[b]) (device int64;
  * starts NULL = 0; both are clamped to the cache); the token at slot p sees slot j when starts[b] <= j <= p and
  * (j > p - window or j < starts[b] + sinks); window <= 0 = no window.  D is 128, NH / NKV in {1, 2, 4, 8}.  Slots
- * that are not visible are not read, or get no weight, whatever they hold; without a visible slot the output is 0. */
+ * that are not visible are not read, or get no weight, whatever they hold; without a visible slot the output is 0 (with
+ * visible scores of -inf alone it is NaN, as a NaN in a visible slot makes it). */
 typedef struct {
   int bits;              /* 16: bf16 rows [B, NKV, S, 128].  4: e2m1 codes [B, NKV, S, 64] uint8 (two per byte, the
                           * even element in the low half) and e4m3 scales [B, NKV, S, 8] uint8, one per 16 values */
