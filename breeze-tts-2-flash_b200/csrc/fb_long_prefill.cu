@@ -156,7 +156,9 @@ __device__ __noinline__ void long_row_again(const LongPrefillArgs& a, int b, int
     o[2] = o[2] * f + w * lo_f(vw.y);
     o[3] = o[3] * f + w * hi_f(vw.y);
   }
-  const float inv = 1.f / sum;                     // scores of -inf alone: 0 / 0, as softmax has it
+  // scores of -inf alone: 0 / 0, as softmax has it; nothing visible (a padded token that shares its tile with tokens that
+  // see the odd value): 0
+  const float inv = row.n == 0 ? 0.f : 1.f / sum;
   d += (lane >> 4) * (LP_Q / 2) + ((((lane & 15) >> 1) ^ x) << 4) + (lane & 1) * 8;
   *reinterpret_cast<uint2*>(d) = make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
 }
