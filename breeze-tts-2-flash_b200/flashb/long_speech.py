@@ -10,8 +10,8 @@ attention weight, in any combination.
 
 ``graph`` carries the attributes that ``flashb.backbone.fused_decode_step`` reads (an official ``BackboneGraph``, or
 ``flashb.engine.SyntheticBackboneGraph``); its own static cache and mask are not used.  Keys enter the cache after their
-rotary embedding, so their slot may change while their position stays; positions go on as far as the graph's rotary
-table.  With ``keep`` the caches are evicted to that many slots when they are full, each layer by its own weights; without
+rotary embedding, so their slot may change while their position stays; a reading that reaches the end of the graph's
+rotary table raises.  With ``keep`` the caches are evicted to that many slots when they are full, each layer by its own weights; without
 it a full cache raises.
 
     python -m flashb.long_speech --frames 200 --slots 256 --four-bits --window 128 --keep 192
@@ -54,6 +54,8 @@ class LongSpeech:
         self.lengths = torch.zeros(B, dtype=torch.int64, device=dev)
         self.starts = torch.zeros(B, dtype=torch.int64, device=dev)
         self.used = 0                                     # the largest length (every row grows by one a step)
+        self.table = st['cos_tab'].shape[0]               # positions that the rotary table has
+        self.next = 0                                     # no row's next position is beyond it
         self.rows = torch.arange(B, device=dev)
         self.zero = torch.zeros(1, dtype=torch.int64, device=dev)
         self.new_k, self.new_v = (torch.empty(B, self.NKV, 1, 128, dtype=torch.bfloat16, device=dev) for _ in range(2))
@@ -99,6 +101,8 @@ class LongSpeech:
         B, L, H = inputs_embeds.shape
         if L > self.slots or self.used:
             raise FlashbError(FB_ERR_STATE, f'long speech: a prompt of {L} into {self.slots} slots, {self.used} in use')
+        if L > self.table and (starts is None or L - int(starts.min()) > self.table):
+            raise FlashbError(FB_ERR_STATE, f'long speech: a prompt of {L} with a rotary table of {self.table} positions')
         if starts is not None:
             self.starts.copy_(starts)
         at = torch.arange(L, device=self.device)
@@ -118,7 +122,7 @@ class LongSpeech:
             x = self._mlp(Lw, ao.view(B * L, -1), x)
         hidden = torch.empty(B, L, H, dtype=torch.bfloat16, device=self.device)
         fx.rmsnorm(x, st['norm_w'], st['norm_eps'], hidden.view(B * L, H))
-        self.used = L
+        self.used = self.next = L
         self.lengths.fill_(L)
         self.graph.position_ids.copy_((L - self.starts).view(B, 1))
         return hidden
@@ -128,11 +132,17 @@ class LongSpeech:
         ``graph.position_ids[b]``, and both move on by one."""
         g, st, fx = self.graph, self.st, kernels.fused()
         B = st['B']
+        if self.next >= self.table:
+            # past the table a token would get no rotary embedding and its key no place; the rows may be padded, so look
+            self.next = int(g.position_ids.max())
+            if self.next >= self.table:
+                raise FlashbError(FB_ERR_STATE, f'long speech: all {self.table} positions of the rotary table are in use')
         if self.used == self.slots:
             self._evict()
         slots = self.lengths.view(B, 1).clone()
         self.lengths += 1
         self.used += 1
+        self.next += 1
         pos = g.position_ids.view(-1)
         fx.embed_rope(g.input_ids_buf.view(B, -1), st['vocab'], st['embed'], pos, st['cos_tab'], st['sin_tab'], st['x0'],
                       st['cos'], st['sin'])
