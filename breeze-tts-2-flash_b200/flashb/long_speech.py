@@ -9,9 +9,11 @@ attention weight, in any combination.
         speech.step()                             # graph.hidden_buf, logits_buf, cfg_logits_buf as after a decode step
 
 ``graph`` carries the attributes that ``flashb.backbone.fused_decode_step`` reads (an official ``BackboneGraph``, or
-``flashb.engine.SyntheticBackboneGraph``); its own static cache and mask are not used.  Keys enter the cache after their
-rotary embedding, so their slot may change while their position stays; a reading that reaches the end of the graph's
-rotary table raises.  With ``keep`` the caches are evicted to that many slots when they are full, each layer by its own weights; without
+``flashb.engine.SyntheticBackboneGraph``); its own static cache and mask are not used, so give it the smallest
+``max_seq_len`` that its other uses need, and the reading's length to ``positions``: a rotary table of that many entries
+(512 bytes each, all that grows with the reading; None: the graph's table, ``max_seq_len`` + 1).  Keys enter the cache
+after their rotary embedding, so their slot may change while their position stays; a reading that reaches the end of the
+table raises.  With ``keep`` the caches are evicted to that many slots when they are full, each layer by its own weights; without
 it a full cache raises.
 
     python -m flashb.long_speech --frames 200 --slots 256 --four-bits --window 128 --keep 192
@@ -26,8 +28,20 @@ from . import kernels, longform
 from ._native import FB_ERR_ARG, FB_ERR_STATE, FlashbError
 
 
+def rotary_table(graph, n, device):
+    """cos / sin [n, 128] bf16 of positions 0 .. n - 1 as the graph's own table has them."""
+    if hasattr(graph, 'model'):
+        with torch.no_grad():
+            x = torch.zeros(1, n, 128, dtype=torch.bfloat16, device=device)
+            cos, sin = graph.model.rotary_emb(x, torch.arange(n, device=device)[None])
+        return tuple(t[0].to(torch.bfloat16).contiguous() for t in (cos, sin))
+    from .engine import rope_table
+    return rope_table(graph.cfg.theta, 128, n, device)
+
+
 class LongSpeech:
-    def __init__(self, graph, slots, four_bits=False, window=None, sinks=4, keep=None, recent=None, decay=1.0):
+    def __init__(self, graph, slots, four_bits=False, window=None, sinks=4, keep=None, recent=None, decay=1.0,
+                 positions=None):
         st = bb._prep(graph)
         if st is None:
             raise FlashbError(FB_ERR_ARG, 'long speech: the graph is outside the fused decode step')
@@ -54,7 +68,11 @@ class LongSpeech:
         self.lengths = torch.zeros(B, dtype=torch.int64, device=dev)
         self.starts = torch.zeros(B, dtype=torch.int64, device=dev)
         self.used = 0                                     # the largest length (every row grows by one a step)
-        self.table = st['cos_tab'].shape[0]               # positions that the rotary table has
+        if positions is not None and positions < 1:
+            raise FlashbError(FB_ERR_ARG, f'long speech: a rotary table of {positions} positions')
+        self.cos_tab, self.sin_tab = ((st['cos_tab'], st['sin_tab']) if positions is None else
+                                      rotary_table(graph, positions, dev))
+        self.table = self.cos_tab.shape[0]                # positions that the rotary table has
         self.next = 0                                     # no row's next position is beyond it
         self.rows = torch.arange(B, device=dev)
         self.zero = torch.zeros(1, dtype=torch.int64, device=dev)
@@ -112,7 +130,7 @@ class LongSpeech:
         x = inputs_embeds.reshape(B * L, H).contiguous()
         for Lw, cache in zip(st['layers'], self.caches):
             qkv = self._qkv(Lw, x)
-            fx.prefill_qkv(qkv, B, L, self.NH, self.NKV, Lw.qn_w, Lw.kn_w, Lw.qk_eps, st['cos_tab'], st['sin_tab'], pos, at,
+            fx.prefill_qkv(qkv, B, L, self.NH, self.NKV, Lw.qn_w, Lw.kn_w, Lw.qk_eps, self.cos_tab, self.sin_tab, pos, at,
                            k, v)
             q = qkv.as_strided((B, self.NH, L, 128), (L * qkv.stride(0), 128, qkv.stride(0), 1))
             self._put(cache, k, v, slots)
@@ -144,12 +162,12 @@ class LongSpeech:
         self.used += 1
         self.next += 1
         pos = g.position_ids.view(-1)
-        fx.embed_rope(g.input_ids_buf.view(B, -1), st['vocab'], st['embed'], pos, st['cos_tab'], st['sin_tab'], st['x0'],
+        fx.embed_rope(g.input_ids_buf.view(B, -1), st['vocab'], st['embed'], pos, self.cos_tab, self.sin_tab, st['x0'],
                       st['cos'], st['sin'])
         x = st['x0']
         for i, (Lw, cache) in enumerate(zip(st['layers'], self.caches)):
             qkv = self._qkv(Lw, x)
-            fx.prefill_qkv(qkv, B, 1, self.NH, self.NKV, Lw.qn_w, Lw.kn_w, Lw.qk_eps, st['cos_tab'], st['sin_tab'], pos,
+            fx.prefill_qkv(qkv, B, 1, self.NH, self.NKV, Lw.qn_w, Lw.kn_w, Lw.qk_eps, self.cos_tab, self.sin_tab, pos,
                            self.zero, self.new_k, self.new_v)
             self._put(cache, self.new_k, self.new_v, slots)
             q = qkv.as_strided((B, self.NH, 1, 128), (qkv.stride(0), 128, qkv.stride(0), 1))
@@ -200,8 +218,9 @@ def main(argv=None):
     ap.add_argument('--keep', type=int)
     a = ap.parse_args(argv)
     cfg = BackboneConfig(layers=a.layers)
-    g = SyntheticBackboneGraph(cfg, batch_size=a.batch, max_seq_len=a.prompt + a.frames + 1)
-    s = LongSpeech(g, a.slots, four_bits=a.four_bits, window=a.window, sinks=a.sinks, keep=a.keep)
+    g = SyntheticBackboneGraph(cfg, batch_size=a.batch, max_seq_len=1)
+    s = LongSpeech(g, a.slots, four_bits=a.four_bits, window=a.window, sinks=a.sinks, keep=a.keep,
+                   positions=a.prompt + a.frames)
     gen = torch.Generator().manual_seed(1)
     s.prefill(torch.randn(a.batch, a.prompt, cfg.hidden, generator=gen).to(torch.bfloat16).cuda())
     ids = torch.randint(0, cfg.vocab, (a.frames, a.batch, 1, cfg.codebooks), generator=gen).cuda()

@@ -39,3 +39,47 @@ def test_prompt_past_the_rotary_table_raises():
     # 31 positions: a padded prompt of 34 fits where no row has more tokens than that
     assert torch.isfinite(s.prefill(_prompt(cfg, 2, 34), torch.tensor([3, 4], device='cuda'))).all()
     assert int(g.position_ids.max()) == 31
+
+
+def test_a_table_of_its_own_instead_of_a_long_graph():
+    """A graph of one slot and ``positions``: the same bits as on a graph whose own cache covers the whole reading."""
+    from flashb._native import FlashbError
+    from flashb.engine import BackboneConfig, SyntheticBackboneGraph
+    from flashb.long_speech import LongSpeech
+    cfg = BackboneConfig(layers=2)
+    long = SyntheticBackboneGraph(cfg, batch_size=2, max_seq_len=119, seed=5)
+    short = SyntheticBackboneGraph(cfg, batch_size=2, max_seq_len=1, weights_from=long)
+    kw = dict(slots=48, keep=30, sinks=2, window=25, four_bits=True)
+    a, b = LongSpeech(long, **kw), LongSpeech(short, positions=120, **kw)
+    assert torch.equal(a.cos_tab, b.cos_tab) and torch.equal(a.sin_tab, b.sin_tab)
+    x = _prompt(cfg, 2, 20)
+    assert torch.equal(a.prefill(x), b.prefill(x))
+    for ids in _ids(cfg, 2, 100):
+        for g, s in ((long, a), (short, b)):
+            g.input_ids_buf.copy_(ids)
+            s.step()
+        assert torch.equal(long.hidden_buf, short.hidden_buf)
+    for s in (a, b):
+        with pytest.raises(FlashbError):
+            s.step()
+    with pytest.raises(FlashbError):
+        LongSpeech(short, positions=0, **kw)
+
+
+def test_command_holds_no_cache_of_the_whole_reading(capsys):
+    """What the command allocates does not grow with the frames, but for the rotary table; its logits are finite."""
+    from flashb import long_speech
+    args = ['--layers', '2', '--prompt', '20', '--slots', '32', '--keep', '24', '--window', '16']
+
+    def peak(frames):
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        long_speech.main(args + ['--frames', str(frames)])
+        assert 'logits finite: True' in capsys.readouterr().out
+        return torch.cuda.max_memory_allocated() - before
+    peak(8)                                                        # what the first use of the libraries takes
+    a, b = peak(8), peak(300)
+    # the ids of the frames (2 rows of 16 int64) and cos and sin of 128 bf16; 4096 for the allocator's rounding
+    assert b - a <= 292 * (2 * 16 * 8 + 2 * 128 * 2) + 4096
