@@ -15,7 +15,7 @@ that are not visible may hold anything, NaN included.  bf16 queries, head_dim 12
 scores, softmax and sums, rounded to bf16 once.  No reference counterpart: the reference's cache holds the whole
 sequence in bf16 (``flash/backbone.py``).
 
-Calls run on the current stream of the cache's device; workspaces come from torch's allocator on that stream.
+Calls run on the current stream of the cache's device (``prefill``: of the query's), whichever device is current; workspaces come from torch's allocator on that stream.
 """
 import ctypes
 import math
@@ -29,6 +29,9 @@ D = 128
 _INT = 2 ** 31 - 1
 _BF16, _I64, _F32 = torch.bfloat16, torch.int64, torch.float32
 _raw_stream = torch._C._cuda_getCurrentRawStream       # device index -> cudaStream_t (current_stream() builds an object)
+# The library launches on the current device and sizes grids and workspaces by it; a default stream's handle does not name
+# one.  So a call for another device's cache enters that device first.
+_current, _on = torch._C._cuda_getDevice, torch.cuda.device
 _lib = None
 
 
@@ -126,6 +129,9 @@ class KV4Cache(KVCache):
     def store(self, k, v, slots):
         """Stores bf16 heads ``k`` / ``v`` [B, NKV, L, 128] at ``slots`` ([L], or [B, L]: one list per row; distinct
         within a row, those outside the cache are skipped).  To nearest, ties to even, as in exact arithmetic."""
+        if _current() != self.index:
+            with _on(self.index):
+                return self.store(k, v, slots)
         L = slots.shape[-1]
         if not self._heads(k, L) or not self._heads(v, L):
             _refuse('k, v: [B, NKV, L, 128] bf16 on the cache\'s device, L as in slots')
@@ -139,6 +145,9 @@ class KV4Cache(KVCache):
 
     def read(self, slots):
         """The values at ``slots`` ([L] or [B, L]) as (k, v), each [B, NKV, L, 128] bf16 (0 outside the cache)."""
+        if _current() != self.index:
+            with _on(self.index):
+                return self.read(slots)
         L = slots.shape[-1]
         sb = self._slots(slots, L)
         k = torch.empty(self.B, self.NKV, L, D, dtype=_BF16, device=self.device)
@@ -193,6 +202,10 @@ def decode(query, cache, lengths, *, starts=None, window=None, sinks=0, scaling=
     ``window`` (None: all) and ``sinks`` choose the visible slots.  With ``acc`` [B, NKV, S] fp32 the weight of every
     slot, summed over the query heads of its group, is added: acc_out = decay acc + weight (``acc_out`` None: in place).
     The same inputs give the same bits."""
+    if _current() != cache.index:
+        with _on(cache.index):
+            return decode(query, cache, lengths, starts=starts, window=window, sinks=sinks, scaling=scaling, acc=acc,
+                          acc_out=acc_out, decay=decay, out=out)
     dev, B = cache.device, cache.B
     shape, st = query.shape, query.stride()
     if query.dtype != _BF16 or query.device != dev or len(shape) != 4 or shape[0] != B or shape[2] != 1 or \
@@ -244,6 +257,10 @@ def prefill(query, key, value, *, window=None, sinks=0, starts=None, q_start=Non
     ``key``): ``query`` [B, NH, L, 128] over ``key`` / ``value`` [B, NKV, S, 128], bf16 with any strides that are
     multiples of 8 elements; ``scaling`` > 0.  Returns out [B, L, NH, 128] bf16.  Slots from q_start + L on are not
     read."""
+    if query.is_cuda and _current() != query.get_device():
+        with _on(query.get_device()):
+            return prefill(query, key, value, window=window, sinks=sinks, starts=starts, q_start=q_start,
+                           scaling=scaling, out=out)
     dev = query.device
     B, NH, L = query.shape[:3]
     if not query.is_cuda or not (_bf16_heads(query, B, dev) and _bf16_heads(key, B, dev) and _bf16_heads(value, B, dev)):
@@ -281,6 +298,10 @@ def evict(cache, acc, lengths, keep, *, into, starts=None, sinks=0, recent=0, ac
     Returns (kept [B, NKV, keep] int32: the slot each came from, -1 beyond; lengths [B] int64 of ``into``; the moved
     weights: ``acc_into`` [B, NKV, >= keep], all of it, or a new [B, NKV, keep]; 0 beyond).  ``into``'s rows start at
     slot 0.  Outputs may not be the inputs' tensors."""
+    if _current() != cache.index:
+        with _on(cache.index):
+            return evict(cache, acc, lengths, keep, into=into, starts=starts, sinks=sinks, recent=recent,
+                         acc_into=acc_into, lengths_into=lengths_into)
     dev, B = cache.device, cache.B
     a = _acc(acc, 'acc', cache, cache.S)
     if into.bits != cache.bits or into.device != dev:

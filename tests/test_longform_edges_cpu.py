@@ -19,3 +19,49 @@ def test_rotary_table_is_the_graphs_own():
     for g in (official, types.SimpleNamespace(cfg=BackboneConfig())):
         c, s = rotary_table(g, 50, 'cpu')
         assert torch.equal(c, cos) and torch.equal(s, sin) and c.dtype == torch.bfloat16 and c.is_contiguous()
+
+
+class OnDevice1(torch.Tensor):
+    """A CPU tensor that says it is on cuda:1."""
+    is_cuda = True
+
+    def get_device(self):
+        return 1
+
+
+@pytest.mark.parametrize('current', [0, 1])
+def test_calls_run_on_the_device_of_their_tensors(monkeypatch, current):
+    """Whichever device is current: the library is entered with the cache's, and the current one is as before after it."""
+    from flashb import longform as lf
+    at, calls = [current], []
+
+    class on:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.before, at[0] = at[0], self.index
+
+        def __exit__(self, *exc):
+            at[0] = self.before
+
+    class Lib:
+        def __getattr__(self, name):
+            return lambda *a: calls.append((name, at[0], a[-1])) or 0
+    monkeypatch.setattr(lf, '_current', lambda: at[0])
+    monkeypatch.setattr(lf, '_on', on)
+    monkeypatch.setattr(lf, '_lib', Lib())
+    monkeypatch.setattr(lf, '_raw_stream', lambda index: f'stream of {index}')
+    z = lambda *s, dt=torch.bfloat16: torch.zeros(*s, dtype=dt).as_subclass(OnDevice1)  # noqa: E731
+    q, k, n = z(2, 4, 1, 128), z(2, 2, 16, 128), z(2, dt=torch.int64)
+    u8 = lambda w: z(2, 2, 16, w, dt=torch.uint8)  # noqa: E731
+    cache, c4 = lf.KVCache(k, z(2, 2, 16, 128)), lf.KV4Cache(u8(64), u8(8), u8(64), u8(8))
+    lf.decode(q, cache, n, acc=z(2, 2, 16, dt=torch.float32))
+    lf.prefill(q, k, k)
+    c4.store(k, k, z(16, dt=torch.int64))
+    c4.read(z(16, dt=torch.int64))
+    lf.evict(cache, z(2, 2, 16, dt=torch.float32), n, 4, into=lf.KVCache(z(2, 2, 4, 128), z(2, 2, 4, 128)))
+    assert [c[0] for c in calls] == ['flashb_long_decode_ws_floats', 'flashb_long_decode', 'flashb_long_prefill',
+                                     'flashb_kv4_store', 'flashb_kv4_read', 'flashb_kv_evict']
+    assert all(c[1] == 1 for c in calls) and all(c[2] == 'stream of 1' for c in calls[1:])
+    assert at[0] == current
