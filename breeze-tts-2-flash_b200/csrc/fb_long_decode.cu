@@ -941,6 +941,7 @@ extern "C" int flashb_long_decode(const fb_kv_cache* cache, const void* q, int64
   if (rc) return rc;
   FB_CHECK_ARG(((uintptr_t)q & 15) == 0 && q_sb % 8 == 0 && q_sh % 8 == 0,
                "long_decode: q must be 16-byte aligned with strides multiple of 8 elements");
+  FB_CHECK_ARG(((uintptr_t)out & 7) == 0, "long_decode: out must be 8-byte aligned");   // the merge stores four values at once
   FB_CHECK_ARG(p.ws_floats == 0 || (ws && ((uintptr_t)ws & 15) == 0 && ws_floats >= p.ws_floats),
                "long_decode: workspace of %lld floats, %lld needed", (long long)ws_floats, (long long)p.ws_floats);
   a.q = (const bf16*)q, a.q_sb = q_sb, a.q_sh = q_sh;

@@ -65,3 +65,13 @@ def test_calls_run_on_the_device_of_their_tensors(monkeypatch, current):
                                      'flashb_kv4_store', 'flashb_kv4_read', 'flashb_kv_evict']
     assert all(c[1] == 1 for c in calls) and all(c[2] == 'stream of 1' for c in calls[1:])
     assert at[0] == current
+
+
+@pytest.mark.parametrize('bits', [16, 4])
+@pytest.mark.parametrize('B', [2, 500])                            # a cluster a row, the shared list
+def test_decode_output_off_its_alignment_is_refused(bits, B):
+    from flashb import _native
+    from test_longform_cpu import decode, desc
+    for off in (2, 4, 6):
+        assert decode(desc(bits=bits, B=B), out=(1 << 27) + off) == _native.FB_ERR_ARG
+        assert '8-byte' in _native.last_error()
