@@ -113,16 +113,16 @@ class LongSpeech:
         return qkv
 
     def prefill(self, inputs_embeds, starts=None):
-        """The prompt [B, L, H] bf16 (row b's tokens from ``starts[b]`` on; positions count from there) into empty caches.
-        Returns the hidden states [B, L, H] after the final norm."""
+        """The prompt [B, L, H] bf16 (row b's tokens from ``starts[b]`` on, clamped to 0 .. L; positions count from there) into empty
+        caches.        Returns the hidden states [B, L, H] after the final norm."""
         fx, st = kernels.fused(), self.st
         B, L, H = inputs_embeds.shape
         if L > self.slots or self.used:
             raise FlashbError(FB_ERR_STATE, f'long speech: a prompt of {L} into {self.slots} slots, {self.used} in use')
-        if L > self.table and (starts is None or L - int(starts.min()) > self.table):
+        if L > self.table and (starts is None or L - max(0, int(starts.min())) > self.table):
             raise FlashbError(FB_ERR_STATE, f'long speech: a prompt of {L} with a rotary table of {self.table} positions')
         if starts is not None:
-            self.starts.copy_(starts)
+            self.starts.copy_(starts).clamp_(0, L)
         at = torch.arange(L, device=self.device)
         pos = (at[None] - self.starts[:, None]).clamp_(min=0).contiguous()
         slots = at[None].expand(B, L)

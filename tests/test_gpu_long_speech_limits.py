@@ -83,3 +83,18 @@ def test_command_holds_no_cache_of_the_whole_reading(capsys):
     a, b = peak(8), peak(300)
     # the ids of the frames (2 rows of 16 int64) and cos and sin of 128 bf16; 4096 for the allocator's rounding
     assert b - a <= 292 * (2 * 16 * 8 + 2 * 128 * 2) + 4096
+
+
+def test_starts_outside_the_prompt_are_clamped():
+    """As the operators clamp them: positions neither begin past 0 nor lie below it."""
+    cfg, g, g2, a = _pair(2, 40, slots=32)
+    from flashb.long_speech import LongSpeech
+    b = LongSpeech(g, 32)
+    x = _prompt(cfg, 2, 20)
+    assert torch.equal(a.prefill(x, torch.tensor([-3, 99], device='cuda')), b.prefill(x, torch.tensor([0, 20], device='cuda')))
+    assert g.position_ids.tolist() == [[20], [0]]
+    for ids in _ids(cfg, 2, 3):
+        for h, s in ((g2, a), (g, b)):
+            h.input_ids_buf.copy_(ids)
+            s.step()
+        assert torch.equal(g2.hidden_buf, g.hidden_buf) and torch.equal(g2.position_ids, g.position_ids)
