@@ -50,6 +50,10 @@ class LongSpeech:
         self.graph, self.st, self.slots = graph, st, slots
         self.window, self.sinks, self.keep, self.decay = window, sinks, keep, decay
         self.recent = max(0, min(keep // 4, keep - sinks)) if keep is not None and recent is None else recent or 0
+        if sinks < 0 or self.recent < 0 or (keep is not None and sinks + self.recent > keep):
+            raise FlashbError(FB_ERR_ARG, f'long speech: {sinks} first and {self.recent} last slots of the {keep} that stay')
+        if window is not None and window < 1:
+            raise FlashbError(FB_ERR_ARG, f'long speech: a window of {window}')
         L0 = st['layers'][0]
         B, self.NH, self.NKV = st['B'], L0.wq.shape[0] // 128, L0.wk.shape[0] // 128
         dev = self.device = L0.wq.device
@@ -113,8 +117,8 @@ class LongSpeech:
         return qkv
 
     def prefill(self, inputs_embeds, starts=None):
-        """The prompt [B, L, H] bf16 (row b's tokens from ``starts[b]`` on, clamped to 0 .. L; positions count from there) into empty
-        caches.        Returns the hidden states [B, L, H] after the final norm."""
+        """The prompt [B, L, H] bf16 (row b's tokens from ``starts[b]`` on, clamped to 0 .. L; positions count from there)
+        into empty caches.  Returns the hidden states [B, L, H] after the final norm."""
         fx, st = kernels.fused(), self.st
         B, L, H = inputs_embeds.shape
         if L > self.slots or self.used:
@@ -189,8 +193,7 @@ class LongSpeech:
             raise FlashbError(FB_ERR_STATE, f'long speech: all {self.slots} slots are in use')
         for i, cache in enumerate(self.caches):
             _, n, acc = longform.evict(cache, self.acc[i], self.lengths, self.keep, into=self.spare, starts=self.starts,
-                                       sinks=min(self.sinks, self.keep - self.recent), recent=self.recent,
-                                       acc_into=self.spare_acc)
+                                       sinks=self.sinks, recent=self.recent, acc_into=self.spare_acc)
             self.caches[i], self.spare = self.spare, cache
             self.acc[i], self.spare_acc = acc, self.acc[i]
         self.lengths.copy_(n)

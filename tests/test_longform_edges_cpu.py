@@ -75,3 +75,16 @@ def test_decode_output_off_its_alignment_is_refused(bits, B):
     for off in (2, 4, 6):
         assert decode(desc(bits=bits, B=B), out=(1 << 27) + off) == _native.FB_ERR_ARG
         assert '8-byte' in _native.last_error()
+
+
+@pytest.mark.parametrize('bad', [dict(keep=20, sinks=4, recent=17), dict(keep=20, sinks=4, recent=21), dict(keep=20, sinks=-1),
+                                 dict(keep=20, recent=-1), dict(keep=3, sinks=4), dict(sinks=-1), dict(window=0),
+                                 dict(keep=0), dict(keep=32)])
+def test_long_speech_refuses_settings_that_cannot_be_kept(bad, monkeypatch):
+    """When it is made, not when the cache is full for the first time; nothing is allocated before."""
+    from flashb import long_speech
+    from flashb._native import FB_ERR_ARG, FlashbError
+    monkeypatch.setattr(long_speech.bb, '_prep', lambda g: dict(layers=None, B=2))
+    with pytest.raises(FlashbError) as e:
+        long_speech.LongSpeech(types.SimpleNamespace(), 32, **bad)
+    assert e.value.rc == FB_ERR_ARG
