@@ -194,13 +194,30 @@ extern "C" int flashb_kv_evict(const fb_kv_cache* cache, const float* acc, int64
                "kv_evict: the two caches differ in bits, rows or heads");
   FB_CHECK_ARG(cache->bits == 16 || (into->k_scale == cache->k_scale && into->v_scale == cache->v_scale),
                "kv_evict: the two caches differ in their tensor scales");
-  FB_CHECK_ARG((const void*)acc_out != (const void*)acc && lengths_out != lengths && lengths_out != starts,
-               "kv_evict: the outputs may not be the inputs");
-  FB_CHECK_ARG(into->k != cache->k && into->v != cache->v, "kv_evict: the cache cannot be evicted into itself");
+  FB_CHECK_ARG(lengths_out != lengths && lengths_out != starts, "kv_evict: the outputs may not be the inputs");
   FB_CHECK_ARG(keep >= 1 && keep <= into->S && sinks >= 0 && recent >= 0 && (int64_t)sinks + recent <= keep,
                "kv_evict: keep %d of %d slots with %d first and %d last", keep, into->S, sinks, recent);
   FB_CHECK_ARG(!acc_out || acc_n >= keep, "kv_evict: acc_out holds %d slots, %d stay", acc_n, keep);
   FB_CHECK_ARG((int64_t)cache->B * cache->NKV <= 65535, "kv_evict: more than 65535 rows and heads");
+  const auto boxes = [](const fb_kv_cache* c, const fb::LongCache& x, fbh::LongBox* o) {
+    const int row = c->bits == 16 ? 2 * fb::LG_D : fb::LG_D / 2;
+    o[0] = fbh::long_box(x.k, c->B, c->NKV, c->S, x.k_sb, x.k_sh, x.k_sp, row);
+    o[1] = fbh::long_box(x.v, c->B, c->NKV, c->S, x.v_sb, x.v_sh, x.v_sp, row);
+    if (c->bits == 16) return 2;
+    o[2] = fbh::long_box(x.ks, c->B, c->NKV, c->S, x.ks_sb, x.ks_sh, x.ks_sp, fb::LG_D / 16);
+    o[3] = fbh::long_box(x.vs, c->B, c->NKV, c->S, x.vs_sb, x.vs_sh, x.vs_sp, fb::LG_D / 16);
+    return 4;
+  };
+  fbh::LongBox from[4], to[4];
+  const int nf = boxes(cache, a.c, from), nt = boxes(into, a.d, to);
+  for (int i = 0; i < nf; ++i)
+    for (int j = 0; j < nt; ++j)
+      FB_CHECK_ARG(!fbh::long_boxes_meet(from[i], to[j]), "kv_evict: the two caches share memory");
+  const auto weights = [&](const float* w, int64_t sb, int64_t sh, int n) {
+    return fbh::long_box(w, cache->B, cache->NKV, 1, 4 * sb, 4 * sh, 0, 4ll * n);
+  };
+  FB_CHECK_ARG(!acc_out || !fbh::long_boxes_meet(weights(acc, acc_sb, acc_sh, cache->S), weights(acc_out, acco_sb, acco_sh, acc_n)),
+               "kv_evict: acc and acc_out share memory");
   a.acc = acc, a.acc_sb = acc_sb, a.acc_sh = acc_sh;
   a.lengths = (const long long*)lengths, a.starts = (const long long*)starts;
   a.NKV = cache->NKV, a.S = cache->S, a.keep = keep, a.sinks = sinks, a.recent = recent;

@@ -112,4 +112,12 @@ __device__ __forceinline__ float ex2(float x) {
 namespace fbh {
 // Checks a public cache descriptor (NULL, shapes, alignment, strides) and fills the kernels' form.
 int long_cache(const fb_kv_cache* c, fb::LongCache* out);
+// Rows of `row` bytes at p + i s[0] + j s[1] + k s[2], i < n[0] and so on (byte strides; long_box makes them >= 0).
+struct LongBox {
+  const void* p;
+  long long n[3], s[3], row;
+};
+LongBox long_box(const void* p, int B, int NKV, long long S, long long sb, long long sh, long long sp, long long row);
+// Whether two share a byte (true also where that would take too long to find out: layouts that no tensor of either has).
+bool long_boxes_meet(const LongBox& a, const LongBox& b);
 }  // namespace fbh

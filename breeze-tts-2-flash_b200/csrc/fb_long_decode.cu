@@ -829,6 +829,73 @@ int long_cache(const fb_kv_cache* c, fb::LongCache* out) {
   return FB_OK;
 }
 
+LongBox long_box(const void* p, int B, int NKV, long long S, long long sb, long long sh, long long sp, long long row) {
+  LongBox x{p, {B, NKV, S}, {sb, sh, sp}, row};
+  for (int i = 0; i < 3; ++i)
+    if (x.s[i] < 0) {                             // the same bytes, counted from the other end
+      x.p = (const unsigned char*)x.p + (x.n[i] - 1) * x.s[i];
+      x.s[i] = -x.s[i];
+    }
+  return x;
+}
+
+namespace {
+// An axis along which the distance of two rows changes by s a step, from lo to hi steps.
+struct BoxAxis {
+  long long s, lo, hi;
+};
+// Whether a choice of steps on axes [i, n) brings the distance d into (-rb, ra).
+bool boxes_reach(const BoxAxis* ax, int n, int i, long long d, long long ra, long long rb, int& budget) {
+  if (i == n) return d < rb && d > -ra;
+  if (--budget < 0) return true;
+  long long lo = -ra + 1, hi = rb - 1;            // what the axes after this one can make up for
+  for (int j = i + 1; j < n; ++j) {
+    lo -= ax[j].s * ax[j].hi;
+    hi -= ax[j].s * ax[j].lo;
+  }
+  // steps x with lo <= d + s x <= hi
+  const long long s = ax[i].s, a = lo - d, b = hi - d;
+  long long x0 = a >= 0 ? (a + s - 1) / s : -(-a / s), x1 = b >= 0 ? b / s : -((-b + s - 1) / s);
+  if (x0 < ax[i].lo) x0 = ax[i].lo;
+  if (x1 > ax[i].hi) x1 = ax[i].hi;
+  for (long long x = x0; x <= x1; ++x)
+    if (boxes_reach(ax, n, i + 1, d + s * x, ra, rb, budget)) return true;
+  return false;
+}
+}  // namespace
+
+bool long_boxes_meet(const LongBox& a, const LongBox& b) {
+  const auto span = [](const LongBox& x) {
+    long long e = x.row;
+    for (int i = 0; i < 3; ++i) e += (x.n[i] - 1) * x.s[i];
+    return e;
+  };
+  const long long d = (const unsigned char*)a.p - (const unsigned char*)b.p;
+  if (d >= span(b) || -d >= span(a)) return false;
+  // views of one buffer, or interleaved tensors: the axes with the largest stride first; strides that both have make one
+  // axis of differences, so that rows that nest leave a step or two to try on each
+  BoxAxis ax[6];
+  int n = 0;
+  const auto add = [&](long long s, long long lo, long long hi) {
+    if (s == 0 || lo == hi) return;
+    for (int i = 0; i < n; ++i)
+      if (ax[i].s == s) {
+        ax[i].lo += lo;
+        ax[i].hi += hi;
+        return;
+      }
+    int i = n++;
+    for (; i > 0 && ax[i - 1].s < s; --i) ax[i] = ax[i - 1];
+    ax[i] = {s, lo, hi};
+  };
+  for (int i = 0; i < 3; ++i) {
+    add(a.s[i], 0, a.n[i] - 1);
+    add(b.s[i], 1 - b.n[i], 0);
+  }
+  int budget = 4096;
+  return boxes_reach(ax, n, 0, d, a.row, b.row, budget);
+}
+
 }  // namespace fbh
 
 namespace {

@@ -25,3 +25,39 @@ def test_prefill_padding_is_zero_beside_a_visible_odd_value(heads, bad):
             assert (got[b, :pad] == 0).all()
             sees = torch.arange(past, past + L) >= max(j, st) if j >= st else torch.zeros(L, dtype=torch.bool)
             assert torch.isfinite(got[b, ~sees]).all() and not torch.isfinite(got[b, sees]).any()
+
+
+@pytest.mark.parametrize('bits', [16, 4])
+def test_evict_between_views_that_share_no_memory(bits):
+    """Two layers of a buffer [B, layers, NKV, S, .], its heads beside its slots, and the two ends of each row's slots."""
+    L = lf()
+    B, NKV, S, keep = 2, 2, 60, 20
+    k, v = randn((B, NKV, S, 128), 34), randn((B, NKV, S, 128), 35)
+    acc = torch.rand(B, NKV, S, generator=torch.Generator().manual_seed(36))
+    lengths = rows([60, 41])
+    want, n_want = ref.evict(acc, lengths, None, keep, 1, 2)
+    widths = (128, 128) if bits == 16 else (64, 8, 64, 8)
+    dt = torch.bfloat16 if bits == 16 else torch.uint8
+    every = lambda f: [f(torch.zeros, w) for w in widths]  # noqa: E731
+    layers = every(lambda z, w: z(B, 2, NKV, S, w, dtype=dt, device='cuda'))
+    sides = every(lambda z, w: z(B, S, NKV, 2, w, dtype=dt, device='cuda'))
+    ends = every(lambda z, w: z(B, NKV, 2 * S, w, dtype=dt, device='cuda'))
+    kind = L.KVCache if bits == 16 else L.KV4Cache
+    for src, dst in ((kind(*(t[:, 0] for t in layers)), kind(*(t[:, 1] for t in layers))),
+                     (kind(*(t[..., 0, :].transpose(1, 2) for t in sides)), kind(*(t[..., 1, :].transpose(1, 2) for t in sides))),
+                     (kind(*(t[:, :, :S] for t in ends)), kind(*(t[:, :, S:] for t in ends)))):
+        if bits == 16:
+            src.keys.copy_(k)
+            src.values.copy_(v)
+        else:
+            src.store(k.cuda(), v.cuda(), torch.arange(S, device='cuda'))
+        both = torch.zeros(B, 2, NKV, S, device='cuda')
+        both[:, 0].copy_(acc)
+        kept, n, moved = L.evict(src, both[:, 0], lengths.cuda(), keep, into=dst, sinks=1, recent=2, acc_into=both[:, 1])
+        assert torch.equal(kept.cpu(), want) and torch.equal(n.cpu(), n_want)
+        gk, gv = (dst.keys, dst.values) if bits == 16 else dst.read(torch.arange(keep, device='cuda'))
+        at = want.clamp(min=0).long()
+        for got, x in ((gk, k), (gv, v)):
+            x = x.double() if bits == 16 else ref.quantise(x)
+            assert torch.equal(got[:, :, :keep].cpu().double(), torch.gather(x, 2, at[..., None].expand(-1, -1, -1, 128)))
+        assert torch.equal(moved[..., :keep].cpu(), torch.gather(acc, 2, at)) and (moved[..., keep:] == 0).all()

@@ -88,3 +88,34 @@ def test_long_speech_refuses_settings_that_cannot_be_kept(bad, monkeypatch):
     with pytest.raises(FlashbError) as e:
         long_speech.LongSpeech(types.SimpleNamespace(), 32, **bad)
     assert e.value.rc == FB_ERR_ARG
+
+
+def evict(a, b, keep=8, acc=1 << 20, acc_out=1 << 21, acc_n=8):
+    import ctypes
+
+    from flashb import _native
+    return _native.lib().flashb_kv_evict(ctypes.byref(a), acc, 128, 64, 1 << 24, None, keep, 0, 0, ctypes.byref(b), acc_out, 128,
+                                         64, acc_n, 1 << 25, 1 << 26, None)
+
+
+def test_evict_refuses_memory_in_common():
+    """Views of one buffer at any offset, not the same tensors alone: reads and writes would race."""
+    from flashb import _native
+    from test_longform_cpu import desc
+    row = 2 * 128
+    far = dict(k=1 << 30, v=1 << 31)
+    src = desc()                                           # 2 rows, 2 heads, 64 slots: 64 KB at 1 MB and at 2 MB
+    for k in ((1 << 20) + row, (1 << 20) + 200 * row, (1 << 20) + 255 * row, (1 << 20) - 255 * row, 1 << 21, (1 << 21) - row):
+        for name in ('k', 'v'):
+            assert evict(src, desc(**{**far, name: k})) == _native.FB_ERR_ARG and 'share memory' in _native.last_error()
+    # other slots a head, so other strides: a slot of the one lies in the other
+    assert evict(src, desc(S=48, **{**far, 'k': (1 << 20) + 100 * row})) == _native.FB_ERR_ARG
+    # positions side by side: the halves of rows of 512 bytes share nothing, the same half does
+    wide = dict(k_sb=65536, k_sh=32768, k_sp=256, v_sb=65536, v_sh=32768, v_sp=256)
+    assert evict(desc(**wide), desc(**{**wide, **far, 'k': (1 << 20) + 512 * 9})) == _native.FB_ERR_ARG
+    four = desc(bits=4)
+    far4 = dict(k=1 << 30, v=1 << 31, ks=1 << 32, vs=1 << 33)
+    for name, at in (('k', (1 << 20) + 64), ('ks', (1 << 22) + 8), ('vs', (1 << 22) + 8), ('ks', (1 << 20) + 64)):
+        assert evict(four, desc(bits=4, **{**far4, name: at})) == _native.FB_ERR_ARG, name
+    for at in ((1 << 20) + 4, (1 << 20) - 4, (1 << 20) + 4 * 255, 1 << 20):
+        assert evict(src, desc(**far), acc_out=at) == _native.FB_ERR_ARG and 'acc' in _native.last_error()
