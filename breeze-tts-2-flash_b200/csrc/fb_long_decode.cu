@@ -1003,6 +1003,14 @@ extern "C" int flashb_long_decode(const fb_kv_cache* cache, const void* q, int64
   if (rc) return rc;
   FB_CHECK_ARG(q && lengths && out, "long_decode: null pointer argument");
   FB_CHECK_ARG((acc == nullptr) == (acc_out == nullptr), "long_decode: acc and acc_out come together");
+  if (acc) {
+    const auto weights = [&](const float* w, int64_t sb, int64_t sh) {
+      return fbh::long_box(w, cache->B, cache->NKV, 1, 4 * sb, 4 * sh, 0, 4ll * cache->S);
+    };
+    const bool in_place = acc == acc_out && (cache->B == 1 || acc_sb == acco_sb) && (cache->NKV == 1 || acc_sh == acco_sh);
+    FB_CHECK_ARG(in_place || !fbh::long_boxes_meet(weights(acc, acc_sb, acc_sh), weights(acc_out, acco_sb, acco_sh)),
+                 "long_decode: acc and acc_out share memory and are not the same");
+  }
   LongPlan p;
   rc = long_plan_host(cache, NH, window, sinks, acc != nullptr, &p);
   if (rc) return rc;

@@ -246,7 +246,7 @@ typedef struct {
 } fb_kv_cache;
 /* Single-token attention: q [B, NH, 1, 128] bf16 (strides q_sb, q_sh), the token at slot lengths[b] - 1 of each row;
  * out [B, 1, NH, 128] bf16 contiguous, 8-byte aligned.  fp32 scores, softmax and sums, rounded to bf16 once.  acc /
- * acc_out (both or neither; fp32 [B, NKV, S], unit stride per slot, may be the same buffer): acc_out[b, h, j] =
+ * acc_out (both or neither; fp32 [B, NKV, S], unit stride per slot, may be the same tensor, else share nothing): acc_out[b, h, j] =
  * decay acc[b, h, j] + the weight of slot j summed over the group's query heads, for every slot of the cache.  ws: 16-byte aligned, at
  * least flashb_long_decode_ws_floats() floats (0 for few rows: then it may be NULL), not shared by calls that can overlap,
  * contents free before and after.

@@ -119,3 +119,20 @@ def test_evict_refuses_memory_in_common():
         assert evict(four, desc(bits=4, **{**far4, name: at})) == _native.FB_ERR_ARG, name
     for at in ((1 << 20) + 4, (1 << 20) - 4, (1 << 20) + 4 * 255, 1 << 20):
         assert evict(src, desc(**far), acc_out=at) == _native.FB_ERR_ARG and 'acc' in _native.last_error()
+
+
+@pytest.mark.parametrize('bits', [16, 4])
+def test_decode_refuses_weights_that_overlap_their_sums(bits):
+    """In place or apart; not shifted, and not in place with other strides."""
+    import ctypes
+
+    from flashb import _native
+    from test_longform_cpu import desc
+    d, acc = desc(bits=bits), 1 << 28                         # 2 rows, 2 heads, 64 slots
+
+    def run(out, sb, sh):
+        return _native.lib().flashb_long_decode(ctypes.byref(d), 1 << 24, 1024, 128, 8, 1 << 25, None, 0, 0, 1.0, acc, 128, 64,
+                                                out, sb, sh, 1.0, None, 0, 1 << 27, None)
+    for out, sb, sh in ((acc + 4, 128, 64), (acc - 4, 128, 64), (acc + 4 * 64, 128, 64), (acc, 256, 64), (acc, 64, 128),
+                        (acc - 4 * 63, 64, 64)):
+        assert run(out, sb, sh) == _native.FB_ERR_ARG and 'acc' in _native.last_error()
