@@ -199,17 +199,10 @@ extern "C" int flashb_kv_evict(const fb_kv_cache* cache, const float* acc, int64
                "kv_evict: keep %d of %d slots with %d first and %d last", keep, into->S, sinks, recent);
   FB_CHECK_ARG(!acc_out || acc_n >= keep, "kv_evict: acc_out holds %d slots, %d stay", acc_n, keep);
   FB_CHECK_ARG((int64_t)cache->B * cache->NKV <= 65535, "kv_evict: more than 65535 rows and heads");
-  const auto boxes = [](const fb_kv_cache* c, const fb::LongCache& x, fbh::LongBox* o) {
-    const int row = c->bits == 16 ? 2 * fb::LG_D : fb::LG_D / 2;
-    o[0] = fbh::long_box(x.k, c->B, c->NKV, c->S, x.k_sb, x.k_sh, x.k_sp, row);
-    o[1] = fbh::long_box(x.v, c->B, c->NKV, c->S, x.v_sb, x.v_sh, x.v_sp, row);
-    if (c->bits == 16) return 2;
-    o[2] = fbh::long_box(x.ks, c->B, c->NKV, c->S, x.ks_sb, x.ks_sh, x.ks_sp, fb::LG_D / 16);
-    o[3] = fbh::long_box(x.vs, c->B, c->NKV, c->S, x.vs_sb, x.vs_sh, x.vs_sp, fb::LG_D / 16);
-    return 4;
-  };
+  rc = fbh::long_cache_written(into, a.d, "kv_evict");
+  if (rc) return rc;
   fbh::LongBox from[4], to[4];
-  const int nf = boxes(cache, a.c, from), nt = boxes(into, a.d, to);
+  const int nf = fbh::long_cache_boxes(cache, a.c, from), nt = fbh::long_cache_boxes(into, a.d, to);
   for (int i = 0; i < nf; ++i)
     for (int j = 0; j < nt; ++j)
       FB_CHECK_ARG(!fbh::long_boxes_meet(from[i], to[j]), "kv_evict: the two caches share memory");
@@ -218,6 +211,7 @@ extern "C" int flashb_kv_evict(const fb_kv_cache* cache, const float* acc, int64
   };
   FB_CHECK_ARG(!acc_out || !fbh::long_boxes_meet(weights(acc, acc_sb, acc_sh, cache->S), weights(acc_out, acco_sb, acco_sh, acc_n)),
                "kv_evict: acc and acc_out share memory");
+  FB_CHECK_ARG(!acc_out || !fbh::long_box_folds(weights(acc_out, acco_sb, acco_sh, acc_n)), "kv_evict: rows of acc_out share memory");
   a.acc = acc, a.acc_sb = acc_sb, a.acc_sh = acc_sh;
   a.lengths = (const long long*)lengths, a.starts = (const long long*)starts;
   a.NKV = cache->NKV, a.S = cache->S, a.keep = keep, a.sinks = sinks, a.recent = recent;

@@ -205,9 +205,13 @@ extern "C" int flashb_kv4_store(const fb_kv_cache* cache, const void* k, int64_t
                                 const void* v, int64_t v_sb, int64_t v_sh, int64_t v_sl, const int64_t* slots,
                                 int64_t slot_sb, int L, void* stream) {
   KV4Args a{};
-  const int rc = kv4_fill(cache, slots, slot_sb, L, &a);
+  int rc = kv4_fill(cache, slots, slot_sb, L, &a);
   if (rc) return rc;
   FB_CHECK_ARG(k && v, "kv4_store: null pointer argument");
+  LongCache lc;
+  fbh::long_cache(cache, &lc);
+  rc = fbh::long_cache_written(cache, lc, "kv4_store");
+  if (rc) return rc;
   FB_CHECK_ARG((((uintptr_t)k | (uintptr_t)v) & 15) == 0 && (k_sb | k_sh | k_sl | v_sb | v_sh | v_sl) % 8 == 0,
                "kv4_store: keys and values must be 16-byte aligned with strides multiple of 8 elements");
   a.k = (const bf16*)k, a.xk_sb = k_sb, a.xk_sh = k_sh, a.xk_sl = k_sl;

@@ -120,4 +120,10 @@ struct LongBox {
 LongBox long_box(const void* p, int B, int NKV, long long S, long long sb, long long sh, long long sp, long long row);
 // Whether two share a byte (true also where that would take too long to find out: layouts that no tensor of either has).
 bool long_boxes_meet(const LongBox& a, const LongBox& b);
+// Whether rows of one share a byte: a stride of 0 (an expanded tensor), or rows that do not nest.
+bool long_box_folds(const LongBox& x);
+// The keys, values and (4 bits) scales of a cache: how many boxes.
+int long_cache_boxes(const fb_kv_cache* c, const fb::LongCache& x, LongBox (&out)[4]);
+// A cache that a kernel writes: FB_OK, or a refusal where two of its slots share memory.
+int long_cache_written(const fb_kv_cache* c, const fb::LongCache& x, const char* who);
 }  // namespace fbh

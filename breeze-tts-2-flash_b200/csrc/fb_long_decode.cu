@@ -896,6 +896,44 @@ bool long_boxes_meet(const LongBox& a, const LongBox& b) {
   return boxes_reach(ax, n, 0, d, a.row, b.row, budget);
 }
 
+bool long_box_folds(const LongBox& x) {
+  int o[3] = {0, 1, 2};
+  for (int i = 1; i < 3; ++i)
+    for (int j = i; j > 0 && x.s[o[j]] < x.s[o[j - 1]]; --j) {
+      const int t = o[j];
+      o[j] = o[j - 1];
+      o[j - 1] = t;
+    }
+  long long e = x.row;                            // bytes from the first to the last row so far
+  for (int i : o) {
+    if (x.n[i] == 1) continue;
+    if (x.s[i] < e) return true;
+    e += (x.n[i] - 1) * x.s[i];
+  }
+  return false;
+}
+
+int long_cache_boxes(const fb_kv_cache* c, const fb::LongCache& x, LongBox (&out)[4]) {
+  const int row = c->bits == 16 ? 2 * fb::LG_D : fb::LG_D / 2;
+  out[0] = long_box(x.k, c->B, c->NKV, c->S, x.k_sb, x.k_sh, x.k_sp, row);
+  out[1] = long_box(x.v, c->B, c->NKV, c->S, x.v_sb, x.v_sh, x.v_sp, row);
+  if (c->bits == 16) return 2;
+  out[2] = long_box(x.ks, c->B, c->NKV, c->S, x.ks_sb, x.ks_sh, x.ks_sp, fb::LG_D / 16);
+  out[3] = long_box(x.vs, c->B, c->NKV, c->S, x.vs_sb, x.vs_sh, x.vs_sp, fb::LG_D / 16);
+  return 4;
+}
+
+int long_cache_written(const fb_kv_cache* c, const fb::LongCache& x, const char* who) {
+  LongBox box[4];
+  const int n = long_cache_boxes(c, x, box);
+  for (int i = 0; i < n; ++i) {
+    FB_CHECK_ARG(!long_box_folds(box[i]), "%s: slots of the cache that is written share memory", who);
+    for (int j = 0; j < i; ++j)
+      FB_CHECK_ARG(!long_boxes_meet(box[i], box[j]), "%s: keys, values and scales of the cache that is written share memory", who);
+  }
+  return FB_OK;
+}
+
 }  // namespace fbh
 
 namespace {
@@ -1010,6 +1048,7 @@ extern "C" int flashb_long_decode(const fb_kv_cache* cache, const void* q, int64
     const bool in_place = acc == acc_out && (cache->B == 1 || acc_sb == acco_sb) && (cache->NKV == 1 || acc_sh == acco_sh);
     FB_CHECK_ARG(in_place || !fbh::long_boxes_meet(weights(acc, acc_sb, acc_sh), weights(acc_out, acco_sb, acco_sh)),
                  "long_decode: acc and acc_out share memory and are not the same");
+    FB_CHECK_ARG(!fbh::long_box_folds(weights(acc_out, acco_sb, acco_sh)), "long_decode: rows of acc_out share memory");
   }
   LongPlan p;
   rc = long_plan_host(cache, NH, window, sinks, acc != nullptr, &p);

@@ -506,6 +506,8 @@ extern "C" int flashb_long_prefill(const void* q, int64_t q_sb, int64_t q_sh, in
                    (NH == 1 || (q_sh > 0 && o_sh > 0)) && (NKV == 1 || (k_sh > 0 && v_sh > 0)) && (B == 1 || o_sb > 0) &&
                    (L == 1 || o_sl > 0),
                "long_prefill: batch and head strides must be positive");
+  FB_CHECK_ARG(!fbh::long_box_folds(fbh::long_box(out, B, NH, L, 2 * o_sb, 2 * o_sh, 2 * o_sl, 2 * LG_D)),
+               "long_prefill: rows of out share memory");
   LongPrefillArgs a{};
   const int nq = LP_ROWS / G;
   const int64_t pairs = (int64_t)B * NKV, ctas = pairs <= 0x7fffffff ? (L + nq - 1) / nq * pairs : pairs;

@@ -136,3 +136,37 @@ def test_decode_refuses_weights_that_overlap_their_sums(bits):
     for out, sb, sh in ((acc + 4, 128, 64), (acc - 4, 128, 64), (acc + 4 * 64, 128, 64), (acc, 256, 64), (acc, 64, 128),
                         (acc - 4 * 63, 64, 64)):
         assert run(out, sb, sh) == _native.FB_ERR_ARG and 'acc' in _native.last_error()
+
+
+def test_outputs_that_overlap_themselves_are_refused():
+    """Expanded tensors (a stride of 0) and keys that are the values: rows of such an output would race."""
+    import ctypes
+
+    from flashb import _native
+    from test_longform_cpu import desc
+    L, p = _native.lib(), 1 << 24
+    far = dict(k=1 << 30, v=1 << 31)
+    far4 = dict(bits=4, ks=1 << 32, vs=1 << 33, **far)
+
+    def store(d):
+        return L.flashb_kv4_store(ctypes.byref(d), p, 1024, 512, 128, p, 1024, 512, 128, p, 0, 4, None)
+    for bad in (dict(k_sb=0), dict(v_sh=0), dict(ks_sb=0), dict(vs_sh=0), dict(k_sb=64 * 32), dict(v=1 << 30), dict(vs=1 << 32),
+                dict(k_sp=128)):
+        assert store(desc(**{**far4, **bad})) == _native.FB_ERR_ARG and 'share memory' in _native.last_error(), bad
+        assert evict(desc(bits=4), desc(**{**far4, **bad})) == _native.FB_ERR_ARG, bad
+    for bad in (dict(k_sb=0), dict(v_sh=0), dict(v=1 << 30), dict(k=(1 << 31) + 256 * 255), dict(k_sb=128 * 64)):
+        assert evict(desc(), desc(**{**far, **bad})) == _native.FB_ERR_ARG and 'share memory' in _native.last_error(), bad
+    acc = 1 << 28
+
+    def sums(sb, sh, out=acc):
+        return L.flashb_long_decode(ctypes.byref(desc()), p, 1024, 128, 8, p, None, 0, 0, 1.0, acc, sb, sh, out, sb, sh, 1.0,
+                                    None, 0, 1 << 27, None)
+    for sb, sh in ((0, 64), (128, 0), (64, 64), (128, 63)):
+        for out in (acc, 1 << 29):
+            assert sums(sb, sh, out) == _native.FB_ERR_ARG and 'acc_out' in _native.last_error()
+
+    def prefill(sb, sl, sh):
+        return L.flashb_long_prefill(p, 16 * 1024, 2048, 128, p, 16 * 256, 2048, 128, p, 16 * 256, 2048, 128, 2, 8, 2, 16, 16, 0,
+                                     None, 0, 0, 1.0, 1 << 27, sb, sl, sh, None)
+    for st in ((16 * 1024, 128, 128), (16 * 1024, 64, 2048), (8 * 1024, 1024, 128)):
+        assert prefill(*st) == _native.FB_ERR_ARG and 'share memory' in _native.last_error()
