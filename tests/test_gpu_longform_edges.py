@@ -61,3 +61,22 @@ def test_evict_between_views_that_share_no_memory(bits):
             x = x.double() if bits == 16 else ref.quantise(x)
             assert torch.equal(got[:, :, :keep].cpu().double(), torch.gather(x, 2, at[..., None].expand(-1, -1, -1, 128)))
         assert torch.equal(moved[..., :keep].cpu(), torch.gather(acc, 2, at)) and (moved[..., keep:] == 0).all()
+
+
+@pytest.mark.parametrize('std', [2.0 ** -40, 2.0 ** -100])
+@pytest.mark.parametrize('scaling', [0.0, 1e-30, -1e-30])
+@pytest.mark.parametrize('bits', [16, 4])
+@pytest.mark.parametrize('B', [1, 70])
+def test_decode_scores_too_small_for_fp32(std, scaling, bits, B):
+    """A scale that underflows gives every visible slot the same weight, and those past the length none."""
+    NH, NKV, S = 8, 2, 150
+    q, k, v = randn((B, NH, 1, 128), 4, std), randn((B, NKV, S, 128), 5), randn((B, NKV, S, 128), 6)
+    lengths = rows([S - 1 - b % 9 for b in range(B)])
+    if bits == 4:
+        cache, k, v = four(k, v)
+    else:
+        cache = lf().KVCache(k.cuda(), v.cuda())
+    acc = torch.zeros(B, NKV, S, device='cuda')
+    out, wt, tol = ref.decode(q, k, v, lengths, None, None, 0, scaling)
+    ref.assert_within(lf().decode(q.cuda(), cache, lengths.cuda(), scaling=scaling, acc=acc), out, tol)
+    ref.assert_within(acc, wt, 2.0 ** -18 * wt)
