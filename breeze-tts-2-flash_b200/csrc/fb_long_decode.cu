@@ -318,9 +318,10 @@ __device__ __forceinline__ void long_piece(const LongDecodeArgs& a, int b, int h
         qf[2 * i + 1][1] = pack_h2(f[6] * down, f[7] * down);
       }
       const float up = __uint_as_float((uint32_t)(127 + ex) << 23);
-      // head 2t lives in lanes 4 (2t) ..; not 0: a masked score stays -inf
-      scA = fmaxf(a.scale * __shfl_sync(FULL, up, 8 * t), FLT_MIN);
-      scB = fmaxf(a.scale * __shfl_sync(FULL, up, 8 * t + 4), FLT_MIN);
+      scA = a.scale * __shfl_sync(FULL, up, 8 * t);          // head 2t lives in lanes 4 (2t) ..
+      scB = a.scale * __shfl_sync(FULL, up, 8 * t + 4);
+      if (scA == 0.f) scA = FLT_MIN;                         // a masked score stays -inf
+      if (scB == 0.f) scB = FLT_MIN;
     }
   }
 

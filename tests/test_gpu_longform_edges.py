@@ -80,3 +80,13 @@ def test_decode_scores_too_small_for_fp32(std, scaling, bits, B):
     out, wt, tol = ref.decode(q, k, v, lengths, None, None, 0, scaling)
     ref.assert_within(lf().decode(q.cuda(), cache, lengths.cuda(), scaling=scaling, acc=acc), out, tol)
     ref.assert_within(acc, wt, 2.0 ** -18 * wt)
+
+
+@pytest.mark.parametrize('bits', [16, 4])
+@pytest.mark.parametrize('B', [1, 70])
+def test_decode_shows_a_nan_scaling(bits, B):
+    q, k, v = randn((B, 8, 1, 128), 4), randn((B, 2, 150, 128), 5), randn((B, 2, 150, 128), 6)
+    cache = four(k, v)[0] if bits == 4 else lf().KVCache(k.cuda(), v.cuda())
+    lengths = rows([149 if b else 0 for b in range(B)][::-1])
+    got = lf().decode(q.cuda(), cache, lengths.cuda(), scaling=float('nan')).cpu()
+    assert torch.isnan(got[:B - 1]).all() and (got[B - 1] == 0).all()
