@@ -65,7 +65,7 @@ struct LongDecodeArgs {
   float v_scale;
   const float* acc;
   float* acc_out;
-  float decay;
+  float decay, shift;                   // shift: LongTile's SHIFT
   long long acc_sb, acc_sh, acco_sb, acco_sh;
   float* po;                            // pieces: unnormalised out [slot][G][128],
   float2* ml;                           //   maximum and sum [slot][G]
@@ -83,7 +83,10 @@ struct LongTile {
   static constexpr int KEYS = BITS == 16 ? 16 : 32;      // keys per warp and step
   static constexpr int CHUNK = KEYS * LD_WARPS;
   static constexpr int EXTRA = 1;                        // empty chunks before a row's own (see LongPlace)
-  static constexpr float SHIFT = BITS == 16 ? 0.f : 6.f; // P x 2^6 in fp16: with the 2^8 of slack below its 65504
+  // P x 2^SHIFT.  fp16: 2^6, with the 2^8 of slack below its 65504.  bf16: 2^-24, so that the unnormalised sums of 2^16 keys
+  // stay in fp32's range for every finite V (from 0 on they left it past 1e34); what falls below the range instead is 2^-125
+  // of the output at most, a bf16 step at its smallest normal values.
+  static constexpr float SHIFT = BITS == 16 ? -24.f : 6.f;
 };
 
 __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -634,8 +637,8 @@ __global__ void __launch_bounds__(LD_THREADS, LongTile<BITS>::CTAS) long_cluster
         const float m = *cluster.map_shared_rank(&c_m[tid], c);
         if (m > -INFINITY) L += ex2(m - M) * *cluster.map_shared_rank(&c_l[tid], c);
       }
-      s_max[tid] = M;
-      s_inv[tid] = 1.f / L;
+      s_max[tid] = M + T::SHIFT;                         // scores near the maximum: a difference near 0 keeps its bits
+      s_inv[tid] = ex2(T::SHIFT) / L;
     }
     __syncthreads();
     const float* ap = a.acc + b * a.acc_sb + h * a.acc_sh;
@@ -689,8 +692,8 @@ __device__ __forceinline__ void long_weights(const LongDecodeArgs& a, const Long
         float M, L;
         stats(gg, M, L);
         if (lane == 0) {
-          s_m[gg] = M;
-          s_inv[gg] = 1.f / L;                   // not used for a row without a visible slot
+          s_m[gg] = M + a.shift;                 // scores near the maximum: a difference near 0 keeps its bits
+          s_inv[gg] = ex2(a.shift) / L;          // not used for a row without a visible slot
         }
       }
       __syncthreads();
@@ -1070,6 +1073,7 @@ extern "C" int flashb_long_decode(const fb_kv_cache* cache, const void* q, int64
   a.flip = scaling < 0.f ? 0x80008000u : 0u;
   a.dense = a.c.k_sp == (four ? 64 : 256) && a.c.v_sp == a.c.k_sp && (!four || (a.c.ks_sp == 8 && a.c.vs_sp == 8));
   a.v_scale = four ? cache->v_scale : 1.f;
+  a.shift = four ? LongTile<4>::SHIFT : LongTile<16>::SHIFT;
   a.acc = acc, a.acc_out = acc_out, a.decay = decay;
   a.acc_sb = acc_sb, a.acc_sh = acc_sh, a.acco_sb = acco_sb, a.acco_sh = acco_sh;
   a.po = ws, a.ml = (float2*)(ws + p.off_ml), a.own = (int2*)(ws + p.off_own), a.sc = ws + p.off_s;

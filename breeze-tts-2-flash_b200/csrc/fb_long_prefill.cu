@@ -47,6 +47,8 @@ constexpr int LP_KV = LP_TILE * LG_D * 2;         // ... of a K or V tile
 constexpr int LP_SMEM = LP_Q + 4 * LP_KV + 1024;  // Q, K and V twice, at a 1024-byte boundary
 constexpr uint32_t LP_COLS = 256;                 // TMEM: S in columns 0-63, P twice in 64-127, O in 128-255
 constexpr float LP_SLACK = 8.f;
+// P x 2^-24: the unnormalised sums of 2^16 keys stay in fp32's range for every finite V
+constexpr float LP_SHIFT = -24.f;
 
 struct alignas(64) LongPrefillArgs {
   CUtensorMap tq, to, tk, tv, tk32, tv32;         // Q and out tiles; K, V: boxes of 64 and of 32 slots
@@ -148,7 +150,7 @@ __device__ __noinline__ void long_row_again(const LongPrefillArgs& a, int b, int
     const uint2 kw = *reinterpret_cast<const uint2*>(kb + j * a.k_sl), vw = *reinterpret_cast<const uint2*>(vb + j * a.v_sl);
     const float s = a.scale * warp_sum(lo_f(qw.x) * lo_f(kw.x) + hi_f(qw.x) * hi_f(kw.x) + lo_f(qw.y) * lo_f(kw.y) +
                                        hi_f(qw.y) * hi_f(kw.y));
-    const float mn = fmaxf(m, s), f = m > -INFINITY ? ex2(m - mn) : 0.f, w = mn > -INFINITY ? ex2(s - mn) : (s == -INFINITY ? 0.f : s);
+    const float mn = fmaxf(m, s), f = m > -INFINITY ? ex2(m - mn) : 0.f, w = mn > -INFINITY ? ex2(s - mn + LP_SHIFT) : (s == -INFINITY ? 0.f : s);
     m = mn;
     sum = sum * f + w;
     o[0] = o[0] * f + w * lo_f(vw.x);
@@ -379,7 +381,7 @@ __global__ void __launch_bounds__(LP_THREADS, 2) long_prefill_kernel(const __gri
       }
       // P's buffer: free once P V of t - 2 is done (asked here, needed after the exponentials)
       const bool free = t < 2 || mbar_test(&bar_o[t & 1], ((t - 2) >> 1) & 1);
-      const float off = m > -INFINITY ? -m : 0.f;
+      const float off = m > -INFINITY ? LP_SHIFT - m : 0.f;
       const uint64_t off2 = f2(off, off);
       uint32_t w[32];
 #pragma unroll

@@ -90,3 +90,48 @@ def test_decode_shows_a_nan_scaling(bits, B):
     lengths = rows([149 if b else 0 for b in range(B)][::-1])
     got = lf().decode(q.cuda(), cache, lengths.cuda(), scaling=float('nan')).cpu()
     assert torch.isnan(got[:B - 1]).all() and (got[B - 1] == 0).all()
+
+
+def large(shape, seed):
+    """Values of one sign up to bf16's largest: their plain sum passes fp32's range, their mean does not."""
+    g = torch.Generator().manual_seed(seed)
+    return ((0.5 + 0.5 * torch.rand(shape, generator=g)) * 3.3e38).to(torch.bfloat16)
+
+
+@pytest.mark.parametrize('B,S', [(1, 300), (1, 9000), (64, 300), (40, 1100)])
+@pytest.mark.parametrize('heads', [(8, 2), (8, 8), (16, 2)])
+def test_decode_values_up_to_the_largest(B, S, heads):
+    NH, NKV = heads
+    q, k, v = randn((B, NH, 1, 128), 7), randn((B, NKV, S, 128), 8), large((B, NKV, S, 128), 9)
+    lengths = rows([S - b % 5 for b in range(B)])
+    out, wt, tol = ref.decode(q, k, v, lengths, None, None, 0, SC)
+    acc = torch.zeros(B, NKV, S, device='cuda')
+    ref.assert_within(lf().decode(q.cuda(), lf().KVCache(k.cuda(), v.cuda()), lengths.cuda(), acc=acc), out, tol)
+    ref.assert_within(acc, wt, 2.0 ** -18 * wt)
+
+
+@pytest.mark.parametrize('odd', [False, True])
+def test_prefill_values_up_to_the_largest(odd):
+    """odd: a later slot's NaN has the rows before it computed again."""
+    NH, NKV, L = 8, 2, 200
+    q, k, v = randn((1, NH, L, 128), 10), randn((1, NKV, L, 128), 11), large((1, NKV, L, 128), 12)
+    out, tol = ref.prefill(q, k, v, 0, None, None, 0, SC)
+    n = L
+    if odd:
+        n = L - 1
+        v[:, :, n] = float('nan')
+    got = lf().prefill(q.cuda(), k.cuda(), v.cuda()).cpu()
+    ref.assert_within(got[:, :n], out[:, :n], tol[:, :n])
+    assert torch.isnan(got[:, n:]).all()
+
+
+@pytest.mark.parametrize('e', [-60, -100])
+def test_values_far_below_one(e):
+    """Down to 2^-100 values keep their relative precision: the bounds without their absolute part."""
+    NH, NKV, S = 8, 2, 150
+    q, k, v = randn((1, NH, S, 128), 13), randn((1, NKV, S, 128), 14), randn((1, NKV, S, 128), 15) * 2.0 ** e
+    out, tol = ref.prefill(q, k, v, 0, None, None, 0, SC)
+    ref.assert_within(lf().prefill(q.cuda(), k.cuda(), v.cuda()), out, tol - 1e-30 + 2.0 ** -125)
+    out, _, tol = ref.decode(q[:, :, -1:], k, v, rows([S]), None, None, 0, SC)
+    got = lf().decode(q[:, :, -1:].cuda(), lf().KVCache(k.cuda(), v.cuda()), rows([S]).cuda())
+    ref.assert_within(got, out, tol - 1e-30 + 2.0 ** -125)
