@@ -82,6 +82,12 @@ class LongSpeech:
         self.zero = torch.zeros(1, dtype=torch.int64, device=dev)
         self.new_k, self.new_v = (torch.empty(B, self.NKV, 1, 128, dtype=torch.bfloat16, device=dev) for _ in range(2))
 
+    def reset(self):
+        """Empty caches for another reading; nothing is allocated."""
+        for t in (self.lengths, self.starts, *(self.acc or ())):
+            t.zero_()
+        self.used = self.next = 0
+
     def _put(self, cache, k, v, slots):
         """k / v [B, NKV, L, 128] to slots [B, L]."""
         if cache.bits == 4:
@@ -118,7 +124,7 @@ class LongSpeech:
 
     def prefill(self, inputs_embeds, starts=None):
         """The prompt [B, L, H] bf16 (row b's tokens from ``starts[b]`` on, clamped to 0 .. L; positions count from there)
-        into empty caches.  Returns the hidden states [B, L, H] after the final norm."""
+        into empty caches (a first reading's, or after ``reset``).  Returns the hidden states [B, L, H] after the final norm."""
         fx, st = kernels.fused(), self.st
         B, L, H = inputs_embeds.shape
         if L > self.slots or self.used:

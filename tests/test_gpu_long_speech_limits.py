@@ -98,3 +98,30 @@ def test_starts_outside_the_prompt_are_clamped():
             h.input_ids_buf.copy_(ids)
             s.step()
         assert torch.equal(g2.hidden_buf, g.hidden_buf) and torch.equal(g2.position_ids, g.position_ids)
+
+
+@pytest.mark.parametrize('four_bits', [False, True])
+def test_a_second_reading_is_like_a_first(four_bits):
+    """After ``reset``, the same bits as from caches made anew, evictions among them."""
+    from flashb._native import FlashbError
+    from flashb.long_speech import LongSpeech
+    kw = dict(slots=40, keep=24, sinks=2, window=30, four_bits=four_bits)
+    cfg, g, g2, used = _pair(2, 70, **kw)
+    used.prefill(_prompt(cfg, 2, 30, seed=12), torch.tensor([7, 0], device='cuda'))
+    for ids in _ids(cfg, 2, 35):
+        g2.input_ids_buf.copy_(ids)
+        used.step()
+    with pytest.raises(FlashbError):
+        used.prefill(_prompt(cfg, 2, 20))
+    used.reset()
+    new = LongSpeech(g, **kw)
+    x = _prompt(cfg, 2, 20)
+    assert torch.equal(used.prefill(x), new.prefill(x))
+    for ids in _ids(cfg, 2, 51):
+        for h, s in ((g2, used), (g, new)):
+            h.input_ids_buf.copy_(ids)
+            s.step()
+        assert torch.equal(g2.hidden_buf, g.hidden_buf) and torch.equal(g2.cfg_logits_buf, g.cfg_logits_buf)
+    for s in (used, new):                                          # the table's end counts from the new beginning
+        with pytest.raises(FlashbError):
+            s.step()
