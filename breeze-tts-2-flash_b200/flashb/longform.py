@@ -132,7 +132,7 @@ class KV4Cache(KVCache):
         if _current() != self.index:
             with _on(self.index):
                 return self.store(k, v, slots)
-        L = slots.shape[-1]
+        L = slots.shape[-1] if slots.dim() else -1
         if not self._heads(k, L) or not self._heads(v, L):
             _refuse('k, v: [B, NKV, L, 128] bf16 on the cache\'s device, L as in slots')
         sb = self._slots(slots, L)
@@ -148,7 +148,7 @@ class KV4Cache(KVCache):
         if _current() != self.index:
             with _on(self.index):
                 return self.read(slots)
-        L = slots.shape[-1]
+        L = slots.shape[-1] if slots.dim() else -1
         sb = self._slots(slots, L)
         k = torch.empty(self.B, self.NKV, L, D, dtype=_BF16, device=self.device)
         v = torch.empty_like(k)
@@ -262,7 +262,7 @@ def prefill(query, key, value, *, window=None, sinks=0, starts=None, q_start=Non
             return prefill(query, key, value, window=window, sinks=sinks, starts=starts, q_start=q_start,
                            scaling=scaling, out=out)
     dev = query.device
-    B, NH, L = query.shape[:3]
+    B, NH, L = query.shape[:3] if query.dim() == 4 else (0, 0, 0)
     if not query.is_cuda or not (_bf16_heads(query, B, dev) and _bf16_heads(key, B, dev) and _bf16_heads(value, B, dev)):
         _refuse('query, key, value: [B, heads, slots, 128] bf16 on one CUDA device')
     NKV, S = key.shape[1], key.shape[2]

@@ -170,3 +170,24 @@ def test_outputs_that_overlap_themselves_are_refused():
                                      None, 0, 0, 1.0, 1 << 27, sb, sl, sh, None)
     for st in ((16 * 1024, 128, 128), (16 * 1024, 64, 2048), (8 * 1024, 1024, 128)):
         assert prefill(*st) == _native.FB_ERR_ARG and 'share memory' in _native.last_error()
+
+
+def test_tensors_of_another_rank_are_refused(monkeypatch):
+    """As bad shapes are, with FlashbError."""
+    from flashb import longform as lf
+    from flashb._native import FB_ERR_ARG, FlashbError
+    monkeypatch.setattr(lf, '_current', lambda: 1)
+    z = lambda *s, dt=torch.bfloat16: torch.zeros(*s, dtype=dt).as_subclass(OnDevice1)  # noqa: E731
+    u8 = lambda w: z(2, 2, 16, w, dt=torch.uint8)  # noqa: E731
+    k, c4, n = z(2, 2, 16, 128), lf.KV4Cache(u8(64), u8(8), u8(64), u8(8)), z(2, dt=torch.int64)
+    cache, acc = lf.KVCache(k, k), z(2, 2, 16, dt=torch.float32)
+    none = z((), dt=torch.int64)
+    for f in (lambda: lf.prefill(z(16, 128), k, k), lambda: lf.prefill(z(()), k, k), lambda: lf.prefill(z(1, 2, 2, 16, 128), k, k),
+              lambda: lf.prefill(z(2, 4, 16, 128), z(16, 128), z(16, 128)), lambda: lf.decode(z(2, 512), cache, n),
+              lambda: lf.decode(z(2, 4, 1, 128), cache, none), lambda: lf.decode(z(2, 4, 1, 128), cache, n, acc=none),
+              lambda: c4.store(k, k, none), lambda: c4.read(none), lambda: c4.store(z(16, 128), z(16, 128), z(16, dt=torch.int64)),
+              lambda: lf.evict(cache, none, n, 4, into=cache), lambda: lf.KVCache(z(16, 128), z(16, 128)),
+              lambda: lf.KV4Cache(none, none, none, none)):
+        with pytest.raises(FlashbError) as e:
+            f()
+        assert e.value.rc == FB_ERR_ARG
