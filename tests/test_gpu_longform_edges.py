@@ -135,3 +135,118 @@ def test_values_far_below_one(e):
     out, _, tol = ref.decode(q[:, :, -1:], k, v, rows([S]), None, None, 0, SC)
     got = lf().decode(q[:, :, -1:].cuda(), lf().KVCache(k.cuda(), v.cuda()), rows([S]).cuda())
     ref.assert_within(got, out, tol - 1e-30 + 2.0 ** -125)
+
+
+@pytest.mark.parametrize('std', [30.0, 300.0])
+@pytest.mark.parametrize('window', [None, 150])
+def test_prefill_scores_of_any_size(std, window):
+    """Nearly one-hot rows whose maximum rises from tile to tile: the sums so far are scaled down again and again."""
+    NH, NKV, L = 8, 2, 400
+    q, k, v = randn((1, NH, L, 128), 16, std), randn((1, NKV, L, 128), 17), randn((1, NKV, L, 128), 18)
+    k = (k.float() * torch.linspace(0.02, 1.0, L)[None, None, :, None]).to(torch.bfloat16)
+    out, tol = ref.prefill(q, k, v, 0, None, window, 3, SC)
+    # a score is off by at most 2^-21 sum |q k| scaling < 2^-21 x 2^11 at std 300
+    got = lf().prefill(q.cuda(), k.cuda(), v.cuda(), window=window, sinks=3)
+    ref.assert_within(got, out, tol + 2.0 ** -9 * std / 300 * v.double().abs().max())
+
+
+@pytest.mark.parametrize('heads,L,window,sinks', [((16, 4), 1500, None, 0), ((16, 4), 1500, 700, 70), ((8, 8), 1300, 1024, 4),
+                                                  ((16, 2), 900, 333, 33)])
+def test_prefill_of_many_tiles(heads, L, window, sinks):
+    NH, NKV = heads
+    q, k, v = randn((1, NH, L, 128), 19), randn((1, NKV, L, 128), 20), randn((1, NKV, L, 128), 21)
+    out, tol = ref.prefill(q, k, v, 0, rows([5]), window, sinks, SC)
+    got = lf().prefill(q.cuda(), k.cuda(), v.cuda(), window=window, sinks=sinks, starts=torch.tensor([5], device='cuda'))
+    ref.assert_within(got, out, tol)
+
+
+@pytest.mark.parametrize('B,NKV,S,keep,sinks,recent', [(1, 2, 13000, 5000, 4, 100), (2, 1, 12000, 64, 0, 0),
+                                                       (40, 8, 700, 333, 4, 50), (300, 2, 260, 100, 1, 0)])
+@pytest.mark.parametrize('bits', [16, 4])
+@pytest.mark.parametrize('ties', [False, True])
+def test_evict_long_rows_and_many(B, NKV, S, keep, sinks, recent, bits, ties):
+    """Rows whose keys do not fit the shared memory, and more rows than CTAs fit the GPU."""
+    L = lf()
+    g = torch.Generator().manual_seed(22)
+    acc = torch.rand(B, NKV, S, generator=g).pow(4)
+    if ties:
+        acc = (acc * 6).floor() / 4
+    lengths = torch.randint(S // 2, S + 1, (B,), generator=g)
+    lengths[0] = S
+    starts = torch.randint(0, 5, (B,), generator=g)
+    k, v = randn((B, NKV, S, 128), 23).cuda(), randn((B, NKV, S, 128), 24).cuda()
+    if bits == 4:
+        src, dst = L.KV4Cache.empty(B, NKV, S), L.KV4Cache.empty(B, NKV, keep)
+        src.store(k, v, torch.arange(S, device='cuda'))
+        k, v = src.read(torch.arange(S, device='cuda'))
+    else:
+        src = L.KVCache(k, v)
+        dst = L.KVCache(*(torch.zeros(B, NKV, keep, 128, dtype=torch.bfloat16, device='cuda') for _ in range(2)))
+    kept, n, moved = L.evict(src, acc.cuda(), lengths.cuda(), keep, into=dst, starts=starts.cuda(), sinks=sinks,
+                             recent=recent)
+    want, n_want = ref.evict(acc, lengths, starts, keep, sinks, recent)
+    assert torch.equal(kept.cpu(), want) and torch.equal(n.cpu(), n_want)
+    gk, gv = dst.read(torch.arange(keep, device='cuda')) if bits == 4 else (dst.keys, dst.values)
+    ok, idx = (want >= 0).cuda(), want.clamp(min=0).long().cuda()
+    for got, x in ((gk, k), (gv, v)):
+        assert torch.equal(got, torch.gather(x, 2, idx[..., None].expand(-1, -1, -1, 128)) * ok[..., None])
+    assert torch.equal(moved, torch.gather(acc.cuda(), 2, idx) * ok)
+
+
+def test_every_call_in_a_graph_follows_the_device():
+    """Prefill, store, read, decode over 4 bits and eviction captured once; the inputs change between replays."""
+    L = lf()
+    B, NH, NKV, S, n = 2, 8, 2, 160, 50
+    q, k, v = randn((B, NH, n, 128), 25).cuda(), randn((B, NKV, n, 128), 26).cuda(), randn((B, NKV, n, 128), 27).cuda()
+    starts, lengths = torch.zeros(B, dtype=torch.int64, device='cuda'), torch.tensor([n, n], device='cuda')
+    slots = torch.arange(n, device='cuda')
+    src, dst = L.KV4Cache.empty(B, NKV, S), L.KV4Cache.empty(B, NKV, S)
+    acc = torch.zeros(B, NKV, S, device='cuda')
+
+    def run():
+        src.store(k, v, slots)
+        kk, vv = src.read(slots)
+        a = L.prefill(q, kk, vv, window=20, sinks=2, starts=starts)
+        o = L.decode(q[:, :, -1:], src, lengths, starts=starts, window=20, sinks=2, acc=acc)
+        return a, o, L.evict(src, acc, lengths, 30, into=dst, starts=starts, sinks=2, recent=4)
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a, o, (kept, m, _) = run()
+    for seed, st, off in ((28, [0, 9], 0), (29, [30, 2], 7)):
+        for x, y in ((q, randn(q.shape, seed)), (k, randn(k.shape, seed + 10)), (v, randn(v.shape, seed + 20))):
+            x.copy_(y)
+        slots.copy_(torch.arange(n) + off)
+        starts.copy_(torch.tensor(st) + off)
+        lengths.fill_(n + off)
+        acc.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        k4, v4 = ref.quantise(k.cpu()), ref.quantise(v.cpu())
+        # the prefill has the read keys at slots 0 .., its rows begin off slots later there
+        want, tol = ref.prefill(q.cpu(), k4, v4, 0, torch.tensor(st) + off, 20, 2, SC)
+        ref.assert_within(a, want, tol)
+        want, wt, tol = ref.decode(q[:, :, -1:].cpu(), k4, v4, rows([n, n]), torch.tensor(st), 20, 2, SC)
+        ref.assert_within(o, want, tol)
+        ref.assert_within(acc[:, :, off:n + off], wt, 2.0 ** -18 * wt + 1e-30)
+        want, n_want = ref.evict(acc.cpu(), [n + off] * B, [s + off for s in st], 30, 2, 4)
+        assert torch.equal(kept.cpu(), want) and torch.equal(m.cpu(), n_want)
+
+
+@pytest.mark.parametrize('bits', [16, 4])
+@pytest.mark.parametrize('B,S', [(1, 3000), (64, 900)])
+def test_the_same_inputs_give_the_same_bits(B, S, bits):
+    L = lf()
+    NH, NKV = 16, 4
+    q, k, v = randn((B, NH, 40, 128), 30).cuda(), randn((B, NKV, S, 128), 31).cuda(), randn((B, NKV, S, 128), 32).cuda()
+    lengths = torch.randint(1, S + 1, (B,), generator=torch.Generator().manual_seed(33)).cuda()
+    cache = four(k.cpu(), v.cpu())[0] if bits == 4 else L.KVCache(k, v)
+    first = None
+    for _ in range(5):
+        acc = torch.zeros(B, NKV, S, device='cuda')
+        got = [L.decode(q[:, :, :1], cache, lengths, window=700, sinks=3), L.decode(q[:, :, :1], cache, lengths, acc=acc), acc]
+        if bits == 16:
+            got.append(L.prefill(q, k, v, window=500, sinks=3))
+        first = got if first is None else first
+        assert all(torch.equal(a, b) for a, b in zip(got, first))
