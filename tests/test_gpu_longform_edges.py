@@ -250,3 +250,29 @@ def test_the_same_inputs_give_the_same_bits(B, S, bits):
             got.append(L.prefill(q, k, v, window=500, sinks=3))
         first = got if first is None else first
         assert all(torch.equal(a, b) for a, b in zip(got, first))
+
+
+@pytest.mark.parametrize('scale', [1.0, 2.0 ** 7])
+def test_kv4_every_scale_against_every_value_that_matters(scale):
+    """Every block maximum's scale, and for each scale every bf16 from its block's maximum down to where codes are 0."""
+    bits = torch.arange(0x0001, 0x7f80, dtype=torch.int32).to(torch.int16)
+    every = bits.view(torch.bfloat16)                       # the positive finite values, in order
+    s = ref.e4m3(every.double() / scale / 6)
+    last = torch.nonzero(torch.cat((s[1:] != s[:-1], torch.tensor([True])))).view(-1)
+    first = torch.cat((torch.zeros(1, dtype=torch.int64), last[:-1] + 1))
+    blocks = []
+    for at in torch.cat((first, last, last[-2:-1] + 500)).tolist():
+        if s[at] == 0:
+            continue
+        below = every[max(0, at - 5 * 128):at + 1]           # five binades: codes 0.25 and less are 1 / 24 of the maximum
+        below = torch.nn.functional.pad(below, (0, -len(below) % 15)).view(-1, 15)
+        blocks.append(torch.cat((every[at].expand(len(below), 1), below), 1))
+    x = torch.cat(blocks)
+    x = torch.cat((x, torch.cat((every, every.new_zeros(-len(every) % 16))).view(-1, 16)))
+    x = torch.where(torch.rand(x.shape, generator=torch.Generator().manual_seed(37)) < 0.5, x, -x)
+    x = torch.nn.functional.pad(x.view(-1), (0, -x.numel() % 128)).view(1, 1, -1, 128)
+    n = x.shape[2]
+    c = lf().KV4Cache.empty(1, 1, n, k_scale=scale, v_scale=1.0)
+    c.store(x.cuda(), x.cuda(), torch.arange(n, device='cuda'))
+    k, v = c.read(torch.arange(n, device='cuda'))
+    assert torch.equal(k.cpu().double(), ref.quantise(x, scale)) and torch.equal(v.cpu().double(), ref.quantise(x))
