@@ -9,8 +9,12 @@
 // integer keys, held in shared memory), counts the slots that stay below each thread's run of slots, and then copies its
 // share of them.  With few rows several CTAs share one: each selects for itself (a few microseconds, and no exchange),
 // and copies its part.  Bound: HBM, the kept rows read and written once (1 KB a slot in bf16).
-// Measured on a B200: 64 rows of up to 8192 slots to 2048 (478 MB) 101 us, 0.72 of the measured copy bandwidth (half the
-// warps copying while the others select took 102); one stream's 1920 slots to 1023 9 us.
+// Measured on a B200: 64 rows of up to 8192 slots to 2048 (478 MB) 99 us, 0.74 of the measured copy bandwidth; the same rows
+// in 4 bits 70 us, 0.31; one stream's 1920 slots to 1023 9 us.  What is lost at many rows: the selection, 17 us (64 slots
+// kept of the same rows), during which memory is idle, and uneven ends (256 CTAs of one ragged row each on 148 SMs: 40 have
+// one CTA, the others two).  The places of the kept slots matter little: adjacent instead of scattered, 98 us for 99 (in 4 bits
+// 62 for 72).  In 4 bits a row is 64 bytes, so 8 of a warp's 32 lanes copy codes, and the scales take a second loop.
+// Half the warps copying while the others select took 102 us for 101 then.
 #include "fb_long.cuh"
 
 namespace fb {

@@ -12,8 +12,8 @@
 // fused multiply-add, and its subtraction, two values an instruction.  max / 6 is rounded to 16 fraction bits in the same
 // way (8 significant bits against the tie's 7).
 //
-// Bound: HBM, 328 bytes a head and token.  Measured on a B200: 8 x 4097 tokens of 4 heads, K and V, 28.5 us stored and read
-// back (0.92 of the measured copy bandwidth; the read finds the codes in L2); a token of 128 rows 3.7 us.  A thread owns a
+// Bound: HBM, 328 bytes a head and token.  Measured on a B200: 8 x 4097 tokens of 4 heads, K and V, 28.2 us stored and read
+// back (0.93 of the measured copy bandwidth; the read finds the codes in L2); a token of 128 rows 3.7 us.  A thread owns a
 // block (two 16-byte loads, 8 bytes of codes, one scale), so the block's maximum, scale and reciprocal are its own; the
 // maximum is taken on the bf16 bit patterns, two at a time, where a NaN or an infinity shows as the largest.
 #include "fb_long.cuh"

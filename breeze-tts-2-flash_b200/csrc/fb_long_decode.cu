@@ -4,14 +4,16 @@
 //   s_j = scaling (q . k_j),  p = softmax(s) over the visible slots,  out = sum_j p_j v_j        (0 without any)
 //   acc_out[j] = decay acc[j] + sum over the q heads of the group of p_j   (every slot; p_j = 0 where not visible)
 //
-// Measured on a B200: 128 rows of 4 KV heads over a window of 2048 (404 MB) 68 us, 0.91 of the measured copy bandwidth; 64
-// ragged rows of up to 8192 slots in 4 bits (152 MB) 39 us, 0.60 (bound by instruction issue: 590 a warp and 32 keys, half
-// of them conversions, scalings and MMAs); weights wanted, up to 4096 slots (277 MB), 51 to 54 us, 0.80; one stream over
-// some hundred keys 5 to 8 us.  K and V through rings of cp.async in shared memory instead of straight to registers took
-// 85 us at the first of these.
+// Measured on a B200 (in a CUDA graph): 128 rows of 4 KV heads over a window of 2048 (404 MB) 66 us, 0.94 of the measured
+// copy bandwidth; 64 ragged rows of up to 8192 slots in 4 bits (152 MB) 36 to 38 us, 0.60 to 0.64; weights wanted, up to
+// 4096 slots (277 MB), 51 to 54 us, 0.80; one stream over some hundred keys 5 to 8 us.  K and V through rings of cp.async in
+// shared memory instead of straight to registers took 85 us at the first of these.
 //
-// Bound: the visible K and V are read once (512 bytes a key and KV head in bf16, 144 in 4 bits) and do 4 G flops per
-// value, so HBM bounds it; below some megabytes the launch and one memory round trip do.
+// Bound: the visible K and V are read once (512 bytes a key and KV head in bf16, 144 in 4 bits) and do 2 G flops per
+// value, so HBM bounds bf16; below some megabytes the launch and one memory round trip do.  In 4 bits nothing is saturated:
+// DRAM at 46% of its nominal rate, issue slots at 54%, the ALU pipe at 46%.  A warp runs 590 instructions on 32 keys, waits
+// for its own loads 38% of the time (128 registers a thread leave no room for the next tile's) and shares its scheduler
+// with three others; a sixth of the (profiled) launch is its beginning and end.
 //
 // Few short rows: long_cluster_kernel, one launch (below).  Else two launches.  long_decode_kernel: the visible keys of
 // every (row, KV head), in chunks, form one list; CTA c of N takes the c-th N-th of it whatever the rows' lengths are, so

@@ -18,20 +18,24 @@
 // columns each).  The running maximum moves only when a tile's exceeds it by 2^8 (the sums are exact either way), so O is
 // hardly ever rescaled.  Masks are applied to the segments that need one for some row of the CTA.
 //
-// Measured on a B200: 8192 tokens, 16 heads over 4, window 1024: 81 us, 795 TFLOP/s; windows of 512 and 2048 55 and 123 us,
-// so about 1150 TFLOP/s and 25 us that do not grow with the window (beginning and ending 3.5 waves of CTAs).  What bounds
-// it is the chain of one softmax warp (wait, TMEM read, maximum, exponentials, TMEM write; about 1700 cycles a tile, two
-// CTAs side by side): with three quarters of P V, seven eighths of S, the exponential unit's share or the copies' traffic
-// left out, the time moved by 5% at most.  Tried, against 83 us then: P over S's columns with S twice (88 us: S waits for P V),
+// Measured on a B200: 8192 tokens, 16 heads over 4, window 1024: 80 us in a CUDA graph, 808 TFLOP/s, and 90 us a call among
+// others (717; clocks fall under the sustained load); windows of 512 and 2048 55 and 123 us, so about 1150 TFLOP/s and 25 us
+// that do not grow with the window (beginning and ending 3.5 waves of CTAs).  What bounds it is the chain of one softmax
+// warp (wait, TMEM read, maximum, exponentials, TMEM write; about 1700 cycles a tile, two CTAs side by side): with three
+// quarters of P V, seven eighths of S, the exponential unit's share or the copies' traffic left out, the time moved by 5%
+// at most.  Tried, against 83 us then: P over S's columns with S twice (88 us: S waits for P V),
 // two threads per row (93), alternate tiles to two groups of warps (93 to 132), one warp issuing everything (113), CTAs
 // that go on to further units (85, and 301 instead of 257 us with a causal mask alone), part of the exponentials as
 // polynomials on the FMA pipe (98 to 106), 128-key tiles with S and P V in turn (127).
 //
-// Rounding: fp32 scores, statistics and sums; P goes to bf16, the type of V's operand, unnormalised.
+// Rounding: fp32 scores, statistics and sums; P goes to bf16, the type of V's operand, unnormalised: one part, where the
+// decode takes two.  Its error against 64 bits (relative, root mean square) is 2.0e-3 to 2.1e-3 at 197 and 8192 tokens where
+// fp32 weights have 1.6e-3, the output's own rounding.  A second part would double P V and P's TMEM columns.
 //
 // A slot that a row does not see gets weight 0, and 0 times an infinity or a NaN in V is NaN.  Slots past the tokens
 // read as zeros (the tensor maps end there), sink segments are zeroed past the sinks; what is left are slots that other
-// rows of the CTA see.  So a row whose output is not finite is computed again, one visible key at a time.
+// rows of the CTA see.  So a row whose output is not finite is computed again, one visible key at a time
+// (a token before its row's start sees none and gives 0).
 #include <type_traits>
 
 #include "fb_long.cuh"
@@ -150,7 +154,8 @@ __device__ __noinline__ void long_row_again(const LongPrefillArgs& a, int b, int
     const uint2 kw = *reinterpret_cast<const uint2*>(kb + j * a.k_sl), vw = *reinterpret_cast<const uint2*>(vb + j * a.v_sl);
     const float s = a.scale * warp_sum(lo_f(qw.x) * lo_f(kw.x) + hi_f(qw.x) * hi_f(kw.x) + lo_f(qw.y) * lo_f(kw.y) +
                                        hi_f(qw.y) * hi_f(kw.y));
-    const float mn = fmaxf(m, s), f = m > -INFINITY ? ex2(m - mn) : 0.f, w = mn > -INFINITY ? ex2(s - mn + LP_SHIFT) : (s == -INFINITY ? 0.f : s);
+    const float mn = fmaxf(m, s), f = m > -INFINITY ? ex2(m - mn) : 0.f;
+    const float w = mn > -INFINITY ? ex2(s - mn + LP_SHIFT) : (s == -INFINITY ? 0.f : s);
     m = mn;
     sum = sum * f + w;
     o[0] = o[0] * f + w * lo_f(vw.x);

@@ -13,8 +13,9 @@ attention weight, in any combination.
 ``max_seq_len`` that its other uses need, and the reading's length to ``positions``: a rotary table of that many entries
 (512 bytes each, all that grows with the reading; None: the graph's table, ``max_seq_len`` + 1).  Keys enter the cache
 after their rotary embedding, so their slot may change while their position stays; a reading that reaches the end of the
-table raises.  With ``keep`` the caches are evicted to that many slots when they are full, each layer by its own weights; without
-it a full cache raises.
+table raises.  With ``keep`` the caches are evicted to that many slots when they are full, each layer by its own weights
+(those of the decode steps: the prompt's slots begin at 0); without it a full cache raises.  ``reset`` empties them for
+another reading.
 
     python -m flashb.long_speech --frames 200 --slots 256 --four-bits --window 128 --keep 192
 """
@@ -124,7 +125,8 @@ class LongSpeech:
 
     def prefill(self, inputs_embeds, starts=None):
         """The prompt [B, L, H] bf16 (row b's tokens from ``starts[b]`` on, clamped to 0 .. L; positions count from there)
-        into empty caches (a first reading's, or after ``reset``).  Returns the hidden states [B, L, H] after the final norm."""
+        into empty caches (a first reading's, or after ``reset``).  Returns the hidden states [B, L, H] after the final
+        norm."""
         fx, st = kernels.fused(), self.st
         B, L, H = inputs_embeds.shape
         if L > self.slots or self.used:

@@ -12,10 +12,13 @@ Row b of a cache holds its keys in slots [starts[b], lengths[b]) (int64 tensors 
 left padding of the prompt), so every call is graph-capturable and needs no host read.  The token at slot p sees slot j
 when starts[b] <= j <= p and (j > p - window or j < starts[b] + sinks); the output without a visible slot is 0.  Slots
 that are not visible may hold anything, NaN included.  bf16 queries, head_dim 128, GQA groups of 1, 2, 4 or 8; fp32
-scores, softmax and sums, rounded to bf16 once.  No reference counterpart: the reference's cache holds the whole
-sequence in bf16 (``flash/backbone.py``).
+scores, softmax statistics and sums.  The weights enter the product with V as two bf16 parts (``decode``, bf16 cache: the
+error of fp32 weights), in fp16 (``decode``, 4 bits: 1 % more) or as one bf16 part (``prefill``: 1.3 times).  Outputs may not
+share memory with inputs or themselves (``acc`` in place is the exception).  No reference counterpart: the reference's
+cache holds the whole sequence in bf16 (``flash/backbone.py``).
 
-Calls run on the current stream of the cache's device (``prefill``: of the query's), whichever device is current; workspaces come from torch's allocator on that stream.
+Calls run on the current stream of the cache's device (``prefill``: of the query's), whichever device is current;
+workspaces come from torch's allocator on that stream.
 """
 import ctypes
 import math
@@ -254,8 +257,8 @@ def _bf16_heads(t, B, dev):
 
 def prefill(query, key, value, *, window=None, sinks=0, starts=None, q_start=None, scaling=None, out=None):
     """Attention of L tokens, those at slots q_start .. q_start + L - 1 (``q_start`` None: the last L slots of
-    ``key``): ``query`` [B, NH, L, 128] over ``key`` / ``value`` [B, NKV, S, 128], bf16 with any strides that are
-    multiples of 8 elements; ``scaling`` > 0.  Returns out [B, L, NH, 128] bf16.  Slots from q_start + L on are not
+    ``key``): ``query`` [B, NH, L, 128] over ``key`` / ``value`` [B, NKV, S, 128], bf16 with positive strides
+    that are multiples of 8 elements; ``scaling`` > 0.  Returns out [B, L, NH, 128] bf16.  Slots from q_start + L on are not
     read."""
     if query.is_cuda and _current() != query.get_device():
         with _on(query.get_device()):

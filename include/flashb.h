@@ -246,10 +246,11 @@ typedef struct {
 } fb_kv_cache;
 /* Single-token attention: q [B, NH, 1, 128] bf16 (strides q_sb, q_sh), the token at slot lengths[b] - 1 of each row;
  * out [B, 1, NH, 128] bf16 contiguous, 8-byte aligned.  fp32 scores, softmax and sums, rounded to bf16 once.  acc /
- * acc_out (both or neither; fp32 [B, NKV, S], unit stride per slot, may be the same tensor, else share nothing): acc_out[b, h, j] =
- * decay acc[b, h, j] + the weight of slot j summed over the group's query heads, for every slot of the cache.  ws: 16-byte aligned, at
- * least flashb_long_decode_ws_floats() floats (0 for few rows: then it may be NULL), not shared by calls that can overlap,
- * contents free before and after.
+ * acc_out (both or neither; fp32 [B, NKV, S], unit stride per slot; the same tensor, or no memory in common):
+ * acc_out[b, h, j] = decay acc[b, h, j] + the weight of slot j summed over the group's query heads, for every slot of the
+ * cache.  ws: 16-byte aligned, at least flashb_long_decode_ws_floats() floats (0 for few rows: then it may be NULL), not
+ * shared by calls that can overlap, contents free before and after.  The weights enter the product with V as two bf16 parts,
+ * or in fp16 over a 4-bit cache; an infinity in a visible V gives an output that is not finite (infinite or NaN).
  * The same inputs give the same bits. */
 int64_t flashb_long_decode_ws_floats(const fb_kv_cache* cache, int NH, int window, int sinks, int scored);
 int flashb_long_decode(const fb_kv_cache* cache, const void* q, int64_t q_sb, int64_t q_sh, int NH,
@@ -258,8 +259,9 @@ int flashb_long_decode(const fb_kv_cache* cache, const void* q, int64_t q_sb, in
                        int64_t acco_sh, float decay, float* ws, int64_t ws_floats, void* out, void* stream);
 /* Attention of the tokens at slots q_start .. q_start + L - 1: q [B, NH, L, 128] bf16 over k / v [B, NKV, S, 128] bf16
  * (strides per batch row, head and position in elements, multiples of 8; 16-byte aligned; q_start + L <= S; later
- * slots are not read; S <= 0x3fffff00; scaling > 0); out [B, L, NH, 128] bf16 with strides o_sb, o_sl, o_sh (multiples
- * of 8; 16-byte aligned).  Arithmetic as above. */
+ * slots are not read; S <= 0x3fffff00; strides and scaling > 0); out [B, L, NH, 128] bf16 with strides o_sb, o_sl, o_sh
+ * (multiples of 8; 16-byte aligned; no two rows share memory).  Arithmetic as above, but that the weights enter the product
+ * with V as one bf16 part. */
 int flashb_long_prefill(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_sl, const void* k, int64_t k_sb,
                         int64_t k_sh, int64_t k_sl, const void* v, int64_t v_sb, int64_t v_sh, int64_t v_sl, int B,
                         int NH, int NKV, int L, int S, int q_start, const int64_t* starts, int window, int sinks,
@@ -267,7 +269,8 @@ int flashb_long_prefill(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_sl,
 /* Stores bf16 heads k / v [B, NKV, L, 128] (strides in elements, multiples of 8; 16-byte aligned) into the 4-bit cache
  * at slots[b * slot_sb + l] (device int64; distinct within a row; slots outside [0, S) are skipped).  Per block of 16
  * values x (divided by the tensor scale): s = e4m3(max |x| / 6), code = e2m1(x / s), to nearest, ties to even,
- * saturating; a block with a NaN or an infinity reads back as NaN.  The result is that of exact arithmetic. */
+ * saturating; a block with a NaN or an infinity reads back as NaN.  The result is that of exact arithmetic.  No two slots
+ * of the cache may share memory. */
 int flashb_kv4_store(const fb_kv_cache* cache, const void* k, int64_t k_sb, int64_t k_sh, int64_t k_sl, const void* v,
                      int64_t v_sb, int64_t v_sh, int64_t v_sl, const int64_t* slots, int64_t slot_sb, int L,
                      void* stream);
@@ -276,11 +279,11 @@ int flashb_kv4_read(const fb_kv_cache* cache, const int64_t* slots, int64_t slot
                     void* stream);
 /* Eviction by accumulated attention weight: of row b's slots [starts[b], lengths[b]) at most `keep` move, in slot
  * order, to slots 0, 1, .. of `into` (a cache of the same bits, rows, heads and tensor scales that shares no memory
- * with `cache`): all when there are no more, else the first `sinks`, the last `recent` (sinks + recent <= keep) and
- * the others of largest acc[b, h, .] (fp32, unit stride per slot; equal weights: the lower slot; NaN above all), each
- * KV head for itself.  kept [B, NKV, keep] int32: the slot each came from, -1 beyond; lengths_out [B] int64: how many
- * (may not be `lengths`); acc_out (or NULL; may not be acc) [B, NKV, acc_n >= keep] fp32: the weights moved along, 0
- * beyond. */
+ * with `cache` and whose slots share none): all when there are no more, else the first `sinks`, the last `recent`
+ * (sinks + recent <= keep) and the others of largest acc[b, h, .] (fp32, unit stride per slot; equal weights: the lower
+ * slot; NaN above all), each KV head for itself.  kept [B, NKV, keep] int32: the slot each came from, -1 beyond;
+ * lengths_out [B] int64: how many (may not be `lengths`); acc_out (or NULL; no memory in common with acc) [B, NKV,
+ * acc_n >= keep] fp32: the weights moved along, 0 beyond. */
 int flashb_kv_evict(const fb_kv_cache* cache, const float* acc, int64_t acc_sb, int64_t acc_sh, const int64_t* lengths,
                     const int64_t* starts, int keep, int sinks, int recent, const fb_kv_cache* into, float* acc_out,
                     int64_t acco_sb, int64_t acco_sh, int acc_n, int32_t* kept, int64_t* lengths_out, void* stream);
