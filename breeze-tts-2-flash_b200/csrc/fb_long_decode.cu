@@ -1033,7 +1033,7 @@ int long_launch(LongDecodeArgs& a, const LongPlan& p, cudaStream_t st) {
 
 extern "C" int64_t flashb_long_decode_ws_floats(const fb_kv_cache* cache, int NH, int window, int sinks, int scored) {
   fb::LongCache lc;
-  LongPlan p;
+  LongPlan p{};
   if (fbh::long_cache(cache, &lc) != FB_OK || long_plan_host(cache, NH, window, sinks, scored != 0, &p) != FB_OK)
     return -1;
   return p.ws_floats;
@@ -1057,7 +1057,7 @@ extern "C" int flashb_long_decode(const fb_kv_cache* cache, const void* q, int64
                  "long_decode: acc and acc_out share memory and are not the same");
     FB_CHECK_ARG(!fbh::long_box_folds(weights(acc_out, acco_sb, acco_sh)), "long_decode: rows of acc_out share memory");
   }
-  LongPlan p;
+  LongPlan p{};
   rc = long_plan_host(cache, NH, window, sinks, acc != nullptr, &p);
   if (rc) return rc;
   FB_CHECK_ARG(((uintptr_t)q & 15) == 0 && q_sb % 8 == 0 && q_sh % 8 == 0,
