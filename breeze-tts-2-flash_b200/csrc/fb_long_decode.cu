@@ -40,8 +40,9 @@
 
 #include <cfloat>
 #include <cmath>
+#include <type_traits>
 
-#include "fb_long.cuh"
+#include "fb_paged.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -75,7 +76,17 @@ struct LongDecodeArgs {
   float* sc;                            // scores [row][cap][G] in log2 units (weights wanted), else null
   int cap;                              // visible keys a row can have
   bf16* out;
+  PagedTable t;                         // a paged cache: c.k_sb and c.v_sb are the pages' strides
 };
+
+// Paged: the visible keys' numbering begins at a multiple of 16 slots (sinks end at one), so that a warp's tile of 16 lies
+// in one page; what it holds beside visible keys gets no weight.
+struct LongPagedRow : LongRow {
+  int vlo, vns;                         // visible: slots below vns, and from vlo on
+  __device__ __forceinline__ bool sees(int j) const { return (j >= vlo || j < vns) && index(j) >= 0; }
+};
+template <bool PAGED>
+using LongRowOf = std::conditional_t<PAGED, LongPagedRow, LongRow>;
 
 template <int BITS>
 struct LongTile {
@@ -135,25 +146,38 @@ __device__ __forceinline__ uint2 ld_nc_v2(const void* p) {
 // with ragged rows the CTAs of many short ones came out last by a quarter of the time without them (the 4-bit case above,
 // one to four of them: 38.4, 38.7, 39.2, 40.1 us).  Every warp works the
 // list out for itself (no barrier): lane i counts the chunks of rows [i per, i per + per).
+template <bool PAGED>
 struct LongPlace {
   int b, before;                        // batch row, chunks of one KV head of all rows before it
-  LongRow row;
+  LongRowOf<PAGED> row;
 };
-__device__ __forceinline__ LongRow long_row_of(const LongDecodeArgs& a, int b) {
-  return long_row(a.lengths[b], a.starts ? a.starts[b] : 0, a.S, a.window, a.sinks);
+template <bool PAGED>
+__device__ __forceinline__ LongRowOf<PAGED> long_row_of(const LongDecodeArgs& a, int b) {
+  if constexpr (PAGED) {
+    LongPagedRow r;
+    const LongRow x = long_row(a.lengths[b], 0, a.S, a.window, a.sinks);
+    const int lo = x.lo & ~15, ns = (x.ns + 15) & ~15, end = x.lo + x.n - x.ns;
+    r.st = 0, r.vlo = x.lo, r.vns = x.ns;
+    r.ns = ns < lo ? ns : 0;
+    r.lo = ns < lo ? lo : 0;
+    r.n = r.ns + end - r.lo;
+    return r;
+  } else {
+    return long_row(a.lengths[b], a.starts ? a.starts[b] : 0, a.S, a.window, a.sinks);
+  }
 }
 template <int BITS>
 __device__ __forceinline__ int long_chunks(const LongRow& row) {
   using T = LongTile<BITS>;
   return row.n > 0 ? (row.n + T::CHUNK - 1) / T::CHUNK + T::EXTRA : 0;
 }
-template <int BITS>
+template <int BITS, bool PAGED>
 __device__ __forceinline__ int long_count(const LongDecodeArgs& a, int per, int lane, int& upto) {   // total; upto: inclusive
   int n = 0;
 #pragma unroll 4
   for (int i = 0; i < per; ++i) {
     const int b = lane * per + i;
-    if (b < a.B) n += long_chunks<BITS>(long_row_of(a, b));
+    if (b < a.B) n += long_chunks<BITS>(long_row_of<PAGED>(a, b));
   }
   upto = n;
 #pragma unroll
@@ -166,14 +190,14 @@ __device__ __forceinline__ int long_count(const LongDecodeArgs& a, int per, int 
   return total;
 }
 // The batch row whose chunks hold number x of one KV head's list (x < total).
-template <int BITS>
-__device__ __forceinline__ LongPlace long_find(const LongDecodeArgs& a, int per, int lane, int before, int x) {
+template <int BITS, bool PAGED>
+__device__ __forceinline__ LongPlace<PAGED> long_find(const LongDecodeArgs& a, int per, int lane, int before, int x) {
   const int owner = 31 - __clz(__ballot_sync(FULL, before <= x));     // empty lanes share a count: the last of them
-  LongPlace p;
+  LongPlace<PAGED> p;
   p.b = owner * per;
   p.before = __shfl_sync(FULL, before, owner);
   while (true) {
-    p.row = long_row_of(a, p.b);
+    p.row = long_row_of<PAGED>(a, p.b);
     const int n = long_chunks<BITS>(p.row);
     if (x < p.before + n) return p;
     p.before += n;
@@ -192,19 +216,20 @@ struct LongStat {
   uint64_t l;             // the two partial sums
 };
 
+// hide (paged): bits 0 and 1, this lane's keys that get no weight.
 // Scores of a step (rows g, g + 8 of each 16-key tile, heads 2t, 2t + 1) -> weights as the B fragments of P^T; bf16:
 // the second parts of the weights in the upper columns (G <= 4) or in pl (G = 8).
-template <int BITS, bool SCORED, int NT>
+template <int BITS, bool SCORED, bool PAGED, int NT>
 __device__ __forceinline__ void long_softmax(float (&s)[NT][4], uint32_t (&pf)[NT][2], uint32_t (&pl)[2], LongStat& st,
-                                             float (&o)[8][4], int i0, int n, bool whole, float scA, float scB, float* scp,
-                                             int G, int g, int t) {
+                                             float (&o)[8][4], int i0, int n, bool whole, uint32_t hide, float scA, float scB,
+                                             float* scp, int G, int g, int t) {
   constexpr float SHIFT = LongTile<BITS>::SHIFT;
   if (!whole) {
 #pragma unroll
     for (int k = 0; k < NT; ++k)
 #pragma unroll
       for (int e = 0; e < 2; ++e)
-        if (i0 + 16 * k + g + 8 * e >= n) s[k][2 * e] = s[k][2 * e + 1] = -INFINITY;
+        if (PAGED ? (hide >> e) & 1u : i0 + 16 * k + g + 8 * e >= n) s[k][2 * e] = s[k][2 * e + 1] = -INFINITY;
   }
   const uint64_t sc = f2(scA, scB);
   float xA = s[0][0], xB = s[0][1];
@@ -269,8 +294,8 @@ __device__ __forceinline__ void long_softmax(float (&s)[NT][4], uint32_t (&pf)[N
 
 // Keys [i_first, i_end) of row (b, h) by the CTA's four warps; each leaves its (max, sum, unnormalised out) in shared
 // memory.  scp: score i of head g goes to scp[i G + g].
-template <int BITS, bool SCORED>
-__device__ __forceinline__ void long_piece(const LongDecodeArgs& a, int b, int h, const LongRow& row, int i_first, int i_end,
+template <int BITS, bool SCORED, bool PAGED>
+__device__ __forceinline__ void long_piece(const LongDecodeArgs& a, int b, int h, const LongRowOf<PAGED>& row, int i_first, int i_end,
                                            float* scp, float (*s_o)[8][LG_D], float (*s_m)[8], float (*s_l)[8]) {
   using T = LongTile<BITS>;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -337,20 +362,54 @@ __device__ __forceinline__ void long_piece(const LongDecodeArgs& a, int b, int h
     for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
   LongStat st{-INFINITY, -INFINITY, 0};
 
-  const unsigned char* kb = a.c.k + b * a.c.k_sb + h * a.c.k_sh;
-  const unsigned char* vb = a.c.v + b * a.c.v_sb + h * a.c.v_sh;
+  const unsigned char* kb = a.c.k + (PAGED ? 0 : b * a.c.k_sb) + h * a.c.k_sh;
+  const unsigned char* vb = a.c.v + (PAGED ? 0 : b * a.c.v_sb) + h * a.c.v_sh;
+  // the tile's page, one tile ahead of its keys
+  const int* table = PAGED ? a.t.table + b * a.t.table_sb : nullptr;
+  int next = 0;
+  bool some = false;                                         // a visible key in a page of the pool
+  if (PAGED && i_first + warp * T::KEYS < i_end) next = table[row.slot(i_first + warp * T::KEYS) >> a.t.shift];
   for (int i0 = i_first + warp * T::KEYS; i0 < i_end; i0 += T::CHUNK) {
     float s[T::KEYS / 16][4];
     uint32_t pf[T::KEYS / 16][2], pl[2];
     // a tile of consecutive slots: with rows of the dense stride every load is one address and a constant
-    const bool whole = i0 + T::KEYS <= row.n && (i0 >= row.ns || i0 + T::KEYS <= row.ns);
+    bool whole = i0 + T::KEYS <= row.n && (i0 >= row.ns || i0 + T::KEYS <= row.ns);
+    long long slot0 = row.slot(i0);
+    uint32_t hide = 0;
+    int pick[2], vpick[4];                                   // paged: offsets in the tile of the keys that are read
+    const unsigned char *kt = kb, *vt = vb;
+    if constexpr (PAGED) {
+      const int j0 = (int)slot0, page = next;
+      if (i0 + T::CHUNK < i_end) next = table[row.slot(i0 + T::CHUNK) >> a.t.shift];
+      if ((unsigned)page >= (unsigned)a.t.pages) continue;   // not in the pool: not visible
+      some = true;
+      slot0 = j0 & (a.t.page - 1);
+      kt += page * a.c.k_sb;
+      vt += page * a.c.v_sb;
+      whole = whole && (j0 >= row.vlo || j0 + T::KEYS <= row.vns);
+      if (!whole || !a.dense) {
+        // the place of a key that is not visible is read as the tile's first visible key
+        const int first = j0 < row.vns ? 0 : max(row.vlo - j0, 0);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int x = g + 8 * e;
+          const bool see = row.sees(j0 + x);
+          pick[e] = see ? x : first;
+          hide |= see ? 0u : 1u << e;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int x = 2 * t + (e & 1) + 8 * (e >> 1);
+          vpick[e] = row.sees(j0 + x) ? x : first;
+        }
+      }
+    }
     const bool fast = whole && a.dense;
-    const long long slot0 = row.slot(i0);
     if constexpr (BITS == 16) {
       __align__(16) uint32_t kw[2][16], vw[4][8];
       if (fast) {
-        const unsigned char* pk = kb + (slot0 + g) * 256 + 16 * t;
-        const unsigned char* pv = vb + (slot0 + 2 * t) * 256 + 16 * g;
+        const unsigned char* pk = kt + (slot0 + g) * 256 + 16 * t;
+        const unsigned char* pv = vt + (slot0 + 2 * t) * 256 + 16 * g;
 #pragma unroll
         for (int e = 0; e < 2; ++e)
 #pragma unroll
@@ -364,14 +423,16 @@ __device__ __forceinline__ void long_piece(const LongDecodeArgs& a, int b, int h
         // keys past the row's end read its last key (a visible one) and get no weight
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const unsigned char* p = kb + row.slot(min(i0 + g + 8 * e, row.n - 1)) * a.c.k_sp + 16 * t;
+          const unsigned char* p =
+              kt + (PAGED ? slot0 + pick[e] : row.slot(min(i0 + g + 8 * e, row.n - 1))) * a.c.k_sp + 16 * t;
 #pragma unroll
           for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(&kw[e][4 * i]) = ld_nc_v4(p + 64 * i);
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const unsigned char* p =
-              vb + row.slot(min(i0 + 2 * t + (e & 1) + 8 * (e >> 1), row.n - 1)) * a.c.v_sp + 16 * g;
+              vt + (PAGED ? slot0 + vpick[e] : row.slot(min(i0 + 2 * t + (e & 1) + 8 * (e >> 1), row.n - 1))) * a.c.v_sp +
+              16 * g;
 #pragma unroll
           for (int i = 0; i < 2; ++i) *reinterpret_cast<uint4*>(&vw[e][4 * i]) = ld_nc_v4(p + 128 * i);
         }
@@ -381,7 +442,7 @@ __device__ __forceinline__ void long_piece(const LongDecodeArgs& a, int b, int h
 #pragma unroll
       for (int i = 0; i < 8; ++i)
         mma_bf16(s[0], kw[0][2 * i], kw[1][2 * i], kw[0][2 * i + 1], kw[1][2 * i + 1], qf[i][0], qf[i][1]);
-      long_softmax<BITS, SCORED>(s, pf, pl, st, o, i0, row.n, whole, scA, scB, scp, G, g, t);
+      long_softmax<BITS, SCORED, PAGED>(s, pf, pl, st, o, i0, row.n, whole, hide, scA, scB, scp, G, g, t);
       // dims: row g of tile i is 8 g + i, row g + 8 is 64 + 8 g + i
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -451,7 +512,7 @@ __device__ __forceinline__ void long_piece(const LongDecodeArgs& a, int b, int h
                   qf[2 * w + 1][1]);
         }
       }
-      long_softmax<BITS, SCORED>(s, pf, pl, st, o, i0, row.n, whole, scA, scB, scp, G, g, t);
+      long_softmax<BITS, SCORED, PAGED>(s, pf, pl, st, o, i0, row.n, whole, hide, scA, scB, scp, G, g, t);
       // dims: row g of tile i is 16 g + i (first code word), row g + 8 is 16 g + 8 + i (second)
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
@@ -494,6 +555,11 @@ __device__ __forceinline__ void long_piece(const LongDecodeArgs& a, int b, int h
   // a NaN score is in the sum and not in the maximum: as the largest part it cannot be lost in the joins
   if (l.x != l.x) st.mA = FLT_MAX;
   if (l.y != l.y) st.mB = FLT_MAX;
+  // paged: visible scores of -inf alone are told from no visible key, whose maximum stays -inf
+  if (PAGED && some) {
+    st.mA = fmaxf(st.mA, -FLT_MAX);
+    st.mB = fmaxf(st.mB, -FLT_MAX);
+  }
   if (g == 0) {
     s_m[warp][2 * t] = st.mA;
     s_m[warp][2 * t + 1] = st.mB;
@@ -532,7 +598,7 @@ __device__ __forceinline__ void long_join(const float (*s_o)[8][LG_D], const flo
   }
 }
 
-template <int BITS, bool SCORED>
+template <int BITS, bool SCORED, bool PAGED>
 __global__ void __launch_bounds__(LD_THREADS, LongTile<BITS>::CTAS) long_decode_kernel(const __grid_constant__ LongDecodeArgs a) {
   using T = LongTile<BITS>;
   __shared__ __align__(16) float s_o[LD_WARPS][8][LG_D];
@@ -541,20 +607,20 @@ __global__ void __launch_bounds__(LD_THREADS, LongTile<BITS>::CTAS) long_decode_
   pdl_wait();
   pdl_trigger();
   int before;
-  const int total = long_count<BITS>(a, a.per, lane, before) * a.NKV;
+  const int total = long_count<BITS, PAGED>(a, a.per, lane, before) * a.NKV;
   const int ncta = min(a.ncta, total);                    // every CTA below it has a chunk at least
   const int cta = blockIdx.x;
   if (cta >= ncta) return;
   int pos = long_share(total, ncta, cta);
   const int end = long_share(total, ncta, cta + 1);
-  LongPlace at = long_find<BITS>(a, a.per, lane, before, pos / a.NKV);
+  LongPlace<PAGED> at = long_find<BITS, PAGED>(a, a.per, lane, before, pos / a.NKV);
   while (true) {
     const int nb = long_chunks<BITS>(at.row), rem = pos - at.before * a.NKV;
     const int h = rem / nb, e0 = rem - h * nb, e1 = min(nb, e0 + (end - pos));
     const int ch0 = max(0, e0 - T::EXTRA), ch1 = e1 - T::EXTRA;      // the row's own chunks
     const int r = at.b * a.NKV + h;
     if (ch1 > ch0) {
-      long_piece<BITS, SCORED>(a, at.b, h, at.row, ch0 * T::CHUNK, min(at.row.n, ch1 * T::CHUNK),
+      long_piece<BITS, SCORED, PAGED>(a, at.b, h, at.row, ch0 * T::CHUNK, min(at.row.n, ch1 * T::CHUNK),
                                SCORED ? a.sc + (long long)r * a.cap * G : nullptr, s_o, s_m, s_l);
       __syncthreads();
       const long long piece = (long long)cta + r;         // pieces in list order have increasing CTA or row: unique
@@ -570,7 +636,7 @@ __global__ void __launch_bounds__(LD_THREADS, LongTile<BITS>::CTAS) long_decode_
     if (pos == end) return;
     if (h == a.NKV - 1 && e1 == nb) {                     // the next row that has keys
       at.before += nb;
-      do at.row = long_row_of(a, ++at.b);
+      do at.row = long_row_of<PAGED>(a, ++at.b);
       while (at.row.n == 0);
     }
     __syncthreads();
@@ -580,7 +646,7 @@ __global__ void __launch_bounds__(LD_THREADS, LongTile<BITS>::CTAS) long_decode_
 // Few rows: a thread-block cluster per (row, KV head), its CTAs on equal runs of chunks; one launch, no workspace.  The
 // parts are joined through distributed shared memory in rank order.  Scores stay in shared memory until the row's
 // maximum and sum are known.
-template <int BITS, bool SCORED>
+template <int BITS, bool SCORED, bool PAGED>
 __global__ void __launch_bounds__(LD_THREADS, LongTile<BITS>::CTAS) long_cluster_kernel(const __grid_constant__ LongDecodeArgs a) {
   using T = LongTile<BITS>;
   extern __shared__ __align__(16) unsigned char smem[];
@@ -594,10 +660,10 @@ __global__ void __launch_bounds__(LD_THREADS, LongTile<BITS>::CTAS) long_cluster
   const int r = blockIdx.y, b = r / a.NKV, h = r - b * a.NKV, G = a.G;
   pdl_wait();
   pdl_trigger();
-  const LongRow row = long_row(a.lengths[b], a.starts ? a.starts[b] : 0, a.S, a.window, a.sinks);
+  const auto row = long_row_of<PAGED>(a, b);
   const int nb = (row.n + T::CHUNK - 1) / T::CHUNK;
   const int i_first = nb * split / ns * T::CHUNK, i_end = min(row.n, nb * (split + 1) / ns * T::CHUNK);
-  long_piece<BITS, SCORED>(a, b, h, row, i_first, i_end, SCORED ? s_sc - (long long)i_first * G : nullptr, s_o, s_m, s_l);
+  long_piece<BITS, SCORED, PAGED>(a, b, h, row, i_first, i_end, SCORED ? s_sc - (long long)i_first * G : nullptr, s_o, s_m, s_l);
   __syncthreads();
   for (int gg = 0; gg < G; ++gg) {
     float M, L, O;
@@ -629,7 +695,8 @@ __global__ void __launch_bounds__(LD_THREADS, LongTile<BITS>::CTAS) long_cluster
         L += f * lv[c];
         O += f * ov[c];
       }
-    a.out[((long long)b * a.NH + h * G + gg) * LG_D + tid] = __float2bfloat16_rn(row.n == 0 ? 0.f : O / L * a.v_scale);
+    a.out[((long long)b * a.NH + h * G + gg) * LG_D + tid] = 
+        __float2bfloat16_rn((PAGED ? M == -INFINITY : row.n == 0) ? 0.f : O / L * a.v_scale);
   }
   if constexpr (SCORED) {
     if (tid < G) {
@@ -720,7 +787,7 @@ __device__ __forceinline__ void long_weights(const LongDecodeArgs& a, const Long
 // warps on every fourth piece and joined in warp order; past those, CTAs of LD_SLICE slots turn scores into weights.
 // Eight CTAs an SM: the weights of 64 rows of up to 4096 slots and 4 heads 54.2 us in all, with the 96 registers of five
 // CTAs 57.1, with the 48 of ten 55.9; slices of 256 or 1024 slots 58.5 and 57.6.
-template <bool SCORED, bool WIDE>
+template <bool SCORED, bool WIDE, bool PAGED>
 __global__ void __launch_bounds__(LM_THREADS, 8) long_merge_kernel(const __grid_constant__ LongDecodeArgs a) {
   __shared__ float s_m[8], s_inv[8];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = a.G;
@@ -729,7 +796,7 @@ __global__ void __launch_bounds__(LM_THREADS, 8) long_merge_kernel(const __grid_
   const bool join = (int)blockIdx.x < joins;
   const int item = join && !WIDE ? blockIdx.x * W + warp : blockIdx.x - (join ? 0 : joins);
   const int r = join ? min(item, heads - 1) / G : item / a.slices, b = r / a.NKV, h = r - b * a.NKV;
-  const LongRow row = long_row_of(a, b);        // written at least two launches back
+  const auto row = long_row_of<PAGED>(a, b);    // written at least two launches back
   pdl_wait();
   pdl_trigger();
   const int2 own = row.n > 0 ? a.own[r] : make_int2(0, -1);   // CTAs [x, y] hold pieces of this row
@@ -778,7 +845,7 @@ __global__ void __launch_bounds__(LM_THREADS, 8) long_merge_kernel(const __grid_
     }
     // visible keys with scores of -inf alone: 0 / 0, as softmax has it
     const float f = a.v_scale / L;
-    const bool none = row.n == 0;
+    const bool none = PAGED ? M == -INFINITY : row.n == 0;
     *reinterpret_cast<uint2*>(a.out + ((long long)b * a.NH + h * G + gg) * LG_D + 4 * lane) =
         make_uint2(none ? 0u : pack_bf16(O.x * f, O.y * f), none ? 0u : pack_bf16(O.z * f, O.w * f));
     return;
@@ -953,7 +1020,8 @@ struct LongPlan {
   int64_t slots, ws_floats, off_ml, off_own, off_s;   // float offsets of the workspace's parts
 };
 
-int long_plan_host(const fb_kv_cache* c, int NH, int window, int sinks, bool scored, LongPlan* p) {
+// edges: slots beside the visible ones that a row's numbering can hold
+int long_plan_host(const fb_kv_cache* c, int NH, int window, int sinks, bool scored, LongPlan* p, int edges = 0) {
   FB_CHECK_ARG(NH >= c->NKV && NH % c->NKV == 0, "long_decode: %d query heads over %d key/value heads", NH, c->NKV);
   const int G = NH / c->NKV;
   if (G != 1 && G != 2 && G != 4 && G != 8) {
@@ -961,7 +1029,7 @@ int long_plan_host(const fb_kv_cache* c, int NH, int window, int sinks, bool sco
     return FB_ERR_UNSUPPORTED;
   }
   FB_CHECK_ARG(sinks >= 0, "long_decode: sinks %d", sinks);
-  p->cap = window > 0 && (int64_t)window + sinks < c->S ? window + sinks : c->S;
+  p->cap = window > 0 && (int64_t)window + sinks + edges < c->S ? window + sinks + edges : c->S;
   const int chunk = c->bits == 16 ? LongTile<16>::CHUNK : LongTile<4>::CHUNK;
   const int64_t most = (int64_t)c->B * c->NKV * ((p->cap + chunk - 1) / chunk);
   const int ctas = c->bits == 16 ? LongTile<16>::CTAS : LongTile<4>::CTAS;
@@ -997,7 +1065,7 @@ int long_plan_host(const fb_kv_cache* c, int NH, int window, int sinks, bool sco
   return FB_OK;
 }
 
-template <int BITS, bool SCORED>
+template <int BITS, bool SCORED, bool PAGED = false>
 int long_launch(LongDecodeArgs& a, const LongPlan& p, cudaStream_t st) {
   void* args[] = {(void*)&a};
   if (p.split) {
@@ -1005,9 +1073,9 @@ int long_launch(LongDecodeArgs& a, const LongPlan& p, cudaStream_t st) {
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev >= 64 || !attr_done[dev]) {
-      cudaError_t e = cudaFuncSetAttribute(long_cluster_kernel<BITS, SCORED>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+      cudaError_t e = cudaFuncSetAttribute(long_cluster_kernel<BITS, SCORED, PAGED>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
       if (e == cudaSuccess && SCORED)
-        e = cudaFuncSetAttribute(long_cluster_kernel<BITS, SCORED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        e = cudaFuncSetAttribute(long_cluster_kernel<BITS, SCORED, PAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  LC_CHUNKS * LongTile<BITS>::CHUNK * 8 * (int)sizeof(float));
       if (e != cudaSuccess) {
         fbh::set_msg("long_decode: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
@@ -1015,17 +1083,17 @@ int long_launch(LongDecodeArgs& a, const LongPlan& p, cudaStream_t st) {
       }
       if (dev < 64) attr_done[dev] = 1;
     }
-    return fbh::launch_pdl((const void*)long_cluster_kernel<BITS, SCORED>, dim3(p.split, a.B * a.NKV), dim3(LD_THREADS),
+    return fbh::launch_pdl((const void*)long_cluster_kernel<BITS, SCORED, PAGED>, dim3(p.split, a.B * a.NKV), dim3(LD_THREADS),
                            p.smem, st, args, true, p.split);
   }
-  int rc = fbh::launch_pdl((const void*)long_decode_kernel<BITS, SCORED>, dim3(p.ncta), dim3(LD_THREADS), p.smem, st,
+  int rc = fbh::launch_pdl((const void*)long_decode_kernel<BITS, SCORED, PAGED>, dim3(p.ncta), dim3(LD_THREADS), p.smem, st,
                            args, true);
   if (rc) return rc;
   const int rows = a.B * a.NKV, heads = rows * a.G, per = LM_THREADS / 32;
   if (p.ncta > 8 * rows)                                 // more than eight pieces a row
-    return fbh::launch_pdl((const void*)long_merge_kernel<SCORED, true>, dim3(heads + rows * p.slices), dim3(LM_THREADS), 0, st,
+    return fbh::launch_pdl((const void*)long_merge_kernel<SCORED, true, PAGED>, dim3(heads + rows * p.slices), dim3(LM_THREADS), 0, st,
                            args, true);
-  return fbh::launch_pdl((const void*)long_merge_kernel<SCORED, false>, dim3((heads + per - 1) / per + rows * p.slices),
+  return fbh::launch_pdl((const void*)long_merge_kernel<SCORED, false, PAGED>, dim3((heads + per - 1) / per + rows * p.slices),
                          dim3(LM_THREADS), 0, st, args, true);
 }
 
@@ -1083,4 +1151,59 @@ extern "C" int flashb_long_decode(const fb_kv_cache* cache, const void* q, int64
   const cudaStream_t s = (cudaStream_t)stream;
   if (four) return acc ? long_launch<4, true>(a, p, s) : long_launch<4, false>(a, p, s);
   return acc ? long_launch<16, true>(a, p, s) : long_launch<16, false>(a, p, s);
+}
+
+namespace {
+// The list of rows as the contiguous form's host code takes it: `rows` rows of width x page slots.
+fb_kv_cache paged_shape(const fb_paged_cache* c, int rows, int width) {
+  fb_kv_cache s{};
+  s.bits = 16, s.B = rows, s.NKV = c->NKV, s.S = width * c->page;
+  return s;
+}
+constexpr int PAGED_EDGES = 30;        // a window's first tile and the sinks' last, at most 15 slots each
+}  // namespace
+
+extern "C" int64_t flashb_paged_decode_ws_floats(const fb_paged_cache* cache, int rows, int width, int NH, int window,
+                                                 int sinks) {
+  fb::PagedPool pool;
+  LongPlan p{};
+  if (fbh::paged_pool(cache, &pool) != FB_OK || fbh::paged_width(cache, rows, width) != FB_OK) return -1;
+  const fb_kv_cache shape = paged_shape(cache, rows, width);
+  if (long_plan_host(&shape, NH, window, sinks, false, &p, PAGED_EDGES) != FB_OK) return -1;
+  return p.ws_floats;
+}
+
+extern "C" int flashb_paged_decode(const fb_paged_cache* cache, const int32_t* table, int64_t table_sb, int rows, int width,
+                                   const int64_t* lengths, const void* q, int64_t q_st, int64_t q_sh, int NH, int window,
+                                   int sinks, float scaling, float* ws, int64_t ws_floats, void* out, void* stream) {
+  LongDecodeArgs a{};
+  fb::PagedPool pool;
+  int rc = fbh::paged_pool(cache, &pool);
+  if (!rc) rc = fbh::paged_width(cache, rows, width);
+  if (rc) return rc;
+  FB_CHECK_ARG(q && lengths && out && table, "paged_decode: null pointer argument");
+  FB_CHECK_ARG(table_sb >= 0, "paged_decode: table stride %lld", (long long)table_sb);
+  const fb_kv_cache shape = paged_shape(cache, rows, width);
+  LongPlan p{};
+  rc = long_plan_host(&shape, NH, window, sinks, false, &p, PAGED_EDGES);
+  if (rc) return rc;
+  FB_CHECK_ARG(((uintptr_t)q & 15) == 0 && q_st % 8 == 0 && q_sh % 8 == 0,
+               "paged_decode: q must be 16-byte aligned with strides multiple of 8 elements");
+  FB_CHECK_ARG(((uintptr_t)out & 7) == 0, "paged_decode: out must be 8-byte aligned");
+  FB_CHECK_ARG(scaling > 0.f, "paged_decode: scaling must be positive");
+  FB_CHECK_ARG(p.ws_floats == 0 || (ws && ((uintptr_t)ws & 15) == 0 && ws_floats >= p.ws_floats),
+               "paged_decode: workspace of %lld floats, %lld needed", (long long)ws_floats, (long long)p.ws_floats);
+  a.c.k = pool.k, a.c.v = pool.v;
+  a.c.k_sb = pool.k_sb, a.c.k_sh = pool.k_sh, a.c.k_sp = pool.k_sl;
+  a.c.v_sb = pool.v_sb, a.c.v_sh = pool.v_sh, a.c.v_sp = pool.v_sl;
+  a.t = fb::PagedTable{table, table_sb, pool.pages, pool.page, pool.shift};
+  a.q = (const bf16*)q, a.q_sb = q_st, a.q_sh = q_sh, a.lengths = (const long long*)lengths;
+  a.B = rows, a.NH = NH, a.NKV = cache->NKV, a.G = NH / cache->NKV, a.S = shape.S;
+  a.window = window > 0 ? window : 0, a.sinks = sinks, a.ncta = p.ncta;
+  a.scale = std::fmax(scaling * LG_LOG2E, FLT_MIN);
+  a.dense = pool.k_sl == 256 && pool.v_sl == 256;
+  a.v_scale = 1.f, a.shift = LongTile<16>::SHIFT, a.decay = 1.f;
+  a.po = ws, a.ml = (float2*)(ws + p.off_ml), a.own = (int2*)(ws + p.off_own);
+  a.per = (a.B + 31) / 32, a.cap = p.cap, a.out = (bf16*)out;
+  return long_launch<16, false, true>(a, p, (cudaStream_t)stream);
 }

@@ -69,6 +69,12 @@ _PROTOS = {
     'flashb_kv4_store': (I, [P, P, L, L, L, P, L, L, L, P, L, I, P]),
     'flashb_kv4_read': (I, [P, P, L, I, P, P, P]),
     'flashb_kv_evict': (I, [P, P, L, L, P, P, I, I, I, P, P, L, L, I, P, P, P]),
+    'flashb_paged_append': (I, [P, P, L, I, I, P, P, I, P, L, I, P, P, F, P, I, I, F, P, P, L, L, P]),
+    'flashb_paged_decode_ws_floats': (L, [P, I, I, I, I, I]),
+    'flashb_paged_decode': (I, [P, P, L, I, I, P, P, L, L, I, I, I, F, P, L, P, P]),
+    'flashb_paged_attend_ws_floats': (L, [P, I, I, I, I, I, I]),
+    'flashb_paged_attend': (I, [P, P, L, I, I, P, P, I, P, L, L, I, I, I, F, P, L, P, L, L, P]),
+    'flashb_token_scores': (I, [P, I, L, I, I, P, F, I, P, P, P, P, P, P]),
     'flashb_ln12_decode': (I, [P, P, P, ctypes.c_uint32, ctypes.c_uint32, I, I, P, L, P]),
     'flashb_lm_head_rows': (I, [P, L, I, I, P, I, P, P]),
     'flashb_dd_scratch_bytes': (L, [P]),
@@ -106,6 +112,12 @@ class FbKVCache(ctypes.Structure):
                 [(n, L) for n in ('k_sb', 'k_sh', 'k_sp', 'v_sb', 'v_sh', 'v_sp')] + [('ks', P), ('vs', P)] +
                 [(n, L) for n in ('ks_sb', 'ks_sh', 'ks_sp', 'vs_sb', 'vs_sh', 'vs_sp')] +
                 [('k_scale', F), ('v_scale', F)])
+
+
+class FbPagedCache(ctypes.Structure):
+    """fb_paged_cache of include/flashb.h."""
+    _fields_ = ([(n, I) for n in ('pages', 'NKV', 'page')] + [('k', P), ('v', P)] +
+                [(n, L) for n in ('k_sb', 'k_sh', 'k_sl', 'v_sb', 'v_sh', 'v_sl')])
 
 
 def lib_path():

@@ -7,7 +7,12 @@ softmax / multinomial) and the multinomial's validity predicate as a device flag
 Here it is one ``flashb_cb0_sample`` launch (one CTA per row) instead of ~10 torch ops.  The multinomial draw is
 ``argmax(probs / q)`` with ``q`` Exp(1) draws (the identity ``torch.multinomial(p, 1) == argmax(p / Exp(1))``): pass
 ``q`` to control the randomness, else it is drawn on the device from torch's generator.
+
+``token_scores`` says what logits say of given tokens: log probability, entropy, rank, the likeliest alternatives (the
+reference has none).
 """
+from typing import NamedTuple
+
 import torch
 
 from . import _native
@@ -84,3 +89,48 @@ def sample_logits(logits, *, temperature, top_k, top_p, do_sample, present=None,
     tok, ok = sample_rows(x, temperature, top_k, top_p, do_sample, pres, repetition_penalty, suppress_idx,
                           q=None if q is None else q.reshape(x.shape).float().contiguous())
     return tok.view(shape), ok.bool().all()
+
+
+class TokenScores(NamedTuple):
+    """``token_scores``'s answer, a row of logits each."""
+    logprob: torch.Tensor        # [rows] fp32: log probability of the given token
+    entropy: torch.Tensor        # [rows] fp32: of the row's distribution, in nats
+    rank: torch.Tensor           # [rows] int64: ids ahead of the given token (0: the greedy choice)
+    top_ids: torch.Tensor        # [rows, top] int64: the likeliest ids, in order
+    top_logprobs: torch.Tensor   # [rows, top] fp32: theirs
+
+
+def token_scores(logits, tokens, *, top=0, temperature=1.0):
+    """What ``logits`` [rows, V] (fp32 or bf16, unit inner stride; CFG logits, or the logits of a given reading) say of
+    ``tokens`` [rows] int64 under softmax(logits / temperature): a ``TokenScores``, in one launch.
+
+    Larger logits come first, equal ones by id, a NaN before all, as in the greedy sampler.  Suppressed ids (-inf) have
+    probability 0; an id outside the vocabulary has log probability -inf and rank V.  A row with a NaN or +inf, or of -inf
+    alone, has no distribution: NaN log probabilities and entropy."""
+    def _ensure(cond, msg):
+        if not cond:
+            raise _native.FlashbError(_native.FB_ERR_ARG, msg)
+
+    _ensure(logits.is_cuda and logits.dtype in (torch.float32, torch.bfloat16) and logits.dim() == 2 and
+            (logits.shape[1] == 1 or logits.stride(1) == 1), 'logits: [rows, V] fp32 or bf16 CUDA with unit inner stride')
+    rows, V = logits.shape
+    dev = logits.device
+    _ensure(tokens.dtype == torch.int64 and tokens.device == dev and tokens.shape == (rows,) and tokens.is_contiguous(),
+            'tokens: [rows] int64 on the logits\' device')
+    _ensure(V >= 1 and 0 <= top <= min(32, V), f'top: 0 to {min(32, V)}')
+    if torch._C._cuda_getDevice() != logits.get_device():
+        with torch.cuda.device(dev):
+            return token_scores(logits, tokens, top=top, temperature=temperature)
+    # one allocation: the 64-bit parts first
+    buf = torch.empty(rows * (3 * top + 4), dtype=torch.float32, device=dev)
+    ids, rest = buf[:rows * (2 * top + 2)].view(torch.int64), buf[rows * (2 * top + 2):]
+    out = TokenScores(rest[:rows], rest[rows:2 * rows], ids[:rows], ids[rows:].view(rows, top),
+                      rest[2 * rows:].view(rows, top))
+    if rows == 0:
+        return out
+    check(_native.lib().flashb_token_scores(
+        logits.data_ptr(), int(logits.dtype == torch.bfloat16), logits.stride(0) if rows > 1 else V, rows, V,
+        tokens.data_ptr(), float(temperature), int(top), out.logprob.data_ptr(), out.entropy.data_ptr(),
+        out.rank.data_ptr(), out.top_ids.data_ptr(), out.top_logprobs.data_ptr(),
+        torch._C._cuda_getCurrentRawStream(logits.get_device())))
+    return out

@@ -288,6 +288,59 @@ int flashb_kv_evict(const fb_kv_cache* cache, const float* acc, int64_t acc_sb, 
                     const int64_t* starts, int keep, int sinks, int recent, const fb_kv_cache* into, float* acc_out,
                     int64_t acco_sb, int64_t acco_sh, int acc_n, int32_t* kept, int64_t* lengths_out, void* stream);
 
+/* ---------------------------------------------------------------------------------------------- paged cache
+ * Many rows (streams, prompts, conditional / unconditional halves) on the pages of one pool: every row has as many slots
+ * as it needs, and a step takes any number of new tokens of each.  No reference counterpart (the reference decodes one
+ * request on a cache of its own).  Slot j of row b lies in page table[b table_sb + j / page] of the pool (int32 on the
+ * device, `width` entries a row).  A step's T tokens: offsets [rows + 1] (device int64, not decreasing) cuts them into
+ * one run per row, possibly empty; tokens outside every run are not touched.  Row b's run ends at slot lengths[b] - 1
+ * (device int64: lengths count the new tokens).  An entry that is not a page of the pool (-1, say) makes its slots
+ * invisible, and nothing is written there; entries of slots that no token sees are not read. */
+typedef struct {
+  int pages, NKV, page;  /* page: slots of a page, a power of two from 16 on */
+  void *k, *v;           /* [pages, NKV, page, 128] bf16, 16-byte aligned; strides per page, head and slot in elements, */
+  int64_t k_sb, k_sh, k_sl, v_sb, v_sh, v_sl; /* multiples of 8; the innermost stride is 1 */
+} fb_paged_cache;
+/* qkv [T, (NH + 2 NKV) 128] bf16 raw projections (row stride ldq, a multiple of 8): the q heads go to q_out [T, NH, 128]
+ * (strides o_st, o_sh, multiples of 8; qkv itself, with its strides, is allowed), the k and v heads to their slots
+ * (slots outside the row's entries are skipped).  q and k heads, in fp32 and rounded once: RMS norm with weights q_norm /
+ * k_norm [128] bf16 (both or neither), then the rotation of their first `rot` dims (a multiple of 16, 0: none) by
+ * position x turns[i] whole turns (turns [rot / 2] fp64 on the device) of pairs (i, i + rot / 2) or, interleaved,
+ * (2 i, 2 i + 1), times amplitude.  positions [T] int64, or NULL: the token's slot.  offsets NULL: T = rows, token b is row
+ * b's. */
+int flashb_paged_append(const fb_paged_cache* cache, const int32_t* table, int64_t table_sb, int rows, int width,
+                        const int64_t* lengths, const int64_t* offsets, int T, const void* qkv, int64_t ldq, int NH,
+                        const void* q_norm, const void* k_norm, float eps, const double* turns, int rot, int interleaved,
+                        float amplitude, const int64_t* positions, void* q_out, int64_t o_st, int64_t o_sh, void* stream);
+/* Attention of the step's tokens: q [T, NH, 128] bf16 (strides q_st, q_sh) -> out [T, NH, 128] (strides o_st, o_sh), all
+ * multiples of 8, 16-byte aligned.  The token at slot p sees slot j when j <= p and (j > p - window or j < sinks); window
+ * <= 0: no window; scaling > 0; lengths are clamped to the row's entries.  NH / NKV in {1, 2, 4, 8}.  Scores, softmax and
+ * sums in fp32; slots that are not visible may hold anything; without a visible slot the output is 0 (with visible scores
+ * of -inf alone NaN).  ws: 16-byte aligned, at least flashb_paged_attend_ws_floats() floats (0: may be NULL), not shared by
+ * calls that can overlap, contents free before and after.  The same inputs give the same bits. */
+int64_t flashb_paged_attend_ws_floats(const fb_paged_cache* cache, int rows, int width, int T, int NH, int window,
+                                      int sinks);
+int flashb_paged_attend(const fb_paged_cache* cache, const int32_t* table, int64_t table_sb, int rows, int width,
+                        const int64_t* lengths, const int64_t* offsets, int T, const void* q, int64_t q_st, int64_t q_sh,
+                        int NH, int window, int sinks, float scaling, float* ws, int64_t ws_floats, void* out,
+                        int64_t o_st, int64_t o_sh, void* stream);
+/* The same for one token a row: q [rows, NH, 128], out [rows, NH, 128] contiguous, 8-byte aligned. */
+int64_t flashb_paged_decode_ws_floats(const fb_paged_cache* cache, int rows, int width, int NH, int window, int sinks);
+int flashb_paged_decode(const fb_paged_cache* cache, const int32_t* table, int64_t table_sb, int rows, int width,
+                        const int64_t* lengths, const void* q, int64_t q_st, int64_t q_sh, int NH, int window, int sinks,
+                        float scaling, float* ws, int64_t ws_floats, void* out, void* stream);
+
+/* ---------------------------------------------------------------------------------------------- token scores
+ * logits [rows, V] fp32 or bf16 (row stride ld elements, any alignment of the type; V <= 2^24) and a token per row (device
+ * int64): logprob [rows] fp32 = log softmax(logits / temperature)[token] (-inf for an id outside [0, V)), entropy [rows]
+ * fp32 in nats, rank [rows] int64 = how many ids come before the token (V for one outside), and the first `top` (0 to 32,
+ * at most V) ids top_id [rows, top] int64 with their log probabilities top_logprob [rows, top] fp32.  The order: larger
+ * logits first, equal ones by id, a NaN before all (as flashb_cb0_sample's argmax).  Rows that hold a NaN or +inf, or -inf
+ * alone, have no distribution: NaN for what is not an id or a rank.  No reference counterpart. */
+int flashb_token_scores(const void* logits, int is_bf16, int64_t ld, int rows, int V, const int64_t* tokens,
+                        float temperature, int top, float* logprob, float* entropy, int64_t* rank, int64_t* top_id,
+                        float* top_logprob, void* stream);
+
 /* LN12 -> bf16 on the device (the reference's lossless 12-bit weight storage, flash/ln12_format.py, read by its depth
  * kernels through dd2_init_ln12, flash/csrc/depth_frame.cu:800-823): a matrix W[N, K] (K % 1024 == 0) stored as
  * data [N][K / 1024][3][32][16 B] (slot 0: low bytes of the chunks 0, 1 of lane l's elements k = 1024 g + 256 c +

@@ -1,0 +1,109 @@
+"""Token scores on the GPU against their definition in 64 bits."""
+import pytest
+import torch
+
+import paged_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+
+def check(x, tokens, top, temperature=1.0):
+    from flashb.sampling import token_scores
+    got = token_scores(x.cuda(), tokens.cuda(), top=top, temperature=temperature)
+    lp, h, rank, ids, tl = ref.scores(x, tokens, top, temperature)
+    assert torch.equal(got.rank.cpu(), rank)
+    assert torch.equal(got.top_ids.cpu(), ids)
+    # differences from the maximum and their scaling in fp32 (2^-22 of them), the sum and its logarithm (2^-18)
+    for a, b in ((got.logprob.cpu().double(), lp), (got.top_logprobs.cpu().double(), tl)):
+        assert torch.equal(torch.isnan(a), torch.isnan(b)) and torch.equal(torch.isinf(a), torch.isinf(b))
+        fin = torch.isfinite(b)
+        assert torch.all((a - b).abs()[fin] <= (2.0 ** -22 * b.abs() + 2.0 ** -18)[fin])
+    a = got.entropy.cpu().double()
+    assert torch.equal(torch.isnan(a), torch.isnan(h))
+    fin = torch.isfinite(h)
+    assert torch.all((a - h).abs()[fin] <= (2.0 ** -18 * (1 + h))[fin])
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('V', [1, 2, 31, 33, 255, 257, 1000, 2049])
+def test_sizes(V, dtype):
+    g = torch.Generator().manual_seed(V)
+    x = (3 * torch.randn(5, V, generator=g)).to(dtype)
+    check(x, torch.randint(0, V, (5,), generator=g), min(V, 7))
+    check(x, torch.randint(0, V, (5,), generator=g), 0, 0.7)
+    check(x, torch.randint(0, V, (5,), generator=g), min(V, 32), 2.5)
+
+
+@pytest.mark.parametrize('V', [4095, 4097, 9001, 40000])
+def test_large_vocabularies(V):
+    g = torch.Generator().manual_seed(V)
+    x = 3 * torch.randn(3, V, generator=g)
+    check(x, torch.randint(0, V, (3,), generator=g), 20)
+    check(x.bfloat16(), torch.randint(0, V, (3,), generator=g), 20)
+
+
+def test_many_rows():
+    g = torch.Generator().manual_seed(4)
+    check(torch.randn(700, 65, generator=g), torch.randint(0, 65, (700,), generator=g), 3)
+
+
+def test_ties_go_to_the_lowest_id():
+    x = torch.randint(-3, 3, (6, 500), generator=torch.Generator().manual_seed(1)).float()
+    x[1] = 2.0
+    x[2, ::2] = -0.0
+    x[2, 1::2] = 0.0
+    t = torch.tensor([3, 499, 77, 0, 250, 499])
+    check(x, t, 32)
+    check(x.bfloat16(), t, 32)
+
+
+def test_suppressed_ids_and_rows_without_a_distribution():
+    inf, nan = float('inf'), float('nan')
+    x = torch.randn(8, 300, generator=torch.Generator().manual_seed(2))
+    x[0, 5:] = -inf
+    x[1] = -inf
+    x[2, 7] = inf
+    x[3, 9] = nan
+    x[4, 1:] = -inf
+    x[5] = 1e30
+    x[5, ::2] = -1e30
+    x[6] = -3e38
+    t = torch.tensor([3, 0, 7, 9, 200, 1, 299, 4])
+    check(x, t, 8)
+    check(x, torch.tensor([9, -1, 300, 10 ** 12, 0, 0, -10 ** 12, 2 ** 32 + 4]), 8)
+
+
+def test_strided_rows_and_unaligned_starts():
+    g = torch.Generator().manual_seed(6)
+    for dtype in (torch.float32, torch.bfloat16):
+        wide = (2 * torch.randn(9, 777, generator=g)).to(dtype)
+        from flashb.sampling import token_scores
+        for lo, hi in ((0, 777), (1, 700), (3, 501), (5, 38)):
+            x, t = wide.cuda()[:, lo:hi], torch.arange(9).cuda()
+            a, b = token_scores(x, t, top=5), token_scores(x.contiguous(), t, top=5)
+            for p, q in zip(a, b):
+                assert torch.allclose(p.double(), q.double(), rtol=1e-5, atol=1e-5)
+            check(wide[:, lo:hi], torch.arange(9), 5)
+
+
+def test_sharp_rows_keep_small_numbers():
+    """An almost certain token: its log probability and the entropy are small, not zero."""
+    x = torch.zeros(3, 2049)
+    x[:, 100] = torch.tensor([20.0, 25.0, 30.0])
+    from flashb.sampling import token_scores
+    got = token_scores(x.cuda(), torch.full((3,), 100).cuda())
+    lp, h, *_ = ref.scores(x, torch.full((3,), 100), 0, 1.0)
+    assert torch.allclose(got.logprob.cpu().double(), lp, rtol=1e-4, atol=0)
+    assert torch.allclose(got.entropy.cpu().double(), h, rtol=1e-4, atol=0)
+
+
+def test_captured():
+    from flashb.sampling import token_scores
+    x, t = torch.randn(4, 100, device='cuda'), torch.arange(4, device='cuda')
+    token_scores(x, t, top=3)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = token_scores(x, t, top=3)
+    x.copy_(torch.randn(4, 100))
+    graph.replay()
+    assert all(torch.equal(p, q) for p, q in zip(out, token_scores(x, t, top=3)))
