@@ -38,21 +38,9 @@
 // (a token before its row's start sees none and gives 0).
 #include <type_traits>
 
-#include "fb_long.cuh"
-#include "fb_tc.cuh"
+#include "fb_long_tc.cuh"
 
 namespace fb {
-
-constexpr int LP_ROWS = 128;                      // rows of a CTA (TMEM lanes)
-constexpr int LP_SEG = 32, LP_TILE = 64;          // keys per segment and tile
-constexpr int LP_THREADS = 224;                   // 4 softmax warps; one each for copies, S and P V
-constexpr int LP_Q = LP_ROWS * LG_D * 2;          // bytes of the Q tile
-constexpr int LP_KV = LP_TILE * LG_D * 2;         // ... of a K or V tile
-constexpr int LP_SMEM = LP_Q + 4 * LP_KV + 1024;  // Q, K and V twice, at a 1024-byte boundary
-constexpr uint32_t LP_COLS = 256;                 // TMEM: S in columns 0-63, P twice in 64-127, O in 128-255
-constexpr float LP_SLACK = 8.f;
-// P x 2^-24: the unnormalised sums of 2^16 keys stay in fp32's range for every finite V
-constexpr float LP_SHIFT = -24.f;
 
 struct alignas(64) LongPrefillArgs {
   CUtensorMap tq, to, tk, tv, tk32, tv32;         // Q and out tiles; K, V: boxes of 64 and of 32 slots
@@ -65,78 +53,6 @@ struct alignas(64) LongPrefillArgs {
   long long o_sb, o_sl, o_sh;
   unsigned* err;
 };
-
-__device__ __forceinline__ void lp_load(void* dst, const CUtensorMap* m, int c1, int c2, int c3, int c4, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, "
-      "%6}], [%7];" ::"r"(smem_u32(dst)),
-      "l"(m), "r"(0), "r"(c1), "r"(c2), "r"(c3), "r"(c4), "r"(smem_u32(bar))
-      : "memory");
-}
-// D (+)= P V: P in TMEM (row = lane, two bf16 per column), V in shared memory with the dims contiguous
-__device__ __forceinline__ void lp_mma_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
-      "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate));
-}
-__device__ __forceinline__ void lp_ld32(uint32_t taddr, float* f) {
-  uint32_t r[32];
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
-      "tcgen05.wait::ld.sync.aligned;"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr));
-#pragma unroll
-  for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(r[i]);
-}
-// 64 consecutive fp32 columns of this thread's TMEM lane.
-__device__ __forceinline__ void lp_ld64(uint32_t taddr, float* f) {
-  uint32_t r[64];
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
-      "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
-      "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];\n\t"
-      "tcgen05.wait::ld.sync.aligned;"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
-        "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
-        "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
-        "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
-        "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
-      : "r"(taddr));
-#pragma unroll
-  for (int i = 0; i < 64; ++i) f[i] = __uint_as_float(r[i]);
-}
-// Bits [lo, hi) of 32, whatever the two are.
-__device__ __forceinline__ uint32_t lp_bits(int lo, int hi) {
-  lo = max(lo, 0);
-  hi = min(hi, 32);
-  return lo < hi ? (0xffffffffu >> (32 - hi)) & (0xffffffffu << lo) : 0u;
-}
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
-__device__ __forceinline__ void lp_st32(uint32_t taddr, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};\n\t"
-      "tcgen05.wait::st.sync.aligned;" ::"r"(r[0]),
-      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
-      "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
-      "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
-      : "memory");
-}
 
 // One row over its visible keys, one at a time (the case of a non-finite output; see the header): a warp, four dims a
 // lane.  d: the row in the output tile (its halves LP_Q / 2 apart), x: the swizzle of its 16-byte units.
@@ -168,17 +84,6 @@ __device__ __noinline__ void long_row_again(const LongPrefillArgs& a, int b, int
   const float inv = row.n == 0 ? 0.f : 1.f / sum;
   d += (lane >> 4) * (LP_Q / 2) + ((((lane & 15) >> 1) ^ x) << 4) + (lane & 1) * 8;
   *reinterpret_cast<uint2*>(d) = make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
-}
-
-// Bounded wait; the clock is read only after a long stretch of polling.
-__device__ __forceinline__ bool lp_wait(uint64_t* bar, unsigned parity, unsigned* err) {
-#pragma unroll 1
-  for (int i = 0; i < 256; ++i)
-    if (mbar_try_wait(bar, parity)) return true;
-  return mbar_wait(bar, parity, err);
-}
-__device__ __forceinline__ bool lp_wait_warp(uint64_t* bar, unsigned parity, unsigned* err) {
-  return __all_sync(FULL, lp_wait(bar, parity, err));
 }
 
 __global__ void __launch_bounds__(LP_THREADS, 2) long_prefill_kernel(const __grid_constant__ LongPrefillArgs a) {

@@ -1,29 +1,156 @@
-// flashb: attention of a step's new tokens (a run of any length per row) over a paged cache.
+// flashb: attention of a step's new tokens (a run of any length per row) over a paged cache, on the 5th-generation tensor
+// cores.
 //
 //   out_t = softmax(scaling q_t k^T over the slots that t sees) v, fp32, rounded once; without a visible slot 0.
 //
-// A warp per token and query head, one key at a time, four dims a lane.
+// The pipeline is fb_long_prefill.cu's (which see): 128 rows a CTA, 64-key tiles of two 32-key segments, S and P V by a
+// thread each, two CTAs an SM, a row's maximum moved only past 2^8.  What differs:
+//
+// Rows of a tile are the run's tokens in order with the G heads of a KV head inner, so a run of few tokens fills the first
+// warps alone; the others do not take part.  Keys come from pages: a segment is one box of 32 slots, or two of 16; a tile of
+// 64 slots in one page is one box.  An entry that is no page is loaded from past the pool's end, which reads as zeros, and
+// its slots get no weight.
+//
+// Pieces.  A step can be one run of a few tokens over a long row, or many rows of which some are long.  So the key tiles of
+// a query tile are cut into s pieces, s = ceil(k / C) with k its row's key tiles and C the work of the whole step over the
+// wanted number of CTAs; a CTA takes one piece.  Every CTA works the list out for itself from lengths and offsets (a warp,
+// some hundred cycles; no launch before it, nothing read on the host).  Pieces of a query tile leave (maximum, sum,
+// unnormalised out) in the workspace and paged_merge_kernel joins them in order: no atomics, the same inputs give the same
+// bits.  A query tile of one piece writes its rows itself.
+//
+// Slots that no row of the CTA sees may hold anything: in V they are zeroed in shared memory (0 times a NaN is NaN), in K
+// their scores are replaced.  A row whose output is not finite all the same (a NaN that another row of the tile sees) is
+// computed again, one visible key at a time.
+#include <climits>
+
+#include "fb_long_tc.cuh"
 #include "fb_paged.cuh"
 
 namespace fb {
 
-struct PagedAttendArgs {
+constexpr int PT_MIN = 4;                         // key tiles of a piece, at least
+
+struct alignas(64) PagedAttendArgs {
+  CUtensorMap tq, tk, tv, tks, tvs;     // Q tile; K, V: boxes of 64 slots, and of 32 or 16 (half of the dims)
   PagedPool pool;
   PagedTable t;
   PagedRows r;
   const bf16* q;
   long long q_st, q_sh;
-  int NH, G, window, sinks;
+  int NH, NKV, G, nq, window, sinks;    // nq = 128 / G tokens a CTA; window 0: none
+  int per, pieces;                      // rows per lane of the plan; CTAs wanted a KV head, 0: one piece a query tile
   float scale;                          // scaling x log2(e)
   bf16* out;
   long long o_st, o_sh;
+  float* po;                            // pieces: unnormalised out [slot][128][128],
+  float2* ml;                           //   maximum and sum [slot][128]
+  int2* own;                            // [row] the first slot and the pieces of a query tile (1: no slot)
+  unsigned* err;
 };
 
-// P x 2^-24: the unnormalised sums of 2^16 keys stay in fp32's range for every finite V
-constexpr float PT_SHIFT = -24.f;
+// Row b's run: n tokens from t0 on, the first at slot p0.
+struct PagedSpan {
+  int t0, n, p0;
+};
+__device__ __forceinline__ PagedSpan paged_span(const PagedRows& r, int b) {
+  const long long f = r.offsets[b], e = r.offsets[b + 1], len = r.lengths[b];
+  const int t0 = (int)min(max(f, 0ll), (long long)r.T), t1 = (int)min(max(e, (long long)t0), (long long)r.T);
+  const long long p0 = min(max(len, 0ll), (long long)r.S) - (e - t0);
+  return PagedSpan{t0, t1 - t0, (int)max(p0, -0x40000000ll)};
+}
+// The key segments of tokens at slots p_lo .. p_hi: ns of sinks from slot 0 on, then those from base to p_hi; lo: the first
+// slot that the window of any of them holds.
+struct PagedSegs {
+  int lo, base, ns, n;
+  __device__ __forceinline__ int at(int s) const { return s < ns ? LP_SEG * s : base + LP_SEG * (s - ns); }
+};
+__device__ __forceinline__ PagedSegs paged_segs(const PagedAttendArgs& a, int p_lo, int p_hi) {
+  PagedSegs g;
+  g.lo = a.window > 0 ? max(p_lo - a.window + 1, 0) : 0;
+  g.base = g.lo & ~(LP_SEG - 1);
+  g.ns = min((a.sinks + LP_SEG - 1) / LP_SEG, g.base / LP_SEG);
+  g.n = p_hi < 0 ? 0 : g.ns + (p_hi - g.base) / LP_SEG + 1;
+  return g;
+}
+// A row's query tiles and the key tiles of its last one (the most that one has).
+__device__ __forceinline__ int2 paged_tiles(const PagedAttendArgs& a, const PagedSpan& x) {
+  if (x.n <= 0) return make_int2(0, 0);
+  const int p_hi = x.p0 + x.n - 1;
+  return make_int2((x.n + a.nq - 1) / a.nq, (paged_segs(a, p_hi - min(x.n, a.nq) + 1, p_hi).n + 1) >> 1);
+}
+
+struct PagedPiece {
+  int b, qt, i, s, slot;                // row, query tile, piece i of s, its slot in the workspace; b = -1: none
+};
+// Number x of the list of pieces: rows in order, a row's latest query tiles first (they have the most keys).  One warp.
+__device__ __forceinline__ PagedPiece paged_plan(const PagedAttendArgs& a, int x, int lane, bool leave) {
+  long long w = 0;
+  for (int i = 0; i < a.per; ++i) {
+    const int b = lane * a.per + i;
+    if (b < a.r.rows) {
+      const int2 k = paged_tiles(a, paged_span(a.r, b));
+      w += (long long)k.x * k.y;
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(FULL, w, o);
+  const long long want = a.pieces > 0 ? (w + a.pieces - 1) / a.pieces : INT_MAX;
+  const int C = (int)min(max(want, (long long)PT_MIN), (long long)INT_MAX);
+  int np = 0, ns = 0;
+  for (int i = 0; i < a.per; ++i) {
+    const int b = lane * a.per + i;
+    if (b < a.r.rows) {
+      const int2 k = paged_tiles(a, paged_span(a.r, b));
+      const int s = k.y > C ? (k.y - 1) / C + 1 : 1;
+      np += k.x * s;
+      ns += s > 1 ? k.x * s : 0;
+    }
+  }
+  int before = np, slots = ns;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(FULL, before, o), z = __shfl_up_sync(FULL, slots, o);
+    if (lane >= o) {
+      before += y;
+      slots += z;
+    }
+  }
+  const int total = __shfl_sync(FULL, before, 31);
+  before -= np;
+  slots -= ns;
+  if (leave) {                          // for the merge
+    int at = slots;
+    for (int i = 0; i < a.per; ++i) {
+      const int b = lane * a.per + i;
+      if (b < a.r.rows) {
+        const int2 k = paged_tiles(a, paged_span(a.r, b));
+        const int s = k.y > C ? (k.y - 1) / C + 1 : 1;
+        a.own[b] = make_int2(at, s);
+        at += s > 1 ? k.x * s : 0;
+      }
+    }
+  }
+  PagedPiece p{-1, 0, 0, 1, 0};
+  if (x >= total) return p;
+  const int owner = 31 - __clz(__ballot_sync(FULL, before <= x));   // empty lanes share a count: the last of them
+  before = __shfl_sync(FULL, before, owner);
+  slots = __shfl_sync(FULL, slots, owner);
+  for (int b = owner * a.per;; ++b) {
+    const int2 k = paged_tiles(a, paged_span(a.r, b));
+    const int s = k.y > C ? (k.y - 1) / C + 1 : 1;
+    if (x < before + k.x * s) {
+      const int rem = x - before;
+      p.b = b, p.qt = k.x - 1 - rem / s, p.i = rem % s, p.s = s, p.slot = slots + rem;
+      return p;
+    }
+    before += k.x * s;
+    slots += s > 1 ? k.x * s : 0;
+  }
+}
 
 // One token and head over its visible keys, one at a time: four dims a lane; the row in bf16.
-__device__ uint2 paged_one(const PagedAttendArgs& a, int b, int p, int hq, const bf16* q) {
+// (A row that saw nothing, or whose output is not finite.)
+__device__ __noinline__ uint2 paged_one(const PagedAttendArgs& a, int b, int p, int hq, const bf16* q) {
   const int lane = threadIdx.x & 31, h = hq / a.G;
   const LongRow row = long_row((long long)p + 1, 0, a.r.S, a.window, a.sinks);
   const unsigned char *kb = a.pool.k + h * a.pool.k_sh + 8 * lane, *vb = a.pool.v + h * a.pool.v_sh + 8 * lane;
@@ -41,7 +168,7 @@ __device__ uint2 paged_one(const PagedAttendArgs& a, int b, int p, int hq, const
     const float s = a.scale * warp_sum(lo_f(qw.x) * lo_f(kw.x) + hi_f(qw.x) * hi_f(kw.x) + lo_f(qw.y) * lo_f(kw.y) +
                                        hi_f(qw.y) * hi_f(kw.y));
     const float mn = fmaxf(m, s), f = m > -INFINITY ? ex2(m - mn) : 0.f;
-    const float w = mn > -INFINITY ? ex2(s - mn + PT_SHIFT) : (s == -INFINITY ? 0.f : s);
+    const float w = mn > -INFINITY ? ex2(s - mn + LP_SHIFT) : (s == -INFINITY ? 0.f : s);
     m = mn;
     sum = sum * f + w;
     o[0] = o[0] * f + w * lo_f(vw.x);
@@ -53,18 +180,403 @@ __device__ uint2 paged_one(const PagedAttendArgs& a, int b, int p, int hq, const
   return make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
 }
 
-__global__ void __launch_bounds__(128) paged_attend_kernel(const __grid_constant__ PagedAttendArgs a) {
-  const int i = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+__global__ void __launch_bounds__(LP_THREADS, 2) paged_attend_kernel(const __grid_constant__ PagedAttendArgs a) {
+  extern __shared__ __align__(16) unsigned char raw[];
+  unsigned char* sq = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);   // Q; the output tile at the end
+  unsigned char* sk = sq + LP_Q;                                          // [2]
+  unsigned char* sv = sk + 2 * LP_KV;                                     // [2]
+  __shared__ __align__(8) uint64_t bar_k[2], bar_v[2], bar_s[2], bar_f, bar_p[2], bar_o[2];
+  __shared__ uint32_t tslot;
+  __shared__ PagedPiece s_piece;
+  __shared__ int s_bad;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int x = blockIdx.x / a.NKV, h = blockIdx.x - x * a.NKV;
   pdl_wait();
   pdl_trigger();
-  const int t = i / a.NH, hq = i - t * a.NH;
+  if (warp == 5) {
+    const PagedPiece p = paged_plan(a, x, lane, blockIdx.x == 0 && a.pieces > 0);
+    if (lane == 0) s_piece = p;
+  }
+  if (tid == 0) s_bad = 0;
+  __syncthreads();
+  const PagedPiece piece = s_piece;
+  if (piece.b < 0) return;
+  const PagedSpan span = paged_span(a.r, piece.b);
+  const int q0 = piece.qt * a.nq, nt = min(a.nq, span.n - q0);      // the tile's tokens
+  const int p_lo = span.p0 + q0, p_hi = p_lo + nt - 1;
+  const int live = nt * a.G, warps = (live + 31) >> 5;
+  const PagedSegs seg = paged_segs(a, p_lo, p_hi);
+  const int all = (seg.n + 1) >> 1;
+  const int first = (int)((long long)all * piece.i / piece.s), tiles = (int)((long long)all * (piece.i + 1) / piece.s) - first;
+  const int segs = seg.n - 2 * first;               // segments from the piece's first tile on
+  const int* table = a.t.table + piece.b * a.t.table_sb;
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bar_k[i], 1);
+      mbar_init(&bar_v[i], 1);
+      mbar_init(&bar_s[i], 1);
+      mbar_init(&bar_p[i], 32 * warps);
+      mbar_init(&bar_o[i], 1);
+    }
+    mbar_init(&bar_f, 32 * warps);
+    fence_mbar_init();
+    for (const CUtensorMap* m : {&a.tq, &a.tk, &a.tv, &a.tks, &a.tvs})
+      asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
+  }
+  if (warp == 4) tc_alloc(&tslot, LP_COLS);
+  tc_before();
+  __syncthreads();
+  tc_after();
+  const uint32_t tmem = tslot, t_o = tmem + 128;
+  // whether any row of the tile sees a slot of [j, j + n)
+  auto seen = [&](int j, int n) { return j <= p_hi && (j + n > seg.lo || j < a.sinks); };
+
+  if (warp == 4) {                                 // copies: one thread; the warp holds the entries of 16 tiles
+    const int small = min(a.t.page, LP_SEG);       // slots of a small box
+    // lane 4 i + c: the page of quarter c (16 slots) of tile 8 g + i of the piece
+    auto entries = [&](int g) {
+      const int tl = 8 * g + (lane >> 2);
+      int e = -1;
+      if (tl < tiles) {
+        const int sg = 2 * (first + tl) + ((lane >> 1) & 1), j = seg.at(sg) + 16 * (lane & 1);
+        // of a page that any row sees a slot of: a box may begin before the first of them
+        if (sg < seg.n && j < a.r.S && seen(j & -a.t.page, a.t.page)) e = table[j >> a.t.shift];
+      }
+      return (unsigned)e < (unsigned)a.t.pages ? e : a.t.pages;   // past the pool: zeros
+    };
+    int e0 = entries(0), e1 = entries(1);
+    auto load = [&](bool is_v, int t) {
+      const int n = min(2, segs - 2 * t), e = (t >> 3) & 1 ? e1 : e0;
+      int pg[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) pg[c] = __shfl_sync(FULL, e, ((t & 7) << 2) + c);
+      if (lane == 0) {
+        uint64_t* bar = is_v ? &bar_v[t & 1] : &bar_k[t & 1];
+        unsigned char* dst = (is_v ? sv : sk) + (t & 1) * LP_KV;
+        mbar_arrive_expect_tx(bar, (unsigned)(n * (LP_KV / 2) + (!is_v && t == 0 ? LP_Q : 0)));
+        const int j0 = seg.at(2 * (first + t)), mask = a.t.page - 1;
+        if (n == 2 && a.t.page >= LP_TILE && (j0 & (LP_TILE - 1)) == 0 && 2 * (first + t) != seg.ns - 1) {
+          lp_load(dst, is_v ? &a.tv : &a.tk, j0 & mask, 0, h, pg[0], bar);
+        } else {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            if ((c >> 1) < n && (small == LP_SEG ? (c & 1) == 0 : true)) {
+              const int j = seg.at(2 * (first + t) + (c >> 1)) + 16 * (c & 1);
+              for (int half = 0; half < 2; ++half)
+                lp_load(dst + half * (LP_KV / 2) + c * (LP_KV / 8), is_v ? &a.tvs : &a.tks, j & mask, half, h, pg[c], bar);
+            }
+        }
+        if (!is_v && t == 0)
+          asm volatile(
+              "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+              "[%6];" ::"r"(smem_u32(sq)),
+              "l"(&a.tq), "r"(0), "r"(h * a.G), "r"(span.t0 + q0), "r"(0), "r"(smem_u32(bar))
+              : "memory");
+      }
+      __syncwarp();
+    };
+    int nk = 0, nv = 0;                            // tiles copied
+    uint64_t since = 0;
+    while (nk < tiles || nv < tiles) {
+      // K and V each as soon as their buffer is free (S of t - 2 has read its K, P V of t - 2 its V)
+      const bool k = __shfl_sync(FULL, nk < tiles && (nk < 2 || mbar_test(&bar_s[nk & 1], ((nk - 2) >> 1) & 1)), 0);
+      if (k) load(false, nk++);
+      const bool v = __shfl_sync(FULL, nv < tiles && (nv < 2 || mbar_test(&bar_o[nv & 1], ((nv - 2) >> 1) & 1)), 0);
+      if (v) {
+        load(true, nv++);
+        // V has passed a group of eight tiles, so K has: the next group but one takes its place
+        if ((nv & 7) == 0) {
+          if ((nv >> 3) & 1) e0 = entries((nv >> 3) + 1);
+          else e1 = entries((nv >> 3) + 1);
+        }
+      }
+      if (k || v) {
+        since = 0;
+      } else if (since == 0) {
+        since = globaltimer();
+      } else if (__any_sync(FULL, globaltimer() - since > WAIT_LIMIT_NS)) {
+        set_error(a.err, FB_ERR_TIMEOUT);
+        break;
+      }
+    }
+    // no copy may be in flight when the CTA ends (after a wait that gave up: nobody else waits for them)
+    for (int t = max(0, nk - 2); t < nk; ++t) lp_wait_warp(&bar_k[t & 1], (t >> 1) & 1, a.err);
+    for (int t = max(0, nv - 2); t < nv; ++t) lp_wait_warp(&bar_v[t & 1], (t >> 1) & 1, a.err);
+  } else if (warp == 5) {                          // S: one thread
+    const uint64_t dq = tc_desc_sw128(smem_u32(sq)), dk = tc_desc_sw128(smem_u32(sk));
+    auto step = [&](auto buf, int t) -> bool {
+      constexpr int B = decltype(buf)::value;
+      if (!lp_wait(&bar_k[B], (t >> 1) & 1, a.err)) return false;
+      if (t >= 1 && !lp_wait(&bar_f, (t - 1) & 1, a.err)) return false;   // the last tile's scores are in registers
+      tc_after();
+      const uint32_t idesc = segs - 2 * t >= 2 ? tc_idesc(2 * LP_SEG) : tc_idesc(LP_SEG);
+#pragma unroll
+      for (int s = 0; s < LG_D / 16; ++s)
+        tc_mma(tmem, dq + (((s >> 2) * (LP_Q / 2) + (s & 3) * 32) >> 4),
+               dk + ((B * LP_KV + (s >> 2) * (LP_KV / 2) + (s & 3) * 32) >> 4), s > 0, idesc);
+      tc_commit(&bar_s[B]);
+      return true;
+    };
+    if (lane == 0)
+      for (int t = 0; t < tiles; t += 2)
+        if (!step(std::integral_constant<int, 0>(), t) ||
+            (t + 1 < tiles && !step(std::integral_constant<int, 1>(), t + 1)))
+          break;
+    __syncwarp();
+  } else if (warp == 6) {                          // P V
+    const uint64_t dv = tc_desc(smem_u32(sv), LP_KV / 2, 1024, 2);   // dims contiguous: two halves of 64, 8-key groups
+    auto step = [&](auto buf, int t) -> bool {
+      constexpr int B = decltype(buf)::value;
+      if (!lp_wait_warp(&bar_v[B], (t >> 1) & 1, a.err)) return false;
+      bool zeroed = false;
+      for (int s = 0; s < 2 && 2 * t + s < segs; ++s) {              // slots that no row of the tile sees
+        const int j0 = seg.at(2 * (first + t) + s);
+        const uint32_t see = lp_bits(seg.lo - j0, p_hi + 1 - j0) | lp_bits(0, min(a.sinks, p_hi + 1) - j0);
+        if (see == FULL) continue;
+        zeroed = true;
+        unsigned char* z = sv + B * LP_KV + s * (LP_KV / 4);
+        for (int i = lane; i < LP_SEG * 16; i += 32)
+          if (!((see >> (i >> 4)) & 1u))
+            *reinterpret_cast<uint4*>(z + ((i >> 3) & 1) * (LP_KV / 2) + (i >> 4) * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+      }
+      if (zeroed) {
+        fence_proxy_async();
+        __syncwarp();
+      }
+      if (!lp_wait_warp(&bar_p[B], (t >> 1) & 1, a.err)) return false;
+      tc_after();
+      if (lane == 0) {
+        constexpr uint32_t idesc = tc_idesc(LG_D) | (1u << 16);   // V: dims contiguous
+        const bool half = segs - 2 * t < 2;
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+          if (s < 2 || !half)
+            lp_mma_ts(t_o, tmem + 64 + 32 * B + 8 * s, dv + ((B * LP_KV + 2048 * s) >> 4), idesc, s > 0 || t > 0);
+        tc_commit(&bar_o[B]);
+      }
+      __syncwarp();
+      return true;
+    };
+    for (int t = 0; t < tiles; t += 2)
+      if (!step(std::integral_constant<int, 0>(), t) || (t + 1 < tiles && !step(std::integral_constant<int, 1>(), t + 1)))
+        break;
+  } else if (warp < warps) {
+    const int r = tid, l = r / a.G;
+    const bool mine = r < live;
+    const int p = mine ? p_lo + l : -1;                     // a row without a token sees nothing
+    const uint32_t my = (uint32_t)(warp * 32) << 16;
+    const int wnd = a.window > 0 ? a.window : 0x40000000;   // none: more than any row has
+    const uint64_t scale2 = f2(a.scale, a.scale);
+    // entries that are no page, among those of the piece's slots that are seen
+    for (int i = tid; i < 4 * tiles; i += 32 * warps) {
+      const int sg = 2 * first + (i >> 1), j = seg.at(sg) + 16 * (i & 1);
+      if (sg < seg.n && j < a.r.S && seen(j, 16) && (unsigned)table[j >> a.t.shift] >= (unsigned)a.t.pages) s_bad = 1;
+    }
+    named_sync(1, 32 * warps);
+    const bool holes = s_bad != 0;
+    float m = -INFINITY;
+    uint64_t sum2[2] = {0, 0};
+    bool ok = true;
+    for (int t = 0; t < tiles; ++t) {
+      ok = lp_wait_warp(&bar_s[t & 1], (t >> 1) & 1, a.err);
+      if (!ok) break;
+      tc_after();
+      float s[LP_TILE];
+      lp_ld64(tmem + my, s);                       // half a tile: the rest is old scores, past every p and masked below
+      tc_before();
+      mbar_arrive(&bar_f);
+#pragma unroll
+      for (int sg = 0; sg < 2; ++sg) {
+        const int j0 = seg.at(2 * (first + t) + sg);
+        if (j0 + LP_SEG - 1 > p_lo || (p_hi - j0 >= wnd && j0 + LP_SEG > a.sinks) || live < 32 * warps || holes) {
+          // the row's keys of the segment as bits: slots p - window + 1 .. p and the sinks
+          uint32_t see = lp_bits(p - wnd + 1 - j0, p + 1 - j0) | lp_bits(0, min(p + 1, a.sinks) - j0);
+          if (holes) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const int j = j0 + 16 * c;
+              if (j < a.r.S && seen(j, 16) && (unsigned)table[j >> a.t.shift] >= (unsigned)a.t.pages) see &= ~(0xffffu << (16 * c));
+            }
+          }
+#pragma unroll
+          for (int c = 0; c < LP_SEG; ++c) s[LP_SEG * sg + c] = (see >> c) & 1u ? s[LP_SEG * sg + c] : -INFINITY;
+        }
+      }
+      float x[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+      for (int c = 4; c < 64; c += 4) {
+        x[(c >> 2) & 3] = max3(x[(c >> 2) & 3], s[c], s[c + 1]);
+        x[((c >> 2) + 2) & 3] = max3(x[((c >> 2) + 2) & 3], s[c + 2], s[c + 3]);
+      }
+      // scale > 0 (checked): the maximum of the scaled scores
+      const float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * a.scale;
+      const bool up = mx > m + LP_SLACK;
+      if (__any_sync(FULL, up)) {
+        const float mn = up ? mx : m, f = up ? (m > -INFINITY ? ex2(m - mn) : 0.f) : 1.f;
+        m = mn;
+        const float2 u = f2_get(f2_add(sum2[0], sum2[1]));
+        sum2[0] = f2(u.x * f, u.y * f);
+        sum2[1] = 0;
+        if (t > 0) {
+          ok = lp_wait_warp(&bar_o[(t - 1) & 1], ((t - 1) >> 1) & 1, a.err);
+          if (!ok) break;
+          tc_after();
+#pragma unroll 1
+          for (int c = 0; c < LG_D; c += 32) {
+            float o[32];
+            lp_ld32(t_o + my + c, o);
+            uint32_t w[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(o[i] * f);
+            lp_st32(t_o + my + c, w);
+          }
+        }
+      }
+      // P's buffer: free once P V of t - 2 is done (asked here, needed after the exponentials)
+      const bool free = t < 2 || mbar_test(&bar_o[t & 1], ((t - 2) >> 1) & 1);
+      const float off = m > -INFINITY ? LP_SHIFT - m : 0.f;
+      const uint64_t off2 = f2(off, off);
+      uint32_t w[32];
+#pragma unroll
+      for (int c = 0; c < 32; ++c) {
+        const float2 e = f2_get(f2_fma(f2(s[2 * c], s[2 * c + 1]), scale2, off2));
+        const float p0 = ex2(e.x), p1 = ex2(e.y);
+        sum2[c & 1] = f2_add(sum2[c & 1], f2(p0, p1));
+        w[c] = pack_bf16(p0, p1);
+      }
+      if (!__all_sync(FULL, free)) {
+        ok = lp_wait_warp(&bar_o[t & 1], ((t - 2) >> 1) & 1, a.err);
+        if (!ok) break;
+      }
+      tc_after();
+      lp_st32(tmem + my + 64 + 32 * (t & 1), w);
+      tc_before();
+      mbar_arrive(&bar_p[t & 1]);
+    }
+    if (ok && tiles > 1) ok = lp_wait_warp(&bar_o[tiles & 1], ((tiles - 2) >> 1) & 1, a.err);
+    if (ok && tiles > 0) ok = lp_wait_warp(&bar_o[(tiles - 1) & 1], ((tiles - 1) >> 1) & 1, a.err);
+    tc_after();
+    const float2 u = f2_get(f2_add(sum2[0], sum2[1]));
+    const float sum = u.x + u.y;
+    if (piece.s > 1) {
+      // ---- a piece: the row's part, unnormalised
+      const long long at = (long long)piece.slot * a.NKV + h;
+      if (mine) a.ml[at * LP_ROWS + r] = make_float2(m, sum);
+      float* po = a.po + (at * LP_ROWS + r) * LG_D;
+#pragma unroll 1
+      for (int c = 0; c < LG_D; c += 32) {
+        float o[32];
+        if (tiles > 0 && ok) {
+          lp_ld32(t_o + my + c, o);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0.f;
+        }
+        if (mine) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(po + c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+        }
+      }
+    } else {
+      // ---- the whole row, through shared memory (over Q, with its swizzle) to 16-byte stores of whole rows
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      const uint64_t inv2 = f2(inv, inv);
+      uint64_t odd = 0;                              // becomes NaN with the first value that is not finite
+#pragma unroll 1
+      for (int c = 0; c < LG_D; c += 32) {
+        float o[32];
+        if (tiles > 0 && ok) {
+          lp_ld32(t_o + my + c, o);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0.f;
+        }
+        uint32_t w[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const uint64_t x = f2(o[2 * i], o[2 * i + 1]);
+          odd = f2_fma(x, 0, odd);
+          const float2 y = f2_get(f2_fma(x, inv2, 0));
+          w[i] = pack_bf16(y.x, y.y);
+        }
+        unsigned char* d = sq + (c >> 6) * (LP_Q / 2) + r * 128;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<uint4*>(d + (((((c & 63) >> 3) + i) ^ (r & 7)) << 4)) =
+              make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+      }
+      const float2 od = f2_get(odd);
+      const bool bad = !isfinite(sum) || !(od.x + od.y == 0.f) || sum == 0.f;
+      __syncwarp();
+      const int half = lane >> 4, c = lane & 15;
+#pragma unroll 4
+      for (int i = 0; i < 32; i += 2) {
+        const int rr = warp * 32 + i + half, ll = rr / a.G, gg = rr - ll * a.G;
+        const uint4 y = *reinterpret_cast<const uint4*>(sq + (c >> 3) * (LP_Q / 2) + rr * 128 + (((c & 7) ^ (rr & 7)) << 4));
+        if (rr < live && ok)
+          *reinterpret_cast<uint4*>(a.out + (long long)(span.t0 + q0 + ll) * a.o_st + (h * a.G + gg) * a.o_sh + 8 * c) = y;
+      }
+      // rows that are not finite, or saw nothing: the warp, a row at a time
+      for (unsigned todo = __ballot_sync(FULL, bad && ok && mine); todo; todo &= todo - 1) {
+        const int rr = warp * 32 + __ffs(todo) - 1, ll = rr / a.G, hq = h * a.G + rr - ll * a.G;
+        const long long t = span.t0 + q0 + ll;
+        const uint2 y = paged_one(a, piece.b, p_lo + ll, hq, a.q + t * a.q_st + hq * a.q_sh);
+        *reinterpret_cast<uint2*>(a.out + t * a.o_st + hq * a.o_sh + 4 * lane) = y;
+      }
+    }
+  }
+  tc_before();
+  __syncthreads();
+  if (warp == 4) {
+    tc_after();
+    tc_dealloc(tmem, LP_COLS);
+  }
+}
+
+// Joins the pieces of the query tiles that were cut, in their order: a warp per token and head.
+__global__ void __launch_bounds__(128) paged_merge_kernel(const __grid_constant__ PagedAttendArgs a) {
+  const int i = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int t = i / a.NH, hq = i - t * a.NH, h = hq / a.G;
+  pdl_wait();
+  pdl_trigger();
   if (t >= a.r.T) return;
   const int b = paged_row(a.r, t);
   if (b < 0) return;
-  const long long len = min(max(a.r.lengths[b], 0ll), (long long)a.r.S);
-  const int p = (int)(len - paged_left(a.r, b, t));
-  const uint2 w = paged_one(a, b, p, hq, a.q + t * a.q_st + hq * a.q_sh);
-  *reinterpret_cast<uint2*>(a.out + t * a.o_st + hq * a.o_sh + 4 * lane) = w;
+  const int2 own = a.own[b];
+  if (own.y <= 1) return;
+  const PagedSpan span = paged_span(a.r, b);
+  const int l = t - span.t0;
+  if (l < 0 || l >= span.n) return;      // offsets that decrease
+  const int qt = l / a.nq, tiles = (span.n + a.nq - 1) / a.nq;
+  const long long at = (long long)(own.x + (tiles - 1 - qt) * own.y) * a.NKV + h;
+  const int r = (l - qt * a.nq) * a.G + hq - h * a.G;
+  const float2* ml = a.ml + at * LP_ROWS + r;
+  const float* po = a.po + (at * LP_ROWS + r) * LG_D + 4 * lane;
+  const long long step = (long long)a.NKV * LP_ROWS;
+  float M = -INFINITY, L = 0.f;
+  for (int s = lane; s < own.y; s += 32) M = fmaxf(M, ml[s * step].x);
+  M = warp_max(M);
+  for (int s = lane; s < own.y; s += 32) {
+    const float2 x = ml[s * step];
+    L += x.x > -INFINITY ? ex2(x.x - M) * x.y : x.y;     // nothing, or a NaN
+  }
+  L = warp_sum(L);
+  float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int s = 0; s < own.y; ++s) {
+    const float m = ml[s * step].x;
+    const float4 x = *reinterpret_cast<const float4*>(po + s * step * LG_D);
+    const float f = m > -INFINITY ? ex2(m - M) : 0.f;
+    O.x += f * x.x;
+    O.y += f * x.y;
+    O.z += f * x.z;
+    O.w += f * x.w;
+  }
+  const float f = 1.f / L;
+  uint2 y = make_uint2(pack_bf16(O.x * f, O.y * f), pack_bf16(O.z * f, O.w * f));
+  const bool bad = L == 0.f || !isfinite(L) || !isfinite(O.x + O.y + O.z + O.w);
+  if (__any_sync(FULL, bad)) y = paged_one(a, b, span.p0 + l, hq, a.q + t * a.q_st + hq * a.q_sh);
+  *reinterpret_cast<uint2*>(a.out + t * a.o_st + hq * a.o_sh + 4 * lane) = y;
 }
 
 }  // namespace fb
@@ -82,13 +594,55 @@ int paged_group(const fb_paged_cache* c, int NH) {
   return FB_OK;
 }
 
+// CTAs wanted: what the SMs hold, twice, so that pieces of unequal size even out.  By the device's SMs, not the calling
+// thread's budget: the workspace's size goes by it.
+constexpr int PT_WAVES = 2;
+struct PagedPlan {
+  int pieces;                           // a KV head, 0: query tiles stay whole
+  int64_t ctas, slots, off_ml, off_own, ws_floats;
+};
+int paged_plan_host(const fb_paged_cache* c, int rows, int width, int T, int NH, int window, int sinks, PagedPlan* p) {
+  const int nq = LP_ROWS / (NH / c->NKV);
+  const int64_t S = (int64_t)width * c->page, runs = rows < T ? rows : T;
+  const int64_t units = (T + runs * (nq - 1)) / nq;                // query tiles, at most
+  // key tiles of a query tile, at most
+  int64_t keys = S;
+  if (window > 0 && (int64_t)window + sinks + nq + 3 * LP_SEG < S) keys = (int64_t)window + sinks + nq + 3 * LP_SEG;
+  const int64_t most = (keys + LP_TILE - 1) / LP_TILE;
+  p->pieces = most > PT_MIN ? (2 * PT_WAVES * fbh::num_sms() + c->NKV - 1) / c->NKV : 0;
+  p->ctas = (units + p->pieces) * c->NKV;
+  FB_CHECK_ARG(p->ctas <= 0x7fffffff, "paged_attend: too many tokens, rows and heads");
+  p->slots = 2ll * p->pieces * c->NKV;  // a cut query tile's pieces are at most twice its share of the work
+  if (p->slots > p->ctas) p->slots = p->ctas;
+  p->off_ml = p->slots * LP_ROWS * LG_D;
+  p->off_own = p->off_ml + p->slots * LP_ROWS * 2;
+  p->ws_floats = p->pieces ? p->off_own + 2 * (int64_t)rows : 0;
+  return FB_OK;
+}
+
+// The pool as (64 dims, slots, half, heads, pages); boxes of 64 slots x both halves, or of `rows` x one.
+int paged_map(CUtensorMap* m, const PagedPool& c, bool v, int rows) {
+  const unsigned long long dims[5] = {64, (unsigned long long)c.page, 2, (unsigned long long)c.NKV, (unsigned long long)c.pages};
+  const unsigned long long st[4] = {(unsigned long long)(v ? c.v_sl : c.k_sl), 128,
+                                    (unsigned long long)(c.NKV > 1 ? (v ? c.v_sh : c.k_sh) : 2 * LG_D),
+                                    (unsigned long long)(c.pages > 1 ? (v ? c.v_sb : c.k_sb) : 2 * LG_D)};
+  const unsigned bx[5] = {64, (unsigned)rows, rows == LP_TILE ? 2u : 1u, 1, 1};
+  return fbh::tmap_bf16(m, v ? c.v : c.k, 5, dims, st, bx);
+}
+
 }  // namespace
 
 extern "C" int64_t flashb_paged_attend_ws_floats(const fb_paged_cache* cache, int rows, int width, int T, int NH,
                                                  int window, int sinks) {
   PagedPool pool;
+  PagedPlan p{};
   if (fbh::paged_pool(cache, &pool) || fbh::paged_width(cache, rows, width) || paged_group(cache, NH)) return -1;
-  return 0;
+  if (T < 1 || sinks < 0) {
+    fbh::set_msg("paged_attend: bad shape T=%d sinks=%d", T, sinks);
+    return -1;
+  }
+  if (paged_plan_host(cache, rows, width, T, NH, window, sinks, &p)) return -1;
+  return p.ws_floats;
 }
 
 extern "C" int flashb_paged_attend(const fb_paged_cache* cache, const int32_t* table, int64_t table_sb, int rows, int width,
@@ -109,6 +663,8 @@ extern "C" int flashb_paged_attend(const fb_paged_cache* cache, const int32_t* t
                "paged_attend: tensors must be 16-byte aligned with strides multiple of 8 elements");
   FB_CHECK_ARG((T == 1 || (q_st > 0 && o_st > 0)) && (NH == 1 || (q_sh > 0 && o_sh > 0)),
                "paged_attend: strides must be positive");
+  FB_CHECK_ARG((cache->pages == 1 || (cache->k_sb > 0 && cache->v_sb > 0)) && (cache->NKV == 1 || (cache->k_sh > 0 && cache->v_sh > 0)),
+               "paged_attend: strides of the cache must be positive");
   FB_CHECK_ARG(!fbh::long_box_folds(fbh::long_box(out, 1, T, NH, 0, 2 * o_st, 2 * o_sh, 2 * LG_D)),
                "paged_attend: rows of out share memory");
   a.t = PagedTable{table, table_sb, a.pool.pages, a.pool.page, a.pool.shift};
@@ -116,8 +672,43 @@ extern "C" int flashb_paged_attend(const fb_paged_cache* cache, const int32_t* t
   a.q = (const bf16*)q, a.q_st = q_st, a.q_sh = q_sh, a.NH = NH, a.G = NH / cache->NKV;
   a.window = window > 0 && window < a.r.S ? window : 0, a.sinks = sinks < a.r.S ? sinks : a.r.S;
   a.scale = scaling * LG_LOG2E, a.out = (bf16*)out, a.o_st = o_st, a.o_sh = o_sh;
-  (void)ws, (void)ws_floats;
+  PagedPlan p{};
+  rc = paged_plan_host(cache, rows, width, T, NH, window, sinks, &p);
+  if (rc) return rc;
+  FB_CHECK_ARG(p.ws_floats == 0 || (ws && ((uintptr_t)ws & 15) == 0 && ws_floats >= p.ws_floats),
+               "paged_attend: workspace of %lld floats, %lld needed", (long long)ws_floats, (long long)p.ws_floats);
+  a.NKV = cache->NKV, a.nq = LP_ROWS / a.G, a.per = (rows + 31) / 32, a.pieces = p.pieces;
+  a.po = ws, a.ml = (float2*)(ws + p.off_ml), a.own = (int2*)(ws + p.off_own);
+  a.err = fbh::device_err_ptr();
+  const unsigned long long qd[4] = {64, (unsigned long long)NH, (unsigned long long)T, 2};
+  const unsigned long long qs[3] = {(unsigned long long)(NH > 1 ? q_sh : LG_D) * 2, (unsigned long long)(T > 1 ? q_st : LG_D) * 2, 128};
+  const unsigned qb[4] = {64, (unsigned)a.G, (unsigned)a.nq, 2};
+  rc = fbh::tmap_bf16(&a.tq, q, 4, qd, qs, qb);
+  const int small = cache->page < LP_SEG ? cache->page : LP_SEG;
+  if (!rc) rc = paged_map(&a.tks, a.pool, false, small);
+  if (!rc) rc = paged_map(&a.tvs, a.pool, true, small);
+  if (cache->page >= LP_TILE) {
+    if (!rc) rc = paged_map(&a.tk, a.pool, false, LP_TILE);
+    if (!rc) rc = paged_map(&a.tv, a.pool, true, LP_TILE);
+  } else {
+    a.tk = a.tks, a.tv = a.tvs;          // not used
+  }
+  if (rc) return rc;
+  static int attr_done[64] = {0};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 64 || !attr_done[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(paged_attend_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, LP_SMEM);
+    if (e != cudaSuccess) {
+      fbh::set_msg("paged_attend: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+      return FB_ERR_CUDA;
+    }
+    if (dev < 64) attr_done[dev] = 1;
+  }
   void* args[] = {(void*)&a};
-  return fbh::launch_pdl((const void*)paged_attend_kernel, dim3((unsigned)(((int64_t)T * NH + 3) / 4)), dim3(128), 0,
+  rc = fbh::launch_pdl((const void*)paged_attend_kernel, dim3((unsigned)p.ctas), dim3(LP_THREADS), LP_SMEM,
+                       (cudaStream_t)stream, args, true);
+  if (rc || !p.pieces) return rc;
+  return fbh::launch_pdl((const void*)paged_merge_kernel, dim3((unsigned)(((int64_t)T * NH + 3) / 4)), dim3(128), 0,
                          (cudaStream_t)stream, args, true);
 }
