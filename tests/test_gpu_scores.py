@@ -57,6 +57,36 @@ def test_ties_go_to_the_lowest_id():
     check(x.bfloat16(), t, 32)
 
 
+def test_rows_whose_largest_logits_crowd():
+    """Equal, rising and falling rows; the largest in one thread's vectors; few ids that are not suppressed."""
+    V = 20000
+    x = torch.zeros(7, V)
+    x[1] = torch.arange(V) / 1000
+    x[2] = -x[1]
+    x[3, ::2048] = torch.arange(10, dtype=torch.float32)
+    x[4] = torch.randn(V, generator=torch.Generator().manual_seed(1))
+    x[4, 5000:7000] = 9.0
+    x[5] = float('-inf')
+    x[5, [7, 19999, 4000]] = torch.tensor([1.0, 2.0, 1.0])
+    x[6, -3:] = 30.0
+    t = torch.tensor([3, 19999, 0, 2048, 6000, 4000, 19998])
+    check(x, t, 32)
+    check(x, t, 1)
+    check(x[:, 1:], t - 1, 20)
+    check(x.bfloat16(), t, 20)
+    check(x.bfloat16()[:, 3:], t - 3, 5, 0.5)
+
+
+def test_large_logits():
+    x = 100 * torch.randn(4, 2500, generator=torch.Generator().manual_seed(9))
+    x[1] *= 1e4
+    x[2] *= 1e18
+    x[3] *= 1e30
+    t = torch.tensor([1, 2, 3, 4])
+    check(x, t, 6)
+    check(x, t, 6, 0.01)
+
+
 def test_suppressed_ids_and_rows_without_a_distribution():
     inf, nan = float('inf'), float('nan')
     x = torch.randn(8, 300, generator=torch.Generator().manual_seed(2))
