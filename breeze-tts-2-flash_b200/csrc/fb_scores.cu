@@ -17,7 +17,9 @@
 //
 // Rows that the fast path cannot take go through scores_slow, a pass per alternative: a NaN or +inf, -inf alone, logits
 // past 2^60, more than SC_CAP logits at the threshold (rows of equal logits), fewer finite logits than alternatives.
+#include <cfloat>
 #include <climits>
+#include <cstdlib>
 
 #include "fb_long.cuh"
 #include "fb_sample.cuh"
@@ -26,7 +28,7 @@ namespace fb {
 
 constexpr int SC_MAX = 512;             // threads of a CTA, at most
 constexpr int SC_CAP = 1024;            // logits collected for the alternatives
-constexpr float SC_LOW = -1e6f;         // 2 to it is 0; what -inf is taken for in e (x c - R)
+constexpr float SC_LOW = -0x1p100f;     // what -inf is taken for in e (x c - R); a largest logit below it: the slow path
 constexpr float SC_LN2 = 0.6931471805599453f;
 
 struct ScoresArgs {
@@ -122,16 +124,37 @@ __device__ __noinline__ void scores_slow(const ScoresArgs& a, int r) {
   }
 }
 
-__device__ __forceinline__ float max_nan(float a, float b) {       // a NaN stays
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+// The largest of the 16 bytes' logits.
+template <typename T>
+__device__ __forceinline__ float score_max(const uint4& w) {
+  if constexpr (sizeof(T) == 4) {
+    return fmaxf(fmaxf(__uint_as_float(w.x), __uint_as_float(w.y)), fmaxf(__uint_as_float(w.z), __uint_as_float(w.w)));
+  } else {
+    uint32_t m;
+    asm("{\n\t.reg .b32 a, b;\n\tmax.bf16x2 a, %1, %2;\n\tmax.bf16x2 b, %3, %4;\n\tmax.bf16x2 %0, a, b;\n\t}"
+        : "=r"(m)
+        : "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w));
+    return fmaxf(lo_f(m), hi_f(m));
+  }
+}
+// Logits below SC_LOW (-inf) as SC_LOW; a NaN stays.
+template <typename T>
+__device__ __forceinline__ uint32_t score_clamp(uint32_t w) {
+  uint32_t r;
+  if constexpr (sizeof(T) == 4) asm("max.NaN.f32 %0, %1, %2;" : "=r"(r) : "r"(w), "r"(__float_as_uint(SC_LOW)));
+  else asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(w), "r"((__float_as_uint(SC_LOW) >> 16) * 0x10001u));
   return r;
 }
 
+// A unit: 32 bytes of logits.
+struct ScoreUnit {
+  uint4 w[2];
+};
+
 template <typename T>
 __global__ void __launch_bounds__(SC_MAX, 2) scores_kernel(const __grid_constant__ ScoresArgs a) {
-  constexpr int N = 16 / sizeof(T);                      // logits of a vector
-  constexpr int UNROLL = 4;
+  constexpr int N = 32 / sizeof(T);                      // logits of a unit
+  constexpr int UNROLL = 2;
   __shared__ unsigned s_max[SC_MAX / 32], s_thr[SC_MAX / 32];
   __shared__ float s_sum[SC_MAX / 32], s_dot[SC_MAX / 32];
   __shared__ int s_cnt[SC_MAX / 32], s_n;
@@ -143,33 +166,40 @@ __global__ void __launch_bounds__(SC_MAX, 2) scores_kernel(const __grid_constant
   const T* x = reinterpret_cast<const T*>(a.x) + (long long)r * a.ld;
   const long long token = a.tokens[r];
   const bool known = token >= 0 && token < a.V;
-  const float xt = known ? score_at(x, (int)token) : INFINITY;
-  // logits before the first 16-byte boundary and behind the last whole vector: one each for the first threads ("vector -1")
-  const int head = min(a.V, (int)(((16u - ((unsigned)(uintptr_t)x & 15u)) & 15u) / sizeof(T)));
-  const int nv = (a.V - head) / N, odd = a.V - nv * N;
-  const int mine = tid < odd ? (tid < head ? tid : nv * N + tid) : -1;   // the thread's odd logit
-  const T* body = x + head;
+  const int tok = known ? (int)token : 0;
+  const float xt = known ? score_at(x, tok) + 0.f : INFINITY, above = known ? ord2f(f2ord(xt) + 1) : NAN;   // the next number
+  // logits before the first 32-byte boundary and behind the last whole unit: one each for the first threads ("unit -1")
+  const int head = min(a.V, (int)(((32u - ((unsigned)(uintptr_t)x & 31u)) & 31u) / sizeof(T)));
+  const int nu = (a.V - head) / N, odd = a.V - nu * N;
+  const int mine = tid < odd ? (tid < head ? tid : nu * N + tid) : -1;   // the thread's odd logit
+  const uint4* body = reinterpret_cast<const uint4*>(x + head);
 
   const float c = a.c;
-  float R = -0x1p100f, sum = 0.f, dot = 0.f, bs = 0.f, bd = 0.f, tm = -INFINITY, tm2 = -INFINITY;
-  int iv = -2, cnt = 0;                                  // iv: the vector that holds tm (-2: none)
-  auto unpack = [&](const uint4& w, float (&f)[N]) {
-    if constexpr (N == 8) {
-      cvt8(w, f);
+  const uint64_t c2 = f2(c, c);
+  float R = -0x1p100f, sum = 0.f, dot = 0.f, bs = 0.f, bd = 0.f, tm = -INFINITY, tm2 = -INFINITY, tm3 = -INFINITY;
+  int iu = -2, iu2 = -2, cnt = 0;                        // the units that hold tm and tm2 (-2: none)
+  ScoreUnit best;
+  best.w[0] = best.w[1] = make_uint4(0, 0, 0, 0);
+  // f(pair of logits, the first one's place in the unit)
+  auto pairs = [&](const ScoreUnit& u, auto f) {
+    const uint32_t w[8] = {u.w[0].x, u.w[0].y, u.w[0].z, u.w[0].w, u.w[1].x, u.w[1].y, u.w[1].z, u.w[1].w};
+    if constexpr (N == 16) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f(lo_f(w[i]), hi_f(w[i]), 2 * i);
     } else {
-      f[0] = __uint_as_float(w.x), f[1] = __uint_as_float(w.y), f[2] = __uint_as_float(w.z), f[3] = __uint_as_float(w.w);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]), 2 * i);
     }
   };
-  // e and e y of one logit
-  auto term = [&](float v, float& s, float& d) {
-    const float y = max_nan(fmaf(v, c, -R), SC_LOW), e = ex2(y);
-    s += e;
-    d = fmaf(e, y, d);
-  };
-  auto feed = [&](const float (&f)[N], int v, int base) {
-    float vm = fmaxf(f[0], f[1]);
+  auto clamped = [&](const ScoreUnit& u) {
+    ScoreUnit o;
 #pragma unroll
-    for (int i = 2; i < N; ++i) vm = fmaxf(vm, f[i]);
+    for (int i = 0; i < 2; ++i)
+      o.w[i] = make_uint4(score_clamp<T>(u.w[i].x), score_clamp<T>(u.w[i].y), score_clamp<T>(u.w[i].z), score_clamp<T>(u.w[i].w));
+    return o;
+  };
+  auto feed = [&](const ScoreUnit& raw, int v, int base) {
+    const float vm = fmaxf(score_max<T>(raw.w[0]), score_max<T>(raw.w[1]));
     if (vm * c > R + 16.f) {
       const float n = vm * c, g = ex2(R - n), by = R - n;
       dot = g * fmaf(by, sum, dot);
@@ -178,55 +208,60 @@ __global__ void __launch_bounds__(SC_MAX, 2) scores_kernel(const __grid_constant
       bs *= g;
       R = n;
     }
-    const uint64_t c2 = f2(c, c), r2 = f2(-R, -R);
+    const uint64_t r2 = f2(-R, -R);
     uint64_t s2 = 0, d2 = 0;
-#pragma unroll
-    for (int i = 0; i < N; i += 2) {
-      const float2 y = f2_get(f2_fma(f2(f[i], f[i + 1]), c2, r2));
-      const float y0 = max_nan(y.x, SC_LOW), y1 = max_nan(y.y, SC_LOW);
-      const uint64_t e = f2(ex2(y0), ex2(y1));
+    pairs(clamped(raw), [&](float p, float q, int) {
+      const uint64_t y2 = f2_fma(f2(p, q), c2, r2);
+      const float2 y = f2_get(y2);
+      const uint64_t e = f2(ex2(y.x), ex2(y.y));
       s2 = f2_add(s2, e);
-      d2 = f2_fma(e, f2(y0, y1), d2);
-    }
+      d2 = f2_fma(e, y2, d2);
+    });
     const float2 s = f2_get(s2), d = f2_get(d2);
     const float vs = s.x + s.y, vd = d.x + d.y;
-    const bool nb = vm > tm;
+    const bool nb = vm > tm, nb2 = vm > tm2;
     sum += nb ? bs : vs;
     dot += nb ? bd : vd;
     bs = nb ? vs : bs;
     bd = nb ? vd : bd;
-    tm2 = nb ? tm : fmaxf(tm2, vm);
+    if (nb) best = raw;
+    tm3 = fmaxf(tm3, fminf(tm2, vm));
+    tm2 = fmaxf(tm2, fminf(tm, vm));
     tm = fmaxf(tm, vm);
-    iv = nb ? v : iv;
+    iu2 = nb ? iu : nb2 ? v : iu2;
+    iu = nb ? v : iu;
     if (vm >= xt) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) cnt += f[i] > xt || (f[i] == xt && base + i < token);
+      const float th = base + N <= tok ? xt : above;
+      pairs(raw, [&](float p, float q, int) { cnt += (p >= th) + (q >= th); });
+      if (base <= tok && tok < base + N)                 // equal logits of lower ids
+        pairs(raw, [&](float p, float q, int i) { cnt += (p == xt && base + i < tok) + (q == xt && base + i + 1 < tok); });
     }
   };
-  const uint4* vec = reinterpret_cast<const uint4*>(body);
-  for (int v0 = tid; v0 < nv; v0 += UNROLL * step) {
-    uint4 w[UNROLL];
+  auto unit = [&](int v) {
+    ScoreUnit u;
+    if (v >= 0) {
+      u.w[0] = body[2 * v];
+      u.w[1] = body[2 * v + 1];
+    } else {                                             // the odd logit, and -inf
+      const uint32_t none = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u, f = __float_as_uint(score_at(x, mine));
+      u.w[0] = u.w[1] = make_uint4(none, none, none, none);
+      u.w[0].x = sizeof(T) == 4 ? f : 0xff800000u | f >> 16;
+    }
+    return u;
+  };
+  for (int v0 = tid; v0 < nu; v0 += UNROLL * step) {
+    ScoreUnit u[UNROLL];
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u)
-      if (v0 + u * step < nv) w[u] = vec[v0 + u * step];
+    for (int i = 0; i < UNROLL; ++i)
+      if (v0 + i * step < nu) u[i] = unit(v0 + i * step);
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u)
-      if (v0 + u * step < nv) {
-        float f[N];
-        unpack(w[u], f);
-        feed(f, v0 + u * step, head + (v0 + u * step) * N);
-      }
+    for (int i = 0; i < UNROLL; ++i)
+      if (v0 + i * step < nu) feed(u[i], v0 + i * step, head + (v0 + i * step) * N);
   }
-  if (mine >= 0) {
-    float f[N];
-    f[0] = score_at(x, mine);
-#pragma unroll
-    for (int i = 1; i < N; ++i) f[i] = -INFINITY;
-    feed(f, -1, mine);
-  }
+  if (mine >= 0) feed(unit(-1), -1, mine);
 
   // ---- the maximum and the threshold
-  const unsigned key = iv == -2 ? 0u : f2ord(tm + 0.f);
+  const unsigned key = iu == -2 ? 0u : f2ord(tm + 0.f);
   {
     const unsigned top = __reduce_max_sync(FULL, key);
     unsigned k = key, at = top;
@@ -241,55 +276,55 @@ __global__ void __launch_bounds__(SC_MAX, 2) scores_kernel(const __grid_constant
     }
   }
   __syncthreads();
-  unsigned M = 0, thr = 0xffffffffu;
-  int holder = 0;
-  for (int w = 0; w < W; ++w) {
-    if (s_max[w] > M) M = s_max[w], holder = w;
-    thr = min(thr, s_thr[w]);
-  }
+  const unsigned wm = lane < W ? s_max[lane] : 0u, M = __reduce_max_sync(FULL, wm);
+  const unsigned thr = __reduce_min_sync(FULL, lane < W ? s_thr[lane] : 0xffffffffu);
+  const int holder = __ffs(__ballot_sync(FULL, wm == M)) - 1;
   const float xm = ord2f(M), hi = xm * c, lo = fmaf(xm, c, -hi);
-  bool fast = M != 0 && fabsf(hi) < 0x1p60f;
+  bool fast = M != 0 && xm > SC_LOW && fabsf(hi) < 0x1p60f;
   const bool owner = warp == holder && lane == __ffs(__ballot_sync(FULL, key == M)) - 1;
   if (fast) {
-    // ---- the vectors that reach the threshold, and the largest's without its own 1
-    if ((a.top > 0 && key >= thr && iv != -2) || owner) {
-      bool skip = owner;
-      auto collect = [&](float v, int id) {
-        const unsigned k = f2ord(v + 0.f);
-        if (a.top > 0 && k >= thr && v > -INFINITY) {     // a vector of -inf alone is not looked at again, so none is collected
-          const int n = atomicAdd(&s_n, 1);
-          if (n < SC_CAP) s_key[n] = ((unsigned long long)k << 32) | (0xffffffffu - (unsigned)id);
-        }
+    // ---- the units that reach the threshold, and the largest's without its own 1
+    const bool wanted = a.top > 0 && key >= thr && iu != -2;
+    if (wanted) {
+      // logits that reach the threshold; a unit of -inf alone is not looked at again, so none is collected
+      const float low = fmaxf(ord2f(max(thr, 0x007fffffu)), -FLT_MAX);
+      auto collect = [&](const ScoreUnit& u, int v) {
+        const int base = v == -1 ? mine : head + v * N;
+        auto put = [&](float f, int id) {
+          if (f >= low) {
+            const int n = atomicAdd(&s_n, 1);
+            if (n < SC_CAP) s_key[n] = ((unsigned long long)f2ord(f + 0.f) << 32) | (0xffffffffu - (unsigned)id);
+          }
+        };
+        pairs(u, [&](float p, float q, int i) {
+          put(p, base + i);
+          put(q, base + i + 1);
+        });
       };
-      if (owner) bs = bd = 0.f;
-      auto again = [&](int v) {                          // the largest's vector
-        if (v == -1) {
-          const float f = score_at(x, mine);
-          collect(f, mine);
-        } else {
-          float f[N];
-          unpack(vec[v], f);
-#pragma unroll
-          for (int i = 0; i < N; ++i) {
-            collect(f[i], head + v * N + i);
-            if (owner) {
-              if (skip && f[i] == xm) skip = false;
-              else term(f[i], bs, bd);
-            }
+      collect(best, iu);
+      if (tm2 >= low) {
+        collect(unit(iu2), iu2);
+        if (tm3 >= low) {
+          for (int v = mine >= 0 ? -1 : tid; v < nu; v = v == -1 ? tid : v + step) {
+            if (v == iu || v == iu2) continue;
+            const ScoreUnit u = unit(v);
+            if (fmaxf(score_max<T>(u.w[0]), score_max<T>(u.w[1])) >= low) collect(u, v);
           }
         }
-      };
-      again(iv);
-      if (a.top > 0 && iv != -2 && tm2 > -INFINITY && f2ord(tm2 + 0.f) >= thr) {
-        for (int v = tid; v < nv; v += step)
-          if (v != iv) {
-            float f[N];
-            unpack(vec[v], f);
-#pragma unroll
-            for (int i = 0; i < N; ++i) collect(f[i], head + v * N + i);
-          }
-        if (mine >= 0 && iv != -1) collect(score_at(x, mine), mine);
       }
+    }
+    if (owner) {
+      bool skip = true;
+      bs = bd = 0.f;
+      pairs(clamped(best), [&](float p, float q, int) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float f = i ? q : p, y = fmaf(f, c, -R), e = skip && f == xm ? 0.f : ex2(y);
+          skip = skip && f != xm;
+          bs += e;
+          bd = fmaf(e, y, bd);
+        }
+      });
     }
     const float by = (hi - R) + lo, g = ex2(-by), all = sum + bs;
     float rest = g * all, ent = g * fmaf(by, all, -(dot + bd));
@@ -306,11 +341,9 @@ __global__ void __launch_bounds__(SC_MAX, 2) scores_kernel(const __grid_constant
   float rest = 0.f, ent = 0.f;
   int before = 0;
   if (fast) {
-    for (int w = 0; w < W; ++w) {
-      rest += s_sum[w];
-      ent += s_dot[w];
-      before += s_cnt[w];
-    }
+    rest = warp_sum(lane < W ? s_sum[lane] : 0.f);
+    ent = warp_sum(lane < W ? s_dot[lane] : 0.f);
+    before = __reduce_add_sync(FULL, lane < W ? s_cnt[lane] : 0);
     fast = rest == rest && s_n <= SC_CAP && s_n >= a.top;   // fewer: -inf among the alternatives
   }
   if (!fast) {
@@ -354,9 +387,10 @@ extern "C" int flashb_token_scores(const void* logits, int is_bf16, int64_t ld, 
   a.logprob = logprob, a.entropy = entropy, a.top_logprob = top_logprob;
   a.rank = (long long*)rank, a.top_id = (long long*)top_id;
   // two vectors a thread or more, up to the CTA's limit
-  const int vectors = V / (is_bf16 ? 8 : 4);
+  const int vectors = V / (is_bf16 ? 16 : 8);
+  const int most = getenv("SC_T") ? atoi(getenv("SC_T")) : SC_MAX;
   int threads = 32;
-  while (threads < SC_MAX && threads * 4 <= vectors) threads *= 2;
+  while (threads < most && threads * 4 <= vectors) threads *= 2;
   void* args[] = {(void*)&a};
   return fbh::launch_pdl(is_bf16 ? (const void*)scores_kernel<uint16_t> : (const void*)scores_kernel<float>, dim3(rows),
                          dim3(threads), 0, (cudaStream_t)stream, args, true);
