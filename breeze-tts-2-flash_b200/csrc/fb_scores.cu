@@ -5,21 +5,25 @@
 //   rank = how many ids come before the token, top = the first k ids and their log probabilities,
 // where ids are ordered by logit, equal ones by id, a NaN first (the greedy sampler's order).
 //
-// Bound: the row is read once from memory.  A CTA per row, 16-byte loads; a thread keeps, over its vectors,
+// Bound: the row is read once from memory, and an exponential a logit takes three quarters of that time.  A CTA per row,
+// units of 32 bytes; a thread keeps, over its units,
 //   the sums of e = 2^(x c - R) and of e (x c - R) with c = log2(e) / temperature and a reference R of its own, which moves
-//   only when a vector's maximum passes it by 2^16 (the sums are exact either way);
-//   the two largest vector maxima, and which vector holds the largest, whose sums are kept apart.
+//   only when a unit's maximum passes it by 2^16 (the sums are exact either way);
+//   the three largest unit maxima, which units hold the first two, and the first one's sums apart from the rest.
 // The block's threshold for the alternatives is the least of the warps' k / W-th largest thread maxima: at least k logits
-// reach it.  Only vectors that reach it are read again (from L1 or L2; mostly one each of some tens of threads), what they
+// reach it.  Only units that reach it are read again (from L1 or L2; mostly one each of some tens of threads), what they
 // hold of it is collected, and each of those finds its place by counting the others above it.
-// The largest logit's own 1 stays out of the sum (its vector's sum is worked out again without it): what the others add to
+// The largest logit's own 1 stays out of the sum (its unit's sum is worked out again without it): what the others add to
 // an almost certain token's 1 is not rounded away.
+//
+// Measured on a B200 (in a CUDA graph): 4095 rows of 32003 in bf16 with 20 alternatives (262 MB) 79 us, 0.51 of the measured
+// copy bandwidth; 1088 rows of 2049 in fp32 with 8 (9 MB) 6.6 us; 17 rows 3.9 us.  The first is bound by issue (0.7 of the
+// slots; some 8 instructions a logit, 1 of them an exponential); without alternatives it takes 62 us.
 //
 // Rows that the fast path cannot take go through scores_slow, a pass per alternative: a NaN or +inf, -inf alone, logits
 // past 2^60, more than SC_CAP logits at the threshold (rows of equal logits), fewer finite logits than alternatives.
 #include <cfloat>
 #include <climits>
-#include <cstdlib>
 
 #include "fb_long.cuh"
 #include "fb_sample.cuh"
@@ -154,7 +158,6 @@ struct ScoreUnit {
 template <typename T>
 __global__ void __launch_bounds__(SC_MAX, 2) scores_kernel(const __grid_constant__ ScoresArgs a) {
   constexpr int N = 32 / sizeof(T);                      // logits of a unit
-  constexpr int UNROLL = 2;
   __shared__ unsigned s_max[SC_MAX / 32], s_thr[SC_MAX / 32];
   __shared__ float s_sum[SC_MAX / 32], s_dot[SC_MAX / 32];
   __shared__ int s_cnt[SC_MAX / 32], s_n;
@@ -164,10 +167,6 @@ __global__ void __launch_bounds__(SC_MAX, 2) scores_kernel(const __grid_constant
   pdl_wait();
   pdl_trigger();
   const T* x = reinterpret_cast<const T*>(a.x) + (long long)r * a.ld;
-  const long long token = a.tokens[r];
-  const bool known = token >= 0 && token < a.V;
-  const int tok = known ? (int)token : 0;
-  const float xt = known ? score_at(x, tok) + 0.f : INFINITY, above = known ? ord2f(f2ord(xt) + 1) : NAN;   // the next number
   // logits before the first 32-byte boundary and behind the last whole unit: one each for the first threads ("unit -1")
   const int head = min(a.V, (int)(((32u - ((unsigned)(uintptr_t)x & 31u)) & 31u) / sizeof(T)));
   const int nu = (a.V - head) / N, odd = a.V - nu * N;
@@ -178,8 +177,6 @@ __global__ void __launch_bounds__(SC_MAX, 2) scores_kernel(const __grid_constant
   const uint64_t c2 = f2(c, c);
   float R = -0x1p100f, sum = 0.f, dot = 0.f, bs = 0.f, bd = 0.f, tm = -INFINITY, tm2 = -INFINITY, tm3 = -INFINITY;
   int iu = -2, iu2 = -2, cnt = 0;                        // the units that hold tm and tm2 (-2: none)
-  ScoreUnit best;
-  best.w[0] = best.w[1] = make_uint4(0, 0, 0, 0);
   // f(pair of logits, the first one's place in the unit)
   auto pairs = [&](const ScoreUnit& u, auto f) {
     const uint32_t w[8] = {u.w[0].x, u.w[0].y, u.w[0].z, u.w[0].w, u.w[1].x, u.w[1].y, u.w[1].z, u.w[1].w};
@@ -198,6 +195,25 @@ __global__ void __launch_bounds__(SC_MAX, 2) scores_kernel(const __grid_constant
       o.w[i] = make_uint4(score_clamp<T>(u.w[i].x), score_clamp<T>(u.w[i].y), score_clamp<T>(u.w[i].z), score_clamp<T>(u.w[i].w));
     return o;
   };
+  auto unit = [&](int v) {
+    ScoreUnit u;
+    if (v >= 0) {
+      u.w[0] = body[2 * v];
+      u.w[1] = body[2 * v + 1];
+    } else {                                             // the odd logit, and -inf
+      const uint32_t none = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u, f = __float_as_uint(score_at(x, mine));
+      u.w[0] = u.w[1] = make_uint4(none, none, none, none);
+      u.w[0].x = sizeof(T) == 4 ? f : 0xff800000u | f >> 16;
+    }
+    return u;
+  };
+  // the next unit is under way while one is worked on; the first before the token, whose logit is a load behind a load
+  ScoreUnit next;
+  if (tid < nu) next = unit(tid);
+  const long long token = a.tokens[r];
+  const bool known = token >= 0 && token < a.V;
+  const int tok = known ? (int)token : 0;
+  const float xt = known ? score_at(x, tok) + 0.f : INFINITY, above = known ? ord2f(f2ord(xt) + 1) : NAN;   // the next number
   auto feed = [&](const ScoreUnit& raw, int v, int base) {
     const float vm = fmaxf(score_max<T>(raw.w[0]), score_max<T>(raw.w[1]));
     if (vm * c > R + 16.f) {
@@ -224,7 +240,6 @@ __global__ void __launch_bounds__(SC_MAX, 2) scores_kernel(const __grid_constant
     dot += nb ? bd : vd;
     bs = nb ? vs : bs;
     bd = nb ? vd : bd;
-    if (nb) best = raw;
     tm3 = fmaxf(tm3, fminf(tm2, vm));
     tm2 = fmaxf(tm2, fminf(tm, vm));
     tm = fmaxf(tm, vm);
@@ -237,26 +252,10 @@ __global__ void __launch_bounds__(SC_MAX, 2) scores_kernel(const __grid_constant
         pairs(raw, [&](float p, float q, int i) { cnt += (p == xt && base + i < tok) + (q == xt && base + i + 1 < tok); });
     }
   };
-  auto unit = [&](int v) {
-    ScoreUnit u;
-    if (v >= 0) {
-      u.w[0] = body[2 * v];
-      u.w[1] = body[2 * v + 1];
-    } else {                                             // the odd logit, and -inf
-      const uint32_t none = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u, f = __float_as_uint(score_at(x, mine));
-      u.w[0] = u.w[1] = make_uint4(none, none, none, none);
-      u.w[0].x = sizeof(T) == 4 ? f : 0xff800000u | f >> 16;
-    }
-    return u;
-  };
-  for (int v0 = tid; v0 < nu; v0 += UNROLL * step) {
-    ScoreUnit u[UNROLL];
-#pragma unroll
-    for (int i = 0; i < UNROLL; ++i)
-      if (v0 + i * step < nu) u[i] = unit(v0 + i * step);
-#pragma unroll
-    for (int i = 0; i < UNROLL; ++i)
-      if (v0 + i * step < nu) feed(u[i], v0 + i * step, head + (v0 + i * step) * N);
+  for (int v = tid; v < nu; v += step) {
+    const ScoreUnit u = next;
+    if (v + step < nu) next = unit(v + step);
+    feed(u, v, head + v * N);
   }
   if (mine >= 0) feed(unit(-1), -1, mine);
 
@@ -301,9 +300,10 @@ __global__ void __launch_bounds__(SC_MAX, 2) scores_kernel(const __grid_constant
           put(q, base + i + 1);
         });
       };
-      collect(best, iu);
+      const ScoreUnit u1 = unit(iu), u2 = unit(tm2 >= low ? iu2 : iu);
+      collect(u1, iu);
       if (tm2 >= low) {
-        collect(unit(iu2), iu2);
+        collect(u2, iu2);
         if (tm3 >= low) {
           for (int v = mine >= 0 ? -1 : tid; v < nu; v = v == -1 ? tid : v + step) {
             if (v == iu || v == iu2) continue;
@@ -316,7 +316,7 @@ __global__ void __launch_bounds__(SC_MAX, 2) scores_kernel(const __grid_constant
     if (owner) {
       bool skip = true;
       bs = bd = 0.f;
-      pairs(clamped(best), [&](float p, float q, int) {
+      pairs(clamped(unit(iu)), [&](float p, float q, int) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const float f = i ? q : p, y = fmaf(f, c, -R), e = skip && f == xm ? 0.f : ex2(y);
@@ -386,11 +386,12 @@ extern "C" int flashb_token_scores(const void* logits, int is_bf16, int64_t ld, 
   a.inv = 1.f / temperature, a.c = a.inv * LG_LOG2E;
   a.logprob = logprob, a.entropy = entropy, a.top_logprob = top_logprob;
   a.rank = (long long*)rank, a.top_id = (long long*)top_id;
-  // two vectors a thread or more, up to the CTA's limit
-  const int vectors = V / (is_bf16 ? 16 : 8);
-  const int most = getenv("SC_T") ? atoi(getenv("SC_T")) : SC_MAX;
+  // Two units a thread or more.  128 threads a row: more of them, with fewer units each, leave more logits at the threshold
+  // (4095 rows of 32003 in bf16: 94, 79, 89 and 128 us with 64, 128, 256 and 512 threads; occupancies of 8 to 12 such CTAs
+  // an SM 79 to 83).  Few rows leave SMs idle, so there a row has up to 512.
+  const int units = V / (is_bf16 ? 16 : 8), most = rows <= 2 * fbh::num_sms() ? SC_MAX : 128;
   int threads = 32;
-  while (threads < most && threads * 4 <= vectors) threads *= 2;
+  while (threads < most && threads * 4 <= units) threads *= 2;
   void* args[] = {(void*)&a};
   return fbh::launch_pdl(is_bf16 ? (const void*)scores_kernel<uint16_t> : (const void*)scores_kernel<float>, dim3(rows),
                          dim3(threads), 0, (cudaStream_t)stream, args, true);
