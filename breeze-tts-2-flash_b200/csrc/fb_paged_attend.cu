@@ -12,11 +12,13 @@
 // its slots get no weight.
 //
 // Pieces.  A step can be one run of a few tokens over a long row, or many rows of which some are long.  So the key tiles of
-// a query tile are cut into s pieces, s = ceil(k / C) with k its row's key tiles and C the work of the whole step over the
-// wanted number of CTAs; a CTA takes one piece.  Every CTA works the list out for itself from lengths and offsets (a warp,
-// some hundred cycles; no launch before it, nothing read on the host).  Pieces of a query tile leave (maximum, sum,
-// unnormalised out) in the workspace and paged_merge_kernel joins them in order: no atomics, the same inputs give the same
-// bits.  A query tile of one piece writes its rows itself.
+// a query tile are cut into s pieces, s = ceil(k / C) with k its row's key tiles; a CTA takes one piece.  paged_plan_kernel
+// (one CTA, from lengths and offsets on the device: nothing is read on the host) writes the list; C is chosen among those
+// with which the list fills one to PT_WAVES rounds of the SMs, and whole query tiles, by what the rounds take.  Pieces of a
+// query tile leave (maximum, sum, unnormalised out) in the workspace and paged_merge_kernel joins them in order: no atomics,
+// the same inputs give the same bits.  A query tile of one piece writes its rows itself.
+//
+// Rows of one token go through the single-token kernel (fb_long_decode.cu) where a row has few tokens on average.
 //
 // Slots that no row of the CTA sees may hold anything: in V they are zeroed in shared memory (0 times a NaN is NaN), in K
 // their scores are replaced.  A row whose output is not finite all the same (a NaN that another row of the tile sees) is
@@ -29,6 +31,10 @@
 namespace fb {
 
 constexpr int PT_MIN = 4;                         // key tiles of a piece, at least
+constexpr int PT_WAVES = 4;                       // rounds of CTAs that the list of pieces may be cut for
+constexpr int PT_COST = 5;                        // what beginning and ending a piece takes, in key tiles
+
+struct PagedPiece;
 
 struct alignas(64) PagedAttendArgs {
   CUtensorMap tq, tk, tv, tks, tvs;     // Q tile; K, V: boxes of 64 slots, and of 32 or 16 (half of the dims)
@@ -38,13 +44,17 @@ struct alignas(64) PagedAttendArgs {
   const bf16* q;
   long long q_st, q_sh;
   int NH, NKV, G, nq, window, sinks;    // nq = 128 / G tokens a CTA; window 0: none
-  int per, pieces;                      // rows per lane of the plan; CTAs wanted a KV head, 0: one piece a query tile
+  int lq;                               // log2 nq
+  int per, pieces, list, cuts;          // rows per thread of the plan; CTAs that the SMs hold a KV head, 0: query tiles stay
+  float rounds;                         // whole; entries of the list, of them cut at most; 1 / pieces
+  int singles;                          // rows of one token are another launch's
   float scale;                          // scaling x log2(e)
   bf16* out;
   long long o_st, o_sh;
   float* po;                            // pieces: unnormalised out [slot][128][128],
   float2* ml;                           //   maximum and sum [slot][128]
-  int2* own;                            // [row] the first slot and the pieces of a query tile (1: no slot)
+  PagedPiece* plan;                     // [list]
+  int4* cut;                            // [cuts / 2] query tiles of two pieces and more: first token, tokens, pieces, slot
   unsigned* err;
 };
 
@@ -72,80 +82,156 @@ __device__ __forceinline__ PagedSegs paged_segs(const PagedAttendArgs& a, int p_
   g.n = p_hi < 0 ? 0 : g.ns + (p_hi - g.base) / LP_SEG + 1;
   return g;
 }
-// A row's query tiles and the key tiles of its last one (the most that one has).
-__device__ __forceinline__ int2 paged_tiles(const PagedAttendArgs& a, const PagedSpan& x) {
-  if (x.n <= 0) return make_int2(0, 0);
+// A row's query tiles and the key tiles of its last one (the most that one has).  Not inlined, nor the plan's other parts
+// repeated: the plan is one pass over cold instructions, which cost it more than its arithmetic.
+__device__ __noinline__ int2 paged_tiles(const PagedAttendArgs& a, int b) {
+  const PagedSpan x = paged_span(a.r, b);
+  if (x.n <= 0 || (a.singles && x.n == 1)) return make_int2(0, 0);
   const int p_hi = x.p0 + x.n - 1;
-  return make_int2((x.n + a.nq - 1) / a.nq, (paged_segs(a, p_hi - min(x.n, a.nq) + 1, p_hi).n + 1) >> 1);
+  return make_int2((x.n + a.nq - 1) >> a.lq, (paged_segs(a, p_hi - min(x.n, a.nq) + 1, p_hi).n + 1) >> 1);
 }
 
-struct PagedPiece {
-  int b, qt, i, s, slot;                // row, query tile, piece i of s, its slot in the workspace; b = -1: none
+// Pieces of a query tile of k key tiles, about C = 1 / r in each.
+__device__ __forceinline__ int paged_cut(int k, float r) { return max(1, (int)ceilf((float)k * r)); }
+
+// Piece i of s of the tokens tok .. tok + nt - 1 of row b, the first at slot p_lo; slot: its place in the workspace.
+struct alignas(16) PagedPiece {
+  int b, tok, nt, p_lo, i, s, slot, pad;   // b = -1: none
 };
-// Number x of the list of pieces: rows in order, a row's latest query tiles first (they have the most keys).  One warp.
-__device__ __forceinline__ PagedPiece paged_plan(const PagedAttendArgs& a, int x, int lane, bool leave) {
-  long long w = 0;
-  for (int i = 0; i < a.per; ++i) {
-    const int b = lane * a.per + i;
-    if (b < a.r.rows) {
-      const int2 k = paged_tiles(a, paged_span(a.r, b));
-      w += (long long)k.x * k.y;
-    }
+
+constexpr int PP_THREADS = 256, PP_WARPS = PP_THREADS / 32;
+constexpr int PP_ROWS = 1024;              // rows whose tiles are kept in shared memory
+
+// The list: rows in order, a row's latest query tiles first (they have the most keys), a query tile's pieces in order.
+__global__ void __launch_bounds__(PP_THREADS) paged_plan_kernel(const __grid_constant__ PagedAttendArgs a) {
+  __shared__ int2 s_k[PP_ROWS];
+  __shared__ int s_units[PP_WARPS], s_longest[PP_WARPS], s_n[PT_WAVES][PP_WARPS], s_most[PT_WAVES][PP_WARPS];
+  __shared__ int s_before[PP_THREADS], s_slots[PP_THREADS], s_cut[PP_THREADS], s_w[PP_WARPS][3];
+  __shared__ float s_work[PP_WARPS];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  pdl_wait();
+  pdl_trigger();
+  const int b0 = tid * a.per, b1 = min(b0 + a.per, a.r.rows);
+  auto tiles = [&](int b) { return b < PP_ROWS ? s_k[b] : paged_tiles(a, b); };
+  // what there is: key tiles, query tiles, the longest row
+  float w = 0.f;
+  int units = 0, longest = 0;
+#pragma unroll 1
+  for (int b = b0; b < b1; ++b) {
+    const int2 k = paged_tiles(a, b);
+    if (b < PP_ROWS) s_k[b] = k;
+    w += (float)k.x * (float)k.y;
+    units += k.x;
+    longest = max(longest, k.y);
   }
+  float r = 0.f;                        // 1 / (key tiles of a piece), 0: query tiles stay whole
+  if (a.pieces > 0) {
+    w = warp_sum(w);
+    units = __reduce_add_sync(FULL, units);
+    longest = __reduce_max_sync(FULL, longest);
+    if (lane == 0) s_work[warp] = w, s_units[warp] = units, s_longest[warp] = longest;
+    __syncthreads();
+    w = warp_sum(lane < PP_WARPS ? s_work[lane] : 0.f);
+    units = __reduce_add_sync(FULL, lane < PP_WARPS ? s_units[lane] : 0);
+    longest = __reduce_max_sync(FULL, lane < PP_WARPS ? s_longest[lane] : 0);
+    // candidates: what a piece may hold for the list to fit that many rounds of the SMs
+    float c[PT_WAVES];
+    int n[PT_WAVES], most[PT_WAVES];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(FULL, w, o);
-  const long long want = a.pieces > 0 ? (w + a.pieces - 1) / a.pieces : INT_MAX;
-  const int C = (int)min(max(want, (long long)PT_MIN), (long long)INT_MAX);
-  int np = 0, ns = 0;
-  for (int i = 0; i < a.per; ++i) {
-    const int b = lane * a.per + i;
-    if (b < a.r.rows) {
-      const int2 k = paged_tiles(a, paged_span(a.r, b));
-      const int s = k.y > C ? (k.y - 1) / C + 1 : 1;
-      np += k.x * s;
-      ns += s > 1 ? k.x * s : 0;
+    for (int j = 0; j < PT_WAVES; ++j) {
+      const int room = (j + 1) * a.pieces - units;
+      c[j] = room > 0 ? fminf(__fdividef((float)room, w), 1.f / PT_MIN) : 0.f;
+      n[j] = most[j] = 0;
+    }
+#pragma unroll 1
+    for (int b = b0; b < b1; ++b) {
+      const int2 x = tiles(b);
+#pragma unroll
+      for (int j = 0; j < PT_WAVES; ++j) {
+        const int s = paged_cut(x.y, c[j]);
+        n[j] += x.x * s;
+        most[j] = max(most[j], (int)__fdividef((float)(x.y + s - 1), (float)s));
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < PT_WAVES; ++j) {
+      n[j] = __reduce_add_sync(FULL, n[j]);
+      most[j] = __reduce_max_sync(FULL, most[j]);
+      if (lane == 0) s_n[j][warp] = n[j], s_most[j][warp] = most[j];
+    }
+    __syncthreads();
+    // those and whole query tiles, each priced by its rounds x (its longest piece and the time that one takes to begin and
+    // end); the places in the workspace are enough for `cuts` pieces
+    float price = ceilf((float)units * a.rounds) * (float)(longest + PT_COST);
+#pragma unroll
+    for (int j = 0; j < PT_WAVES; ++j) {
+      const int count = __reduce_add_sync(FULL, lane < PP_WARPS ? s_n[j][lane] : 0);
+      const float len = (float)__reduce_max_sync(FULL, lane < PP_WARPS ? s_most[j][lane] : 0);
+      const float p = ceilf((float)count * a.rounds) * (len + PT_COST);
+      if (p < price && count <= a.cuts) price = p, r = c[j];
     }
   }
-  int before = np, slots = ns;
+  int np = 0, ns = 0, nc = 0;
+#pragma unroll 1
+  for (int b = b0; b < b1; ++b) {
+    const int2 k = tiles(b);
+    const int s = paged_cut(k.y, r);
+    np += k.x * s;
+    ns += s > 1 ? k.x * s : 0;
+    nc += s > 1 ? k.x : 0;
+  }
+  int before = np, slots = ns, cuts = nc;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(FULL, before, o), z = __shfl_up_sync(FULL, slots, o);
+    const int y = __shfl_up_sync(FULL, before, o), z = __shfl_up_sync(FULL, slots, o), v = __shfl_up_sync(FULL, cuts, o);
     if (lane >= o) {
       before += y;
       slots += z;
+      cuts += v;
     }
   }
-  const int total = __shfl_sync(FULL, before, 31);
-  before -= np;
-  slots -= ns;
-  if (leave) {                          // for the merge
-    int at = slots;
-    for (int i = 0; i < a.per; ++i) {
-      const int b = lane * a.per + i;
-      if (b < a.r.rows) {
-        const int2 k = paged_tiles(a, paged_span(a.r, b));
-        const int s = k.y > C ? (k.y - 1) / C + 1 : 1;
-        a.own[b] = make_int2(at, s);
-        at += s > 1 ? k.x * s : 0;
+  if (lane == 31) s_w[warp][0] = before, s_w[warp][1] = slots, s_w[warp][2] = cuts;
+  __syncthreads();
+  int total = 0, used = 0, joins = 0;
+#pragma unroll
+  for (int i = 0; i < PP_WARPS; ++i) {
+    if (i == warp) before += total, slots += used, cuts += joins;
+    total += s_w[i][0];
+    used += s_w[i][1];
+    joins += s_w[i][2];
+  }
+  s_before[tid] = before - np;
+  s_slots[tid] = slots - ns;
+  s_cut[tid] = cuts - nc;
+  __syncthreads();
+#pragma unroll 1
+  for (int x = tid; x < a.list; x += PP_THREADS) {
+    PagedPiece p{-1, 0, 0, 0, 0, 1, used, 0};
+    if (x < total) {
+      int o = 0;                        // the last thread whose pieces begin at x or before
+#pragma unroll 1
+      for (int h = PP_THREADS / 2; h > 0; h >>= 1)
+        if (s_before[o + h] <= x) o += h;
+      int at = s_before[o], slot = s_slots[o], join = s_cut[o], b = o * a.per, s, n;
+#pragma unroll 1
+      for (;; ++b) {
+        const int2 k = tiles(b);
+        s = paged_cut(k.y, r);
+        n = k.x * s;
+        if (x < at + n) break;
+        at += n;
+        slot += s > 1 ? n : 0;
+        join += s > 1 ? k.x : 0;
       }
+      const PagedSpan span = paged_span(a.r, b);
+      const int rem = x - at, u = rem / s, q0 = (n / s - 1 - u) << a.lq;
+      p = PagedPiece{b, span.t0 + q0, min(a.nq, span.n - q0), span.p0 + q0, rem - u * s, s, slot + rem, 0};
+      if (s > 1 && p.i == 0) a.cut[join + u] = make_int4(p.tok, p.nt, s, p.slot);
     }
+    *reinterpret_cast<int4*>(&a.plan[x]) = *reinterpret_cast<const int4*>(&p);
+    reinterpret_cast<int4*>(&a.plan[x])[1] = reinterpret_cast<const int4*>(&p)[1];
   }
-  PagedPiece p{-1, 0, 0, 1, 0};
-  if (x >= total) return p;
-  const int owner = 31 - __clz(__ballot_sync(FULL, before <= x));   // empty lanes share a count: the last of them
-  before = __shfl_sync(FULL, before, owner);
-  slots = __shfl_sync(FULL, slots, owner);
-  for (int b = owner * a.per;; ++b) {
-    const int2 k = paged_tiles(a, paged_span(a.r, b));
-    const int s = k.y > C ? (k.y - 1) / C + 1 : 1;
-    if (x < before + k.x * s) {
-      const int rem = x - before;
-      p.b = b, p.qt = k.x - 1 - rem / s, p.i = rem % s, p.s = s, p.slot = slots + rem;
-      return p;
-    }
-    before += k.x * s;
-    slots += s > 1 ? k.x * s : 0;
-  }
+  for (int x = joins + tid; x < a.cuts / 2; x += PP_THREADS) a.cut[x] = make_int4(0, 0, 0, 0);   // the merge's other CTAs
 }
 
 // One token and head over its visible keys, one at a time: four dims a lane; the row in bf16.
@@ -187,24 +273,25 @@ __global__ void __launch_bounds__(LP_THREADS, 2) paged_attend_kernel(const __gri
   unsigned char* sv = sk + 2 * LP_KV;                                     // [2]
   __shared__ __align__(8) uint64_t bar_k[2], bar_v[2], bar_s[2], bar_f, bar_p[2], bar_o[2];
   __shared__ uint32_t tslot;
-  __shared__ PagedPiece s_piece;
   __shared__ int s_bad;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int x = blockIdx.x / a.NKV, h = blockIdx.x - x * a.NKV;
-  pdl_wait();
-  pdl_trigger();
-  if (warp == 5) {
-    const PagedPiece p = paged_plan(a, x, lane, blockIdx.x == 0 && a.pieces > 0);
-    if (lane == 0) s_piece = p;
+  if (tid == 0) {
+    s_bad = 0;
+    for (const CUtensorMap* m : {&a.tq, &a.tk, &a.tv, &a.tks, &a.tvs})
+      asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
   }
-  if (tid == 0) s_bad = 0;
-  __syncthreads();
-  const PagedPiece piece = s_piece;
-  if (piece.b < 0) return;
-  const PagedSpan span = paged_span(a.r, piece.b);
-  const int q0 = piece.qt * a.nq, nt = min(a.nq, span.n - q0);      // the tile's tokens
-  const int p_lo = span.p0 + q0, p_hi = p_lo + nt - 1;
-  const int live = nt * a.G, warps = (live + 31) >> 5;
+  // With single tokens in a launch between the plan and this one, that launch began after the plan had ended; what it writes
+  // is not read here.  It is waited for at the end, so that it has ended when this one has.
+  if (!a.singles) pdl_wait();
+  pdl_trigger();
+  const PagedPiece piece = a.plan[x];
+  if (piece.b < 0) {
+    if (a.singles) pdl_wait();
+    return;
+  }
+  const int p_lo = piece.p_lo, p_hi = p_lo + piece.nt - 1;
+  const int live = piece.nt * a.G, warps = (live + 31) >> 5;
   const PagedSegs seg = paged_segs(a, p_lo, p_hi);
   const int all = (seg.n + 1) >> 1;
   const int first = (int)((long long)all * piece.i / piece.s), tiles = (int)((long long)all * (piece.i + 1) / piece.s) - first;
@@ -220,8 +307,6 @@ __global__ void __launch_bounds__(LP_THREADS, 2) paged_attend_kernel(const __gri
     }
     mbar_init(&bar_f, 32 * warps);
     fence_mbar_init();
-    for (const CUtensorMap* m : {&a.tq, &a.tk, &a.tv, &a.tks, &a.tvs})
-      asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
   }
   if (warp == 4) tc_alloc(&tslot, LP_COLS);
   tc_before();
@@ -232,7 +317,7 @@ __global__ void __launch_bounds__(LP_THREADS, 2) paged_attend_kernel(const __gri
   auto seen = [&](int j, int n) { return j <= p_hi && (j + n > seg.lo || j < a.sinks); };
 
   if (warp == 4) {                                 // copies: one thread; the warp holds the entries of 16 tiles
-    const int small = min(a.t.page, LP_SEG);       // slots of a small box
+    const int small = min(a.t.page, LP_SEG);       // slots of a small box: 32, or 16
     // lane 4 i + c: the page of quarter c (16 slots) of tile 8 g + i of the piece
     auto entries = [&](int g) {
       const int tl = 8 * g + (lane >> 2);
@@ -247,31 +332,25 @@ __global__ void __launch_bounds__(LP_THREADS, 2) paged_attend_kernel(const __gri
     int e0 = entries(0), e1 = entries(1);
     auto load = [&](bool is_v, int t) {
       const int n = min(2, segs - 2 * t), e = (t >> 3) & 1 ? e1 : e0;
-      int pg[4];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) pg[c] = __shfl_sync(FULL, e, ((t & 7) << 2) + c);
+      const int qc = (lane >> 1) & 3, pg = __shfl_sync(FULL, e, ((t & 7) << 2) + qc);   // lane 2 c + i: quarter c, half i
+      uint64_t* bar = is_v ? &bar_v[t & 1] : &bar_k[t & 1];
+      unsigned char* dst = (is_v ? sv : sk) + (t & 1) * LP_KV;
+      const int j0 = seg.at(2 * (first + t)), mask = a.t.page - 1;
       if (lane == 0) {
-        uint64_t* bar = is_v ? &bar_v[t & 1] : &bar_k[t & 1];
-        unsigned char* dst = (is_v ? sv : sk) + (t & 1) * LP_KV;
         mbar_arrive_expect_tx(bar, (unsigned)(n * (LP_KV / 2) + (!is_v && t == 0 ? LP_Q : 0)));
-        const int j0 = seg.at(2 * (first + t)), mask = a.t.page - 1;
-        if (n == 2 && a.t.page >= LP_TILE && (j0 & (LP_TILE - 1)) == 0 && 2 * (first + t) != seg.ns - 1) {
-          lp_load(dst, is_v ? &a.tv : &a.tk, j0 & mask, 0, h, pg[0], bar);
-        } else {
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-            if ((c >> 1) < n && (small == LP_SEG ? (c & 1) == 0 : true)) {
-              const int j = seg.at(2 * (first + t) + (c >> 1)) + 16 * (c & 1);
-              for (int half = 0; half < 2; ++half)
-                lp_load(dst + half * (LP_KV / 2) + c * (LP_KV / 8), is_v ? &a.tvs : &a.tks, j & mask, half, h, pg[c], bar);
-            }
-        }
         if (!is_v && t == 0)
           asm volatile(
               "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
               "[%6];" ::"r"(smem_u32(sq)),
-              "l"(&a.tq), "r"(0), "r"(h * a.G), "r"(span.t0 + q0), "r"(0), "r"(smem_u32(bar))
+              "l"(&a.tq), "r"(0), "r"(h * a.G), "r"(piece.tok), "r"(0), "r"(smem_u32(bar))
               : "memory");
+      }
+      if (n == 2 && a.t.page >= LP_TILE && (j0 & (LP_TILE - 1)) == 0 && 2 * (first + t) != seg.ns - 1) {
+        if (lane == 0) lp_load(dst, is_v ? &a.tv : &a.tk, j0 & mask, 0, h, pg, bar);
+      } else if ((qc >> 1) < n && lane < 8 && (small < LP_SEG || (qc & 1) == 0)) {
+        // a lane a box: one thread after the other takes 40 ns each
+        lp_load(dst + (lane & 1) * (LP_KV / 2) + qc * (LP_KV / 8), is_v ? &a.tvs : &a.tks,
+                (seg.at(2 * (first + t) + (qc >> 1)) + 16 * (qc & 1)) & mask, lane & 1, h, pg, bar);
       }
       __syncwarp();
     };
@@ -462,7 +541,8 @@ __global__ void __launch_bounds__(LP_THREADS, 2) paged_attend_kernel(const __gri
       // ---- a piece: the row's part, unnormalised
       const long long at = (long long)piece.slot * a.NKV + h;
       if (mine) a.ml[at * LP_ROWS + r] = make_float2(m, sum);
-      float* po = a.po + (at * LP_ROWS + r) * LG_D;
+      // through shared memory (K and V are read), so that a store is a whole row
+      unsigned char* st = sk + warp * (32 * LG_D * 4);
 #pragma unroll 1
       for (int c = 0; c < LG_D; c += 32) {
         float o[32];
@@ -472,11 +552,17 @@ __global__ void __launch_bounds__(LP_THREADS, 2) paged_attend_kernel(const __gri
 #pragma unroll
           for (int i = 0; i < 32; ++i) o[i] = 0.f;
         }
-        if (mine) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(po + c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-        }
+        for (int i = 0; i < 32; i += 4)
+          *reinterpret_cast<float4*>(st + lane * (LG_D * 4) + ((((c + i) >> 2) ^ lane) << 4)) =
+              make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
       }
+      __syncwarp();
+      float* po = a.po + (at * LP_ROWS + warp * 32) * LG_D + 4 * lane;
+      const int rows = min(32, live - warp * 32);
+#pragma unroll 4
+      for (int i = 0; i < rows; ++i)
+        *reinterpret_cast<float4*>(po + i * LG_D) = *reinterpret_cast<const float4*>(st + i * (LG_D * 4) + ((lane ^ i) << 4));
     } else {
       // ---- the whole row, through shared memory (over Q, with its swizzle) to 16-byte stores of whole rows
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -514,12 +600,12 @@ __global__ void __launch_bounds__(LP_THREADS, 2) paged_attend_kernel(const __gri
         const int rr = warp * 32 + i + half, ll = rr / a.G, gg = rr - ll * a.G;
         const uint4 y = *reinterpret_cast<const uint4*>(sq + (c >> 3) * (LP_Q / 2) + rr * 128 + (((c & 7) ^ (rr & 7)) << 4));
         if (rr < live && ok)
-          *reinterpret_cast<uint4*>(a.out + (long long)(span.t0 + q0 + ll) * a.o_st + (h * a.G + gg) * a.o_sh + 8 * c) = y;
+          *reinterpret_cast<uint4*>(a.out + (long long)(piece.tok + ll) * a.o_st + (h * a.G + gg) * a.o_sh + 8 * c) = y;
       }
       // rows that are not finite, or saw nothing: the warp, a row at a time
       for (unsigned todo = __ballot_sync(FULL, bad && ok && mine); todo; todo &= todo - 1) {
         const int rr = warp * 32 + __ffs(todo) - 1, ll = rr / a.G, hq = h * a.G + rr - ll * a.G;
-        const long long t = span.t0 + q0 + ll;
+        const long long t = piece.tok + ll;
         const uint2 y = paged_one(a, piece.b, p_lo + ll, hq, a.q + t * a.q_st + hq * a.q_sh);
         *reinterpret_cast<uint2*>(a.out + t * a.o_st + hq * a.o_sh + 4 * lane) = y;
       }
@@ -531,52 +617,64 @@ __global__ void __launch_bounds__(LP_THREADS, 2) paged_attend_kernel(const __gri
     tc_after();
     tc_dealloc(tmem, LP_COLS);
   }
+  if (a.singles) pdl_wait();
 }
 
-// Joins the pieces of the query tiles that were cut, in their order: a warp per token and head.
-__global__ void __launch_bounds__(128) paged_merge_kernel(const __grid_constant__ PagedAttendArgs a) {
-  const int i = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  const int t = i / a.NH, hq = i - t * a.NH, h = hq / a.G;
+// Joins the pieces of the query tiles that were cut, in their order: a CTA per PM_ROWS rows of a query tile and head (801
+// tokens of 32 rows, 3 pieces: 24 us with a CTA of 8 warps per tile and head), four rows a warp.
+constexpr int PM_ROWS = 16, PM_THREADS = 128;
+__global__ void __launch_bounds__(PM_THREADS) paged_merge_kernel(const __grid_constant__ PagedAttendArgs a) {
+  const int group = blockIdx.y, x = blockIdx.x / a.NKV, h = blockIdx.x - x * a.NKV, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
   pdl_trigger();
-  if (t >= a.r.T) return;
-  const int b = paged_row(a.r, t);
-  if (b < 0) return;
-  const int2 own = a.own[b];
-  if (own.y <= 1) return;
-  const PagedSpan span = paged_span(a.r, b);
-  const int l = t - span.t0;
-  if (l < 0 || l >= span.n) return;      // offsets that decrease
-  const int qt = l / a.nq, tiles = (span.n + a.nq - 1) / a.nq;
-  const long long at = (long long)(own.x + (tiles - 1 - qt) * own.y) * a.NKV + h;
-  const int r = (l - qt * a.nq) * a.G + hq - h * a.G;
-  const float2* ml = a.ml + at * LP_ROWS + r;
-  const float* po = a.po + (at * LP_ROWS + r) * LG_D + 4 * lane;
-  const long long step = (long long)a.NKV * LP_ROWS;
-  float M = -INFINITY, L = 0.f;
-  for (int s = lane; s < own.y; s += 32) M = fmaxf(M, ml[s * step].x);
-  M = warp_max(M);
-  for (int s = lane; s < own.y; s += 32) {
-    const float2 x = ml[s * step];
-    L += x.x > -INFINITY ? ex2(x.x - M) * x.y : x.y;     // nothing, or a NaN
+  const int4 cut = a.cut[x];
+  const int pieces = cut.z, live = min(cut.y * a.G, (group + 1) * PM_ROWS);
+  if (pieces == 0) return;
+  const long long at = (long long)cut.w * a.NKV + h, step = (long long)a.NKV * LP_ROWS;
+#pragma unroll 1
+  for (int r = group * PM_ROWS + warp; r < live; r += PM_THREADS / 32) {
+    const float2* ml = a.ml + at * LP_ROWS + r;
+    const float* po = a.po + (at * LP_ROWS + r) * LG_D + 4 * lane;
+    // four pieces at a time, their loads together
+    float M = -INFINITY, L = 0.f;
+    float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+    for (int s0 = 0; s0 < pieces; s0 += 4) {
+      float2 y[4];
+      float4 o[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int s = min(s0 + i, pieces - 1);
+        y[i] = ml[s * step];
+        o[i] = *reinterpret_cast<const float4*>(po + s * step * LG_D);
+      }
+      const float m = fmaxf(fmaxf(fmaxf(y[0].x, y[1].x), fmaxf(y[2].x, y[3].x)), M);
+      const float g = M > -INFINITY ? ex2(M - m) : 0.f;
+      M = m;
+      L *= g;
+      O.x *= g, O.y *= g, O.z *= g, O.w *= g;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (s0 + i < pieces) {
+          const float f = y[i].x > -INFINITY ? ex2(y[i].x - m) : 0.f;
+          L += y[i].x > -INFINITY ? f * y[i].y : y[i].y;     // nothing, or a NaN
+          O.x += f * o[i].x;
+          O.y += f * o[i].y;
+          O.z += f * o[i].z;
+          O.w += f * o[i].w;
+        }
+    }
+    const float f = 1.f / L;
+    uint2 y = make_uint2(pack_bf16(O.x * f, O.y * f), pack_bf16(O.z * f, O.w * f));
+    const int l = r / a.G, hq = h * a.G + r - l * a.G;
+    const long long t = cut.x + l;
+    if (__any_sync(FULL, L == 0.f || !isfinite(L) || !isfinite(O.x + O.y + O.z + O.w))) {
+      const int b = paged_row(a.r, (int)t);
+      const PagedSpan span = paged_span(a.r, b);
+      y = paged_one(a, b, span.p0 + (int)t - span.t0, hq, a.q + t * a.q_st + hq * a.q_sh);
+    }
+    *reinterpret_cast<uint2*>(a.out + t * a.o_st + hq * a.o_sh + 4 * lane) = y;
   }
-  L = warp_sum(L);
-  float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int s = 0; s < own.y; ++s) {
-    const float m = ml[s * step].x;
-    const float4 x = *reinterpret_cast<const float4*>(po + s * step * LG_D);
-    const float f = m > -INFINITY ? ex2(m - M) : 0.f;
-    O.x += f * x.x;
-    O.y += f * x.y;
-    O.z += f * x.z;
-    O.w += f * x.w;
-  }
-  const float f = 1.f / L;
-  uint2 y = make_uint2(pack_bf16(O.x * f, O.y * f), pack_bf16(O.z * f, O.w * f));
-  const bool bad = L == 0.f || !isfinite(L) || !isfinite(O.x + O.y + O.z + O.w);
-  if (__any_sync(FULL, bad)) y = paged_one(a, b, span.p0 + l, hq, a.q + t * a.q_st + hq * a.q_sh);
-  *reinterpret_cast<uint2*>(a.out + t * a.o_st + hq * a.o_sh + 4 * lane) = y;
 }
 
 }  // namespace fb
@@ -594,12 +692,13 @@ int paged_group(const fb_paged_cache* c, int NH) {
   return FB_OK;
 }
 
-// CTAs wanted: what the SMs hold, twice, so that pieces of unequal size even out.  By the device's SMs, not the calling
-// thread's budget: the workspace's size goes by it.
-constexpr int PT_WAVES = 2;
+// Rows of one token go through the single-token kernel, a launch of its own before this one, where a row has few tokens on
+// average: it reads their keys at 0.95 of the copy bandwidth where a tile of 128 rows, G of them in use, reaches 0.8.
+constexpr int PT_SINGLES = 32;
 struct PagedPlan {
   int pieces;                           // a KV head, 0: query tiles stay whole
-  int64_t ctas, slots, off_ml, off_own, ws_floats;
+  bool singles;
+  int64_t list, cuts, slots, off_ml, off_plan, off_cut, off_singles, ws_floats;
 };
 int paged_plan_host(const fb_paged_cache* c, int rows, int width, int T, int NH, int window, int sinks, PagedPlan* p) {
   const int nq = LP_ROWS / (NH / c->NKV);
@@ -609,14 +708,26 @@ int paged_plan_host(const fb_paged_cache* c, int rows, int width, int T, int NH,
   int64_t keys = S;
   if (window > 0 && (int64_t)window + sinks + nq + 3 * LP_SEG < S) keys = (int64_t)window + sinks + nq + 3 * LP_SEG;
   const int64_t most = (keys + LP_TILE - 1) / LP_TILE;
-  p->pieces = most > PT_MIN ? (2 * PT_WAVES * fbh::num_sms() + c->NKV - 1) / c->NKV : 0;
-  p->ctas = (units + p->pieces) * c->NKV;
-  FB_CHECK_ARG(p->ctas <= 0x7fffffff, "paged_attend: too many tokens, rows and heads");
-  p->slots = 2ll * p->pieces * c->NKV;  // a cut query tile's pieces are at most twice its share of the work
-  if (p->slots > p->ctas) p->slots = p->ctas;
+  p->singles = rows > 1 && T <= (int64_t)PT_SINGLES * rows;
+  // CTAs that the SMs hold.  By the device's SMs, not the calling thread's budget: the workspace's size goes by it.
+  p->pieces = most > PT_MIN ? (2 * fbh::num_sms() + c->NKV - 1) / c->NKV : 0;
+  // a list is cut for PT_WAVES rounds at most and into pieces of PT_MIN at least, or is its query tiles
+  p->cuts = (int64_t)PT_WAVES * p->pieces;
+  if (p->cuts > units * ((most + PT_MIN - 1) / PT_MIN)) p->cuts = units * ((most + PT_MIN - 1) / PT_MIN);
+  p->list = units > p->cuts ? units : p->cuts;
+  FB_CHECK_ARG(p->list * c->NKV <= 0x7fffffff, "paged_attend: too many tokens, rows and heads");
+  p->slots = p->cuts * c->NKV;
   p->off_ml = p->slots * LP_ROWS * LG_D;
-  p->off_own = p->off_ml + p->slots * LP_ROWS * 2;
-  p->ws_floats = p->pieces ? p->off_own + 2 * (int64_t)rows : 0;
+  p->off_plan = p->off_ml + p->slots * LP_ROWS * 2;
+  p->off_cut = p->off_plan + p->list * (int64_t)(sizeof(PagedPiece) / 4);
+  p->off_singles = p->off_cut + (p->cuts / 2 + 1) * 4;
+  p->ws_floats = p->off_singles;
+  if (p->singles) {
+    int64_t floats;
+    const int rc = fbh::paged_decode_floats(c, rows, width, NH, window, sinks, &floats);
+    if (rc) return rc;
+    p->ws_floats += floats;
+  }
   return FB_OK;
 }
 
@@ -677,8 +788,9 @@ extern "C" int flashb_paged_attend(const fb_paged_cache* cache, const int32_t* t
   if (rc) return rc;
   FB_CHECK_ARG(p.ws_floats == 0 || (ws && ((uintptr_t)ws & 15) == 0 && ws_floats >= p.ws_floats),
                "paged_attend: workspace of %lld floats, %lld needed", (long long)ws_floats, (long long)p.ws_floats);
-  a.NKV = cache->NKV, a.nq = LP_ROWS / a.G, a.per = (rows + 31) / 32, a.pieces = p.pieces;
-  a.po = ws, a.ml = (float2*)(ws + p.off_ml), a.own = (int2*)(ws + p.off_own);
+  a.NKV = cache->NKV, a.nq = LP_ROWS / a.G, a.lq = a.G == 1 ? 7 : a.G == 2 ? 6 : a.G == 4 ? 5 : 4, a.per = (rows + PP_THREADS - 1) / PP_THREADS, a.pieces = p.pieces, a.list = (int)p.list, a.cuts = (int)p.cuts;
+  a.rounds = p.pieces ? 1.f / p.pieces : 0.f;
+  a.po = ws, a.ml = (float2*)(ws + p.off_ml), a.plan = (PagedPiece*)(ws + p.off_plan), a.cut = (int4*)(ws + p.off_cut);
   a.err = fbh::device_err_ptr();
   const unsigned long long qd[4] = {64, (unsigned long long)NH, (unsigned long long)T, 2};
   const unsigned long long qs[3] = {(unsigned long long)(NH > 1 ? q_sh : LG_D) * 2, (unsigned long long)(T > 1 ? q_st : LG_D) * 2, 128};
@@ -705,10 +817,17 @@ extern "C" int flashb_paged_attend(const fb_paged_cache* cache, const int32_t* t
     }
     if (dev < 64) attr_done[dev] = 1;
   }
+  a.singles = p.singles;
+  const cudaStream_t st = (cudaStream_t)stream;
   void* args[] = {(void*)&a};
-  rc = fbh::launch_pdl((const void*)paged_attend_kernel, dim3((unsigned)p.ctas), dim3(LP_THREADS), LP_SMEM,
-                       (cudaStream_t)stream, args, true);
-  if (rc || !p.pieces) return rc;
-  return fbh::launch_pdl((const void*)paged_merge_kernel, dim3((unsigned)(((int64_t)T * NH + 3) / 4)), dim3(128), 0,
-                         (cudaStream_t)stream, args, true);
+  rc = fbh::launch_pdl((const void*)paged_plan_kernel, dim3(1), dim3(PP_THREADS), 0, st, args, true);
+  if (!rc && p.singles)
+    rc = fbh::paged_decode(cache, a.pool, table, table_sb, rows, width, lengths, offsets, T, q, q_st, q_sh, NH, window, sinks,
+                           scaling, ws + p.off_singles, out, o_st, o_sh, stream);
+  if (!rc)
+    rc = fbh::launch_pdl((const void*)paged_attend_kernel, dim3((unsigned)(p.list * a.NKV)), dim3(LP_THREADS), LP_SMEM, st,
+                         args, true);
+  if (rc || p.cuts < 2) return rc;
+  return fbh::launch_pdl((const void*)paged_merge_kernel, dim3((unsigned)(p.cuts / 2 * a.NKV), LP_ROWS / PM_ROWS),
+                         dim3(PM_THREADS), 0, st, args, true);
 }
