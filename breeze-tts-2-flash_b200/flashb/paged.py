@@ -27,8 +27,10 @@ import torch
 
 from . import _native
 from ._native import FbPagedCache, check
-from .longform import D, _BF16, _F32, _I64, _current, _ensure, _on, _raw_stream, _refuse, _span
+from .longform import D, _BF16, _I64, _current, _ensure, _on, _raw_stream, _refuse, _span
 
+_I32 = torch.int32
+_HEAD = (D,)
 _SCALING = D ** -0.5
 _lib = None
 
@@ -98,7 +100,9 @@ class Rotary:
         self.amplitude = float(amp if amplitude is None else amplitude)
         _ensure(math.isfinite(self.amplitude), 'rotary: amplitude not finite')
         self.turns = (freq / (2 * math.pi)).to(device)
-        self.device = self.turns.device
+        _ensure(self.turns.is_cuda, 'rotary: a CUDA device')
+        self.device, self._index = self.turns.device, self.turns.get_device()
+        self._args = (self.turns.data_ptr(), dim, int(layout == 'interleaved'), self.amplitude)
 
     @staticmethod
     def _freq(dim, base, how):
@@ -126,34 +130,41 @@ class Rotary:
         return freq, amp
 
 
-def _step(cache, table, lengths, offsets, T):
+# The checks below are what a call of some microseconds spends its time on: attributes once, devices by index.
+def _step(index, table, lengths, offsets, T):
     """The step's (table, its row stride, rows, width, lengths, offsets) as the library takes them."""
-    dev = cache.device
-    if table.dtype != torch.int32 or table.device != dev or table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
-        _refuse('table: [B, W] int32 on the cache\'s device with unit inner stride')
+    if table.dtype is not _I32 or table.get_device() != index or table.dim() != 2:
+        _refuse('table: [B, W] int32 on the cache\'s device')
     B, W = table.shape
-    if B < 1 or W < 1:
-        _refuse(f'table: {B} rows of {W} pages')
-    if lengths.dtype != _I64 or lengths.device != dev or lengths.shape != (B,) or not lengths.is_contiguous():
+    tb, tw = table.stride()
+    if B < 1 or W < 1 or (tw != 1 and W > 1):
+        _refuse('table: [B, W] with unit inner stride, not empty')
+    if lengths.dtype is not _I64 or lengths.get_device() != index or lengths.shape != (B,) or not lengths.is_contiguous():
         _refuse('lengths: [B] int64 on the cache\'s device')
     if offsets is None:
         if T != B:
             _refuse(f'{T} tokens of {B} rows without offsets')
-        op = None
-    else:
-        if offsets.dtype != _I64 or offsets.device != dev or offsets.shape != (B + 1,) or not offsets.is_contiguous():
-            _refuse('offsets: [B + 1] int64 on the cache\'s device')
-        op = offsets.data_ptr()
-    return table.data_ptr(), table.stride(0) if B > 1 else W, B, W, lengths.data_ptr(), op
+        return table.data_ptr(), tb if B > 1 else W, B, W, lengths.data_ptr(), None
+    if offsets.dtype is not _I64 or offsets.get_device() != index or offsets.shape != (B + 1,) or not offsets.is_contiguous():
+        _refuse('offsets: [B + 1] int64 on the cache\'s device')
+    return table.data_ptr(), tb if B > 1 else W, B, W, lengths.data_ptr(), offsets.data_ptr()
 
 
-def _tokens(t, name, dev):
-    """(token, head) strides of [T, heads, 128] bf16."""
-    if t.dtype != _BF16 or t.device != dev or t.dim() != 3 or t.shape[2] != D or t.stride(2) != 1:
-        _refuse(f'{name}: [T, heads, 128] bf16 on the cache\'s device with unit inner stride')
-    T, H, _ = t.shape
-    st, sh, _ = t.stride()
-    return st if T > 1 else H * D, sh if H > 1 else D
+def _tokens(t, name, index, T=None, H=None):
+    """(tokens, heads, token stride, head stride) of [T, heads, 128] bf16."""
+    if t.dtype is not _BF16 or t.get_device() != index or t.dim() != 3:
+        _refuse(f'{name}: [T, heads, 128] bf16 on the cache\'s device')
+    n, h, d = t.shape
+    st, sh, sd = t.stride()
+    if d != D or sd != 1 or (T is not None and (n != T or h != H)):
+        _refuse(f'{name}: {f"[{T}, {H}, 128]" if T is not None else "[T, heads, 128]"} with unit inner stride')
+    return n, h, st if n > 1 else h * D, sh if h > 1 else D
+
+
+def _norm(w, name, index):
+    if w.dtype is not _BF16 or w.get_device() != index or w.shape != _HEAD or not w.is_contiguous():
+        _refuse(f'{name}: [128] bf16 on the cache\'s device')
+    return w.data_ptr()
 
 
 def append(qkv, cache, table, lengths, *, offsets=None, rotary=None, q_norm=None, k_norm=None, eps=1e-6, positions=None,
@@ -165,38 +176,40 @@ def append(qkv, cache, table, lengths, *, offsets=None, rotary=None, q_norm=None
     Row b's run ends at slot lengths[b] - 1; ``positions`` [T] int64 (None: the slot) is what rotates.  In fp32, rounded
     once; the angle is reduced in 64 bits (off by 2^-20 radians at position 2^31).  Slots outside a row's pages are skipped.
     No two tokens may have the same slot."""
-    if _current() != cache.index:
-        with _on(cache.index):
+    index = cache.index
+    if _current() != index:
+        with _on(index):
             return append(qkv, cache, table, lengths, offsets=offsets, rotary=rotary, q_norm=q_norm, k_norm=k_norm, eps=eps,
                           positions=positions, out=out)
-    dev = cache.device
-    if qkv.dtype != _BF16 or qkv.device != dev or qkv.dim() != 2 or qkv.shape[1] % D or qkv.stride(1) != 1:
-        _refuse('qkv: [T, (NH + 2 NKV) 128] bf16 on the cache\'s device with unit inner stride')
-    T, NH = qkv.shape[0], qkv.shape[1] // D - 2 * cache.NKV
-    if NH < 1:
-        _refuse(f'qkv: {qkv.shape[1] // D} heads, 2 x {cache.NKV} of them keys and values')
-    step = _step(cache, table, lengths, offsets, T)
-    for w, n in ((q_norm, 'q_norm'), (k_norm, 'k_norm')):
-        if w is not None and (w.dtype != _BF16 or w.device != dev or w.shape != (D,) or not w.is_contiguous()):
-            _refuse(f'{n}: [128] bf16 on the cache\'s device')
-    if rotary is not None and rotary.device != dev:
-        _refuse('rotary: on another device')
-    if positions is not None and (positions.dtype != _I64 or positions.device != dev or positions.shape != (T,) or
-                                  not positions.is_contiguous()):
+    if qkv.dtype is not _BF16 or qkv.get_device() != index or qkv.dim() != 2:
+        _refuse('qkv: [T, (NH + 2 NKV) 128] bf16 on the cache\'s device')
+    T, n = qkv.shape
+    ld, one = qkv.stride()
+    NH = n // D - 2 * cache.NKV
+    if NH < 1 or n % D or one != 1:
+        _refuse(f'qkv: [T, {n}] with unit inner stride, 128 a head, 2 x {cache.NKV} heads of them keys and values')
+    step = _step(index, table, lengths, offsets, T)
+    qn = None if q_norm is None else _norm(q_norm, 'q_norm', index)
+    kn = None if k_norm is None else _norm(k_norm, 'k_norm', index)
+    if rotary is None:
+        rot = _NO_ROTARY
+    else:
+        rot = rotary._args
+        if rotary._index != index:
+            _refuse('rotary: on another device')
+    if positions is not None and (positions.dtype is not _I64 or positions.get_device() != index or
+                                  positions.shape != (T,) or not positions.is_contiguous()):
         _refuse('positions: [T] int64 on the cache\'s device')
     if out is None:
-        out = torch.empty(T, NH, D, dtype=_BF16, device=dev)
-    elif out.shape != (T, NH, D):
-        _refuse('out: [T, NH, 128]')
-    st, sh = _tokens(out, 'out', dev)
+        out = qkv.new_empty((T, NH, D))
+        st, sh = NH * D, D
+    else:
+        _, _, st, sh = _tokens(out, 'out', index, T, NH)
     if T == 0:
         return out
     rc = (_lib or _bind()).flashb_paged_append(
-        cache._ref, *step, T, qkv.data_ptr(), qkv.stride(0) if T > 1 else qkv.shape[1], NH,
-        None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(), eps,
-        *_NO_ROTARY if rotary is None else (rotary.turns.data_ptr(), rotary.dim, rotary.layout == 'interleaved',
-                                            rotary.amplitude),
-        None if positions is None else positions.data_ptr(), out.data_ptr(), st, sh, _raw_stream(cache.index))
+        cache._ref, *step, T, qkv.data_ptr(), ld if T > 1 else n, NH, qn, kn, eps, *rot,
+        None if positions is None else positions.data_ptr(), out.data_ptr(), st, sh, _raw_stream(index))
     if rc:
         check(rc)
     return out
@@ -214,24 +227,26 @@ def attend(query, cache, table, lengths, *, offsets=None, window=None, sinks=0, 
     seen; a token that sees none gives 0.  Slots that are not seen may hold anything, NaN included; entries of pages that
     no token sees are not read.  ``scaling`` > 0 (None: 128^-0.5).  The same inputs give the same bits.  Without ``offsets``
     out is contiguous."""
-    if _current() != cache.index:
-        with _on(cache.index):
+    index = cache.index
+    if _current() != index:
+        with _on(index):
             return attend(query, cache, table, lengths, offsets=offsets, window=window, sinks=sinks, scaling=scaling,
                           out=out)
-    dev = cache.device
-    q_st, q_sh = _tokens(query, 'query', dev)
-    T, NH, _ = query.shape
-    step = _step(cache, table, lengths, offsets, T)
-    window, sinks = _span(window, sinks)
+    T, NH, q_st, q_sh = _tokens(query, 'query', index)
+    step = _step(index, table, lengths, offsets, T)
+    if window is None and sinks == 0:
+        window = 0
+    else:
+        window, sinks = _span(window, sinks)
     if out is None:
-        out = torch.empty(T, NH, D, dtype=_BF16, device=dev)
-    elif out.shape != (T, NH, D):
-        _refuse('out: [T, NH, 128]')
-    o_st, o_sh = _tokens(out, 'out', dev)
+        out = query.new_empty((T, NH, D))
+        o_st, o_sh = NH * D, D
+    else:
+        _, _, o_st, o_sh = _tokens(out, 'out', index, T, NH)
+        if offsets is None and not out.is_contiguous():
+            _refuse('out: contiguous without offsets')
     if T == 0:
         return out
-    if offsets is None and not out.is_contiguous():
-        _refuse('out: contiguous without offsets')
     lib = _lib or _bind()
     B, W = step[2], step[3]
     key = (B, W, T, NH, window, sinks, offsets is None)   # the workspace's size follows from the shapes alone
@@ -243,15 +258,18 @@ def attend(query, cache, table, lengths, *, offsets=None, window=None, sinks=0, 
             if len(cache._ws) >= 256:                     # steps of ever other sizes
                 cache._ws.clear()
             cache._ws[key] = n
-    ws = torch.empty(n, dtype=_F32, device=dev) if n > 0 else None
-    scaling = _SCALING if scaling is None else scaling
-    wp = None if ws is None else ws.data_ptr()
+    ws, wp = None, None
+    if n > 0:
+        ws = query.new_empty(2 * n)                       # bf16: two a float
+        wp = ws.data_ptr()
+    if scaling is None:
+        scaling = _SCALING
     if offsets is None:
         rc = lib.flashb_paged_decode(cache._ref, *step[:5], query.data_ptr(), q_st, q_sh, NH, window, sinks, scaling, wp, n,
-                                     out.data_ptr(), _raw_stream(cache.index))
+                                     out.data_ptr(), _raw_stream(index))
     else:
         rc = lib.flashb_paged_attend(cache._ref, *step, T, query.data_ptr(), q_st, q_sh, NH, window, sinks, scaling, wp, n,
-                                     out.data_ptr(), o_st, o_sh, _raw_stream(cache.index))
+                                     out.data_ptr(), o_st, o_sh, _raw_stream(index))
     if rc:
         check(rc)
     return out

@@ -19,6 +19,21 @@ from . import _native
 from ._native import check
 
 _INF = float('inf')
+_F32, _BF16, _I64 = torch.float32, torch.bfloat16, torch.int64
+_AS_F32, _AS_IS = dict(dtype=_F32), {}
+_current, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+_lib = None
+
+
+def _bind():
+    """The library, looked up once (``_native.lib()`` takes a lock)."""
+    global _lib
+    _lib = _native.lib()
+    return _lib
+
+
+def _refuse(msg):
+    raise _native.FlashbError(_native.FB_ERR_ARG, msg)
 
 
 class InvalidDistribution(RuntimeError):
@@ -107,30 +122,30 @@ def token_scores(logits, tokens, *, top=0, temperature=1.0):
     Larger logits come first, equal ones by id, a NaN before all, as in the greedy sampler.  Suppressed ids (-inf) have
     probability 0; an id outside the vocabulary has log probability -inf and rank V.  A row with a NaN or +inf, or of -inf
     alone, has no distribution: NaN log probabilities and entropy."""
-    def _ensure(cond, msg):
-        if not cond:
-            raise _native.FlashbError(_native.FB_ERR_ARG, msg)
-
-    _ensure(logits.is_cuda and logits.dtype in (torch.float32, torch.bfloat16) and logits.dim() == 2 and
-            (logits.shape[1] == 1 or logits.stride(1) == 1), 'logits: [rows, V] fp32 or bf16 CUDA with unit inner stride')
+    kind = logits.dtype
+    index = logits.get_device()
+    if index < 0 or logits.dim() != 2 or (kind is not _F32 and kind is not _BF16):
+        _refuse('logits: [rows, V] fp32 or bf16 on a CUDA device')
     rows, V = logits.shape
-    dev = logits.device
-    _ensure(tokens.dtype == torch.int64 and tokens.device == dev and tokens.shape == (rows,) and tokens.is_contiguous(),
-            'tokens: [rows] int64 on the logits\' device')
-    _ensure(V >= 1 and 0 <= top <= min(32, V), f'top: 0 to {min(32, V)}')
-    if torch._C._cuda_getDevice() != logits.get_device():
-        with torch.cuda.device(dev):
+    ld, one = logits.stride()
+    if V < 1 or (one != 1 and V > 1):
+        _refuse('logits: [rows, V] with unit inner stride, V at least 1')
+    if tokens.dtype is not _I64 or tokens.get_device() != index or tokens.shape != (rows,) or not tokens.is_contiguous():
+        _refuse('tokens: [rows] int64 on the logits\' device')
+    if not 0 <= top <= 32 or top > V:
+        _refuse(f'top: 0 to {min(32, V)}')
+    if _current() != index:
+        with torch.cuda.device(index):
             return token_scores(logits, tokens, top=top, temperature=temperature)
-    # one allocation: the 64-bit parts first
-    buf = torch.empty(rows * (3 * top + 4), dtype=torch.float32, device=dev)
-    ids, rest = buf[:rows * (2 * top + 2)].view(torch.int64), buf[rows * (2 * top + 2):]
-    out = TokenScores(rest[:rows], rest[rows:2 * rows], ids[:rows], ids[rows:].view(rows, top),
-                      rest[2 * rows:].view(rows, top))
+    kw = _AS_F32 if kind is _BF16 else _AS_IS
+    out = TokenScores(logits.new_empty(rows, **kw), logits.new_empty(rows, **kw), tokens.new_empty(rows),
+                      tokens.new_empty((rows, top)), logits.new_empty((rows, top), **kw))
     if rows == 0:
         return out
-    check(_native.lib().flashb_token_scores(
-        logits.data_ptr(), int(logits.dtype == torch.bfloat16), logits.stride(0) if rows > 1 else V, rows, V,
-        tokens.data_ptr(), float(temperature), int(top), out.logprob.data_ptr(), out.entropy.data_ptr(),
-        out.rank.data_ptr(), out.top_ids.data_ptr(), out.top_logprobs.data_ptr(),
-        torch._C._cuda_getCurrentRawStream(logits.get_device())))
+    logprob, entropy, rank, ids, logprobs = out
+    rc = (_lib or _bind()).flashb_token_scores(
+        logits.data_ptr(), kind is _BF16, ld if rows > 1 else V, rows, V, tokens.data_ptr(), temperature, top,
+        logprob.data_ptr(), entropy.data_ptr(), rank.data_ptr(), ids.data_ptr(), logprobs.data_ptr(), _raw_stream(index))
+    if rc:
+        check(rc)
     return out
