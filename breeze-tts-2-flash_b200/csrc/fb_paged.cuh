@@ -24,17 +24,32 @@ struct PagedRows {
   int rows, T, S;                       // S: slots that a row's table entries span
 };
 
-// The row whose run holds token t, -1: none.  A warp together: rows whose run begins at t or before, counted 32 at a time
-// with no load waiting for another (a search by halves is a chain of them).
-__device__ __forceinline__ int paged_row(const PagedRows& r, int t) {
-  if (!r.offsets) return t < r.rows ? t : -1;
+// The rows whose runs hold tokens t .. t + N - 1, -1: none; lane i < N gets that of t + i.  A warp together: rows whose run
+// begins at the token or before, counted 32 at a time with no load waiting for another (a search by halves is a chain of
+// them).
+template <int N>
+__device__ __forceinline__ int paged_rows(const PagedRows& r, int t) {
   const int lane = threadIdx.x & 31;
-  int n = 0;
+  if (!r.offsets) return t + lane < r.rows ? t + lane : -1;
+  int n[N], mine = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) n[i] = 0;
 #pragma unroll 4
-  for (int b = lane; b <= r.rows; b += 32) n += r.offsets[b] <= t;
-  n = __reduce_add_sync(FULL, n);
-  return n <= r.rows ? n - 1 : -1;
+  for (int b = lane; b <= r.rows; b += 32) {
+    if (b < r.rows) asm volatile("prefetch.global.L1 [%0];" ::"l"(r.lengths + b));    // the row's is read next
+    const long long f = r.offsets[b];
+#pragma unroll
+    for (int i = 0; i < N; ++i) n[i] += f <= t + i;
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    n[i] = __reduce_add_sync(FULL, n[i]);
+    mine = lane == i ? n[i] : mine;
+  }
+  return mine <= r.rows ? mine - 1 : -1;
 }
+// That of one token, for every lane.
+__device__ __forceinline__ int paged_row(const PagedRows& r, int t) { return __shfl_sync(FULL, paged_rows<1>(r, t), 0); }
 // How many tokens of row b's run come after token t, itself counted.
 __device__ __forceinline__ long long paged_left(const PagedRows& r, int b, int t) {
   return r.offsets ? r.offsets[b + 1] - t : 1;
