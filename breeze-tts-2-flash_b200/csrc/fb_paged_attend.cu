@@ -32,6 +32,7 @@ namespace fb {
 
 constexpr int PT_MIN = 4;                         // key tiles of a piece, at least
 constexpr int PT_WAVES = 4;                       // rounds of CTAs that the list of pieces may be cut for
+constexpr float PT_LIMIT = 0x1p-16f;              // 2^(8 + LP_SHIFT): a tile's weights below it leave the reference as it is
 constexpr int PT_COST = 5;                        // what beginning and ending a piece takes, in key tiles
 
 struct PagedPiece;
@@ -453,9 +454,9 @@ __global__ void __launch_bounds__(LP_THREADS, 2) paged_attend_kernel(const __gri
     }
     named_sync(1, 32 * warps);
     const bool holes = s_bad != 0;
-    float m = -INFINITY;
-    uint64_t sum2[2] = {0, 0};
-    bool ok = true;
+    // the reference m of the weights, 2^(score - m + LP_SHIFT); fresh: none yet (a row that sees nothing needs none)
+    float m = p < 0 ? 0.f : -INFINITY, off = 0.f, sum = 0.f;
+    bool fresh = p >= 0, ok = true;
     for (int t = 0; t < tiles; ++t) {
       ok = lp_wait_warp(&bar_s[t & 1], (t >> 1) & 1, a.err);
       if (!ok) break;
@@ -481,21 +482,41 @@ __global__ void __launch_bounds__(LP_THREADS, 2) paged_attend_kernel(const __gri
           for (int c = 0; c < LP_SEG; ++c) s[LP_SEG * sg + c] = (see >> c) & 1u ? s[LP_SEG * sg + c] : -INFINITY;
         }
       }
-      float x[4] = {s[0], s[1], s[2], s[3]};
+      // P's buffer: free once P V of t - 2 is done (asked here, needed after the exponentials)
+      const bool free = t < 2 || mbar_test(&bar_o[t & 1], ((t - 2) >> 1) & 1);
+      uint32_t w[32];
+      uint64_t part[2];
+      auto weights = [&] {
+        const uint64_t off2 = f2(off, off);
+        part[0] = part[1] = 0;
 #pragma unroll
-      for (int c = 4; c < 64; c += 4) {
-        x[(c >> 2) & 3] = max3(x[(c >> 2) & 3], s[c], s[c + 1]);
-        x[((c >> 2) + 2) & 3] = max3(x[((c >> 2) + 2) & 3], s[c + 2], s[c + 3]);
-      }
-      // scale > 0 (checked): the maximum of the scaled scores
-      const float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * a.scale;
-      const bool up = mx > m + LP_SLACK;
-      if (__any_sync(FULL, up)) {
-        const float mn = up ? mx : m, f = up ? (m > -INFINITY ? ex2(m - mn) : 0.f) : 1.f;
-        m = mn;
-        const float2 u = f2_get(f2_add(sum2[0], sum2[1]));
-        sum2[0] = f2(u.x * f, u.y * f);
-        sum2[1] = 0;
+        for (int c = 0; c < 32; ++c) {
+          const float2 e = f2_get(f2_fma(f2(s[2 * c], s[2 * c + 1]), scale2, off2));
+          const float p0 = ex2(e.x), p1 = ex2(e.y);
+          part[c & 1] = f2_add(part[c & 1], f2(p0, p1));
+          w[c] = pack_bf16(p0, p1);
+        }
+      };
+      weights();
+      float2 u = f2_get(f2_add(part[0], part[1]));
+      // the tile's sum tells whether a score passes the reference by 2^8 (or there is none yet)
+      if (__any_sync(FULL, !(u.x + u.y <= PT_LIMIT) || fresh)) {
+        float x[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+        for (int c = 4; c < 64; c += 4) {
+          x[(c >> 2) & 3] = max3(x[(c >> 2) & 3], s[c], s[c + 1]);
+          x[((c >> 2) + 2) & 3] = max3(x[((c >> 2) + 2) & 3], s[c + 2], s[c + 3]);
+        }
+        // scale > 0 (checked): the maximum of the scaled scores
+        const float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * a.scale;
+        const bool up = mx > -INFINITY && (fresh || mx > m);
+        const float f = up ? (fresh ? 0.f : ex2(m - mx)) : 1.f;
+        if (up) {
+          m = mx;
+          fresh = false;
+          off = LP_SHIFT - mx;
+        }
+        sum *= f;
         if (t > 0) {
           ok = lp_wait_warp(&bar_o[(t - 1) & 1], ((t - 1) >> 1) & 1, a.err);
           if (!ok) break;
@@ -504,25 +525,16 @@ __global__ void __launch_bounds__(LP_THREADS, 2) paged_attend_kernel(const __gri
           for (int c = 0; c < LG_D; c += 32) {
             float o[32];
             lp_ld32(t_o + my + c, o);
-            uint32_t w[32];
+            uint32_t v[32];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(o[i] * f);
-            lp_st32(t_o + my + c, w);
+            for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(o[i] * f);
+            lp_st32(t_o + my + c, v);
           }
         }
+        weights();
+        u = f2_get(f2_add(part[0], part[1]));
       }
-      // P's buffer: free once P V of t - 2 is done (asked here, needed after the exponentials)
-      const bool free = t < 2 || mbar_test(&bar_o[t & 1], ((t - 2) >> 1) & 1);
-      const float off = m > -INFINITY ? LP_SHIFT - m : 0.f;
-      const uint64_t off2 = f2(off, off);
-      uint32_t w[32];
-#pragma unroll
-      for (int c = 0; c < 32; ++c) {
-        const float2 e = f2_get(f2_fma(f2(s[2 * c], s[2 * c + 1]), scale2, off2));
-        const float p0 = ex2(e.x), p1 = ex2(e.y);
-        sum2[c & 1] = f2_add(sum2[c & 1], f2(p0, p1));
-        w[c] = pack_bf16(p0, p1);
-      }
+      sum += u.x + u.y;
       if (!__all_sync(FULL, free)) {
         ok = lp_wait_warp(&bar_o[t & 1], ((t - 2) >> 1) & 1, a.err);
         if (!ok) break;
@@ -535,8 +547,6 @@ __global__ void __launch_bounds__(LP_THREADS, 2) paged_attend_kernel(const __gri
     if (ok && tiles > 1) ok = lp_wait_warp(&bar_o[tiles & 1], ((tiles - 2) >> 1) & 1, a.err);
     if (ok && tiles > 0) ok = lp_wait_warp(&bar_o[(tiles - 1) & 1], ((tiles - 1) >> 1) & 1, a.err);
     tc_after();
-    const float2 u = f2_get(f2_add(sum2[0], sum2[1]));
-    const float sum = u.x + u.y;
     if (piece.s > 1) {
       // ---- a piece: the row's part, unnormalised
       const long long at = (long long)piece.slot * a.NKV + h;
