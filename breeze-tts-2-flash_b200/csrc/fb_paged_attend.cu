@@ -30,7 +30,7 @@
 
 namespace fb {
 
-constexpr int PT_MIN = 4;                         // key tiles of a piece, at least
+constexpr int PT_MIN = 8;                         // key tiles of a piece, at least
 constexpr int PT_WAVES = 4;                       // rounds of CTAs that the list of pieces may be cut for
 constexpr float PT_LIMIT = 0x1p-16f;              // 2^(8 + LP_SHIFT): a tile's weights below it leave the reference as it is
 constexpr int PT_COST = 5;                        // what beginning and ending a piece takes, in key tiles
@@ -38,7 +38,7 @@ constexpr int PT_COST = 5;                        // what beginning and ending a
 struct PagedPiece;
 
 struct alignas(64) PagedAttendArgs {
-  CUtensorMap tq, tk, tv, tks, tvs;     // Q tile; K, V: boxes of 64 slots, and of 32 or 16 (half of the dims)
+  CUtensorMap tq, tk, tv, tks, tvs;     // Q tile; K, V: boxes of 64 slots, and of 32 or 16 (of K half of the dims)
   PagedPool pool;
   PagedTable t;
   PagedRows r;
@@ -48,6 +48,7 @@ struct alignas(64) PagedAttendArgs {
   int lq;                               // log2 nq
   int per, pieces, list, cuts;          // rows per thread of the plan; CTAs that the SMs hold a KV head, 0: query tiles stay
   float rounds;                         // whole; entries of the list, of them cut at most; 1 / pieces
+  int per32;                            // rows per lane where a CTA finds its query tile itself
   int singles;                          // rows of one token are another launch's
   float scale;                          // scaling x log2(e)
   bf16* out;
@@ -235,6 +236,37 @@ __global__ void __launch_bounds__(PP_THREADS) paged_plan_kernel(const __grid_con
   for (int x = joins + tid; x < a.cuts / 2; x += PP_THREADS) a.cut[x] = make_int4(0, 0, 0, 0);   // the merge's other CTAs
 }
 
+// Piece x of the list whose query tiles stay whole, for a CTA without a plan: a warp, lane i counts rows [i per32, ..).
+__device__ __forceinline__ PagedPiece paged_direct(const PagedAttendArgs& a, int x, int lane) {
+  int n = 0;
+#pragma unroll 1
+  for (int i = 0; i < a.per32; ++i) {
+    const int b = lane * a.per32 + i;
+    if (b < a.r.rows) n += paged_tiles(a, b).x;
+  }
+  int before = n;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(FULL, before, o);
+    if (lane >= o) before += y;
+  }
+  PagedPiece p{-1, 0, 0, 0, 0, 1, 0, 0};
+  if (x >= __shfl_sync(FULL, before, 31)) return p;
+  before -= n;
+  const int owner = 31 - __clz(__ballot_sync(FULL, before <= x));   // empty lanes share a count: the last of them
+  int at = __shfl_sync(FULL, before, owner), b = owner * a.per32;
+#pragma unroll 1
+  for (;; ++b) {
+    n = paged_tiles(a, b).x;
+    if (x < at + n) break;
+    at += n;
+  }
+  const PagedSpan span = paged_span(a.r, b);
+  const int q0 = (n - 1 - (x - at)) << a.lq;
+  p.b = b, p.tok = span.t0 + q0, p.nt = min(a.nq, span.n - q0), p.p_lo = span.p0 + q0;
+  return p;
+}
+
 // One token and head over its visible keys, one at a time: four dims a lane; the row in bf16.
 // (A row that saw nothing, or whose output is not finite.)
 __device__ __noinline__ uint2 paged_one(const PagedAttendArgs& a, int b, int p, int hq, const bf16* q) {
@@ -275,6 +307,7 @@ __global__ void __launch_bounds__(LP_THREADS, 2) paged_attend_kernel(const __gri
   __shared__ __align__(8) uint64_t bar_k[2], bar_v[2], bar_s[2], bar_f, bar_p[2], bar_o[2];
   __shared__ uint32_t tslot;
   __shared__ int s_bad;
+  __shared__ PagedPiece s_piece;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int x = blockIdx.x / a.NKV, h = blockIdx.x - x * a.NKV;
   if (tid == 0) {
@@ -286,7 +319,17 @@ __global__ void __launch_bounds__(LP_THREADS, 2) paged_attend_kernel(const __gri
   // is not read here.  It is waited for at the end, so that it has ended when this one has.
   if (!a.singles) pdl_wait();
   pdl_trigger();
-  const PagedPiece piece = a.plan[x];
+  PagedPiece piece;
+  if (a.plan) {
+    piece = a.plan[x];
+  } else {
+    if (warp == 0) {
+      const PagedPiece y = paged_direct(a, x, lane);
+      if (lane == 0) s_piece = y;
+    }
+    __syncthreads();
+    piece = s_piece;
+  }
   if (piece.b < 0) {
     if (a.singles) pdl_wait();
     return;
@@ -317,8 +360,15 @@ __global__ void __launch_bounds__(LP_THREADS, 2) paged_attend_kernel(const __gri
   // whether any row of the tile sees a slot of [j, j + n)
   auto seen = [&](int j, int n) { return j <= p_hi && (j + n > seg.lo || j < a.sinks); };
 
+  // A tile is one box where it lies in one page, else boxes of `small` slots: of K one half of the dims each (its 64 keys
+  // are rows of one operand), of V both (a step of its product takes 16 keys, whose halves may lie anywhere).
+  const int small = min(a.t.page, LP_SEG);
+  auto whole = [&](int t) {
+    const int sg = 2 * (first + t);
+    return segs - 2 * t >= 2 && a.t.page >= LP_TILE && (seg.at(sg) & (LP_TILE - 1)) == 0 && sg != seg.ns - 1;
+  };
+
   if (warp == 4) {                                 // copies: one thread; the warp holds the entries of 16 tiles
-    const int small = min(a.t.page, LP_SEG);       // slots of a small box: 32, or 16
     // lane 4 i + c: the page of quarter c (16 slots) of tile 8 g + i of the piece
     auto entries = [&](int g) {
       const int tl = 8 * g + (lane >> 2);
@@ -346,12 +396,13 @@ __global__ void __launch_bounds__(LP_THREADS, 2) paged_attend_kernel(const __gri
               "l"(&a.tq), "r"(0), "r"(h * a.G), "r"(piece.tok), "r"(0), "r"(smem_u32(bar))
               : "memory");
       }
-      if (n == 2 && a.t.page >= LP_TILE && (j0 & (LP_TILE - 1)) == 0 && 2 * (first + t) != seg.ns - 1) {
+      if (whole(t)) {
         if (lane == 0) lp_load(dst, is_v ? &a.tv : &a.tk, j0 & mask, 0, h, pg, bar);
-      } else if ((qc >> 1) < n && lane < 8 && (small < LP_SEG || (qc & 1) == 0)) {
+      } else if ((qc >> 1) < n && lane < 8 && (small == LP_SEG / 2 || (qc & 1) == 0)) {
         // a lane a box: one thread after the other takes 40 ns each
-        lp_load(dst + (lane & 1) * (LP_KV / 2) + qc * (LP_KV / 8), is_v ? &a.tvs : &a.tks,
-                (seg.at(2 * (first + t) + (qc >> 1)) + 16 * (qc & 1)) & mask, lane & 1, h, pg, bar);
+        const int j = (seg.at(2 * (first + t) + (qc >> 1)) + 16 * (qc & 1)) & mask;
+        if (!is_v) lp_load(dst + (lane & 1) * (LP_KV / 2) + qc * (LP_KV / 8), &a.tks, j, lane & 1, h, pg, bar);
+        else if ((lane & 1) == 0) lp_load(dst + qc * (LP_KV / 4), &a.tvs, j, 0, h, pg, bar);
       }
       __syncwarp();
     };
@@ -404,9 +455,13 @@ __global__ void __launch_bounds__(LP_THREADS, 2) paged_attend_kernel(const __gri
           break;
     __syncwarp();
   } else if (warp == 6) {                          // P V
-    const uint64_t dv = tc_desc(smem_u32(sv), LP_KV / 2, 1024, 2);   // dims contiguous: two halves of 64, 8-key groups
+    // dims contiguous: two halves of 64, 8-key groups; in a box of n slots the halves are n x 128 bytes apart, and the next
+    // box is n x 256 on
+    const uint64_t dv = tc_desc(smem_u32(sv), LP_KV / 2, 1024, 2), ds = tc_desc(smem_u32(sv), small * 128, 1024, 2);
+    const int odd = small == LP_SEG ? 2048 : 4096;   // 16 keys on
     auto step = [&](auto buf, int t) -> bool {
       constexpr int B = decltype(buf)::value;
+      const bool one = whole(t);                   // worked out before the waits: between P and its product every cycle counts
       if (!lp_wait_warp(&bar_v[B], (t >> 1) & 1, a.err)) return false;
       bool zeroed = false;
       for (int s = 0; s < 2 && 2 * t + s < segs; ++s) {              // slots that no row of the tile sees
@@ -414,10 +469,13 @@ __global__ void __launch_bounds__(LP_THREADS, 2) paged_attend_kernel(const __gri
         const uint32_t see = lp_bits(seg.lo - j0, p_hi + 1 - j0) | lp_bits(0, min(a.sinks, p_hi + 1) - j0);
         if (see == FULL) continue;
         zeroed = true;
-        unsigned char* z = sv + B * LP_KV + s * (LP_KV / 4);
+        const int rows = one ? LP_TILE : small;
         for (int i = lane; i < LP_SEG * 16; i += 32)
-          if (!((see >> (i >> 4)) & 1u))
-            *reinterpret_cast<uint4*>(z + ((i >> 3) & 1) * (LP_KV / 2) + (i >> 4) * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+          if (!((see >> (i >> 4)) & 1u)) {
+            const int key = LP_SEG * s + (i >> 4), in = key & (rows - 1);
+            *reinterpret_cast<uint4*>(sv + B * LP_KV + (key - in) * 256 + ((i >> 3) & 1) * rows * 128 + in * 128 + (i & 7) * 16) =
+                make_uint4(0, 0, 0, 0);
+          }
       }
       if (zeroed) {
         fence_proxy_async();
@@ -428,10 +486,17 @@ __global__ void __launch_bounds__(LP_THREADS, 2) paged_attend_kernel(const __gri
       if (lane == 0) {
         constexpr uint32_t idesc = tc_idesc(LG_D) | (1u << 16);   // V: dims contiguous
         const bool half = segs - 2 * t < 2;
+        if (one) {
 #pragma unroll
-        for (int s = 0; s < 4; ++s)
-          if (s < 2 || !half)
+          for (int s = 0; s < 4; ++s)
             lp_mma_ts(t_o, tmem + 64 + 32 * B + 8 * s, dv + ((B * LP_KV + 2048 * s) >> 4), idesc, s > 0 || t > 0);
+        } else {
+#pragma unroll
+          for (int s = 0; s < 4; ++s)
+            if (s < 2 || !half)
+              lp_mma_ts(t_o, tmem + 64 + 32 * B + 8 * s, ds + ((B * LP_KV + (s >> 1) * 8192 + (s & 1) * odd) >> 4), idesc,
+                        s > 0 || t > 0);
+        }
         tc_commit(&bar_o[B]);
       }
       __syncwarp();
@@ -704,10 +769,10 @@ int paged_group(const fb_paged_cache* c, int NH) {
 
 // Rows of one token go through the single-token kernel, a launch of its own before this one, where a row has few tokens on
 // average: it reads their keys at 0.95 of the copy bandwidth where a tile of 128 rows, G of them in use, reaches 0.8.
-constexpr int PT_SINGLES = 32;
+constexpr int PT_SINGLES = 16;
 struct PagedPlan {
   int pieces;                           // a KV head, 0: query tiles stay whole
-  bool singles;
+  bool singles, direct;                 // direct: nothing to cut and no other launch: no plan, CTAs find their query tiles
   int64_t list, cuts, slots, off_ml, off_plan, off_cut, off_singles, ws_floats;
 };
 int paged_plan_host(const fb_paged_cache* c, int rows, int width, int T, int NH, int window, int sinks, PagedPlan* p) {
@@ -721,6 +786,7 @@ int paged_plan_host(const fb_paged_cache* c, int rows, int width, int T, int NH,
   p->singles = rows > 1 && T <= (int64_t)PT_SINGLES * rows;
   // CTAs that the SMs hold.  By the device's SMs, not the calling thread's budget: the workspace's size goes by it.
   p->pieces = most > PT_MIN ? (2 * fbh::num_sms() + c->NKV - 1) / c->NKV : 0;
+  p->direct = p->pieces == 0 && !p->singles;
   // a list is cut for PT_WAVES rounds at most and into pieces of PT_MIN at least, or is its query tiles
   p->cuts = (int64_t)PT_WAVES * p->pieces;
   if (p->cuts > units * ((most + PT_MIN - 1) / PT_MIN)) p->cuts = units * ((most + PT_MIN - 1) / PT_MIN);
@@ -729,8 +795,8 @@ int paged_plan_host(const fb_paged_cache* c, int rows, int width, int T, int NH,
   p->slots = p->cuts * c->NKV;
   p->off_ml = p->slots * LP_ROWS * LG_D;
   p->off_plan = p->off_ml + p->slots * LP_ROWS * 2;
-  p->off_cut = p->off_plan + p->list * (int64_t)(sizeof(PagedPiece) / 4);
-  p->off_singles = p->off_cut + (p->cuts / 2 + 1) * 4;
+  p->off_cut = p->off_plan + (p->direct ? 0 : p->list * (int64_t)(sizeof(PagedPiece) / 4));
+  p->off_singles = p->off_cut + p->cuts / 2 * 4;
   p->ws_floats = p->off_singles;
   if (p->singles) {
     int64_t floats;
@@ -741,13 +807,13 @@ int paged_plan_host(const fb_paged_cache* c, int rows, int width, int T, int NH,
   return FB_OK;
 }
 
-// The pool as (64 dims, slots, half, heads, pages); boxes of 64 slots x both halves, or of `rows` x one.
-int paged_map(CUtensorMap* m, const PagedPool& c, bool v, int rows) {
+// The pool as (64 dims, slots, half, heads, pages); boxes of `rows` slots x `halves`.
+int paged_map(CUtensorMap* m, const PagedPool& c, bool v, int rows, int halves) {
   const unsigned long long dims[5] = {64, (unsigned long long)c.page, 2, (unsigned long long)c.NKV, (unsigned long long)c.pages};
   const unsigned long long st[4] = {(unsigned long long)(v ? c.v_sl : c.k_sl), 128,
                                     (unsigned long long)(c.NKV > 1 ? (v ? c.v_sh : c.k_sh) : 2 * LG_D),
                                     (unsigned long long)(c.pages > 1 ? (v ? c.v_sb : c.k_sb) : 2 * LG_D)};
-  const unsigned bx[5] = {64, (unsigned)rows, rows == LP_TILE ? 2u : 1u, 1, 1};
+  const unsigned bx[5] = {64, (unsigned)rows, (unsigned)halves, 1, 1};
   return fbh::tmap_bf16(m, v ? c.v : c.k, 5, dims, st, bx);
 }
 
@@ -800,18 +866,18 @@ extern "C" int flashb_paged_attend(const fb_paged_cache* cache, const int32_t* t
                "paged_attend: workspace of %lld floats, %lld needed", (long long)ws_floats, (long long)p.ws_floats);
   a.NKV = cache->NKV, a.nq = LP_ROWS / a.G, a.lq = a.G == 1 ? 7 : a.G == 2 ? 6 : a.G == 4 ? 5 : 4, a.per = (rows + PP_THREADS - 1) / PP_THREADS, a.pieces = p.pieces, a.list = (int)p.list, a.cuts = (int)p.cuts;
   a.rounds = p.pieces ? 1.f / p.pieces : 0.f;
-  a.po = ws, a.ml = (float2*)(ws + p.off_ml), a.plan = (PagedPiece*)(ws + p.off_plan), a.cut = (int4*)(ws + p.off_cut);
+  a.po = ws, a.ml = (float2*)(ws + p.off_ml), a.per32 = (rows + 31) / 32, a.plan = p.direct ? nullptr : (PagedPiece*)(ws + p.off_plan), a.cut = (int4*)(ws + p.off_cut);
   a.err = fbh::device_err_ptr();
   const unsigned long long qd[4] = {64, (unsigned long long)NH, (unsigned long long)T, 2};
   const unsigned long long qs[3] = {(unsigned long long)(NH > 1 ? q_sh : LG_D) * 2, (unsigned long long)(T > 1 ? q_st : LG_D) * 2, 128};
   const unsigned qb[4] = {64, (unsigned)a.G, (unsigned)a.nq, 2};
   rc = fbh::tmap_bf16(&a.tq, q, 4, qd, qs, qb);
   const int small = cache->page < LP_SEG ? cache->page : LP_SEG;
-  if (!rc) rc = paged_map(&a.tks, a.pool, false, small);
-  if (!rc) rc = paged_map(&a.tvs, a.pool, true, small);
+  if (!rc) rc = paged_map(&a.tks, a.pool, false, small, 1);
+  if (!rc) rc = paged_map(&a.tvs, a.pool, true, small, 2);
   if (cache->page >= LP_TILE) {
-    if (!rc) rc = paged_map(&a.tk, a.pool, false, LP_TILE);
-    if (!rc) rc = paged_map(&a.tv, a.pool, true, LP_TILE);
+    if (!rc) rc = paged_map(&a.tk, a.pool, false, LP_TILE, 2);
+    if (!rc) rc = paged_map(&a.tv, a.pool, true, LP_TILE, 2);
   } else {
     a.tk = a.tks, a.tv = a.tvs;          // not used
   }
@@ -830,7 +896,7 @@ extern "C" int flashb_paged_attend(const fb_paged_cache* cache, const int32_t* t
   a.singles = p.singles;
   const cudaStream_t st = (cudaStream_t)stream;
   void* args[] = {(void*)&a};
-  rc = fbh::launch_pdl((const void*)paged_plan_kernel, dim3(1), dim3(PP_THREADS), 0, st, args, true);
+  if (!p.direct) rc = fbh::launch_pdl((const void*)paged_plan_kernel, dim3(1), dim3(PP_THREADS), 0, st, args, true);
   if (!rc && p.singles)
     rc = fbh::paged_decode(cache, a.pool, table, table_sb, rows, width, lengths, offsets, T, q, q_st, q_sh, NH, window, sinks,
                            scaling, ws + p.off_singles, out, o_st, o_sh, stream);

@@ -94,7 +94,7 @@ def test_workspace_sizes():
     L = _native.lib()
     d = ctypes.byref(desc(page=64))
     attend_ws = lambda rows, width, T, NH=8, w=0, s=0: L.flashb_paged_attend_ws_floats(d, rows, width, T, NH, w, s)  # noqa: E731
-    assert attend_ws(2, 4, 400) > 0
+    assert attend_ws(2, 4, 400) == 0 and attend_ws(2, 100, 400) > 0                     # few keys: nothing to cut
     assert attend_ws(1, 1000, 100) >= attend_ws(1, 1000, 100, w=64)                     # a short window needs no pieces
     assert attend_ws(0, 4, 10) == -1 and attend_ws(1, 4, 0) == -1 and attend_ws(1, 4, 10, NH=6) == -1
     assert L.flashb_paged_decode_ws_floats(d, 2, 4, 8, 0, 0) == 0
