@@ -267,6 +267,16 @@ __device__ __forceinline__ PagedPiece paged_direct(const PagedAttendArgs& a, int
   return p;
 }
 
+constexpr int PT_K = 3;                          // buffers of K: with two, S waited for K a quarter of the time
+struct alignas(16) PagedShared {
+  uint64_t bar_k[PT_K], bar_s[PT_K], bar_v[2], bar_p[2], bar_o[2], bar_f;
+  uint32_t tslot;
+  int bad;
+  PagedPiece piece;
+};
+constexpr int PT_SMEM = LP_Q + (PT_K + 2) * LP_KV + (int)sizeof(PagedShared);
+static_assert(2 * (PT_SMEM + 1024) <= 228 * 1024, "two CTAs an SM");
+
 // One token and head over its visible keys, one at a time: four dims a lane; the row in bf16.
 // (A row that saw nothing, or whose output is not finite.)
 __device__ __noinline__ uint2 paged_one(const PagedAttendArgs& a, int b, int p, int hq, const bf16* q) {
@@ -300,18 +310,20 @@ __device__ __noinline__ uint2 paged_one(const PagedAttendArgs& a, int b, int p, 
 }
 
 __global__ void __launch_bounds__(LP_THREADS, 2) paged_attend_kernel(const __grid_constant__ PagedAttendArgs a) {
-  extern __shared__ __align__(16) unsigned char raw[];
-  unsigned char* sq = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);   // Q; the output tile at the end
-  unsigned char* sk = sq + LP_Q;                                          // [2]
-  unsigned char* sv = sk + 2 * LP_KV;                                     // [2]
-  __shared__ __align__(8) uint64_t bar_k[2], bar_v[2], bar_s[2], bar_f, bar_p[2], bar_o[2];
-  __shared__ uint32_t tslot;
-  __shared__ int s_bad;
-  __shared__ PagedPiece s_piece;
+  // nothing but this: with 1 KB of the system's, two CTAs fill an SM, and the base is at a 1024-byte boundary (checked)
+  extern __shared__ __align__(1024) unsigned char sq[];                   // Q; the output tile at the end
+  unsigned char* sk = sq + LP_Q;                                          // [PT_K]
+  unsigned char* sv = sk + PT_K * LP_KV;                                  // [2]
+  PagedShared& sh = *reinterpret_cast<PagedShared*>(sv + 2 * LP_KV);
+  uint64_t *bar_k = sh.bar_k, *bar_v = sh.bar_v, *bar_s = sh.bar_s, *bar_p = sh.bar_p, *bar_o = sh.bar_o, &bar_f = sh.bar_f;
+  uint32_t& tslot = sh.tslot;
+  int& s_bad = sh.bad;
+  PagedPiece& s_piece = sh.piece;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int x = blockIdx.x / a.NKV, h = blockIdx.x - x * a.NKV;
   if (tid == 0) {
     s_bad = 0;
+    if (smem_u32(sq) & 1023u) set_error(a.err, FB_ERR_DEVICE);
     for (const CUtensorMap* m : {&a.tq, &a.tk, &a.tv, &a.tks, &a.tvs})
       asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
   }
@@ -343,11 +355,13 @@ __global__ void __launch_bounds__(LP_THREADS, 2) paged_attend_kernel(const __gri
   const int* table = a.t.table + piece.b * a.t.table_sb;
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&bar_k[i], 1);
       mbar_init(&bar_v[i], 1);
-      mbar_init(&bar_s[i], 1);
       mbar_init(&bar_p[i], 32 * warps);
       mbar_init(&bar_o[i], 1);
+    }
+    for (int i = 0; i < PT_K; ++i) {
+      mbar_init(&bar_k[i], 1);
+      mbar_init(&bar_s[i], 1);
     }
     mbar_init(&bar_f, 32 * warps);
     fence_mbar_init();
@@ -381,11 +395,11 @@ __global__ void __launch_bounds__(LP_THREADS, 2) paged_attend_kernel(const __gri
       return (unsigned)e < (unsigned)a.t.pages ? e : a.t.pages;   // past the pool: zeros
     };
     int e0 = entries(0), e1 = entries(1);
-    auto load = [&](bool is_v, int t) {
+    auto load = [&](bool is_v, int t, int buf) {
       const int n = min(2, segs - 2 * t), e = (t >> 3) & 1 ? e1 : e0;
       const int qc = (lane >> 1) & 3, pg = __shfl_sync(FULL, e, ((t & 7) << 2) + qc);   // lane 2 c + i: quarter c, half i
-      uint64_t* bar = is_v ? &bar_v[t & 1] : &bar_k[t & 1];
-      unsigned char* dst = (is_v ? sv : sk) + (t & 1) * LP_KV;
+      uint64_t* bar = is_v ? &bar_v[buf] : &bar_k[buf];
+      unsigned char* dst = (is_v ? sv : sk) + buf * LP_KV;
       const int j0 = seg.at(2 * (first + t)), mask = a.t.page - 1;
       if (lane == 0) {
         mbar_arrive_expect_tx(bar, (unsigned)(n * (LP_KV / 2) + (!is_v && t == 0 ? LP_Q : 0)));
@@ -406,15 +420,20 @@ __global__ void __launch_bounds__(LP_THREADS, 2) paged_attend_kernel(const __gri
       }
       __syncwarp();
     };
-    int nk = 0, nv = 0;                            // tiles copied
+    int nk = 0, nv = 0, kb = 0;                    // tiles copied, K's buffer of the next
+    unsigned kp = 1;                               // the parity of its last use
     uint64_t since = 0;
     while (nk < tiles || nv < tiles) {
-      // K and V each as soon as their buffer is free (S of t - 2 has read its K, P V of t - 2 its V)
-      const bool k = __shfl_sync(FULL, nk < tiles && (nk < 2 || mbar_test(&bar_s[nk & 1], ((nk - 2) >> 1) & 1)), 0);
-      if (k) load(false, nk++);
+      // K and V each as soon as their buffer is free (S of t - 3 has read its K, P V of t - 2 its V)
+      const bool k = __shfl_sync(FULL, nk < tiles && (nk < PT_K || mbar_test(&bar_s[kb], kp)), 0);
+      if (k) {
+        load(false, nk++, kb);
+        if (++kb == PT_K) kb = 0, kp ^= 1;
+      }
       const bool v = __shfl_sync(FULL, nv < tiles && (nv < 2 || mbar_test(&bar_o[nv & 1], ((nv - 2) >> 1) & 1)), 0);
       if (v) {
-        load(true, nv++);
+        load(true, nv, nv & 1);
+        ++nv;
         // V has passed a group of eight tiles, so K has: the next group but one takes its place
         if ((nv & 7) == 0) {
           if ((nv >> 3) & 1) e0 = entries((nv >> 3) + 1);
@@ -431,13 +450,13 @@ __global__ void __launch_bounds__(LP_THREADS, 2) paged_attend_kernel(const __gri
       }
     }
     // no copy may be in flight when the CTA ends (after a wait that gave up: nobody else waits for them)
-    for (int t = max(0, nk - 2); t < nk; ++t) lp_wait_warp(&bar_k[t & 1], (t >> 1) & 1, a.err);
+    for (int t = max(0, nk - PT_K); t < nk; ++t) lp_wait_warp(&bar_k[t % PT_K], (t / PT_K) & 1, a.err);
     for (int t = max(0, nv - 2); t < nv; ++t) lp_wait_warp(&bar_v[t & 1], (t >> 1) & 1, a.err);
   } else if (warp == 5) {                          // S: one thread
     const uint64_t dq = tc_desc_sw128(smem_u32(sq)), dk = tc_desc_sw128(smem_u32(sk));
-    auto step = [&](auto buf, int t) -> bool {
+    auto step = [&](auto buf, int t, unsigned parity) -> bool {
       constexpr int B = decltype(buf)::value;
-      if (!lp_wait(&bar_k[B], (t >> 1) & 1, a.err)) return false;
+      if (t >= tiles || !lp_wait(&bar_k[B], parity, a.err)) return false;
       if (t >= 1 && !lp_wait(&bar_f, (t - 1) & 1, a.err)) return false;   // the last tile's scores are in registers
       tc_after();
       const uint32_t idesc = segs - 2 * t >= 2 ? tc_idesc(2 * LP_SEG) : tc_idesc(LP_SEG);
@@ -448,11 +467,14 @@ __global__ void __launch_bounds__(LP_THREADS, 2) paged_attend_kernel(const __gri
       tc_commit(&bar_s[B]);
       return true;
     };
-    if (lane == 0)
-      for (int t = 0; t < tiles; t += 2)
-        if (!step(std::integral_constant<int, 0>(), t) ||
-            (t + 1 < tiles && !step(std::integral_constant<int, 1>(), t + 1)))
-          break;
+    if (lane == 0) {
+      unsigned parity = 0;
+      for (int t = 0; step(std::integral_constant<int, 0>(), t, parity) &&
+                      step(std::integral_constant<int, 1>(), t + 1, parity) &&
+                      step(std::integral_constant<int, 2>(), t + 2, parity);
+           t += PT_K)
+        parity ^= 1;
+    }
     __syncwarp();
   } else if (warp == 6) {                          // P V
     // dims contiguous: two halves of 64, 8-key groups; in a box of n slots the halves are n x 128 bytes apart, and the next
@@ -522,8 +544,11 @@ __global__ void __launch_bounds__(LP_THREADS, 2) paged_attend_kernel(const __gri
     // the reference m of the weights, 2^(score - m + LP_SHIFT); fresh: none yet (a row that sees nothing needs none)
     float m = p < 0 ? 0.f : -INFINITY, off = 0.f, sum = 0.f;
     bool fresh = p >= 0, ok = true;
+    int sb = 0;                                    // S's barrier of the next tile, its parity
+    unsigned sp = 0;
     for (int t = 0; t < tiles; ++t) {
-      ok = lp_wait_warp(&bar_s[t & 1], (t >> 1) & 1, a.err);
+      ok = lp_wait_warp(&bar_s[sb], sp, a.err);
+      if (++sb == PT_K) sb = 0, sp ^= 1;
       if (!ok) break;
       tc_after();
       float s[LP_TILE];
@@ -886,7 +911,7 @@ extern "C" int flashb_paged_attend(const fb_paged_cache* cache, const int32_t* t
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev >= 64 || !attr_done[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(paged_attend_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, LP_SMEM);
+    const cudaError_t e = cudaFuncSetAttribute(paged_attend_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PT_SMEM);
     if (e != cudaSuccess) {
       fbh::set_msg("paged_attend: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
       return FB_ERR_CUDA;
@@ -901,7 +926,7 @@ extern "C" int flashb_paged_attend(const fb_paged_cache* cache, const int32_t* t
     rc = fbh::paged_decode(cache, a.pool, table, table_sb, rows, width, lengths, offsets, T, q, q_st, q_sh, NH, window, sinks,
                            scaling, ws + p.off_singles, out, o_st, o_sh, stream);
   if (!rc)
-    rc = fbh::launch_pdl((const void*)paged_attend_kernel, dim3((unsigned)(p.list * a.NKV)), dim3(LP_THREADS), LP_SMEM, st,
+    rc = fbh::launch_pdl((const void*)paged_attend_kernel, dim3((unsigned)(p.list * a.NKV)), dim3(LP_THREADS), PT_SMEM, st,
                          args, true);
   if (rc || p.cuts < 2) return rc;
   return fbh::launch_pdl((const void*)paged_merge_kernel, dim3((unsigned)(p.cuts / 2 * a.NKV), LP_ROWS / PM_ROWS),
