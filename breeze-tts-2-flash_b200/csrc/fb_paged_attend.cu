@@ -530,7 +530,7 @@ __global__ void __launch_bounds__(LP_THREADS, 2) paged_attend_kernel(const __gri
   } else if (warp < warps) {
     const int r = tid, l = r / a.G;
     const bool mine = r < live;
-    const int p = mine ? p_lo + l : -1;                     // a row without a token sees nothing
+    const int p = mine ? p_lo + l : -1;                     // a row without a token: its weights may be anything
     const uint32_t my = (uint32_t)(warp * 32) << 16;
     const int wnd = a.window > 0 ? a.window : 0x40000000;   // none: more than any row has
     const uint64_t scale2 = f2(a.scale, a.scale);
@@ -558,7 +558,7 @@ __global__ void __launch_bounds__(LP_THREADS, 2) paged_attend_kernel(const __gri
 #pragma unroll
       for (int sg = 0; sg < 2; ++sg) {
         const int j0 = seg.at(2 * (first + t) + sg);
-        if (j0 + LP_SEG - 1 > p_lo || (p_hi - j0 >= wnd && j0 + LP_SEG > a.sinks) || live < 32 * warps || holes) {
+        if (j0 + LP_SEG - 1 > p_lo || (p_hi - j0 >= wnd && j0 + LP_SEG > a.sinks) || holes) {
           // the row's keys of the segment as bits: slots p - window + 1 .. p and the sinks
           uint32_t see = lp_bits(p - wnd + 1 - j0, p + 1 - j0) | lp_bits(0, min(p + 1, a.sinks) - j0);
           if (holes) {
@@ -587,10 +587,15 @@ __global__ void __launch_bounds__(LP_THREADS, 2) paged_attend_kernel(const __gri
           w[c] = pack_bf16(p0, p1);
         }
       };
-      weights();
-      float2 u = f2_get(f2_add(part[0], part[1]));
-      // the tile's sum tells whether a score passes the reference by 2^8 (or there is none yet)
-      if (__any_sync(FULL, !(u.x + u.y <= PT_LIMIT) || fresh)) {
+      bool move = __any_sync(FULL, fresh);
+      float2 u;
+      if (!move) {
+        // the tile's sum tells whether a score passes the reference by 2^8
+        weights();
+        u = f2_get(f2_add(part[0], part[1]));
+        move = __any_sync(FULL, mine && !(u.x + u.y <= PT_LIMIT));
+      }
+      if (move) {
         float x[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
         for (int c = 4; c < 64; c += 4) {
