@@ -45,7 +45,7 @@ struct alignas(64) PagedAttendArgs {
   const bf16* q;
   long long q_st, q_sh;
   int NH, NKV, G, nq, window, sinks;    // nq = 128 / G tokens a CTA; window 0: none
-  int lq;                               // log2 nq
+  int lq, lg;                           // log2 of nq and of G
   int per, pieces, list, cuts;          // rows per thread of the plan; CTAs that the SMs hold a KV head, 0: query tiles stay
   float rounds;                         // whole; entries of the list, of them cut at most; 1 / pieces
   int per32;                            // rows per lane where a CTA finds its query tile itself
@@ -267,6 +267,7 @@ __device__ __forceinline__ PagedPiece paged_direct(const PagedAttendArgs& a, int
   return p;
 }
 
+constexpr int PT_THREADS = 256;                  // 4 softmax warps; one each for S, P V, the copies of K and of V
 constexpr int PT_K = 3;                          // buffers of K: with two, S waited for K a quarter of the time
 struct alignas(16) PagedShared {
   uint64_t bar_k[PT_K], bar_s[PT_K], bar_v[2], bar_p[2], bar_o[2], bar_f;
@@ -309,7 +310,7 @@ __device__ __noinline__ uint2 paged_one(const PagedAttendArgs& a, int b, int p, 
   return make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
 }
 
-__global__ void __launch_bounds__(LP_THREADS, 2) paged_attend_kernel(const __grid_constant__ PagedAttendArgs a) {
+__global__ void __launch_bounds__(PT_THREADS, 2) paged_attend_kernel(const __grid_constant__ PagedAttendArgs a) {
   // nothing but this: with 1 KB of the system's, two CTAs fill an SM, and the base is at a 1024-byte boundary (checked)
   extern __shared__ __align__(1024) unsigned char sq[];                   // Q; the output tile at the end
   unsigned char* sk = sq + LP_Q;                                          // [PT_K]
@@ -382,8 +383,10 @@ __global__ void __launch_bounds__(LP_THREADS, 2) paged_attend_kernel(const __gri
     return segs - 2 * t >= 2 && a.t.page >= LP_TILE && (seg.at(sg) & (LP_TILE - 1)) == 0 && sg != seg.ns - 1;
   };
 
-  if (warp == 4) {                                 // copies: one thread; the warp holds the entries of 16 tiles
-    // lane 4 i + c: the page of quarter c (16 slots) of tile 8 g + i of the piece
+  if (warp == 4 || warp == 7) {                    // copies of K, of V; the warp holds the entries of 16 tiles
+    const bool is_v = warp == 7;
+    const int mask = a.t.page - 1, qc = (lane >> 1) & 3;             // lane 2 c + i: quarter c (16 slots), half i
+    // lane 4 i + c: the page of quarter c of tile 8 g + i of the piece
     auto entries = [&](int g) {
       const int tl = 8 * g + (lane >> 2);
       int e = -1;
@@ -392,66 +395,50 @@ __global__ void __launch_bounds__(LP_THREADS, 2) paged_attend_kernel(const __gri
         // of a page that any row sees a slot of: a box may begin before the first of them
         if (sg < seg.n && j < a.r.S && seen(j & -a.t.page, a.t.page)) e = table[j >> a.t.shift];
       }
-      return (unsigned)e < (unsigned)a.t.pages ? e : a.t.pages;   // past the pool: zeros
+      return (unsigned)e < (unsigned)a.t.pages ? e : a.t.pages;      // past the pool: zeros
     };
-    int e0 = entries(0), e1 = entries(1);
-    auto load = [&](bool is_v, int t, int buf) {
-      const int n = min(2, segs - 2 * t), e = (t >> 3) & 1 ? e1 : e0;
-      const int qc = (lane >> 1) & 3, pg = __shfl_sync(FULL, e, ((t & 7) << 2) + qc);   // lane 2 c + i: quarter c, half i
-      uint64_t* bar = is_v ? &bar_v[buf] : &bar_k[buf];
+    int e0 = entries(0), e1 = entries(1), buf = 0;
+    unsigned parity = 1;                           // of the buffer's last use
+    uint64_t *full = is_v ? bar_v : bar_k, *freed = is_v ? bar_o : bar_s;
+    const int bufs = is_v ? 2 : PT_K;
+    const CUtensorMap *big = is_v ? &a.tv : &a.tk, *little = is_v ? &a.tvs : &a.tks;
+    bool ok = true;
+    int t = 0;
+    for (; t < tiles; ++t) {
+      // everything but the copy itself before the wait
+      const int sg = 2 * (first + t), n = min(2, segs - 2 * t);
+      const int pg = __shfl_sync(FULL, (t >> 3) & 1 ? e1 : e0, ((t & 7) << 2) + qc);
+      const bool one = whole(t);
+      const int j = (one ? seg.at(sg) : seg.at(sg + (qc >> 1)) + 16 * (qc & 1)) & mask;
+      const bool mine = one ? lane == 0
+                            : (qc >> 1) < n && lane < 8 && (small == LP_SEG / 2 || (qc & 1) == 0) && (!is_v || (lane & 1) == 0);
       unsigned char* dst = (is_v ? sv : sk) + buf * LP_KV;
-      const int j0 = seg.at(2 * (first + t)), mask = a.t.page - 1;
-      if (lane == 0) {
-        mbar_arrive_expect_tx(bar, (unsigned)(n * (LP_KV / 2) + (!is_v && t == 0 ? LP_Q : 0)));
-        if (!is_v && t == 0)
-          asm volatile(
-              "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
-              "[%6];" ::"r"(smem_u32(sq)),
-              "l"(&a.tq), "r"(0), "r"(h * a.G), "r"(piece.tok), "r"(0), "r"(smem_u32(bar))
-              : "memory");
-      }
-      if (whole(t)) {
-        if (lane == 0) lp_load(dst, is_v ? &a.tv : &a.tk, j0 & mask, 0, h, pg, bar);
-      } else if ((qc >> 1) < n && lane < 8 && (small == LP_SEG / 2 || (qc & 1) == 0)) {
-        // a lane a box: one thread after the other takes 40 ns each
-        const int j = (seg.at(2 * (first + t) + (qc >> 1)) + 16 * (qc & 1)) & mask;
-        if (!is_v) lp_load(dst + (lane & 1) * (LP_KV / 2) + qc * (LP_KV / 8), &a.tks, j, lane & 1, h, pg, bar);
-        else if ((lane & 1) == 0) lp_load(dst + qc * (LP_KV / 4), &a.tvs, j, 0, h, pg, bar);
-      }
-      __syncwarp();
-    };
-    int nk = 0, nv = 0, kb = 0;                    // tiles copied, K's buffer of the next
-    unsigned kp = 1;                               // the parity of its last use
-    uint64_t since = 0;
-    while (nk < tiles || nv < tiles) {
-      // K and V each as soon as their buffer is free (S of t - 3 has read its K, P V of t - 2 its V)
-      const bool k = __shfl_sync(FULL, nk < tiles && (nk < PT_K || mbar_test(&bar_s[kb], kp)), 0);
-      if (k) {
-        load(false, nk++, kb);
-        if (++kb == PT_K) kb = 0, kp ^= 1;
-      }
-      const bool v = __shfl_sync(FULL, nv < tiles && (nv < 2 || mbar_test(&bar_o[nv & 1], ((nv - 2) >> 1) & 1)), 0);
-      if (v) {
-        load(true, nv, nv & 1);
-        ++nv;
-        // V has passed a group of eight tiles, so K has: the next group but one takes its place
-        if ((nv & 7) == 0) {
-          if ((nv >> 3) & 1) e0 = entries((nv >> 3) + 1);
-          else e1 = entries((nv >> 3) + 1);
-        }
-      }
-      if (k || v) {
-        since = 0;
-      } else if (since == 0) {
-        since = globaltimer();
-      } else if (__any_sync(FULL, globaltimer() - since > WAIT_LIMIT_NS)) {
-        set_error(a.err, FB_ERR_TIMEOUT);
+      if (!one) dst += is_v ? qc * (LP_KV / 4) : (lane & 1) * (LP_KV / 2) + qc * (LP_KV / 8);
+      const unsigned bytes = (unsigned)(n * (LP_KV / 2) + (!is_v && t == 0 ? LP_Q : 0));
+      // free: S of t - 3 has read its K, P V of t - 2 its V
+      if (t >= bufs && !lp_wait_warp(&freed[buf], parity, a.err)) {
+        ok = false;
         break;
+      }
+      if (lane == 0) mbar_arrive_expect_tx(&full[buf], bytes);
+      // a lane a box: one thread after the other takes 40 ns each
+      if (mine) lp_load(dst, one ? big : little, j, one || is_v ? 0 : lane & 1, h, pg, &full[buf]);
+      if (!is_v && t == 0 && lane == 0)
+        asm volatile(
+            "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+            "[%6];" ::"r"(smem_u32(sq)),
+            "l"(&a.tq), "r"(0), "r"(h * a.G), "r"(piece.tok), "r"(0), "r"(smem_u32(&full[buf]))
+            : "memory");
+      __syncwarp();
+      if (++buf == bufs) buf = 0, parity ^= 1;
+      if ((t & 7) == 7) {                          // the next group of eight tiles but one
+        if ((t >> 3) & 1) e1 = entries((t >> 3) + 2);
+        else e0 = entries((t >> 3) + 2);
       }
     }
     // no copy may be in flight when the CTA ends (after a wait that gave up: nobody else waits for them)
-    for (int t = max(0, nk - PT_K); t < nk; ++t) lp_wait_warp(&bar_k[t % PT_K], (t / PT_K) & 1, a.err);
-    for (int t = max(0, nv - 2); t < nv; ++t) lp_wait_warp(&bar_v[t & 1], (t >> 1) & 1, a.err);
+    if (!ok)
+      for (int i = max(0, t - bufs); i < t; ++i) lp_wait_warp(&full[i % bufs], (i / bufs) & 1, a.err);
   } else if (warp == 5) {                          // S: one thread
     const uint64_t dq = tc_desc_sw128(smem_u32(sq)), dk = tc_desc_sw128(smem_u32(sk));
     auto step = [&](auto buf, int t, unsigned parity) -> bool {
@@ -528,17 +515,21 @@ __global__ void __launch_bounds__(LP_THREADS, 2) paged_attend_kernel(const __gri
       if (!step(std::integral_constant<int, 0>(), t) || (t + 1 < tiles && !step(std::integral_constant<int, 1>(), t + 1)))
         break;
   } else if (warp < warps) {
-    const int r = tid, l = r / a.G;
+    const int r = tid, l = r >> a.lg;
     const bool mine = r < live;
     const int p = mine ? p_lo + l : -1;                     // a row without a token: its weights may be anything
     const uint32_t my = (uint32_t)(warp * 32) << 16;
     const int wnd = a.window > 0 ? a.window : 0x40000000;   // none: more than any row has
     const uint64_t scale2 = f2(a.scale, a.scale);
-    // entries that are no page, among those of the piece's slots that are seen
+    // entries that are no page, among those of the piece's slots that are seen (known before the loop: with a flag of the
+    // copying warp's read in every tile the loop was 6% slower)
+    bool hole = false;
+#pragma unroll 8
     for (int i = tid; i < 4 * tiles; i += 32 * warps) {
       const int sg = 2 * first + (i >> 1), j = seg.at(sg) + 16 * (i & 1);
-      if (sg < seg.n && j < a.r.S && seen(j, 16) && (unsigned)table[j >> a.t.shift] >= (unsigned)a.t.pages) s_bad = 1;
+      if (sg < seg.n && j < a.r.S && seen(j, 16)) hole |= (unsigned)table[j >> a.t.shift] >= (unsigned)a.t.pages;
     }
+    if (hole) s_bad = 1;
     named_sync(1, 32 * warps);
     const bool holes = s_bad != 0;
     // the reference m of the weights, 2^(score - m + LP_SHIFT); fresh: none yet (a row that sees nothing needs none)
@@ -702,14 +693,14 @@ __global__ void __launch_bounds__(LP_THREADS, 2) paged_attend_kernel(const __gri
       const int half = lane >> 4, c = lane & 15;
 #pragma unroll 4
       for (int i = 0; i < 32; i += 2) {
-        const int rr = warp * 32 + i + half, ll = rr / a.G, gg = rr - ll * a.G;
+        const int rr = warp * 32 + i + half, ll = rr >> a.lg, gg = rr & (a.G - 1);
         const uint4 y = *reinterpret_cast<const uint4*>(sq + (c >> 3) * (LP_Q / 2) + rr * 128 + (((c & 7) ^ (rr & 7)) << 4));
         if (rr < live && ok)
           *reinterpret_cast<uint4*>(a.out + (long long)(piece.tok + ll) * a.o_st + (h * a.G + gg) * a.o_sh + 8 * c) = y;
       }
       // rows that are not finite, or saw nothing: the warp, a row at a time
       for (unsigned todo = __ballot_sync(FULL, bad && ok && mine); todo; todo &= todo - 1) {
-        const int rr = warp * 32 + __ffs(todo) - 1, ll = rr / a.G, hq = h * a.G + rr - ll * a.G;
+        const int rr = warp * 32 + __ffs(todo) - 1, ll = rr >> a.lg, hq = h * a.G + (rr & (a.G - 1));
         const long long t = piece.tok + ll;
         const uint2 y = paged_one(a, piece.b, p_lo + ll, hq, a.q + t * a.q_st + hq * a.q_sh);
         *reinterpret_cast<uint2*>(a.out + t * a.o_st + hq * a.o_sh + 4 * lane) = y;
@@ -771,7 +762,7 @@ __global__ void __launch_bounds__(PM_THREADS) paged_merge_kernel(const __grid_co
     }
     const float f = 1.f / L;
     uint2 y = make_uint2(pack_bf16(O.x * f, O.y * f), pack_bf16(O.z * f, O.w * f));
-    const int l = r / a.G, hq = h * a.G + r - l * a.G;
+    const int l = r >> a.lg, hq = h * a.G + (r & (a.G - 1));
     const long long t = cut.x + l;
     if (__any_sync(FULL, L == 0.f || !isfinite(L) || !isfinite(O.x + O.y + O.z + O.w))) {
       const int b = paged_row(a.r, (int)t);
@@ -894,7 +885,7 @@ extern "C" int flashb_paged_attend(const fb_paged_cache* cache, const int32_t* t
   if (rc) return rc;
   FB_CHECK_ARG(p.ws_floats == 0 || (ws && ((uintptr_t)ws & 15) == 0 && ws_floats >= p.ws_floats),
                "paged_attend: workspace of %lld floats, %lld needed", (long long)ws_floats, (long long)p.ws_floats);
-  a.NKV = cache->NKV, a.nq = LP_ROWS / a.G, a.lq = a.G == 1 ? 7 : a.G == 2 ? 6 : a.G == 4 ? 5 : 4, a.per = (rows + PP_THREADS - 1) / PP_THREADS, a.pieces = p.pieces, a.list = (int)p.list, a.cuts = (int)p.cuts;
+  a.NKV = cache->NKV, a.nq = LP_ROWS / a.G, a.lg = a.G == 1 ? 0 : a.G == 2 ? 1 : a.G == 4 ? 2 : 3, a.lq = 7 - a.lg, a.per = (rows + PP_THREADS - 1) / PP_THREADS, a.pieces = p.pieces, a.list = (int)p.list, a.cuts = (int)p.cuts;
   a.rounds = p.pieces ? 1.f / p.pieces : 0.f;
   a.po = ws, a.ml = (float2*)(ws + p.off_ml), a.per32 = (rows + 31) / 32, a.plan = p.direct ? nullptr : (PagedPiece*)(ws + p.off_plan), a.cut = (int4*)(ws + p.off_cut);
   a.err = fbh::device_err_ptr();
@@ -931,7 +922,7 @@ extern "C" int flashb_paged_attend(const fb_paged_cache* cache, const int32_t* t
     rc = fbh::paged_decode(cache, a.pool, table, table_sb, rows, width, lengths, offsets, T, q, q_st, q_sh, NH, window, sinks,
                            scaling, ws + p.off_singles, out, o_st, o_sh, stream);
   if (!rc)
-    rc = fbh::launch_pdl((const void*)paged_attend_kernel, dim3((unsigned)(p.list * a.NKV)), dim3(LP_THREADS), PT_SMEM, st,
+    rc = fbh::launch_pdl((const void*)paged_attend_kernel, dim3((unsigned)(p.list * a.NKV)), dim3(PT_THREADS), PT_SMEM, st,
                          args, true);
   if (rc || p.cuts < 2) return rc;
   return fbh::launch_pdl((const void*)paged_merge_kernel, dim3((unsigned)(p.cuts / 2 * a.NKV), LP_ROWS / PM_ROWS),
