@@ -1245,7 +1245,9 @@ extern "C" int flashb_paged_decode(const fb_paged_cache* cache, const int32_t* t
   FB_CHECK_ARG(((uintptr_t)q & 15) == 0 && q_st % 8 == 0 && q_sh % 8 == 0,
                "paged_decode: q must be 16-byte aligned with strides multiple of 8 elements");
   FB_CHECK_ARG(((uintptr_t)out & 7) == 0, "paged_decode: out must be 8-byte aligned");
-  FB_CHECK_ARG(scaling > 0.f, "paged_decode: scaling must be positive");
+  FB_CHECK_ARG(scaling > 0.f && scaling < INFINITY, "paged_decode: scaling must be positive and finite");
+  rc = fbh::paged_apart(pool, rows, NH, q, q_st, q_sh, out, (int64_t)NH * LG_D, LG_D);
+  if (rc) return rc;
   FB_CHECK_ARG(floats == 0 || (ws && ((uintptr_t)ws & 15) == 0 && ws_floats >= floats),
                "paged_decode: workspace of %lld floats, %lld needed", (long long)ws_floats, (long long)floats);
   return fbh::paged_decode(cache, pool, table, table_sb, rows, width, lengths, nullptr, rows, q, q_st, q_sh, NH, window, sinks,

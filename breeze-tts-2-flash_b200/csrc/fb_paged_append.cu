@@ -170,14 +170,14 @@ __global__ void __launch_bounds__(PA_THREADS, PA_CTAS) paged_append_kernel(const
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] *= f * g[e];
       }
-      if (a.interleaved) {
+      if (turn && a.interleaved) {                           // (the other lanes' dims stay: 0 x an infinity is not 0)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float q = v[2 * e], m = v[2 * e + 1];
           v[2 * e] = q * cs[e].x - m * cs[e].y;
           v[2 * e + 1] = m * cs[e].x + q * cs[e].y;
         }
-      } else {
+      } else if (turn) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float q = v[e], m = v[4 + e];
@@ -224,6 +224,17 @@ int paged_pool(const fb_paged_cache* c, fb::PagedPool* out) {
 int paged_width(const fb_paged_cache* c, int rows, int width) {
   FB_CHECK_ARG(rows >= 1 && width >= 1, "paged rows: bad shape rows=%d width=%d", rows, width);
   FB_CHECK_ARG((int64_t)width * c->page <= 0x3fffff00, "paged rows: %d pages of %d slots a row", width, c->page);
+  return FB_OK;
+}
+
+int paged_apart(const fb::PagedPool& c, int T, int NH, const void* q, int64_t q_st, int64_t q_sh, const void* out, int64_t o_st,
+                int64_t o_sh) {
+  const LongBox o = long_box(out, 1, T, NH, 0, 2 * o_st, 2 * o_sh, 2 * fb::LG_D);
+  FB_CHECK_ARG(!long_boxes_meet(o, long_box(q, 1, T, NH, 0, 2 * q_st, 2 * q_sh, 2 * fb::LG_D)),
+               "paged attention: out and q share memory");
+  FB_CHECK_ARG(!long_boxes_meet(o, long_box(c.k, c.pages, c.NKV, c.page, c.k_sb, c.k_sh, c.k_sl, 2 * fb::LG_D)) &&
+                   !long_boxes_meet(o, long_box(c.v, c.pages, c.NKV, c.page, c.v_sb, c.v_sh, c.v_sl, 2 * fb::LG_D)),
+               "paged attention: out and the cache share memory");
   return FB_OK;
 }
 

@@ -866,7 +866,7 @@ extern "C" int flashb_paged_attend(const fb_paged_cache* cache, const int32_t* t
   FB_CHECK_ARG(table_sb >= 0, "paged_attend: table stride %lld", (long long)table_sb);
   FB_CHECK_ARG(T >= 1 && (int64_t)T * NH <= 0x7fffffff, "paged_attend: %d tokens of %d heads", T, NH);
   FB_CHECK_ARG(sinks >= 0, "paged_attend: sinks %d", sinks);
-  FB_CHECK_ARG(scaling > 0.f, "paged_attend: scaling must be positive");
+  FB_CHECK_ARG(scaling > 0.f && scaling < INFINITY, "paged_attend: scaling must be positive and finite");
   FB_CHECK_ARG((((uintptr_t)q | (uintptr_t)out) & 15) == 0 && (q_st | q_sh | o_st | o_sh) % 8 == 0,
                "paged_attend: tensors must be 16-byte aligned with strides multiple of 8 elements");
   FB_CHECK_ARG((T == 1 || (q_st > 0 && o_st > 0)) && (NH == 1 || (q_sh > 0 && o_sh > 0)),
@@ -875,6 +875,8 @@ extern "C" int flashb_paged_attend(const fb_paged_cache* cache, const int32_t* t
                "paged_attend: strides of the cache must be positive");
   FB_CHECK_ARG(!fbh::long_box_folds(fbh::long_box(out, 1, T, NH, 0, 2 * o_st, 2 * o_sh, 2 * LG_D)),
                "paged_attend: rows of out share memory");
+  rc = fbh::paged_apart(a.pool, T, NH, q, q_st, q_sh, out, o_st, o_sh);
+  if (rc) return rc;
   a.t = PagedTable{table, table_sb, a.pool.pages, a.pool.page, a.pool.shift};
   a.r = PagedRows{(const long long*)lengths, (const long long*)offsets, rows, T, width * a.pool.page};
   a.q = (const bf16*)q, a.q_st = q_st, a.q_sh = q_sh, a.NH = NH, a.G = NH / cache->NKV;
