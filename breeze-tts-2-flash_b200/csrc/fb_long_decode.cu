@@ -36,6 +36,12 @@
 // The maximum moves only when a tile's exceeds it by 2^8: the sums are exact either way, and the 32 accumulators are
 // rescaled a few times a piece instead of every tile, and the lanes that share a head compare maxima only then (with the
 // scale and the subtraction in one multiply-add, two scores an instruction: 40.4 to 39.3 us at the 4-bit case above).
+//
+// PAGED: slot j of a row lies in page table[j >> shift] of a pool.  A warp's tile of 16 keys is in one page (pages have 16
+// slots at least, and a window's numbering begins at a multiple of 16), whose entry is read a tile ahead; a tile whose entry is
+// no page is left out.  Rows may be those of a step whose run is one token, the others left alone.  128 ragged rows of up
+// to 8192 slots (1.07 GB) 179 us in a CUDA graph and 166 a call among others, 0.92 to 0.98 of the measured copy bandwidth, in
+// pages of 16 as of 64, in order or not; 2 rows of 2049 slots 7.7 us.
 #include <cooperative_groups.h>
 
 #include <cfloat>

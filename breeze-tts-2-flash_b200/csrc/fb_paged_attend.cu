@@ -3,26 +3,42 @@
 //
 //   out_t = softmax(scaling q_t k^T over the slots that t sees) v, fp32, rounded once; without a visible slot 0.
 //
-// The pipeline is fb_long_prefill.cu's (which see): 128 rows a CTA, 64-key tiles of two 32-key segments, S and P V by a
-// thread each, two CTAs an SM, a row's maximum moved only past 2^8.  What differs:
+// The pipeline is fb_long_prefill.cu's: 128 rows a CTA, 64-key tiles of two 32-key segments, S = Q K^T and O += P V issued by
+// a thread each, P kept in TMEM, four softmax warps with a thread per row, two CTAs an SM.  What differs:
 //
 // Rows of a tile are the run's tokens in order with the G heads of a KV head inner, so a run of few tokens fills the first
-// warps alone; the others do not take part.  Keys come from pages: a segment is one box of 32 slots, or two of 16; a tile of
-// 64 slots in one page is one box.  An entry that is no page is loaded from past the pool's end, which reads as zeros, and
+// warps alone; the others do not take part.  Keys come from pages: a tile in one page is one box, else 32-key segments are
+// boxes of 32 slots or two of 16.  An entry that is no page is loaded from past the pool's end, which reads as zeros, and
 // its slots get no weight.
 //
+// The weights are 2^(s - m - 24) with a reference m of the row's own that is hardly ever moved: they are taken with the old
+// m first, and only when a tile's sum shows that some score passed it by 2^8 is the tile's maximum worked out, O and the
+// sum rescaled and the weights taken again.  (The maximum first, for every tile: 600 instead of 530 us at the largest
+// case below.  The sums are exact either way; sum and reference are fp32, P goes to bf16, one part, as in the prefill.)
+//
 // Pieces.  A step can be one run of a few tokens over a long row, or many rows of which some are long.  So the key tiles of
-// a query tile are cut into s pieces, s = ceil(k / C) with k its row's key tiles; a CTA takes one piece.  paged_plan_kernel
-// (one CTA, from lengths and offsets on the device: nothing is read on the host) writes the list; C is chosen among those
-// with which the list fills one to PT_WAVES rounds of the SMs, and whole query tiles, by what the rounds take.  Pieces of a
-// query tile leave (maximum, sum, unnormalised out) in the workspace and paged_merge_kernel joins them in order: no atomics,
-// the same inputs give the same bits.  A query tile of one piece writes its rows itself.
+// a query tile are cut into s pieces of about C; a CTA takes one piece.  paged_plan_kernel (one CTA, from lengths and offsets
+// on the device: nothing is read on the host) writes the list; C is chosen among those with which the list fills one to
+// PT_WAVES rounds of the SMs, and whole query tiles, by what the rounds take (where rows are too short to cut, there is no
+// plan and CTAs find their query tiles themselves: a short prompt 11.2 instead of 15.0 us).  Pieces of a query tile leave
+// (reference, sum, unnormalised out) in the workspace and paged_merge_kernel joins them in order: no atomics, the same
+// inputs give the same bits.  A query tile of one piece writes its rows itself.
 //
 // Rows of one token go through the single-token kernel (fb_long_decode.cu) where a row has few tokens on average.
 //
 // Slots that no row of the CTA sees may hold anything: in V they are zeroed in shared memory (0 times a NaN is NaN), in K
 // their scores are replaced.  A row whose output is not finite all the same (a NaN that another row of the tile sees) is
 // computed again, one visible key at a time.
+//
+// Measured on a B200 (in a CUDA graph, 16 heads over 4): 2048 tokens over 32768 slots of one row 520 us, 1090 TFLOP/s, in
+// pages of 16 to 128 alike; 801 tokens of 32 rows over a window of 2048 (131 MB) 51 us; 512 tokens of one row beside one each
+// of 63, over up to 8000 slots (530 MB), 128 us; two prompts of 197 tokens 10 to 11 us.  A tile takes 1500 cycles with two
+// CTAs an SM: 700 to 870 are exponentials (the unit's bound for both CTAs is 1024), 100 the read of S, 240 masks, the rest
+// waits and stores; issuing S takes its thread 480 cycles and P V 290, both beside the exponentials.  Under the largest
+// case's load clocks fall to 1.5 GHz.  With few keys a piece it is beginning and ending (9000 cycles) that counts.  Tried
+// and slower: one copying warp for K and V (8 boxes one after the other take 900 cycles), a flag for missing pages read in
+// the loop (6%), arrivals by one lane a warp (4%), P V's waits by one lane (10%), cuts priced with the joins (10% at the
+// window), the second CTA of an SM begun half a tile later (the same).
 #include <climits>
 
 #include "fb_long_tc.cuh"
@@ -30,7 +46,7 @@
 
 namespace fb {
 
-constexpr int PT_MIN = 8;                         // key tiles of a piece, at least
+constexpr int PT_MIN = 8;                         // key tiles of a piece, at least (4 and 2: no faster, and more calls need a plan)
 constexpr int PT_WAVES = 4;                       // rounds of CTAs that the list of pieces may be cut for
 constexpr float PT_LIMIT = 0x1p-16f;              // 2^(8 + LP_SHIFT): a tile's weights below it leave the reference as it is
 constexpr int PT_COST = 5;                        // what beginning and ending a piece takes, in key tiles
@@ -788,8 +804,9 @@ int paged_group(const fb_paged_cache* c, int NH) {
   return FB_OK;
 }
 
-// Rows of one token go through the single-token kernel, a launch of its own before this one, where a row has few tokens on
-// average: it reads their keys at 0.95 of the copy bandwidth where a tile of 128 rows, G of them in use, reaches 0.8.
+// Rows of one token go through the single-token kernel, a launch of its own before this one, where a row has at most so many
+// tokens on average: it reads their keys at 0.95 of the copy bandwidth where a tile of 128 rows, G of them in use, reaches 0.8
+// (512 tokens of one row beside 63 of others, 9 a row: 137 instead of 175 us; with no such row it costs 5 us).
 constexpr int PT_SINGLES = 16;
 struct PagedPlan {
   int pieces;                           // a KV head, 0: query tiles stay whole

@@ -10,6 +10,9 @@ Drop-in modules with the call surface of the reference's hook package (AsherHou/
                        (no reference module: the reference runs the eager layers with its attention hook)
   flashb.longform      windowed attention with sinks, 4-bit KV cache, eviction by attention weight (no reference module)
   flashb.long_speech   the backbone prefill and decode step on those caches; ``python -m flashb.long_speech``
+  flashb.paged         a paged cache of many rows: rotary positions and K / V into pages, attention of runs of tokens
+  flashb.paged_speech  the backbone on it, prompts in chunks beside other rows' frames; ``python -m flashb.paged_speech``
+  flashb.sampling      the backbone sampler (flash/sampling.py); ``token_scores``: log probabilities of given tokens
 
 ``install(api)`` installs the hot-path hooks on the official runtime, as ``flash.install`` does for them
 (``flash/__init__.py:37-70``; the reference's other hooks -- weight packing, codec, streaming loop, reference cache --
