@@ -39,7 +39,7 @@
 //
 // PAGED: slot j of a row lies in page table[j >> shift] of a pool.  A warp's tile of 16 keys is in one page (pages have 16
 // slots at least, and a window's numbering begins at a multiple of 16), whose entry is read a tile ahead; a tile whose entry is
-// no page is left out.  Rows may be those of a step whose run is one token, the others left alone.  128 ragged rows of up
+// no page is left out.  128 ragged rows of up
 // to 8192 slots (1.07 GB) 179 us in a CUDA graph and 166 a call among others, 0.92 to 0.98 of the measured copy bandwidth, in
 // pages of 16 as of 64, in order or not; 2 rows of 2049 slots 7.7 us.
 #include <cooperative_groups.h>
@@ -83,16 +83,12 @@ struct LongDecodeArgs {
   int cap;                              // visible keys a row can have
   bf16* out;
   PagedTable t;                         // a paged cache: c.k_sb and c.v_sb are the pages' strides
-  const long long* offsets;             // paged: rows with a run of one token alone (null: token b is row b's); T tokens
-  int T;
-  long long o_st, o_sh;                 // paged: strides of out
 };
 
 // Paged: the visible keys' numbering begins at a multiple of 16 slots (sinks end at one), so that a warp's tile of 16 lies
 // in one page; what it holds beside visible keys gets no weight.
 struct LongPagedRow : LongRow {
   int vlo, vns;                         // visible: slots below vns, and from vlo on
-  int tok;                              // the row's token, -1: the row has another number of them and is left alone
   __device__ __forceinline__ bool sees(int j) const { return (j >= vlo || j < vns) && index(j) >= 0; }
 };
 template <bool PAGED>
@@ -165,12 +161,7 @@ template <bool PAGED>
 __device__ __forceinline__ LongRowOf<PAGED> long_row_of(const LongDecodeArgs& a, int b) {
   if constexpr (PAGED) {
     LongPagedRow r;
-    r.tok = b;
-    if (a.offsets) {
-      const long long f = a.offsets[b];
-      r.tok = f >= 0 && f < a.T && a.offsets[b + 1] == f + 1 ? (int)f : -1;
-    }
-    const LongRow x = long_row(r.tok < 0 ? 0 : a.lengths[b], 0, a.S, a.window, a.sinks);
+    const LongRow x = long_row(a.lengths[b], 0, a.S, a.window, a.sinks);
     const int lo = x.lo & ~15, ns = (x.ns + 15) & ~15, end = x.lo + x.n - x.ns;
     r.st = 0, r.vlo = x.lo, r.vns = x.ns;
     r.ns = ns < lo ? ns : 0;
@@ -320,9 +311,7 @@ __device__ __forceinline__ void long_piece(const LongDecodeArgs& a, int b, int h
   const int qh = BITS == 16 && G <= 4 ? g & 3 : g;
   float scA = a.scale, scB = a.scale;
   {
-    int at = b;
-    if constexpr (PAGED) at = max(row.tok, 0);
-    const bf16* qp = a.q + at * a.q_sb + (long long)(h * G + qh) * a.q_sh;
+    const bf16* qp = a.q + b * a.q_sb + (long long)(h * G + qh) * a.q_sh;
     uint4 w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -712,14 +701,8 @@ __global__ void __launch_bounds__(LD_THREADS, LongTile<BITS>::CTAS) long_cluster
         L += f * lv[c];
         O += f * ov[c];
       }
-    bool none = row.n == 0;
-    bf16* out = a.out + ((long long)b * a.NH + h * G + gg) * LG_D;
-    if constexpr (PAGED) {
-      if (row.tok < 0) break;
-      none = M == -INFINITY;
-      out = a.out + row.tok * a.o_st + (h * G + gg) * a.o_sh;
-    }
-    out[tid] = __float2bfloat16_rn(none ? 0.f : O / L * a.v_scale);
+    const bool none = PAGED ? M == -INFINITY : row.n == 0;
+    a.out[((long long)b * a.NH + h * G + gg) * LG_D + tid] = __float2bfloat16_rn(none ? 0.f : O / L * a.v_scale);
   }
   if constexpr (SCORED) {
     if (tid < G) {
@@ -822,8 +805,6 @@ __global__ void __launch_bounds__(LM_THREADS, 8) long_merge_kernel(const __grid_
   const auto row = long_row_of<PAGED>(a, b);    // written at least two launches back
   pdl_wait();
   pdl_trigger();
-  if constexpr (PAGED)
-    if (row.tok < 0) return;
   const int2 own = row.n > 0 ? a.own[r] : make_int2(0, -1);   // CTAs [x, y] hold pieces of this row
   // a head's maximum and sum over the pieces (every lane)
   auto stats = [&](int gg, float& M, float& L) {
@@ -870,13 +851,8 @@ __global__ void __launch_bounds__(LM_THREADS, 8) long_merge_kernel(const __grid_
     }
     // visible keys with scores of -inf alone: 0 / 0, as softmax has it
     const float f = a.v_scale / L;
-    bool none = row.n == 0;
-    bf16* out = a.out + ((long long)b * a.NH + h * G + gg) * LG_D;
-    if constexpr (PAGED) {
-      none = M == -INFINITY;
-      out = a.out + row.tok * a.o_st + (h * G + gg) * a.o_sh;
-    }
-    *reinterpret_cast<uint2*>(out + 4 * lane) =
+    const bool none = PAGED ? M == -INFINITY : row.n == 0;
+    *reinterpret_cast<uint2*>(a.out + ((long long)b * a.NH + h * G + gg) * LG_D + 4 * lane) =
         make_uint2(none ? 0u : pack_bf16(O.x * f, O.y * f), none ? 0u : pack_bf16(O.z * f, O.w * f));
     return;
   }
@@ -1193,47 +1169,14 @@ fb_kv_cache paged_shape(const fb_paged_cache* c, int rows, int width) {
 constexpr int PAGED_EDGES = 30;        // a window's first tile and the sinks' last, at most 15 slots each
 }  // namespace
 
-int fbh::paged_decode_floats(const fb_paged_cache* cache, int rows, int width, int NH, int window, int sinks, int64_t* floats) {
-  LongPlan p{};
-  const fb_kv_cache shape = paged_shape(cache, rows, width);
-  const int rc = long_plan_host(&shape, NH, window, sinks, false, &p, PAGED_EDGES);
-  *floats = p.ws_floats;
-  return rc;
-}
-
-int fbh::paged_decode(const fb_paged_cache* cache, const fb::PagedPool& pool, const int32_t* table, int64_t table_sb, int rows,
-                      int width, const int64_t* lengths, const int64_t* offsets, int T, const void* q, int64_t q_st,
-                      int64_t q_sh, int NH, int window, int sinks, float scaling, float* ws, void* out, int64_t o_st,
-                      int64_t o_sh, void* stream) {
-  LongDecodeArgs a{};
-  const fb_kv_cache shape = paged_shape(cache, rows, width);
-  LongPlan p{};
-  const int rc = long_plan_host(&shape, NH, window, sinks, false, &p, PAGED_EDGES);
-  if (rc) return rc;
-  a.c.k = pool.k, a.c.v = pool.v;
-  a.c.k_sb = pool.k_sb, a.c.k_sh = pool.k_sh, a.c.k_sp = pool.k_sl;
-  a.c.v_sb = pool.v_sb, a.c.v_sh = pool.v_sh, a.c.v_sp = pool.v_sl;
-  a.t = fb::PagedTable{table, table_sb, pool.pages, pool.page, pool.shift};
-  a.q = (const bf16*)q, a.q_sb = q_st, a.q_sh = q_sh, a.lengths = (const long long*)lengths;
-  a.offsets = (const long long*)offsets, a.T = T;
-  a.B = rows, a.NH = NH, a.NKV = cache->NKV, a.G = NH / cache->NKV, a.S = shape.S;
-  a.window = window > 0 ? window : 0, a.sinks = sinks, a.ncta = p.ncta;
-  a.scale = std::fmax(scaling * LG_LOG2E, FLT_MIN);
-  a.dense = pool.k_sl == 256 && pool.v_sl == 256;
-  a.v_scale = 1.f, a.shift = LongTile<16>::SHIFT, a.decay = 1.f;
-  a.po = ws, a.ml = (float2*)(ws + p.off_ml), a.own = (int2*)(ws + p.off_own);
-  a.per = (a.B + 31) / 32, a.cap = p.cap, a.out = (bf16*)out, a.o_st = o_st, a.o_sh = o_sh;
-  return long_launch<16, false, true>(a, p, (cudaStream_t)stream);
-}
-
 extern "C" int64_t flashb_paged_decode_ws_floats(const fb_paged_cache* cache, int rows, int width, int NH, int window,
                                                  int sinks) {
   fb::PagedPool pool;
-  int64_t floats;
-  if (fbh::paged_pool(cache, &pool) || fbh::paged_width(cache, rows, width) ||
-      fbh::paged_decode_floats(cache, rows, width, NH, window, sinks, &floats))
-    return -1;
-  return floats;
+  LongPlan p{};
+  if (fbh::paged_pool(cache, &pool) != FB_OK || fbh::paged_width(cache, rows, width) != FB_OK) return -1;
+  const fb_kv_cache shape = paged_shape(cache, rows, width);
+  if (long_plan_host(&shape, NH, window, sinks, false, &p, PAGED_EDGES) != FB_OK) return -1;
+  return p.ws_floats;
 }
 
 extern "C" int flashb_paged_decode(const fb_paged_cache* cache, const int32_t* table, int64_t table_sb, int rows, int width,
@@ -1245,8 +1188,10 @@ extern "C" int flashb_paged_decode(const fb_paged_cache* cache, const int32_t* t
   if (rc) return rc;
   FB_CHECK_ARG(q && lengths && out && table, "paged_decode: null pointer argument");
   FB_CHECK_ARG(table_sb >= 0, "paged_decode: table stride %lld", (long long)table_sb);
-  int64_t floats = 0;
-  rc = fbh::paged_decode_floats(cache, rows, width, NH, window, sinks, &floats);
+  LongDecodeArgs a{};
+  LongPlan p{};
+  const fb_kv_cache shape = paged_shape(cache, rows, width);
+  rc = long_plan_host(&shape, NH, window, sinks, false, &p, PAGED_EDGES);
   if (rc) return rc;
   FB_CHECK_ARG(((uintptr_t)q & 15) == 0 && q_st % 8 == 0 && q_sh % 8 == 0,
                "paged_decode: q must be 16-byte aligned with strides multiple of 8 elements");
@@ -1254,8 +1199,19 @@ extern "C" int flashb_paged_decode(const fb_paged_cache* cache, const int32_t* t
   FB_CHECK_ARG(scaling > 0.f && scaling < INFINITY, "paged_decode: scaling must be positive and finite");
   rc = fbh::paged_apart(pool, rows, NH, q, q_st, q_sh, out, (int64_t)NH * LG_D, LG_D);
   if (rc) return rc;
-  FB_CHECK_ARG(floats == 0 || (ws && ((uintptr_t)ws & 15) == 0 && ws_floats >= floats),
-               "paged_decode: workspace of %lld floats, %lld needed", (long long)ws_floats, (long long)floats);
-  return fbh::paged_decode(cache, pool, table, table_sb, rows, width, lengths, nullptr, rows, q, q_st, q_sh, NH, window, sinks,
-                           scaling, ws, out, (int64_t)NH * LG_D, LG_D, stream);
+  FB_CHECK_ARG(p.ws_floats == 0 || (ws && ((uintptr_t)ws & 15) == 0 && ws_floats >= p.ws_floats),
+               "paged_decode: workspace of %lld floats, %lld needed", (long long)ws_floats, (long long)p.ws_floats);
+  a.c.k = pool.k, a.c.v = pool.v;
+  a.c.k_sb = pool.k_sb, a.c.k_sh = pool.k_sh, a.c.k_sp = pool.k_sl;
+  a.c.v_sb = pool.v_sb, a.c.v_sh = pool.v_sh, a.c.v_sp = pool.v_sl;
+  a.t = fb::PagedTable{table, table_sb, pool.pages, pool.page, pool.shift};
+  a.q = (const bf16*)q, a.q_sb = q_st, a.q_sh = q_sh, a.lengths = (const long long*)lengths;
+  a.B = rows, a.NH = NH, a.NKV = cache->NKV, a.G = NH / cache->NKV, a.S = shape.S;
+  a.window = window > 0 ? window : 0, a.sinks = sinks, a.ncta = p.ncta;
+  a.scale = std::fmax(scaling * LG_LOG2E, FLT_MIN);
+  a.dense = pool.k_sl == 256 && pool.v_sl == 256;
+  a.v_scale = 1.f, a.shift = LongTile<16>::SHIFT, a.decay = 1.f;
+  a.po = ws, a.ml = (float2*)(ws + p.off_ml), a.own = (int2*)(ws + p.off_own);
+  a.per = (a.B + 31) / 32, a.cap = p.cap, a.out = (bf16*)out;
+  return long_launch<16, false, true>(a, p, (cudaStream_t)stream);
 }

@@ -65,11 +65,4 @@ int paged_width(const fb_paged_cache* c, int rows, int width);
 // Refuses an out [T, NH, 128] that shares memory with q or the cache.
 int paged_apart(const fb::PagedPool& c, int T, int NH, const void* q, int64_t q_st, int64_t q_sh, const void* out, int64_t o_st,
                 int64_t o_sh);
-// Single-token attention (fb_long_decode.cu; arguments checked by the caller) of the rows whose run is one token (offsets
-// null: token b is row b's), and the floats of workspace that it takes.
-int paged_decode_floats(const fb_paged_cache* cache, int rows, int width, int NH, int window, int sinks, int64_t* floats);
-int paged_decode(const fb_paged_cache* cache, const fb::PagedPool& pool, const int32_t* table, int64_t table_sb, int rows,
-                 int width, const int64_t* lengths, const int64_t* offsets, int T, const void* q, int64_t q_st,
-                 int64_t q_sh, int NH, int window, int sinks, float scaling, float* ws, void* out, int64_t o_st,
-                 int64_t o_sh, void* stream);
 }  // namespace fbh

@@ -24,7 +24,8 @@
 // (reference, sum, unnormalised out) in the workspace and paged_merge_kernel joins them in order: no atomics, the same
 // inputs give the same bits.  A query tile of one piece writes its rows itself.
 //
-// Rows of one token go through the single-token kernel (fb_long_decode.cu) where a row has few tokens on average.
+// Rows of one token are runs as others are.  (The single-token kernel for them, in a launch of its own: 128 instead of 133 us
+// for 512 tokens beside 63 single ones over long rows, but 19 instead of 14 over short ones, and 5 us where there are none.)
 //
 // Slots that no row of the CTA sees may hold anything: in V they are zeroed in shared memory (0 times a NaN is NaN), in K
 // their scores are replaced.  A row whose output is not finite all the same (a NaN that another row of the tile sees) is
@@ -65,7 +66,6 @@ struct alignas(64) PagedAttendArgs {
   int per, pieces, list, cuts;          // rows per thread of the plan; CTAs that the SMs hold a KV head, 0: query tiles stay
   float rounds;                         // whole; entries of the list, of them cut at most; 1 / pieces
   int per32;                            // rows per lane where a CTA finds its query tile itself
-  int singles;                          // rows of one token are another launch's
   float scale;                          // scaling x log2(e)
   bf16* out;
   long long o_st, o_sh;
@@ -104,7 +104,7 @@ __device__ __forceinline__ PagedSegs paged_segs(const PagedAttendArgs& a, int p_
 // repeated: the plan is one pass over cold instructions, which cost it more than its arithmetic.
 __device__ __noinline__ int2 paged_tiles(const PagedAttendArgs& a, int b) {
   const PagedSpan x = paged_span(a.r, b);
-  if (x.n <= 0 || (a.singles && x.n == 1)) return make_int2(0, 0);
+  if (x.n <= 0) return make_int2(0, 0);
   const int p_hi = x.p0 + x.n - 1;
   return make_int2((x.n + a.nq - 1) >> a.lq, (paged_segs(a, p_hi - min(x.n, a.nq) + 1, p_hi).n + 1) >> 1);
 }
@@ -344,9 +344,7 @@ __global__ void __launch_bounds__(PT_THREADS, 2) paged_attend_kernel(const __gri
     for (const CUtensorMap* m : {&a.tq, &a.tk, &a.tv, &a.tks, &a.tvs})
       asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
   }
-  // With single tokens in a launch between the plan and this one, that launch began after the plan had ended; what it writes
-  // is not read here.  It is waited for at the end, so that it has ended when this one has.
-  if (!a.singles) pdl_wait();
+  pdl_wait();
   pdl_trigger();
   PagedPiece piece;
   if (a.plan) {
@@ -359,10 +357,7 @@ __global__ void __launch_bounds__(PT_THREADS, 2) paged_attend_kernel(const __gri
     __syncthreads();
     piece = s_piece;
   }
-  if (piece.b < 0) {
-    if (a.singles) pdl_wait();
-    return;
-  }
+  if (piece.b < 0) return;
   const int p_lo = piece.p_lo, p_hi = p_lo + piece.nt - 1;
   const int live = piece.nt * a.G, warps = (live + 31) >> 5;
   const PagedSegs seg = paged_segs(a, p_lo, p_hi);
@@ -729,7 +724,6 @@ __global__ void __launch_bounds__(PT_THREADS, 2) paged_attend_kernel(const __gri
     tc_after();
     tc_dealloc(tmem, LP_COLS);
   }
-  if (a.singles) pdl_wait();
 }
 
 // Joins the pieces of the query tiles that were cut, in their order: a CTA per PM_ROWS rows of a query tile and head (801
@@ -804,14 +798,10 @@ int paged_group(const fb_paged_cache* c, int NH) {
   return FB_OK;
 }
 
-// Rows of one token go through the single-token kernel, a launch of its own before this one, where a row has at most so many
-// tokens on average: it reads their keys at 0.95 of the copy bandwidth where a tile of 128 rows, G of them in use, reaches 0.8
-// (512 tokens of one row beside 63 of others, 9 a row: 137 instead of 175 us; with no such row it costs 5 us).
-constexpr int PT_SINGLES = 16;
 struct PagedPlan {
   int pieces;                           // a KV head, 0: query tiles stay whole
-  bool singles, direct;                 // direct: nothing to cut and no other launch: no plan, CTAs find their query tiles
-  int64_t list, cuts, slots, off_ml, off_plan, off_cut, off_singles, ws_floats;
+  bool direct;                          // nothing to cut: no plan, CTAs find their query tiles
+  int64_t list, cuts, slots, off_ml, off_plan, off_cut, ws_floats;
 };
 int paged_plan_host(const fb_paged_cache* c, int rows, int width, int T, int NH, int window, int sinks, PagedPlan* p) {
   const int nq = LP_ROWS / (NH / c->NKV);
@@ -821,10 +811,9 @@ int paged_plan_host(const fb_paged_cache* c, int rows, int width, int T, int NH,
   int64_t keys = S;
   if (window > 0 && (int64_t)window + sinks + nq + 3 * LP_SEG < S) keys = (int64_t)window + sinks + nq + 3 * LP_SEG;
   const int64_t most = (keys + LP_TILE - 1) / LP_TILE;
-  p->singles = rows > 1 && T <= (int64_t)PT_SINGLES * rows;
   // CTAs that the SMs hold.  By the device's SMs, not the calling thread's budget: the workspace's size goes by it.
   p->pieces = most > PT_MIN ? (2 * fbh::num_sms() + c->NKV - 1) / c->NKV : 0;
-  p->direct = p->pieces == 0 && !p->singles;
+  p->direct = p->pieces == 0;
   // a list is cut for PT_WAVES rounds at most and into pieces of PT_MIN at least, or is its query tiles
   p->cuts = (int64_t)PT_WAVES * p->pieces;
   if (p->cuts > units * ((most + PT_MIN - 1) / PT_MIN)) p->cuts = units * ((most + PT_MIN - 1) / PT_MIN);
@@ -834,14 +823,7 @@ int paged_plan_host(const fb_paged_cache* c, int rows, int width, int T, int NH,
   p->off_ml = p->slots * LP_ROWS * LG_D;
   p->off_plan = p->off_ml + p->slots * LP_ROWS * 2;
   p->off_cut = p->off_plan + (p->direct ? 0 : p->list * (int64_t)(sizeof(PagedPiece) / 4));
-  p->off_singles = p->off_cut + p->cuts / 2 * 4;
-  p->ws_floats = p->off_singles;
-  if (p->singles) {
-    int64_t floats;
-    const int rc = fbh::paged_decode_floats(c, rows, width, NH, window, sinks, &floats);
-    if (rc) return rc;
-    p->ws_floats += floats;
-  }
+  p->ws_floats = p->off_cut + p->cuts / 2 * 4;
   return FB_OK;
 }
 
@@ -933,13 +915,9 @@ extern "C" int flashb_paged_attend(const fb_paged_cache* cache, const int32_t* t
     }
     if (dev < 64) attr_done[dev] = 1;
   }
-  a.singles = p.singles;
   const cudaStream_t st = (cudaStream_t)stream;
   void* args[] = {(void*)&a};
   if (!p.direct) rc = fbh::launch_pdl((const void*)paged_plan_kernel, dim3(1), dim3(PP_THREADS), 0, st, args, true);
-  if (!rc && p.singles)
-    rc = fbh::paged_decode(cache, a.pool, table, table_sb, rows, width, lengths, offsets, T, q, q_st, q_sh, NH, window, sinks,
-                           scaling, ws + p.off_singles, out, o_st, o_sh, stream);
   if (!rc)
     rc = fbh::launch_pdl((const void*)paged_attend_kernel, dim3((unsigned)(p.list * a.NKV)), dim3(PT_THREADS), PT_SMEM, st,
                          args, true);
