@@ -77,6 +77,19 @@ def test_rows_whose_largest_logits_crowd():
     check(x.bfloat16()[:, 3:], t - 3, 5, 0.5)
 
 
+@pytest.mark.parametrize('V,top', [(100, 32), (276, 32), (300, 9), (511, 20), (600, 31)])
+def test_small_vocabularies_many_alternatives(V, top):
+    """More logits at the threshold than two a thread, with ties among the last that count."""
+    g = torch.Generator().manual_seed(V)
+    x = 2 * torch.randn(40, V, generator=g)
+    x[:10] = x[:10].round()
+    x[10] = 1.0
+    x[11, :V // 2] = 5.0
+    t = torch.randint(0, V, (40,), generator=g)
+    check(x, t, top)
+    check(x.bfloat16(), t, top, 0.7)
+
+
 def test_large_logits():
     x = 100 * torch.randn(4, 2500, generator=torch.Generator().manual_seed(9))
     x[1] *= 1e4
