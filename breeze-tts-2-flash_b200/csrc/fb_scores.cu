@@ -432,9 +432,10 @@ extern "C" int flashb_token_scores(const void* logits, int is_bf16, int64_t ld, 
   a.rank = (long long*)rank, a.top_id = (long long*)top_id;
   // Two units a thread or more.  128 threads a row: more of them, with fewer units each, leave more logits at the threshold
   // (4095 rows of 32003 in bf16: 94, 79, 89 and 128 us with 64, 128, 256 and 512 threads; occupancies of 8 to 12 such CTAs
-  // an SM 79 to 83).  Few rows leave SMs idle, so there a row has up to 512.
-  const int units = V / (is_bf16 ? 16 : 8), most = rows <= 2 * fbh::num_sms() ? SC_MAX : 128;
-  int threads = 32;
+  // an SM 79 to 83).  Where the rows leave SMs half empty, up to 512 (500 rows of 65536 in fp32: 68 us with 128, 42 with 256).
+  const int units = V / (is_bf16 ? 16 : 8);
+  int most = 128, threads = 32;
+  while (most < SC_MAX && (int64_t)rows * most * 2 <= 1024ll * fbh::num_sms()) most *= 2;
   while (threads < most && threads * 4 <= units) threads *= 2;
   void* args[] = {(void*)&a};
   return fbh::launch_pdl(is_bf16 ? (const void*)scores_kernel<uint16_t> : (const void*)scores_kernel<float>, dim3(rows),
