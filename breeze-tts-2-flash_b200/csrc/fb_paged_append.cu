@@ -9,13 +9,15 @@
 // off by 2^-24 of the angle, 0.01 radians at position 200000 of the fastest pair.
 //
 // Bound: 512 (NH + 2 NKV) bytes a token, read and written once; for a few tokens a chain of loads (offsets, lengths, page).
-// A warp takes units of up to eight heads through a ring of its own in shared memory (bulk copies of 2 KB, five under way),
-// a half-warp a head; the first copies are issued before the tokens' places are known.  Places (up to seven tokens a warp,
-// no load waiting for another token's) and one sine and cosine for each pair and token are worked out once a CTA.
+// A warp takes units of up to twelve heads through a ring of its own in shared memory (bulk copies of 3 KB, three under
+// way), eight lanes a head; the first copies are issued before the tokens' places are known.  Places (up to seven tokens a
+// warp, no load waiting for another token's) and one sine and cosine for each pair and token are worked out once a CTA.
 //
-// Measured on a B200 (in a CUDA graph): 16391 tokens of 24 heads (201 MB) 39 us, 0.78 of the measured copy bandwidth; one
-// token of 128 rows 3.6 us, of 2 rows 3.4 us.  Three CTAs an SM with rings of three 42 us, units of four heads 46 to 48;
-// loads straight to registers, six a thread, 48 to 58 whatever the occupancy (too few bytes under way).
+// Measured on a B200 (in a CUDA graph): 16391 tokens of 24 heads (201 MB) 41 us, 0.74 of the measured copy bandwidth, with
+// head norms 40 us; one token of 128 rows 3.0 us, of 2 rows 2.9 us.  Sixteen lanes a head 41 us, but 53 with norms (twice
+// the instructions a head) and 3.4 for one token.  Rings of five units of eight heads 42 us, 30 instead of 23 for tokens of
+// twelve heads (a unit of eight and one of four); four tokens a warp 39, but 47 with norms; three CTAs an SM 45; loads
+// straight to registers, six a thread, 48 to 58 whatever the occupancy (too few bytes under way).
 #include <climits>
 
 #include "fb_long_tc.cuh"
@@ -24,11 +26,11 @@
 namespace fb {
 
 constexpr int PA_THREADS = 256, PA_WARPS = PA_THREADS / 32;
-constexpr int PA_CTAS = 2;               // an SM: 108 KB
+constexpr int PA_CTAS = 2;               // an SM: 100 KB
 constexpr int PA_EACH = 7;               // tokens of a CTA whose places a warp finds, at most
 constexpr int PA_TOKENS = PA_EACH * PA_WARPS;
-constexpr int PA_HEADS = 8;              // heads of a unit, at most
-constexpr int PA_RING = 5;               // units of a warp under way
+constexpr int PA_HEADS = 12;             // heads of a unit, at most
+constexpr int PA_RING = 3;               // units of a warp under way
 constexpr int PA_SLOT = PA_HEADS * LG_D * 2;
 constexpr int PA_SMEM = PA_WARPS * PA_RING * PA_SLOT + PA_TOKENS * (LG_D / 2) * (int)sizeof(float2);
 
@@ -48,10 +50,9 @@ struct PagedAppendArgs {
   unsigned* err;
 };
 
-// Eight dims of a head: those that this lane's pairs join, in two runs of four.
-struct PagedDims {
-  uint2 a, b;
-};
+__device__ __forceinline__ uint4 paged_pack(const float* v) {
+  return make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+}
 
 __global__ void __launch_bounds__(PA_THREADS, PA_CTAS) paged_append_kernel(const __grid_constant__ PagedAppendArgs a) {
   extern __shared__ __align__(128) unsigned char smem[];
@@ -60,11 +61,14 @@ __global__ void __launch_bounds__(PA_THREADS, PA_CTAS) paged_append_kernel(const
   __shared__ __align__(8) uint64_t bars[PA_WARPS][PA_RING];
   __shared__ long long s_pos[PA_TOKENS];
   __shared__ unsigned char *s_k[PA_TOKENS], *s_v[PA_TOKENS];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, l = tid & 15;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, l = tid & 7;
   const int t0 = blockIdx.x * a.tokens, tokens = min(a.tokens, a.r.T - t0), pairs = a.rot >> 1, heads = a.NH + 2 * a.NKV;
-  // half layout: dims 4 l .. + 3 and their partners rot / 2 further, no exchange between lanes; else eight in a row
-  const bool turn = 8 * l < a.rot, apart = turn && !a.interleaved;
-  const int d1 = apart ? 4 * l : 8 * l, d2 = apart ? pairs + 4 * l : 8 * l + 4;
+  // a lane's two runs of eight dims.  Half layout: the second run holds the first one's partners, or is not turned either;
+  // interleaved: every run holds whole pairs.
+  const int l2 = l - (pairs >> 3);
+  const int d1 = a.interleaved || l2 < 0 ? 8 * l : a.rot + 16 * l2;
+  const int d2 = a.interleaved ? LG_D / 2 + 8 * l : l2 < 0 ? pairs + 8 * l : d1 + 8;
+  const bool turn1 = d1 < a.rot, turn2 = d2 < a.rot;
   uint64_t* bar = bars[warp];
   if (lane == 0) {
     for (int i = 0; i < PA_RING; ++i) mbar_init(&bar[i], 1);
@@ -84,10 +88,10 @@ __global__ void __launch_bounds__(PA_THREADS, PA_CTAS) paged_append_kernel(const
     for (int i = 0; i < PA_RING; ++i)
       if (warp + i * PA_WARPS < units) copy(warp + i * PA_WARPS, i);
   __syncwarp();
-  PagedDims qn{}, kn{};
+  uint4 qn[2]{}, kn[2]{};
   if (a.q_norm) {
-    qn = PagedDims{*reinterpret_cast<const uint2*>(a.q_norm + d1), *reinterpret_cast<const uint2*>(a.q_norm + d2)};
-    kn = PagedDims{*reinterpret_cast<const uint2*>(a.k_norm + d1), *reinterpret_cast<const uint2*>(a.k_norm + d2)};
+    qn[0] = *reinterpret_cast<const uint4*>(a.q_norm + d1), qn[1] = *reinterpret_cast<const uint4*>(a.q_norm + d2);
+    kn[0] = *reinterpret_cast<const uint4*>(a.k_norm + d1), kn[1] = *reinterpret_cast<const uint4*>(a.k_norm + d2);
   }
   // ---- the tokens' places (a few a warp), the turns of their pairs
   const int each = (a.tokens + PA_WARPS - 1) / PA_WARPS;
@@ -126,16 +130,22 @@ __global__ void __launch_bounds__(PA_THREADS, PA_CTAS) paged_append_kernel(const
       s_cs[t][p] = make_float2(a.amplitude * c, a.amplitude * s);
     }
   __syncthreads();
-  // ---- the heads, two at a time
-  const unsigned mask = lane < 16 ? 0xffffu : 0xffff0000u;
+  // ---- the heads, four at a time
+  const unsigned mask = 0xffu << (lane & 24);
   int slot = 0;
   unsigned phase = 0;
 #pragma unroll 1
   for (int u = warp; u < units; u += PA_WARPS) {
     const int j = u / per, h0 = (u - j * per) * a.each, n = min(a.each, heads - h0);
-    float2 cs[4];
+    float2 cs[8];
+    if (turn1) {
+      const int p1 = a.interleaved ? 4 * l : 8 * l, p2 = a.interleaved ? LG_D / 4 + 4 * l : 8 * l + 4;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) cs[e] = turn ? s_cs[j][4 * l + e] : make_float2(1.f, 0.f);
+      for (int e = 0; e < 4; ++e) {
+        cs[e] = s_cs[j][p1 + e];
+        cs[4 + e] = s_cs[j][p2 + e];
+      }
+    }
     const bool live = s_pos[j] != LLONG_MIN;
     unsigned char *kp = s_k[j], *vp = s_v[j];
     bf16* qp = a.q_out + (t0 + j) * a.o_st;
@@ -145,50 +155,55 @@ __global__ void __launch_bounds__(PA_THREADS, PA_CTAS) paged_append_kernel(const
       break;
     }
     const bf16* x = reinterpret_cast<const bf16*>(ring + slot * PA_SLOT);
-#pragma unroll 2
-    for (int i = lane >> 4; i < n; i += 2) {
+#pragma unroll 1
+    for (int i = lane >> 3; i < n; i += 4) {
       const int h = h0 + i;
+      const uint4 x1 = *reinterpret_cast<const uint4*>(x + i * LG_D + d1), x2 = *reinterpret_cast<const uint4*>(x + i * LG_D + d2);
       if (h >= a.NH + a.NKV) {
-        if (live && vp)
-          *reinterpret_cast<uint4*>(vp + (h - a.NH - a.NKV) * a.pool.v_sh + 16 * l) =
-              *reinterpret_cast<const uint4*>(x + i * LG_D + 8 * l);
+        if (live && vp) {
+          bf16* y = reinterpret_cast<bf16*>(vp + (h - a.NH - a.NKV) * a.pool.v_sh);
+          *reinterpret_cast<uint4*>(y + d1) = x1;
+          *reinterpret_cast<uint4*>(y + d2) = x2;
+        }
         continue;
       }
-      PagedDims w{*reinterpret_cast<const uint2*>(x + i * LG_D + d1), *reinterpret_cast<const uint2*>(x + i * LG_D + d2)};
-      float v[8];
-      cvt8(make_uint4(w.a.x, w.a.y, w.b.x, w.b.y), v);
+      float v[16];
+      cvt8(x1, v);
+      cvt8(x2, v + 8);
       if (a.q_norm) {
-        float ss = 0.f;
+        float s0 = 0.f, s1 = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss += v[e] * v[e];
+        for (int e = 0; e < 8; ++e) s0 += v[e] * v[e], s1 += v[8 + e] * v[8 + e];
+        s0 += s1;
 #pragma unroll
-        for (int o = 8; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
-        const float f = rsqrtf(ss * (1.f / LG_D) + a.eps);
-        w = h < a.NH ? qn : kn;
-        float g[8];
-        cvt8(make_uint4(w.a.x, w.a.y, w.b.x, w.b.y), g);
+        for (int o = 4; o > 0; o >>= 1) s0 += __shfl_xor_sync(mask, s0, o);
+        const float f = rsqrtf(s0 * (1.f / LG_D) + a.eps);
+        float g[16];
+        cvt8(h < a.NH ? qn[0] : kn[0], g);
+        cvt8(h < a.NH ? qn[1] : kn[1], g + 8);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] *= f * g[e];
+        for (int e = 0; e < 16; ++e) v[e] *= f * g[e];
       }
-      if (turn && a.interleaved) {                           // (the other lanes' dims stay: 0 x an infinity is not 0)
+      if (a.interleaved) {                                   // (dims that do not turn stay: 0 x an infinity is not 0)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float q = v[2 * e], m = v[2 * e + 1];
-          v[2 * e] = q * cs[e].x - m * cs[e].y;
-          v[2 * e + 1] = m * cs[e].x + q * cs[e].y;
-        }
-      } else if (turn) {
+        for (int e = 0; e < 8; ++e)
+          if (e < 4 ? turn1 : turn2) {
+            const float q = v[2 * e], m = v[2 * e + 1];
+            v[2 * e] = q * cs[e].x - m * cs[e].y;
+            v[2 * e + 1] = m * cs[e].x + q * cs[e].y;
+          }
+      } else if (turn1) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float q = v[e], m = v[4 + e];
+        for (int e = 0; e < 8; ++e) {
+          const float q = v[e], m = v[8 + e];
           v[e] = q * cs[e].x - m * cs[e].y;
-          v[4 + e] = m * cs[e].x + q * cs[e].y;
+          v[8 + e] = m * cs[e].x + q * cs[e].y;
         }
       }
       bf16* y = h < a.NH ? qp + h * a.o_sh : reinterpret_cast<bf16*>(kp + (h - a.NH) * a.pool.k_sh);
       if (live && (h < a.NH || kp)) {
-        *reinterpret_cast<uint2*>(y + d1) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
-        *reinterpret_cast<uint2*>(y + d2) = make_uint2(pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+        *reinterpret_cast<uint4*>(y + d1) = paged_pack(v);
+        *reinterpret_cast<uint4*>(y + d2) = paged_pack(v + 8);
       }
     }
     __syncwarp();
@@ -284,7 +299,8 @@ extern "C" int flashb_paged_append(const fb_paged_cache* cache, const int32_t* t
   const int at_once = PA_CTAS * fbh::grid_sms();
   a.tokens = (T - 1) / at_once + 1;
   if (a.tokens > PA_TOKENS) a.tokens = PA_TOKENS;
-  a.each = a.tokens * heads >= PA_WARPS * PA_HEADS ? PA_HEADS : 2;   // few tokens: a unit for every warp
+  const int parts = (heads + PA_HEADS - 1) / PA_HEADS;       // of a token, equal but for whole fours of heads
+  a.each = a.tokens * parts >= PA_WARPS ? ((heads + parts - 1) / parts + 3) / 4 * 4 : 4;   // few tokens: a unit for every warp
   a.err = fbh::device_err_ptr();
   static int attr_done[64] = {0};
   int dev = 0;
