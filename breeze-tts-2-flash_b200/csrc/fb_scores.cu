@@ -16,8 +16,8 @@
 // The largest logit's own 1 stays out of the sum (its unit's sum is worked out again without it): what the others add to
 // an almost certain token's 1 is not rounded away.
 //
-// Measured on a B200 (in a CUDA graph): 4095 rows of 32003 in bf16 with 20 alternatives (262 MB) 79 us, 0.51 of the measured
-// copy bandwidth; 1088 rows of 2049 in fp32 with 8 (9 MB) 6.6 us; 17 rows 3.9 us.  The first is bound by issue (0.7 of the
+// Measured on a B200 (in a CUDA graph): 4095 rows of 32003 in bf16 with 20 alternatives (262 MB) 73 us, 0.55 of the measured
+// copy bandwidth; 1088 rows of 2049 in fp32 with 8 (9 MB) 6.4 us; 17 rows 3.8 us.  The first is bound by issue (0.7 of the
 // slots; some 8 instructions a logit, 1 of them an exponential); without alternatives it takes 62 us.
 //
 // Rows that the fast path cannot take go through scores_slow, a pass per alternative: a NaN or +inf, -inf alone, logits
@@ -129,19 +129,6 @@ __device__ __noinline__ void scores_slow(const ScoresArgs& a, int r) {
   }
 }
 
-// The largest of the 16 bytes' logits.
-template <typename T>
-__device__ __forceinline__ float score_max(const uint4& w) {
-  if constexpr (sizeof(T) == 4) {
-    return fmaxf(fmaxf(__uint_as_float(w.x), __uint_as_float(w.y)), fmaxf(__uint_as_float(w.z), __uint_as_float(w.w)));
-  } else {
-    uint32_t m;
-    asm("{\n\t.reg .b32 a, b;\n\tmax.bf16x2 a, %1, %2;\n\tmax.bf16x2 b, %3, %4;\n\tmax.bf16x2 %0, a, b;\n\t}"
-        : "=r"(m)
-        : "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w));
-    return fmaxf(lo_f(m), hi_f(m));
-  }
-}
 // Logits below SC_LOW (-inf) as SC_LOW; a NaN stays.
 template <typename T>
 __device__ __forceinline__ uint32_t score_clamp(uint32_t w) {
@@ -155,6 +142,46 @@ __device__ __forceinline__ uint32_t score_clamp(uint32_t w) {
 struct ScoreUnit {
   uint4 w[2];
 };
+__device__ __forceinline__ uint32_t score_max2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ float score_max(const ScoreUnit& u) {
+  const uint32_t w[8] = {u.w[0].x, u.w[0].y, u.w[0].z, u.w[0].w, u.w[1].x, u.w[1].y, u.w[1].z, u.w[1].w};
+  if constexpr (sizeof(T) == 4) {
+    float m = __uint_as_float(w[0]);
+#pragma unroll
+    for (int i = 1; i < 8; ++i) m = fmaxf(m, __uint_as_float(w[i]));
+    return m;
+  } else {
+    const uint32_t m = score_max2(score_max2(score_max2(w[0], w[1]), score_max2(w[2], w[3])),
+                                  score_max2(score_max2(w[4], w[5]), score_max2(w[6], w[7])));
+    return fmaxf(lo_f(m), hi_f(m));
+  }
+}
+// How many of the unit's logits are `th` (a number of the logits' type) or more.
+template <typename T>
+__device__ __forceinline__ int score_count(const ScoreUnit& u, float th) {
+  const uint32_t w[8] = {u.w[0].x, u.w[0].y, u.w[0].z, u.w[0].w, u.w[1].x, u.w[1].y, u.w[1].z, u.w[1].w};
+  if constexpr (sizeof(T) == 4) {
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) n += __uint_as_float(w[i]) >= th;
+    return n;
+  } else {                                               // ones in bf16, added in pairs (at most 8 each: exact)
+    const uint32_t t = (__float_as_uint(th) >> 16) * 0x10001u;
+    uint32_t n[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) asm("set.ge.bf16x2.bf16x2 %0, %1, %2;" : "=r"(n[i]) : "r"(w[i]), "r"(t));
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1)
+#pragma unroll
+      for (int i = 0; i < o; ++i) asm("add.rn.bf16x2 %0, %0, %1;" : "+r"(n[i]) : "r"(n[i + o]));
+    return (int)(lo_f(n[0]) + hi_f(n[0]));
+  }
+}
 
 template <typename T>
 __global__ void __launch_bounds__(SC_MAX, 2) scores_kernel(const __grid_constant__ ScoresArgs a) {
@@ -196,11 +223,11 @@ __global__ void __launch_bounds__(SC_MAX, 2) scores_kernel(const __grid_constant
       o.w[i] = make_uint4(score_clamp<T>(u.w[i].x), score_clamp<T>(u.w[i].y), score_clamp<T>(u.w[i].z), score_clamp<T>(u.w[i].w));
     return o;
   };
+  auto whole = [&](int v) { return ScoreUnit{body[2 * v], body[2 * v + 1]}; };
   auto unit = [&](int v) {
     ScoreUnit u;
     if (v >= 0) {
-      u.w[0] = body[2 * v];
-      u.w[1] = body[2 * v + 1];
+      u = whole(v);
     } else {                                             // the odd logit, and -inf
       const uint32_t none = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u, f = __float_as_uint(score_at(x, mine));
       u.w[0] = u.w[1] = make_uint4(none, none, none, none);
@@ -209,14 +236,16 @@ __global__ void __launch_bounds__(SC_MAX, 2) scores_kernel(const __grid_constant
     return u;
   };
   // the next unit is under way while one is worked on; the first before the token, whose logit is a load behind a load
+  int v = mine >= 0 ? -1 : tid;
   ScoreUnit next;
-  if (tid < nu) next = unit(tid);
+  if (v < nu) next = unit(v);
   const long long token = a.tokens[r];
   const bool known = token >= 0 && token < a.V;
   const int tok = known ? (int)token : 0;
-  const float xt = known ? score_at(x, tok) + 0.f : INFINITY, above = known ? ord2f(f2ord(xt) + 1) : NAN;   // the next number
+  const float xt = known ? score_at(x, tok) + 0.f : INFINITY, above = known ? ord2f(f2ord(xt) + (sizeof(T) == 4 ? 1u : 0x10000u)) : NAN;
+  // (the next number of the type)
   auto feed = [&](const ScoreUnit& raw, int v, int base) {
-    const float vm = fmaxf(score_max<T>(raw.w[0]), score_max<T>(raw.w[1]));
+    const float vm = score_max<T>(raw);
     if (vm * c > R + 16.f) {
       const float n = vm * c, g = ex2(R - n), by = R - n;
       dot = g * fmaf(by, sum, dot);
@@ -247,18 +276,19 @@ __global__ void __launch_bounds__(SC_MAX, 2) scores_kernel(const __grid_constant
     iu2 = nb ? iu : nb2 ? v : iu2;
     iu = nb ? v : iu;
     if (vm >= xt) {
-      const float th = base + N <= tok ? xt : above;
-      pairs(raw, [&](float p, float q, int) { cnt += (p >= th) + (q >= th); });
+      cnt += score_count<T>(raw, base + N <= tok ? xt : above);
       if (base <= tok && tok < base + N)                 // equal logits of lower ids
         pairs(raw, [&](float p, float q, int i) { cnt += (p == xt && base + i < tok) + (q == xt && base + i + 1 < tok); });
     }
   };
-  for (int v = tid; v < nu; v += step) {
+#pragma unroll 1
+  while (v < nu) {
     const ScoreUnit u = next;
-    if (v + step < nu) next = unit(v + step);
-    feed(u, v, head + v * N);
+    const int w = v < 0 ? tid : v + step;
+    if (w < nu) next = whole(w);
+    feed(u, v, v < 0 ? mine : head + v * N);
+    v = w;
   }
-  if (mine >= 0) feed(unit(-1), -1, mine);
 
   // ---- the maximum and the threshold
   const unsigned key = iu == -2 ? 0u : f2ord(tm + 0.f);
@@ -299,29 +329,26 @@ __global__ void __launch_bounds__(SC_MAX, 2) scores_kernel(const __grid_constant
     if (wanted) {
       // logits that reach the threshold; a unit of -inf alone is not looked at again, so none is collected
       const float low = fmaxf(ord2f(max(thr, 0x007fffffu)), -FLT_MAX);
-      auto collect = [&](const ScoreUnit& u, int v) {
-        const int base = v == -1 ? mine : head + v * N;
-        auto put = [&](float f, int id) {
-          if (f >= low) {
-            const int n = atomicAdd(&s_n, 1);
-            if (n < SC_CAP) s_key[n] = ((unsigned long long)f2ord(f + 0.f) << 32) | (0xffffffffu - (unsigned)id);
-          }
-        };
-        pairs(u, [&](float p, float q, int i) {
-          put(p, base + i);
-          put(q, base + i + 1);
-        });
+      auto reach = [&](const ScoreUnit& u) {             // which of them do
+        unsigned m = 0;
+        pairs(u, [&](float p, float q, int i) { m |= (p >= low ? 1u << i : 0u) | (q >= low ? 2u << i : 0u); });
+        return m;
       };
-      const ScoreUnit u1 = unit(iu), u2 = unit(tm2 >= low ? iu2 : iu);
-      collect(u1, iu);
-      if (tm2 >= low) {
-        collect(u2, iu2);
-        if (tm3 >= low) {
-          for (int v = mine >= 0 ? -1 : tid; v < nu; v = v == -1 ? tid : v + step) {
-            if (v == iu || v == iu2) continue;
-            const ScoreUnit u = unit(v);
-            if (fmaxf(score_max<T>(u.w[0]), score_max<T>(u.w[1])) >= low) collect(u, v);
-          }
+      auto collect = [&](unsigned m, int v1, int v2) {   // of unit v1, and 16 bits up of v2
+        int n = atomicAdd(&s_n, __popc(m));
+        for (; m; m &= m - 1, ++n) {
+          const int i = __ffs(m) - 1, v = i < 16 ? v1 : v2, id = v < 0 ? mine : head + v * N + (i & 15);
+          if (n < SC_CAP) s_key[n] = score_key(score_at(x, id), id);
+        }
+      };
+      const bool two = tm2 >= low;
+      const ScoreUnit u1 = unit(iu), u2 = unit(two ? iu2 : iu);
+      collect(reach(u1) | (two ? reach(u2) << 16 : 0u), iu, iu2);
+      if (tm3 >= low) {
+        for (int v = mine >= 0 ? -1 : tid; v < nu; v = v < 0 ? tid : v + step) {
+          if (v == iu || v == iu2) continue;
+          const ScoreUnit u = unit(v);
+          if (score_max<T>(u) >= low) collect(reach(u), v, v);
         }
       }
     }
