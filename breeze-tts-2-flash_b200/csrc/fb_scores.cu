@@ -289,6 +289,7 @@ __global__ void __launch_bounds__(SC_MAX, 2) scores_kernel(const __grid_constant
     feed(u, v, v < 0 ? mine : head + v * N);
     v = w;
   }
+  if (mine >= 0 && xt == -INFINITY) cnt -= min(N - 1, max(0, tok - mine - 1));   // what stood beside the odd logit
 
   // ---- the maximum and the threshold
   const unsigned key = iu == -2 ? 0u : f2ord(tm + 0.f);

@@ -7,10 +7,10 @@ import paged_ref as ref
 pytestmark = pytest.mark.gpu
 
 
-def check(x, tokens, top, temperature=1.0):
+def check(x, tokens, top, temperature=1.0, times=1):
     from flashb.sampling import token_scores
-    got = token_scores(x.cuda(), tokens.cuda(), top=top, temperature=temperature)
-    lp, h, rank, ids, tl = ref.scores(x, tokens, top, temperature)
+    got = token_scores(x.cuda().repeat(times, 1), tokens.cuda().repeat(times), top=top, temperature=temperature)
+    lp, h, rank, ids, tl = (a.repeat(times, *[1] * (a.dim() - 1)) for a in ref.scores(x, tokens, top, temperature))
     assert torch.equal(got.rank.cpu(), rank)
     assert torch.equal(got.top_ids.cpu(), ids)
     # differences from the maximum and their scaling in fp32 (2^-22 of them), the sum and its logarithm (2^-18)
@@ -45,6 +45,44 @@ def test_large_vocabularies(V):
 def test_many_rows():
     g = torch.Generator().manual_seed(4)
     check(torch.randn(700, 65, generator=g), torch.randint(0, 65, (700,), generator=g), 3)
+
+
+@pytest.mark.parametrize('V,top,dtype', [(590, 20, torch.float32), (1056, 5, torch.bfloat16), (1056, 32, torch.bfloat16),
+                                         (2149, 32, torch.float32), (2149, 3, torch.bfloat16), (2149, 32, torch.bfloat16)])
+def test_more_rows_than_the_device_holds(V, top, dtype):
+    """Fewer threads a row, more units each."""
+    g = torch.Generator().manual_seed(V + top)
+    x = 2 * torch.randn(167, V, generator=g)
+    x[::7, ::3] = float('-inf')
+    t = x.argmax(1)
+    t[::2] = torch.randint(0, V, (84,), generator=g)
+    t[7::14] -= t[7::14] % 3                                 # ids that are masked themselves
+    check(x.to(dtype), t, top, times=30)
+
+
+@pytest.mark.parametrize('V', [16, 40, 513, 5000])
+def test_ranks_among_zeros_and_the_smallest_numbers(V):
+    """-0 equals 0; the numbers next to it, on both sides, do not."""
+    g = torch.Generator().manual_seed(V)
+    for dtype, tiny in ((torch.bfloat16, 2.0 ** -133), (torch.float32, 2.0 ** -149)):
+        some = torch.tensor([0.0, -0.0, tiny, -tiny, 2 * tiny], dtype=dtype)
+        x = some[torch.randint(0, 5, (20, V), generator=g)]
+        assert ((x == 0).sum() > 0) and ((x.abs() == tiny).sum() > 0)
+        t = torch.randint(0, V, (20,), generator=g)
+        x[0] = 0.0
+        x[1, 1:] = tiny
+        t[1] = 0                                             # after all of them
+        check(x, t, min(V, 9))
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_the_rank_of_a_masked_id(dtype):
+    """Ids that are masked as well come before it by their number alone, wherever the row's ends lie."""
+    g = torch.Generator().manual_seed(11)
+    for V in (3, 20, 45, 333):
+        x = torch.randn(40, V, generator=g)
+        x[:, ::2] = float('-inf')
+        check(x.to(dtype), torch.arange(40) * 2 % V // 2 * 2, min(V // 2, 4))
 
 
 def test_ties_go_to_the_lowest_id():
