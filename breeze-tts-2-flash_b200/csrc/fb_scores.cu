@@ -10,14 +10,15 @@
 //   the sums of e = 2^(x c - R) and of e (x c - R) with c = log2(e) / temperature and a reference R of its own, which moves
 //   only when a unit's maximum passes it by 2^16 (the sums are exact either way);
 //   the three largest unit maxima, which units hold the first two, and the first one's sums apart from the rest.
-// The block's threshold for the alternatives is the least of the warps' k / W-th largest thread maxima: at least k logits
-// reach it.  Only units that reach it are read again (from L1 or L2; mostly one each of some tens of threads), what they
-// hold of it is collected, and each of those finds its place by counting the others above it.
+// The block's threshold for the alternatives is the least of the warps' k / W-th largest unit maxima (of each thread's first,
+// where k / W is small, else of its first two): at least k logits reach it.  Only units that reach it are read again (from
+// L1 or L2; mostly one each of some tens of threads), what they hold of it is collected, and each of those finds its place by
+// counting the others above it.
 // The largest logit's own 1 stays out of the sum (its unit's sum is worked out again without it): what the others add to
 // an almost certain token's 1 is not rounded away.
 //
 // Measured on a B200 (in a CUDA graph): 4095 rows of 32003 in bf16 with 20 alternatives (262 MB) 73 us, 0.55 of the measured
-// copy bandwidth; 1088 rows of 2049 in fp32 with 8 (9 MB) 6.4 us; 17 rows 3.8 us.  The first is bound by issue (0.7 of the
+// copy bandwidth; 1088 rows of 2049 in fp32 with 8 (9 MB) 6.6 us; 17 rows 3.9 us.  The first is bound by issue (0.7 of the
 // slots; some 8 instructions a logit, 1 of them an exponential); without alternatives it takes 62 us.
 //
 // Rows that the fast path cannot take go through scores_slow, a pass per alternative: a NaN or +inf, -inf alone, logits
@@ -242,8 +243,8 @@ __global__ void __launch_bounds__(SC_MAX, 2) scores_kernel(const __grid_constant
   const long long token = a.tokens[r];
   const bool known = token >= 0 && token < a.V;
   const int tok = known ? (int)token : 0;
-  const float xt = known ? score_at(x, tok) + 0.f : INFINITY, above = known ? ord2f(f2ord(xt) + (sizeof(T) == 4 ? 1u : 0x10000u)) : NAN;
-  // (the next number of the type)
+  const float xt = known ? score_at(x, tok) + 0.f : INFINITY;
+  const float above = known ? ord2f(f2ord(xt) + (sizeof(T) == 4 ? 1u : 0x10000u)) : NAN;   // the type's next number
   auto feed = [&](const ScoreUnit& raw, int v, int base) {
     const float vm = score_max<T>(raw);
     if (vm * c > R + 16.f) {
@@ -302,14 +303,23 @@ __global__ void __launch_bounds__(SC_MAX, 2) scores_kernel(const __grid_constant
         if (lane == __ffs(__ballot_sync(FULL, k == at)) - 1) k = 0;
         at = __reduce_max_sync(FULL, k);
       }
-    } else {                                             // the lanes sorted, the largest first
+    } else {                                             // the lanes' first and second units sorted, the largest first
+      unsigned k2 = f2ord(tm2 + 0.f);
 #pragma unroll
       for (int size = 2; size <= 32; size *= 2)
 #pragma unroll
         for (int o = size / 2; o > 0; o /= 2) {
-          const unsigned y = __shfl_xor_sync(FULL, k, o);
-          k = ((lane & o) == 0) == ((lane & size) == 0) ? max(k, y) : min(k, y);
+          const unsigned y = __shfl_xor_sync(FULL, k, o), y2 = __shfl_xor_sync(FULL, k2, o);
+          const bool large = ((lane & o) == 0) == ((lane & size) == 0);
+          k = large ? max(k, y) : min(k, y);
+          k2 = large ? max(k2, y2) : min(k2, y2);
         }
+      k = max(k, __shfl_sync(FULL, k2, 31 - lane));      // the largest 32 of both
+#pragma unroll
+      for (int o = 16; o > 0; o /= 2) {
+        const unsigned y = __shfl_xor_sync(FULL, k, o);
+        k = (lane & o) == 0 ? max(k, y) : min(k, y);
+      }
       at = __shfl_sync(FULL, k, kw - 1);
     }
     if (lane == 0) {
@@ -397,8 +407,8 @@ __global__ void __launch_bounds__(SC_MAX, 2) scores_kernel(const __grid_constant
     a.rank[r] = known ? before : a.V;
   }
   int n = s_n;
-  // More than two a thread (rows of few units, whose maxima say little): the first warp finds the last logit that counts, by halves of the
-  // ordered numbers between, and keeps what reaches it (1387 rows of 276 with 32 alternatives: 22 and 10.6 us).
+  // More than two a thread (rows of few units, whose maxima say little): the first warp finds the last logit that counts, by
+  // halves of the ordered numbers between, and keeps what reaches it.
   if (n > 2 * step && n <= 32 * SC_EACH) {
     if (warp == 0) {
       unsigned v[SC_EACH];
@@ -458,13 +468,18 @@ extern "C" int flashb_token_scores(const void* logits, int is_bf16, int64_t ld, 
   a.inv = 1.f / temperature, a.c = a.inv * LG_LOG2E;
   a.logprob = logprob, a.entropy = entropy, a.top_logprob = top_logprob;
   a.rank = (long long*)rank, a.top_id = (long long*)top_id;
-  // Two units a thread or more.  128 threads a row: more of them, with fewer units each, leave more logits at the threshold
-  // (4095 rows of 32003 in bf16: 94, 79, 89 and 128 us with 64, 128, 256 and 512 threads; occupancies of 8 to 12 such CTAs
-  // an SM 79 to 83).  Where the rows leave SMs half empty, up to 512 (500 rows of 65536 in fp32: 68 us with 128, 42 with 256).
+  // Threads of a row.  While the rows leave SMs half empty, up to 512, of four units and more (500 rows of 65536 in fp32: 68
+  // us with 128, 38 with 256).  Else up to 128 (4095 rows of 32003 in bf16: 88, 73 and 81 us with 64, 128 and 256), of
+  // sixteen units and more (12000 rows of 8200 in bf16, 8 alternatives: 63 us with 64, 73 with 128; of 2149 31 with 32, 39
+  // with 64), or eight where a warp would have to yield more than 24 alternatives (32 of them, rows of 4100: 59 with 64, 65
+  // with 32).
   const int units = V / (is_bf16 ? 16 : 8);
-  int most = 128, threads = 32;
-  while (most < SC_MAX && (int64_t)rows * most * 2 <= 1024ll * fbh::num_sms()) most *= 2;
-  while (threads < most && threads * 4 <= units) threads *= 2;
+  int threads = 32;
+  for (; threads < SC_MAX; threads *= 2) {
+    const bool full = (int64_t)rows * threads * 2 > 1024ll * fbh::num_sms();
+    if (full && threads == 128) break;
+    if (threads * (!full ? 4 : top > threads * 3 / 4 ? 8 : 16) > units) break;
+  }
   void* args[] = {(void*)&a};
   return fbh::launch_pdl(is_bf16 ? (const void*)scores_kernel<uint16_t> : (const void*)scores_kernel<float>, dim3(rows),
                          dim3(threads), 0, (cudaStream_t)stream, args, true);
