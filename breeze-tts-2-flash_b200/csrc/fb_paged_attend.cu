@@ -18,9 +18,9 @@
 //
 // Pieces.  A step can be one run of a few tokens over a long row, or many rows of which some are long.  So the key tiles of
 // a query tile are cut into s pieces of about C; a CTA takes one piece.  paged_plan_kernel (one CTA, from lengths and offsets
-// on the device: nothing is read on the host) writes the list; C is chosen among those with which the list fills one to
-// PT_WAVES rounds of the SMs, and whole query tiles, by what the rounds take (where rows are too short to cut, there is no
-// plan and CTAs find their query tiles themselves: a short prompt 11.2 instead of 15.0 us).  Pieces of a query tile leave
+// on the device: nothing is read on the host) writes the list; C is chosen among those with which the list fills one or
+// two rounds of the SMs, and whole query tiles, by what they take (where rows are too short to cut, there is no plan and CTAs
+// find their query tiles themselves: a short prompt 11.2 instead of 15.0 us).  Pieces of a query tile leave
 // (reference, sum, unnormalised out) in the workspace and paged_merge_kernel joins them in order: no atomics, the same
 // inputs give the same bits.  A query tile of one piece writes its rows itself.
 //
@@ -32,14 +32,14 @@
 // computed again, one visible key at a time.
 //
 // Measured on a B200 (in a CUDA graph, 16 heads over 4): 2048 tokens over 32768 slots of one row 520 us, 1090 TFLOP/s, in
-// pages of 16 to 128 alike; 801 tokens of 32 rows over a window of 2048 (131 MB) 51 us; 512 tokens of one row beside one each
-// of 63, over up to 8000 slots (530 MB), 128 us; two prompts of 197 tokens 10 to 11 us.  A tile takes 1500 cycles with two
+// pages of 16 to 128 alike; 801 tokens of 32 rows over a window of 2048 (131 MB) 47 us; 512 tokens of one row beside one each
+// of 63, over up to 8000 slots (530 MB), 126 us; two prompts of 197 tokens 10 to 11 us.  A tile takes 1500 cycles with two
 // CTAs an SM: 700 to 870 are exponentials (the unit's bound for both CTAs is 1024), 100 the read of S, 240 masks, the rest
 // waits and stores; issuing S takes its thread 480 cycles and P V 290, both beside the exponentials.  Under the largest
 // case's load clocks fall to 1.5 GHz.  With few keys a piece it is beginning and ending (9000 cycles) that counts.  Tried
 // and slower: one copying warp for K and V (8 boxes one after the other take 900 cycles), a flag for missing pages read in
-// the loop (6%), arrivals by one lane a warp (4%), P V's waits by one lane (10%), cuts priced with the joins (10% at the
-// window), the second CTA of an SM begun half a tile later (the same).
+// the loop (6%), arrivals by one lane a warp (4%), P V's waits by one lane (10%), the
+// second CTA of an SM begun half a tile later (the same).
 #include <climits>
 
 #include "fb_long_tc.cuh"
@@ -47,10 +47,15 @@
 
 namespace fb {
 
-constexpr int PT_MIN = 8;                         // key tiles of a piece, at least (4 and 2: no faster, and more calls need a plan)
-constexpr int PT_WAVES = 4;                       // rounds of CTAs that the list of pieces may be cut for
+constexpr int PT_WHOLE = 8;                       // query tiles of so few key tiles stay whole, without a plan
+constexpr int PT_MIN = 6;                         // key tiles of a piece, at least
+constexpr int PT_WAVES = 2;                       // rounds of CTAs that the list of pieces may be cut for
 constexpr float PT_LIMIT = 0x1p-16f;              // 2^(8 + LP_SHIFT): a tile's weights below it leave the reference as it is
-constexpr int PT_COST = 5;                        // what beginning and ending a piece takes, in key tiles
+// What a list costs, in the time of a key tile: max(1, rounds) (longest piece + PT_COST), and where anything is cut that
+// PT_MORE times (under the power limit all SMs at work are no faster than seven eighths of them), PT_JOIN a round (parts
+// written and read again) and PT_JOINS.  Fitted to 430 lists of 45 drawn steps (pieces of 5 to 128 tiles, and whole): its
+// choices take 2% more time than the best of each step, 9% at most; those by rounds x (longest + 5) 7%, 36% at most.
+constexpr float PT_COST = 20.f, PT_MORE = 1.125f, PT_JOIN = 9.f, PT_JOINS = 3.f;
 
 struct PagedPiece;
 
@@ -72,7 +77,7 @@ struct alignas(64) PagedAttendArgs {
   float* po;                            // pieces: unnormalised out [slot][128][128],
   float2* ml;                           //   maximum and sum [slot][128]
   PagedPiece* plan;                     // [list]
-  int4* cut;                            // [cuts / 2] query tiles of two pieces and more: first token, tokens, pieces, slot
+  int4* cut;                            // [cuts / 2] query tiles of two pieces and more: first token, tokens, pieces, slot; then their number
   unsigned* err;
 };
 
@@ -178,14 +183,13 @@ __global__ void __launch_bounds__(PP_THREADS) paged_plan_kernel(const __grid_con
       if (lane == 0) s_n[j][warp] = n[j], s_most[j][warp] = most[j];
     }
     __syncthreads();
-    // those and whole query tiles, each priced by its rounds x (its longest piece and the time that one takes to begin and
-    // end); the places in the workspace are enough for `cuts` pieces
-    float price = ceilf((float)units * a.rounds) * (float)(longest + PT_COST);
+    // the cheapest of those and of whole query tiles; the places in the workspace are enough for `cuts` pieces
+    float price = fmaxf(1.f, (float)units * a.rounds) * ((float)longest + PT_COST);
 #pragma unroll
     for (int j = 0; j < PT_WAVES; ++j) {
       const int count = __reduce_add_sync(FULL, lane < PP_WARPS ? s_n[j][lane] : 0);
       const float len = (float)__reduce_max_sync(FULL, lane < PP_WARPS ? s_most[j][lane] : 0);
-      const float p = ceilf((float)count * a.rounds) * (len + PT_COST);
+      const float rounds = (float)count * a.rounds, p = fmaxf(1.f, rounds) * (len + PT_COST) * PT_MORE + rounds * PT_JOIN + PT_JOINS;
       if (p < price && count <= a.cuts) price = p, r = c[j];
     }
   }
@@ -249,7 +253,7 @@ __global__ void __launch_bounds__(PP_THREADS) paged_plan_kernel(const __grid_con
     *reinterpret_cast<int4*>(&a.plan[x]) = *reinterpret_cast<const int4*>(&p);
     reinterpret_cast<int4*>(&a.plan[x])[1] = reinterpret_cast<const int4*>(&p)[1];
   }
-  for (int x = joins + tid; x < a.cuts / 2; x += PP_THREADS) a.cut[x] = make_int4(0, 0, 0, 0);   // the merge's other CTAs
+  if (tid == 0 && a.cuts > 1) a.cut[a.cuts / 2] = make_int4(joins, 0, 0, 0);
 }
 
 // Piece x of the list whose query tiles stay whole, for a CTA without a plan: a warp, lane i counts rows [i per32, ..).
@@ -726,21 +730,26 @@ __global__ void __launch_bounds__(PT_THREADS, 2) paged_attend_kernel(const __gri
   }
 }
 
-// Joins the pieces of the query tiles that were cut, in their order: a CTA per PM_ROWS rows of a query tile and head (801
-// tokens of 32 rows, 3 pieces: 24 us with a CTA of 8 warps per tile and head), four rows a warp.
-constexpr int PM_ROWS = 16, PM_THREADS = 128;
-__global__ void __launch_bounds__(PM_THREADS) paged_merge_kernel(const __grid_constant__ PagedAttendArgs a) {
-  const int group = blockIdx.y, x = blockIdx.x / a.NKV, h = blockIdx.x - x * a.NKV, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+// Joins the pieces of the query tiles that were cut, in their order: a warp a row, the CTAs that the SMs hold go round (how many
+// rows there are only the device knows).  For 801 tokens of 32 rows in 3 pieces (24 MB) 7.5 us, 1.5 of them the launch; with a
+// CTA for every 16 rows that there might be 8.7, two rows a warp at a time 8 to 10.
+constexpr int PM_THREADS = 256, PM_CTAS = 4;
+__global__ void __launch_bounds__(PM_THREADS, PM_CTAS) paged_merge_kernel(const __grid_constant__ PagedAttendArgs a) {
+  constexpr int W = PM_THREADS / 32;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
   pdl_trigger();
-  const int4 cut = a.cut[x];
-  const int pieces = cut.z, live = min(cut.y * a.G, (group + 1) * PM_ROWS);
-  if (pieces == 0) return;
-  const long long at = (long long)cut.w * a.NKV + h, step = (long long)a.NKV * LP_ROWS;
+  const long long n = (long long)a.cut[a.cuts / 2].x * a.NKV * LP_ROWS, step = (long long)a.NKV * LP_ROWS;
 #pragma unroll 1
-  for (int r = group * PM_ROWS + warp; r < live; r += PM_THREADS / 32) {
-    const float2* ml = a.ml + at * LP_ROWS + r;
-    const float* po = a.po + (at * LP_ROWS + r) * LG_D + 4 * lane;
+  for (long long k = (long long)blockIdx.x * W + warp; k < n; k += (long long)gridDim.x * W) {
+    const int xh = (int)(k / LP_ROWS), x = xh / a.NKV, h = xh - x * a.NKV;
+    const int4 cut = a.cut[x];
+    // (turned from tile to tile: a warp's rows would be the same in each, and tiles of few tokens all with the same warps)
+    const int pieces = cut.z, live = cut.y * a.G, r = (int)(k + 5 * xh) & (LP_ROWS - 1);
+    if (r >= live) continue;
+    const long long at = ((long long)cut.w * a.NKV + h) * LP_ROWS + r;
+    const float2* ml = a.ml + at;
+    const float* po = a.po + at * LG_D + 4 * lane;
     // four pieces at a time, their loads together
     float M = -INFINITY, L = 0.f;
     float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -812,7 +821,7 @@ int paged_plan_host(const fb_paged_cache* c, int rows, int width, int T, int NH,
   if (window > 0 && (int64_t)window + sinks + nq + 3 * LP_SEG < S) keys = (int64_t)window + sinks + nq + 3 * LP_SEG;
   const int64_t most = (keys + LP_TILE - 1) / LP_TILE;
   // CTAs that the SMs hold.  By the device's SMs, not the calling thread's budget: the workspace's size goes by it.
-  p->pieces = most > PT_MIN ? (2 * fbh::num_sms() + c->NKV - 1) / c->NKV : 0;
+  p->pieces = most > PT_WHOLE ? (2 * fbh::num_sms() + c->NKV - 1) / c->NKV : 0;
   p->direct = p->pieces == 0;
   // a list is cut for PT_WAVES rounds at most and into pieces of PT_MIN at least, or is its query tiles
   p->cuts = (int64_t)PT_WAVES * p->pieces;
@@ -823,7 +832,7 @@ int paged_plan_host(const fb_paged_cache* c, int rows, int width, int T, int NH,
   p->off_ml = p->slots * LP_ROWS * LG_D;
   p->off_plan = p->off_ml + p->slots * LP_ROWS * 2;
   p->off_cut = p->off_plan + (p->direct ? 0 : p->list * (int64_t)(sizeof(PagedPiece) / 4));
-  p->ws_floats = p->off_cut + p->cuts / 2 * 4;
+  p->ws_floats = p->off_cut + (p->cuts > 1 ? p->cuts / 2 + 1 : 0) * 4;
   return FB_OK;
 }
 
@@ -922,6 +931,8 @@ extern "C" int flashb_paged_attend(const fb_paged_cache* cache, const int32_t* t
     rc = fbh::launch_pdl((const void*)paged_attend_kernel, dim3((unsigned)(p.list * a.NKV)), dim3(PT_THREADS), PT_SMEM, st,
                          args, true);
   if (rc || p.cuts < 2) return rc;
-  return fbh::launch_pdl((const void*)paged_merge_kernel, dim3((unsigned)(p.cuts / 2 * a.NKV), LP_ROWS / PM_ROWS),
+  const int64_t joins = (p.cuts / 2 * a.NKV * LP_ROWS + PM_THREADS / 32 - 1) / (PM_THREADS / 32);
+  const int64_t at_once = (int64_t)PM_CTAS * fbh::grid_sms();
+  return fbh::launch_pdl((const void*)paged_merge_kernel, dim3((unsigned)(joins < at_once ? joins : at_once)),
                          dim3(PM_THREADS), 0, st, args, true);
 }
