@@ -39,7 +39,8 @@
 // case's load clocks fall to 1.5 GHz.  With few keys a piece it is beginning and ending (9000 cycles) that counts.  Tried
 // and slower: one copying warp for K and V (8 boxes one after the other take 900 cycles), a flag for missing pages read in
 // the loop (6%), arrivals by one lane a warp (4%), P V's waits by one lane (10%), the
-// second CTA of an SM begun half a tile later (the same).
+// second CTA of an SM begun half a tile later (the same), copies to L2 a buffer ahead (4 to 30%: more boxes), half of Q in
+// the place of P's second buffer in TMEM (3 to 10%).
 #include <climits>
 
 #include "fb_long_tc.cuh"
