@@ -20,7 +20,7 @@
 // a query tile are cut into s pieces of about C; a CTA takes one piece.  paged_plan_kernel (one CTA, from lengths and offsets
 // on the device: nothing is read on the host) writes the list; C is chosen among those with which the list fills one or
 // two rounds of the SMs, and whole query tiles, by what they take (where rows are too short to cut, there is no plan and CTAs
-// find their query tiles themselves: a short prompt 11.2 instead of 15.0 us).  Pieces of a query tile leave
+// find their query tiles themselves: a short prompt 10 instead of 15 us).  Pieces of a query tile leave
 // (reference, sum, unnormalised out) in the workspace and paged_merge_kernel joins them in order: no atomics, the same
 // inputs give the same bits.  A query tile of one piece writes its rows itself.
 //
@@ -86,11 +86,13 @@ struct alignas(64) PagedAttendArgs {
 struct PagedSpan {
   int t0, n, p0;
 };
-__device__ __forceinline__ PagedSpan paged_span(const PagedRows& r, int b) {
-  const long long f = r.offsets[b], e = r.offsets[b + 1], len = r.lengths[b];
+__device__ __forceinline__ PagedSpan paged_span(const PagedRows& r, long long f, long long e, long long len) {
   const int t0 = (int)min(max(f, 0ll), (long long)r.T), t1 = (int)min(max(e, (long long)t0), (long long)r.T);
   const long long p0 = min(max(len, 0ll), (long long)r.S) - (e - t0);
   return PagedSpan{t0, t1 - t0, (int)max(p0, -0x40000000ll)};
+}
+__device__ __forceinline__ PagedSpan paged_span(const PagedRows& r, int b) {
+  return paged_span(r, r.offsets[b], r.offsets[b + 1], r.lengths[b]);
 }
 // The key segments of tokens at slots p_lo .. p_hi: ns of sinks from slot 0 on, then those from base to p_hi; lo: the first
 // slot that the window of any of them holds.
@@ -257,35 +259,46 @@ __global__ void __launch_bounds__(PP_THREADS) paged_plan_kernel(const __grid_con
   if (tid == 0 && a.cuts > 1) a.cut[a.cuts / 2] = make_int4(joins, 0, 0, 0);
 }
 
-// Piece x of the list whose query tiles stay whole, for a CTA without a plan: a warp, lane i counts rows [i per32, ..).
-__device__ __forceinline__ PagedPiece paged_direct(const PagedAttendArgs& a, int x, int lane) {
-  int n = 0;
-#pragma unroll 1
-  for (int i = 0; i < a.per32; ++i) {
-    const int b = lane * a.per32 + i;
-    if (b < a.r.rows) n += paged_tiles(a, b).x;
+// Piece x of the list whose query tiles stay whole, for a CTA without a plan: a warp, lane i counts rows [i per32, ..), the
+// first four of them from registers (108 rows of two tokens: 24 us; a row after the other, each load behind the last, 30).
+__device__ __forceinline__ void paged_direct(const PagedAttendArgs& a, int x, int lane, PagedPiece* piece) {
+  const int b0 = min(lane * a.per32, a.r.rows), b1 = min(b0 + a.per32, a.r.rows);
+  long long f[5], len[4];
+  int k[4], n = 0;
+  f[0] = a.r.offsets[b0];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[i + 1] = a.r.offsets[min(b0 + i + 1, b1)], len[i] = a.r.lengths[min(b0 + i, a.r.rows - 1)];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    k[i] = b0 + i < b1 ? (paged_span(a.r, f[i], f[i + 1], len[i]).n + a.nq - 1) >> a.lq : 0;
+    n += k[i];
   }
+#pragma unroll 1
+  for (int b = b0 + 4; b < b1; ++b) n += (paged_span(a.r, b).n + a.nq - 1) >> a.lq;
   int before = n;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int y = __shfl_up_sync(FULL, before, o);
     if (lane >= o) before += y;
   }
-  PagedPiece p{-1, 0, 0, 0, 0, 1, 0, 0};
-  if (x >= __shfl_sync(FULL, before, 31)) return p;
-  before -= n;
-  const int owner = 31 - __clz(__ballot_sync(FULL, before <= x));   // empty lanes share a count: the last of them
-  int at = __shfl_sync(FULL, before, owner), b = owner * a.per32;
-#pragma unroll 1
-  for (;; ++b) {
-    n = paged_tiles(a, b).x;
-    if (x < at + n) break;
-    at += n;
+  if (x >= before || x < before - n) {
+    if (lane == 31 && x >= before) *piece = PagedPiece{-1, 0, 0, 0, 0, 1, 0, 0};
+    return;
   }
-  const PagedSpan span = paged_span(a.r, b);
-  const int q0 = (n - 1 - (x - at)) << a.lq;
-  p.b = b, p.tok = span.t0 + q0, p.nt = min(a.nq, span.n - q0), p.p_lo = span.p0 + q0;
-  return p;
+  int at = x - (before - n), b = b0;                         // the lane's query tile `at`, of row b
+  PagedSpan span = paged_span(a.r, f[0], f[1], len[0]);
+  int tiles = k[0];
+#pragma unroll
+  for (int i = 1; i < 4; ++i)
+    if (b == b0 + i - 1 && at >= tiles) at -= tiles, ++b, tiles = k[i], span = paged_span(a.r, f[i], f[i + 1], len[i]);
+#pragma unroll 1
+  while (at >= tiles) {
+    at -= tiles, ++b;
+    span = paged_span(a.r, b);
+    tiles = (span.n + a.nq - 1) >> a.lq;
+  }
+  const int q0 = (tiles - 1 - at) << a.lq;
+  *piece = PagedPiece{b, span.t0 + q0, min(a.nq, span.n - q0), span.p0 + q0, 0, 1, 0, 0};
 }
 
 constexpr int PT_THREADS = 256;                  // 4 softmax warps; one each for S, P V, the copies of K and of V
@@ -331,6 +344,8 @@ __device__ __noinline__ uint2 paged_one(const PagedAttendArgs& a, int b, int p, 
   return make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
 }
 
+// PLAN: pieces come from the plan, else CTAs find their query tiles.
+template <bool PLAN>
 __global__ void __launch_bounds__(PT_THREADS, 2) paged_attend_kernel(const __grid_constant__ PagedAttendArgs a) {
   // nothing but this: with 1 KB of the system's, two CTAs fill an SM, and the base is at a 1024-byte boundary (checked)
   extern __shared__ __align__(1024) unsigned char sq[];                   // Q; the output tile at the end
@@ -352,13 +367,10 @@ __global__ void __launch_bounds__(PT_THREADS, 2) paged_attend_kernel(const __gri
   pdl_wait();
   pdl_trigger();
   PagedPiece piece;
-  if (a.plan) {
+  if constexpr (PLAN) {
     piece = a.plan[x];
   } else {
-    if (warp == 0) {
-      const PagedPiece y = paged_direct(a, x, lane);
-      if (lane == 0) s_piece = y;
-    }
+    if (warp == 0) paged_direct(a, x, lane, &s_piece);
     __syncthreads();
     piece = s_piece;
   }
@@ -540,7 +552,7 @@ __global__ void __launch_bounds__(PT_THREADS, 2) paged_attend_kernel(const __gri
     // entries that are no page, among those of the piece's slots that are seen (known before the loop: with a flag of the
     // copying warp's read in every tile the loop was 6% slower)
     bool hole = false;
-#pragma unroll 8
+#pragma unroll 4
     for (int i = tid; i < 4 * tiles; i += 32 * warps) {
       const int sg = 2 * first + (i >> 1), j = seg.at(sg) + 16 * (i & 1);
       if (sg < seg.n && j < a.r.S && seen(j, 16)) hole |= (unsigned)table[j >> a.t.shift] >= (unsigned)a.t.pages;
@@ -914,23 +926,22 @@ extern "C" int flashb_paged_attend(const fb_paged_cache* cache, const int32_t* t
     a.tk = a.tks, a.tv = a.tvs;          // not used
   }
   if (rc) return rc;
-  static int attr_done[64] = {0};
+  const void* attend = p.direct ? (const void*)paged_attend_kernel<false> : (const void*)paged_attend_kernel<true>;
+  static int attr_done[64][2] = {{0}};
   int dev = 0;
   cudaGetDevice(&dev);
-  if (dev >= 64 || !attr_done[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(paged_attend_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PT_SMEM);
+  if (dev >= 64 || !attr_done[dev][p.direct]) {
+    const cudaError_t e = cudaFuncSetAttribute(attend, cudaFuncAttributeMaxDynamicSharedMemorySize, PT_SMEM);
     if (e != cudaSuccess) {
       fbh::set_msg("paged_attend: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
       return FB_ERR_CUDA;
     }
-    if (dev < 64) attr_done[dev] = 1;
+    if (dev < 64) attr_done[dev][p.direct] = 1;
   }
   const cudaStream_t st = (cudaStream_t)stream;
   void* args[] = {(void*)&a};
   if (!p.direct) rc = fbh::launch_pdl((const void*)paged_plan_kernel, dim3(1), dim3(PP_THREADS), 0, st, args, true);
-  if (!rc)
-    rc = fbh::launch_pdl((const void*)paged_attend_kernel, dim3((unsigned)(p.list * a.NKV)), dim3(PT_THREADS), PT_SMEM, st,
-                         args, true);
+  if (!rc) rc = fbh::launch_pdl(attend, dim3((unsigned)(p.list * a.NKV)), dim3(PT_THREADS), PT_SMEM, st, args, true);
   if (rc || p.cuts < 2) return rc;
   const int64_t joins = (p.cuts / 2 * a.NKV * LP_ROWS + PM_THREADS / 32 - 1) / (PM_THREADS / 32);
   const int64_t at_once = (int64_t)PM_CTAS * fbh::grid_sms();

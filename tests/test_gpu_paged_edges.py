@@ -33,6 +33,23 @@ def test_many_rows_without_a_plan():
     check_attend(make(counts, [0] * 70, NH=4, NKV=4, page=16))
 
 
+@pytest.mark.parametrize('rows', [33, 128, 131])
+def test_runs_of_very_different_lengths_without_a_plan(rows):
+    """Query tiles of one row up to seven, empty rows before, between and behind, two to five rows a lane of the search."""
+    g = torch.Generator().manual_seed(rows)
+    counts = [0] * rows
+    for b in torch.randperm(rows, generator=g)[:12].tolist():
+        counts[b] = int(torch.randint(1, 200, (1,), generator=g))
+    check_attend(make(counts, torch.randint(0, 200, (rows,), generator=g).tolist(), page=16))
+
+
+def test_many_query_tiles_joined():
+    """More rows to join than warps that join them, most of a query tile's rows without a token."""
+    g = torch.Generator().manual_seed(9)
+    pasts = torch.randint(900, 2400, (24,), generator=g).tolist()
+    check_attend(make([1] * 20 + [3, 2, 20, 1], pasts, NH=8, NKV=2, page=64))
+
+
 @pytest.mark.parametrize('page', [256, 1024])
 def test_large_pages(page):
     check_attend(make([3, 40, 1], [300, 0, 1500], page=page))
