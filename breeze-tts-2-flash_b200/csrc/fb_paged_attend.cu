@@ -17,12 +17,13 @@
 // case below.  The sums are exact either way; sum and reference are fp32, P goes to bf16, one part, as in the prefill.)
 //
 // Pieces.  A step can be one run of a few tokens over a long row, or many rows of which some are long.  So the key tiles of
-// a query tile are cut into s pieces of about C; a CTA takes one piece.  paged_plan_kernel (one CTA, from lengths and offsets
-// on the device: nothing is read on the host) writes the list; C is chosen among those with which the list fills one or
-// two rounds of the SMs, and whole query tiles, by what they take (where rows are too short to cut, there is no plan and CTAs
-// find their query tiles themselves: a short prompt 10 instead of 15 us).  Pieces of a query tile leave
-// (reference, sum, unnormalised out) in the workspace and paged_merge_kernel joins them in order: no atomics, the same
-// inputs give the same bits.  A query tile of one piece writes its rows itself.
+// a query tile are cut into s pieces of about C; a CTA takes one piece of the list that lengths and offsets, on the device,
+// come to (nothing is read on the host).  C is chosen among those with which the list fills one or two rounds of the SMs, and
+// whole query tiles, by what they take.  Up to 32 rows, and query tiles for one round at most, every CTA works this out itself,
+// a row a lane (1 us; a prompt of 17 tokens over 2000 slots 13.8 us, 16.0 with a kernel before it).  For more rows
+// paged_plan_kernel (one CTA) writes the list, 4 us: many CTAs that each work it out took up to 9% longer.  Where rows are too
+// short to cut, CTAs just find their query tiles.  Pieces of a query tile leave (reference, sum, unnormalised out) in the
+// workspace and paged_merge_kernel joins them in order: no atomics, the same inputs give the same bits.
 //
 // Rows of one token are runs as others are.  (The single-token kernel for them, in a launch of its own: 128 instead of 133 us
 // for 512 tokens beside 63 single ones over long rows, but 19 instead of 14 over short ones, and 5 us where there are none.)
@@ -32,8 +33,8 @@
 // computed again, one visible key at a time.
 //
 // Measured on a B200 (in a CUDA graph, 16 heads over 4): 2048 tokens over 32768 slots of one row 520 us, 1090 TFLOP/s, in
-// pages of 16 to 128 alike; 801 tokens of 32 rows over a window of 2048 (131 MB) 47 us; 512 tokens of one row beside one each
-// of 63, over up to 8000 slots (530 MB), 126 us; two prompts of 197 tokens 10 to 11 us.  A tile takes 1500 cycles with two
+// pages of 16 to 128 alike; 801 tokens of 32 rows over a window of 2048 (131 MB) 46 us; 512 tokens of one row beside one each
+// of 63, over up to 8000 slots (530 MB), 128 us; two prompts of 197 tokens 9.5 us.  A tile takes 1500 cycles with two
 // CTAs an SM: 700 to 870 are exponentials (the unit's bound for both CTAs is 1024), 100 the read of S, 240 masks, the rest
 // waits and stores; issuing S takes its thread 480 cycles and P V 290, both beside the exponentials.  Under the largest
 // case's load clocks fall to 1.5 GHz.  With few keys a piece it is beginning and ending (9000 cycles) that counts.  Tried
@@ -125,6 +126,17 @@ struct alignas(16) PagedPiece {
   int b, tok, nt, p_lo, i, s, slot, pad;   // b = -1: none
 };
 
+// Of a list with the longest piece: what it costs.
+__device__ __forceinline__ float paged_price(float rounds, float longest, bool cut) {
+  const float p = fmaxf(1.f, rounds) * (longest + PT_COST);
+  return cut ? p * PT_MORE + rounds * PT_JOIN + PT_JOINS : p;
+}
+// 1 / (key tiles of a piece) for which the list has room in j + 1 rounds of the SMs, 0: none.
+__device__ __forceinline__ float paged_room(const PagedAttendArgs& a, int j, int units, float work) {
+  const int room = (j + 1) * a.pieces - units;
+  return room > 0 ? fminf(__fdividef((float)room, work), 1.f / PT_MIN) : 0.f;
+}
+
 constexpr int PP_THREADS = 256, PP_WARPS = PP_THREADS / 32;
 constexpr int PP_ROWS = 1024;              // rows whose tiles are kept in shared memory
 
@@ -165,8 +177,7 @@ __global__ void __launch_bounds__(PP_THREADS) paged_plan_kernel(const __grid_con
     int n[PT_WAVES], most[PT_WAVES];
 #pragma unroll
     for (int j = 0; j < PT_WAVES; ++j) {
-      const int room = (j + 1) * a.pieces - units;
-      c[j] = room > 0 ? fminf(__fdividef((float)room, w), 1.f / PT_MIN) : 0.f;
+      c[j] = paged_room(a, j, units, w);
       n[j] = most[j] = 0;
     }
 #pragma unroll 1
@@ -187,12 +198,12 @@ __global__ void __launch_bounds__(PP_THREADS) paged_plan_kernel(const __grid_con
     }
     __syncthreads();
     // the cheapest of those and of whole query tiles; the places in the workspace are enough for `cuts` pieces
-    float price = fmaxf(1.f, (float)units * a.rounds) * ((float)longest + PT_COST);
+    float price = paged_price((float)units * a.rounds, (float)longest, false);
 #pragma unroll
     for (int j = 0; j < PT_WAVES; ++j) {
       const int count = __reduce_add_sync(FULL, lane < PP_WARPS ? s_n[j][lane] : 0);
       const float len = (float)__reduce_max_sync(FULL, lane < PP_WARPS ? s_most[j][lane] : 0);
-      const float rounds = (float)count * a.rounds, p = fmaxf(1.f, rounds) * (len + PT_COST) * PT_MORE + rounds * PT_JOIN + PT_JOINS;
+      const float p = paged_price((float)count * a.rounds, len, true);
       if (p < price && count <= a.cuts) price = p, r = c[j];
     }
   }
@@ -259,46 +270,92 @@ __global__ void __launch_bounds__(PP_THREADS) paged_plan_kernel(const __grid_con
   if (tid == 0 && a.cuts > 1) a.cut[a.cuts / 2] = make_int4(joins, 0, 0, 0);
 }
 
-// Piece x of the list whose query tiles stay whole, for a CTA without a plan: a warp, lane i counts rows [i per32, ..), the
-// first four of them from registers (108 rows of two tokens: 24 us; a row after the other, each load behind the last, 30).
-__device__ __forceinline__ void paged_direct(const PagedAttendArgs& a, int x, int lane, PagedPiece* piece) {
+// Piece x of the list, for a CTA without a plan: a warp, lane i has rows [i per32, ..), the first four of them in registers
+// (108 rows of two tokens: 24 us; a row after the other, each load behind the last, 30).  CUT (a row a lane): cut as the plan
+// would; the first head's CTAs also write what the merge needs.  Else query tiles stay whole.
+template <bool CUT>
+__device__ __forceinline__ void paged_find(const PagedAttendArgs& a, int x, int h, int lane, PagedPiece* piece) {
+  constexpr int R = CUT ? 1 : 4;
   const int b0 = min(lane * a.per32, a.r.rows), b1 = min(b0 + a.per32, a.r.rows);
-  long long f[5], len[4];
-  int k[4], n = 0;
+  long long f[R + 1], len[R];
+  int q[R], k[R], n = 0, slots = 0, joins = 0;               // query tiles of the rows, key tiles of their last
   f[0] = a.r.offsets[b0];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) f[i + 1] = a.r.offsets[min(b0 + i + 1, b1)], len[i] = a.r.lengths[min(b0 + i, a.r.rows - 1)];
+  for (int i = 0; i < R; ++i) f[i + 1] = a.r.offsets[min(b0 + i + 1, b1)], len[i] = a.r.lengths[min(b0 + i, a.r.rows - 1)];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    k[i] = b0 + i < b1 ? (paged_span(a.r, f[i], f[i + 1], len[i]).n + a.nq - 1) >> a.lq : 0;
-    n += k[i];
+  for (int i = 0; i < R; ++i) {
+    const PagedSpan y = paged_span(a.r, f[i], f[i + 1], len[i]);
+    const int p_hi = y.p0 + y.n - 1;
+    q[i] = b0 + i < b1 ? (y.n + a.nq - 1) >> a.lq : 0;
+    k[i] = CUT && q[i] > 0 ? (paged_segs(a, p_hi - min(y.n, a.nq) + 1, p_hi).n + 1) >> 1 : 0;
+    n += q[i];
   }
+  float r = 0.f;
+  if (CUT) {
+    float w = 0.f;
+    int longest = 0;
+#pragma unroll
+    for (int i = 0; i < R; ++i) w += (float)q[i] * (float)k[i], longest = max(longest, k[i]);
+    w = warp_sum(w);
+    const int units = __reduce_add_sync(FULL, n);
+    longest = __reduce_max_sync(FULL, longest);
+    float price = paged_price((float)units * a.rounds, (float)longest, false);
+#pragma unroll
+    for (int j = 0; j < PT_WAVES; ++j) {
+      const float c = paged_room(a, j, units, w);
+      int count = 0, most = 0;
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        const int s = paged_cut(k[i], c);
+        count += q[i] * s;
+        most = max(most, (int)__fdividef((float)(k[i] + s - 1), (float)s));
+      }
+      count = __reduce_add_sync(FULL, count);
+      const float p = paged_price((float)count * a.rounds, (float)__reduce_max_sync(FULL, most), true);
+      if (p < price && count <= a.cuts) price = p, r = c;
+    }
+    n = 0;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int s = paged_cut(k[i], r);
+      n += q[i] * s;
+      slots += s > 1 ? q[i] * s : 0;
+      joins += s > 1 ? q[i] : 0;
+    }
+  } else {
 #pragma unroll 1
-  for (int b = b0 + 4; b < b1; ++b) n += (paged_span(a.r, b).n + a.nq - 1) >> a.lq;
-  int before = n;
+    for (int b = b0 + R; b < b1; ++b) n += (paged_span(a.r, b).n + a.nq - 1) >> a.lq;
+  }
+  int before = n, slot = slots, join = joins;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(FULL, before, o);
-    if (lane >= o) before += y;
+    const int y = __shfl_up_sync(FULL, before, o), z = CUT ? __shfl_up_sync(FULL, slot, o) : 0, v = CUT ? __shfl_up_sync(FULL, join, o) : 0;
+    if (lane >= o) before += y, slot += z, join += v;
   }
+  if (CUT && lane == 31 && x == 0 && h == 0 && a.cuts > 1) a.cut[a.cuts / 2] = make_int4(join, 0, 0, 0);
   if (x >= before || x < before - n) {
     if (lane == 31 && x >= before) *piece = PagedPiece{-1, 0, 0, 0, 0, 1, 0, 0};
     return;
   }
-  int at = x - (before - n), b = b0;                         // the lane's query tile `at`, of row b
+  int at = x - (before - n), b = b0, tiles = q[0];           // the lane's piece `at`, of row b
+  const int s = CUT ? paged_cut(k[0], r) : 1;
+  slot -= slots;
+  join -= joins;
   PagedSpan span = paged_span(a.r, f[0], f[1], len[0]);
-  int tiles = k[0];
 #pragma unroll
-  for (int i = 1; i < 4; ++i)
-    if (b == b0 + i - 1 && at >= tiles) at -= tiles, ++b, tiles = k[i], span = paged_span(a.r, f[i], f[i + 1], len[i]);
+  for (int i = 1; i < R; ++i)
+    if (b == b0 + i - 1 && at >= tiles) at -= tiles, ++b, tiles = q[i], span = paged_span(a.r, f[i], f[i + 1], len[i]);
+  if (!CUT)
 #pragma unroll 1
-  while (at >= tiles) {
-    at -= tiles, ++b;
-    span = paged_span(a.r, b);
-    tiles = (span.n + a.nq - 1) >> a.lq;
-  }
-  const int q0 = (tiles - 1 - at) << a.lq;
-  *piece = PagedPiece{b, span.t0 + q0, min(a.nq, span.n - q0), span.p0 + q0, 0, 1, 0, 0};
+    while (at >= tiles) {
+      at -= tiles, ++b;
+      span = paged_span(a.r, b);
+      tiles = (span.n + a.nq - 1) >> a.lq;
+    }
+  const int u = CUT ? at / s : at, q0 = (tiles - 1 - u) << a.lq;
+  const PagedPiece p{b, span.t0 + q0, min(a.nq, span.n - q0), span.p0 + q0, at - u * s, s, slot + at, 0};
+  *piece = p;
+  if (CUT && s > 1 && p.i == 0 && h == 0) a.cut[join + u] = make_int4(p.tok, p.nt, s, p.slot);
 }
 
 constexpr int PT_THREADS = 256;                  // 4 softmax warps; one each for S, P V, the copies of K and of V
@@ -344,8 +401,9 @@ __device__ __noinline__ uint2 paged_one(const PagedAttendArgs& a, int b, int p, 
   return make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
 }
 
-// PLAN: pieces come from the plan, else CTAs find their query tiles.
-template <bool PLAN>
+// Pieces come from the plan (PT_PLAN), or CTAs find theirs: of query tiles that stay whole, or cut.
+enum { PT_FIND, PT_CUT, PT_PLAN };
+template <int HOW>
 __global__ void __launch_bounds__(PT_THREADS, 2) paged_attend_kernel(const __grid_constant__ PagedAttendArgs a) {
   // nothing but this: with 1 KB of the system's, two CTAs fill an SM, and the base is at a 1024-byte boundary (checked)
   extern __shared__ __align__(1024) unsigned char sq[];                   // Q; the output tile at the end
@@ -367,10 +425,10 @@ __global__ void __launch_bounds__(PT_THREADS, 2) paged_attend_kernel(const __gri
   pdl_wait();
   pdl_trigger();
   PagedPiece piece;
-  if constexpr (PLAN) {
+  if constexpr (HOW == PT_PLAN) {
     piece = a.plan[x];
   } else {
-    if (warp == 0) paged_direct(a, x, lane, &s_piece);
+    if (warp == 0) paged_find<HOW == PT_CUT>(a, x, h, lane, &s_piece);
     __syncthreads();
     piece = s_piece;
   }
@@ -823,12 +881,13 @@ int paged_group(const fb_paged_cache* c, int NH) {
 struct PagedPlan {
   int pieces;                           // a KV head, 0: query tiles stay whole
   bool direct;                          // nothing to cut: no plan, CTAs find their query tiles
-  int64_t list, cuts, slots, off_ml, off_plan, off_cut, ws_floats;
+  int64_t units, list, cuts, slots, off_ml, off_plan, off_cut, ws_floats;
 };
 int paged_plan_host(const fb_paged_cache* c, int rows, int width, int T, int NH, int window, int sinks, PagedPlan* p) {
   const int nq = LP_ROWS / (NH / c->NKV);
   const int64_t S = (int64_t)width * c->page, runs = rows < T ? rows : T;
   const int64_t units = (T + runs * (nq - 1)) / nq;                // query tiles, at most
+  p->units = units;
   // key tiles of a query tile, at most
   int64_t keys = S;
   if (window > 0 && (int64_t)window + sinks + nq + 3 * LP_SEG < S) keys = (int64_t)window + sinks + nq + 3 * LP_SEG;
@@ -836,8 +895,9 @@ int paged_plan_host(const fb_paged_cache* c, int rows, int width, int T, int NH,
   // CTAs that the SMs hold.  By the device's SMs, not the calling thread's budget: the workspace's size goes by it.
   p->pieces = most > PT_WHOLE ? (2 * fbh::num_sms() + c->NKV - 1) / c->NKV : 0;
   p->direct = p->pieces == 0;
-  // a list is cut for PT_WAVES rounds at most and into pieces of PT_MIN at least, or is its query tiles
-  p->cuts = (int64_t)PT_WAVES * p->pieces;
+  // a list is cut for PT_WAVES rounds at most (one where query tiles fill less than half of it: two gain nothing by the price
+  // below rows of 12800 slots) and into pieces of PT_MIN at least, or is its query tiles
+  p->cuts = (int64_t)(2 * units <= p->pieces ? 1 : PT_WAVES) * p->pieces;
   if (p->cuts > units * ((most + PT_MIN - 1) / PT_MIN)) p->cuts = units * ((most + PT_MIN - 1) / PT_MIN);
   p->list = units > p->cuts ? units : p->cuts;
   FB_CHECK_ARG(p->list * c->NKV <= 0x7fffffff, "paged_attend: too many tokens, rows and heads");
@@ -926,21 +986,24 @@ extern "C" int flashb_paged_attend(const fb_paged_cache* cache, const int32_t* t
     a.tk = a.tks, a.tv = a.tvs;          // not used
   }
   if (rc) return rc;
-  const void* attend = p.direct ? (const void*)paged_attend_kernel<false> : (const void*)paged_attend_kernel<true>;
-  static int attr_done[64][2] = {{0}};
+  const int how = p.direct ? PT_FIND : rows <= 32 && p.units <= p.pieces ? PT_CUT : PT_PLAN;
+  const void* attend = how == PT_FIND  ? (const void*)paged_attend_kernel<PT_FIND>
+                       : how == PT_CUT ? (const void*)paged_attend_kernel<PT_CUT>
+                                       : (const void*)paged_attend_kernel<PT_PLAN>;
+  static int attr_done[64][3] = {{0}};
   int dev = 0;
   cudaGetDevice(&dev);
-  if (dev >= 64 || !attr_done[dev][p.direct]) {
+  if (dev >= 64 || !attr_done[dev][how]) {
     const cudaError_t e = cudaFuncSetAttribute(attend, cudaFuncAttributeMaxDynamicSharedMemorySize, PT_SMEM);
     if (e != cudaSuccess) {
       fbh::set_msg("paged_attend: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
       return FB_ERR_CUDA;
     }
-    if (dev < 64) attr_done[dev][p.direct] = 1;
+    if (dev < 64) attr_done[dev][how] = 1;
   }
   const cudaStream_t st = (cudaStream_t)stream;
   void* args[] = {(void*)&a};
-  if (!p.direct) rc = fbh::launch_pdl((const void*)paged_plan_kernel, dim3(1), dim3(PP_THREADS), 0, st, args, true);
+  if (how == PT_PLAN) rc = fbh::launch_pdl((const void*)paged_plan_kernel, dim3(1), dim3(PP_THREADS), 0, st, args, true);
   if (!rc) rc = fbh::launch_pdl(attend, dim3((unsigned)(p.list * a.NKV)), dim3(PT_THREADS), PT_SMEM, st, args, true);
   if (rc || p.cuts < 2) return rc;
   const int64_t joins = (p.cuts / 2 * a.NKV * LP_ROWS + PM_THREADS / 32 - 1) / (PM_THREADS / 32);

@@ -43,6 +43,23 @@ def test_runs_of_very_different_lengths_without_a_plan(rows):
     check_attend(make(counts, torch.randint(0, 200, (rows,), generator=g).tolist(), page=16))
 
 
+@pytest.mark.parametrize('rows,NH,NKV', [(32, 8, 2), (33, 8, 2), (60, 4, 4), (300, 2, 1)])
+def test_cut_rows_among_many(rows, NH, NKV):
+    """Lists that every CTA works out and lists of the plan, of one row a thread and more."""
+    g = torch.Generator().manual_seed(rows)
+    counts = torch.randint(0, 4, (rows,), generator=g).tolist()
+    pasts = torch.randint(0, 100, (rows,), generator=g).tolist()
+    for b in (0, 5, rows // 2, rows - 1):
+        counts[b], pasts[b] = 1 + b % 3, 1500 + 100 * (b % 7)
+    check_attend(make(counts, pasts, NH, NKV, page=32))
+    check_attend(make(counts, pasts, NH, NKV, page=32), 900, 3)
+
+
+def test_more_query_tiles_than_a_round():
+    """Few rows of many tokens: the plan again, most query tiles whole."""
+    check_attend(make([2, 1500, 1], [700, 40, 600], NH=8, NKV=8, page=64))
+
+
 def test_many_query_tiles_joined():
     """More rows to join than warps that join them, most of a query tile's rows without a token."""
     g = torch.Generator().manual_seed(9)
