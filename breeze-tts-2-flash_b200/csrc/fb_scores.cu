@@ -19,7 +19,7 @@
 //
 // Measured on a B200 (in a CUDA graph): 4095 rows of 32003 in bf16 with 20 alternatives (262 MB) 73 us, 0.55 of the measured
 // copy bandwidth; 1088 rows of 2049 in fp32 with 8 (9 MB) 6.6 us; 17 rows 3.9 us.  The first is bound by issue (0.7 of the
-// slots; some 10 instructions a logit, 1 of them an exponential).
+// slots; 12.5 instructions a logit in all, 1 of them an exponential).
 //
 // Rows that the fast path cannot take go through scores_slow, a pass per alternative: a NaN or +inf, -inf alone, logits
 // past 2^60, more than SC_CAP logits at the threshold (rows of equal logits), fewer finite logits than alternatives.
