@@ -18,8 +18,8 @@
 //
 // Pieces.  A step can be one run of a few tokens over a long row, or many rows of which some are long.  So the key tiles of
 // a query tile are cut into s pieces of about C; a CTA takes one piece of the list that lengths and offsets, on the device,
-// come to (nothing is read on the host).  C is chosen among those with which the list fills one or two rounds of the SMs, and
-// whole query tiles, by what they take.  Up to 32 rows, and query tiles for one round at most, every CTA works this out itself,
+// come to (nothing is read on the host).  C is chosen among those with which the list fills one round or about two, and whole
+// query tiles, by what they take.  Up to 32 rows, and query tiles for one round at most, every CTA works this out itself,
 // a row a lane (1 us; a prompt of 17 tokens over 2000 slots 13.8 us, 16.0 with a kernel before it).  For more rows
 // paged_plan_kernel (one CTA) writes the list, 4 us: many CTAs that each work it out took up to 9% longer.  Where rows are too
 // short to cut, CTAs just find their query tiles.  Pieces of a query tile leave (reference, sum, unnormalised out) in the
@@ -34,7 +34,7 @@
 //
 // Measured on a B200 (in a CUDA graph, 16 heads over 4): 2048 tokens over 32768 slots of one row 520 us, 1090 TFLOP/s, in
 // pages of 16 to 128 alike; 801 tokens of 32 rows over a window of 2048 (131 MB) 46 us; 512 tokens of one row beside one each
-// of 63, over up to 8000 slots (530 MB), 128 us; two prompts of 197 tokens 9.5 us.  A tile takes 1500 cycles with two
+// of 63, over up to 8000 slots (530 MB), 116 us; two prompts of 197 tokens 9.5 us.  A tile takes 1500 cycles with two
 // CTAs an SM: 700 to 870 are exponentials (the unit's bound for both CTAs is 1024), 100 the read of S, 240 masks, the rest
 // waits and stores; issuing S takes its thread 480 cycles and P V 290, both beside the exponentials.  Under the largest
 // case's load clocks fall to 1.5 GHz.  With few keys a piece it is beginning and ending (9000 cycles) that counts.  Tried
@@ -51,13 +51,13 @@ namespace fb {
 
 constexpr int PT_WHOLE = 8;                       // query tiles of so few key tiles stay whole, without a plan
 constexpr int PT_MIN = 6;                         // key tiles of a piece, at least
-constexpr int PT_WAVES = 2;                       // rounds of CTAs that the list of pieces may be cut for
+constexpr int PT_WAVES = 2;                       // rounds of CTAs that the list of pieces may be cut for (and an eighth)
 constexpr float PT_LIMIT = 0x1p-16f;              // 2^(8 + LP_SHIFT): a tile's weights below it leave the reference as it is
-// What a list costs, in the time of a key tile: max(1, rounds) (longest piece + PT_COST), and where anything is cut that
-// PT_MORE times (under the power limit all SMs at work are no faster than seven eighths of them), PT_JOIN a round (parts
-// written and read again) and PT_JOINS.  Fitted to 430 lists of 45 drawn steps (pieces of 5 to 128 tiles, and whole): its
-// choices take 2% more time than the best of each step, 9% at most; those by rounds x (longest + 5) 7%, 36% at most.
-constexpr float PT_COST = 20.f, PT_MORE = 1.125f, PT_JOIN = 9.f, PT_JOINS = 3.f;
+// What a list costs, in the time of a key tile: the longest piece + PT_COST where it fits one round of the SMs, else what all
+// pieces are to an SM's place and a share PT_LAST of the longest; and where anything is cut PT_JOIN a round (parts written and
+// read again) and PT_JOINS.  Fitted to 430 lists of 45 drawn steps (pieces of 5 to 128 tiles, and whole): its choices take
+// 1.5% more time than the best of each step, 7% at most; those by rounds x (longest + 5) 7%, 36% at most.
+constexpr float PT_COST = 8.f, PT_LAST = 0.5f, PT_JOIN = 2.f, PT_JOINS = 4.f;
 
 struct PagedPiece;
 
@@ -126,15 +126,17 @@ struct alignas(16) PagedPiece {
   int b, tok, nt, p_lo, i, s, slot, pad;   // b = -1: none
 };
 
-// Of a list with the longest piece: what it costs.
-__device__ __forceinline__ float paged_price(float rounds, float longest, bool cut) {
-  const float p = fmaxf(1.f, rounds) * (longest + PT_COST);
-  return cut ? p * PT_MORE + rounds * PT_JOIN + PT_JOINS : p;
+// What a list of n pieces, of so many key tiles in all and in the longest, costs.
+__device__ __forceinline__ float paged_price(const PagedAttendArgs& a, int n, float work, float longest, bool cut) {
+  const float rounds = (float)n * a.rounds;
+  const float p = rounds <= 1.f ? longest + PT_COST : (work + PT_COST * (float)n) * a.rounds + PT_LAST * longest;
+  return cut ? p + rounds * PT_JOIN + PT_JOINS : p;
 }
-// 1 / (key tiles of a piece) for which the list has room in j + 1 rounds of the SMs, 0: none.
+// 1 / (key tiles of a piece) for which the list has room in a round of the SMs, or (j = 1) comes to about two: a query tile
+// has up to one piece more than its key tiles come to.  0: no room.
 __device__ __forceinline__ float paged_room(const PagedAttendArgs& a, int j, int units, float work) {
-  const int room = (j + 1) * a.pieces - units;
-  return room > 0 ? fminf(__fdividef((float)room, work), 1.f / PT_MIN) : 0.f;
+  const float room = (float)((j + 1) * a.pieces) - (j ? 0.6f : 1.f) * (float)units;
+  return room > 0.f ? fminf(__fdividef(room, work), 1.f / PT_MIN) : 0.f;
 }
 
 constexpr int PP_THREADS = 256, PP_WARPS = PP_THREADS / 32;
@@ -198,12 +200,12 @@ __global__ void __launch_bounds__(PP_THREADS) paged_plan_kernel(const __grid_con
     }
     __syncthreads();
     // the cheapest of those and of whole query tiles; the places in the workspace are enough for `cuts` pieces
-    float price = paged_price((float)units * a.rounds, (float)longest, false);
+    float price = paged_price(a, units, w, (float)longest, false);
 #pragma unroll
     for (int j = 0; j < PT_WAVES; ++j) {
       const int count = __reduce_add_sync(FULL, lane < PP_WARPS ? s_n[j][lane] : 0);
       const float len = (float)__reduce_max_sync(FULL, lane < PP_WARPS ? s_most[j][lane] : 0);
-      const float p = paged_price((float)count * a.rounds, len, true);
+      const float p = paged_price(a, count, w, len, true);
       if (p < price && count <= a.cuts) price = p, r = c[j];
     }
   }
@@ -299,7 +301,7 @@ __device__ __forceinline__ void paged_find(const PagedAttendArgs& a, int x, int 
     w = warp_sum(w);
     const int units = __reduce_add_sync(FULL, n);
     longest = __reduce_max_sync(FULL, longest);
-    float price = paged_price((float)units * a.rounds, (float)longest, false);
+    float price = paged_price(a, units, w, (float)longest, false);
 #pragma unroll
     for (int j = 0; j < PT_WAVES; ++j) {
       const float c = paged_room(a, j, units, w);
@@ -311,7 +313,7 @@ __device__ __forceinline__ void paged_find(const PagedAttendArgs& a, int x, int 
         most = max(most, (int)__fdividef((float)(k[i] + s - 1), (float)s));
       }
       count = __reduce_add_sync(FULL, count);
-      const float p = paged_price((float)count * a.rounds, (float)__reduce_max_sync(FULL, most), true);
+      const float p = paged_price(a, count, w, (float)__reduce_max_sync(FULL, most), true);
       if (p < price && count <= a.cuts) price = p, r = c;
     }
     n = 0;
@@ -897,7 +899,7 @@ int paged_plan_host(const fb_paged_cache* c, int rows, int width, int T, int NH,
   p->direct = p->pieces == 0;
   // a list is cut for PT_WAVES rounds at most (one where query tiles fill less than half of it: two gain nothing by the price
   // below rows of 12800 slots) and into pieces of PT_MIN at least, or is its query tiles
-  p->cuts = (int64_t)(2 * units <= p->pieces ? 1 : PT_WAVES) * p->pieces;
+  p->cuts = 2 * units <= p->pieces ? p->pieces : (int64_t)PT_WAVES * p->pieces + p->pieces / 8;
   if (p->cuts > units * ((most + PT_MIN - 1) / PT_MIN)) p->cuts = units * ((most + PT_MIN - 1) / PT_MIN);
   p->list = units > p->cuts ? units : p->cuts;
   FB_CHECK_ARG(p->list * c->NKV <= 0x7fffffff, "paged_attend: too many tokens, rows and heads");
