@@ -79,7 +79,8 @@ struct alignas(64) PagedAttendArgs {
   float* po;                            // pieces: unnormalised out [slot][128][128],
   float2* ml;                           //   maximum and sum [slot][128]
   PagedPiece* plan;                     // [list]
-  int4* cut;                            // [cuts / 2] query tiles of two pieces and more: first token, tokens, pieces, slot; then their number
+  int4* cut;                            // [cuts / 2] query tiles of two pieces and more (first token, tokens, pieces, slot),
+                                        //   then their number
   unsigned* err;
 };
 
@@ -129,7 +130,7 @@ struct alignas(16) PagedPiece {
 // What a list of n pieces, of so many key tiles in all and in the longest, costs.
 __device__ __forceinline__ float paged_price(const PagedAttendArgs& a, int n, float work, float longest, bool cut) {
   const float rounds = (float)n * a.rounds;
-  const float p = rounds <= 1.f ? longest + PT_COST : (work + PT_COST * (float)n) * a.rounds + PT_LAST * longest;
+  const float p = n <= a.pieces ? longest + PT_COST : (work + PT_COST * (float)n) * a.rounds + PT_LAST * longest;
   return cut ? p + rounds * PT_JOIN + PT_JOINS : p;
 }
 // 1 / (key tiles of a piece) for which the list has room in a round of the SMs, or (j = 1) comes to about two: a query tile
@@ -331,7 +332,8 @@ __device__ __forceinline__ void paged_find(const PagedAttendArgs& a, int x, int 
   int before = n, slot = slots, join = joins;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(FULL, before, o), z = CUT ? __shfl_up_sync(FULL, slot, o) : 0, v = CUT ? __shfl_up_sync(FULL, join, o) : 0;
+    const int y = __shfl_up_sync(FULL, before, o);
+    const int z = CUT ? __shfl_up_sync(FULL, slot, o) : 0, v = CUT ? __shfl_up_sync(FULL, join, o) : 0;
     if (lane >= o) before += y, slot += z, join += v;
   }
   if (CUT && lane == 31 && x == 0 && h == 0 && a.cuts > 1) a.cut[a.cuts / 2] = make_int4(join, 0, 0, 0);
@@ -803,8 +805,8 @@ __global__ void __launch_bounds__(PT_THREADS, 2) paged_attend_kernel(const __gri
   }
 }
 
-// Joins the pieces of the query tiles that were cut, in their order: a warp a row, the CTAs that the SMs hold go round (how many
-// rows there are only the device knows).  For 801 tokens of 32 rows in 3 pieces (24 MB) 7.5 us, 1.5 of them the launch; with a
+// Joins the pieces of the query tiles that were cut, in their order: a warp a row, the CTAs that the SMs hold go round (how
+// many rows there are only the device knows).  For 801 tokens of 32 rows in 3 pieces (24 MB) 7.5 us, 1.5 of them the launch; with a
 // CTA for every 16 rows that there might be 8.7, two rows a warp at a time 8 to 10.
 constexpr int PM_THREADS = 256, PM_CTAS = 4;
 __global__ void __launch_bounds__(PM_THREADS, PM_CTAS) paged_merge_kernel(const __grid_constant__ PagedAttendArgs a) {
@@ -970,9 +972,12 @@ extern "C" int flashb_paged_attend(const fb_paged_cache* cache, const int32_t* t
   if (rc) return rc;
   FB_CHECK_ARG(p.ws_floats == 0 || (ws && ((uintptr_t)ws & 15) == 0 && ws_floats >= p.ws_floats),
                "paged_attend: workspace of %lld floats, %lld needed", (long long)ws_floats, (long long)p.ws_floats);
-  a.NKV = cache->NKV, a.nq = LP_ROWS / a.G, a.lg = a.G == 1 ? 0 : a.G == 2 ? 1 : a.G == 4 ? 2 : 3, a.lq = 7 - a.lg, a.per = (rows + PP_THREADS - 1) / PP_THREADS, a.pieces = p.pieces, a.list = (int)p.list, a.cuts = (int)p.cuts;
+  a.NKV = cache->NKV, a.nq = LP_ROWS / a.G, a.lg = a.G == 1 ? 0 : a.G == 2 ? 1 : a.G == 4 ? 2 : 3, a.lq = 7 - a.lg;
+  a.per = (rows + PP_THREADS - 1) / PP_THREADS, a.per32 = (rows + 31) / 32;
+  a.pieces = p.pieces, a.list = (int)p.list, a.cuts = (int)p.cuts;
   a.rounds = p.pieces ? 1.f / p.pieces : 0.f;
-  a.po = ws, a.ml = (float2*)(ws + p.off_ml), a.per32 = (rows + 31) / 32, a.plan = p.direct ? nullptr : (PagedPiece*)(ws + p.off_plan), a.cut = (int4*)(ws + p.off_cut);
+  a.po = ws, a.ml = (float2*)(ws + p.off_ml), a.plan = p.direct ? nullptr : (PagedPiece*)(ws + p.off_plan);
+  a.cut = (int4*)(ws + p.off_cut);
   a.err = fbh::device_err_ptr();
   const unsigned long long qd[4] = {64, (unsigned long long)NH, (unsigned long long)T, 2};
   const unsigned long long qs[3] = {(unsigned long long)(NH > 1 ? q_sh : LG_D) * 2, (unsigned long long)(T > 1 ? q_st : LG_D) * 2, 128};
