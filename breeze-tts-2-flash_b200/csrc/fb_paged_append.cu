@@ -13,11 +13,11 @@
 // way), eight lanes a head; the first copies are issued before the tokens' places are known.  Places (up to seven tokens a
 // warp, no load waiting for another token's) and one sine and cosine for each pair and token are worked out once a CTA.
 //
-// Measured on a B200 (in a CUDA graph): 16391 tokens of 24 heads (201 MB) 41 us, 0.74 of the measured copy bandwidth, with
-// head norms 40 us; one token of 128 rows 3.0 us, of 2 rows 2.9 us.  Sixteen lanes a head 41 us, but 53 with norms (twice
-// the instructions a head) and 3.4 for one token.  Rings of five units of eight heads 42 us, 30 instead of 23 for tokens of
-// twelve heads (a unit of eight and one of four); four tokens a warp 39, but 47 with norms; three CTAs an SM 45; loads
-// straight to registers, six a thread, 48 to 58 whatever the occupancy (too few bytes under way).
+// Measured on a B200 (in a CUDA graph): 16391 tokens of 24 heads (201 MB) 39 us, 0.79 of the measured copy bandwidth, with
+// head norms 40 us; one token of 128 rows 3.0 us, of 2 rows 2.9 us.  Sixteen lanes a head (and one round of CTAs) 41 us, 53
+// with norms (twice the instructions a head) and 3.4 for one token.  Rings of five units of eight heads 42 us, 30 instead of
+// 23 for tokens of twelve heads (a unit of eight and one of four); three CTAs an SM 45; loads straight to registers, six a
+// thread, 48 to 58 whatever the occupancy (too few bytes under way).
 #include <climits>
 
 #include "fb_long_tc.cuh"
@@ -297,8 +297,10 @@ extern "C" int flashb_paged_append(const fb_paged_cache* cache, const int32_t* t
   a.turns = turns, a.positions = (const long long*)positions;
   a.q_out = (bf16*)q_out, a.o_st = o_st, a.o_sh = o_sh;
   const int at_once = PA_CTAS * fbh::grid_sms();
-  a.tokens = (T - 1) / at_once + 1;
-  if (a.tokens > PA_TOKENS) a.tokens = PA_TOKENS;
+  // Rounds of CTAs, all of them full (20000 tokens in CTAs of 56 56 us, in two rounds 46).  Where there are no norms to work
+  // out, shorter CTAs begin and end beside others' streams: 16391 tokens in CTAs of 56 41 us, of 28 38 us; with norms 40 and 43.
+  const int most = q_norm ? PA_TOKENS : 32, rounds = (T - 1) / (at_once * most) + 1;
+  a.tokens = (T - 1) / (at_once * rounds) + 1;
   const int parts = (heads + PA_HEADS - 1) / PA_HEADS;       // of a token, equal but for whole fours of heads
   a.each = a.tokens * parts >= PA_WARPS ? ((heads + parts - 1) / parts + 3) / 4 * 4 : 4;   // few tokens: a unit for every warp
   a.err = fbh::device_err_ptr();

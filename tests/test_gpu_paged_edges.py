@@ -172,6 +172,39 @@ def test_steps_without_dependent_launch():
     check_attend(s)
 
 
+@pytest.mark.parametrize('norm', [False, True])
+@pytest.mark.parametrize('T,NH,NKV', [(9473, 1, 1), (17001, 2, 1), (20011, 7, 3), (33333, 1, 2), (40001, 11, 1)])
+def test_append_in_rounds(T, NH, NKV, norm):
+    """More tokens than the CTAs that an SM holds take at once: each token's bits are those of a call of its row's part alone."""
+    m = paged()
+    g = torch.Generator().manual_seed(T)
+    cut = [0, 37, 37, T // 3, T - 5000, T]                      # runs, one of them empty
+    offsets = torch.tensor(cut)
+    lengths = offsets.diff() + torch.tensor([3, 5, 100, 0, 71])
+    width = int((lengths.max() + 63) // 64)
+    table = torch.randperm(5 * width, generator=g).view(5, width).int()
+    qkv = torch.randn(T, (NH + 2 * NKV) * D, generator=g).bfloat16().cuda()
+    w = [torch.randn(D, generator=g).bfloat16().cuda() for _ in range(2)] if norm else [None, None]
+    rot = m.Rotary(96, layout='interleaved')
+    got = []
+    for parts in (1, 5):
+        keys, values = (torch.zeros(5 * width, NKV, 64, D, dtype=torch.bfloat16, device='cuda') for _ in range(2))
+        c = m.PagedCache(keys, values)
+        if parts == 1:
+            q = m.append(qkv, c, table.cuda(), lengths.cuda(), offsets=offsets.cuda(), rotary=rot, q_norm=w[0], k_norm=w[1])
+        else:
+            q = torch.zeros_like(got[0][0])
+            for b in range(5):
+                for lo in range(cut[b], cut[b + 1], 3000):      # pieces of the row's run
+                    hi = min(lo + 3000, cut[b + 1])
+                    q[lo:hi] = m.append(qkv[lo:hi], c, table[b:b + 1].cuda(), (lengths[b:b + 1] - (cut[b + 1] - hi)).cuda(),
+                                        offsets=torch.tensor([0, hi - lo]).cuda(), rotary=rot, q_norm=w[0], k_norm=w[1])
+        got.append((q, keys, values))
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+    assert int((got[0][2] != 0).any(-1).sum()) == T * NKV       # every token's values are somewhere
+
+
 def test_infinities_beside_rotated_dims():
     """What is not rotated is copied: an infinity there stays alone, whatever stands beside it."""
     m = paged()
