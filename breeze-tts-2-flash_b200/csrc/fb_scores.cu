@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(SC_MAX, 2) scores_kernel(const __grid_constant
   constexpr int N = 32 / sizeof(T);                      // logits of a unit
   __shared__ unsigned s_max[SC_MAX / 32], s_thr[SC_MAX / 32];
   __shared__ float s_sum[SC_MAX / 32], s_dot[SC_MAX / 32];
-  __shared__ int s_cnt[SC_MAX / 32], s_n;
+  __shared__ int s_cnt[SC_MAX / 32], s_n, s_kept;
   __shared__ unsigned long long s_key[SC_CAP];
   const int r = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, step = blockDim.x, W = step >> 5;
   if (tid == 0) s_n = 0;
@@ -434,10 +434,10 @@ __global__ void __launch_bounds__(SC_MAX, 2) scores_kernel(const __grid_constant
         m += __popc(keep);
         __syncwarp();
       }
-      if (lane == 0) s_n = m;
+      if (lane == 0) s_kept = m;                         // not s_n: other warps may still be on their way to this branch
     }
     __syncthreads();
-    n = s_n;
+    n = s_kept;
   }
   for (int i = tid; i < n; i += step) {
     const unsigned long long k = s_key[i];
