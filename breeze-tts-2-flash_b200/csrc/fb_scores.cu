@@ -21,10 +21,12 @@
 // copy bandwidth; 1088 rows of 2049 in fp32 with 8 (9 MB) 6.6 us; 17 rows 3.9 us.  The first is bound by issue (0.7 of the
 // slots; 12.5 instructions a logit in all, 1 of them an exponential).
 //
-// Rows that the fast path cannot take go through scores_slow, a pass per alternative: a NaN or +inf, -inf alone, logits
-// past 2^60, more than SC_CAP logits at the threshold (rows of equal logits), fewer finite logits than alternatives.
+// Rows that the fast path cannot take go through scores_slow, a pass per alternative: a NaN or +inf, -inf alone, a largest
+// logit of more than 2^27 temperatures, temperatures past 10^29, more than SC_CAP logits at the threshold (rows of equal
+// logits), fewer finite logits than alternatives.
 #include <cfloat>
 #include <climits>
+#include <cmath>
 
 #include "fb_long.cuh"
 #include "fb_sample.cuh"
@@ -34,7 +36,12 @@ namespace fb {
 constexpr int SC_MAX = 512;             // threads of a CTA, at most
 constexpr int SC_CAP = 1024;            // logits collected for the alternatives
 constexpr int SC_EACH = 16;             // so many of them a lane, at most, where they are thinned out first
-constexpr float SC_LOW = -0x1p100f;     // what -inf is taken for in e (x c - R); a largest logit below it: the slow path
+// Exponents x c on the fast path.  The largest one of a row is below SC_FAR in size: an exponent less its own rounding (the
+// first reference of a unit) is then 2^3 at most, and 2^5 for those that are masked by a finite value.  Threads begin at
+// SC_START; what lies below is taken for `low`, whose exponent is SC_START to twice that at every temperature: finite, never
+// above a reference, and 0 beside the row's largest.  (A fixed -2^100 for it: products past fp32's range at temperatures
+// below 5e-9, exponentials of more than a reference above 1.44, and masked ids of some probability from 10^28 on.)
+constexpr float SC_FAR = 0x1p28f, SC_START = -0x1p30f;
 constexpr float SC_LN2 = 0.6931471805599453f;
 
 struct ScoresArgs {
@@ -42,7 +49,7 @@ struct ScoresArgs {
   long long ld;
   int rows, V, top;
   const long long* tokens;
-  float inv, c;                         // 1 / temperature; that x log2(e)
+  float inv, c, low;                    // 1 / temperature; that x log2(e); the least logit of the fast path (-inf: none)
   float *logprob, *entropy, *top_logprob;
   long long *rank, *top_id;
 };
@@ -130,12 +137,12 @@ __device__ __noinline__ void scores_slow(const ScoresArgs& a, int r) {
   }
 }
 
-// Logits below SC_LOW (-inf) as SC_LOW; a NaN stays.
+// Logits below `low` (a power of two: exact in bf16), -inf among them, as `low`; a NaN stays.
 template <typename T>
-__device__ __forceinline__ uint32_t score_clamp(uint32_t w) {
+__device__ __forceinline__ uint32_t score_clamp(uint32_t w, float low) {
   uint32_t r;
-  if constexpr (sizeof(T) == 4) asm("max.NaN.f32 %0, %1, %2;" : "=r"(r) : "r"(w), "r"(__float_as_uint(SC_LOW)));
-  else asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(w), "r"((__float_as_uint(SC_LOW) >> 16) * 0x10001u));
+  if constexpr (sizeof(T) == 4) asm("max.NaN.f32 %0, %1, %2;" : "=r"(r) : "r"(w), "r"(__float_as_uint(low)));
+  else asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(w), "r"((__float_as_uint(low) >> 16) * 0x10001u));
   return r;
 }
 
@@ -204,7 +211,7 @@ __global__ void __launch_bounds__(SC_MAX, 2) scores_kernel(const __grid_constant
 
   const float c = a.c;
   const uint64_t c2 = f2(c, c);
-  float R = -0x1p100f, sum = 0.f, dot = 0.f, bs = 0.f, bd = 0.f, tm = -INFINITY, tm2 = -INFINITY, tm3 = -INFINITY;
+  float R = SC_START, sum = 0.f, dot = 0.f, bs = 0.f, bd = 0.f, tm = -INFINITY, tm2 = -INFINITY, tm3 = -INFINITY;
   int iu = -2, iu2 = -2, cnt = 0;                        // the units that hold tm and tm2 (-2: none)
   // f(pair of logits, the first one's place in the unit)
   auto pairs = [&](const ScoreUnit& u, auto f) {
@@ -221,7 +228,8 @@ __global__ void __launch_bounds__(SC_MAX, 2) scores_kernel(const __grid_constant
     ScoreUnit o;
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-      o.w[i] = make_uint4(score_clamp<T>(u.w[i].x), score_clamp<T>(u.w[i].y), score_clamp<T>(u.w[i].z), score_clamp<T>(u.w[i].w));
+      o.w[i] = make_uint4(score_clamp<T>(u.w[i].x, a.low), score_clamp<T>(u.w[i].y, a.low), score_clamp<T>(u.w[i].z, a.low),
+                          score_clamp<T>(u.w[i].w, a.low));
     return o;
   };
   auto whole = [&](int v) { return ScoreUnit{body[2 * v], body[2 * v + 1]}; };
@@ -332,7 +340,7 @@ __global__ void __launch_bounds__(SC_MAX, 2) scores_kernel(const __grid_constant
   const unsigned thr = __reduce_min_sync(FULL, lane < W ? s_thr[lane] : 0xffffffffu);
   const int holder = __ffs(__ballot_sync(FULL, wm == M)) - 1;
   const float xm = ord2f(M), hi = xm * c, lo = fmaf(xm, c, -hi);
-  bool fast = M != 0 && xm > SC_LOW && fabsf(hi) < 0x1p60f;
+  bool fast = M != 0 && a.low > -INFINITY && fabsf(hi) < SC_FAR;
   const bool owner = warp == holder && lane == __ffs(__ballot_sync(FULL, key == M)) - 1;
   if (fast) {
     // ---- the units that reach the threshold, and the largest's without its own 1
@@ -466,6 +474,9 @@ extern "C" int flashb_token_scores(const void* logits, int is_bf16, int64_t ld, 
   ScoresArgs a{};
   a.x = logits, a.ld = ld, a.rows = rows, a.V = V, a.top = top, a.tokens = (const long long*)tokens;
   a.inv = 1.f / temperature, a.c = a.inv * LG_LOG2E;
+  int e = 0;
+  std::frexp(a.c, &e);                                   // c in [2^(e - 1), 2^e): low c in (2 SC_START, SC_START]
+  a.low = std::isfinite(a.c) && 31 - e <= 127 ? -std::ldexp(1.f, 31 - e) : -INFINITY;
   a.logprob = logprob, a.entropy = entropy, a.top_logprob = top_logprob;
   a.rank = (long long*)rank, a.top_id = (long long*)top_id;
   // Threads of a row.  While the rows leave SMs half empty, up to 512, of four units and more (500 rows of 65536 in fp32: 68
