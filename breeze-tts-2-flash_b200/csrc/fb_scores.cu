@@ -64,6 +64,11 @@ __device__ __forceinline__ float score_at(const T* x, int i) {
   if constexpr (sizeof(T) == 4) return x[i];
   else return __uint_as_float((uint32_t)x[i] << 16);
 }
+// (x - m) / temperature, m the row's maximum.  A difference past fp32's range may be within it once divided: from halves.
+__device__ __forceinline__ float score_below(float x, float m, float inv) {
+  const float d = x - m;
+  return d == -INFINITY ? (0.5f * x - 0.5f * m) * inv * 2.f : d * inv;
+}
 template <typename T, class F>
 __device__ __forceinline__ T block_reduce(T v, T* s, F f) {
 #pragma unroll
@@ -109,7 +114,7 @@ __device__ __noinline__ void scores_slow(const ScoresArgs& a, int r) {
   const bool none = !(fabsf(m) < INFINITY);              // no distribution: a NaN or +inf first, or -inf alone
   float rest = 0.f, dot = 0.f;
   for (int i = tid; i < a.V; i += step) {
-    const float d = (score_at(x, i) - m) * a.inv, e = i == i0 ? 0.f : __expf(d);
+    const float d = score_below(score_at(x, i), m, a.inv), e = i == i0 ? 0.f : __expf(d);
     rest += e;
     if (e > 0.f) dot -= e * d;
   }
@@ -117,7 +122,7 @@ __device__ __noinline__ void scores_slow(const ScoresArgs& a, int r) {
   dot = block_reduce(dot, s_f, ScoreAdd());
   const float logz = log1pf(rest);
   if (tid == 0) {
-    a.logprob[r] = none ? NAN : known ? (xt - m) * a.inv - logz : -INFINITY;
+    a.logprob[r] = none ? NAN : known ? score_below(xt, m, a.inv) - logz : -INFINITY;
     a.entropy[r] = none ? NAN : logz + dot / (1.f + rest);
     a.rank[r] = before;
   }
@@ -132,7 +137,7 @@ __device__ __noinline__ void scores_slow(const ScoresArgs& a, int r) {
     if (tid == 0) {
       const int id = (int)(0xffffffffu - (unsigned)last);
       a.top_id[(long long)r * a.top + k] = id;
-      a.top_logprob[(long long)r * a.top + k] = none ? NAN : (score_at(x, id) - m) * a.inv - logz;
+      a.top_logprob[(long long)r * a.top + k] = none ? NAN : score_below(score_at(x, id), m, a.inv) - logz;
     }
   }
 }
@@ -410,7 +415,7 @@ __global__ void __launch_bounds__(SC_MAX, 2) scores_kernel(const __grid_constant
   }
   const float logz = log1pf(rest);
   if (tid == 0) {
-    a.logprob[r] = known ? (xt - xm) * a.inv - logz : -INFINITY;
+    a.logprob[r] = known ? score_below(xt, xm, a.inv) - logz : -INFINITY;
     a.entropy[r] = logz + SC_LN2 * ent / (1.f + rest);
     a.rank[r] = known ? before : a.V;
   }
@@ -453,7 +458,7 @@ __global__ void __launch_bounds__(SC_MAX, 2) scores_kernel(const __grid_constant
     for (int j = 0; j < n; ++j) at += s_key[j] > k;
     if (at < a.top) {
       a.top_id[(long long)r * a.top + at] = (int)(0xffffffffu - (unsigned)k);
-      a.top_logprob[(long long)r * a.top + at] = (ord2f((unsigned)(k >> 32)) - xm) * a.inv - logz;
+      a.top_logprob[(long long)r * a.top + at] = score_below(ord2f((unsigned)(k >> 32)), xm, a.inv) - logz;
     }
   }
 }

@@ -75,3 +75,22 @@ def test_masked_ids_leave_the_bits_of_any_far_logit(temperature, V, dtype):
     for other in got[1:]:
         for name, a, b in zip(other._fields, got[0], other):
             assert torch.equal(a[some], b[some]), name
+
+
+@pytest.mark.parametrize('temperature', [1.0, 2.0, 4.0, 1e20, 1e38])
+def test_differences_past_the_largest_number(temperature):
+    """Logits of both ends of fp32: their difference is past its range, divided by the temperature it need not be."""
+    x = torch.tensor([[3e38, -3e38, 1e38, 0.0, 2.9e38, 3e38], [-3e38, -3.2e38, -3.1e38, -3e38, 3.4e38, 0.0]])
+    if temperature < 2:
+        x = x / 2
+    for t in ([1, 1], [3, 0], [0, 4]):
+        check_far(x, torch.tensor(t), 6, temperature)
+
+
+def test_the_lowest_number_below_a_large_logit():
+    """... on the fast path: its limit is on the largest logit's exponent alone."""
+    x = torch.randn(3, 700, generator=torch.Generator().manual_seed(1)) * 1e35
+    x[:, 5] = -MAX
+    x[:, 600] = 2e36
+    check_far(x, torch.tensor([5, 600, 7]), 9, 2e28)
+    check_far(x.bfloat16(), torch.tensor([5, 600, 7]), 9, 2e28)
