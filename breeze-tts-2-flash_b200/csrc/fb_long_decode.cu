@@ -217,6 +217,15 @@ __device__ __forceinline__ int long_owner(int total, int n, int x) {
   return x < big ? x / (q + 1) : total % n + (x - big) / q;
 }
 
+// Paged: head hq of batch row b again, a key at a time, where an output is not finite (a weight's two parts, and the places
+// of hidden keys, make a NaN of an infinity in a visible slot).
+__device__ __noinline__ uint2 long_paged_again(const LongDecodeArgs& a, int b, int hq) {
+  const PagedPool pool{const_cast<unsigned char*>(a.c.k), const_cast<unsigned char*>(a.c.v), a.c.k_sb, a.c.k_sh, a.c.k_sp,
+                       a.c.v_sb, a.c.v_sh, a.c.v_sp, a.t.pages, a.NKV, a.t.page, a.t.shift};
+  const LongRow row = long_row(a.lengths[b], 0, a.S, a.window, a.sinks);
+  return paged_one(pool, a.t, row, a.scale, b, hq / a.G, a.q + b * a.q_sb + (long long)hq * a.q_sh);
+}
+
 struct LongStat {
   float mA, mB;           // heads 2t, 2t + 1: the subtracted maximum (the same in the eight lanes of a t)
   uint64_t l;             // the two partial sums
@@ -702,7 +711,14 @@ __global__ void __launch_bounds__(LD_THREADS, LongTile<BITS>::CTAS) long_cluster
         O += f * ov[c];
       }
     const bool none = PAGED ? M == -INFINITY : row.n == 0;
-    a.out[((long long)b * a.NH + h * G + gg) * LG_D + tid] = __float2bfloat16_rn(none ? 0.f : O / L * a.v_scale);
+    const float y = none ? 0.f : O / L * a.v_scale;
+    bf16* out = a.out + ((long long)b * a.NH + h * G + gg) * LG_D;
+    if (PAGED && __any_sync(FULL, !isfinite(y))) {       // the warp's own 32 dims: lanes 8 warp .. of the head
+      const uint2 w = long_paged_again(a, b, h * G + gg);
+      if ((tid & 31) >> 3 == tid >> 5) *reinterpret_cast<uint2*>(out + 4 * (tid & 31)) = w;
+    } else {
+      out[tid] = __float2bfloat16_rn(y);
+    }
   }
   if constexpr (SCORED) {
     if (tid < G) {
@@ -852,8 +868,10 @@ __global__ void __launch_bounds__(LM_THREADS, 8) long_merge_kernel(const __grid_
     // visible keys with scores of -inf alone: 0 / 0, as softmax has it
     const float f = a.v_scale / L;
     const bool none = PAGED ? M == -INFINITY : row.n == 0;
-    *reinterpret_cast<uint2*>(a.out + ((long long)b * a.NH + h * G + gg) * LG_D + 4 * lane) =
-        make_uint2(none ? 0u : pack_bf16(O.x * f, O.y * f), none ? 0u : pack_bf16(O.z * f, O.w * f));
+    uint2 y = make_uint2(none ? 0u : pack_bf16(O.x * f, O.y * f), none ? 0u : pack_bf16(O.z * f, O.w * f));
+    if (PAGED && !none && __any_sync(FULL, !isfinite(f) || !isfinite(O.x) || !isfinite(O.y) || !isfinite(O.z) || !isfinite(O.w)))
+      y = long_paged_again(a, b, h * G + gg);
+    *reinterpret_cast<uint2*>(a.out + ((long long)b * a.NH + h * G + gg) * LG_D + 4 * lane) = y;
     return;
   }
   if constexpr (SCORED) {

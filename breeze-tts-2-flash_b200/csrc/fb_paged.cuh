@@ -55,6 +55,40 @@ __device__ __forceinline__ long long paged_left(const PagedRows& r, int b, int t
   return r.offsets ? r.offsets[b + 1] - t : 1;
 }
 
+// One token and head over the visible keys `row` of batch row b, one at a time: four dims a lane; the output row in bf16, 0
+// without a key in a page of the pool.  The weight is fp32 and one factor, so that an infinity in a visible slot comes out as
+// itself: for tokens that saw nothing, or whose output is not finite.  h: KV head; q: the token's head.
+__device__ __forceinline__ uint2 paged_one(const PagedPool& pool, const PagedTable& t, const LongRow& row, float scale, int b, int h,
+                                           const bf16* q) {
+  constexpr float SHIFT = -24.f;                  // sums of 2^16 keys stay in fp32's range for every finite V
+  const int lane = threadIdx.x & 31;
+  const unsigned char *kb = pool.k + h * pool.k_sh + 8 * lane, *vb = pool.v + h * pool.v_sh + 8 * lane;
+  const int* table = t.table + b * t.table_sb;
+  const uint2 qw = *reinterpret_cast<const uint2*>(q + 4 * lane);
+  float m = -INFINITY, sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+  bool some = false;
+#pragma unroll 4
+  for (int i = 0; i < row.n; ++i) {
+    const int j = (int)row.slot(i), page = table[j >> t.shift], in = j & (t.page - 1);
+    if ((unsigned)page >= (unsigned)t.pages) continue;
+    some = true;
+    const uint2 kw = *reinterpret_cast<const uint2*>(kb + page * pool.k_sb + in * pool.k_sl);
+    const uint2 vw = *reinterpret_cast<const uint2*>(vb + page * pool.v_sb + in * pool.v_sl);
+    const float s = scale * warp_sum(lo_f(qw.x) * lo_f(kw.x) + hi_f(qw.x) * hi_f(kw.x) + lo_f(qw.y) * lo_f(kw.y) +
+                                     hi_f(qw.y) * hi_f(kw.y));
+    const float mn = fmaxf(m, s), f = m > -INFINITY ? ex2(m - mn) : 0.f;
+    const float w = mn > -INFINITY ? ex2(s - mn + SHIFT) : (s == -INFINITY ? 0.f : s);
+    m = mn;
+    sum = sum * f + w;
+    o[0] = o[0] * f + w * lo_f(vw.x);
+    o[1] = o[1] * f + w * hi_f(vw.x);
+    o[2] = o[2] * f + w * lo_f(vw.y);
+    o[3] = o[3] * f + w * hi_f(vw.y);
+  }
+  const float inv = some ? 1.f / sum : 0.f;       // scores of -inf alone: 0 / 0, as softmax has it
+  return make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
+}
+
 }  // namespace fb
 
 namespace fbh {

@@ -373,36 +373,9 @@ struct alignas(16) PagedShared {
 constexpr int PT_SMEM = LP_Q + (PT_K + 2) * LP_KV + (int)sizeof(PagedShared);
 static_assert(2 * (PT_SMEM + 1024) <= 228 * 1024, "two CTAs an SM");
 
-// One token and head over its visible keys, one at a time: four dims a lane; the row in bf16.
-// (A row that saw nothing, or whose output is not finite.)
-__device__ __noinline__ uint2 paged_one(const PagedAttendArgs& a, int b, int p, int hq, const bf16* q) {
-  const int lane = threadIdx.x & 31, h = hq / a.G;
-  const LongRow row = long_row((long long)p + 1, 0, a.r.S, a.window, a.sinks);
-  const unsigned char *kb = a.pool.k + h * a.pool.k_sh + 8 * lane, *vb = a.pool.v + h * a.pool.v_sh + 8 * lane;
-  const int* table = a.t.table + b * a.t.table_sb;
-  const uint2 qw = *reinterpret_cast<const uint2*>(q + 4 * lane);
-  float m = -INFINITY, sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  bool some = false;
-#pragma unroll 4
-  for (int i = 0; i < row.n; ++i) {
-    const int j = (int)row.slot(i), page = table[j >> a.t.shift], in = j & (a.t.page - 1);
-    if ((unsigned)page >= (unsigned)a.t.pages) continue;
-    some = true;
-    const uint2 kw = *reinterpret_cast<const uint2*>(kb + page * a.pool.k_sb + in * a.pool.k_sl);
-    const uint2 vw = *reinterpret_cast<const uint2*>(vb + page * a.pool.v_sb + in * a.pool.v_sl);
-    const float s = a.scale * warp_sum(lo_f(qw.x) * lo_f(kw.x) + hi_f(qw.x) * hi_f(kw.x) + lo_f(qw.y) * lo_f(kw.y) +
-                                       hi_f(qw.y) * hi_f(kw.y));
-    const float mn = fmaxf(m, s), f = m > -INFINITY ? ex2(m - mn) : 0.f;
-    const float w = mn > -INFINITY ? ex2(s - mn + LP_SHIFT) : (s == -INFINITY ? 0.f : s);
-    m = mn;
-    sum = sum * f + w;
-    o[0] = o[0] * f + w * lo_f(vw.x);
-    o[1] = o[1] * f + w * hi_f(vw.x);
-    o[2] = o[2] * f + w * lo_f(vw.y);
-    o[3] = o[3] * f + w * hi_f(vw.y);
-  }
-  const float inv = some ? 1.f / sum : 0.f;       // scores of -inf alone: 0 / 0, as softmax has it
-  return make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
+// The token at slot p of row b, its head hq, again: where it saw nothing, or its output is not finite.
+__device__ __noinline__ uint2 paged_again(const PagedAttendArgs& a, int b, int p, int hq, const bf16* q) {
+  return paged_one(a.pool, a.t, long_row((long long)p + 1, 0, a.r.S, a.window, a.sinks), a.scale, b, hq / a.G, q);
 }
 
 // Pieces come from the plan (PT_PLAN), or CTAs find theirs: of query tiles that stay whole, or cut.
@@ -792,7 +765,7 @@ __global__ void __launch_bounds__(PT_THREADS, 2) paged_attend_kernel(const __gri
       for (unsigned todo = __ballot_sync(FULL, bad && ok && mine); todo; todo &= todo - 1) {
         const int rr = warp * 32 + __ffs(todo) - 1, ll = rr >> a.lg, hq = h * a.G + (rr & (a.G - 1));
         const long long t = piece.tok + ll;
-        const uint2 y = paged_one(a, piece.b, p_lo + ll, hq, a.q + t * a.q_st + hq * a.q_sh);
+        const uint2 y = paged_again(a, piece.b, p_lo + ll, hq, a.q + t * a.q_st + hq * a.q_sh);
         *reinterpret_cast<uint2*>(a.out + t * a.o_st + hq * a.o_sh + 4 * lane) = y;
       }
     }
@@ -861,7 +834,7 @@ __global__ void __launch_bounds__(PM_THREADS, PM_CTAS) paged_merge_kernel(const 
     if (__any_sync(FULL, L == 0.f || !isfinite(L) || !isfinite(O.x + O.y + O.z + O.w))) {
       const int b = paged_row(a.r, (int)t);
       const PagedSpan span = paged_span(a.r, b);
-      y = paged_one(a, b, span.p0 + (int)t - span.t0, hq, a.q + t * a.q_st + hq * a.q_sh);
+      y = paged_again(a, b, span.p0 + (int)t - span.t0, hq, a.q + t * a.q_st + hq * a.q_sh);
     }
     *reinterpret_cast<uint2*>(a.out + t * a.o_st + hq * a.o_sh + 4 * lane) = y;
   }
