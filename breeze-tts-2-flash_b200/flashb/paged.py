@@ -12,7 +12,9 @@ the rows' runs one after the other:
 [B] int64: how many slots of each row are in use, the step's tokens among them; ``offsets`` [B + 1] int64: row b's tokens
 are offsets[b] .. offsets[b + 1] - 1 of the step's (not decreasing; None: one token a row).  All of them are on the device
 and read there, so every call is graph-capturable; tokens behind offsets[B] are left as they are, so that a graph may be
-captured for more tokens than a step has.  bf16, head_dim 128, GQA groups of 1, 2, 4 or 8; fp32 scores, softmax statistics
+captured for more tokens than a step has.  In a step of at most one token a row leave idle rows out of ``table`` and
+``lengths`` and call without ``offsets``: the form of single tokens is more exact and quicker (128 rows to 8192 slots, a
+quarter of them idle: 133 us, as runs 150).  bf16, head_dim 128, GQA groups of 1, 2, 4 or 8; fp32 scores, softmax statistics
 and sums, rounded once; the weights enter the product with V as two bf16 parts (one token a row) or one (runs).  Outputs
 may not share memory with inputs (``append``'s q in place of its projections is the exception).  No reference counterpart:
 the reference's cache is one request's (``flash/backbone.py``).

@@ -124,19 +124,28 @@ class PagedSpeech:
         changed = self._take(counts)
         if changed:
             self.table.copy_(self._host)
-        single = all(n == 1 for n in counts)
-        n = torch.tensor(counts, dtype=torch.int64)
-        offsets = None if single else torch.cat((n.new_zeros(1), n.cumsum(0))).to(self.device)
-        self.lengths += 1 if single else n.to(self.device)
+        table, lengths, offsets = self.table, self.lengths, None
+        if max(counts) > 1:
+            n = torch.tensor(counts, dtype=torch.int64)
+            offsets = torch.cat((n.new_zeros(1), n.cumsum(0))).to(self.device)
+            self.lengths += n.to(self.device)
+        elif T == len(counts):
+            self.lengths += 1
+        else:
+            # at most one token a row: the rows that have one, in the form of single tokens, so that what a frame's attention
+            # rounds does not hang on who else is idle
+            rows = torch.tensor([r for r, m in enumerate(counts) if m], dtype=torch.int64).to(self.device)
+            self.lengths[rows] += 1
+            table, lengths = self.table[rows], self.lengths[rows]
         for r, m in enumerate(counts):
             self.used[r] += m
         fx, st = kernels.fused(), self.st
         x = embeds.contiguous()
         for Lw, cache in zip(st['layers'], self.caches):
             qkv = self._qkv(Lw, x)
-            q = paged.append(qkv, cache, self.table, self.lengths, offsets=offsets, rotary=self.rotary, q_norm=Lw.qn_w,
-                             k_norm=Lw.kn_w, eps=Lw.qk_eps, out=qkv[:, :self.NH * 128].view(T, self.NH, 128))
-            ao = paged.attend(q, cache, self.table, self.lengths, offsets=offsets, window=self.window, sinks=self.sinks,
+            q = paged.append(qkv, cache, table, lengths, offsets=offsets, rotary=self.rotary, q_norm=Lw.qn_w, k_norm=Lw.kn_w,
+                             eps=Lw.qk_eps, out=qkv[:, :self.NH * 128].view(T, self.NH, 128))
+            ao = paged.attend(q, cache, table, lengths, offsets=offsets, window=self.window, sinks=self.sinks,
                               scaling=Lw.scaling)
             x = self._mlp(Lw, ao.view(T, -1), x)
         hidden = torch.empty_like(x)

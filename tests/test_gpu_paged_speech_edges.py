@@ -1,0 +1,25 @@
+"""The backbone over pages where steps are unusual: rows that have nothing this time, inputs that are refused."""
+import pytest
+import torch
+
+from test_gpu_paged_speech import _graph, _speech, _x
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize('window', [None, 24])
+def test_a_frame_beside_idle_rows(window):
+    """Frames of some rows, others without a token: the bits of a step of those rows alone."""
+    cfg, g = _graph(layers=2)
+    wide = _speech(g, rows=5, max_slots=320, window=window)
+    narrow = _speech(g, rows=2, max_slots=320, window=window)
+    x = _x(cfg, 90, 3)
+    assert torch.equal(wide.extend(x[:80], [0, 50, 0, 30, 0]), narrow.extend(x[:80], [50, 30]))
+    for i in range(80, 88, 2):
+        a, b = wide.extend(x[i:i + 2], [0, 1, 0, 1, 0]), narrow.extend(x[i:i + 2], [1, 1])
+        assert torch.equal(a, b)
+    assert wide.used == [0, 54, 0, 34, 0] and wide.lengths.tolist() == wide.used
+    # all idle but one, and a row that begins
+    a = wide.extend(x[88:90], [1, 0, 0, 1, 0])
+    assert a.shape == (2, cfg.hidden) and wide.used == [1, 54, 0, 35, 0]
+    assert torch.equal(wide.extend(x[:1], [0, 0, 0, 0, 1]), _speech(g, rows=1, max_slots=320, window=window).extend(x[:1], [1]))
