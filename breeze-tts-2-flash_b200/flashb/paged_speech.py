@@ -114,8 +114,12 @@ class PagedSpeech:
 
     def extend(self, embeds, counts):
         """The next ``counts[r]`` tokens of each row r, one row's after the other's in ``embeds`` [T, H] bf16.  Returns
-        their hidden states [T, H] after the final norm.  Raises, with nothing changed, when pages run out."""
-        T, H = embeds.shape
+        their hidden states [T, H] after the final norm.  Raises, with nothing changed, when an argument is wrong or pages run
+        out."""
+        if embeds.device != self.device or embeds.dtype != torch.bfloat16 or embeds.dim() != 2 or (
+                embeds.shape[1] != self.st['embed'].shape[1]):
+            raise FlashbError(FB_ERR_ARG, f'paged speech: embeds [T, {self.st["embed"].shape[1]}] bf16 on {self.device}')
+        T = embeds.shape[0]
         if len(counts) != len(self.used) or min(counts) < 0 or sum(counts) != T:
             raise FlashbError(FB_ERR_ARG, f'paged speech: counts of {len(counts)} rows and {sum(counts)} tokens for '
                                           f'{len(self.used)} rows and {T}')

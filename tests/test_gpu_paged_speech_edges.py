@@ -23,3 +23,18 @@ def test_a_frame_beside_idle_rows(window):
     a = wide.extend(x[88:90], [1, 0, 0, 1, 0])
     assert a.shape == (2, cfg.hidden) and wide.used == [1, 54, 0, 35, 0]
     assert torch.equal(wide.extend(x[:1], [0, 0, 0, 0, 1]), _speech(g, rows=1, max_slots=320, window=window).extend(x[:1], [1]))
+
+
+def test_refused_inputs_change_nothing():
+    from flashb._native import FB_ERR_ARG, FlashbError
+    cfg, g = _graph(layers=1)
+    s = _speech(g, max_slots=64)
+    x = _x(cfg, 20, 1)
+    s.extend(x[:5], [5, 0])
+    before = list(s.free), list(s.used), s.lengths.clone(), s.table.clone()
+    for bad in (x.float(), x.cpu(), x[:, :-8], x.half(), x[None]):
+        with pytest.raises(FlashbError) as e:
+            s.extend(bad, [18, 2])
+        assert e.value.rc == FB_ERR_ARG
+        assert (s.free, s.used) == before[:2] and torch.equal(s.lengths, before[2]) and torch.equal(s.table, before[3])
+    assert s.extend(x[:18], [16, 2]).shape == (18, cfg.hidden) and s.used == [21, 2]
