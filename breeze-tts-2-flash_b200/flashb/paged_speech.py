@@ -52,6 +52,7 @@ class PagedSpeech:
         L0 = st['layers'][0]
         dev = self.device = L0.wq.device
         self.st, self.page, self.window, self.sinks = st, page, window, sinks
+        self.codebooks = graph.input_ids_buf.shape[-1]
         self.NH, self.NKV = L0.wq.shape[0] // 128, L0.wk.shape[0] // 128
         self.rotary = graph_rotary(graph, dev) if rotary is None else rotary
         self.caches = [paged.PagedCache.empty(pages, self.NKV, page, device=dev) for _ in st['layers']]
@@ -106,7 +107,12 @@ class PagedSpeech:
     def embed(self, ids):
         """The input embeddings [T, H] of frames ``ids`` [T, codebooks] int64."""
         st = self.st
+        if ids.device != self.device or ids.dtype != torch.int64 or ids.dim() != 2 or ids.shape[1] != self.codebooks:
+            raise FlashbError(FB_ERR_ARG, f'paged speech: ids [T, {self.codebooks}] int64 on {self.device}')
+        ids = ids.contiguous()
         x = torch.empty(ids.shape[0], st['embed'].shape[1], dtype=torch.bfloat16, device=self.device)
+        if ids.shape[0] == 0:
+            return x
         cs = torch.empty(2, ids.shape[0], 128, dtype=torch.bfloat16, device=self.device)
         pos = torch.zeros(ids.shape[0], dtype=torch.int64, device=self.device)
         kernels.fused().embed_rope(ids, st['vocab'], st['embed'], pos, st['cos_tab'], st['sin_tab'], x, cs[0], cs[1])

@@ -38,3 +38,19 @@ def test_refused_inputs_change_nothing():
         assert e.value.rc == FB_ERR_ARG
         assert (s.free, s.used) == before[:2] and torch.equal(s.lengths, before[2]) and torch.equal(s.table, before[3])
     assert s.extend(x[:18], [16, 2]).shape == (18, cfg.hidden) and s.used == [21, 2]
+
+
+def test_refused_frames():
+    from flashb._native import FB_ERR_ARG, FlashbError
+    cfg, g = _graph(layers=1)
+    s = _speech(g)
+    ids = torch.randint(0, cfg.vocab, (3, cfg.codebooks)).cuda()
+    for bad in (ids.cpu(), ids.int(), ids[:, :-1], ids[:, :1].expand(-1, cfg.codebooks + 1), ids[0], ids[None]):
+        with pytest.raises(FlashbError) as e:
+            s.embed(bad)
+        assert e.value.rc == FB_ERR_ARG
+    want = s.embed(ids)
+    wide = torch.zeros(3, 2 * cfg.codebooks, dtype=torch.int64, device='cuda')
+    wide[:, ::2] = ids
+    assert want.shape == (3, cfg.hidden) and torch.equal(s.embed(wide[:, ::2]), want)
+    assert s.embed(ids[:0]).shape == (0, cfg.hidden)
