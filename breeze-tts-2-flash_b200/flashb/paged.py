@@ -108,7 +108,9 @@ class Rotary:
 
     @staticmethod
     def _freq(dim, base, how):
-        kind, f = how.pop('kind', None), float(how.pop('factor', 1.0))
+        kind = how.pop('kind', None)
+        _ensure(kind is not None or not how, f'rotary: scaling {sorted(how)} without a kind')
+        f = float(how.pop('factor', 1.0))
         _ensure(kind in (None, 'linear', 'ntk', 'yarn'), f'rotary: scaling {kind!r}')
         _ensure(f > 0 and math.isfinite(f), f'rotary: factor {f}')
         if kind == 'ntk':
