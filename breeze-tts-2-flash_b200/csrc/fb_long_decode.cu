@@ -1214,7 +1214,7 @@ extern "C" int flashb_paged_decode(const fb_paged_cache* cache, const int32_t* t
   FB_CHECK_ARG(((uintptr_t)q & 15) == 0 && q_st % 8 == 0 && q_sh % 8 == 0,
                "paged_decode: q must be 16-byte aligned with strides multiple of 8 elements");
   FB_CHECK_ARG(((uintptr_t)out & 7) == 0, "paged_decode: out must be 8-byte aligned");
-  FB_CHECK_ARG(scaling > 0.f && scaling < INFINITY, "paged_decode: scaling must be positive and finite");
+  FB_CHECK_ARG(scaling > 0.f && scaling * LG_LOG2E < INFINITY, "paged_decode: scaling must be positive, and finite times log2(e)");
   rc = fbh::paged_apart(pool, rows, NH, q, q_st, q_sh, out, (int64_t)NH * LG_D, LG_D);
   if (rc) return rc;
   FB_CHECK_ARG(p.ws_floats == 0 || (ws && ((uintptr_t)ws & 15) == 0 && ws_floats >= p.ws_floats),

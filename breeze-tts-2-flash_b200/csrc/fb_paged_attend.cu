@@ -924,7 +924,7 @@ extern "C" int flashb_paged_attend(const fb_paged_cache* cache, const int32_t* t
   FB_CHECK_ARG(table_sb >= 0, "paged_attend: table stride %lld", (long long)table_sb);
   FB_CHECK_ARG(T >= 1 && (int64_t)T * NH <= 0x7fffffff, "paged_attend: %d tokens of %d heads", T, NH);
   FB_CHECK_ARG(sinks >= 0, "paged_attend: sinks %d", sinks);
-  FB_CHECK_ARG(scaling > 0.f && scaling < INFINITY, "paged_attend: scaling must be positive and finite");
+  FB_CHECK_ARG(scaling > 0.f && scaling * LG_LOG2E < INFINITY, "paged_attend: scaling must be positive, and finite times log2(e)");
   FB_CHECK_ARG((((uintptr_t)q | (uintptr_t)out) & 15) == 0 && (q_st | q_sh | o_st | o_sh) % 8 == 0,
                "paged_attend: tensors must be 16-byte aligned with strides multiple of 8 elements");
   FB_CHECK_ARG((T == 1 || (q_st > 0 && o_st > 0)) && (NH == 1 || (q_sh > 0 && o_sh > 0)),
