@@ -14,7 +14,12 @@
 // The weights are 2^(s - m - 24) with a reference m of the row's own that is hardly ever moved: they are taken with the old
 // m first, and only when a tile's sum shows that some score passed it by 2^8 is the tile's maximum worked out, O and the
 // sum rescaled and the weights taken again.  (The maximum first, for every tile: 600 instead of 530 us at the largest
-// case below.  The sums are exact either way; sum and reference are fp32, P goes to bf16, one part, as in the prefill.)
+// case below.  The sums are exact either way; sum and reference are fp32.)
+//
+// P goes to bf16, one part, as in the prefill: the tensor cores take it in V's type, half a step of 2^-8 off at most.  Against
+// 64 bits the output is 2.0e-3 to 2.4e-3 off, where single tokens, whose kernel takes P in two parts, have 1.7e-3, their own
+// rounding.  A second part here would need half as much again of the tensor cores (1536 cycles for the two tiles of an SM,
+// which take 1500 in all now) and 32 columns of TMEM more for either buffer of P, where S, P and O of two CTAs fill all 512.
 //
 // Pieces.  A step can be one run of a few tokens over a long row, or many rows of which some are long.  So the key tiles of
 // a query tile are cut into s pieces of about C; a CTA takes one piece of the list that lengths and offsets, on the device,
@@ -25,23 +30,25 @@
 // short to cut, CTAs just find their query tiles.  Pieces of a query tile leave (reference, sum, unnormalised out) in the
 // workspace and paged_merge_kernel joins them in order: no atomics, the same inputs give the same bits.
 //
-// Rows of one token are runs as others are.  (The single-token kernel for them, in a launch of its own: 128 instead of 133 us
-// for 512 tokens beside 63 single ones over long rows, but 19 instead of 14 over short ones, and 5 us where there are none.)
+// Rows of one token are runs as others are.  (The single-token kernel for them, in a launch of its own, measured before pieces
+// were priced as they are now: 128 instead of 133 us for 512 tokens beside 63 single ones over long rows, but 19 instead of 14
+// over short ones, and 5 us where there are none.)
 //
 // Slots that no row of the CTA sees may hold anything: in V they are zeroed in shared memory (0 times a NaN is NaN), in K
 // their scores are replaced.  A row whose output is not finite all the same (a NaN that another row of the tile sees) is
 // computed again, one visible key at a time.
 //
-// Measured on a B200 (in a CUDA graph, 16 heads over 4): 2048 tokens over 32768 slots of one row 520 us, 1090 TFLOP/s, in
-// pages of 16 to 128 alike; 801 tokens of 32 rows over a window of 2048 (131 MB) 46 us; 512 tokens of one row beside one each
-// of 63, over up to 8000 slots (530 MB), 116 us; two prompts of 197 tokens 9.5 us.  A tile takes 1500 cycles with two
-// CTAs an SM: 700 to 870 are exponentials (the unit's bound for both CTAs is 1024), 100 the read of S, 240 masks, the rest
-// waits and stores; issuing S takes its thread 480 cycles and P V 290, both beside the exponentials.  Under the largest
-// case's load clocks fall to 1.5 GHz.  With few keys a piece it is beginning and ending (9000 cycles) that counts.  Tried
-// and slower: one copying warp for K and V (8 boxes one after the other take 900 cycles), a flag for missing pages read in
-// the loop (6%), arrivals by one lane a warp (4%), P V's waits by one lane (10%), the
-// second CTA of an SM begun half a tile later (the same), copies to L2 a buffer ahead (4 to 30%: more boxes), half of Q in
-// the place of P's second buffer in TMEM (3 to 10%).
+// Measured on a B200 (in a CUDA graph, 16 heads over 4): 2048 tokens over 32768 slots of one row 520 to 577 us by the box, 983
+// to 1090 TFLOP/s, in pages of 16 to 128 alike; 801 tokens of 32 rows over a window of 2048 (131 MB) 46 us; 512 tokens of one
+// row beside one each of 63, over up to 8000 slots (530 MB), 97 to 129 us by their lengths, 116 on average over ten sets of
+// them; two prompts of 197 tokens 9.1 us, in a table of 16384 slots, by whose width the form is chosen, 11.5.  A tile takes
+// 1500 cycles with two CTAs an SM: 700 to 870 are exponentials (the unit's bound for both CTAs is 1024), 100 the read of S,
+// 240 masks, the rest waits and stores; issuing S takes its thread 480 cycles and P V 290, both beside the exponentials.
+// Under the largest case's load clocks fall to 1.5 GHz.  With few keys a piece it is beginning and ending (9000 cycles) that
+// counts.  Tried and slower: one copying warp for K and V (8 boxes one after the other take 900 cycles), a flag for missing
+// pages read in the loop (6%), arrivals by one lane a warp (4%), P V's waits by one lane (10%), the second CTA of an SM begun
+// half a tile later (the same), copies to L2 a buffer ahead (4 to 30%: more boxes), half of Q in the place of P's second
+// buffer in TMEM (3 to 10%).
 #include <climits>
 
 #include "fb_long_tc.cuh"

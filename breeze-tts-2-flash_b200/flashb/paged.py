@@ -15,9 +15,11 @@ and read there, so every call is graph-capturable; tokens behind offsets[B] are 
 captured for more tokens than a step has.  In a step of at most one token a row leave idle rows out of ``table`` and
 ``lengths`` and call without ``offsets``: the form of single tokens is more exact and quicker (128 rows to 8192 slots, a
 quarter of them idle: 133 us, as runs 150).  bf16, head_dim 128, GQA groups of 1, 2, 4 or 8; fp32 scores, softmax statistics
-and sums, rounded once; the weights enter the product with V as two bf16 parts (one token a row) or one (runs).  Outputs
-may not share memory with inputs (``append``'s q in place of its projections is the exception).  No reference counterpart:
-the reference's cache is one request's (``flash/backbone.py``).
+and sums, rounded once; the weights enter the product with V as two bf16 parts (one token a row: the error of fp32 weights)
+or one (runs: 1.2 to 1.4 times that).  The form and the workspace of ``attend`` go by the table's width: give it no more
+columns than the longest row needs (``table[:, :n]``).  Outputs may not share memory with inputs (``append``'s q in place of
+its projections is the exception).  No reference counterpart: the reference's cache is one request's
+(``flash/backbone.py``).
 
 Calls run on the current stream of the cache's device, whichever device is current; workspaces come from torch's allocator
 on that stream.

@@ -116,8 +116,8 @@ class TokenScores(NamedTuple):
 
 
 def token_scores(logits, tokens, *, top=0, temperature=1.0):
-    """What ``logits`` [rows, V] (fp32 or bf16, unit inner stride; CFG logits, or the logits of a given reading) say of
-    ``tokens`` [rows] int64 under softmax(logits / temperature): a ``TokenScores``, in one launch.
+    """What ``logits`` [rows, V] (fp32 or bf16, unit inner stride, rows at least V apart; CFG logits, or the logits of a given
+    reading) say of ``tokens`` [rows] int64 under softmax(logits / temperature): a ``TokenScores``, in one launch.
 
     Larger logits come first, equal ones by id, a NaN before all, as in the greedy sampler.  Suppressed ids (-inf) have
     probability 0; an id outside the vocabulary has log probability -inf and rank V.  A row with a NaN or +inf, or of -inf

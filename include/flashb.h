@@ -314,10 +314,11 @@ int flashb_paged_append(const fb_paged_cache* cache, const int32_t* table, int64
                         float amplitude, const int64_t* positions, void* q_out, int64_t o_st, int64_t o_sh, void* stream);
 /* Attention of the step's tokens: q [T, NH, 128] bf16 (strides q_st, q_sh) -> out [T, NH, 128] (strides o_st, o_sh), all
  * multiples of 8, 16-byte aligned.  The token at slot p sees slot j when j <= p and (j > p - window or j < sinks); window
- * <= 0: no window; scaling > 0, finite times log2(e); lengths are clamped to the row's entries.  NH / NKV in {1, 2, 4, 8}.  Scores, softmax and
- * sums in fp32; slots that are not visible may hold anything; without a visible slot the output is 0 (with visible scores
- * of -inf alone NaN).  ws: 16-byte aligned, at least flashb_paged_attend_ws_floats() floats (0: may be NULL), not shared by
- * calls that can overlap, contents free before and after.  The same inputs give the same bits. */
+ * <= 0: no window; scaling > 0, finite times log2(e); lengths are clamped to the row's entries.  NH / NKV in {1, 2, 4, 8}.
+ * Scores, softmax and sums in fp32; slots that are not visible may hold anything, an infinity in a visible one comes out as
+ * itself; without a visible slot the output is 0 (with visible scores of -inf alone NaN).  ws: 16-byte aligned, at least
+ * flashb_paged_attend_ws_floats() floats (0: may be NULL), not shared by calls that can overlap, contents free before and
+ * after.  The same inputs give the same bits. */
 int64_t flashb_paged_attend_ws_floats(const fb_paged_cache* cache, int rows, int width, int T, int NH, int window,
                                       int sinks);
 int flashb_paged_attend(const fb_paged_cache* cache, const int32_t* table, int64_t table_sb, int rows, int width,
