@@ -49,6 +49,8 @@ class PagedSpeech:
             raise FlashbError(FB_ERR_ARG, f'paged speech: {rows} rows on {pages} pages of {page} slots')
         if (window is not None and window < 1) or sinks < 0:
             raise FlashbError(FB_ERR_ARG, f'paged speech: a window of {window} and {sinks} first slots')
+        if max_slots is not None and max_slots < 1:
+            raise FlashbError(FB_ERR_ARG, f'paged speech: {max_slots} slots a row')
         L0 = st['layers'][0]
         dev = self.device = L0.wq.device
         self.st, self.page, self.window, self.sinks = st, page, window, sinks
@@ -56,7 +58,8 @@ class PagedSpeech:
         self.NH, self.NKV = L0.wq.shape[0] // 128, L0.wk.shape[0] // 128
         self.rotary = graph_rotary(graph, dev) if rotary is None else rotary
         self.caches = [paged.PagedCache.empty(pages, self.NKV, page, device=dev) for _ in st['layers']]
-        self.width = pages if max_slots is None else -(-max_slots // page)
+        self.slots = pages * page if max_slots is None else max_slots      # of a row, at most
+        self.width = -(-self.slots // page)
         self.free = list(range(pages - 1, -1, -1))          # pages of no row; the same page of every layer's pool
         self.pages = [[] for _ in range(rows)]              # each row's, -1: given back
         self.gone = [0] * rows                              # how many pages from the sinks' on a row has given back
@@ -71,9 +74,8 @@ class PagedSpeech:
         """Pages for the step's tokens; all of them or none."""
         want = [-(-(self.used[r] + n) // self.page) - len(self.pages[r]) if n else 0 for r, n in enumerate(counts)]
         for r, n in enumerate(counts):
-            if n and len(self.pages[r]) + want[r] > self.width:
-                raise FlashbError(FB_ERR_STATE, f'paged speech: row {r} at {self.used[r] + n} slots, {self.width * self.page} '
-                                                f'at most')
+            if n and self.used[r] + n > self.slots:
+                raise FlashbError(FB_ERR_STATE, f'paged speech: row {r} at {self.used[r] + n} slots, {self.slots} at most')
         if sum(want) > len(self.free):
             raise FlashbError(FB_ERR_STATE, f'paged speech: {sum(want)} pages wanted, {len(self.free)} free')
         for r, n in enumerate(want):

@@ -54,3 +54,23 @@ def test_refused_frames():
     wide[:, ::2] = ids
     assert want.shape == (3, cfg.hidden) and torch.equal(s.embed(wide[:, ::2]), want)
     assert s.embed(ids[:0]).shape == (0, cfg.hidden)
+
+
+def test_rows_end_at_their_last_slot():
+    """``max_slots`` that is no whole number of pages is the limit all the same."""
+    from flashb._native import FB_ERR_ARG, FB_ERR_STATE, FlashbError
+    from flashb.paged_speech import PagedSpeech
+    cfg, g = _graph(layers=1)
+    s = _speech(g, max_slots=40)
+    x = _x(cfg, 50, 1)
+    s.extend(x[:39], [39, 0])
+    for counts in ([2, 0], [0, 41]):
+        with pytest.raises(FlashbError) as e:
+            s.extend(x[:sum(counts)], counts)
+        assert e.value.rc == FB_ERR_STATE and s.used == [39, 0] and s.lengths.tolist() == [39, 0]
+    s.extend(x[:41], [1, 40])
+    assert s.used == [40, 40]
+    for n in (0, -16):
+        with pytest.raises(FlashbError) as e:
+            PagedSpeech(g, 2, 40, max_slots=n)
+        assert e.value.rc == FB_ERR_ARG
