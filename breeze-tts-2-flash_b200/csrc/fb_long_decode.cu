@@ -219,7 +219,8 @@ __device__ __forceinline__ int long_owner(int total, int n, int x) {
 }
 
 // Paged: head hq of batch row b again, a key at a time, where an output is not finite (a weight's two parts, and the places
-// of hidden keys, make a NaN of an infinity in a visible slot).
+// of hidden keys, make a NaN of an infinity in a visible slot) though the weights' sum L is a number above 0.  Without one the
+// output is NaN whatever V holds, and a row that has gone bad does not hold up the others.
 __device__ __noinline__ uint2 long_paged_again(const LongDecodeArgs& a, int b, int hq) {
   const PagedPool pool{const_cast<unsigned char*>(a.c.k), const_cast<unsigned char*>(a.c.v), a.c.k_sb, a.c.k_sh, a.c.k_sp,
                        a.c.v_sb, a.c.v_sh, a.c.v_sp, a.t.pages, a.NKV, a.t.page, a.t.shift};
@@ -714,7 +715,7 @@ __global__ void __launch_bounds__(LD_THREADS, LongTile<BITS>::CTAS) long_cluster
     const bool none = PAGED ? M == -INFINITY : row.n == 0;
     const float y = none ? 0.f : O / L * a.v_scale;
     bf16* out = a.out + ((long long)b * a.NH + h * G + gg) * LG_D;
-    if (PAGED && __any_sync(FULL, !isfinite(y))) {       // the warp's own 32 dims: lanes 8 warp .. of the head
+    if (PAGED && L > 0.f && __any_sync(FULL, !isfinite(y))) {       // the warp's own 32 dims: lanes 8 warp .. of the head
       const uint2 w = long_paged_again(a, b, h * G + gg);
       if ((tid & 31) >> 3 == tid >> 5) *reinterpret_cast<uint2*>(out + 4 * (tid & 31)) = w;
     } else {
@@ -870,7 +871,7 @@ __global__ void __launch_bounds__(LM_THREADS, 8) long_merge_kernel(const __grid_
     const float f = a.v_scale / L;
     const bool none = PAGED ? M == -INFINITY : row.n == 0;
     uint2 y = make_uint2(none ? 0u : pack_bf16(O.x * f, O.y * f), none ? 0u : pack_bf16(O.z * f, O.w * f));
-    if (PAGED && !none && __any_sync(FULL, !isfinite(f) || !isfinite(O.x) || !isfinite(O.y) || !isfinite(O.z) || !isfinite(O.w)))
+    if (PAGED && L > 0.f && __any_sync(FULL, !isfinite(O.x) || !isfinite(O.y) || !isfinite(O.z) || !isfinite(O.w)))
       y = long_paged_again(a, b, h * G + gg);
     *reinterpret_cast<uint2*>(a.out + ((long long)b * a.NH + h * G + gg) * LG_D + 4 * lane) = y;
     return;

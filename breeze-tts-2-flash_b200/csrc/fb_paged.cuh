@@ -57,7 +57,9 @@ __device__ __forceinline__ long long paged_left(const PagedRows& r, int b, int t
 
 // One token and head over the visible keys `row` of batch row b, one at a time: four dims a lane; the output row in bf16, 0
 // without a key in a page of the pool.  The weight is fp32 and one factor, so that an infinity in a visible slot comes out as
-// itself: for tokens that saw nothing, or whose output is not finite.  h: KV head; q: the token's head.
+// itself: for tokens that saw nothing, or whose output is not finite.  h: KV head; q: the token's head.  (0.6 us a key, which
+// only a row with an infinity or a NaN in V takes; eight keys' loads together took 0.3, but 64 registers that spill into the
+// kernels that call it, 1% of them.)
 __device__ __forceinline__ uint2 paged_one(const PagedPool& pool, const PagedTable& t, const LongRow& row, float scale, int b, int h,
                                            const bf16* q) {
   constexpr float SHIFT = -24.f;                  // sums of 2^16 keys stay in fp32's range for every finite V

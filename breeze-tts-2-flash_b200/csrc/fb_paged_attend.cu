@@ -35,8 +35,8 @@
 // over short ones, and 5 us where there are none.)
 //
 // Slots that no row of the CTA sees may hold anything: in V they are zeroed in shared memory (0 times a NaN is NaN), in K
-// their scores are replaced.  A row whose output is not finite all the same (a NaN that another row of the tile sees) is
-// computed again, one visible key at a time.
+// their scores are replaced.  A row whose output is not finite all the same (a NaN that another row of the tile sees), though
+// its weights' sum is a number, is computed again, one visible key at a time.
 //
 // Measured on a B200 (in a CUDA graph, 16 heads over 4): 2048 tokens over 32768 slots of one row 520 to 577 us by the box, 983
 // to 1090 TFLOP/s, in pages of 16 to 128 alike; 801 tokens of 32 rows over a window of 2048 (131 MB) 46 us; 512 tokens of one
@@ -758,7 +758,7 @@ __global__ void __launch_bounds__(PT_THREADS, 2) paged_attend_kernel(const __gri
               make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
       }
       const float2 od = f2_get(odd);
-      const bool bad = !isfinite(sum) || !(od.x + od.y == 0.f) || sum == 0.f;
+      const bool bad = sum == 0.f || (sum > 0.f && !(od.x + od.y == 0.f));   // (a NaN of the weights stays one)
       __syncwarp();
       const int half = lane >> 4, c = lane & 15;
 #pragma unroll 4
@@ -838,7 +838,7 @@ __global__ void __launch_bounds__(PM_THREADS, PM_CTAS) paged_merge_kernel(const 
     uint2 y = make_uint2(pack_bf16(O.x * f, O.y * f), pack_bf16(O.z * f, O.w * f));
     const int l = r >> a.lg, hq = h * a.G + (r & (a.G - 1));
     const long long t = cut.x + l;
-    if (__any_sync(FULL, L == 0.f || !isfinite(L) || !isfinite(O.x + O.y + O.z + O.w))) {
+    if (__any_sync(FULL, L == 0.f || (L > 0.f && !isfinite(O.x + O.y + O.z + O.w)))) {
       const int b = paged_row(a.r, (int)t);
       const PagedSpan span = paged_span(a.r, b);
       y = paged_again(a, b, span.p0 + (int)t - span.t0, hq, a.q + t * a.q_st + hq * a.q_sh);
