@@ -67,3 +67,35 @@ def test_runs():
     check_infinities(s, edits([(0, (0, 99)), (1, (50, 64)), (2, (0, 29))]))
     s = make([20, 3], [2000, 1500], 8, 2, 16)
     check_infinities(s, edits([(0, (0, 1999)), (1, (700, 1499))]))
+
+
+@pytest.mark.parametrize('single', [True, False])
+def test_a_row_gone_bad_does_not_hold_up_the_step(single):
+    """A long row of NaN among others: NaN for itself, and the step's time (a key at a time it was 30 times and more)."""
+    m = paged()
+    rows, page, n = 16, 64, 4096
+    g = torch.Generator(device='cuda').manual_seed(1)
+    k, v = (torch.randn(rows * n // page, 4, page, 128, generator=g, device='cuda').bfloat16() for _ in range(2))
+    table = torch.arange(rows * n // page, device='cuda', dtype=torch.int32).view(rows, -1)
+    lengths = torch.full((rows,), n, device='cuda')
+    offsets = None if single else torch.arange(rows + 1, device='cuda')
+    q = torch.randn(rows, 16, 128, generator=g, device='cuda').bfloat16()
+    c = m.PagedCache(k, v)
+
+    def took():
+        best = float('inf')
+        for _ in range(10):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            for _ in range(5):
+                out = m.attend(q, c, table, lengths, offsets=offsets)
+            b.record()
+            torch.cuda.synchronize()
+            best = min(best, a.elapsed_time(b))
+        return out, best
+    good, before = took()
+    k[table[3].long()] = float('nan')
+    bad, after = took()
+    others = [r for r in range(rows) if r != 3]
+    assert torch.equal(bad[others], good[others]) and bad[3].isnan().all()
+    assert after < 8 * before, (before, after)
